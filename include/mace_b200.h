@@ -41,7 +41,11 @@ enum {
   MB_ST_BAD_RECEIVER = 16,
   MB_ST_TC_TIMEOUT = 32,      /* a tensor-core kernel gave up waiting on its MMA barrier (bounded wait) */
   MB_ST_UNSORTED = 64,        /* mace_b200_csr_rows: pair_i not receiver-sorted inside a chunk */
+  MB_ST_BAD_EXPERT = 128,     /* mace_b200_expert_plan: an expert index outside [-1, E) (the slot gets no expert) */
 };
+
+/* element types of the operators below that take more than fp32 */
+enum { MB_F32 = 0, MB_BF16 = 1, MB_F16 = 2 };
 
 /* Folded, device-resident model (fp32 unless noted).  S = number of species present (compact indices),
  * C = 128, NT1 / NT2 = symmetric-contraction coefficient counts (mace_b200_sc_layout). */
@@ -336,6 +340,62 @@ int mace_b200_csr_rows(const int32_t* pair_i, int64_t e0, int64_t e1, int32_t a,
  * every pass-B chunk as soon as pass A has produced the features of all its senders while later chunks still
  * arrive. */
 int mace_b200_sender_range(const int32_t* pair_j, int64_t e0, int64_t e1, int32_t* out, void* stream);
+
+/* ---------------------------------------------------------------- layer norm (no counterpart in the reference)
+ * y = (x - mean) rstd w + b over the last d elements of n rows that are ldx elements apart (y is dense), mean and
+ * rstd = 1 / sqrt(var + eps) in fp32; w / b may be null (1 / 0) and have type ptype (the type of x, or fp32).
+ * mean / rstd [n] are written when not null (both or none); the backward pass reads them.
+ * bwd: dx (may be null) dense [n][d]; dw / db [d] of type ptype (may be null), summed over the rows in a fixed order
+ * through `workspace` (mace_b200_layer_norm_bwd_workspace floats; unused when both are null). */
+int mace_b200_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean,
+                             float* rstd, int64_t n, int32_t d, double eps, int32_t dtype, int32_t ptype, void* stream);
+int mace_b200_layer_norm_bwd_workspace(int64_t n, int32_t d, int64_t* floats);
+int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                             const float* mean, const float* rstd, void* dx, void* dw, void* db, float* workspace,
+                             int64_t n, int32_t d, int32_t dtype, int32_t ptype, void* stream);
+
+/* ---------------------------------------------------------------- routing to experts (no counterpart in the reference)
+ * For each of n rows of E logits (ldl apart): scores s = softmax or sigmoid; the k experts of highest s + bias[e]
+ * (bias null: of highest logit), ties to the lowest index, NaN first.  Logits of -inf are closed.  groups > 1 (a
+ * divisor of E, at most 32): only the top_groups groups with the highest sum of their two best open values stay open.
+ * experts [n][k] (best first; -1 where nothing is open), weights [n][k] = scale s / sum of the chosen s (renormalize)
+ * or scale s; 0 for -1, and 0 when that sum is 0.
+ * bwd: dlogits [n][E] (dense, type of the logits) from dweights [n][k]; the choice is constant. */
+#define MB_ROUTE_MAX_EXPERTS 512
+#define MB_ROUTE_MAX_K 32
+int mace_b200_route_fwd(const void* logits, int64_t ldl, const float* bias, float* weights, int32_t* experts, int64_t n,
+                        int32_t E, int32_t k, int32_t softmax, int32_t groups, int32_t top_groups, int32_t renormalize,
+                        float scale, int32_t dtype, void* stream);
+int mace_b200_route_bwd(const float* dweights, const void* logits, int64_t ldl, const int32_t* experts, void* dlogits,
+                        int64_t n, int32_t E, int32_t k, int32_t softmax, int32_t renormalize, float scale,
+                        int32_t dtype, void* stream);
+
+/* ---------------------------------------------------------------- expert products (no counterpart in the reference)
+ * Slot s = t k + j of token t goes through W[experts[s]], W [E][O][D]; experts[s] = -1: no contribution, zero gradient.
+ *   weights [tokens][k]: out [tokens][O] = sum_j weights[t][j] W x;   weights null: out [tokens][k][O] = W x.
+ * x: rows of D elements, ldx apart, one per token or (x_per_slot) one per slot; dtype of x, W, out, dy, dx, dW;
+ * products accumulate in fp32 (fp32 data at fp32 accuracy).
+ * expert_plan sorts the slots by expert (mace_b200_expert_plan_words int32 words at `plan`); word 1 holds status bits
+ * (MB_ST_BAD_EXPERT, MB_ST_TC_TIMEOUT).  fwd and bwd run on the tensor cores and need a plan and
+ * mace_b200_expert_linear_workspace bytes (256-byte aligned); few needs neither and reads the indices directly (at
+ * most MB_FEW_MAX_SLOTS slots; an index outside [0, E) counts as -1).
+ * bwd: dy as out; dx as x but dense, dw [E][O][D], dweights [tokens][k]; any may be null (dweights needs weights). */
+#define MB_PLAN_MAX_EXPERTS 1024
+#define MB_FEW_MAX_SLOTS 4096
+int mace_b200_expert_plan_words(int64_t slots, int32_t E, int64_t* words);
+int mace_b200_expert_plan(const int32_t* experts, int64_t slots, int32_t E, int32_t* plan, void* stream);
+int mace_b200_expert_linear_workspace(int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O, int32_t dtype,
+                                      int32_t x_per_slot, int32_t weighted, int32_t backward, int64_t* bytes);
+int mace_b200_expert_linear_few(const void* x, int64_t ldx, int32_t x_per_slot, const void* w, const int32_t* experts,
+                                const float* weights, void* out, int64_t tokens, int32_t k, int32_t E, int32_t D,
+                                int32_t O, int32_t dtype, void* stream);
+int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x_per_slot, const void* w, const int32_t* plan,
+                                const float* weights, void* out, void* workspace, int64_t tokens, int32_t k, int32_t E,
+                                int32_t D, int32_t O, int32_t dtype, void* stream);
+int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_t ldx, int32_t x_per_slot, const void* w,
+                                const int32_t* plan, const float* weights, void* dx, void* dw, float* dweights,
+                                void* workspace, int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
+                                int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,656 @@
+// Products with per-token experts: slot s = (t, j) of a token's k choices goes through the matrix W[experts[s]].
+//   z_s = W_e x_t (or x_s),   out_t = sum_j g_tj z_tj  (or out_s = z_s without weights)
+//   dx_t = sum_j g_tj W_e^T dy_t,  dW_e = sum over e's slots of g_s dy_t x_t^T,  dg_s = <dy_t, W_e x_t> = <x_t, W_e^T dy_t>
+// This file holds the plan (slots sorted by expert), the few-slots form, and the kernels that move rows: gather into
+// expert order, sum of a token's rows.  The products themselves are in experts_gemm.cu.
+//
+// fp32 operands become three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits
+// of mantissa, and bf16 has the exponent range of fp32, so nothing overflows that fp32 holds.
+#include "experts.cuh"
+
+namespace mb {
+
+// ------------------------------------------------------------------------------------------------ plan
+// Stable counting sort of the slots by expert.  count: per-block histograms; scan: rows of each (expert, block);
+// place: rank of a slot among its expert's slots of the block, warp by warp (match_any), so the order is the slots'.
+// Slots with expert -1 get no row; other values outside [0, E) set MB_ST_BAD_EXPERT and get none either.
+
+__device__ __forceinline__ int xp_expert(const int32_t* experts, int64_t s, int64_t R, int E, bool& bad) {
+  if (s >= R) return -1;
+  const int e = experts[s];
+  bad |= e < -1 || e >= E;
+  return e >= 0 && e < E ? e : -1;
+}
+
+__global__ void __launch_bounds__(256) k_plan_count(const int32_t* experts, const XPlan p, int32_t* plan) {
+  extern __shared__ int cnt[];
+  for (int e = threadIdx.x; e < p.E; e += 256) cnt[e] = 0;
+  __syncthreads();
+  bool bad = false;
+  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK;
+  for (int i = threadIdx.x; i < XP_CHUNK; i += 256) {
+    const int e = xp_expert(experts, s0 + i, p.R, p.E, bad);
+    if (e >= 0) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += 256) plan[p.o_hist + (int64_t)e * p.nblk + blockIdx.x] = cnt[e];
+}
+
+// Segments, tiles and padding rows from the counts of all experts (cnt in shared memory; the whole block calls it)
+__device__ __forceinline__ void xp_segments(const XPlan& p, int32_t* plan, const int* cnt, int* seg) {
+  if (threadIdx.x < 32) {
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + threadIdx.x;
+      const int rows = e < p.E ? (cnt[e] + XP_BM - 1) / XP_BM * XP_BM : 0;
+      int inc = rows;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if ((int)threadIdx.x >= o) inc += v;
+      }
+      if (e < p.E) seg[e] = run + inc - rows;
+      run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (threadIdx.x == 0) {
+      seg[p.E] = run;
+      plan[0] = run / XP_BM;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= p.E; e += blockDim.x) {
+    plan[p.o_seg + e] = seg[e];
+    if (e < p.E) plan[p.o_cnt + e] = cnt[e];
+  }
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  for (int e = threadIdx.x >> 5; e < p.E; e += nw) {
+    for (int r = seg[e] + cnt[e] + lane; r < seg[e + 1]; r += 32) plan[p.o_row + r] = -1;
+    for (int t = seg[e] / XP_BM + lane; t < seg[e + 1] / XP_BM; t += 32) plan[p.o_tile + t] = e;
+  }
+}
+
+__global__ void __launch_bounds__(1024) k_plan_scan(const XPlan p, int32_t* plan) {
+  extern __shared__ int sm[];
+  int *cnt = sm, *seg = sm + p.E;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) plan[1] = 0;
+  for (int e = threadIdx.x >> 5; e < p.E; e += 32) {
+    int32_t* h = plan + p.o_hist + (int64_t)e * p.nblk;
+    int run = 0;
+    for (int b0 = 0; b0 < p.nblk; b0 += 32) {
+      const int v = b0 + lane < p.nblk ? h[b0 + lane] : 0;
+      int inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int q = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += q;
+      }
+      if (b0 + lane < p.nblk) h[b0 + lane] = run + inc - v;
+      run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) cnt[e] = run;
+  }
+  __syncthreads();
+  xp_segments(p, plan, cnt, seg);
+}
+
+// Places the slots [s0, s0 + nw * per) of this block, warp w the w-th `per` of them; base[w][e] = next row of expert e
+// for warp w (shared memory), advanced here.
+__device__ __forceinline__ void xp_place(const int32_t* experts, const XPlan& p, int32_t* plan, int64_t s0, int per,
+                                         int* base) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int* mine = base + warp * p.E;
+  bool bad = false;
+  for (int i = 0; i < per; i += 32) {
+    const int64_t s = s0 + (int64_t)warp * per + i + lane;
+    const int e = xp_expert(experts, s, p.R, p.E, bad);
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    const int first = __ffs(same) - 1;
+    int at = 0;
+    if (e >= 0 && lane == first) {
+      at = mine[e];
+      mine[e] = at + __popc(same);
+    }
+    at = __shfl_sync(0xffffffffu, at, first) + rank;
+    if (e >= 0) plan[p.o_row + at] = (int)s;
+    if (s < p.R) plan[p.o_slot + s] = e >= 0 ? at : -1;
+    __syncwarp();
+  }
+  if (bad) atomicOr((unsigned*)plan + 1, (unsigned)MB_ST_BAD_EXPERT);
+}
+
+// counts per (warp, expert) of the block's slots into base[w][e] (zeroed by the caller)
+__device__ __forceinline__ void xp_warp_counts(const int32_t* experts, const XPlan& p, int64_t s0, int per, int* base) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool bad = false;
+  for (int i = 0; i < per; i += 32) {
+    const int e = xp_expert(experts, s0 + (int64_t)warp * per + i + lane, p.R, p.E, bad);
+    if (e >= 0) atomicAdd(&base[warp * p.E + e], 1);
+  }
+}
+
+__global__ void __launch_bounds__(256) k_plan_place(const int32_t* experts, const XPlan p, int32_t* plan) {
+  extern __shared__ int base[];                  // [8][E]
+  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK;
+  for (int i = threadIdx.x; i < 8 * p.E; i += 256) base[i] = 0;
+  __syncthreads();
+  xp_warp_counts(experts, p, s0, XP_CHUNK / 8, base);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += 256) {
+    int run = plan[p.o_seg + e] + plan[p.o_hist + (int64_t)e * p.nblk + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const int c = base[w * p.E + e];
+      base[w * p.E + e] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+  xp_place(experts, p, plan, s0, XP_CHUNK / 8, base);
+}
+
+// All three steps in one block, for few slots: one launch instead of three
+__global__ void __launch_bounds__(1024) k_plan_one(const int32_t* experts, const XPlan p, int32_t* plan, int per) {
+  extern __shared__ int sm[];
+  int *cnt = sm, *seg = cnt + p.E, *base = seg + p.E + 1;   // base [32][E]
+  for (int i = threadIdx.x; i < 32 * p.E; i += 1024) base[i] = 0;
+  if (threadIdx.x == 0) plan[1] = 0;
+  __syncthreads();
+  xp_warp_counts(experts, p, 0, per, base);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += 1024) {
+    int run = 0;
+#pragma unroll 8
+    for (int w = 0; w < 32; ++w) {
+      const int c = base[w * p.E + e];
+      base[w * p.E + e] = run;
+      run += c;
+    }
+    cnt[e] = run;
+  }
+  __syncthreads();
+  xp_segments(p, plan, cnt, seg);
+  for (int i = threadIdx.x; i < 32 * p.E; i += 1024) base[i] += seg[i % p.E];
+  __syncthreads();
+  xp_place(experts, p, plan, 0, per, base);
+}
+
+// ------------------------------------------------------------------------------------------------ row movement
+// 8 columns [c0, c0 + 8) of a row as floats (0 beyond d)
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c0, int d, bool vec, float (&f)[8]) {
+  if (vec && c0 + 8 <= d) {
+    if constexpr (sizeof(T) == 2) {
+      unpack16(*reinterpret_cast<const uint4*>(row + c0), f, T());
+    } else {
+      load_p<float, 8>(row + c0, f);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = c0 + q < d ? to_f(row[c0 + q]) : 0.f;
+  }
+}
+
+// Writes 8 columns as one vector of a 16-bit plane, or of three bf16 planes (fp32 data)
+template <typename T>
+__device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64_t at, const float (&f)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(dst + at) = pack16<T>(f);
+  } else {
+    float r[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) r[q] = f[q];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint4 u = pack16<bf16>(r);
+      *reinterpret_cast<uint4*>(dst + p * plane + at) = u;
+      float h[8];
+      unpack16(u, h, bf16());
+#pragma unroll
+      for (int q = 0; q < 8; ++q) r[q] -= h[q];
+    }
+  }
+}
+
+// Rows in expert order: out0[row] = src[slot / kdiv], out1[row] = scale[slot] src[slot / kdiv] (either may be null),
+// zeros in padding rows and in the columns that pad the width to dp.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_gather(const T* src, int64_t lds, int d, int dp, bool vec, int kdiv,
+                                                     const int32_t* plan, const XPlan p, const float* scale,
+                                                     uint16_t* out0, uint16_t* out1, int64_t plane) {
+  const int lane = threadIdx.x & 31;
+  const int64_t used = (int64_t)plan[0] * XP_BM;
+  const int64_t step = (int64_t)gridDim.x * 8;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < used; row += step) {
+    const int slot = plan[p.o_row + row];
+    const T* s = src + (slot < 0 ? 0 : slot / kdiv) * lds;
+    const float g = scale && slot >= 0 ? scale[slot] : 1.f;
+    for (int c = lane * 8; c < dp; c += 256) {
+      float f[8];
+      if (slot >= 0) {
+        load8(s, c, d, vec, f);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = 0.f;
+      }
+      if (out0) store_planes<T>(out0, plane, row * dp + c, f);
+      if (out1) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] *= g;
+        store_planes<T>(out1, plane, row * dp + c, f);
+      }
+    }
+  }
+}
+
+// [rows][d] -> 16-bit planes [rows][dp], columns padded with zeros
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_stage(const T* src, int64_t rows, int d, int dp, bool vec, uint16_t* out,
+                                                    int64_t plane) {
+  const int nv = dp / 8;
+  const int64_t total = rows * nv, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t r = i / nv;
+    const int c = (int)(i - r * nv) * 8;
+    float f[8];
+    load8(src + r * d, c, d, vec, f);
+    store_planes<T>(out, plane, r * dp + c, f);
+  }
+}
+
+// out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an expert; dg[slot] = sum of
+// the partial products.  buf null: only dg.  One warp per token.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
+                                                  bool vec, const int32_t* slot_row, const float* dgpart, int nparts,
+                                                  float* dg) {
+  const int lane = threadIdx.x & 31;
+  const int64_t R = tokens * k;
+  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)gridDim.x * 8) {
+    if (dg)
+      for (int j = lane; j < k; j += 32) {
+        float s = 0.f;
+        if (slot_row[t * k + j] >= 0)
+          for (int q = 0; q < nparts; ++q) s += dgpart[q * R + t * k + j];
+        dg[t * k + j] = s;
+      }
+    if (!buf) continue;
+    for (int c = lane * 8; c < d; c += 256) {
+      float s[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s[q] = 0.f;
+#pragma unroll 4
+      for (int j = 0; j < k; ++j) {
+        if (slot_row[t * k + j] < 0) continue;
+        float f[8];
+        load8(buf + (t * k + j) * ldb, c, d, true, f);   // ldb is padded: whole vectors wherever c + 8 <= d
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[q] += f[q];
+      }
+      T* o = out + t * d + c;
+      if (vec && c + 8 <= d) {
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(o) = pack16<T>(s);
+        } else {
+          reinterpret_cast<float4*>(o)[0] = make_float4(s[0], s[1], s[2], s[3]);
+          reinterpret_cast<float4*>(o)[1] = make_float4(s[4], s[5], s[6], s[7]);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (c + q < d) o[q] = from_f<T>(s[q]);
+      }
+    }
+  }
+}
+
+// Zeros the rows of slots without an expert (the products write every other row)
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_zero(T* out, int64_t slots, int d, const int32_t* slot_row) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t s = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); s < slots; s += (int64_t)gridDim.x * 8)
+    if (slot_row[s] < 0)
+      for (int c = lane; c < d; c += 32) out[s * d + c] = from_f<T>(0.f);
+}
+
+// ------------------------------------------------------------------------------------------------ few slots
+// out[t][o] = sum_j g_tj <W[e_tj][o], x> without a plan: one warp per (token, output), the k rows of W side by side in
+// flight.  Bound by the bytes of W; a row of W that several tokens use comes from L2 after the first.
+// SLOTS: out[slot][o] = <W[e][o], x>, one warp per (slot, output).
+template <typename T, int V, bool SLOTS>
+__global__ void __launch_bounds__(128) k_expert_few(const T* x, int64_t ldx, int kx, const T* w, const int32_t* experts,
+                                                    const float* g, T* out, int k, int E, int d, int o_n) {
+  const int lane = threadIdx.x & 31, o = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (o >= o_n) return;
+  const int64_t t = blockIdx.y;
+  const int n = SLOTS ? 1 : k;
+  float total = 0.f;
+  for (int j0 = 0; j0 < n; j0 += 4) {
+    const T *wr[4], *xr[4];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int J = SLOTS ? 1 : 4;
+#pragma unroll
+    for (int q = 0; q < J; ++q) {
+      const int64_t s = SLOTS ? t : t * k + j0 + q;
+      const int e = j0 + q < n ? experts[s] : -1;
+      wr[q] = e >= 0 && e < E ? w + ((int64_t)e * o_n + o) * d : nullptr;
+      xr[q] = x + s / kx * ldx;
+    }
+#pragma unroll 4
+    for (int c = lane * V; c < d; c += 32 * V) {
+#pragma unroll
+      for (int q = 0; q < J; ++q) {
+        if (!wr[q]) continue;
+        float a[V], b[V];
+        load_v<T, V>(wr[q] + c, a);
+        load_v<T, V>(xr[q] + c, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[q] = fmaf(a[i], b[i], acc[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < J; ++q) {
+      const float z = warp_sum(acc[q]);
+      if (wr[q]) total += SLOTS ? z : g[t * k + j0 + q] * z;
+    }
+  }
+  if (lane == 0) out[t * o_n + o] = from_f<T>(total);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+static inline int pad8(int d) { return (d + 7) / 8 * 8; }
+
+struct XShape {
+  int64_t T, R;
+  int32_t k, E, D, O, dtype, np, Dp, Op;
+  XPlan lay;
+  int64_t rows;
+};
+
+static int x_shape(const char* who, XShape& s, int64_t T, int32_t k, int32_t E, int32_t D, int32_t O, int32_t dtype) {
+  if (T < 0 || k < 1 || E < 1 || E > MB_PLAN_MAX_EXPERTS || D < 1 || O < 1 || D > (1 << 24) || O > (1 << 24) ||
+      T > (int64_t)(1 << 29) / k) {
+    set_error("%s: bad sizes (tokens %lld, k %d, experts %d (at most %d), widths %d -> %d, at most 2^29 slots)", who,
+              (long long)T, k, E, MB_PLAN_MAX_EXPERTS, D, O);
+    return MB_E_ARG;
+  }
+  if (!dtype_ok(dtype)) {
+    set_error("%s: unsupported type %d", who, dtype);
+    return MB_E_ARG;
+  }
+  if (sm_count() < 1) {
+    set_error("%s: no CUDA device", who);
+    return MB_E_CUDA;
+  }
+  s.T = T; s.k = k; s.R = T * k; s.E = E; s.D = D; s.O = O; s.dtype = dtype;
+  s.np = dtype == MB_F32 ? 3 : 1;
+  s.Dp = pad8(D);
+  s.Op = pad8(O);
+  s.lay = xplan(s.R, E);
+  s.rows = s.lay.tiles * XP_BM;
+  return 0;
+}
+
+struct XWork {                                   // workspace cursor: byte offsets, 256-byte aligned
+  int64_t used = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
+struct XFwd {
+  int64_t xs = 0, ws = -1, y = -1, bytes = 0;
+};
+// the 16-bit matrices can be read as they are when their rows are whole 16-byte vectors
+static bool w_direct(const XShape& s, const void* w) { return s.dtype != MB_F32 && s.D % 8 == 0 && aligned16(w); }
+
+static XFwd x_fwd_layout(const XShape& s, bool combine, bool direct) {
+  XWork c;
+  XFwd f;
+  f.xs = c.take((int64_t)s.np * s.rows * s.Dp * 2);
+  if (!direct) f.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
+  if (combine && s.k > 1) f.y = c.take(s.R * s.Op * dtype_size(s.dtype));
+  f.bytes = c.used;
+  return f;
+}
+
+struct XBwd {
+  int64_t xs = -1, dys = -1, gdy = -1, ws = -1, dxb = -1, dgp = -1, bytes = 0;
+};
+static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direct, bool need_x, bool need_w,
+                         bool need_g) {
+  XWork c;
+  XBwd b;
+  const int64_t row2 = (int64_t)s.np * s.rows * 2;
+  if (need_w) b.xs = c.take(row2 * s.Dp);
+  if (need_x || need_g || (need_w && !combine)) b.dys = c.take(row2 * s.Op);
+  if (need_w && combine) b.gdy = c.take(row2 * s.Op);
+  if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
+  if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * dtype_size(s.dtype));
+  if (need_g) b.dgp = c.take(s.R * 4 * xgemm_n_tiles(XG_DGRAD, s.D));
+  b.bytes = c.used;
+  return b;
+}
+
+static unsigned x_grid(int64_t units) {
+  const int64_t most = (int64_t)16 * sm_count();
+  return (unsigned)(units < 1 ? 1 : units < most ? units : most);
+}
+
+template <typename F>
+static int x_types(int dtype, const F& f) {
+  if (dtype == MB_F32) return f(float());
+  return dtype == MB_BF16 ? f(bf16()) : f(f16());
+}
+
+template <typename T>
+static int x_stage_w(const XShape& s, const void* w, void* ws, cudaStream_t st) {
+  const int64_t rows = (int64_t)s.E * s.O;
+  k_rows_stage<T><<<x_grid((rows * (s.Dp / 8) + 255) / 256), 256, 0, st>>>(
+      (const T*)w, rows, s.D, s.Dp, aligned16(w) && s.D % 8 == 0, (uint16_t*)ws, rows * s.Dp);
+  return check_launch("expert_linear (stage)");
+}
+
+template <typename T>
+static int x_gather(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const int32_t* plan,
+                    const float* scale, void* out0, void* out1, cudaStream_t st) {
+  const bool vec = aligned16(src) && lds % 8 == 0;
+  k_rows_gather<T><<<x_grid((s.rows + 7) / 8), 256, 0, st>>>((const T*)src, lds, d, dp, vec, kdiv, plan, s.lay, scale,
+                                                             (uint16_t*)out0, (uint16_t*)out1, s.rows * dp);
+  return check_launch("expert_linear (gather)");
+}
+
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" int mace_b200_expert_plan_words(int64_t slots, int32_t E, int64_t* words) {
+  if (slots < 0 || slots > (int64_t)1 << 29 || E < 1 || E > MB_PLAN_MAX_EXPERTS || !words) {
+    set_error("expert_plan: bad sizes (slots %lld, experts %d, at most %d)", (long long)slots, E, MB_PLAN_MAX_EXPERTS);
+    return MB_E_ARG;
+  }
+  *words = xplan(slots, E).words;
+  return 0;
+}
+
+extern "C" int mace_b200_expert_plan(const int32_t* experts, int64_t slots, int32_t E, int32_t* plan, void* stream) {
+  int64_t words = 0;
+  if (int rc = mace_b200_expert_plan_words(slots, E, &words)) return rc;
+  if (!plan || (slots > 0 && !experts)) {
+    set_error("expert_plan: null pointer");
+    return MB_E_ARG;
+  }
+  const XPlan p = xplan(slots, E);
+  cudaStream_t st = (cudaStream_t)stream;
+  // one block up to 8192 slots (its 32 warps then take 256 slots each, as a block of the three-launch form does)
+  if (slots <= 8192 && E <= 256) {
+    const int per = (int)((slots + 1023) / 1024) * 32;
+    k_plan_one<<<1, 1024, (2 * E + 1 + 32 * E) * 4, st>>>(experts, p, plan, per);
+    return check_launch("expert_plan");
+  }
+  if (p.nblk > 0) {
+    k_plan_count<<<p.nblk, 256, E * 4, st>>>(experts, p, plan);
+    if (int rc = check_launch("expert_plan")) return rc;
+  }
+  k_plan_scan<<<1, 1024, (2 * E + 1) * 4, st>>>(p, plan);
+  if (int rc = check_launch("expert_plan")) return rc;
+  if (p.nblk > 0) {
+    k_plan_place<<<p.nblk, 256, 8 * E * 4, st>>>(experts, p, plan);
+    return check_launch("expert_plan");
+  }
+  return 0;
+}
+
+extern "C" int mace_b200_expert_linear_workspace(int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
+                                                 int32_t dtype, int32_t x_per_slot, int32_t weighted, int32_t backward,
+                                                 int64_t* bytes) {
+  XShape s;
+  if (int rc = x_shape("expert_linear_workspace", s, tokens, k, E, D, O, dtype)) return rc;
+  if (!bytes) {
+    set_error("expert_linear_workspace: null pointer");
+    return MB_E_ARG;
+  }
+  *bytes = backward ? x_bwd_layout(s, weighted != 0, x_per_slot != 0, false, true, true, weighted != 0).bytes
+                    : x_fwd_layout(s, weighted != 0, false).bytes;
+  return 0;
+}
+
+extern "C" int mace_b200_expert_linear_few(const void* x, int64_t ldx, int32_t x_per_slot, const void* w,
+                                           const int32_t* experts, const float* weights, void* out, int64_t tokens,
+                                           int32_t k, int32_t E, int32_t D, int32_t O, int32_t dtype, void* stream) {
+  XShape s;
+  if (int rc = x_shape("expert_linear_few", s, tokens, k, E, D, O, dtype)) return rc;
+  if (s.R > MB_FEW_MAX_SLOTS) {
+    set_error("expert_linear_few: %lld slots (at most %d)", (long long)s.R, MB_FEW_MAX_SLOTS);
+    return MB_E_ARG;
+  }
+  if (s.R == 0) return 0;
+  if (!x || !w || !experts || !out || ldx < D) {
+    set_error("expert_linear_few: null pointer or row stride %lld below the width", (long long)ldx);
+    return MB_E_ARG;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  return x_types(dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = kVec<T>;
+    const bool vec = D % V == 0 && ldx % V == 0 && aligned16(x) && aligned16(w);
+    const int kx = x_per_slot ? 1 : k;
+    const dim3 grid((O + 3) / 4, (unsigned)(weights ? tokens : s.R));
+    auto go = [&](auto kern) {
+      kern<<<grid, 128, 0, st>>>((const T*)x, ldx, kx, (const T*)w, experts, weights, (T*)out, k, E, D, O);
+      return check_launch("expert_linear_few");
+    };
+    if (weights) return vec ? go(k_expert_few<T, V, false>) : go(k_expert_few<T, 1, false>);
+    return vec ? go(k_expert_few<T, V, true>) : go(k_expert_few<T, 1, true>);
+  });
+}
+
+extern "C" int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x_per_slot, const void* w,
+                                           const int32_t* plan, const float* weights, void* out, void* workspace,
+                                           int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O, int32_t dtype,
+                                           void* stream) {
+  XShape s;
+  if (int rc = x_shape("expert_linear_fwd", s, tokens, k, E, D, O, dtype)) return rc;
+  if (s.R == 0) return 0;
+  if (!x || !w || !plan || !out || !workspace || ldx < D) {
+    set_error("expert_linear_fwd: null pointer or row stride %lld below the width", (long long)ldx);
+    return MB_E_ARG;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool combine = weights != nullptr, direct = w_direct(s, w);
+  const XFwd f = x_fwd_layout(s, combine, direct);
+  char* base = (char*)workspace;
+  return x_types(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (!direct)
+      if (int rc = x_stage_w<T>(s, w, base + f.ws, st)) return rc;
+    if (int rc = x_gather<T>(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, plan, nullptr, base + f.xs, nullptr, st)) return rc;
+    XGemm g{};
+    g.mode = XG_FWD; g.dtype = dtype;
+    g.a = base + f.xs; g.rows = s.rows; g.lda = s.Dp;
+    g.b = direct ? w : base + f.ws; g.ldb = s.Dp;
+    g.E = E; g.M = 0; g.N = O; g.K = D;
+    g.plan = plan; g.lay = s.lay; g.scale = weights;
+    const bool sum = f.y >= 0;
+    g.out = sum ? (void*)(base + f.y) : out;
+    g.ldo = sum ? s.Op : O;
+    if (int rc = xgemm_launch(g, st)) return rc;
+    const int32_t* slot_row = plan + s.lay.o_slot;
+    if (sum)
+      k_rows_sum<T><<<x_grid((tokens + 7) / 8), 256, 0, st>>>((const T*)(base + f.y), s.Op, (T*)out, tokens, k, O,
+                                                              aligned16(out) && O % 8 == 0, slot_row, nullptr, 0, nullptr);
+    else
+      k_rows_zero<T><<<x_grid((s.R + 7) / 8), 256, 0, st>>>((T*)out, s.R, O, slot_row);
+    return check_launch("expert_linear_fwd");
+  });
+}
+
+extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_t ldx, int32_t x_per_slot,
+                                           const void* w, const int32_t* plan, const float* weights, void* dx, void* dw,
+                                           float* dweights, void* workspace, int64_t tokens, int32_t k, int32_t E,
+                                           int32_t D, int32_t O, int32_t dtype, void* stream) {
+  XShape s;
+  if (int rc = x_shape("expert_linear_bwd", s, tokens, k, E, D, O, dtype)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (s.R == 0) {
+    if (dw && cudaMemsetAsync(dw, 0, (int64_t)E * O * D * dtype_size(dtype), st) != cudaSuccess)
+      return check_launch("expert_linear_bwd");
+    return 0;
+  }
+  if (!dy || !x || !w || !plan || !workspace || ldx < D || (dweights && !weights)) {
+    set_error("expert_linear_bwd: null pointer or row stride %lld below the width", (long long)ldx);
+    return MB_E_ARG;
+  }
+  const bool combine = weights != nullptr, direct = w_direct(s, w);
+  const XBwd b = x_bwd_layout(s, combine, x_per_slot != 0, direct, dx != nullptr, dw != nullptr, dweights != nullptr);
+  char* base = (char*)workspace;
+  const int kx = x_per_slot ? 1 : k, ky = combine ? k : 1;
+  return x_types(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (b.dys >= 0 || b.gdy >= 0)
+      if (int rc = x_gather<T>(s, dy, O, O, s.Op, ky, plan, weights, b.dys >= 0 ? base + b.dys : nullptr,
+                               b.gdy >= 0 ? base + b.gdy : nullptr, st))
+        return rc;
+    if (dw) {
+      if (int rc = x_gather<T>(s, x, ldx, D, s.Dp, kx, plan, nullptr, base + b.xs, nullptr, st)) return rc;
+      XGemm g{};
+      g.mode = XG_WGRAD; g.dtype = dtype;
+      g.a = combine ? base + b.gdy : base + b.dys; g.lda = s.Op;
+      g.b = base + b.xs; g.ldb = s.Dp;
+      g.rows = s.rows;
+      g.E = E; g.M = O; g.N = D; g.K = 0;
+      g.plan = plan; g.lay = s.lay; g.out = dw; g.ldo = D;
+      if (int rc = xgemm_launch(g, st)) return rc;
+    }
+    if (!dx && !dweights) return 0;
+    if (!direct)
+      if (int rc = x_stage_w<T>(s, w, base + b.ws, st)) return rc;
+    XGemm g{};
+    g.mode = XG_DGRAD; g.dtype = dtype;
+    g.a = base + b.dys; g.rows = s.rows; g.lda = s.Op;
+    g.b = direct ? w : base + b.ws; g.ldb = s.Dp;
+    g.E = E; g.M = 0; g.N = D; g.K = O;
+    g.plan = plan; g.lay = s.lay; g.scale = weights;
+    const bool sum = b.dxb >= 0;
+    g.out = sum ? (void*)(base + b.dxb) : dx;
+    g.ldo = sum ? s.Dp : D;
+    if (dweights) {
+      g.x = x; g.ldx = ldx; g.kdiv = kx;
+      g.dgpart = (float*)(base + b.dgp);
+    }
+    if (int rc = xgemm_launch(g, st)) return rc;
+    const int32_t* slot_row = plan + s.lay.o_slot;
+    if (dx && !sum) {
+      k_rows_zero<T><<<x_grid((s.R + 7) / 8), 256, 0, st>>>((T*)dx, s.R, D, slot_row);
+      if (int rc = check_launch("expert_linear_bwd")) return rc;
+    }
+    if (!sum && !dweights) return 0;
+    k_rows_sum<T><<<x_grid((tokens + 7) / 8), 256, 0, st>>>(
+        sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, aligned16(dx) && D % 8 == 0, slot_row,
+        (const float*)(base + b.dgp), dweights ? xgemm_n_tiles(XG_DGRAD, D) : 0, dweights);
+    return check_launch("expert_linear_bwd");
+  });
+}

@@ -1,0 +1,61 @@
+// Expert products: what the planning / data-movement kernels (experts.cu) and the tensor-core kernel
+// (experts_gemm.cu) share.
+#pragma once
+
+#include "dtypes.cuh"
+
+namespace mb {
+
+// Layout of a plan (int32 words) for R slots and E experts.  The slots of one expert become consecutive rows, padded to
+// whole tiles of XP_BM rows, so that a tile belongs to one expert.
+constexpr int XP_BM = 128;                       // rows of a tile
+constexpr int XP_CHUNK = 2048;                   // slots per block of the counting and placing kernels
+struct XPlan {
+  int64_t R;
+  int32_t E, nblk;
+  int64_t tiles;                                 // most tiles there can be
+  int64_t o_seg, o_cnt, o_tile, o_row, o_slot, o_hist, words;
+};
+// header words: 0 = tiles in use, 1 = status bits
+inline XPlan xplan(int64_t R, int32_t E) {
+  XPlan p;
+  p.R = R;
+  p.E = E;
+  p.nblk = (int32_t)((R + XP_CHUNK - 1) / XP_CHUNK);
+  p.tiles = R / XP_BM + (R < E ? R : E);
+  p.o_seg = 8;                                   // [E + 1] first row of each expert
+  p.o_cnt = p.o_seg + E + 1;                     // [E] slots of each expert
+  p.o_tile = p.o_cnt + E;                        // [tiles] expert of each tile
+  p.o_row = p.o_tile + p.tiles;                  // [tiles * XP_BM] slot of each row, -1 = padding
+  p.o_slot = p.o_row + p.tiles * XP_BM;          // [R] row of each slot, -1 = no expert
+  p.o_hist = p.o_slot + R;                       // [E][nblk] scratch
+  p.words = p.o_hist + (int64_t)E * p.nblk;
+  return p;
+}
+
+enum { XG_FWD = 0, XG_DGRAD = 1, XG_WGRAD = 2 };
+
+// One launch of the tensor-core kernel.  Operands are 16-bit planes (fp32 data: three bf16 planes).
+//   FWD    rows of `a` [planes][rows][lda] (expert-sorted), b = w [planes][E][O][ldb]: C[row][o] = sum_d a[row][d] w[e][o][d]
+//   DGRAD  the same rows with width O, b = w: C[row][d] = sum_o a[row][o] w[e][o][d]
+//   WGRAD  a [planes][rows][lda] (width M = O), b [planes][rows][ldb] (width N = D): C[e][o][d] = sum over e's rows
+struct XGemm {
+  int mode, dtype;
+  const void *a, *b;
+  int64_t rows, lda, ldb;                        // rows per plane; strides in elements, multiples of 8
+  int32_t E, M, N, K;                            // WGRAD: M = O, N = D; else N, K of the product
+  const int32_t* plan;
+  XPlan lay;
+  const float* scale;                            // per slot, or null
+  void* out;                                     // FWD / DGRAD: [slots][ldo] (null: only dgpart); WGRAD: [E][M][N]
+  int64_t ldo;
+  // DGRAD: dgpart[n tile][slot] = partial <x, C> of the slot's x row (null: off)
+  const void* x;
+  int64_t ldx;
+  int32_t kdiv;                                  // slot / kdiv = row of x
+  float* dgpart;
+};
+int xgemm_n_tiles(int mode, int64_t N);
+int xgemm_launch(const XGemm& g, cudaStream_t st);
+
+}  // namespace mb

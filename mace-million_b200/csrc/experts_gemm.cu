@@ -1,0 +1,445 @@
+// The three expert products on the 5th-generation tensor cores (tcgen05 kind::f16, fp32 accumulators in TMEM):
+//   FWD    C[row][o] = sum_d x[row][d] W[e][o][d]        both operands K-major
+//   DGRAD  C[row][d] = sum_o dy[row][o] W[e][o][d]       W is MN-major (its rows run along N)
+//   WGRAD  C[e][o][d] = sum over e's rows dy[row][o] x[row][d]   both MN-major, K = the expert's rows
+// Rows are sorted by expert and padded to 128, so a 128-row tile (FWD, DGRAD) or a 64-row K block (WGRAD) has one expert,
+// and no matrix is transposed in memory: the MN-major operands are read as they lie.
+// fp32 data comes as three bf16 planes; the products of the planes whose ranks add up to at most 2 (six of nine, small
+// ones first) accumulate in the same fp32 accumulator, the rest is below 2^-24 of the result.
+//
+// Persistent CTA, one per SM: warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
+// (128 x BN x 16) into one of two TMEM accumulators, warps 2-5 drain the other one (one row per lane), scale the row by
+// its slot's weight and write it to the slot's place in the output.  Every wait is bounded: on expiry the kernel sets
+// MB_ST_TC_TIMEOUT in the plan's status word, drains its copies and MMAs, frees its TMEM and returns.
+#include <cuda.h>
+
+#include "experts.cuh"
+#include "tc.cuh"
+
+namespace mb {
+
+constexpr int XG_BM = XP_BM, XG_BK = 64, XG_THREADS = 192;
+constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
+
+template <int BN>
+struct XgCfg {
+  static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN * XG_BK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 196608 / STAGE;              // 192 KB ring: 4 stages at BN = 256, 6 at 128
+  static constexpr int TMEM = 2 * BN;
+  static constexpr int SMEM = STAGES * STAGE + 256 + 1024;   // + barriers, alignment slack
+};
+
+struct XgParams {
+  int32_t E, M, N, K, tn, tm, np;                // tn / tm: tiles along N, along M (WGRAD)
+  int64_t rows;                                  // rows per plane of the sorted operands
+  int32_t w_rows;                                // E (planes of w follow each other)
+  const int32_t* plan;
+  XPlan lay;
+  const float* scale;
+  void* out;
+  int64_t ldo;
+  const void* x;
+  int64_t ldx;
+  int32_t kdiv;
+  float* dgpart;
+};
+
+struct XgBars {
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int failed;
+};
+
+// planes of A and B multiplied in pass p (of 6): small products first
+__device__ __forceinline__ int xg_plane_a(int p) { return (0x021010 >> (4 * (5 - p))) & 0xF; }
+__device__ __forceinline__ int xg_plane_b(int p) { return (0x201100 >> (4 * (5 - p))) & 0xF; }
+
+// Writes up to 32 consecutive values of one row (16-byte stores when the row pointer allows them)
+template <typename T>
+__device__ __forceinline__ void xg_store32(T* dst, const float (&f)[32], int n, bool vec) {
+  constexpr int V = kVec<T>;
+  if (vec && n >= 32) {
+#pragma unroll
+    for (int q = 0; q < 32 / V; ++q) {
+      float t[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) t[i] = f[q * V + i];
+      *reinterpret_cast<uint4*>(dst + q * V) = pack16<T>(t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) dst[i] = from_f<T>(f[i]);
+  }
+}
+
+template <int MODE, typename T, int BN>
+__global__ void __launch_bounds__(XG_THREADS, 1)
+    k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
+  using C = XgCfg<BN>;
+  constexpr bool A_MN = MODE == XG_WGRAD, B_MN = MODE != XG_FWD;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  XgBars& B = *reinterpret_cast<XgBars*>(smem + C::STAGES * C::STAGE);
+  volatile int* failed = &B.failed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
+                 "r"(C::TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (lane == 0) {
+      for (int s = 0; s < C::STAGES; ++s) {
+        mbar_init(&B.full[s], 1);
+        mbar_init(&B.empty[s], 1);
+      }
+      for (int a = 0; a < 2; ++a) {
+        mbar_init(&B.acc_full[a], 1);
+        mbar_init(&B.acc_empty[a], 128);
+      }
+      B.failed = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = B.tmem;
+  const int32_t* plan = g.plan;
+  const int tiles = MODE == XG_WGRAD ? g.E * g.tm * g.tn : plan[0] * g.tn;
+
+  // tile -> (expert, first row of A / first output row, first column, K blocks)
+  struct Tile {
+    int e, m0, n0, r0, nk;
+  };
+  auto tile_of = [&](int t) {
+    Tile o;
+    const int m = t / g.tn;
+    o.n0 = (t - m * g.tn) * BN;
+    if constexpr (MODE == XG_WGRAD) {
+      o.e = m / g.tm;
+      o.m0 = (m - o.e * g.tm) * XG_BM;
+      o.r0 = plan[g.lay.o_seg + o.e];
+      o.nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK;
+    } else {
+      o.e = plan[g.lay.o_tile + m];
+      o.m0 = o.r0 = m * XG_BM;
+      o.nk = (g.K + XG_BK - 1) / XG_BK;
+    }
+    return o;
+  };
+  const int p0 = g.np == 3 ? 0 : 5;              // passes over the planes: p0 .. 5
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------ loads
+    if (lane == 0) {
+      int seq = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const Tile w = tile_of(t);
+        for (int p = p0; ok && p < 6; ++p) {
+          const int pa = xg_plane_a(p), pb = xg_plane_b(p);
+          for (int kb = 0; kb < w.nk; ++kb, ++seq) {
+            const int s = seq % C::STAGES;
+            if (*failed || !mbar_wait_ns(&B.empty[s], ((seq / C::STAGES) & 1) ^ 1, XG_WAIT_NS)) {
+              *failed = 1;
+              ok = false;
+              break;
+            }
+            const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+            uint64_t* bar = &B.full[s];
+            mbar_arrive_tx(bar, C::STAGE);
+            const int k0 = kb * XG_BK;
+            if constexpr (MODE == XG_WGRAD) {
+#pragma unroll
+              for (int c = 0; c < XG_BM / 64; ++c)
+                tma_load_2d(a + c * 8192, &map_a, w.m0 + 64 * c, (int)(pa * g.rows) + w.r0 + k0, bar);
+#pragma unroll
+              for (int c = 0; c < BN / 64; ++c)
+                tma_load_2d(b + c * 8192, &map_b, w.n0 + 64 * c, (int)(pb * g.rows) + w.r0 + k0, bar);
+            } else {
+              tma_load_2d(a, &map_a, k0, (int)(pa * g.rows) + w.m0, bar);
+              if constexpr (MODE == XG_FWD) {
+                tma_load_3d(b, &map_b, k0, w.n0, pb * g.w_rows + w.e, bar);
+              } else {
+#pragma unroll
+                for (int c = 0; c < BN / 64; ++c)
+                  tma_load_3d(b + c * 8192, &map_b, w.n0 + 64 * c, k0, pb * g.w_rows + w.e, bar);
+              }
+            }
+          }
+        }
+      }
+      // after a timeout: the copies already issued land before the block ends (bounded)
+      if (!ok)
+        for (int q = seq - C::STAGES < 0 ? 0 : seq - C::STAGES; q < seq; ++q)
+          mbar_wait_ns(&B.full[q % C::STAGES], (q / C::STAGES) & 1, XG_WAIT_NS);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      constexpr uint32_t idesc = f16_idesc(XG_BM, BN, !std::is_same<T, f16>::value, A_MN, B_MN);
+      int seq = 0, tc = 0;
+      bool ok = true;
+      uint64_t* last_bar = nullptr;
+      uint32_t last_par = 0;
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const Tile w = tile_of(t);
+        if (w.nk == 0) continue;
+        const int acc = tc & 1;
+        if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, XG_WAIT_NS)) {
+          *failed = 1;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)(acc * BN);
+        const int total = w.nk * (6 - p0);
+        for (int kb = 0; kb < total; ++kb, ++seq) {
+          const int s = seq % C::STAGES;
+          if (!mbar_wait_ns(&B.full[s], (seq / C::STAGES) & 1, XG_WAIT_NS)) {
+            *failed = 1;
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < XG_BK / 16; ++kk) {
+            // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
+            const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
+            const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
+            mma_f16_ss(d, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          mma_commit(&B.empty[s]);
+          last_bar = &B.empty[s];
+          last_par = (seq / C::STAGES) & 1;
+        }
+        if (!ok) break;
+        mma_commit(&B.acc_full[acc]);
+        last_bar = &B.acc_full[acc];
+        last_par = (tc >> 1) & 1;
+        ++tc;
+      }
+      // after a timeout: wait (bounded) for the MMAs already issued before the TMEM is freed
+      if (*failed && last_bar) mbar_wait_ns(last_bar, last_par, XG_WAIT_NS);
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------ epilogue
+    const int q4 = warp & 3, row = q4 * 32 + lane;
+    int tc = 0;
+    // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      if (__shfl_sync(0xffffffffu, *failed, 0)) break;
+      const Tile w = tile_of(t);
+      T* dst = nullptr;
+      float sc = 1.f, dot = 0.f;
+      const T* xr = nullptr;
+      int slot = -1;
+      if constexpr (MODE == XG_WGRAD) {
+        if (w.m0 + row < g.M) dst = (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo;
+      } else {
+        slot = plan[g.lay.o_row + w.m0 + row];
+        if (slot >= 0) {
+          if (g.out) dst = (T*)g.out + (int64_t)slot * g.ldo;
+          if (g.scale) sc = g.scale[slot];
+          if (MODE == XG_DGRAD && g.dgpart) xr = (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx;
+        }
+      }
+      const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+      const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
+      const int acc = tc & 1;
+      if (w.nk > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS))) {
+          *failed = 1;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const int nc = g.N - w.n0 < BN ? g.N - w.n0 : BN;
+#pragma unroll 1
+      for (int h = 0; h < BN / 32; ++h) {
+        if (32 * h >= nc) break;
+        float f[32];
+        if (w.nk > 0) {
+          uint32_t u[32];
+          tmem_ld32(tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + 32 * h), u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.f;
+        }
+        const int n = nc - 32 * h;
+        if (MODE == XG_DGRAD && xr) {
+          const T* xp = xr + w.n0 + 32 * h;
+          if (xvec && n >= 32) {
+#pragma unroll
+            for (int q = 0; q < 32 / kVec<T>; ++q) {
+              float v[kVec<T>];
+              load_v<T, kVec<T>>(xp + q * kVec<T>, v);
+#pragma unroll
+              for (int i = 0; i < kVec<T>; ++i) dot = fmaf(v[i], f[q * kVec<T> + i], dot);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < n) dot = fmaf(to_f(xp[i]), f[i], dot);
+          }
+        }
+        if (dst) {
+          if (MODE != XG_WGRAD) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] *= sc;
+          }
+          xg_store32<T>(dst + w.n0 + 32 * h, f, n, vec);
+        }
+      }
+      if (MODE == XG_DGRAD && xr) g.dgpart[(int64_t)(w.n0 / BN) * g.lay.R + slot] = dot;
+      if (w.nk > 0) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        mbar_arrive(&B.acc_empty[acc]);
+        ++tc;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (tid == 0 && *failed) atomicOr((unsigned*)plan + 1, (unsigned)MB_ST_TC_TIMEOUT);
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
+}
+
+// Tensor map of a 16-bit tensor, dimensions inner to outer, SWIZZLE_128B boxes 64 elements wide
+static int xg_map(CUtensorMap* m, bool is_bf16, int rank, const void* p, const int64_t* dims, const int64_t* strides,
+                  const int* box) {
+  EncodeTiled enc = encode_tiled();
+  if (!enc) {
+    set_error("expert_linear: the driver has no cuTensorMapEncodeTiled");
+    return MB_E_CUDA;
+  }
+  cuuint64_t d[3], s[2];
+  cuuint32_t b[3], es[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    if (i) s[i - 1] = (cuuint64_t)strides[i - 1] * 2;
+  }
+  const CUresult rc = enc(m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                          const_cast<void*>(p), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) {
+    set_error("expert_linear: cuTensorMapEncodeTiled failed (%d)", (int)rc);
+    return MB_E_CUDA;
+  }
+  return 0;
+}
+
+static int xg_bn(int64_t N) { return N <= 128 ? 128 : 256; }
+int xgemm_n_tiles(int mode, int64_t N) {
+  (void)mode;
+  return (int)((N + xg_bn(N) - 1) / xg_bn(N));
+}
+
+template <int MODE, typename T, int BN>
+static int xg_go(const XGemm& x, cudaStream_t st) {
+  using C = XgCfg<BN>;
+  static int ready_dev = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
+  auto kern = k_expert_gemm<MODE, T, BN>;
+  if (ready_dev != dev) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+      set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
+      return MB_E_CUDA;
+    }
+    ready_dev = dev;
+  }
+  const bool is_bf16 = !std::is_same<T, f16>::value;
+  const int np = x.dtype == MB_F32 ? 3 : 1;
+  CUtensorMap ma, mbm;
+  {
+    const int64_t dims[2] = {x.lda, np * x.rows}, str[1] = {x.lda};
+    const int box[2] = {64, MODE == XG_WGRAD ? XG_BK : XG_BM};
+    if (int rc = xg_map(&ma, is_bf16, 2, x.a, dims, str, box)) return rc;
+  }
+  if (MODE == XG_WGRAD) {
+    const int64_t dims[2] = {x.ldb, np * x.rows}, str[1] = {x.ldb};
+    const int box[2] = {64, XG_BK};
+    if (int rc = xg_map(&mbm, is_bf16, 2, x.b, dims, str, box)) return rc;
+  } else {
+    const int64_t O = MODE == XG_FWD ? x.N : x.K;
+    const int64_t dims[3] = {x.ldb, O, (int64_t)np * x.E}, str[2] = {x.ldb, x.ldb * O};
+    const int box[3] = {64, MODE == XG_FWD ? BN : XG_BK, 1};
+    if (int rc = xg_map(&mbm, is_bf16, 3, x.b, dims, str, box)) return rc;
+  }
+  XgParams g{};
+  g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K; g.np = np;
+  g.tn = (x.N + BN - 1) / BN;
+  g.tm = (x.M + XG_BM - 1) / XG_BM;
+  g.rows = x.rows; g.w_rows = x.E;
+  g.plan = x.plan; g.lay = x.lay; g.scale = x.scale;
+  g.out = x.out; g.ldo = x.ldo;
+  g.x = x.x; g.ldx = x.ldx; g.kdiv = x.kdiv; g.dgpart = x.dgpart;
+  const int64_t most = MODE == XG_WGRAD ? (int64_t)x.E * g.tm * g.tn : x.lay.tiles * g.tn;
+  if (most > 0x7fffffff || np * x.rows > 0x7fffffff) {
+    set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)most, (long long)(np * x.rows));
+    return MB_E_ARG;
+  }
+  if (most == 0) return 0;
+  const int sms = sm_count();
+  kern<<<(unsigned)(most < sms ? most : sms), XG_THREADS, C::SMEM, st>>>(ma, mbm, g);
+  return check_launch("expert_linear");
+}
+
+template <int MODE, typename T>
+static int xg_bn_any(const XGemm& x, cudaStream_t st) {
+  return xg_bn(x.N) == 128 ? xg_go<MODE, T, 128>(x, st) : xg_go<MODE, T, 256>(x, st);
+}
+
+template <int MODE>
+static int xg_type(const XGemm& x, cudaStream_t st) {
+  if (x.dtype == MB_F32) return xg_bn_any<MODE, float>(x, st);
+  return x.dtype == MB_BF16 ? xg_bn_any<MODE, bf16>(x, st) : xg_bn_any<MODE, f16>(x, st);
+}
+
+int xgemm_launch(const XGemm& x, cudaStream_t st) {
+  if (x.mode == XG_FWD) return xg_type<XG_FWD>(x, st);
+  return x.mode == XG_DGRAD ? xg_type<XG_DGRAD>(x, st) : xg_type<XG_WGRAD>(x, st);
+}
+
+int sm_count() {
+  static int dev_known = -1, sms = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev != dev_known) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    sms = n;
+    dev_known = dev;
+  }
+  return sms;
+}
+
+}  // namespace mb

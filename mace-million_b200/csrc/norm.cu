@@ -1,0 +1,530 @@
+// Layer norm over the last dimension of rows that may be strided (the 0e block of the node features has rows 512 apart):
+//   mu = mean(x), var = mean((x - mu)^2), r = 1 / sqrt(var + eps), xh = (x - mu) r, y = xh w + b
+// and its backward pass, with a = dy w:
+//   dx = r (a - mean(a) - xh mean(a xh)), dw = sum over rows of dy xh, db = sum over rows of dy.
+// Statistics and sums are fp32 whatever the type of x; every output is rounded once.
+//
+// Bound: HBM bytes (forward x and y, backward x, dy and dx, each once).  A row stays in registers between the sums
+// and the output, so nothing is read twice.  Groups of G threads own a row; an element's column belongs to the same
+// thread in every row, so the backward pass accumulates dw and db in registers over the rows of a block, and a second
+// small kernel adds the blocks' partial sums in a fixed order (no atomics: results do not depend on the schedule).
+// V is the elements per access: 16 bytes where the width, the row strides and the addresses allow it, else 1.
+// Widths that no group holds in registers take the *_wide kernels, which read the row once per sum.
+#include "dtypes.cuh"
+
+namespace mb {
+
+struct LnArgs {
+  const void *x, *dy, *w, *b;
+  void *y, *dx;
+  float *mean, *rstd, *partial;
+  int64_t ldx, lddy, n;
+  int32_t d;
+  float eps;
+};
+
+// Sums of K values over the G threads of a group (all threads of the block call it; `red` holds
+// (threads / 32) * K floats and is free to be overwritten two calls later: callers alternate two buffers).
+template <int G, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
+  static_assert(G >= 32, "a group is whole warps");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int W = G / 32;
+  float s = 0.f;
+  if constexpr (K == 8) {
+    // transposed: after three halving steps lane L holds a partial sum of value L >> 2 (9 shuffles instead of 40)
+#pragma unroll
+    for (int h = 4, bit = 16; h >= 1; h >>= 1, bit >>= 1) {
+      const bool up = lane & bit;
+#pragma unroll
+      for (int q = 0; q < h; ++q) {
+        const float send = up ? v[q] : v[q + h];
+        const float keep = up ? v[q + h] : v[q];
+        v[q] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
+      }
+    }
+    s = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 2);
+    s += __shfl_xor_sync(0xffffffffu, s, 1);
+  }
+  if constexpr (G == 32) {
+    if constexpr (K == 8) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, 4 * k);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    }
+  } else {
+    if constexpr (K == 8) {
+      if ((lane & 3) == 0) red[warp * K + (lane >> 2)] = s;
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) red[warp * K + k] = v[k];
+    }
+    __syncthreads();
+    const int w0 = warp / W * W;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = 0.f;
+#pragma unroll
+    for (int q = 0; q < W; ++q)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += red[(w0 + q) * K + k];
+  }
+}
+
+template <int G>
+constexpr int ln_threads = G < 256 ? 256 : G;
+
+template <typename T, typename P, int G, int NV, int V>
+__global__ void __launch_bounds__(ln_threads<G>) k_ln_fwd(const LnArgs a) {
+  constexpr int RPB = ln_threads<G> / G;
+  constexpr bool KEEP = NV * V <= 32;             // parameters stay in registers over the rows, else from L1 per row
+  __shared__ float red[2][ln_threads<G> / 32];
+  const int t = threadIdx.x % G, g = threadIdx.x / G, d = a.d;
+  const P *w = (const P*)a.w, *b = (const P*)a.b;
+  float pw[KEEP ? NV : 1][V], pb[KEEP ? NV : 1][V];
+  auto params = [&](int i, float (&fw)[V], float (&fb)[V]) {
+    const int j = (i * G + t) * V;
+#pragma unroll
+    for (int q = 0; q < V; ++q) fw[q] = 1.f, fb[q] = 0.f;
+    if (j < d) {
+      if (w) load_p<P, V>(w + j, fw);
+      if (b) load_p<P, V>(b + j, fb);
+    }
+  };
+  if constexpr (KEEP)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) params(i, pw[i], pb[i]);
+  const float inv = 1.f / (float)d;
+  // the trip count is the same for every group of a block (group_sum synchronises the block)
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.n; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + g;
+    const bool live = row < a.n;
+    const T* x = (const T*)a.x + (live ? row : 0) * a.ldx;
+    float v[NV][V], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * G + t) * V;
+#pragma unroll
+      for (int q = 0; q < V; ++q) v[i][q] = 0.f;
+      if (live && j < d) load_v<T, V>(x + j, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int q = 0; q < V; ++q) s[0] += v[i][q];
+    group_sum<G, 1>(s, red[0]);
+    const float mu = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * G + t) * V < d)
+#pragma unroll
+        for (int q = 0; q < V; ++q) s[0] += (v[i][q] - mu) * (v[i][q] - mu);
+    group_sum<G, 1>(s, red[1]);
+    const float r = rsqrtf(s[0] * inv + a.eps);
+    if (!live) continue;
+    T* y = (T*)a.y + row * d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * G + t) * V;
+      if (j >= d) continue;
+      float fw[V], fb[V], o[V];
+      if constexpr (!KEEP) params(i, fw, fb);
+#pragma unroll
+      for (int q = 0; q < V; ++q)
+        o[q] = KEEP ? fmaf((v[i][q] - mu) * r, pw[KEEP ? i : 0][q], pb[KEEP ? i : 0][q])
+                    : fmaf((v[i][q] - mu) * r, fw[q], fb[q]);
+      store_v<T, V>(y + j, o);
+    }
+    if (t == 0 && a.mean) {
+      a.mean[row] = mu;
+      a.rstd[row] = r;
+    }
+  }
+}
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(1024) k_ln_fwd_wide(const LnArgs a) {
+  __shared__ float red[2][32];
+  const int t = threadIdx.x, d = a.d;
+  const P *w = (const P*)a.w, *b = (const P*)a.b;
+  const float inv = 1.f / (float)d;
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T* x = (const T*)a.x + row * a.ldx;
+    float s[1] = {0.f};
+    for (int j = t; j < d; j += 1024) s[0] += to_f(x[j]);
+    group_sum<1024, 1>(s, red[0]);
+    const float mu = s[0] * inv;
+    s[0] = 0.f;
+    for (int j = t; j < d; j += 1024) {
+      const float c = to_f(x[j]) - mu;
+      s[0] += c * c;
+    }
+    group_sum<1024, 1>(s, red[1]);
+    const float r = rsqrtf(s[0] * inv + a.eps);
+    T* y = (T*)a.y + row * d;
+    for (int j = t; j < d; j += 1024)
+      y[j] = from_f<T>(fmaf((to_f(x[j]) - mu) * r, w ? to_f(w[j]) : 1.f, b ? to_f(b[j]) : 0.f));
+    if (t == 0 && a.mean) {
+      a.mean[row] = mu;
+      a.rstd[row] = r;
+    }
+  }
+}
+
+// partial[block][0 .. d) = sum of dy xh, [d .. 2 d) = sum of dy over the block's rows.  RB rows at a time, so that a
+// group has 2 RB loads in flight and one synchronisation per RB rows.
+template <typename T, typename P, int G, int NV, int V, int RB>
+__global__ void __launch_bounds__(ln_threads<G>) k_ln_bwd(const LnArgs a) {
+  constexpr int TH = ln_threads<G>, RPB = TH / G;
+  __shared__ float red[2][TH / 32 * 2 * RB];
+  extern __shared__ float cols[];                 // [RPB][2][d] when RPB > 1
+  const int t = threadIdx.x % G, g = threadIdx.x / G, d = a.d;
+  const P* w = (const P*)a.w;
+  float pw[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * G + t) * V;
+#pragma unroll
+    for (int q = 0; q < V; ++q) pw[i][q] = 1.f, aw[i][q] = 0.f, ab[i][q] = 0.f;
+    if (w && j < d) load_p<P, V>(w + j, pw[i]);
+  }
+  const float inv = 1.f / (float)d;
+  int buf = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB * RB; r0 < a.n; r0 += (int64_t)gridDim.x * RPB * RB, buf ^= 1) {
+    float xv[RB][NV][V], dv[RB][NV][V], rs[RB], s[2 * RB], mu[RB];
+#pragma unroll
+    for (int k = 0; k < RB; ++k) {
+      const int64_t row = r0 + g * RB + k;
+      const bool live = row < a.n;
+      const T* x = (const T*)a.x + (live ? row : 0) * a.ldx;
+      const T* dy = (const T*)a.dy + (live ? row : 0) * a.lddy;
+      rs[k] = live ? a.rstd[row] : 0.f;
+      mu[k] = live ? a.mean[row] : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = (i * G + t) * V;
+#pragma unroll
+        for (int q = 0; q < V; ++q) xv[k][i][q] = 0.f, dv[k][i][q] = 0.f;
+        if (live && j < d) {
+          load_v<T, V>(x + j, xv[k][i]);
+          load_v<T, V>(dy + j, dv[k][i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < RB; ++k) {
+      s[2 * k] = s[2 * k + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if ((i * G + t) * V >= d) continue;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          const float xh = (xv[k][i][q] - mu[k]) * rs[k], dy = dv[k][i][q];
+          const float up = __fmul_rn(dy, pw[i][q]);   // the same rounding here and below: dx of a constant is 0
+          s[2 * k] += up;
+          s[2 * k + 1] += up * xh;
+          aw[i][q] += dy * xh;
+          ab[i][q] += dy;
+        }
+      }
+    }
+    group_sum<G, 2 * RB>(s, red[buf]);
+    if (a.dx) {
+#pragma unroll
+      for (int k = 0; k < RB; ++k) {
+        const int64_t row = r0 + g * RB + k;
+        if (row >= a.n) continue;
+        T* dx = (T*)a.dx + row * d;
+        const float m1 = s[2 * k] * inv, m2 = s[2 * k + 1] * inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int j = (i * G + t) * V;
+          if (j >= d) continue;
+          float o[V];
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            const float xh = (xv[k][i][q] - mu[k]) * rs[k];
+            o[q] = rs[k] * (__fmul_rn(dv[k][i][q], pw[i][q]) - m1 - xh * m2);
+          }
+          store_v<T, V>(dx + j, o);
+        }
+      }
+    }
+  }
+  if (!a.partial) return;
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * d;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const int j = (i * G + t) * V + q;
+        if (j < d) {
+          out[j] = aw[i][q];
+          out[d + j] = ab[i][q];
+        }
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const int j = (i * G + t) * V + q;
+        if (j < d) {
+          cols[(2 * g) * d + j] = aw[i][q];
+          cols[(2 * g + 1) * d + j] = ab[i][q];
+        }
+      }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * d; j += TH) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < RPB; ++q) s += cols[q * 2 * d + j];
+      out[j] = s;
+    }
+  }
+}
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(1024) k_ln_bwd_wide(const LnArgs a) {
+  __shared__ float red[2][64];
+  const int t = threadIdx.x, d = a.d;
+  const P* w = (const P*)a.w;
+  const float inv = 1.f / (float)d;
+  int buf = 0;
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x, buf ^= 1) {
+    const T *x = (const T*)a.x + row * a.ldx, *dy = (const T*)a.dy + row * a.lddy;
+    const float mu = a.mean[row], r = a.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (int j = t; j < d; j += 1024) {
+      const float up = to_f(dy[j]) * (w ? to_f(w[j]) : 1.f);
+      s[0] += up;
+      s[1] += up * ((to_f(x[j]) - mu) * r);
+    }
+    group_sum<1024, 2>(s, red[buf]);
+    T* dx = (T*)a.dx + row * d;
+    for (int j = t; j < d; j += 1024)
+      dx[j] = from_f<T>(r * (to_f(dy[j]) * (w ? to_f(w[j]) : 1.f) - s[0] * inv - (to_f(x[j]) - mu) * r * s[1] * inv));
+  }
+}
+
+// dw / db partial sums of wide rows: block (column tile of 128, row split), one column per thread
+template <typename T>
+__global__ void __launch_bounds__(128) k_ln_cols_wide(const LnArgs a) {
+  const int j = blockIdx.x * 128 + threadIdx.x, d = a.d;
+  if (j >= d) return;
+  float sw = 0.f, sb = 0.f;
+  for (int64_t row = blockIdx.y; row < a.n; row += gridDim.y) {
+    const float dy = to_f(((const T*)a.dy)[row * a.lddy + j]);
+    sw += dy * (to_f(((const T*)a.x)[row * a.ldx + j]) - a.mean[row]) * a.rstd[row];
+    sb += dy;
+  }
+  float* out = a.partial + (int64_t)blockIdx.y * 2 * d;
+  out[j] = sw;
+  out[d + j] = sb;
+}
+
+// Adds the partial sums of the blocks in a fixed order: 32 columns x 8 interleaved sets of partials per block
+template <typename P>
+__global__ void __launch_bounds__(256) k_ln_reduce(const float* partial, int nb, int32_t d, P* dw, P* db) {
+  __shared__ float red[8][33];
+  const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (j < 2 * (int64_t)d)
+    for (int k = q; k < nb; k += 8) s += partial[(int64_t)k * 2 * d + j];
+  red[q][c] = s;
+  __syncthreads();
+  if (q == 0 && j < 2 * (int64_t)d) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += red[k][c];
+    if (j < d) {
+      if (dw) dw[j] = from_f<P>(s);
+    } else if (db) {
+      db[j - d] = from_f<P>(s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+constexpr int LN_BLOCKS_PER_SM = 3;              // of the backward kernel: the row count of the partial sums
+
+static int ln_bwd_blocks(int64_t n, int rows_per_pass) {
+  const int64_t want = (n + rows_per_pass - 1) / rows_per_pass, most = (int64_t)LN_BLOCKS_PER_SM * sm_count();
+  return (int)(want < most ? want : most);
+}
+
+template <typename T, typename P, int G, int NV, int V>
+static int ln_fwd_launch(const LnArgs& a, cudaStream_t st) {
+  constexpr int RPB = ln_threads<G> / G;
+  const int64_t want = (a.n + RPB - 1) / RPB, most = (int64_t)8 * sm_count();
+  k_ln_fwd<T, P, G, NV, V><<<(unsigned)(want < most ? want : most), ln_threads<G>, 0, st>>>(a);
+  return check_launch("layer_norm_fwd");
+}
+
+template <typename T, typename P>
+static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
+  constexpr int V = kVec<T>;
+  if (vec) {                                      // one warp per row up to 64 values per lane, then 4 and 16 warps
+    const int nv = (a.d / V + 31) / 32;
+    if (nv <= 1) return ln_fwd_launch<T, P, 32, 1, V>(a, st);
+    if (nv <= 2) return ln_fwd_launch<T, P, 32, 2, V>(a, st);
+    if (nv <= 4) return ln_fwd_launch<T, P, 32, 4, V>(a, st);
+    if (nv * V <= 64) return ln_fwd_launch<T, P, 32, 64 / V, V>(a, st);
+    if (nv * V <= 256) return ln_fwd_launch<T, P, 128, 64 / V, V>(a, st);
+    if (nv * V <= 1024) return ln_fwd_launch<T, P, 512, 64 / V, V>(a, st);
+  } else {
+    if (a.d <= 128) return ln_fwd_launch<T, P, 32, 4, 1>(a, st);
+    if (a.d <= 512) return ln_fwd_launch<T, P, 32, 16, 1>(a, st);
+    if (a.d <= 1024) return ln_fwd_launch<T, P, 32, 32, 1>(a, st);
+    if (a.d <= 4096) return ln_fwd_launch<T, P, 128, 32, 1>(a, st);
+    if (a.d <= 16384) return ln_fwd_launch<T, P, 512, 32, 1>(a, st);
+  }
+  const int64_t most = (int64_t)2 * sm_count();
+  k_ln_fwd_wide<T, P><<<(unsigned)(a.n < most ? a.n : most), 1024, 0, st>>>(a);
+  return check_launch("layer_norm_fwd");
+}
+
+// Number of partial-sum rows, or the launch (when `go`)
+template <typename T, typename P, int G, int NV, int V, int RB>
+static int ln_bwd_launch(const LnArgs& a, bool go, int* nb, cudaStream_t st) {
+  constexpr int TH = ln_threads<G>, RPB = TH / G;
+  *nb = ln_bwd_blocks(a.n, RPB * RB);
+  if (!go) return 0;
+  const int smem = RPB > 1 && a.partial ? RPB * 2 * a.d * 4 : 0;
+  static_assert(RPB == 1 || RPB * 2 * G * NV * V * 4 <= 48 * 1024, "column sums in shared memory");
+  k_ln_bwd<T, P, G, NV, V, RB><<<*nb, TH, smem, st>>>(a);
+  return check_launch("layer_norm_bwd");
+}
+
+template <typename T, typename P>
+static int ln_bwd_any(const LnArgs& a, bool vec, bool go, int* nb, cudaStream_t st) {
+  constexpr int V = kVec<T>;
+  if (vec) {
+    const int c = a.d / V;
+    if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 4>(a, go, nb, st);
+    if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 4>(a, go, nb, st);
+    if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 4>(a, go, nb, st);
+    if (c <= 256) return ln_bwd_launch<T, P, 256, 1, V, 4>(a, go, nb, st);
+    if (c <= 512) return ln_bwd_launch<T, P, 512, 1, V, 4>(a, go, nb, st);
+    if (c <= 1024) return ln_bwd_launch<T, P, 512, 2, V, 1>(a, go, nb, st);
+  } else {
+    if (a.d <= 128) return ln_bwd_launch<T, P, 32, 4, 1, 4>(a, go, nb, st);
+    if (a.d <= 256) return ln_bwd_launch<T, P, 64, 4, 1, 4>(a, go, nb, st);
+    if (a.d <= 512) return ln_bwd_launch<T, P, 128, 4, 1, 4>(a, go, nb, st);
+    if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 4>(a, go, nb, st);
+    if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 4>(a, go, nb, st);
+  }
+  const int64_t most = (int64_t)2 * sm_count();
+  *nb = (int)(a.n < 64 ? a.n : 64);
+  if (!go) return 0;
+  if (a.dx) {
+    k_ln_bwd_wide<T, P><<<(unsigned)(a.n < most ? a.n : most), 1024, 0, st>>>(a);
+    if (int rc = check_launch("layer_norm_bwd")) return rc;
+  }
+  if (a.partial) {
+    k_ln_cols_wide<T><<<dim3((a.d + 127) / 128, *nb), 128, 0, st>>>(a);
+    return check_launch("layer_norm_bwd");
+  }
+  return 0;
+}
+
+template <typename F>
+static int ln_types(int dtype, int ptype, const F& f) {
+  if (dtype == MB_F32) return f(float(), float());
+  if (dtype == MB_BF16) return ptype == MB_F32 ? f(bf16(), float()) : f(bf16(), bf16());
+  return ptype == MB_F32 ? f(f16(), float()) : f(f16(), f16());
+}
+
+static int ln_check(const char* who, int64_t n, int32_t d, int64_t ldx, int32_t dtype, int32_t ptype) {
+  if (n < 0 || d < 1 || ldx < d) {
+    set_error("%s: bad sizes (rows %lld, width %d, row stride %lld)", who, (long long)n, d, (long long)ldx);
+    return MB_E_ARG;
+  }
+  if (!dtype_ok(dtype) || (ptype != dtype && ptype != MB_F32)) {
+    set_error("%s: unsupported types (x %d, parameters %d)", who, dtype, ptype);
+    return MB_E_ARG;
+  }
+  if (sm_count() < 1) {
+    set_error("%s: no CUDA device", who);
+    return MB_E_CUDA;
+  }
+  return 0;
+}
+
+// 16-byte accesses: width and strides whole vectors, every address 16-byte aligned
+static bool ln_vec(int32_t d, int64_t ldx, int64_t lddy, int dtype, const void* p0, const void* p1, const void* p2,
+                   const void* p3, const void* p4) {
+  const int v = 16 / dtype_size(dtype);
+  return d % v == 0 && ldx % v == 0 && lddy % v == 0 && aligned16(p0) && aligned16(p1) && aligned16(p2) &&
+         aligned16(p3) && aligned16(p4);
+}
+
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" int mace_b200_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean,
+                                        float* rstd, int64_t n, int32_t d, double eps, int32_t dtype, int32_t ptype,
+                                        void* stream) {
+  if (int rc = ln_check("layer_norm_fwd", n, d, ldx, dtype, ptype)) return rc;
+  if (n == 0) return 0;
+  if (!x || !y || !mean != !rstd) {
+    set_error("layer_norm_fwd: null pointer");
+    return MB_E_ARG;
+  }
+  LnArgs a{};
+  a.x = x; a.w = w; a.b = b; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.ldx = ldx; a.n = n; a.d = d; a.eps = (float)eps;
+  const bool vec = ln_vec(d, ldx, 0, dtype, x, w, b, y, nullptr);
+  return ln_types(dtype, ptype, [&](auto t, auto p) {
+    return ln_fwd_any<decltype(t), decltype(p)>(a, vec, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int mace_b200_layer_norm_bwd_workspace(int64_t n, int32_t d, int64_t* floats) {
+  if (n < 0 || d < 1 || !floats) {
+    set_error("layer_norm_bwd_workspace: bad arguments (rows %lld, width %d)", (long long)n, d);
+    return MB_E_ARG;
+  }
+  const int64_t most = (int64_t)LN_BLOCKS_PER_SM * (sm_count() > 0 ? sm_count() : 1);
+  *floats = 2 * (int64_t)d * (n < most ? n : most);
+  return 0;
+}
+
+extern "C" int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                                        const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                                        float* workspace, int64_t n, int32_t d, int32_t dtype, int32_t ptype,
+                                        void* stream) {
+  if (int rc = ln_check("layer_norm_bwd", n, d, ldx < lddy ? ldx : lddy, dtype, ptype)) return rc;
+  if (n > 0 && (!dy || !x || !mean || !rstd || ((dw || db) && !workspace))) {
+    set_error("layer_norm_bwd: null pointer");
+    return MB_E_ARG;
+  }
+  LnArgs a{};
+  a.x = x; a.dy = dy; a.w = w; a.dx = dx; a.mean = (float*)mean; a.rstd = (float*)rstd;
+  a.partial = (dw || db) ? workspace : nullptr;
+  a.ldx = ldx; a.lddy = lddy; a.n = n; a.d = d;
+  const bool vec = ln_vec(d, ldx, lddy, dtype, x, dy, w, dx, nullptr);
+  return ln_types(dtype, ptype, [&](auto t, auto p) {
+    using T = decltype(t);
+    using P = decltype(p);
+    int nb = 0;
+    if (n > 0)
+      if (int rc = ln_bwd_any<T, P>(a, vec, true, &nb, (cudaStream_t)stream)) return rc;
+    if (!dw && !db) return 0;
+    k_ln_reduce<P><<<(unsigned)((2 * (int64_t)d + 31) / 32), 256, 0, (cudaStream_t)stream>>>(workspace, nb, d, (P*)dw,
+                                                                                             (P*)db);
+    return check_launch("layer_norm_bwd");
+  });
+}

@@ -18,6 +18,8 @@ c_vp = ctypes.c_void_p
 
 ABI_VERSION = 4          # MB_ABI_VERSION of include/mace_b200.h this binding mirrors
 ST_UNSORTED = 64         # MB_ST_UNSORTED
+ST_TC_TIMEOUT = 32       # MB_ST_TC_TIMEOUT
+ST_BAD_EXPERT = 128      # MB_ST_BAD_EXPERT
 
 
 class MBModel(ctypes.Structure):
@@ -91,6 +93,25 @@ _SIGS = {
     "mace_b200_csr_rows": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "mace_b200_sender_range": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp]),
     "mace_b200_tc_test_hooks": (c_i32, [c_u64, c_i32]),
+    "mace_b200_layer_norm_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_f64, c_i32, c_i32,
+                                         c_vp]),
+    "mace_b200_layer_norm_bwd_workspace": (c_i32, [c_i64, c_i32, ctypes.POINTER(c_i64)]),
+    "mace_b200_layer_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
+                                         c_i32, c_i32, c_i32, c_vp]),
+    "mace_b200_route_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+                                    c_f32, c_i32, c_vp]),
+    "mace_b200_route_bwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,
+                                    c_vp]),
+    "mace_b200_expert_plan_words": (c_i32, [c_i64, c_i32, ctypes.POINTER(c_i64)]),
+    "mace_b200_expert_plan": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp]),
+    "mace_b200_expert_linear_workspace": (c_i32, [c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+                                                  ctypes.POINTER(c_i64)]),
+    "mace_b200_expert_linear_few": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32,
+                                            c_i32, c_i32, c_vp]),
+    "mace_b200_expert_linear_fwd": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32,
+                                            c_i32, c_i32, c_i32, c_vp]),
+    "mace_b200_expert_linear_bwd": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
+                                            c_i32, c_i32, c_i32, c_i32, c_i32, c_vp]),
 }
 
 _lib = None
@@ -123,7 +144,8 @@ def lib():
 
 OPS_PATH = os.path.join(_HERE, "_lib", "libmace_b200_torch.so")
 OPS = ("conv_tp", "conv_tp_backward", "build_tables", "edge_l1_fwd", "edge_l1_bwd", "edge_l2_fwd", "edge_l2_bwd",
-       "node_gemm", "symcon_fwd", "symcon_bwd", "pack_halo", "unpack_halo_add", "csr_rows", "guard")
+       "node_gemm", "symcon_fwd", "symcon_bwd", "pack_halo", "unpack_halo_add", "csr_rows", "guard", "layer_norm",
+       "layer_norm_fwd", "layer_norm_bwd", "route", "route_bwd", "expert_plan", "expert_linear", "expert_linear_bwd")
 _ops = None
 
 
@@ -159,6 +181,19 @@ def _register_python_side(torch):
     @tl.register_fake("mace_b200::pack_halo")
     def _pack_fake(src, idx):
         return src.new_empty((idx.shape[0], src.shape[1]))
+
+    @tl.register_fake("mace_b200::layer_norm")
+    def _ln_fake(x, weight, bias, eps):
+        return x.new_empty(x.shape)
+
+    @tl.register_fake("mace_b200::route")
+    def _route_fake(logits, bias, k, softmax, groups, top_groups, renormalize, scale):
+        shape = (logits.shape[0], k)
+        return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+    @tl.register_fake("mace_b200::expert_linear")
+    def _expert_fake(x, w, experts, plan, weights):
+        return x.new_empty((*(experts.shape if weights is None else experts.shape[:1]), w.shape[1]))
 
     def _setup(ctx, inputs, output):
         node_feats, edge_attrs, tp_weights, edge_index, terms, coef, n_out = inputs
