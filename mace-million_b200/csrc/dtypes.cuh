@@ -81,6 +81,24 @@ __device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
   else
     *reinterpret_cast<uint4*>(p) = pack16<T>(f);
 }
+// The same, kept as loaded until used: V elements of T in the fewest registers
+template <typename T, int V>
+struct Raw {
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&f)[V]) const { unpack16(u, f, T()); }
+  // unpack again at the next use instead of keeping the floats
+  __device__ __forceinline__ void again() { asm volatile("" : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w)); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void zero() { v = from_f<T>(0.f); }
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f(v); }
+  __device__ __forceinline__ void again() {}
+};
 // V parameters of type P (as many bytes as V elements of a possibly narrower type need)
 template <typename P, int V>
 __device__ __forceinline__ void load_p(const P* p, float (&f)[V]) {

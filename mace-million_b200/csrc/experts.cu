@@ -213,136 +213,170 @@ __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64
   }
 }
 
-// Rows in expert order: out0[row] = src[slot / kdiv], out1[row] = scale[slot] src[slot / kdiv] (either may be null),
-// zeros in padding rows and in the columns that pad the width to dp.
+// One job of k_rows_move; a launch runs up to four side by side, each on its own blocks (few launches: every one costs a
+// small call more than its work).
+struct XMove {
+  int kind;                                      // MOVE_*
+  int d, dp, kdiv, vec;
+  unsigned block0, blocks;                       // first block and number of blocks
+  int64_t rows, lds, plane;
+  const void* src;
+  const float* scale;
+  void* out;
+};
+enum {
+  // out[row] = scale[slot] src[slot / kdiv] in planes, rows in expert order, zeros in padding rows and padding columns
+  MOVE_GATHER = 0,
+  MOVE_STAGE = 1,                                // out[row] = src[row] in planes, zeros in padding columns
+  MOVE_ZERO = 2,                                 // out[slot] = 0 for slots without an expert (elements of T)
+};
+struct XMoves {
+  XMove m[4];
+  int n;
+};
+
+// Narrow rows share a warp (lpr lanes a row, a power of two); wide ones take several passes, four vectors in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) k_rows_gather(const T* src, int64_t lds, int d, int dp, bool vec, int kdiv,
-                                                     const int32_t* plan, const XPlan p, const float* scale,
-                                                     uint16_t* out0, uint16_t* out1, int64_t plane) {
-  const int lane = threadIdx.x & 31;
-  const int64_t used = (int64_t)plan[0] * XP_BM;
-  const int64_t step = (int64_t)gridDim.x * 8;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < used; row += step) {
-    const int slot = plan[p.o_row + row];
-    const T* s = src + (slot < 0 ? 0 : slot / kdiv) * lds;
-    const float g = scale && slot >= 0 ? scale[slot] : 1.f;
-    for (int c = lane * 8; c < dp; c += 256) {
-      float f[8];
-      if (slot >= 0) {
-        load8(s, c, d, vec, f);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] = 0.f;
-      }
-      if (out0) store_planes<T>(out0, plane, row * dp + c, f);
-      if (out1) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] *= g;
-        store_planes<T>(out1, plane, row * dp + c, f);
+__global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_t* plan, const XPlan p) {
+  int q = 0;
+  while (q + 1 < mv.n && blockIdx.x >= mv.m[q + 1].block0) ++q;
+  const XMove& m = mv.m[q];
+  const int lane = threadIdx.x & 31, nv = m.dp / 8;
+  int lpr = 1;
+  while (lpr < 32 && lpr < nv) lpr *= 2;
+  const int rpw = 32 / lpr, sub = lane & (lpr - 1);
+  const int64_t rows = m.kind == MOVE_GATHER ? (int64_t)plan[0] * XP_BM : m.rows;
+  const int64_t step = (int64_t)m.blocks * 8 * rpw;
+  if (m.kind == MOVE_ZERO) {                     // 32 slots a warp; the whole warp zeros a row (rpw = 32)
+    for (int64_t r0 = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * 32; r0 < rows; r0 += step) {
+      unsigned todo = __ballot_sync(0xffffffffu, r0 + lane < rows && plan[p.o_slot + r0 + lane] < 0);
+      for (; todo; todo &= todo - 1) {
+        T* o = (T*)m.out + (r0 + __ffs(todo) - 1) * m.d;
+        for (int c = lane; c < m.d; c += 32) o[c] = from_f<T>(0.f);
       }
     }
+    return;
   }
-}
-
-// [rows][d] -> 16-bit planes [rows][dp], columns padded with zeros
-template <typename T>
-__global__ void __launch_bounds__(256) k_rows_stage(const T* src, int64_t rows, int d, int dp, bool vec, uint16_t* out,
-                                                    int64_t plane) {
-  const int nv = dp / 8;
-  const int64_t total = rows * nv, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t r = i / nv;
-    const int c = (int)(i - r * nv) * 8;
-    float f[8];
-    load8(src + r * d, c, d, vec, f);
-    store_planes<T>(out, plane, r * dp + c, f);
-  }
-}
-
-// out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an expert; dg[slot] = sum of
-// the partial products.  buf null: only dg.  One warp per token.
-template <typename T>
-__global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
-                                                  bool vec, const int32_t* slot_row, const float* dgpart, int nparts,
-                                                  float* dg) {
-  const int lane = threadIdx.x & 31;
-  const int64_t R = tokens * k;
-  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)gridDim.x * 8) {
-    if (dg)
-      for (int j = lane; j < k; j += 32) {
-        float s = 0.f;
-        if (slot_row[t * k + j] >= 0)
-          for (int q = 0; q < nparts; ++q) s += dgpart[q * R + t * k + j];
-        dg[t * k + j] = s;
-      }
-    if (!buf) continue;
-    for (int c = lane * 8; c < d; c += 256) {
-      float s[8];
+  for (int64_t row = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * rpw + lane / lpr; row < rows;
+       row += step) {
+    const int64_t slot = m.kind == MOVE_GATHER ? (int64_t)plan[p.o_row + row] : row;
+    const T* s = (const T*)m.src + (slot < 0 ? 0 : slot / m.kdiv) * m.lds;
+    const float g = m.scale && slot >= 0 ? m.scale[slot] : 1.f;
+    uint16_t* out = (uint16_t*)m.out;
+    for (int c0 = sub * 8; c0 < m.dp; c0 += 32 * lpr) {
+      float f[4][8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) s[q] = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < k; ++j) {
-        if (slot_row[t * k + j] < 0) continue;
-        float f[8];
-        load8(buf + (t * k + j) * ldb, c, d, true, f);   // ldb is padded: whole vectors wherever c + 8 <= d
-#pragma unroll
-        for (int q = 0; q < 8; ++q) s[q] += f[q];
-      }
-      T* o = out + t * d + c;
-      if (vec && c + 8 <= d) {
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint4*>(o) = pack16<T>(s);
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + u * 8 * lpr;
+        if (slot >= 0 && c < m.dp) {
+          load8(s, c, m.d, m.vec != 0, f[u]);
         } else {
-          reinterpret_cast<float4*>(o)[0] = make_float4(s[0], s[1], s[2], s[3]);
-          reinterpret_cast<float4*>(o)[1] = make_float4(s[4], s[5], s[6], s[7]);
-        }
-      } else {
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (c + q < d) o[q] = from_f<T>(s[q]);
+          for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + u * 8 * lpr;
+        if (c >= m.dp) break;
+        if (m.scale)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[u][i] *= g;
+        store_planes<T>(out, m.plane, row * m.dp + c, f[u]);
       }
     }
   }
 }
 
-// Zeros the rows of slots without an expert (the products write every other row)
+// Blocks [0, sum_blocks): out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an
+// expert; a thread adds one V-element piece of a token's rows, four loads in flight; ldb is padded to whole vectors.
+// The other blocks: dg[slot] = sum of its nparts partial products (0 without an expert).
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
+                                                  const int32_t* slot_row, unsigned sum_blocks, const float* dgpart,
+                                                  int nparts, float* dg) {
+  if (blockIdx.x >= sum_blocks) {
+    const int64_t R = tokens * k, step = (int64_t)(gridDim.x - sum_blocks) * 256;
+    for (int64_t s = (int64_t)(blockIdx.x - sum_blocks) * 256 + threadIdx.x; s < R; s += step) {
+      float v = 0.f;
+      if (slot_row[s] >= 0)
+        for (int q = 0; q < nparts; ++q) v += dgpart[q * R + s];
+      dg[s] = v;
+    }
+    return;
+  }
+  const unsigned nv = d / V;
+  const int64_t total = tokens * nv, step = (int64_t)sum_blocks * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t t = total >> 32 ? i / nv : (unsigned)i / nv;
+    const int c = (int)(i - t * nv) * V;
+    float s[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) s[q] = 0.f;
+    const T* p = buf + t * k * ldb + c;
+    const int32_t* row = slot_row + t * k;
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      Raw<T, V> r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        r[j].zero();
+        if (j0 + j < k && row[j0 + j] >= 0) r[j].load(p + (j0 + j) * ldb);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[V];
+        r[j].get(f);
+#pragma unroll
+        for (int q = 0; q < V; ++q) s[q] += f[q];
+      }
+    }
+    store_v<T, V>(out + t * d + c, s);
+  }
+}
+
+// dw = sum over the `parts` partial sums (in their order) of a product whose rows were split
 template <typename T>
-__global__ void __launch_bounds__(256) k_rows_zero(T* out, int64_t slots, int d, const int32_t* slot_row) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t s = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); s < slots; s += (int64_t)gridDim.x * 8)
-    if (slot_row[s] < 0)
-      for (int c = lane; c < d; c += 32) out[s * d + c] = from_f<T>(0.f);
+__global__ void __launch_bounds__(256) k_parts_sum(const float* part, int parts, int64_t n, T* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int q = 0; q < parts; ++q) s += part[q * n + i];
+    out[i] = from_f<T>(s);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ few slots
-// out[t][o] = sum_j g_tj <W[e_tj][o], x> without a plan: one warp per (token, output), the k rows of W side by side in
-// flight.  Bound by the bytes of W; a row of W that several tokens use comes from L2 after the first.
-// SLOTS: out[slot][o] = <W[e][o], x>, one warp per (slot, output).
-template <typename T, int V, bool SLOTS>
+// out[t][o] = sum_j g_tj <W[e_tj][o], x> without a plan: L lanes per (token, output), the rows of W of four choices side
+// by side in flight.  Bound by the bytes of W; a row of W that several tokens use comes from L2 after the first.
+// SLOTS: out[slot][o] = <W[e][o], x>, L lanes per (slot, output).
+template <typename T, int V, int L, bool SLOTS>
 __global__ void __launch_bounds__(128) k_expert_few(const T* x, int64_t ldx, int kx, const T* w, const int32_t* experts,
                                                     const float* g, T* out, int k, int E, int d, int o_n) {
-  const int lane = threadIdx.x & 31, o = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (o >= o_n) return;
+  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
+  const int o = (blockIdx.x * 4 + (threadIdx.x >> 5)) * (32 / L) + lane / L;
+  const bool live = o < o_n;
   const int64_t t = blockIdx.y;
   const int n = SLOTS ? 1 : k;
+  constexpr int J = SLOTS ? 1 : 4;
   float total = 0.f;
-  for (int j0 = 0; j0 < n; j0 += 4) {
-    const T *wr[4], *xr[4];
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    constexpr int J = SLOTS ? 1 : 4;
+  for (int j0 = 0; j0 < n; j0 += J) {
+    const T *wr[J], *xr[J];
+    float acc[J];
 #pragma unroll
     for (int q = 0; q < J; ++q) {
       const int64_t s = SLOTS ? t : t * k + j0 + q;
       const int e = j0 + q < n ? experts[s] : -1;
-      wr[q] = e >= 0 && e < E ? w + ((int64_t)e * o_n + o) * d : nullptr;
+      wr[q] = live && e >= 0 && e < E ? w + ((int64_t)e * o_n + o) * d : nullptr;
       xr[q] = x + s / kx * ldx;
+      acc[q] = 0.f;
     }
 #pragma unroll 4
-    for (int c = lane * V; c < d; c += 32 * V) {
+    for (int c = sub * V; c < d; c += L * V) {
+      float b[V];
 #pragma unroll
       for (int q = 0; q < J; ++q) {
         if (!wr[q]) continue;
-        float a[V], b[V];
+        float a[V];
         load_v<T, V>(wr[q] + c, a);
         load_v<T, V>(xr[q] + c, b);
 #pragma unroll
@@ -351,11 +385,12 @@ __global__ void __launch_bounds__(128) k_expert_few(const T* x, int64_t ldx, int
     }
 #pragma unroll
     for (int q = 0; q < J; ++q) {
-      const float z = warp_sum(acc[q]);
-      if (wr[q]) total += SLOTS ? z : g[t * k + j0 + q] * z;
+#pragma unroll
+      for (int h = L / 2; h > 0; h >>= 1) acc[q] += __shfl_xor_sync(0xffffffffu, acc[q], h);
+      if (wr[q]) total += SLOTS ? acc[q] : g[t * k + j0 + q] * acc[q];
     }
   }
-  if (lane == 0) out[t * o_n + o] = from_f<T>(total);
+  if (sub == 0 && live) out[t * o_n + o] = from_f<T>(total);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -418,7 +453,8 @@ static XFwd x_fwd_layout(const XShape& s, bool combine, bool direct) {
 }
 
 struct XBwd {
-  int64_t xs = -1, dys = -1, gdy = -1, ws = -1, dxb = -1, dgp = -1, bytes = 0;
+  int64_t xs = -1, dys = -1, ws = -1, dxb = -1, dgp = -1, parts = -1, bytes = 0;
+  int split = 1;
 };
 static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direct, bool need_x, bool need_w,
                          bool need_g) {
@@ -426,11 +462,14 @@ static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direc
   XBwd b;
   const int64_t row2 = (int64_t)s.np * s.rows * 2;
   if (need_w) b.xs = c.take(row2 * s.Dp);
-  if (need_x || need_g || (need_w && !combine)) b.dys = c.take(row2 * s.Op);
-  if (need_w && combine) b.gdy = c.take(row2 * s.Op);
+  b.dys = c.take(row2 * s.Op);
   if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
   if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * dtype_size(s.dtype));
   if (need_g) b.dgp = c.take(s.R * 4 * xgemm_n_tiles(XG_DGRAD, s.D));
+  if (need_w) {
+    b.split = xgemm_split(s.E, s.O, s.D, s.R, s.np);
+    if (b.split > 1) b.parts = c.take((int64_t)b.split * s.E * s.O * s.D * 4);
+  }
   b.bytes = c.used;
   return b;
 }
@@ -446,21 +485,64 @@ static int x_types(int dtype, const F& f) {
   return dtype == MB_BF16 ? f(bf16()) : f(f16());
 }
 
-template <typename T>
-static int x_stage_w(const XShape& s, const void* w, void* ws, cudaStream_t st) {
-  const int64_t rows = (int64_t)s.E * s.O;
-  k_rows_stage<T><<<x_grid((rows * (s.Dp / 8) + 255) / 256), 256, 0, st>>>(
-      (const T*)w, rows, s.D, s.Dp, aligned16(w) && s.D % 8 == 0, (uint16_t*)ws, rows * s.Dp);
-  return check_launch("expert_linear (stage)");
+static XMove move_gather(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const float* scale,
+                         void* out) {
+  XMove m{};
+  m.kind = MOVE_GATHER;
+  m.d = d; m.dp = dp; m.kdiv = kdiv; m.vec = aligned16(src) && lds % 8 == 0;
+  m.rows = s.rows; m.lds = lds; m.plane = s.rows * dp;
+  m.src = src; m.scale = scale; m.out = out;
+  return m;
+}
+static XMove move_stage(const XShape& s, const void* w, void* out) {
+  XMove m{};
+  m.kind = MOVE_STAGE;
+  m.d = s.D; m.dp = s.Dp; m.kdiv = 1; m.vec = aligned16(w) && s.D % 8 == 0;
+  m.rows = (int64_t)s.E * s.O; m.lds = s.D; m.plane = m.rows * s.Dp;
+  m.src = w; m.out = out;
+  return m;
+}
+static XMove move_zero(const XShape& s, void* out, int d) {
+  XMove m{};
+  m.kind = MOVE_ZERO;
+  m.d = d; m.dp = 8; m.kdiv = 1;                 // one lane reads a slot: almost all have an expert
+  m.rows = s.R; m.out = out;
+  return m;
 }
 
+// Blocks in proportion to the vectors that each job moves
 template <typename T>
-static int x_gather(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const int32_t* plan,
-                    const float* scale, void* out0, void* out1, cudaStream_t st) {
-  const bool vec = aligned16(src) && lds % 8 == 0;
-  k_rows_gather<T><<<x_grid((s.rows + 7) / 8), 256, 0, st>>>((const T*)src, lds, d, dp, vec, kdiv, plan, s.lay, scale,
-                                                             (uint16_t*)out0, (uint16_t*)out1, s.rows * dp);
-  return check_launch("expert_linear (gather)");
+static int x_moves(const XShape& s, XMoves& mv, const int32_t* plan, cudaStream_t st) {
+  int64_t units[4], all = 0;
+  for (int q = 0; q < mv.n; ++q) {
+    units[q] = (mv.m[q].rows * (mv.m[q].dp / 8) + 255) / 256;
+    all += units[q];
+  }
+  const int64_t most = (int64_t)16 * sm_count();
+  unsigned at = 0;
+  for (int q = 0; q < mv.n; ++q) {
+    const int64_t b = all <= most ? units[q] : units[q] * most / all;
+    mv.m[q].block0 = at;
+    mv.m[q].blocks = (unsigned)(b < 1 ? 1 : b);
+    at += mv.m[q].blocks;
+  }
+  k_rows_move<T><<<at, 256, 0, st>>>(mv, plan, s.lay);
+  return check_launch("expert_linear (rows)");
+}
+
+// sums of rows (buf not null) and of partial weight gradients (dg not null) in one launch
+template <typename T>
+static int x_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d, const int32_t* slot_row,
+                      const float* dgpart, int nparts, float* dg, cudaStream_t st) {
+  constexpr int V = kVec<T>;
+  const bool vec = d % V == 0 && aligned16(out);
+  const unsigned nb = buf ? x_grid((tokens * (vec ? d / V : d) + 255) / 256) : 0;
+  const unsigned ng = dg ? x_grid((tokens * k + 255) / 256) : 0;
+  if (vec)
+    k_rows_sum<T, V><<<nb + ng, 256, 0, st>>>(buf, ldb, out, tokens, k, d, slot_row, nb, dgpart, nparts, dg);
+  else
+    k_rows_sum<T, 1><<<nb + ng, 256, 0, st>>>(buf, ldb, out, tokens, k, d, slot_row, nb, dgpart, nparts, dg);
+  return check_launch("expert_linear (sum)");
 }
 
 }  // namespace mb
@@ -538,13 +620,22 @@ extern "C" int mace_b200_expert_linear_few(const void* x, int64_t ldx, int32_t x
     constexpr int V = kVec<T>;
     const bool vec = D % V == 0 && ldx % V == 0 && aligned16(x) && aligned16(w);
     const int kx = x_per_slot ? 1 : k;
-    const dim3 grid((O + 3) / 4, (unsigned)(weights ? tokens : s.R));
+    const int L = (vec ? D / V : D) <= 64 ? 8 : 32;   // narrow rows: four outputs per warp
+    const dim3 grid((O + 128 / L - 1) / (128 / L), (unsigned)(weights ? tokens : s.R));
     auto go = [&](auto kern) {
       kern<<<grid, 128, 0, st>>>((const T*)x, ldx, kx, (const T*)w, experts, weights, (T*)out, k, E, D, O);
       return check_launch("expert_linear_few");
     };
-    if (weights) return vec ? go(k_expert_few<T, V, false>) : go(k_expert_few<T, 1, false>);
-    return vec ? go(k_expert_few<T, V, true>) : go(k_expert_few<T, 1, true>);
+    auto form = [&](auto v, auto l) {
+      constexpr int VV = decltype(v)::value, LL = decltype(l)::value;
+      return weights ? go(k_expert_few<T, VV, LL, false>) : go(k_expert_few<T, VV, LL, true>);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Vec = std::integral_constant<int, V>;
+    using Narrow = std::integral_constant<int, 8>;
+    using Wide = std::integral_constant<int, 32>;
+    if (vec) return L == 8 ? form(Vec(), Narrow()) : form(Vec(), Wide());
+    return L == 8 ? form(One(), Narrow()) : form(One(), Wide());
   });
 }
 
@@ -565,26 +656,23 @@ extern "C" int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x
   char* base = (char*)workspace;
   return x_types(dtype, [&](auto t) {
     using T = decltype(t);
-    if (!direct)
-      if (int rc = x_stage_w<T>(s, w, base + f.ws, st)) return rc;
-    if (int rc = x_gather<T>(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, plan, nullptr, base + f.xs, nullptr, st)) return rc;
+    const bool sum = f.y >= 0;
+    XMoves mv{};
+    mv.m[mv.n++] = move_gather(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, nullptr, base + f.xs);
+    if (!direct) mv.m[mv.n++] = move_stage(s, w, base + f.ws);
+    if (!sum) mv.m[mv.n++] = move_zero(s, out, O);
+    if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
     XGemm g{};
     g.mode = XG_FWD; g.dtype = dtype;
     g.a = base + f.xs; g.rows = s.rows; g.lda = s.Dp;
     g.b = direct ? w : base + f.ws; g.ldb = s.Dp;
     g.E = E; g.M = 0; g.N = O; g.K = D;
     g.plan = plan; g.lay = s.lay; g.scale = weights;
-    const bool sum = f.y >= 0;
     g.out = sum ? (void*)(base + f.y) : out;
     g.ldo = sum ? s.Op : O;
     if (int rc = xgemm_launch(g, st)) return rc;
-    const int32_t* slot_row = plan + s.lay.o_slot;
-    if (sum)
-      k_rows_sum<T><<<x_grid((tokens + 7) / 8), 256, 0, st>>>((const T*)(base + f.y), s.Op, (T*)out, tokens, k, O,
-                                                              aligned16(out) && O % 8 == 0, slot_row, nullptr, 0, nullptr);
-    else
-      k_rows_zero<T><<<x_grid((s.R + 7) / 8), 256, 0, st>>>((T*)out, s.R, O, slot_row);
-    return check_launch("expert_linear_fwd");
+    if (!sum) return 0;
+    return x_rows_sum<T>((const T*)(base + f.y), s.Op, (T*)out, tokens, k, O, plan + s.lay.o_slot, nullptr, 0, nullptr, st);
   });
 }
 
@@ -610,31 +698,38 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
   const int kx = x_per_slot ? 1 : k, ky = combine ? k : 1;
   return x_types(dtype, [&](auto t) {
     using T = decltype(t);
-    if (b.dys >= 0 || b.gdy >= 0)
-      if (int rc = x_gather<T>(s, dy, O, O, s.Op, ky, plan, weights, b.dys >= 0 ? base + b.dys : nullptr,
-                               b.gdy >= 0 ? base + b.gdy : nullptr, st))
-        return rc;
+    const bool sum = b.dxb >= 0;
+    XMoves mv{};
+    mv.m[mv.n++] = move_gather(s, dy, O, O, s.Op, ky, nullptr, base + b.dys);
+    // the weights scale the rows of x, not those of dy: dy stays exact for dx and dweights, and x is read only here
+    if (dw) mv.m[mv.n++] = move_gather(s, x, ldx, D, s.Dp, kx, weights, base + b.xs);
+    if (b.ws >= 0) mv.m[mv.n++] = move_stage(s, w, base + b.ws);
+    if (dx && !sum) mv.m[mv.n++] = move_zero(s, dx, D);
+    if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
     if (dw) {
-      if (int rc = x_gather<T>(s, x, ldx, D, s.Dp, kx, plan, nullptr, base + b.xs, nullptr, st)) return rc;
       XGemm g{};
       g.mode = XG_WGRAD; g.dtype = dtype;
-      g.a = combine ? base + b.gdy : base + b.dys; g.lda = s.Op;
+      g.a = base + b.dys; g.lda = s.Op;
       g.b = base + b.xs; g.ldb = s.Dp;
       g.rows = s.rows;
       g.E = E; g.M = O; g.N = D; g.K = 0;
-      g.plan = plan; g.lay = s.lay; g.out = dw; g.ldo = D;
+      g.plan = plan; g.lay = s.lay; g.split = b.split;
+      g.out = b.split > 1 ? (void*)(base + b.parts) : dw;
+      g.ldo = D;
       if (int rc = xgemm_launch(g, st)) return rc;
+      if (b.split > 1) {
+        const int64_t n = (int64_t)E * O * D;
+        k_parts_sum<T><<<x_grid((n + 255) / 256), 256, 0, st>>>((const float*)(base + b.parts), b.split, n, (T*)dw);
+        if (int rc = check_launch("expert_linear (parts)")) return rc;
+      }
     }
     if (!dx && !dweights) return 0;
-    if (!direct)
-      if (int rc = x_stage_w<T>(s, w, base + b.ws, st)) return rc;
     XGemm g{};
     g.mode = XG_DGRAD; g.dtype = dtype;
     g.a = base + b.dys; g.rows = s.rows; g.lda = s.Op;
     g.b = direct ? w : base + b.ws; g.ldb = s.Dp;
     g.E = E; g.M = 0; g.N = D; g.K = O;
     g.plan = plan; g.lay = s.lay; g.scale = weights;
-    const bool sum = b.dxb >= 0;
     g.out = sum ? (void*)(base + b.dxb) : dx;
     g.ldo = sum ? s.Dp : D;
     if (dweights) {
@@ -642,15 +737,8 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
       g.dgpart = (float*)(base + b.dgp);
     }
     if (int rc = xgemm_launch(g, st)) return rc;
-    const int32_t* slot_row = plan + s.lay.o_slot;
-    if (dx && !sum) {
-      k_rows_zero<T><<<x_grid((s.R + 7) / 8), 256, 0, st>>>((T*)dx, s.R, D, slot_row);
-      if (int rc = check_launch("expert_linear_bwd")) return rc;
-    }
     if (!sum && !dweights) return 0;
-    k_rows_sum<T><<<x_grid((tokens + 7) / 8), 256, 0, st>>>(
-        sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, aligned16(dx) && D % 8 == 0, slot_row,
-        (const float*)(base + b.dgp), dweights ? xgemm_n_tiles(XG_DGRAD, D) : 0, dweights);
-    return check_launch("expert_linear_bwd");
+    return x_rows_sum<T>(sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, plan + s.lay.o_slot,
+                         dweights ? (const float*)(base + b.dgp) : nullptr, xgemm_n_tiles(XG_DGRAD, D), dweights, st);
   });
 }

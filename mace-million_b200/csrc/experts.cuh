@@ -49,6 +49,7 @@ struct XGemm {
   const float* scale;                            // per slot, or null
   void* out;                                     // FWD / DGRAD: [slots][ldo] (null: only dgpart); WGRAD: [E][M][N]
   int64_t ldo;
+  int32_t split;                                 // WGRAD: parts of each expert's rows; > 1: out is fp32 [split][E][M][N]
   // DGRAD: dgpart[n tile][slot] = partial <x, C> of the slot's x row (null: off)
   const void* x;
   int64_t ldx;
@@ -56,6 +57,7 @@ struct XGemm {
   float* dgpart;
 };
 int xgemm_n_tiles(int mode, int64_t N);
+int xgemm_split(int64_t E, int64_t M, int64_t N, int64_t slots, int planes);
 int xgemm_launch(const XGemm& g, cudaStream_t st);
 
 }  // namespace mb

@@ -31,6 +31,7 @@ struct XgCfg {
 
 struct XgParams {
   int32_t E, M, N, K, tn, tm, np;                // tn / tm: tiles along N, along M (WGRAD)
+  int32_t split;                                 // WGRAD: parts of an expert's rows
   int64_t rows;                                  // rows per plane of the sorted operands
   int32_t w_rows;                                // E (planes of w follow each other)
   const int32_t* plan;
@@ -73,7 +74,8 @@ __device__ __forceinline__ void xg_store32(T* dst, const float (&f)[32], int n, 
   }
 }
 
-template <int MODE, typename T, int BN>
+// OUT: element type of the output (T, or float for partial sums)
+template <int MODE, typename T, typename OUT, int BN>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
   using C = XgCfg<BN>;
@@ -107,21 +109,25 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = B.tmem;
   const int32_t* plan = g.plan;
-  const int tiles = MODE == XG_WGRAD ? g.E * g.tm * g.tn : plan[0] * g.tn;
+  const int tiles = MODE == XG_WGRAD ? g.split * g.E * g.tm * g.tn : plan[0] * g.tn;
 
   // tile -> (expert, first row of A / first output row, first column, K blocks)
   struct Tile {
-    int e, m0, n0, r0, nk;
+    int e, m0, n0, r0, nk, se;
   };
   auto tile_of = [&](int t) {
     Tile o;
     const int m = t / g.tn;
     o.n0 = (t - m * g.tn) * BN;
     if constexpr (MODE == XG_WGRAD) {
-      o.e = m / g.tm;
-      o.m0 = (m - o.e * g.tm) * XG_BM;
-      o.r0 = plan[g.lay.o_seg + o.e];
-      o.nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK;
+      const int se = m / g.tm, part = se / g.E;
+      o.e = se - part * g.E;
+      o.m0 = (m - se * g.tm) * XG_BM;
+      o.se = se;
+      const int nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK;
+      const int k0 = (int)((int64_t)nk * part / g.split);
+      o.r0 = plan[g.lay.o_seg + o.e] + k0 * XG_BK;
+      o.nk = (int)((int64_t)nk * (part + 1) / g.split) - k0;
     } else {
       o.e = plan[g.lay.o_tile + m];
       o.m0 = o.r0 = m * XG_BM;
@@ -232,21 +238,21 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       if (__shfl_sync(0xffffffffu, *failed, 0)) break;
       const Tile w = tile_of(t);
-      T* dst = nullptr;
+      OUT* dst = nullptr;
       float sc = 1.f, dot = 0.f;
       const T* xr = nullptr;
       int slot = -1;
       if constexpr (MODE == XG_WGRAD) {
-        if (w.m0 + row < g.M) dst = (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo;
+        if (w.m0 + row < g.M) dst = (OUT*)g.out + ((int64_t)w.se * g.M + w.m0 + row) * g.ldo;
       } else {
         slot = plan[g.lay.o_row + w.m0 + row];
         if (slot >= 0) {
-          if (g.out) dst = (T*)g.out + (int64_t)slot * g.ldo;
+          if (g.out) dst = (OUT*)g.out + (int64_t)slot * g.ldo;
           if (g.scale) sc = g.scale[slot];
           if (MODE == XG_DGRAD && g.dgpart) xr = (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx;
         }
       }
-      const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+      const bool vec = g.ldo % kVec<OUT> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
       const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
       const int acc = tc & 1;
       if (w.nk > 0) {
@@ -275,17 +281,27 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         if (MODE == XG_DGRAD && xr) {
           const T* xp = xr + w.n0 + 32 * h;
           if (xvec && n >= 32) {
+            // one short chain per vector, added up as a tree over the chunk: the rounding of 256 terms in a row shows
+            float part[32 / kVec<T>];
 #pragma unroll
             for (int q = 0; q < 32 / kVec<T>; ++q) {
               float v[kVec<T>];
               load_v<T, kVec<T>>(xp + q * kVec<T>, v);
+              part[q] = 0.f;
 #pragma unroll
-              for (int i = 0; i < kVec<T>; ++i) dot = fmaf(v[i], f[q * kVec<T> + i], dot);
+              for (int i = 0; i < kVec<T>; ++i) part[q] = fmaf(v[i], f[q * kVec<T> + i], part[q]);
             }
+#pragma unroll
+            for (int w = 16 / kVec<T>; w >= 1; w >>= 1)
+#pragma unroll
+              for (int q = 0; q < w; ++q) part[q] += part[q + w];
+            dot += part[0];
           } else {
+            float part = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i < n) dot = fmaf(to_f(xp[i]), f[i], dot);
+              if (i < n) part = fmaf(to_f(xp[i]), f[i], part);
+            dot += part;
           }
         }
         if (dst) {
@@ -293,7 +309,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] *= sc;
           }
-          xg_store32<T>(dst + w.n0 + 32 * h, f, n, vec);
+          xg_store32<OUT>(dst + w.n0 + 32 * h, f, n, vec);
         }
       }
       if (MODE == XG_DGRAD && xr) g.dgpart[(int64_t)(w.n0 / BN) * g.lay.R + slot] = dot;
@@ -362,13 +378,23 @@ int xgemm_n_tiles(int mode, int64_t N) {
   return (int)((N + xg_bn(N) - 1) / xg_bn(N));
 }
 
-template <int MODE, typename T, int BN>
+// Parts of each expert's rows in WGRAD: enough tiles for four per SM when there are few, with at least 16 K blocks left
+// in an average part (below that the partial sums cost more than the idle SMs)
+int xgemm_split(int64_t E, int64_t M, int64_t N, int64_t slots, int planes) {
+  const int64_t tiles = E * ((M + XG_BM - 1) / XG_BM) * ((N + xg_bn(N) - 1) / xg_bn(N));
+  const int64_t blocks = slots / E / XG_BK * (planes == 3 ? 6 : 1);
+  int64_t s = 4 * (int64_t)sm_count() / tiles;
+  if (s > blocks / 16) s = blocks / 16;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+template <int MODE, typename T, typename OUT, int BN>
 static int xg_go(const XGemm& x, cudaStream_t st) {
   using C = XgCfg<BN>;
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
-  auto kern = k_expert_gemm<MODE, T, BN>;
+  auto kern = k_expert_gemm<MODE, T, OUT, BN>;
   if (ready_dev != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -401,8 +427,9 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   g.rows = x.rows; g.w_rows = x.E;
   g.plan = x.plan; g.lay = x.lay; g.scale = x.scale;
   g.out = x.out; g.ldo = x.ldo;
+  g.split = x.split > 1 ? x.split : 1;
   g.x = x.x; g.ldx = x.ldx; g.kdiv = x.kdiv; g.dgpart = x.dgpart;
-  const int64_t most = MODE == XG_WGRAD ? (int64_t)x.E * g.tm * g.tn : x.lay.tiles * g.tn;
+  const int64_t most = MODE == XG_WGRAD ? (int64_t)g.split * x.E * g.tm * g.tn : x.lay.tiles * g.tn;
   if (most > 0x7fffffff || np * x.rows > 0x7fffffff) {
     set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)most, (long long)(np * x.rows));
     return MB_E_ARG;
@@ -415,7 +442,9 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
 
 template <int MODE, typename T>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
-  return xg_bn(x.N) == 128 ? xg_go<MODE, T, 128>(x, st) : xg_go<MODE, T, 256>(x, st);
+  if constexpr (MODE == XG_WGRAD)
+    if (x.split > 1) return xg_bn(x.N) == 128 ? xg_go<MODE, T, float, 128>(x, st) : xg_go<MODE, T, float, 256>(x, st);
+  return xg_bn(x.N) == 128 ? xg_go<MODE, T, T, 128>(x, st) : xg_go<MODE, T, T, 256>(x, st);
 }
 
 template <int MODE>

@@ -45,11 +45,25 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
     }
     s = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 2);
     s += __shfl_xor_sync(0xffffffffu, s, 1);
+  } else if constexpr (K == 4) {                  // likewise: lane L holds value L >> 3 (6 shuffles instead of 20)
+#pragma unroll
+    for (int h = 2, bit = 16; h >= 1; h >>= 1, bit >>= 1) {
+      const bool up = lane & bit;
+#pragma unroll
+      for (int q = 0; q < h; ++q) {
+        const float send = up ? v[q] : v[q + h];
+        const float keep = up ? v[q + h] : v[q];
+        v[q] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
+      }
+    }
+    s = v[0];
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
   if constexpr (G == 32) {
-    if constexpr (K == 8) {
+    if constexpr (K == 8 || K == 4) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, 4 * k);
+      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, 32 / K * k);
     } else {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
@@ -57,8 +71,8 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
         for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
   } else {
-    if constexpr (K == 8) {
-      if ((lane & 3) == 0) red[warp * K + (lane >> 2)] = s;
+    if constexpr (K == 8 || K == 4) {
+      if (lane % (32 / K) == 0) red[warp * K + lane / (32 / K)] = s;
     } else {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
@@ -81,11 +95,20 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
 
 template <int G>
 constexpr int ln_threads = G < 256 ? 256 : G;
+// blocks per SM that the registers of a thread are budgeted for (nothing spills beyond a few words)
+#ifndef MB_LN8
+#define MB_LN8 768
+#endif
+template <int G, int NV, int V>
+constexpr int ln_fwd_blocks = (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> > 0 ? (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> : 1;
+template <int G>
+constexpr int ln_bwd_blocks = G == 32 || G == 256 ? 3 : G < 256 ? 2 : 1;
 
+// The row is held as loaded (16-bit rows take half the registers of fp32 values) and unpacked at each use.
 template <typename T, typename P, int G, int NV, int V>
-__global__ void __launch_bounds__(ln_threads<G>) k_ln_fwd(const LnArgs a) {
+__global__ void __launch_bounds__(ln_threads<G>, ln_fwd_blocks<G, NV, V>) k_ln_fwd(const LnArgs a) {
   constexpr int RPB = ln_threads<G> / G;
-  constexpr bool KEEP = NV * V <= 32;             // parameters stay in registers over the rows, else from L1 per row
+  constexpr bool KEEP = NV * V <= 8;              // parameters stay in registers over the rows, else from L1 per row
   __shared__ float red[2][ln_threads<G> / 32];
   const int t = threadIdx.x % G, g = threadIdx.x / G, d = a.d;
   const P *w = (const P*)a.w, *b = (const P*)a.b;
@@ -108,26 +131,31 @@ __global__ void __launch_bounds__(ln_threads<G>) k_ln_fwd(const LnArgs a) {
     const int64_t row = r0 + g;
     const bool live = row < a.n;
     const T* x = (const T*)a.x + (live ? row : 0) * a.ldx;
-    float v[NV][V], s[1] = {0.f};
+    Raw<T, V> v[NV];
+    float s[1] = {0.f}, f[V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * G + t) * V;
-#pragma unroll
-      for (int q = 0; q < V; ++q) v[i][q] = 0.f;
-      if (live && j < d) load_v<T, V>(x + j, v[i]);
+      v[i].zero();
+      if (live && j < d) v[i].load(x + j);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      v[i].get(f);
 #pragma unroll
-      for (int q = 0; q < V; ++q) s[0] += v[i][q];
+      for (int q = 0; q < V; ++q) s[0] += f[q];
+    }
     group_sum<G, 1>(s, red[0]);
     const float mu = s[0] * inv;
     s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if ((i * G + t) * V < d)
+      if ((i * G + t) * V < d) {
+        v[i].again();
+        v[i].get(f);
 #pragma unroll
-        for (int q = 0; q < V; ++q) s[0] += (v[i][q] - mu) * (v[i][q] - mu);
+        for (int q = 0; q < V; ++q) s[0] += (f[q] - mu) * (f[q] - mu);
+      }
     group_sum<G, 1>(s, red[1]);
     const float r = rsqrtf(s[0] * inv + a.eps);
     if (!live) continue;
@@ -136,13 +164,14 @@ __global__ void __launch_bounds__(ln_threads<G>) k_ln_fwd(const LnArgs a) {
     for (int i = 0; i < NV; ++i) {
       const int j = (i * G + t) * V;
       if (j >= d) continue;
-      float fw[V], fb[V], o[V];
+      float fw[V], fb[V];
       if constexpr (!KEEP) params(i, fw, fb);
+      v[i].again();
+      v[i].get(f);
 #pragma unroll
       for (int q = 0; q < V; ++q)
-        o[q] = KEEP ? fmaf((v[i][q] - mu) * r, pw[KEEP ? i : 0][q], pb[KEEP ? i : 0][q])
-                    : fmaf((v[i][q] - mu) * r, fw[q], fb[q]);
-      store_v<T, V>(y + j, o);
+        f[q] = KEEP ? fmaf((f[q] - mu) * r, pw[KEEP ? i : 0][q], pb[KEEP ? i : 0][q]) : fmaf((f[q] - mu) * r, fw[q], fb[q]);
+      store_v<T, V>(y + j, f);
     }
     if (t == 0 && a.mean) {
       a.mean[row] = mu;
@@ -180,10 +209,10 @@ __global__ void __launch_bounds__(1024) k_ln_fwd_wide(const LnArgs a) {
   }
 }
 
-// partial[block][0 .. d) = sum of dy xh, [d .. 2 d) = sum of dy over the block's rows.  RB rows at a time, so that a
-// group has 2 RB loads in flight and one synchronisation per RB rows.
-template <typename T, typename P, int G, int NV, int V, int RB>
-__global__ void __launch_bounds__(ln_threads<G>) k_ln_bwd(const LnArgs a) {
+// partial[block][0 .. d) = sum of dy xh, [d .. 2 d) = sum of dy over the block's rows.  RB rows at a time with one
+// synchronisation, and the next RB rows' loads in flight meanwhile (PRE).
+template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
+__global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G>) k_ln_bwd(const LnArgs a) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
   __shared__ float red[2][TH / 32 * 2 * RB];
   extern __shared__ float cols[];                 // [RPB][2][d] when RPB > 1
@@ -198,9 +227,9 @@ __global__ void __launch_bounds__(ln_threads<G>) k_ln_bwd(const LnArgs a) {
     if (w && j < d) load_p<P, V>(w + j, pw[i]);
   }
   const float inv = 1.f / (float)d;
-  int buf = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB * RB; r0 < a.n; r0 += (int64_t)gridDim.x * RPB * RB, buf ^= 1) {
-    float xv[RB][NV][V], dv[RB][NV][V], rs[RB], s[2 * RB], mu[RB];
+  Raw<T, V> xv[RB][NV], dv[RB][NV];
+  float rs[RB], mu[RB];
+  auto fetch = [&](int64_t r0) {
 #pragma unroll
     for (int k = 0; k < RB; ++k) {
       const int64_t row = r0 + g * RB + k;
@@ -212,28 +241,48 @@ __global__ void __launch_bounds__(ln_threads<G>) k_ln_bwd(const LnArgs a) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int j = (i * G + t) * V;
-#pragma unroll
-        for (int q = 0; q < V; ++q) xv[k][i][q] = 0.f, dv[k][i][q] = 0.f;
+        xv[k][i].zero();
+        dv[k][i].zero();
         if (live && j < d) {
-          load_v<T, V>(x + j, xv[k][i]);
-          load_v<T, V>(dy + j, dv[k][i]);
+          xv[k][i].load(x + j);
+          dv[k][i].load(dy + j);
         }
       }
     }
+  };
+  int buf = 0;
+  const int64_t step = (int64_t)gridDim.x * RPB * RB;
+  if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB * RB);
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB * RB; r0 < a.n; r0 += step, buf ^= 1) {
+    if constexpr (!PRE) fetch(r0);
+    Raw<T, V> xc[RB][NV], dc[RB][NV];
+    float rc[RB], mc[RB], s[2 * RB];
+#pragma unroll
+    for (int k = 0; k < RB; ++k) {
+      rc[k] = rs[k];
+      mc[k] = mu[k];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) xc[k][i] = xv[k][i], dc[k][i] = dv[k][i];
+    }
+    if constexpr (PRE)
+      if (r0 + step < a.n) fetch(r0 + step);
 #pragma unroll
     for (int k = 0; k < RB; ++k) {
       s[2 * k] = s[2 * k + 1] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if ((i * G + t) * V >= d) continue;
+        float fx[V], fd[V];
+        xc[k][i].get(fx);
+        dc[k][i].get(fd);
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-          const float xh = (xv[k][i][q] - mu[k]) * rs[k], dy = dv[k][i][q];
-          const float up = __fmul_rn(dy, pw[i][q]);   // the same rounding here and below: dx of a constant is 0
+          const float xh = (fx[q] - mc[k]) * rc[k];
+          const float up = __fmul_rn(fd[q], pw[i][q]);   // the same rounding here and below: dx of a constant is 0
           s[2 * k] += up;
           s[2 * k + 1] += up * xh;
-          aw[i][q] += dy * xh;
-          ab[i][q] += dy;
+          aw[i][q] += fd[q] * xh;
+          ab[i][q] += fd[q];
         }
       }
     }
@@ -249,13 +298,17 @@ __global__ void __launch_bounds__(ln_threads<G>) k_ln_bwd(const LnArgs a) {
         for (int i = 0; i < NV; ++i) {
           const int j = (i * G + t) * V;
           if (j >= d) continue;
-          float o[V];
+          float fx[V], fd[V];
+          xc[k][i].again();
+          dc[k][i].again();
+          xc[k][i].get(fx);
+          dc[k][i].get(fd);
 #pragma unroll
           for (int q = 0; q < V; ++q) {
-            const float xh = (xv[k][i][q] - mu[k]) * rs[k];
-            o[q] = rs[k] * (__fmul_rn(dv[k][i][q], pw[i][q]) - m1 - xh * m2);
+            const float xh = (fx[q] - mc[k]) * rc[k];
+            fx[q] = rc[k] * (__fmul_rn(fd[q], pw[i][q]) - m1 - xh * m2);
           }
-          store_v<T, V>(dx + j, o);
+          store_v<T, V>(dx + j, fx);
         }
       }
     }
@@ -333,41 +386,38 @@ __global__ void __launch_bounds__(128) k_ln_cols_wide(const LnArgs a) {
   out[d + j] = sb;
 }
 
-// Adds the partial sums of the blocks in a fixed order: 32 columns x 8 interleaved sets of partials per block
+// Adds the partial sums of the blocks in a fixed order: 32 columns x 32 interleaved sets of partials per block
 template <typename P>
-__global__ void __launch_bounds__(256) k_ln_reduce(const float* partial, int nb, int32_t d, P* dw, P* db) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) k_ln_reduce(const float* partial, int nb, int32_t d, P* dw, P* db) {
+  __shared__ float red[32][33];
   const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + c;
   float s = 0.f;
-  if (j < 2 * (int64_t)d)
-    for (int k = q; k < nb; k += 8) s += partial[(int64_t)k * 2 * d + j];
+  if (j < 2 * (int64_t)d) {
+    const float* p = partial + j;
+#pragma unroll 8
+    for (int k = q; k < nb; k += 32) s += p[(int64_t)k * 2 * d];
+  }
   red[q][c] = s;
   __syncthreads();
-  if (q == 0 && j < 2 * (int64_t)d) {
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s += red[k][c];
-    if (j < d) {
-      if (dw) dw[j] = from_f<P>(s);
-    } else if (db) {
-      db[j - d] = from_f<P>(s);
+  s = warp_sum(red[c][q]);                        // warp q: column q
+  const int64_t o = (int64_t)blockIdx.x * 32 + q;
+  if (c == 0) {
+    if (o < d) {
+      if (dw) dw[o] = from_f<P>(s);
+    } else if (o < 2 * (int64_t)d && db) {
+      db[o - d] = from_f<P>(s);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int LN_BLOCKS_PER_SM = 3;              // of the backward kernel: the row count of the partial sums
-
-static int ln_bwd_blocks(int64_t n, int rows_per_pass) {
-  const int64_t want = (n + rows_per_pass - 1) / rows_per_pass, most = (int64_t)LN_BLOCKS_PER_SM * sm_count();
-  return (int)(want < most ? want : most);
-}
+constexpr int LN_BLOCKS_PER_SM = 3;              // at most, of the backward kernel: bounds the rows of partial sums
 
 template <typename T, typename P, int G, int NV, int V>
 static int ln_fwd_launch(const LnArgs& a, cudaStream_t st) {
   constexpr int RPB = ln_threads<G> / G;
-  const int64_t want = (a.n + RPB - 1) / RPB, most = (int64_t)8 * sm_count();
+  const int64_t want = (a.n + RPB - 1) / RPB, most = (int64_t)ln_fwd_blocks<G, NV, V> * sm_count();
   k_ln_fwd<T, P, G, NV, V><<<(unsigned)(want < most ? want : most), ln_threads<G>, 0, st>>>(a);
   return check_launch("layer_norm_fwd");
 }
@@ -375,59 +425,60 @@ static int ln_fwd_launch(const LnArgs& a, cudaStream_t st) {
 template <typename T, typename P>
 static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
   constexpr int V = kVec<T>;
-  if (vec) {                                      // one warp per row up to 64 values per lane, then 4 and 16 warps
+  if (vec) {                                      // one warp per row up to 8 vectors per lane, then 4 and 16 warps
     const int nv = (a.d / V + 31) / 32;
     if (nv <= 1) return ln_fwd_launch<T, P, 32, 1, V>(a, st);
     if (nv <= 2) return ln_fwd_launch<T, P, 32, 2, V>(a, st);
     if (nv <= 4) return ln_fwd_launch<T, P, 32, 4, V>(a, st);
-    if (nv * V <= 64) return ln_fwd_launch<T, P, 32, 64 / V, V>(a, st);
-    if (nv * V <= 256) return ln_fwd_launch<T, P, 128, 64 / V, V>(a, st);
-    if (nv * V <= 1024) return ln_fwd_launch<T, P, 512, 64 / V, V>(a, st);
+    if (nv <= 8) return ln_fwd_launch<T, P, 32, 8, V>(a, st);
+    if (nv <= 32) return ln_fwd_launch<T, P, 128, 8, V>(a, st);
+    if (nv <= 128) return ln_fwd_launch<T, P, 512, 8, V>(a, st);
   } else {
     if (a.d <= 128) return ln_fwd_launch<T, P, 32, 4, 1>(a, st);
-    if (a.d <= 512) return ln_fwd_launch<T, P, 32, 16, 1>(a, st);
-    if (a.d <= 1024) return ln_fwd_launch<T, P, 32, 32, 1>(a, st);
-    if (a.d <= 4096) return ln_fwd_launch<T, P, 128, 32, 1>(a, st);
-    if (a.d <= 16384) return ln_fwd_launch<T, P, 512, 32, 1>(a, st);
+    if (a.d <= 256) return ln_fwd_launch<T, P, 32, 8, 1>(a, st);
+    if (a.d <= 640) return ln_fwd_launch<T, P, 128, 5, 1>(a, st);
+    if (a.d <= 1024) return ln_fwd_launch<T, P, 128, 8, 1>(a, st);
+    if (a.d <= 2048) return ln_fwd_launch<T, P, 256, 8, 1>(a, st);
+    if (a.d <= 8192) return ln_fwd_launch<T, P, 1024, 8, 1>(a, st);
   }
   const int64_t most = (int64_t)2 * sm_count();
   k_ln_fwd_wide<T, P><<<(unsigned)(a.n < most ? a.n : most), 1024, 0, st>>>(a);
   return check_launch("layer_norm_fwd");
 }
 
-// Number of partial-sum rows, or the launch (when `go`)
-template <typename T, typename P, int G, int NV, int V, int RB>
-static int ln_bwd_launch(const LnArgs& a, bool go, int* nb, cudaStream_t st) {
+// Launches and says how many rows of partial sums there are
+template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
+static int ln_bwd_launch(const LnArgs& a, int* nb, cudaStream_t st) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
-  *nb = ln_bwd_blocks(a.n, RPB * RB);
-  if (!go) return 0;
+  const int64_t want = (a.n + RPB * RB - 1) / (RPB * RB), most = (int64_t)ln_bwd_blocks<G> * sm_count();
+  *nb = (int)(want < most ? want : most);
   const int smem = RPB > 1 && a.partial ? RPB * 2 * a.d * 4 : 0;
-  static_assert(RPB == 1 || RPB * 2 * G * NV * V * 4 <= 48 * 1024, "column sums in shared memory");
-  k_ln_bwd<T, P, G, NV, V, RB><<<*nb, TH, smem, st>>>(a);
+  static_assert(RPB == 1 || RPB * 2 * G * NV * V * 4 <= 40 * 1024, "column sums in shared memory");
+  k_ln_bwd<T, P, G, NV, V, RB, PRE><<<*nb, TH, smem, st>>>(a);
   return check_launch("layer_norm_bwd");
 }
 
 template <typename T, typename P>
-static int ln_bwd_any(const LnArgs& a, bool vec, bool go, int* nb, cudaStream_t st) {
+static int ln_bwd_any(const LnArgs& a, bool vec, int* nb, cudaStream_t st) {
   constexpr int V = kVec<T>;
   if (vec) {
     const int c = a.d / V;
-    if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 4>(a, go, nb, st);
-    if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 4>(a, go, nb, st);
-    if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 4>(a, go, nb, st);
-    if (c <= 256) return ln_bwd_launch<T, P, 256, 1, V, 4>(a, go, nb, st);
-    if (c <= 512) return ln_bwd_launch<T, P, 512, 1, V, 4>(a, go, nb, st);
-    if (c <= 1024) return ln_bwd_launch<T, P, 512, 2, V, 1>(a, go, nb, st);
+    if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 2, true>(a, nb, st);
+    if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 2, true>(a, nb, st);
+    if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 2, true>(a, nb, st);
+    if (c <= 256) return ln_bwd_launch<T, P, 256, 1, V, 2, true>(a, nb, st);
+    if (c <= 512) return ln_bwd_launch<T, P, 512, 1, V, 2, true>(a, nb, st);
+    if (c <= 1024) return ln_bwd_launch<T, P, 512, 2, V, 1, true>(a, nb, st);
   } else {
-    if (a.d <= 128) return ln_bwd_launch<T, P, 32, 4, 1, 4>(a, go, nb, st);
-    if (a.d <= 256) return ln_bwd_launch<T, P, 64, 4, 1, 4>(a, go, nb, st);
-    if (a.d <= 512) return ln_bwd_launch<T, P, 128, 4, 1, 4>(a, go, nb, st);
-    if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 4>(a, go, nb, st);
-    if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 4>(a, go, nb, st);
+    if (a.d <= 128) return ln_bwd_launch<T, P, 32, 4, 1, 2, true>(a, nb, st);
+    if (a.d <= 256) return ln_bwd_launch<T, P, 64, 4, 1, 2, true>(a, nb, st);
+    if (a.d <= 640) return ln_bwd_launch<T, P, 128, 5, 1, 2, true>(a, nb, st);
+    if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 2, true>(a, nb, st);
+    if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 2, true>(a, nb, st);
+    if (a.d <= 4096) return ln_bwd_launch<T, P, 1024, 4, 1, 2, true>(a, nb, st);
   }
   const int64_t most = (int64_t)2 * sm_count();
   *nb = (int)(a.n < 64 ? a.n : 64);
-  if (!go) return 0;
   if (a.dx) {
     k_ln_bwd_wide<T, P><<<(unsigned)(a.n < most ? a.n : most), 1024, 0, st>>>(a);
     if (int rc = check_launch("layer_norm_bwd")) return rc;
@@ -521,9 +572,9 @@ extern "C" int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void
     using P = decltype(p);
     int nb = 0;
     if (n > 0)
-      if (int rc = ln_bwd_any<T, P>(a, vec, true, &nb, (cudaStream_t)stream)) return rc;
+      if (int rc = ln_bwd_any<T, P>(a, vec, &nb, (cudaStream_t)stream)) return rc;
     if (!dw && !db) return 0;
-    k_ln_reduce<P><<<(unsigned)((2 * (int64_t)d + 31) / 32), 256, 0, (cudaStream_t)stream>>>(workspace, nb, d, (P*)dw,
+    k_ln_reduce<P><<<(unsigned)((2 * (int64_t)d + 31) / 32), 1024, 0, (cudaStream_t)stream>>>(workspace, nb, d, (P*)dw,
                                                                                              (P*)db);
     return check_launch("layer_norm_bwd");
   });

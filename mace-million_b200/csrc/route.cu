@@ -8,8 +8,14 @@
 //   renormalise: ds_j = scale (dw_j - sum_i dw_i q_i) / S, else ds_j = scale dw_j;
 //   softmax: dl_i = s_i (ds_i - sum_j s_j ds_j), sigmoid: dl_i = ds_i s_i (1 - s_i).
 //
-// One warp per token, expert i in lane i % 32 (coalesced rows), all scores in registers.  The k choices are k warp-wide
-// maxima of order-preserving integer keys (redux), so the comparisons are exact.  The algorithm reads each logit once.
+// Forward: L lanes of a warp per token, lane q holding the c experts q c .. q c + c - 1 in registers, so that a warp
+// works on 32 / L tokens.  A choice is a maximum of order-preserving integer keys over the lane's registers and L lanes,
+// and the lowest lane that has it wins (the lowest index among equals); comparisons are exact.  Bound by issued
+// instructions (k maxima over E keys, E exponentials where all scores count), not by the logits' bytes: 131,072 x 128 bf16
+// sigmoid, 8 groups, k = 8 takes FWDUS us against 5.2 us for the bytes; a whole warp per token took 162 us (its reductions
+// cross 32 lanes for 4 keys a lane).  Few tokens take L = 32, which has the shortest chain.
+// Backward: only the chosen logits enter, except for plain softmax weights; a warp fills a tile of zeros in shared memory
+// with the k values of its tokens and copies it out in whole vectors.
 #include "dtypes.cuh"
 
 namespace mb {
@@ -17,6 +23,7 @@ namespace mb {
 constexpr int RT_WARPS = 8;
 
 struct RouteArgs {
+  int32_t c, vec, all;                            // forward: experts per lane, vector loads, all scores needed
   const void* logits;
   const float *bias, *dw;
   float* w;
@@ -36,15 +43,235 @@ __device__ __forceinline__ unsigned order_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Scores of one token's experts (lane holds i = lane + 32 j): softmax numerators and their sum, or sigmoids (sum 1).
-// The functions and roundings are those of exp() and division in plain fp32 arithmetic.
-template <int NE>
-__device__ __forceinline__ float route_scores(const float (&l)[NE], int softmax, float (&s)[NE]) {
-  if (!softmax) {
+// The score's parts in plain fp32 arithmetic (exp, and a correctly rounded reciprocal): the same bits as those operations
+// give anywhere, so that biased scores rank alike
+__device__ __forceinline__ float sigmoid_f(float l) { return __frcp_rn(1.f + expf(-l)); }
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int j = 0; j < NE; ++j) s[j] = 1.f / (1.f + expf(-l[j]));
-    return 1.f;
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+  if constexpr (L == 32) {
+    return __reduce_max_sync(0xffffffffu, v);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
   }
+}
+// lowest lane of the group of L lanes (counted in the group) for which p holds, 32 or more if none
+template <int L>
+__device__ __forceinline__ int lanes_first(bool p, int base) {
+  unsigned b = __ballot_sync(0xffffffffu, p) >> base;
+  if constexpr (L < 32) b &= (1u << L) - 1u;
+  return b ? __ffs(b) - 1 : 32;
+}
+
+template <typename T, int L, int NE>
+__global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) {
+  constexpr int TPW = 32 / L;                     // tokens per warp
+  extern __shared__ unsigned char sm_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (L - 1), base = lane & ~(L - 1);
+  int* chosen = reinterpret_cast<int*>(sm_raw) + (warp * TPW + lane / L) * a.k;            // [k] of this token
+  float* val = reinterpret_cast<float*>(sm_raw) + RT_WARPS * TPW * a.k + (warp * TPW + lane / L) * a.e;  // [E]
+  const int c = a.c, i0 = sub * c;
+  const int n = i0 >= a.e ? 0 : a.e - i0 < c ? a.e - i0 : c;                               // experts of this lane
+  const int per = a.e / a.groups;
+  // a group's experts lie in the registers of a power of two of lanes: its best two by shuffles, else through `val`
+  const int span = a.groups > 1 && per % c == 0 && ((per / c) & (per / c - 1)) == 0 ? per / c : 0;
+  float b[NE];
+  if (a.bias)
+#pragma unroll
+    for (int j = 0; j < NE; ++j) b[j] = j < n ? a.bias[i0 + j] : 0.f;
+  const int64_t step = (int64_t)gridDim.x * RT_WARPS * TPW;
+  // every lane of a warp runs the same number of passes (the collectives are warp-wide)
+  for (int64_t r0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * TPW; r0 < a.t; r0 += step) {
+    const int64_t row = r0 + lane / L;
+    const bool live = row < a.t;
+    const T* p = (const T*)a.logits + (live ? row : 0) * a.ldl;
+    float l[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) l[j] = -INFINITY;
+    if (a.vec) {
+      constexpr int V = kVec<T>;
+#pragma unroll
+      for (int j = 0; j + V <= NE; j += V)
+        if (live && j < n) {
+          float f[V];
+          load_v<T, V>(p + i0 + j, f);
+#pragma unroll
+          for (int q = 0; q < V; ++q) l[j + q] = f[q];
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (live && j < n) l[j] = to_f(p[i0 + j]);
+    }
+    unsigned key[NE];
+    float m = 0.f, sum = 1.f;
+    if (!a.all) {
+#pragma unroll
+      for (int j = 0; j < NE; ++j) key[j] = order_key(l[j]);
+    } else {
+      float s[NE];
+      if (a.softmax) {
+        m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) m = fmaxf(m, l[j]);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m == -INFINITY) m = 0.f;
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          s[j] = expf(l[j] - m);
+          sum += s[j];
+        }
+        sum = lanes_sum<L>(sum);
+        if (a.bias)
+#pragma unroll
+          for (int j = 0; j < NE; ++j) s[j] = s[j] / sum;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NE; ++j) s[j] = sigmoid_f(l[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < NE; ++j) {
+        if (a.bias) s[j] += b[j];
+        if (l[j] == -INFINITY) s[j] = -INFINITY;  // closed
+        key[j] = order_key(a.bias ? s[j] : l[j]);
+      }
+      if (a.groups > 1) {
+        unsigned open = 0u;                       // bit g: group g stays open (up to 32 groups)
+        if (span) {
+          float m1 = -INFINITY, m2 = -INFINITY;
+          bool nan = false;
+#pragma unroll
+          for (int j = 0; j < NE; ++j) {
+            nan |= s[j] != s[j];
+            m2 = fmaxf(m2, fminf(m1, s[j]));
+            m1 = fmaxf(m1, s[j]);
+          }
+          for (int o = 1; o < span; o <<= 1) {
+            const float o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
+            m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+            m1 = fmaxf(m1, o1);
+            nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+          }
+          unsigned gk = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
+          if (n == 0) gk = 0u;
+          const int mine = sub / span;
+          for (int q = 0; q < a.top_groups; ++q) {
+            const unsigned best = lanes_max<L>(gk);
+            const int g = lanes_first<L>(gk == best, base) / span;
+            if (best == 0u) continue;             // nothing open is left for this token
+            open |= 1u << g;
+            if (g == mine) gk = 0u;
+          }
+          if (!((open >> mine) & 1u))
+#pragma unroll
+            for (int j = 0; j < NE; ++j) key[j] = 0u;
+        } else {
+#pragma unroll
+          for (int j = 0; j < NE; ++j)
+            if (j < n) val[i0 + j] = s[j];
+          __syncwarp();
+          // lane q of the token's L lanes values the groups q, q + L, ..; their keys replace the first E / per values
+          unsigned gk[32 / L > 8 ? 8 : 32 / L];
+          constexpr int GL = 32 / L > 8 ? 8 : 32 / L;
+#pragma unroll
+          for (int u = 0; u < GL; ++u) {
+            const int g = sub + u * L;
+            gk[u] = 0u;
+            if (g < a.groups) {
+              float m1 = -INFINITY, m2 = -INFINITY;
+              bool nan = false;
+              for (int i = 0; i < per; ++i) {
+                const float f = val[g * per + i];
+                nan |= f != f;
+                m2 = fmaxf(m2, fminf(m1, f));
+                m1 = fmaxf(m1, f);
+              }
+              gk[u] = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
+            }
+          }
+          __syncwarp();
+          for (int q = 0; q < a.top_groups; ++q) {
+            unsigned mx = 0u;
+#pragma unroll
+            for (int u = 0; u < GL; ++u) mx = max(mx, gk[u]);
+            const unsigned best = lanes_max<L>(mx);
+            // the lowest group index that has it: groups of the lower u come first
+            int g = 64;
+#pragma unroll
+            for (int u = GL - 1; u >= 0; --u) {
+              const int f = lanes_first<L>(gk[u] == best, base);
+              if (f < 32) g = f + u * L;
+            }
+            if (best == 0u) continue;
+            open |= 1u << g;
+#pragma unroll
+            for (int u = 0; u < GL; ++u)
+              if (g == sub + u * L) gk[u] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < NE; ++j)
+            if (j < n && !((open >> ((i0 + j) / per)) & 1u)) key[j] = 0u;
+        }
+      }
+    }
+    for (int q = 0; q < a.k; ++q) {
+      unsigned mx = 0u;
+      int at = 0;
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (key[j] > mx) mx = key[j], at = j;
+      const unsigned best = lanes_max<L>(mx);
+      const int first = lanes_first<L>(mx == best, base);
+      if (sub == first) {
+        chosen[q] = best ? i0 + at : -1;
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+          if (j == at) key[j] = 0u;
+      }
+    }
+    __syncwarp();
+    // weights: the chosen logits once more, L slots at a time
+    if (!a.all && a.softmax) {                    // only the chosen ones count: relative to the best of them
+      const int i = chosen[0];
+      m = live && i >= 0 ? to_f(p[i]) : 0.f;
+    }
+    float tot = 0.f;
+    for (int q = sub; q < a.k; q += L) {
+      const int i = chosen[q];
+      if (live && i >= 0) {
+        const float v = to_f(p[i]);
+        tot += a.softmax ? expf(v - m) : sigmoid_f(v);
+      }
+    }
+    tot = a.renorm ? lanes_sum<L>(tot) : sum;
+    if (live)
+      for (int q = sub; q < a.k; q += L) {
+        const int i = chosen[q];
+        float w = 0.f;
+        if (i >= 0 && (tot > 0.f || tot != tot)) {
+          const float v = to_f(p[i]);
+          w = a.scale * ((a.softmax ? expf(v - m) : sigmoid_f(v)) / tot);
+        }
+        a.w[row * a.k + q] = w;
+        a.idx[row * a.k + q] = i;
+      }
+    __syncwarp();
+  }
+}
+
+// Scores of one token's experts, one warp per token (lane holds i = lane + 32 j): softmax numerators and their sum
+template <int NE>
+__device__ __forceinline__ float route_scores(const float (&l)[NE], float (&s)[NE]) {
   float m = -INFINITY;
 #pragma unroll
   for (int j = 0; j < NE; ++j) m = fmaxf(m, l[j]);
@@ -60,6 +287,63 @@ __device__ __forceinline__ float route_scores(const float (&l)[NE], int softmax,
   return warp_sum(sum);
 }
 
+// Gradient of weights that depend on the chosen logits alone: slots in lanes, K2 >= k lanes per token, `tpw` tokens per
+// warp.  The tile of dense rows is built in shared memory.
+template <typename T, int K2>
+__global__ void __launch_bounds__(32 * RT_WARPS) k_route_bwd_sparse(const RouteArgs a, int tpw, int tile_bytes) {
+  extern __shared__ __align__(16) unsigned char sm_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = lane / K2, q = lane & (K2 - 1);
+  T* tile = reinterpret_cast<T*>(sm_raw + (int64_t)warp * tile_bytes);
+  const int64_t step = (int64_t)gridDim.x * RT_WARPS * tpw;
+  for (int64_t r0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * tpw; r0 < a.t; r0 += step) {
+    const int rows = a.t - r0 < tpw ? (int)(a.t - r0) : tpw;
+    const int64_t row = r0 + tok;
+    int i = -1;
+    float dw = 0.f, l = -INFINITY;
+    if (tok < rows && q < a.k) {
+      i = a.cidx[row * a.k + q];
+      if (i < 0 || i >= a.e) i = -1;
+      if (i >= 0) {
+        dw = a.scale * a.dw[row * a.k + q];
+        l = to_f(((const T*)a.logits)[row * a.ldl + i]);
+      }
+    }
+    for (int o = lane * 16; o < tile_bytes; o += 512)
+      *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(tile) + o) = make_uint4(0u, 0u, 0u, 0u);
+    float sc;
+    if (a.softmax) {
+      float m = l;
+#pragma unroll
+      for (int o = K2 / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      sc = i >= 0 ? expf(l - (m == -INFINITY ? 0.f : m)) : 0.f;
+    } else {
+      sc = i >= 0 ? sigmoid_f(l) : 0.f;
+    }
+    float up;
+    if (a.renorm) {
+      const float tot = lanes_sum<K2>(sc);
+      const float w = tot > 0.f || tot != tot ? sc / tot : 0.f;
+      up = w * (dw - lanes_sum<K2>(dw * w));
+    } else {
+      up = dw * sc;
+    }
+    if (!a.softmax) up *= 1.f - sc;
+    __syncwarp();
+    if (i >= 0) tile[tok * a.e + i] = from_f<T>(up);
+    __syncwarp();
+    T* dl = (T*)a.dl + r0 * a.e;
+    const int total = rows * a.e;
+    if ((reinterpret_cast<uintptr_t>(dl) & 15) == 0) {
+      const int nv = total / kVec<T>;
+      for (int o = lane; o < nv; o += 32) reinterpret_cast<uint4*>(dl)[o] = reinterpret_cast<const uint4*>(tile)[o];
+      for (int o = nv * kVec<T> + lane; o < total; o += 32) dl[o] = tile[o];
+    } else {
+      for (int o = lane; o < total; o += 32) dl[o] = tile[o];
+    }
+    __syncwarp();
+  }
+}
+
 template <typename T, int NE>
 __device__ __forceinline__ void route_load(const RouteArgs& a, int64_t row, int lane, float (&l)[NE]) {
   const T* p = (const T*)a.logits + row * a.ldl;
@@ -70,154 +354,110 @@ __device__ __forceinline__ void route_load(const RouteArgs& a, int64_t row, int 
   }
 }
 
-template <typename T, int NE>
-__global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) {
-  extern __shared__ float sm[];                   // groups > 1: [RT_WARPS][32 NE] ranking values
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t row = (int64_t)blockIdx.x * RT_WARPS + warp; row < a.t; row += (int64_t)gridDim.x * RT_WARPS) {
-    float l[NE], s[NE];
-    route_load<T, NE>(a, row, lane, l);
-    const float sum = route_scores<NE>(l, a.softmax, s);
-    unsigned key[NE];
-    float rank[NE];
-#pragma unroll
-    for (int j = 0; j < NE; ++j) {
-      const int i = lane + 32 * j;
-      rank[j] = s[j];
-      if (a.bias && i < a.e) rank[j] = (a.softmax ? s[j] / sum : s[j]) + a.bias[i];
-      key[j] = l[j] == -INFINITY ? 0u : order_key(a.bias ? rank[j] : l[j]);
-    }
-    if (a.groups > 1) {
-      float* v = sm + warp * 32 * NE;
-#pragma unroll
-      for (int j = 0; j < NE; ++j) v[lane + 32 * j] = l[j] == -INFINITY ? -INFINITY : rank[j];
-      __syncwarp();
-      const int per = a.e / a.groups;
-      unsigned gk = 0u;                           // lane g: key of group g's value
-      if (lane < a.groups) {
-        float m1 = -INFINITY, m2 = -INFINITY;
-        bool nan = false;
-        for (int i = 0; i < per; ++i) {
-          const float f = v[lane * per + i];
-          nan |= f != f;
-          m2 = fmaxf(m2, fminf(m1, f));
-          m1 = fmaxf(m1, f);
-        }
-        if (nan)
-          gk = 0xFFFFFFFFu;
-        else if (m1 > -INFINITY)
-          gk = order_key(m2 > -INFINITY ? m1 + m2 : m1);
-      }
-      __syncwarp();
-      unsigned open = 0u;                         // bit g: group g stays open
-      for (int q = 0; q < a.top_groups; ++q) {
-        const unsigned best = __reduce_max_sync(0xffffffffu, gk);
-        if (best == 0u) break;
-        const int g = __ffs(__ballot_sync(0xffffffffu, gk == best)) - 1;
-        open |= 1u << g;
-        if (lane == g) gk = 0u;
-      }
-#pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (lane + 32 * j < a.e && !((open >> ((lane + 32 * j) / per)) & 1u)) key[j] = 0u;
-    }
-    float mine = 0.f;                             // lane q: score and expert of slot q
-    int expert = -1;
-    for (int q = 0; q < a.k; ++q) {
-      unsigned b = 0u;
-      int at = 0;
-      float sc = 0.f;
-#pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (key[j] > b) b = key[j], at = j, sc = s[j];
-      const unsigned best = __reduce_max_sync(0xffffffffu, b);
-      if (best == 0u) break;
-      const unsigned i = __reduce_min_sync(0xffffffffu, b == best ? (unsigned)(lane + 32 * at) : 0xFFFFFFFFu);
-      sc = __shfl_sync(0xffffffffu, sc, i & 31);
-      if (lane == q) mine = sc, expert = (int)i;
-      if (lane == (int)(i & 31))
-#pragma unroll
-        for (int j = 0; j < NE; ++j)
-          if (j == at) key[j] = 0u;
-    }
-    const float tot = a.renorm ? warp_sum(mine) : sum;
-    if (lane < a.k) {
-      a.w[row * a.k + lane] = tot > 0.f || tot != tot ? a.scale * (mine / tot) : 0.f;
-      a.idx[row * a.k + lane] = expert;
-    }
-  }
-}
-
+// Gradient of plain softmax weights (not renormalised), one warp per token: dl_i = s_i (ds_i - sum_j s_j ds_j)
 template <typename T, int NE>
 __global__ void __launch_bounds__(32 * RT_WARPS) k_route_bwd(const RouteArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t row = (int64_t)blockIdx.x * RT_WARPS + warp; row < a.t; row += (int64_t)gridDim.x * RT_WARPS) {
     float l[NE], s[NE];
     route_load<T, NE>(a, row, lane, l);
-    const float sum = route_scores<NE>(l, a.softmax, s);
+    const float sum = route_scores<NE>(l, s);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const int mine = lane < a.k ? a.cidx[row * a.k + lane] : -1;
     const float dw = lane < a.k && mine >= 0 ? a.scale * a.dw[row * a.k + lane] : 0.f;
-    // scores of the chosen experts, one slot per lane
-    float sc = 0.f;
+    float out[NE], all = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      s[j] *= inv;
+      out[j] = 0.f;
+    }
     for (int q = 0; q < a.k; ++q) {
       const int i = __shfl_sync(0xffffffffu, mine, q);
-      if (i < 0 || i >= a.e) continue;
-      float got = 0.f;
+      const float v = __shfl_sync(0xffffffffu, dw, q);
 #pragma unroll
       for (int j = 0; j < NE; ++j)
-        if (j == (i >> 5)) got = s[j];
-      got = __shfl_sync(0xffffffffu, got, i & 31);
-      if (lane == q) sc = got;
+        if (i == lane + 32 * j) out[j] = s[j] * v, all += out[j];
     }
-    // up = s_j ds_j for the chosen slot of this lane
-    float up;
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    if (a.renorm) {
-      const float tot = warp_sum(sc);
-      const float q = tot > 0.f || tot != tot ? sc / tot : 0.f;
-      up = q * (dw - warp_sum(dw * q));
-    } else {
-      up = dw * (sc * inv);
-    }
-    if (!a.softmax) up *= 1.f - sc;
-    // renormalised softmax weights do not depend on the other experts: sum_j s_j ds_j = 0
-    const float all = a.softmax && !a.renorm ? warp_sum(up) * inv : 0.f;
-    float out[NE];
-#pragma unroll
-    for (int j = 0; j < NE; ++j) out[j] = -s[j] * all;
-    for (int q = 0; q < a.k; ++q) {
-      const int i = __shfl_sync(0xffffffffu, mine, q);
-      const float v = __shfl_sync(0xffffffffu, up, q);
-#pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (i == lane + 32 * j) out[j] += v;
-    }
+    all = warp_sum(all);
     T* dl = (T*)a.dl + row * a.e;
 #pragma unroll
     for (int j = 0; j < NE; ++j)
-      if (lane + 32 * j < a.e) dl[lane + 32 * j] = from_f<T>(out[j]);
+      if (lane + 32 * j < a.e) dl[lane + 32 * j] = from_f<T>(out[j] - s[j] * all);
   }
+}
+
+static unsigned route_grid(int64_t tokens, int per_block, int blocks_per_sm) {
+  const int64_t want = (tokens + per_block - 1) / per_block, most = (int64_t)blocks_per_sm * sm_count();
+  return (unsigned)(want < most ? want : most);
 }
 
 template <typename T, int NE>
-static int route_launch(const RouteArgs& a, bool bwd, cudaStream_t st) {
-  const int64_t want = (a.t + RT_WARPS - 1) / RT_WARPS, most = (int64_t)16 * sm_count();
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  if (bwd) {
-    k_route_bwd<T, NE><<<grid, 32 * RT_WARPS, 0, st>>>(a);
-    return check_launch("route_bwd");
-  }
-  k_route_fwd<T, NE><<<grid, 32 * RT_WARPS, a.groups > 1 ? RT_WARPS * 32 * NE * 4 : 0, st>>>(a);
-  return check_launch("route_fwd");
+static int route_bwd_dense(const RouteArgs& a, cudaStream_t st) {
+  k_route_bwd<T, NE><<<route_grid(a.t, RT_WARPS, 16), 32 * RT_WARPS, 0, st>>>(a);
+  return check_launch("route_bwd");
+}
+
+template <typename T, int K2>
+static int route_bwd_sparse(const RouteArgs& a, cudaStream_t st) {
+  // tokens per warp: as many as there are lanes for, within 4 KB of rows
+  const int row = a.e * (int)sizeof(T);
+  int tpw = 32 / K2;
+  while (tpw > 1 && tpw * row > 4096) tpw /= 2;
+  const int tile = (tpw * row + 15) / 16 * 16;
+  k_route_bwd_sparse<T, K2><<<route_grid(a.t, RT_WARPS * tpw, 8), 32 * RT_WARPS, RT_WARPS * tile, st>>>(a, tpw, tile);
+  return check_launch("route_bwd");
 }
 
 template <typename T>
-static int route_any(const RouteArgs& a, bool bwd, cudaStream_t st) {
-  if (a.e <= 32) return route_launch<T, 1>(a, bwd, st);
-  if (a.e <= 64) return route_launch<T, 2>(a, bwd, st);
-  if (a.e <= 128) return route_launch<T, 4>(a, bwd, st);
-  if (a.e <= 256) return route_launch<T, 8>(a, bwd, st);
-  return route_launch<T, 16>(a, bwd, st);
+static int route_bwd_any(const RouteArgs& a, cudaStream_t st) {
+  if (!a.softmax || a.renorm) {
+    if (a.k == 1) return route_bwd_sparse<T, 1>(a, st);
+    if (a.k <= 2) return route_bwd_sparse<T, 2>(a, st);
+    if (a.k <= 4) return route_bwd_sparse<T, 4>(a, st);
+    if (a.k <= 8) return route_bwd_sparse<T, 8>(a, st);
+    if (a.k <= 16) return route_bwd_sparse<T, 16>(a, st);
+    return route_bwd_sparse<T, 32>(a, st);
+  }
+  if (a.e <= 32) return route_bwd_dense<T, 1>(a, st);
+  if (a.e <= 64) return route_bwd_dense<T, 2>(a, st);
+  if (a.e <= 128) return route_bwd_dense<T, 4>(a, st);
+  if (a.e <= 256) return route_bwd_dense<T, 8>(a, st);
+  return route_bwd_dense<T, 16>(a, st);
+}
+
+template <typename T, int L, int NE>
+static int route_fwd_launch(RouteArgs a, int c, cudaStream_t st) {
+  constexpr int TPW = 32 / L, V = kVec<T>;
+  a.c = c;
+  a.vec = c % V == 0 && a.e % V == 0 && a.ldl % V == 0 && aligned16(a.logits);
+  // the values pass through shared memory when a group is not a power of two of lanes
+  const int per = a.e / a.groups, m = per % c == 0 ? per / c : 0;
+  const bool through = a.groups > 1 && (m == 0 || (m & (m - 1)));
+  const int smem = RT_WARPS * TPW * (a.k + (through ? a.e : 0)) * 4;
+  k_route_fwd<T, L, NE><<<route_grid(a.t, RT_WARPS * TPW, 8), 32 * RT_WARPS, smem, st>>>(a);
+  return check_launch("route_fwd");
+}
+
+// Lanes per token and experts per lane.  Below 8 tokens per scheduler a whole warp takes a token.
+template <typename T>
+static int route_fwd_any(RouteArgs a, cudaStream_t st) {
+  a.all = a.bias || a.groups > 1 || (a.softmax && !a.renorm);
+  const int e = a.e;
+  const bool few = a.t < (int64_t)32 * sm_count();
+  if (few || e > 256) {
+    const int c = (e + 31) / 32;
+    if (c <= 4) return route_fwd_launch<T, 32, 4>(a, c, st);
+    return route_fwd_launch<T, 32, 16>(a, c, st);
+  }
+  // groups of 4, 8 or 16 experts fit a lane
+  const int per = a.groups > 1 ? e / a.groups : 0;
+  if (per == 8 && e > 32 && e <= 64) return route_fwd_launch<T, 8, 8>(a, 8, st);
+  if (e <= 16) return route_fwd_launch<T, 4, 4>(a, 4, st);
+  if (e <= 32) return route_fwd_launch<T, 4, 8>(a, 8, st);
+  if (e <= 64) return route_fwd_launch<T, 4, 16>(a, 16, st);
+  if (e <= 96) return route_fwd_launch<T, 8, 12>(a, 12, st);
+  if (e <= 128) return route_fwd_launch<T, 8, 16>(a, 16, st);
+  return route_fwd_launch<T, 16, 16>(a, 16, st);
 }
 
 static int route_check(const char* who, const RouteArgs& a, int dtype) {
@@ -238,8 +478,9 @@ static int route_check(const char* who, const RouteArgs& a, int dtype) {
 }
 
 static int route_types(const RouteArgs& a, int dtype, bool bwd, cudaStream_t st) {
-  if (dtype == MB_F32) return route_any<float>(a, bwd, st);
-  return dtype == MB_BF16 ? route_any<bf16>(a, bwd, st) : route_any<f16>(a, bwd, st);
+  if (dtype == MB_F32) return bwd ? route_bwd_any<float>(a, st) : route_fwd_any<float>(a, st);
+  if (dtype == MB_BF16) return bwd ? route_bwd_any<bf16>(a, st) : route_fwd_any<bf16>(a, st);
+  return bwd ? route_bwd_any<f16>(a, st) : route_fwd_any<f16>(a, st);
 }
 
 }  // namespace mb
