@@ -60,7 +60,12 @@ __device__ __forceinline__ void xp_segments(const XPlan& p, int32_t* plan, const
   __syncthreads();
   for (int e = threadIdx.x; e <= p.E; e += blockDim.x) {
     plan[p.o_seg + e] = seg[e];
-    if (e < p.E) plan[p.o_cnt + e] = cnt[e];
+    if (e < p.E) {
+      plan[p.o_cnt + e] = cnt[e];
+      int rank = 0;
+      for (int i = 0; i < p.E; ++i) rank += cnt[i] > cnt[e] || (cnt[i] == cnt[e] && i < e);
+      plan[p.o_order + rank] = e;
+    }
   }
   const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   for (int e = threadIdx.x >> 5; e < p.E; e += nw) {
@@ -257,39 +262,64 @@ __global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_
     }
     return;
   }
-  for (int64_t row = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * rpw + lane / lpr; row < rows;
-       row += step) {
-    const int64_t slot = m.kind == MOVE_GATHER ? (int64_t)plan[p.o_row + row] : row;
-    const T* s = (const T*)m.src + (slot < 0 ? 0 : slot / m.kdiv) * m.lds;
+  const bool gather = m.kind == MOVE_GATHER;
+  const int32_t* row_slot = plan + p.o_row;
+  int64_t row = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * rpw + lane / lpr;
+  int next = gather && row < rows ? row_slot[row] : 0;
+  for (; row < rows; row += step) {
+    const int64_t slot = gather ? (int64_t)next : row;
+    if (gather && row + step < rows) next = row_slot[row + step];   // in flight while this row is copied
+    const T* s = (const T*)m.src + (slot < 0 ? 0 : gather ? (int)slot / m.kdiv : slot) * m.lds;
     const float g = m.scale && slot >= 0 ? m.scale[slot] : 1.f;
-    uint16_t* out = (uint16_t*)m.out;
-    for (int c0 = sub * 8; c0 < m.dp; c0 += 32 * lpr) {
-      float f[4][8];
+    uint16_t* out = (uint16_t*)m.out + row * m.dp;
+    if (sizeof(T) == 2 && m.vec) {
+      for (int c0 = sub * 8; c0 < m.dp; c0 += 32 * lpr) {
+        uint4 u[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = c0 + u * 8 * lpr;
-        if (slot >= 0 && c < m.dp) {
-          load8(s, c, m.d, m.vec != 0, f[u]);
-        } else {
+        for (int q = 0; q < 4; ++q) {
+          const int c = c0 + q * 8 * lpr;
+          u[q] = make_uint4(0u, 0u, 0u, 0u);
+          if (slot >= 0 && c + 8 <= m.d) u[q] = *reinterpret_cast<const uint4*>(s + c);
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+        for (int q = 0; q < 4; ++q) {
+          const int c = c0 + q * 8 * lpr;
+          if (slot >= 0 && c < m.d && c + 8 > m.d) {       // the ragged end of a row
+            float f[8];
+            load8(s, c, m.d, false, f);
+            if constexpr (sizeof(T) == 2) u[q] = pack16<T>(f);
+          }
+          if constexpr (sizeof(T) == 2)
+            if (m.scale) {
+              float f[8];
+              unpack16(u[q], f, T());
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] *= g;
+              u[q] = pack16<T>(f);
+            }
+          if (c < m.dp) *reinterpret_cast<uint4*>(out + c) = u[q];
         }
       }
+    } else {
+      for (int c = sub * 8; c < m.dp; c += 8 * lpr) {
+        float f[8];
+        if (slot >= 0) {
+          load8(s, c, m.d, m.vec != 0, f);
+        } else {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = c0 + u * 8 * lpr;
-        if (c >= m.dp) break;
+          for (int i = 0; i < 8; ++i) f[i] = 0.f;
+        }
         if (m.scale)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[u][i] *= g;
-        store_planes<T>(out, m.plane, row * m.dp + c, f[u]);
+          for (int i = 0; i < 8; ++i) f[i] *= g;
+        store_planes<T>(out, m.plane, c, f);
       }
     }
   }
 }
 
 // Blocks [0, sum_blocks): out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an
-// expert; a thread adds one V-element piece of a token's rows, four loads in flight; ldb is padded to whole vectors.
+// expert; a thread adds one vector of a token's rows, four loads in flight; ldb is padded to whole vectors.
 // The other blocks: dg[slot] = sum of its nparts partial products (0 without an expert).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
@@ -302,6 +332,27 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
       if (slot_row[s] >= 0)
         for (int q = 0; q < nparts; ++q) v += dgpart[q * R + s];
       dg[s] = v;
+    }
+    return;
+  }
+  if constexpr (V == 1) {                        // odd widths: a warp per token, four columns a lane in flight
+    const int lane = threadIdx.x & 31;
+    for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)sum_blocks * 8) {
+      const unsigned have = __ballot_sync(0xffffffffu, lane < k && slot_row[t * k + (lane < k ? lane : 0)] >= 0);
+      for (int c0 = lane; c0 < d; c0 += 128) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) {
+          const bool ok = j < 32 ? (have >> j) & 1u : slot_row[t * k + j] >= 0;
+          const T* p = buf + (t * k + j) * ldb;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (ok && c0 + 32 * q < d) s[q] += to_f(p[c0 + 32 * q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (c0 + 32 * q < d) out[t * d + c0 + 32 * q] = from_f<T>(s[q]);
+      }
     }
     return;
   }
@@ -334,12 +385,25 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
   }
 }
 
-// dw = sum over the `parts` partial sums (in their order) of a product whose rows were split
+// dw = sum over the `parts` partial sums (in their order) of a product whose rows were split; n4 = whole float4s (n / 4
+// where every part starts on 16 bytes, else 0)
 template <typename T>
-__global__ void __launch_bounds__(256) k_parts_sum(const float* part, int parts, int64_t n, T* out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
+__global__ void __launch_bounds__(256) k_parts_sum(const float* part, int parts, int64_t n, int64_t n4, T* out) {
+  const int64_t step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = i0; i < n4; i += step) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
+    for (int q = 0; q < parts; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(part + q * n + 4 * i);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(out + 4 * i) = s;
+    else
+      *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+  }
+  for (int64_t i = 4 * n4 + i0; i < n; i += step) {
+    float s = 0.f;
     for (int q = 0; q < parts; ++q) s += part[q * n + i];
     out[i] = from_f<T>(s);
   }
@@ -536,7 +600,7 @@ static int x_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, 
                       const float* dgpart, int nparts, float* dg, cudaStream_t st) {
   constexpr int V = kVec<T>;
   const bool vec = d % V == 0 && aligned16(out);
-  const unsigned nb = buf ? x_grid((tokens * (vec ? d / V : d) + 255) / 256) : 0;
+  const unsigned nb = buf ? x_grid(vec ? (tokens * (d / V) + 255) / 256 : (tokens + 7) / 8) : 0;
   const unsigned ng = dg ? x_grid((tokens * k + 255) / 256) : 0;
   if (vec)
     k_rows_sum<T, V><<<nb + ng, 256, 0, st>>>(buf, ldb, out, tokens, k, d, slot_row, nb, dgpart, nparts, dg);
@@ -719,7 +783,9 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
       if (int rc = xgemm_launch(g, st)) return rc;
       if (b.split > 1) {
         const int64_t n = (int64_t)E * O * D;
-        k_parts_sum<T><<<x_grid((n + 255) / 256), 256, 0, st>>>((const float*)(base + b.parts), b.split, n, (T*)dw);
+        const int64_t n4 = n % 4 == 0 && aligned16(dw) ? n / 4 : 0;
+        k_parts_sum<T><<<x_grid(((n4 ? n4 : n) + 255) / 256), 256, 0, st>>>((const float*)(base + b.parts), b.split, n, n4,
+                                                                            (T*)dw);
         if (int rc = check_launch("expert_linear (parts)")) return rc;
       }
     }

@@ -14,7 +14,7 @@ struct XPlan {
   int64_t R;
   int32_t E, nblk;
   int64_t tiles;                                 // most tiles there can be
-  int64_t o_seg, o_cnt, o_tile, o_row, o_slot, o_hist, words;
+  int64_t o_seg, o_cnt, o_order, o_tile, o_row, o_slot, o_hist, words;
 };
 // header words: 0 = tiles in use, 1 = status bits
 inline XPlan xplan(int64_t R, int32_t E) {
@@ -25,7 +25,8 @@ inline XPlan xplan(int64_t R, int32_t E) {
   p.tiles = R / XP_BM + (R < E ? R : E);
   p.o_seg = 8;                                   // [E + 1] first row of each expert
   p.o_cnt = p.o_seg + E + 1;                     // [E] slots of each expert
-  p.o_tile = p.o_cnt + E;                        // [tiles] expert of each tile
+  p.o_order = p.o_cnt + E;                       // [E] experts, most slots first (ties: lowest index)
+  p.o_tile = p.o_order + E;                      // [tiles] expert of each tile
   p.o_row = p.o_tile + p.tiles;                  // [tiles * XP_BM] slot of each row, -1 = padding
   p.o_slot = p.o_row + p.tiles * XP_BM;          // [R] row of each slot, -1 = no expert
   p.o_hist = p.o_slot + R;                       // [E][nblk] scratch

@@ -21,12 +21,13 @@ namespace mb {
 constexpr int XG_BM = XP_BM, XG_BK = 64, XG_THREADS = 192;
 constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
 
+constexpr int XG_STG = 4096;                     // row staging of one epilogue warp
 template <int BN>
 struct XgCfg {
   static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN * XG_BK * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 196608 / STAGE;              // 192 KB ring: 4 stages at BN = 256, 6 at 128
   static constexpr int TMEM = 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE + 256 + 1024;   // + barriers, alignment slack
+  static constexpr int SMEM = STAGES * STAGE + 4 * XG_STG + 256 + 1024;   // + row staging, barriers, alignment slack
 };
 
 struct XgParams {
@@ -55,23 +56,10 @@ struct XgBars {
 __device__ __forceinline__ int xg_plane_a(int p) { return (0x021010 >> (4 * (5 - p))) & 0xF; }
 __device__ __forceinline__ int xg_plane_b(int p) { return (0x201100 >> (4 * (5 - p))) & 0xF; }
 
-// Writes up to 32 consecutive values of one row (16-byte stores when the row pointer allows them)
-template <typename T>
-__device__ __forceinline__ void xg_store32(T* dst, const float (&f)[32], int n, bool vec) {
-  constexpr int V = kVec<T>;
-  if (vec && n >= 32) {
-#pragma unroll
-    for (int q = 0; q < 32 / V; ++q) {
-      float t[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) t[i] = f[q * V + i];
-      *reinterpret_cast<uint4*>(dst + q * V) = pack16<T>(t);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) dst[i] = from_f<T>(f[i]);
-  }
+// Row staging of the epilogue: a warp's 32 rows x 128 bytes, 16-byte piece c of row r at piece c ^ (r % 8), so that a lane's
+// access to its own row and the warp's access to four whole row segments are both free of bank conflicts.
+__device__ __forceinline__ uint4* xg_stg(unsigned char* stg, int row, int c) {
+  return reinterpret_cast<uint4*>(stg + row * 128 + ((c ^ (row & 7)) << 4));
 }
 
 // OUT: element type of the output (T, or float for partial sums)
@@ -82,7 +70,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   constexpr bool A_MN = MODE == XG_WGRAD, B_MN = MODE != XG_FWD;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  XgBars& B = *reinterpret_cast<XgBars*>(smem + C::STAGES * C::STAGE);
+  XgBars& B = *reinterpret_cast<XgBars*>(smem + C::STAGES * C::STAGE + 4 * XG_STG);
   volatile int* failed = &B.failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -111,6 +99,13 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   const int32_t* plan = g.plan;
   const int tiles = MODE == XG_WGRAD ? g.split * g.E * g.tm * g.tn : plan[0] * g.tn;
 
+  // This CTA's n-th tile.  WGRAD: experts come longest first and odd rounds run backwards over the CTAs, so that every CTA
+  // gets about the same number of K blocks.
+  auto tile_at = [&](int n) {
+    const int t = n * gridDim.x + (MODE == XG_WGRAD && (n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    return t;
+  };
+  const int rounds = (tiles + gridDim.x - 1) / gridDim.x;
   // tile -> (expert, first row of A / first output row, first column, K blocks)
   struct Tile {
     int e, m0, n0, r0, nk, se;
@@ -120,10 +115,10 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     const int m = t / g.tn;
     o.n0 = (t - m * g.tn) * BN;
     if constexpr (MODE == XG_WGRAD) {
-      const int se = m / g.tm, part = se / g.E;
-      o.e = se - part * g.E;
-      o.m0 = (m - se * g.tm) * XG_BM;
-      o.se = se;
+      const int sr = m / g.tm, part = sr / g.E;
+      o.e = plan[g.lay.o_order + sr - part * g.E];
+      o.m0 = (m - sr * g.tm) * XG_BM;
+      o.se = part * g.E + o.e;
       const int nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK;
       const int k0 = (int)((int64_t)nk * part / g.split);
       o.r0 = plan[g.lay.o_seg + o.e] + k0 * XG_BK;
@@ -142,7 +137,9 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     if (lane == 0) {
       int seq = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int r = 0; ok && r < rounds; ++r) {
+        const int t = tile_at(r);
+        if (t >= tiles) break;                     // only in the last round
         const Tile w = tile_of(t);
         for (int p = p0; ok && p < 6; ++p) {
           const int pa = xg_plane_a(p), pb = xg_plane_b(p);
@@ -190,7 +187,9 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       bool ok = true;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int r = 0; ok && r < rounds; ++r) {
+        const int t = tile_at(r);
+        if (t >= tiles) break;
         const Tile w = tile_of(t);
         if (w.nk == 0) continue;
         const int acc = tc & 1;
@@ -232,29 +231,62 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------------------------------ epilogue
+    // One row per lane out of TMEM; rows pass through shared memory in pieces of 128 bytes so that global accesses are
+    // whole 128-byte segments of four rows (one row per lane: 32 scattered 16-byte pieces per access, which held a tile
+    // for longer than its products at K <= 1024).
     const int q4 = warp & 3, row = q4 * 32 + lane;
+    unsigned char* stg = smem + C::STAGES * C::STAGE + (warp - 2) * XG_STG;
+    constexpr int NC = 128 / (int)sizeof(OUT);     // columns of a piece
+    constexpr int XV = kVec<T>;
+    const int r8 = lane >> 3, c8 = lane & 7;       // this lane's row (of four) and 16-byte piece in whole-segment accesses
+    const bool vec = g.ldo % kVec<OUT> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+    const bool xvec = MODE == XG_DGRAD && g.ldx % XV == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
     int tc = 0;
     // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    for (int r = 0; r < rounds; ++r) {
       if (__shfl_sync(0xffffffffu, *failed, 0)) break;
+      const int t = tile_at(r);
+      if (t >= tiles) break;
       const Tile w = tile_of(t);
       OUT* dst = nullptr;
       float sc = 1.f, dot = 0.f;
       const T* xr = nullptr;
       int slot = -1;
       if constexpr (MODE == XG_WGRAD) {
-        if (w.m0 + row < g.M) dst = (OUT*)g.out + ((int64_t)w.se * g.M + w.m0 + row) * g.ldo;
+        if (w.m0 + row < g.M) dst = (OUT*)g.out + ((int64_t)w.se * g.M + w.m0 + row) * g.ldo + w.n0;
       } else {
         slot = plan[g.lay.o_row + w.m0 + row];
         if (slot >= 0) {
-          if (g.out) dst = (OUT*)g.out + (int64_t)slot * g.ldo;
+          if (g.out) dst = (OUT*)g.out + (int64_t)slot * g.ldo + w.n0;
           if (g.scale) sc = g.scale[slot];
-          if (MODE == XG_DGRAD && g.dgpart) xr = (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx;
+          if (MODE == XG_DGRAD && g.dgpart) xr = (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + w.n0;
         }
       }
-      const bool vec = g.ldo % kVec<OUT> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-      const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
-      const int acc = tc & 1;
+      const int acc = tc & 1, nc = g.N - w.n0 < BN ? g.N - w.n0 : BN;
+      // the x rows' pieces for the dot products, loaded one piece ahead (and the first before the wait)
+      uint4 xq[MODE == XG_DGRAD ? 8 : 1];
+      auto fetch_x = [&](int h) {
+        const int n = nc - h * NC < NC ? nc - h * NC : NC;
+#pragma unroll
+        for (int i = 0; i < (MODE == XG_DGRAD ? 8 : 0); ++i) {
+          const T* xp =
+              reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 4 * i + r8));
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (xp) {
+            xp += h * NC + c8 * XV;
+            if (xvec && (c8 + 1) * XV <= n) {
+              v = *reinterpret_cast<const uint4*>(xp);
+            } else {
+              float f[XV];
+#pragma unroll
+              for (int q = 0; q < XV; ++q) f[q] = c8 * XV + q < n ? to_f(xp[q]) : 0.f;
+              v = pack16<T>(f);
+            }
+          }
+          xq[i] = v;
+        }
+      };
+      if (MODE == XG_DGRAD && g.dgpart) fetch_x(0);
       if (w.nk > 0) {
         if (!__all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS))) {
           *failed = 1;
@@ -262,54 +294,71 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
-      const int nc = g.N - w.n0 < BN ? g.N - w.n0 : BN;
 #pragma unroll 1
-      for (int h = 0; h < BN / 32; ++h) {
-        if (32 * h >= nc) break;
-        float f[32];
+      for (int h = 0; h * NC < nc; ++h) {
+        const int n = nc - h * NC < NC ? nc - h * NC : NC;
+        uint32_t u[NC];
         if (w.nk > 0) {
-          uint32_t u[32];
-          tmem_ld32(tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + 32 * h), u);
-          tmem_wait_ld();
+          const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + NC * h);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
+          for (int q = 0; q < NC / 32; ++q) tmem_ld32(ta + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * q));
+          tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = 0.f;
+          for (int i = 0; i < NC; ++i) u[i] = 0u;
         }
-        const int n = nc - 32 * h;
-        if (MODE == XG_DGRAD && xr) {
-          const T* xp = xr + w.n0 + 32 * h;
-          if (xvec && n >= 32) {
-            // one short chain per vector, added up as a tree over the chunk: the rounding of 256 terms in a row shows
-            float part[32 / kVec<T>];
+        if constexpr (MODE == XG_DGRAD) {          // dot += <x row, row> over this piece's columns
+          if (g.dgpart) {
+            // a piece of 128 bytes of x holds as many columns as one of the output: T = OUT here
 #pragma unroll
-            for (int q = 0; q < 32 / kVec<T>; ++q) {
-              float v[kVec<T>];
-              load_v<T, kVec<T>>(xp + q * kVec<T>, v);
-              part[q] = 0.f;
+            for (int i = 0; i < (MODE == XG_DGRAD ? 8 : 0); ++i) *xg_stg(stg, 4 * i + r8, c8) = xq[i];
+            if ((h + 1) * NC < nc) fetch_x(h + 1);
+            __syncwarp();
+            // one short chain per vector, added up as a tree: the rounding of 256 terms in a row would show
+            float part[8];
 #pragma unroll
-              for (int i = 0; i < kVec<T>; ++i) part[q] = fmaf(v[i], f[q * kVec<T> + i], part[q]);
+            for (int c = 0; c < 8; ++c) {
+              float f[XV];
+              unpack16(*xg_stg(stg, lane, c), f, T());
+              part[c] = 0.f;
+#pragma unroll
+              for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], __uint_as_float(u[c * XV + q]), part[c]);
             }
-#pragma unroll
-            for (int w = 16 / kVec<T>; w >= 1; w >>= 1)
-#pragma unroll
-              for (int q = 0; q < w; ++q) part[q] += part[q + w];
-            dot += part[0];
-          } else {
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < n) part = fmaf(to_f(xp[i]), f[i], part);
-            dot += part;
+            dot += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+            __syncwarp();
           }
         }
-        if (dst) {
-          if (MODE != XG_WGRAD) {
+        if (MODE == XG_WGRAD || g.out) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] *= sc;
+          for (int c = 0; c < 8; ++c) {
+            float f[kVec<OUT>];
+#pragma unroll
+            for (int q = 0; q < kVec<OUT>; ++q) {
+              const float v = __uint_as_float(u[c * kVec<OUT> + q]);
+              f[q] = MODE == XG_WGRAD ? v : v * sc;
+            }
+            *xg_stg(stg, lane, c) = pack16<OUT>(f);
           }
-          xg_store32<OUT>(dst + w.n0 + 32 * h, f, n, vec);
+          __syncwarp();
+          if (vec && n == NC) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 4 * i + r8));
+              if (p) *reinterpret_cast<uint4*>(p + h * NC + c8 * kVec<OUT>) = *xg_stg(stg, 4 * i + r8, c8);
+            }
+          } else {                                 // odd strides and the last columns: one row at a time, lanes along it
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+              OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), r));
+#pragma unroll
+              for (int q = 0; q < NC / 32; ++q) {
+                const int c = lane + 32 * q;
+                if (p && c < n)
+                  p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, r, c / kVec<OUT>))[c % kVec<OUT>];
+              }
+            }
+          }
+          __syncwarp();
         }
       }
       if (MODE == XG_DGRAD && xr) g.dgpart[(int64_t)(w.n0 / BN) * g.lay.R + slot] = dot;

@@ -283,7 +283,8 @@ def test_plan_sorts_the_slots(T, k, E):
     assert torch.equal(words[o:o + E + 1].long(), seg)
     assert torch.equal(words[o + E + 1:o + 2 * E + 1].long(), cnt)
     tiles = T * k // 128 + min(T * k, E)
-    o_tile, o_row = o + 2 * E + 1, o + 2 * E + 1 + tiles
+    o_order, o_tile, o_row = o + 2 * E + 1, o + 3 * E + 1, o + 3 * E + 1 + tiles
+    assert words[o_order:o_tile].tolist() == sorted(range(E), key=lambda e: (-int(cnt[e]), e))
     rows = words[o_row:o_row + int(seg[-1])].long()
     want = torch.full((int(seg[-1]),), -1, dtype=torch.int64)
     flat = ex.reshape(-1)
