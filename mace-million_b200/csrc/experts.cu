@@ -7,178 +7,283 @@
 // fp32 operands become three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits
 // of mantissa, and bf16 has the exponent range of fp32, so nothing overflows that fp32 holds.
 #include "experts.cuh"
+#include "tc.cuh"
 
 namespace mb {
 
 // ------------------------------------------------------------------------------------------------ plan
-// Stable counting sort of the slots by expert.  count: per-block histograms; scan: rows of each (expert, block);
-// place: rank of a slot among its expert's slots of the block, warp by warp (match_any), so the order is the slots'.
-// Slots with expert -1 get no row; other values outside [0, E) set MB_ST_BAD_EXPERT and get none either.
+// Stable counting sort of the slots by expert.  Every warp counts its run of slots per expert, prefix sums over the warps
+// (and blocks) and over the experts' padded segments give each (warp, expert) its first row, and the warp places its slots
+// in order (ranks inside a warp by ballots): the rows of an expert keep the slots' order, and no result depends on a
+// schedule.  Slots with expert -1 get no row; other values outside [0, E) set MB_ST_BAD_EXPERT and get none either.
+// Up to XP_CLUSTER_SLOTS it is one launch: a cluster of 8 CTAs that exchange their counts through distributed shared
+// memory, one CTA up to 4096 slots; above, three launches over all SMs.  Latency bounds both (B200, one launch / three):
+// 200 slots, 8 experts 5.5 / 7.6 us; 16,384, 89 experts 11.6 / 13.2; 65,536, 16 experts 9.5 / 9.3; 131,072, 16 experts
+// 14.6 / 10.2; 262,144, 64 experts 29 / 15.
 
-__device__ __forceinline__ int xp_expert(const int32_t* experts, int64_t s, int64_t R, int E, bool& bad) {
-  if (s >= R) return -1;
+__device__ __forceinline__ int xp_expert(const int32_t* experts, int64_t s, int64_t end, int E, bool& bad) {
+  if (s >= end) return -1;
   const int e = experts[s];
   bad |= e < -1 || e >= E;
   return e >= 0 && e < E ? e : -1;
 }
 
-__global__ void __launch_bounds__(256) k_plan_count(const int32_t* experts, const XPlan p, int32_t* plan) {
-  extern __shared__ int cnt[];
-  for (int e = threadIdx.x; e < p.E; e += 256) cnt[e] = 0;
-  __syncthreads();
-  bool bad = false;
-  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK;
-  for (int i = threadIdx.x; i < XP_CHUNK; i += 256) {
-    const int e = xp_expert(experts, s0 + i, p.R, p.E, bad);
-    if (e >= 0) atomicAdd(&cnt[e], 1);
+// inclusive sum over the warp's lanes
+__device__ __forceinline__ int warp_prefix(int v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int q = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += q;
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += 256) plan[p.o_hist + (int64_t)e * p.nblk + blockIdx.x] = cnt[e];
+  return v;
 }
 
-// Segments, tiles and padding rows from the counts of all experts (cnt in shared memory; the whole block calls it)
-__device__ __forceinline__ void xp_segments(const XPlan& p, int32_t* plan, const int* cnt, int* seg) {
-  if (threadIdx.x < 32) {
-    int run = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + threadIdx.x;
-      const int rows = e < p.E ? (cnt[e] + XP_BM - 1) / XP_BM * XP_BM : 0;
-      int inc = rows;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((int)threadIdx.x >= o) inc += v;
-      }
-      if (e < p.E) seg[e] = run + inc - rows;
-      run += __shfl_sync(0xffffffffu, inc, 31);
+// seg[e] = first row of expert e, pair[e] = its first pair of tiles, for e <= E, by one warp
+__device__ __forceinline__ void xp_segments(int E, const int* cnt, int* seg, int* pair) {
+  const int lane = threadIdx.x & 31;
+  int run = 0, prun = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    const int tiles = e < E ? (cnt[e] + XP_BM - 1) / XP_BM : 0, pairs = (tiles + 1) / 2;
+    const int inc = warp_prefix(tiles), pinc = warp_prefix(pairs);
+    if (e < E) {
+      seg[e] = (run + inc - tiles) * XP_BM;
+      pair[e] = prun + pinc - pairs;
     }
-    if (threadIdx.x == 0) {
-      seg[p.E] = run;
-      plan[0] = run / XP_BM;
-    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+    prun += __shfl_sync(0xffffffffu, pinc, 31);
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e <= p.E; e += blockDim.x) {
-    plan[p.o_seg + e] = seg[e];
-    if (e < p.E) {
-      plan[p.o_cnt + e] = cnt[e];
-      int rank = 0;
-      for (int i = 0; i < p.E; ++i) rank += cnt[i] > cnt[e] || (cnt[i] == cnt[e] && i < e);
+  if (lane == 0) {
+    seg[E] = run * XP_BM;
+    pair[E] = prun;
+  }
+}
+
+// The plan's tables, by block `b` of `nb` (whole blocks; the experts e = b, b + nb, .. warp by warp)
+__device__ __forceinline__ void xp_tables(const XPlan& p, int32_t* plan, const int* cnt, const int* seg, const int* pair,
+                                          int b, int nb) {
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (b == 0 && threadIdx.x == 0) {
+    plan[0] = seg[p.E] / XP_BM;
+    plan[2] = pair[p.E];
+    plan[p.o_seg + p.E] = seg[p.E];
+  }
+  for (int e = b + nb * (threadIdx.x >> 5); e < p.E; e += nb * nw) {
+    const int c = cnt[e], r0 = seg[e], r1 = seg[e + 1];
+    int rank = 0;                                // experts with more slots, or as many and a lower index
+    for (int i = lane; i < p.E; i += 32) rank += cnt[i] > c || (cnt[i] == c && i < e);
+    rank = __reduce_add_sync(0xffffffffu, rank);
+    if (lane == 0) {
+      plan[p.o_seg + e] = r0;
+      plan[p.o_cnt + e] = c;
       plan[p.o_order + rank] = e;
     }
+    for (int t = r0 / XP_BM + lane; t < r1 / XP_BM; t += 32) plan[p.o_tile + t] = e;
+    for (int i = lane; i < pair[e + 1] - pair[e]; i += 32) plan[p.o_pair + pair[e] + i] = r0 / XP_BM + 2 * i;
+    for (int r = r0 + c + lane; r < r1; r += 32) plan[p.o_row + r] = -1;
   }
-  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  for (int e = threadIdx.x >> 5; e < p.E; e += nw) {
-    for (int r = seg[e] + cnt[e] + lane; r < seg[e + 1]; r += 32) plan[p.o_row + r] = -1;
-    for (int t = seg[e] / XP_BM + lane; t < seg[e + 1] / XP_BM; t += 32) plan[p.o_tile + t] = e;
+}
+
+// Lanes of the warp with the same expert, by one ballot per bit of the index (-1 counts as E); match_any takes a step per
+// distinct value and made the plan of 262,144 slots on 64 experts three times as long
+__device__ __forceinline__ unsigned same_expert(int e, int E) {
+  const int v = e < 0 ? E : e;
+  unsigned m = 0xffffffffu;
+  for (int b = 1; b <= E; b <<= 1) {
+    const unsigned on = __ballot_sync(0xffffffffu, v & b);
+    m &= v & b ? on : ~on;
+  }
+  return m;
+}
+
+// Counts of the slots [s0, end) per expert into mine[E] (zeroed), by one warp; eight loads in flight
+__device__ __forceinline__ void xp_count(const int32_t* experts, int64_t s0, int64_t end, int E, int* mine) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (; s0 < end; s0 += 256) {
+    int ev[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) ev[q] = xp_expert(experts, s0 + 32 * q + lane, end, E, bad);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (ev[q] >= 0) atomicAdd(&mine[ev[q]], 1);
+  }
+}
+
+// Places the slots [s0, end); next[e] = next row of expert e for this warp, advanced here
+__device__ __forceinline__ void xp_place(const int32_t* experts, const XPlan& p, int32_t* plan, int64_t s0, int64_t end,
+                                         int* next) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (; s0 < end; s0 += 256) {
+    int ev[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) ev[q] = xp_expert(experts, s0 + 32 * q + lane, end, p.E, bad);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int64_t s = s0 + 32 * q + lane;
+      const int e = ev[q];
+      const unsigned same = same_expert(e, p.E);
+      const int first = __ffs(same) - 1;
+      int at = 0;
+      if (e >= 0 && lane == first) {
+        at = next[e];
+        next[e] = at + __popc(same);
+      }
+      at = __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1));
+      if (e >= 0) plan[p.o_row + at] = (int)s;
+      if (s < end) plan[p.o_slot + s] = e >= 0 ? at : -1;
+      __syncwarp();
+    }
+  }
+  if (bad) atomicOr((unsigned*)plan + 1, (unsigned)MB_ST_BAD_EXPERT);
+}
+
+// One launch: CL CTAs of 32 warps (a cluster when CL > 1), each warp `per` slots.
+// Shared memory: total[E], seg[E + 1], pair[E + 1], own[E], next[32][E].
+constexpr int64_t XP_CLUSTER_SLOTS = 1 << 16;
+template <int CL>
+__global__ void __launch_bounds__(1024) k_plan_one(const int32_t* experts, const XPlan p, int32_t* plan, int64_t per) {
+  extern __shared__ int sm[];
+  const int E = p.E, tid = threadIdx.x, warp = tid >> 5;
+  int *total = sm, *seg = total + E, *pair = seg + E + 1, *own = pair + E + 1, *next = own + E;
+  const int rank = CL > 1 ? (int)cluster_ctarank() : 0;
+  for (int i = tid; i < 32 * E; i += 1024) next[i] = 0;
+  if (rank == 0 && tid == 0) plan[1] = 0;        // status: set below, after the first barrier
+  __syncthreads();
+  const int64_t s0 = ((int64_t)rank * 32 + warp) * per;
+  const int64_t end = s0 + per < p.R ? s0 + per : p.R;
+  xp_count(experts, s0, end, E, next + warp * E);
+  __syncthreads();
+  for (int e = tid; e < E; e += 1024) {          // first slot of each warp within the CTA's run of the expert
+    int run = 0;
+#pragma unroll 8
+    for (int w = 0; w < 32; ++w) {
+      const int c = next[w * E + e];
+      next[w * E + e] = run;
+      run += c;
+    }
+    own[e] = run;
+  }
+  if constexpr (CL > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  for (int e = tid; e < E; e += 1024) {
+    int all = 0, before = 0;
+    if constexpr (CL > 1) {
+#pragma unroll
+      for (int q = 0; q < CL; ++q) {
+        const int c = ld_cluster_s32(mapa_u32(smem_u32(own + e), q));
+        before += q < rank ? c : 0;
+        all += c;
+      }
+    } else {
+      all = own[e];
+    }
+    total[e] = all;
+    pair[e] = before;                            // until the segments are known
+  }
+  __syncthreads();
+  for (int i = tid; i < 32 * E; i += 1024) next[i] += pair[i % E];
+  __syncthreads();
+  if (warp == 0) xp_segments(E, total, seg, pair);
+  __syncthreads();
+  for (int i = tid; i < 32 * E; i += 1024) next[i] += seg[i % E];
+  __syncthreads();
+  xp_place(experts, p, plan, s0, end, next + warp * E);
+  xp_tables(p, plan, total, seg, pair, rank, CL);
+  if constexpr (CL > 1) cluster_sync();          // no CTA leaves while another can still read its counts
+}
+
+// Three launches, for more slots: XP_CHUNK slots per block, hist[e][block] in the plan
+__global__ void __launch_bounds__(256) k_plan_count(const int32_t* experts, const XPlan p, int32_t* plan) {
+  extern __shared__ int next[];                  // [8][E]
+  for (int i = threadIdx.x; i < 8 * p.E; i += 256) next[i] = 0;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5;
+  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK + warp * (XP_CHUNK / 8);
+  const int64_t end = s0 + XP_CHUNK / 8 < p.R ? s0 + XP_CHUNK / 8 : p.R;
+  xp_count(experts, s0, end, p.E, next + warp * p.E);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += 256) {
+    int run = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) run += next[w * p.E + e];
+    plan[p.o_hist + (int64_t)e * p.nblk + blockIdx.x] = run;
   }
 }
 
 __global__ void __launch_bounds__(1024) k_plan_scan(const XPlan p, int32_t* plan) {
   extern __shared__ int sm[];
-  int *cnt = sm, *seg = sm + p.E;
+  int *cnt = sm, *seg = cnt + p.E, *pair = seg + p.E + 1;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) plan[1] = 0;
   for (int e = threadIdx.x >> 5; e < p.E; e += 32) {
     int32_t* h = plan + p.o_hist + (int64_t)e * p.nblk;
     int run = 0;
     for (int b0 = 0; b0 < p.nblk; b0 += 32) {
-      const int v = b0 + lane < p.nblk ? h[b0 + lane] : 0;
-      int inc = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int q = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += q;
-      }
+      const int v = b0 + lane < p.nblk ? h[b0 + lane] : 0, inc = warp_prefix(v);
       if (b0 + lane < p.nblk) h[b0 + lane] = run + inc - v;
       run += __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) cnt[e] = run;
   }
   __syncthreads();
-  xp_segments(p, plan, cnt, seg);
-}
-
-// Places the slots [s0, s0 + nw * per) of this block, warp w the w-th `per` of them; base[w][e] = next row of expert e
-// for warp w (shared memory), advanced here.
-__device__ __forceinline__ void xp_place(const int32_t* experts, const XPlan& p, int32_t* plan, int64_t s0, int per,
-                                         int* base) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int* mine = base + warp * p.E;
-  bool bad = false;
-  for (int i = 0; i < per; i += 32) {
-    const int64_t s = s0 + (int64_t)warp * per + i + lane;
-    const int e = xp_expert(experts, s, p.R, p.E, bad);
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    const int first = __ffs(same) - 1;
-    int at = 0;
-    if (e >= 0 && lane == first) {
-      at = mine[e];
-      mine[e] = at + __popc(same);
-    }
-    at = __shfl_sync(0xffffffffu, at, first) + rank;
-    if (e >= 0) plan[p.o_row + at] = (int)s;
-    if (s < p.R) plan[p.o_slot + s] = e >= 0 ? at : -1;
-    __syncwarp();
-  }
-  if (bad) atomicOr((unsigned*)plan + 1, (unsigned)MB_ST_BAD_EXPERT);
-}
-
-// counts per (warp, expert) of the block's slots into base[w][e] (zeroed by the caller)
-__device__ __forceinline__ void xp_warp_counts(const int32_t* experts, const XPlan& p, int64_t s0, int per, int* base) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  bool bad = false;
-  for (int i = 0; i < per; i += 32) {
-    const int e = xp_expert(experts, s0 + (int64_t)warp * per + i + lane, p.R, p.E, bad);
-    if (e >= 0) atomicAdd(&base[warp * p.E + e], 1);
-  }
+  if (threadIdx.x < 32) xp_segments(p.E, cnt, seg, pair);
+  __syncthreads();
+  xp_tables(p, plan, cnt, seg, pair, 0, 1);
 }
 
 __global__ void __launch_bounds__(256) k_plan_place(const int32_t* experts, const XPlan p, int32_t* plan) {
-  extern __shared__ int base[];                  // [8][E]
-  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK;
-  for (int i = threadIdx.x; i < 8 * p.E; i += 256) base[i] = 0;
+  extern __shared__ int next[];                  // [8][E]
+  for (int i = threadIdx.x; i < 8 * p.E; i += 256) next[i] = 0;
   __syncthreads();
-  xp_warp_counts(experts, p, s0, XP_CHUNK / 8, base);
+  const int warp = threadIdx.x >> 5;
+  const int64_t s0 = (int64_t)blockIdx.x * XP_CHUNK + warp * (XP_CHUNK / 8);
+  const int64_t end = s0 + XP_CHUNK / 8 < p.R ? s0 + XP_CHUNK / 8 : p.R;
+  xp_count(experts, s0, end, p.E, next + warp * p.E);
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += 256) {
     int run = plan[p.o_seg + e] + plan[p.o_hist + (int64_t)e * p.nblk + blockIdx.x];
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const int c = base[w * p.E + e];
-      base[w * p.E + e] = run;
+      const int c = next[w * p.E + e];
+      next[w * p.E + e] = run;
       run += c;
     }
   }
   __syncthreads();
-  xp_place(experts, p, plan, s0, XP_CHUNK / 8, base);
+  xp_place(experts, p, plan, s0, end, next + warp * p.E);
 }
 
-// All three steps in one block, for few slots: one launch instead of three
-__global__ void __launch_bounds__(1024) k_plan_one(const int32_t* experts, const XPlan p, int32_t* plan, int per) {
-  extern __shared__ int sm[];
-  int *cnt = sm, *seg = cnt + p.E, *base = seg + p.E + 1;   // base [32][E]
-  for (int i = threadIdx.x; i < 32 * p.E; i += 1024) base[i] = 0;
-  if (threadIdx.x == 0) plan[1] = 0;
-  __syncthreads();
-  xp_warp_counts(experts, p, 0, per, base);
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += 1024) {
-    int run = 0;
-#pragma unroll 8
-    for (int w = 0; w < 32; ++w) {
-      const int c = base[w * p.E + e];
-      base[w * p.E + e] = run;
-      run += c;
+template <int CL>
+static int plan_one(const int32_t* experts, const XPlan& p, int32_t* plan, cudaStream_t st) {
+  static int ready_dev = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_plan (device)");
+  if (ready_dev != dev) {
+    const int most = (4 * MB_PLAN_MAX_EXPERTS + 2 + 32 * MB_PLAN_MAX_EXPERTS) * 4;
+    if (cudaFuncSetAttribute(k_plan_one<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
+      set_error("expert_plan: cannot reserve %d bytes of shared memory", most);
+      return MB_E_CUDA;
     }
-    cnt[e] = run;
+    ready_dev = dev;
   }
-  __syncthreads();
-  xp_segments(p, plan, cnt, seg);
-  for (int i = threadIdx.x; i < 32 * p.E; i += 1024) base[i] += seg[i % p.E];
-  __syncthreads();
-  xp_place(experts, p, plan, 0, per, base);
+  const int64_t per = (p.R + 32 * CL * 32 - 1) / (32 * CL * 32) * 32;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(CL);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = (4 * p.E + 2 + 32 * p.E) * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CL;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, k_plan_one<CL>, experts, p, plan, per);
+  return check_launch("expert_plan");
 }
 
 // ------------------------------------------------------------------------------------------------ row movement
@@ -385,30 +490,6 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
   }
 }
 
-// dw = sum over the `parts` partial sums (in their order) of a product whose rows were split; n4 = whole float4s (n / 4
-// where every part starts on 16 bytes, else 0)
-template <typename T>
-__global__ void __launch_bounds__(256) k_parts_sum(const float* part, int parts, int64_t n, int64_t n4, T* out) {
-  const int64_t step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  for (int64_t i = i0; i < n4; i += step) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int q = 0; q < parts; ++q) {
-      const float4 v = *reinterpret_cast<const float4*>(part + q * n + 4 * i);
-      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-    }
-    if constexpr (sizeof(T) == 4)
-      *reinterpret_cast<float4*>(out + 4 * i) = s;
-    else
-      *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
-  }
-  for (int64_t i = 4 * n4 + i0; i < n; i += step) {
-    float s = 0.f;
-    for (int q = 0; q < parts; ++q) s += part[q * n + i];
-    out[i] = from_f<T>(s);
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ few slots
 // out[t][o] = sum_j g_tj <W[e_tj][o], x> without a plan: L lanes per (token, output), the rows of W of four choices side
 // by side in flight.  Bound by the bytes of W; a row of W that several tokens use comes from L2 after the first.
@@ -517,8 +598,8 @@ static XFwd x_fwd_layout(const XShape& s, bool combine, bool direct) {
 }
 
 struct XBwd {
-  int64_t xs = -1, dys = -1, ws = -1, dxb = -1, dgp = -1, parts = -1, bytes = 0;
-  int split = 1;
+  int64_t xs = -1, dys = -1, ws = -1, dxb = -1, dgp = -1, parts = -1, pre = -1, bytes = 0;
+  int kc = 0;
 };
 static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direct, bool need_x, bool need_w,
                          bool need_g) {
@@ -529,10 +610,14 @@ static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direc
   b.dys = c.take(row2 * s.Op);
   if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
   if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * dtype_size(s.dtype));
-  if (need_g) b.dgp = c.take(s.R * 4 * xgemm_n_tiles(XG_DGRAD, s.D));
+  if (need_g) b.dgp = c.take(s.R * 4 * xgemm_n_tiles(s.D, s.dtype));
   if (need_w) {
-    b.split = xgemm_split(s.E, s.O, s.D, s.R, s.np);
-    if (b.split > 1) b.parts = c.take((int64_t)b.split * s.E * s.O * s.D * 4);
+    b.kc = xgemm_kc(s.E, s.O, s.D, s.R, s.dtype);
+    const int64_t parts = xgemm_parts(s.E, s.R, b.kc);
+    if (parts) {
+      b.parts = c.take(parts * s.O * s.D * 4);
+      b.pre = c.take((s.E + 1) * 4);
+    }
   }
   b.bytes = c.used;
   return b;
@@ -631,23 +716,14 @@ extern "C" int mace_b200_expert_plan(const int32_t* experts, int64_t slots, int3
   }
   const XPlan p = xplan(slots, E);
   cudaStream_t st = (cudaStream_t)stream;
-  // one block up to 8192 slots (its 32 warps then take 256 slots each, as a block of the three-launch form does)
-  if (slots <= 8192 && E <= 256) {
-    const int per = (int)((slots + 1023) / 1024) * 32;
-    k_plan_one<<<1, 1024, (2 * E + 1 + 32 * E) * 4, st>>>(experts, p, plan, per);
-    return check_launch("expert_plan");
-  }
-  if (p.nblk > 0) {
-    k_plan_count<<<p.nblk, 256, E * 4, st>>>(experts, p, plan);
-    if (int rc = check_launch("expert_plan")) return rc;
-  }
-  k_plan_scan<<<1, 1024, (2 * E + 1) * 4, st>>>(p, plan);
+  if (slots <= 4096) return plan_one<1>(experts, p, plan, st);
+  if (slots <= XP_CLUSTER_SLOTS) return plan_one<8>(experts, p, plan, st);
+  k_plan_count<<<p.nblk, 256, 8 * E * 4, st>>>(experts, p, plan);
   if (int rc = check_launch("expert_plan")) return rc;
-  if (p.nblk > 0) {
-    k_plan_place<<<p.nblk, 256, 8 * E * 4, st>>>(experts, p, plan);
-    return check_launch("expert_plan");
-  }
-  return 0;
+  k_plan_scan<<<1, 1024, (3 * E + 2) * 4, st>>>(p, plan);
+  if (int rc = check_launch("expert_plan")) return rc;
+  k_plan_place<<<p.nblk, 256, 8 * E * 4, st>>>(experts, p, plan);
+  return check_launch("expert_plan");
 }
 
 extern "C" int mace_b200_expert_linear_workspace(int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
@@ -777,17 +853,13 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
       g.b = base + b.xs; g.ldb = s.Dp;
       g.rows = s.rows;
       g.E = E; g.M = O; g.N = D; g.K = 0;
-      g.plan = plan; g.lay = s.lay; g.split = b.split;
-      g.out = b.split > 1 ? (void*)(base + b.parts) : dw;
-      g.ldo = D;
-      if (int rc = xgemm_launch(g, st)) return rc;
-      if (b.split > 1) {
-        const int64_t n = (int64_t)E * O * D;
-        const int64_t n4 = n % 4 == 0 && aligned16(dw) ? n / 4 : 0;
-        k_parts_sum<T><<<x_grid(((n4 ? n4 : n) + 255) / 256), 256, 0, st>>>((const float*)(base + b.parts), b.split, n, n4,
-                                                                            (T*)dw);
-        if (int rc = check_launch("expert_linear (parts)")) return rc;
+      g.plan = plan; g.lay = s.lay;
+      g.out = dw; g.ldo = D; g.kc = b.kc;
+      if (b.parts >= 0) {
+        g.parts = (float*)(base + b.parts);
+        g.pre = (int32_t*)(base + b.pre);
       }
+      if (int rc = xgemm_launch(g, st)) return rc;
     }
     if (!dx && !dweights) return 0;
     XGemm g{};
@@ -805,6 +877,6 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
     if (int rc = xgemm_launch(g, st)) return rc;
     if (!sum && !dweights) return 0;
     return x_rows_sum<T>(sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, plan + s.lay.o_slot,
-                         dweights ? (const float*)(base + b.dgp) : nullptr, xgemm_n_tiles(XG_DGRAD, D), dweights, st);
+                         dweights ? (const float*)(base + b.dgp) : nullptr, xgemm_n_tiles(D, dtype), dweights, st);
   });
 }

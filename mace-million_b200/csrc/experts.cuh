@@ -14,9 +14,9 @@ struct XPlan {
   int64_t R;
   int32_t E, nblk;
   int64_t tiles;                                 // most tiles there can be
-  int64_t o_seg, o_cnt, o_order, o_tile, o_row, o_slot, o_hist, words;
+  int64_t o_seg, o_cnt, o_order, o_tile, o_pair, o_row, o_slot, o_hist, words;
 };
-// header words: 0 = tiles in use, 1 = status bits
+// header words: 0 = tiles in use, 1 = status bits, 2 = pairs of tiles in use
 inline XPlan xplan(int64_t R, int32_t E) {
   XPlan p;
   p.R = R;
@@ -27,7 +27,8 @@ inline XPlan xplan(int64_t R, int32_t E) {
   p.o_cnt = p.o_seg + E + 1;                     // [E] slots of each expert
   p.o_order = p.o_cnt + E;                       // [E] experts, most slots first (ties: lowest index)
   p.o_tile = p.o_order + E;                      // [tiles] expert of each tile
-  p.o_row = p.o_tile + p.tiles;                  // [tiles * XP_BM] slot of each row, -1 = padding
+  p.o_pair = p.o_tile + p.tiles;                 // [tiles] first tile of each pair of an expert's tiles
+  p.o_row = p.o_pair + p.tiles;                  // [tiles * XP_BM] slot of each row, -1 = padding
   p.o_slot = p.o_row + p.tiles * XP_BM;          // [R] row of each slot, -1 = no expert
   p.o_hist = p.o_slot + R;                       // [E][nblk] scratch
   p.words = p.o_hist + (int64_t)E * p.nblk;
@@ -50,15 +51,18 @@ struct XGemm {
   const float* scale;                            // per slot, or null
   void* out;                                     // FWD / DGRAD: [slots][ldo] (null: only dgpart); WGRAD: [E][M][N]
   int64_t ldo;
-  int32_t split;                                 // WGRAD: parts of each expert's rows; > 1: out is fp32 [split][E][M][N]
+  int32_t kc;                                    // WGRAD: K blocks of a part (xgemm_kc)
+  float* parts;                                  // WGRAD: xgemm_parts partial sums [M][N] (null: there are none)
+  int32_t* pre;                                  // WGRAD with parts: [E + 1] scratch
   // DGRAD: dgpart[n tile][slot] = partial <x, C> of the slot's x row (null: off)
   const void* x;
   int64_t ldx;
   int32_t kdiv;                                  // slot / kdiv = row of x
   float* dgpart;
 };
-int xgemm_n_tiles(int mode, int64_t N);
-int xgemm_split(int64_t E, int64_t M, int64_t N, int64_t slots, int planes);
+int xgemm_n_tiles(int64_t N, int dtype);
+int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype);
+int64_t xgemm_parts(int64_t E, int64_t slots, int kc);
 int xgemm_launch(const XGemm& g, cudaStream_t st);
 
 }  // namespace mb

@@ -4,14 +4,22 @@
 //   WGRAD  C[e][o][d] = sum over e's rows dy[row][o] x[row][d]   both MN-major, K = the expert's rows
 // Rows are sorted by expert and padded to 128, so a 128-row tile (FWD, DGRAD) or a 64-row K block (WGRAD) has one expert,
 // and no matrix is transposed in memory: the MN-major operands are read as they lie.
-// fp32 data comes as three bf16 planes; the products of the planes whose ranks add up to at most 2 (six of nine, small
-// ones first) accumulate in the same fp32 accumulator, the rest is below 2^-24 of the result.
+// fp32 data comes as three bf16 planes; a stage holds all three of both operands, and the products of the planes whose
+// ranks add up to at most 2 (six of nine, small ones first) go to the same fp32 accumulator; the rest is below 2^-24 of
+// the result.
 //
-// Persistent CTA, one per SM: warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
-// (128 x BN x 16) into one of two TMEM accumulators, warps 2-5 drain the other one (one row per lane), scale the row by
-// its slot's weight and write it to the slot's place in the output.  Every wait is bounded: on expiry the kernel sets
-// MB_ST_TC_TIMEOUT in the plan's status word, drains its copies and MMAs, frees its TMEM and returns.
+// Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
+// into one of two TMEM accumulators, warps 2-5 drain the other one.  CG = 2: a cluster of two CTAs works on a 256-row tile
+// (cta_group::2, each CTA holds its 128 rows of A and half of B's columns), which halves the B bytes a CTA fetches.
+// The N tile is the smallest multiple of 64 that cuts N into ceil(N / 256) tiles.
+// WGRAD cuts an expert's rows into parts of kc K blocks when there are few tiles; parts of an expert with several are
+// added up afterwards in their order.  Items come longest expert first and odd rounds run backwards over the CTAs, so
+// that every CTA gets about the same number of K blocks.
+// Every wait is bounded: on expiry the kernel sets MB_ST_TC_TIMEOUT in the plan's status word, drains its copies and
+// MMAs, frees its TMEM and returns.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "experts.cuh"
 #include "tc.cuh"
@@ -20,25 +28,30 @@ namespace mb {
 
 constexpr int XG_BM = XP_BM, XG_BK = 64, XG_THREADS = 192;
 constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
-
 constexpr int XG_STG = 4096;                     // row staging of one epilogue warp
-template <int BN>
+
+// T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for
+template <typename T, int BN, int CG>
 struct XgCfg {
-  static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN * XG_BK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 196608 / STAGE;              // 192 KB ring: 4 stages at BN = 256, 6 at 128
+  static constexpr int PL = sizeof(T) == 4 ? 3 : 1;          // planes of a stage
+  static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN / CG * XG_BK * 2;
+  static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
+  static constexpr int STAGES = 196608 / STAGE;
   static constexpr int TMEM = 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE + 4 * XG_STG + 256 + 1024;   // + row staging, barriers, alignment slack
+  static constexpr int PRE = 4352;                           // [E + 1] first item of each expert (WGRAD)
+  static constexpr int SMEM = STAGES * STAGE + 4 * XG_STG + PRE + 256 + 1024;   // + barriers, alignment slack
+  static_assert(STAGES >= 2 && STAGES <= 8 && SMEM <= 227 * 1024 && PRE >= 4 * (MB_PLAN_MAX_EXPERTS + 1), "shared memory");
 };
 
 struct XgParams {
-  int32_t E, M, N, K, tn, tm, np;                // tn / tm: tiles along N, along M (WGRAD)
-  int32_t split;                                 // WGRAD: parts of an expert's rows
+  int32_t E, M, N, K, bn, tn, tm, kc;            // bn columns a tile, tn / tm tiles along N / M (WGRAD), kc see above
   int64_t rows;                                  // rows per plane of the sorted operands
-  int32_t w_rows;                                // E (planes of w follow each other)
   const int32_t* plan;
   XPlan lay;
   const float* scale;
   void* out;
+  float* parts;
+  int32_t* pre;
   int64_t ldo;
   const void* x;
   int64_t ldx;
@@ -52,9 +65,11 @@ struct XgBars {
   int failed;
 };
 
-// planes of A and B multiplied in pass p (of 6): small products first
-__device__ __forceinline__ int xg_plane_a(int p) { return (0x021010 >> (4 * (5 - p))) & 0xF; }
-__device__ __forceinline__ int xg_plane_b(int p) { return (0x201100 >> (4 * (5 - p))) & 0xF; }
+struct XgTile {
+  int e, m0, n0, r0, nk;                         // expert; first row, column; first K row (WGRAD); K blocks
+  int part;                                      // WGRAD: >= 0: the item's place in the partial sums
+  bool rows_ok;                                  // FWD / DGRAD: this CTA's rows belong to the expert
+};
 
 // Row staging of the epilogue: a warp's 32 rows x 128 bytes, 16-byte piece c of row r at piece c ^ (r % 8), so that a lane's
 // access to its own row and the warp's access to four whole row segments are both free of bank conflicts.
@@ -62,23 +77,132 @@ __device__ __forceinline__ uint4* xg_stg(unsigned char* stg, int row, int c) {
   return reinterpret_cast<uint4*>(stg + row * 128 + ((c ^ (row & 7)) << 4));
 }
 
-// OUT: element type of the output (T, or float for partial sums)
-template <int MODE, typename T, typename OUT, int BN>
+// Drains one accumulator: one row per lane out of TMEM, scaled, through shared memory in pieces of 128 bytes, so that
+// global accesses are whole 128-byte segments of four rows (one row per lane would be 32 scattered 16-byte pieces per
+// access, and held a tile for longer than its products at K <= 1024).  dst: this lane's row (null: not stored);
+// xr: the row of x that `dot` takes the scalar product with (DOT).
+template <typename OUT, typename T, bool DOT>
+__device__ __forceinline__ float xg_drain(uint32_t tacc, bool zero, unsigned char* stg, OUT* dst, bool vec, float sc, int nc,
+                                          const T* xr, bool xvec, uint64_t* wait_bar, uint32_t wait_par, bool& ok) {
+  constexpr int NC = 128 / (int)sizeof(OUT);     // columns of a piece
+  constexpr int XV = kVec<T>;
+  const int lane = threadIdx.x & 31;
+  const int r8 = lane >> 3, c8 = lane & 7;       // this lane's row (of four) and 16-byte piece in whole-segment accesses
+  float dot = 0.f;
+  // the x rows' pieces are loaded one piece ahead, the first before the accumulator is waited for
+  uint4 xq[DOT ? 8 : 1];
+  auto fetch_x = [&](int h) {
+    const int n = nc - h * NC < NC ? nc - h * NC : NC;
+#pragma unroll
+    for (int i = 0; i < (DOT ? 8 : 0); ++i) {
+      const T* xp = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 4 * i + r8));
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (xp) {
+        xp += h * NC + c8 * XV;
+        if (xvec && (c8 + 1) * XV <= n) {
+          v = *reinterpret_cast<const uint4*>(xp);
+        } else {
+          float f[XV];
+#pragma unroll
+          for (int q = 0; q < XV; ++q) f[q] = c8 * XV + q < n ? to_f(xp[q]) : 0.f;
+          v = pack16<T>(f);
+        }
+      }
+      xq[i] = v;
+    }
+  };
+  if (DOT) fetch_x(0);
+  if (!zero) {
+    ok = __all_sync(0xffffffffu, mbar_wait_ns(wait_bar, wait_par, XG_WAIT_NS));
+    if (!ok) return 0.f;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
+#pragma unroll 1
+  for (int h = 0; h * NC < nc; ++h) {
+    const int n = nc - h * NC < NC ? nc - h * NC : NC;
+    uint32_t u[NC];
+    if (!zero) {
+#pragma unroll
+      for (int q = 0; q < NC / 32; ++q) tmem_ld32(tacc + NC * h + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * q));
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) u[i] = 0u;
+    }
+    if constexpr (DOT) {
+      // a piece of 128 bytes of x holds as many columns as one of the output: T = OUT here
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *xg_stg(stg, 4 * i + r8, c8) = xq[i];
+      if ((h + 1) * NC < nc) fetch_x(h + 1);
+      __syncwarp();
+      // one short chain per vector, added up as a tree: the rounding of 256 terms in a row would show
+      float part[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float f[XV];
+        unpack16(*xg_stg(stg, lane, c), f, T());
+        part[c] = 0.f;
+#pragma unroll
+        for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], __uint_as_float(u[c * XV + q]), part[c]);
+      }
+      dot += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+      __syncwarp();
+    }
+    if (!__any_sync(0xffffffffu, dst != nullptr)) continue;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      float f[kVec<OUT>];
+#pragma unroll
+      for (int q = 0; q < kVec<OUT>; ++q) f[q] = __uint_as_float(u[c * kVec<OUT> + q]) * sc;
+      *xg_stg(stg, lane, c) = pack16<OUT>(f);
+    }
+    __syncwarp();
+    if (vec) {
+      const int left = n - c8 * kVec<OUT>;       // columns of this lane's piece
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 4 * i + r8));
+        if (!p || left <= 0) continue;
+        p += h * NC + c8 * kVec<OUT>;
+        const uint4* s = xg_stg(stg, 4 * i + r8, c8);
+        if (left >= kVec<OUT>)
+          *reinterpret_cast<uint4*>(p) = *s;
+        else
+          for (int q = 0; q < left; ++q) p[q] = reinterpret_cast<const OUT*>(s)[q];
+      }
+    } else {                                     // odd strides: one row at a time, lanes along it
+#pragma unroll 4
+      for (int r = 0; r < 32; ++r) {
+        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), r));
+#pragma unroll
+        for (int q = 0; q < NC / 32; ++q) {
+          const int c = lane + 32 * q;
+          if (p && c < n) p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, r, c / kVec<OUT>))[c % kVec<OUT>];
+        }
+      }
+    }
+    __syncwarp();
+  }
+  return dot;
+}
+
+template <int MODE, typename T, int BN, int CG>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
-  using C = XgCfg<BN>;
+  using C = XgCfg<T, BN, CG>;
   constexpr bool A_MN = MODE == XG_WGRAD, B_MN = MODE != XG_FWD;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  XgBars& B = *reinterpret_cast<XgBars*>(smem + C::STAGES * C::STAGE + 4 * XG_STG);
+  unsigned char* stg0 = smem + C::STAGES * C::STAGE;
+  int* pre = reinterpret_cast<int*>(stg0 + 4 * XG_STG);
+  XgBars& B = *reinterpret_cast<XgBars*>(stg0 + 4 * XG_STG + C::PRE);
   volatile int* failed = &B.failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CG == 2 ? (int)cluster_ctarank() : 0, cta = blockIdx.x / CG, ctas = gridDim.x / CG;
+  const int32_t* plan = g.plan;
 
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
-                 "r"(C::TMEM)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc<CG>(&B.tmem, C::TMEM);
     if (lane == 0) {
       for (int s = 0; s < C::STAGES; ++s) {
         mbar_init(&B.full[s], 1);
@@ -86,103 +210,132 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       }
       for (int a = 0; a < 2; ++a) {
         mbar_init(&B.acc_full[a], 1);
-        mbar_init(&B.acc_empty[a], 128);
+        mbar_init(&B.acc_empty[a], 128 * CG);
       }
       B.failed = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
+  if (MODE == XG_WGRAD && warp == 0) {           // first item of each expert, longest first
+    int run = 0;
+    for (int e0 = 0; e0 < g.E; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0;
+      if (e < g.E) {
+        const int nk = (plan[g.lay.o_cnt + plan[g.lay.o_order + e]] + XG_BK - 1) / XG_BK;
+        n = nk <= g.kc ? 1 : (nk + g.kc - 1) / g.kc;
+      }
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (e < g.E) pre[e] = run + inc - n;
+      run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) pre[g.E] = run;
+    __syncwarp();
+    if (g.pre && blockIdx.x == 0)
+      for (int e = lane; e <= g.E; e += 32) g.pre[e] = pre[e];
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();         // the peer's barriers are initialised
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = B.tmem;
-  const int32_t* plan = g.plan;
-  const int tiles = MODE == XG_WGRAD ? g.split * g.E * g.tm * g.tn : plan[0] * g.tn;
-
-  // This CTA's n-th tile.  WGRAD: experts come longest first and odd rounds run backwards over the CTAs, so that every CTA
-  // gets about the same number of K blocks.
-  auto tile_at = [&](int n) {
-    const int t = n * gridDim.x + (MODE == XG_WGRAD && (n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    return t;
-  };
-  const int rounds = (tiles + gridDim.x - 1) / gridDim.x;
-  // tile -> (expert, first row of A / first output row, first column, K blocks)
-  struct Tile {
-    int e, m0, n0, r0, nk, se;
-  };
+  const int tiles = MODE == XG_WGRAD ? pre[g.E] * g.tm * g.tn : plan[CG == 2 ? 2 : 0] * g.tn;
+  const int rounds = (tiles + ctas - 1) / ctas;
+  auto tile_at = [&](int n) { return n * ctas + (MODE == XG_WGRAD && (n & 1) ? ctas - 1 - cta : cta); };
   auto tile_of = [&](int t) {
-    Tile o;
+    XgTile o;
     const int m = t / g.tn;
-    o.n0 = (t - m * g.tn) * BN;
+    o.n0 = (t - m * g.tn) * g.bn;
+    o.part = -1;
+    o.rows_ok = true;
     if constexpr (MODE == XG_WGRAD) {
-      const int sr = m / g.tm, part = sr / g.E;
-      o.e = plan[g.lay.o_order + sr - part * g.E];
-      o.m0 = (m - sr * g.tm) * XG_BM;
-      o.se = part * g.E + o.e;
-      const int nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK;
-      const int k0 = (int)((int64_t)nk * part / g.split);
+      const int item = m / g.tm;
+      o.m0 = (m - item * g.tm) * (XG_BM * CG) + rank * XG_BM;
+      int lo = 0, hi = g.E - 1;                  // last expert whose first item is <= item
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (pre[mid] <= item)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      o.e = plan[g.lay.o_order + lo];
+      const int nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK, parts = pre[lo + 1] - pre[lo], q = item - pre[lo];
+      const int k0 = (int)((int64_t)nk * q / parts);
       o.r0 = plan[g.lay.o_seg + o.e] + k0 * XG_BK;
-      o.nk = (int)((int64_t)nk * (part + 1) / g.split) - k0;
+      o.nk = (int)((int64_t)nk * (q + 1) / parts) - k0;
+      if (parts > 1) o.part = item;
     } else {
-      o.e = plan[g.lay.o_tile + m];
-      o.m0 = o.r0 = m * XG_BM;
+      const int tile = CG == 2 ? plan[g.lay.o_pair + m] : m;
+      o.e = plan[g.lay.o_tile + tile];
+      o.m0 = (tile + rank) * XG_BM;
+      o.r0 = 0;
+      if (CG == 2 && rank == 1) o.rows_ok = o.m0 < plan[g.lay.o_seg + o.e + 1];
       o.nk = (g.K + XG_BK - 1) / XG_BK;
     }
     return o;
   };
-  const int p0 = g.np == 3 ? 0 : 5;              // passes over the planes: p0 .. 5
+  const int bh = g.bn / CG;                      // columns of B that this CTA loads
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------ loads
     if (lane == 0) {
       int seq = 0;
       bool ok = true;
+      const uint32_t b_bytes = B_MN ? (uint32_t)((bh + 63) / 64) * 8192u : (uint32_t)bh * 128u;
+      const uint32_t bytes = CG * C::PL * (C::A_BYTES + b_bytes);
       for (int r = 0; ok && r < rounds; ++r) {
         const int t = tile_at(r);
-        if (t >= tiles) break;                     // only in the last round
-        const Tile w = tile_of(t);
-        for (int p = p0; ok && p < 6; ++p) {
-          const int pa = xg_plane_a(p), pb = xg_plane_b(p);
-          for (int kb = 0; kb < w.nk; ++kb, ++seq) {
-            const int s = seq % C::STAGES;
-            if (*failed || !mbar_wait_ns(&B.empty[s], ((seq / C::STAGES) & 1) ^ 1, XG_WAIT_NS)) {
-              *failed = 1;
-              ok = false;
-              break;
-            }
-            const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
-            uint64_t* bar = &B.full[s];
-            mbar_arrive_tx(bar, C::STAGE);
-            const int k0 = kb * XG_BK;
+        if (t >= tiles) break;                   // only in the last round
+        const XgTile w = tile_of(t);
+        for (int kb = 0; kb < w.nk; ++kb, ++seq) {
+          const int s = seq % C::STAGES;
+          if (*failed || !mbar_wait_ns(&B.empty[s], ((seq / C::STAGES) & 1) ^ 1, XG_WAIT_NS)) {
+            *failed = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t bar = CG == 2 ? mapa_u32(smem_u32(&B.full[s]), 0) : smem_u32(&B.full[s]);
+          if (rank == 0) mbar_arrive_tx(&B.full[s], bytes);   // both CTAs' bytes arrive at the first one's barrier
+          const int k0 = kb * XG_BK;
+#pragma unroll
+          for (int p = 0; p < C::PL; ++p) {
+            const uint32_t a = smem_u32(smem + s * C::STAGE) + p * C::A_BYTES;
+            const uint32_t b = smem_u32(smem + s * C::STAGE) + C::PL * C::A_BYTES + p * C::B_BYTES;
+            const int row0 = (int)(p * g.rows);
             if constexpr (MODE == XG_WGRAD) {
 #pragma unroll
               for (int c = 0; c < XG_BM / 64; ++c)
-                tma_load_2d(a + c * 8192, &map_a, w.m0 + 64 * c, (int)(pa * g.rows) + w.r0 + k0, bar);
+                tma_load_2d<CG>(a + c * 8192, &map_a, w.m0 + 64 * c, row0 + w.r0 + k0, bar);
 #pragma unroll
-              for (int c = 0; c < BN / 64; ++c)
-                tma_load_2d(b + c * 8192, &map_b, w.n0 + 64 * c, (int)(pb * g.rows) + w.r0 + k0, bar);
+              for (int c = 0; c < BN / CG / 64; ++c)
+                if (c * 64 < bh) tma_load_2d<CG>(b + c * 8192, &map_b, w.n0 + rank * bh + 64 * c, row0 + w.r0 + k0, bar);
             } else {
-              tma_load_2d(a, &map_a, k0, (int)(pa * g.rows) + w.m0, bar);
-              if constexpr (MODE == XG_FWD) {
-                tma_load_3d(b, &map_b, k0, w.n0, pb * g.w_rows + w.e, bar);
-              } else {
+              tma_load_2d<CG>(a, &map_a, k0, row0 + w.m0, bar);
+              if constexpr (MODE == XG_FWD)
+                tma_load_3d<CG>(b, &map_b, k0, w.n0 + rank * bh, p * g.E + w.e, bar);
+              else
 #pragma unroll
-                for (int c = 0; c < BN / 64; ++c)
-                  tma_load_3d(b + c * 8192, &map_b, w.n0 + 64 * c, k0, pb * g.w_rows + w.e, bar);
-              }
+                for (int c = 0; c < BN / CG / 64; ++c)
+                  if (c * 64 < bh) tma_load_3d<CG>(b + c * 8192, &map_b, w.n0 + rank * bh + 64 * c, k0, p * g.E + w.e, bar);
             }
           }
         }
       }
-      // after a timeout: the copies already issued land before the block ends (bounded)
-      if (!ok)
+      // after a timeout: the copies already issued land before the block ends (bounded; a pair's land at rank 0)
+      if (!ok && rank == 0)
         for (int q = seq - C::STAGES < 0 ? 0 : seq - C::STAGES; q < seq; ++q)
           mbar_wait_ns(&B.full[q % C::STAGES], (q / C::STAGES) & 1, XG_WAIT_NS);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      constexpr uint32_t idesc = f16_idesc(XG_BM, BN, !std::is_same<T, f16>::value, A_MN, B_MN);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = f16_idesc(XG_BM * CG, g.bn, !std::is_same<T, f16>::value, A_MN, B_MN);
       int seq = 0, tc = 0;
       bool ok = true;
       uint64_t* last_bar = nullptr;
@@ -190,8 +343,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       for (int r = 0; ok && r < rounds; ++r) {
         const int t = tile_at(r);
         if (t >= tiles) break;
-        const Tile w = tile_of(t);
-        if (w.nk == 0) continue;
+        const int nk = tile_of(t).nk;
+        if (nk == 0) continue;
         const int acc = tc & 1;
         if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, XG_WAIT_NS)) {
           *failed = 1;
@@ -199,8 +352,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + (uint32_t)(acc * BN);
-        const int total = w.nk * (6 - p0);
-        for (int kb = 0; kb < total; ++kb, ++seq) {
+        for (int kb = 0; kb < nk; ++kb, ++seq) {
           const int s = seq % C::STAGES;
           if (!mbar_wait_ns(&B.full[s], (seq / C::STAGES) & 1, XG_WAIT_NS)) {
             *failed = 1;
@@ -208,20 +360,26 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+          const uint32_t a0 = smem_u32(smem + s * C::STAGE), b0 = a0 + C::PL * C::A_BYTES;
 #pragma unroll
-          for (int kk = 0; kk < XG_BK / 16; ++kk) {
-            // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
-            const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
-            const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
-            mma_f16_ss(d, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          for (int p = 0; p < (C::PL == 3 ? 6 : 1); ++p) {
+            // planes (a, b): (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+            constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
+            const uint32_t a = a0 + (C::PL == 3 ? PA[p] * C::A_BYTES : 0), b = b0 + (C::PL == 3 ? PB[p] * C::B_BYTES : 0);
+#pragma unroll
+            for (int kk = 0; kk < XG_BK / 16; ++kk) {
+              // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
+              const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
+              const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
+              mma_f16_ss<CG>(d, ad, bd, idesc, (kb > 0 || kk > 0 || p > 0) ? 1u : 0u);
+            }
           }
-          mma_commit(&B.empty[s]);
+          mma_commit_to<CG>(&B.empty[s]);
           last_bar = &B.empty[s];
           last_par = (seq / C::STAGES) & 1;
         }
         if (!ok) break;
-        mma_commit(&B.acc_full[acc]);
+        mma_commit_to<CG>(&B.acc_full[acc]);
         last_bar = &B.acc_full[acc];
         last_par = (tc >> 1) & 1;
         ++tc;
@@ -231,140 +389,54 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------------------------------ epilogue
-    // One row per lane out of TMEM; rows pass through shared memory in pieces of 128 bytes so that global accesses are
-    // whole 128-byte segments of four rows (one row per lane: 32 scattered 16-byte pieces per access, which held a tile
-    // for longer than its products at K <= 1024).
     const int q4 = warp & 3, row = q4 * 32 + lane;
-    unsigned char* stg = smem + C::STAGES * C::STAGE + (warp - 2) * XG_STG;
-    constexpr int NC = 128 / (int)sizeof(OUT);     // columns of a piece
-    constexpr int XV = kVec<T>;
-    const int r8 = lane >> 3, c8 = lane & 7;       // this lane's row (of four) and 16-byte piece in whole-segment accesses
-    const bool vec = g.ldo % kVec<OUT> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-    const bool xvec = MODE == XG_DGRAD && g.ldx % XV == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
+    unsigned char* stg = stg0 + (warp - 2) * XG_STG;
+    const bool out16 = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+    const bool vec = g.ldo % kVec<T> == 0 && out16;
+    const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
     int tc = 0;
     // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
     for (int r = 0; r < rounds; ++r) {
       if (__shfl_sync(0xffffffffu, *failed, 0)) break;
       const int t = tile_at(r);
       if (t >= tiles) break;
-      const Tile w = tile_of(t);
-      OUT* dst = nullptr;
-      float sc = 1.f, dot = 0.f;
-      const T* xr = nullptr;
-      int slot = -1;
+      const XgTile w = tile_of(t);
+      const int acc = tc & 1, nc = g.N - w.n0 < g.bn ? g.N - w.n0 : g.bn;
+      const uint32_t tacc = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN);
+      uint64_t* bar = &B.acc_full[acc];
+      const uint32_t par = (tc >> 1) & 1;
+      bool ok = true;
       if constexpr (MODE == XG_WGRAD) {
-        if (w.m0 + row < g.M) dst = (OUT*)g.out + ((int64_t)w.se * g.M + w.m0 + row) * g.ldo + w.n0;
-      } else {
-        slot = plan[g.lay.o_row + w.m0 + row];
-        if (slot >= 0) {
-          if (g.out) dst = (OUT*)g.out + (int64_t)slot * g.ldo + w.n0;
-          if (g.scale) sc = g.scale[slot];
-          if (MODE == XG_DGRAD && g.dgpart) xr = (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + w.n0;
-        }
-      }
-      const int acc = tc & 1, nc = g.N - w.n0 < BN ? g.N - w.n0 : BN;
-      // the x rows' pieces for the dot products, loaded one piece ahead (and the first before the wait)
-      uint4 xq[MODE == XG_DGRAD ? 8 : 1];
-      auto fetch_x = [&](int h) {
-        const int n = nc - h * NC < NC ? nc - h * NC : NC;
-#pragma unroll
-        for (int i = 0; i < (MODE == XG_DGRAD ? 8 : 0); ++i) {
-          const T* xp =
-              reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 4 * i + r8));
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (xp) {
-            xp += h * NC + c8 * XV;
-            if (xvec && (c8 + 1) * XV <= n) {
-              v = *reinterpret_cast<const uint4*>(xp);
-            } else {
-              float f[XV];
-#pragma unroll
-              for (int q = 0; q < XV; ++q) f[q] = c8 * XV + q < n ? to_f(xp[q]) : 0.f;
-              v = pack16<T>(f);
-            }
-          }
-          xq[i] = v;
-        }
-      };
-      if (MODE == XG_DGRAD && g.dgpart) fetch_x(0);
-      if (w.nk > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS))) {
-          *failed = 1;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      }
-#pragma unroll 1
-      for (int h = 0; h * NC < nc; ++h) {
-        const int n = nc - h * NC < NC ? nc - h * NC : NC;
-        uint32_t u[NC];
-        if (w.nk > 0) {
-          const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + NC * h);
-#pragma unroll
-          for (int q = 0; q < NC / 32; ++q) tmem_ld32(ta + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * q));
-          tmem_wait_ld();
+        const bool in = w.m0 + row < g.M;
+        if (w.part >= 0) {
+          float* dst = in ? g.parts + ((int64_t)w.part * g.M + w.m0 + row) * g.N + w.n0 : nullptr;
+          xg_drain<float, T, false>(tacc, w.nk == 0, stg, dst, g.N % 4 == 0, 1.f, nc, nullptr, false, bar, par, ok);
         } else {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) u[i] = 0u;
+          T* dst = in ? (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo + w.n0 : nullptr;
+          xg_drain<T, T, false>(tacc, w.nk == 0, stg, dst, vec, 1.f, nc, nullptr, false, bar, par, ok);
         }
-        if constexpr (MODE == XG_DGRAD) {          // dot += <x row, row> over this piece's columns
-          if (g.dgpart) {
-            // a piece of 128 bytes of x holds as many columns as one of the output: T = OUT here
-#pragma unroll
-            for (int i = 0; i < (MODE == XG_DGRAD ? 8 : 0); ++i) *xg_stg(stg, 4 * i + r8, c8) = xq[i];
-            if ((h + 1) * NC < nc) fetch_x(h + 1);
-            __syncwarp();
-            // one short chain per vector, added up as a tree: the rounding of 256 terms in a row would show
-            float part[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float f[XV];
-              unpack16(*xg_stg(stg, lane, c), f, T());
-              part[c] = 0.f;
-#pragma unroll
-              for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], __uint_as_float(u[c * XV + q]), part[c]);
-            }
-            dot += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-            __syncwarp();
-          }
-        }
-        if (MODE == XG_WGRAD || g.out) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float f[kVec<OUT>];
-#pragma unroll
-            for (int q = 0; q < kVec<OUT>; ++q) {
-              const float v = __uint_as_float(u[c * kVec<OUT> + q]);
-              f[q] = MODE == XG_WGRAD ? v : v * sc;
-            }
-            *xg_stg(stg, lane, c) = pack16<OUT>(f);
-          }
-          __syncwarp();
-          if (vec && n == NC) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 4 * i + r8));
-              if (p) *reinterpret_cast<uint4*>(p + h * NC + c8 * kVec<OUT>) = *xg_stg(stg, 4 * i + r8, c8);
-            }
-          } else {                                 // odd strides and the last columns: one row at a time, lanes along it
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-              OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), r));
-#pragma unroll
-              for (int q = 0; q < NC / 32; ++q) {
-                const int c = lane + 32 * q;
-                if (p && c < n)
-                  p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, r, c / kVec<OUT>))[c % kVec<OUT>];
-              }
-            }
-          }
-          __syncwarp();
+      } else {
+        const int slot = w.rows_ok ? plan[g.lay.o_row + w.m0 + row] : -1;
+        T* dst = slot >= 0 && g.out ? (T*)g.out + (int64_t)slot * g.ldo + w.n0 : nullptr;
+        const float sc = slot >= 0 && g.scale ? g.scale[slot] : 1.f;
+        if (MODE == XG_DGRAD && g.dgpart) {
+          const T* xr = slot >= 0 ? (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + w.n0 : nullptr;
+          const float dot = xg_drain<T, T, true>(tacc, false, stg, dst, vec, sc, nc, xr, xvec, bar, par, ok);
+          if (ok && slot >= 0) g.dgpart[(int64_t)(w.n0 / g.bn) * g.lay.R + slot] = dot;
+        } else {
+          xg_drain<T, T, false>(tacc, false, stg, dst, vec, sc, nc, nullptr, false, bar, par, ok);
         }
       }
-      if (MODE == XG_DGRAD && xr) g.dgpart[(int64_t)(w.n0 / BN) * g.lay.R + slot] = dot;
+      if (!ok) {
+        *failed = 1;
+        break;
+      }
       if (w.nk > 0) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        mbar_arrive(&B.acc_empty[acc]);
+        if constexpr (CG == 2)
+          mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
+        else
+          mbar_arrive(&B.acc_empty[acc]);
         ++tc;
       }
     }
@@ -372,10 +444,40 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (tid == 0 && *failed) atomicOr((unsigned*)plan + 1, (unsigned)MB_ST_TC_TIMEOUT);
+  if constexpr (CG == 2) cluster_sync();         // no CTA leaves while its peer can still signal it or read its operands
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    tmem_dealloc<CG>(tmem, C::TMEM);
+  }
+}
+
+// dW of the experts whose rows were cut into parts: the sum of the parts, in their order.  Block row y: expert order[y].
+template <typename T>
+__global__ void __launch_bounds__(256) k_parts_sum(const float* parts, const int32_t* pre, const int32_t* order, int64_t n,
+                                                   bool vec, T* out) {
+  const int first = pre[blockIdx.y], np = pre[blockIdx.y + 1] - first;
+  if (np < 2) return;                            // written by the product itself
+  T* o = out + (int64_t)order[blockIdx.y] * n;
+  const float* p = parts + (int64_t)first * n;
+  const int64_t step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t n4 = vec ? n / 4 : 0;
+  for (int64_t i = i0; i < n4; i += step) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < np; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(p + q * n + 4 * i);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(o + 4 * i) = s;
+    else
+      *reinterpret_cast<uint2*>(o + 4 * i) = make_uint2(pack2(s.x, s.y, T()), pack2(s.z, s.w, T()));
+  }
+  for (int64_t i = 4 * n4 + i0; i < n; i += step) {
+    float s = 0.f;
+    for (int q = 0; q < np; ++q) s += p[q * n + i];
+    o[i] = from_f<T>(s);
   }
 }
 
@@ -421,29 +523,36 @@ static int xg_map(CUtensorMap* m, bool is_bf16, int rank, const void* p, const i
   return 0;
 }
 
-static int xg_bn(int64_t N) { return N <= 128 ? 128 : 256; }
-int xgemm_n_tiles(int mode, int64_t N) {
-  (void)mode;
-  return (int)((N + xg_bn(N) - 1) / xg_bn(N));
+static int xg_bn_max(int64_t N, int dtype) { return dtype == MB_F32 || N <= 128 ? 128 : 256; }
+int xgemm_n_tiles(int64_t N, int dtype) {
+  const int bn = xg_bn_max(N, dtype);
+  return (int)((N + bn - 1) / bn);
 }
 
-// Parts of each expert's rows in WGRAD: enough tiles for four per SM when there are few, with at least 16 K blocks left
-// in an average part (below that the partial sums cost more than the idle SMs)
-int xgemm_split(int64_t E, int64_t M, int64_t N, int64_t slots, int planes) {
-  const int64_t tiles = E * ((M + XG_BM - 1) / XG_BM) * ((N + xg_bn(N) - 1) / xg_bn(N));
-  const int64_t blocks = slots / E / XG_BK * (planes == 3 ? 6 : 1);
-  int64_t s = 4 * (int64_t)sm_count() / tiles;
-  if (s > blocks / 16) s = blocks / 16;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// K blocks of a part in WGRAD: whole experts when that makes four or more rounds of tiles, else parts that make about
+// that many, of at least 8 K blocks (below that the partial sums' traffic outweighs the idle SMs)
+int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype) {
+  const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype), want = 4 * (int64_t)sm_count();
+  const int64_t blocks = slots / XG_BK;          // K blocks of all experts
+  if (E * per >= want) return 0x3fffffff;
+  int64_t kc = blocks * per / want;
+  const int64_t least = dtype == MB_F32 ? 4 : 8;
+  return (int)(kc < least ? least : kc);
+}
+// most partial sums there can be: a part has kc K blocks but the last of an expert, and an expert of one part has none
+int64_t xgemm_parts(int64_t E, int64_t slots, int kc) {
+  if (kc >= 0x3fffffff) return 0;
+  const int64_t blocks = slots / XG_BK + E;
+  return blocks / kc + E;
 }
 
-template <int MODE, typename T, typename OUT, int BN>
+template <int MODE, typename T, int BN, int CG>
 static int xg_go(const XGemm& x, cudaStream_t st) {
-  using C = XgCfg<BN>;
+  using C = XgCfg<T, BN, CG>;
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
-  auto kern = k_expert_gemm<MODE, T, OUT, BN>;
+  auto kern = k_expert_gemm<MODE, T, BN, CG>;
   if (ready_dev != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -451,49 +560,86 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
     }
     ready_dev = dev;
   }
+  XgParams g{};
+  g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K;
+  g.tn = xgemm_n_tiles(x.N, x.dtype);
+  g.bn = (int)(((x.N + g.tn - 1) / g.tn + 63) / 64 * 64);
+  g.tm = (x.M + XG_BM * CG - 1) / (XG_BM * CG);
+  g.kc = x.kc;
   const bool is_bf16 = !std::is_same<T, f16>::value;
-  const int np = x.dtype == MB_F32 ? 3 : 1;
   CUtensorMap ma, mbm;
   {
-    const int64_t dims[2] = {x.lda, np * x.rows}, str[1] = {x.lda};
+    const int64_t dims[2] = {x.lda, C::PL * x.rows}, str[1] = {x.lda};
     const int box[2] = {64, MODE == XG_WGRAD ? XG_BK : XG_BM};
     if (int rc = xg_map(&ma, is_bf16, 2, x.a, dims, str, box)) return rc;
   }
   if (MODE == XG_WGRAD) {
-    const int64_t dims[2] = {x.ldb, np * x.rows}, str[1] = {x.ldb};
+    const int64_t dims[2] = {x.ldb, C::PL * x.rows}, str[1] = {x.ldb};
     const int box[2] = {64, XG_BK};
     if (int rc = xg_map(&mbm, is_bf16, 2, x.b, dims, str, box)) return rc;
   } else {
     const int64_t O = MODE == XG_FWD ? x.N : x.K;
-    const int64_t dims[3] = {x.ldb, O, (int64_t)np * x.E}, str[2] = {x.ldb, x.ldb * O};
-    const int box[3] = {64, MODE == XG_FWD ? BN : XG_BK, 1};
+    const int64_t dims[3] = {x.ldb, O, (int64_t)C::PL * x.E}, str[2] = {x.ldb, x.ldb * O};
+    const int box[3] = {64, MODE == XG_FWD ? g.bn / CG : XG_BK, 1};
     if (int rc = xg_map(&mbm, is_bf16, 3, x.b, dims, str, box)) return rc;
   }
-  XgParams g{};
-  g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K; g.np = np;
-  g.tn = (x.N + BN - 1) / BN;
-  g.tm = (x.M + XG_BM - 1) / XG_BM;
-  g.rows = x.rows; g.w_rows = x.E;
+  g.rows = x.rows;
   g.plan = x.plan; g.lay = x.lay; g.scale = x.scale;
   g.out = x.out; g.ldo = x.ldo;
-  g.split = x.split > 1 ? x.split : 1;
+  g.parts = x.parts; g.pre = x.pre;
   g.x = x.x; g.ldx = x.ldx; g.kdiv = x.kdiv; g.dgpart = x.dgpart;
-  const int64_t most = MODE == XG_WGRAD ? (int64_t)g.split * x.E * g.tm * g.tn : x.lay.tiles * g.tn;
-  if (most > 0x7fffffff || np * x.rows > 0x7fffffff) {
-    set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)most, (long long)(np * x.rows));
+  const int64_t items = MODE == XG_WGRAD ? (xgemm_parts(x.E, x.lay.R, x.kc) + x.E) * g.tm : x.lay.tiles;
+  if (items * g.tn > 0x7fffffff || C::PL * x.rows > 0x7fffffff) {
+    set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)(items * g.tn), (long long)(C::PL * x.rows));
     return MB_E_ARG;
   }
-  if (most == 0) return 0;
-  const int sms = sm_count();
-  kern<<<(unsigned)(most < sms ? most : sms), XG_THREADS, C::SMEM, st>>>(ma, mbm, g);
-  return check_launch("expert_linear");
+  if (items == 0) return 0;
+  const int sms = sm_count() / CG;
+  const int grid = (int)(items * g.tn < sms ? items * g.tn : sms) * CG;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(XG_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kern, ma, mbm, g);
+  if (int rc = check_launch("expert_linear")) return rc;
+  if (MODE == XG_WGRAD && x.parts) {
+    const int64_t n = (int64_t)x.M * x.N;
+    const bool vec = n % 4 == 0 && aligned16(x.out);
+    const int64_t bx = (n / (vec ? 4 : 1) + 255) / 256, most = 16 * (int64_t)sm_count() / x.E + 1;
+    k_parts_sum<T><<<dim3((unsigned)(bx < most ? bx : most), x.E), 256, 0, st>>>(x.parts, x.pre, x.plan + x.lay.o_order, n,
+                                                                               vec, (T*)x.out);
+    return check_launch("expert_linear (parts)");
+  }
+  return 0;
+}
+
+// Pairs of CTAs pay with long K loops, full 256-row tiles and several rounds of them.  B200, one CTA / pairs: forward
+// 262,144 slots on 64 experts, 1024 -> 2048 853 / 821 us, its dx 878 / 766, its dW 950 / 842; 48,000 slots on 16 experts,
+// 512 -> 515 (8 K blocks; 5 or 3 row tiles of dW) forward 36 / 43 us, dW 49 / 55; 65,536 slots on 128 experts, 512 -> 256
+// (two tiles an expert) forward and sum 60 / 69 us.
+static bool xg_pairs(const XGemm& x) {
+  const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype);
+  const int64_t blocks = x.mode == XG_WGRAD ? rows / XG_BK : x.K / XG_BK;
+  const int64_t m = x.mode == XG_WGRAD ? x.M : rows, tiles = x.E * ((m + 255) / 256) * tn;
+  const int64_t waste = x.mode == XG_WGRAD ? (m + 255) / 256 * 256 - m : 128;
+  return blocks >= 16 && 8 * waste <= m && tiles >= 8 * (int64_t)(sm_count() / 2);
 }
 
 template <int MODE, typename T>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
-  if constexpr (MODE == XG_WGRAD)
-    if (x.split > 1) return xg_bn(x.N) == 128 ? xg_go<MODE, T, float, 128>(x, st) : xg_go<MODE, T, float, 256>(x, st);
-  return xg_bn(x.N) == 128 ? xg_go<MODE, T, T, 128>(x, st) : xg_go<MODE, T, T, 256>(x, st);
+  if constexpr (sizeof(T) == 4) {
+    return xg_go<MODE, T, 128, 1>(x, st);
+  } else {
+    if (xg_bn_max(x.N, x.dtype) == 128) return xg_go<MODE, T, 128, 1>(x, st);
+    return xg_pairs(x) ? xg_go<MODE, T, 256, 2>(x, st) : xg_go<MODE, T, 256, 1>(x, st);
+  }
 }
 
 template <int MODE>

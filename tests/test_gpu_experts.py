@@ -266,7 +266,8 @@ def test_route_refusals():
 
 # ------------------------------------------------------------------------------------------------ plan
 @pytest.mark.parametrize("T,k,E", [(0, 1, 3), (1, 1, 1), (5, 3, 2), (64, 8, 64), (1000, 2, 89), (8192, 1, 256), (8193, 1, 256),
-                                   (5000, 2, 1000), (30000, 4, 16)])
+                                   (5000, 2, 1000), (30000, 4, 16), (300000, 4, 20), (4097, 1, 3),
+                                   (1050000, 1, 7)])
 def test_plan_sorts_the_slots(T, k, E):
     g = _gen(T + E)
     ex = torch.randint(-1, E, (T, k), generator=g)
@@ -281,13 +282,16 @@ def test_plan_sorts_the_slots(T, k, E):
     assert int(words[0]) == int(seg[-1]) // 128
     o = 8
     assert torch.equal(words[o:o + E + 1].long(), seg)
+    pairs = [int(seg[e]) // 128 + 2 * i for e in range(E) for i in range((int(seg[e + 1] - seg[e]) // 128 + 1) // 2)]
+    assert int(words[2]) == len(pairs)
     assert torch.equal(words[o + E + 1:o + 2 * E + 1].long(), cnt)
     tiles = T * k // 128 + min(T * k, E)
-    o_order, o_tile, o_row = o + 2 * E + 1, o + 3 * E + 1, o + 3 * E + 1 + tiles
-    assert words[o_order:o_tile].tolist() == sorted(range(E), key=lambda e: (-int(cnt[e]), e))
+    o_order, o_tile, o_row = o + 2 * E + 1, o + 3 * E + 1, o + 3 * E + 1 + 2 * tiles
+    assert words[o_order:o_order + E].tolist() == sorted(range(E), key=lambda e: (-int(cnt[e]), e))
     rows = words[o_row:o_row + int(seg[-1])].long()
     want = torch.full((int(seg[-1]),), -1, dtype=torch.int64)
     flat = ex.reshape(-1)
+    assert words[o_tile + tiles:o_tile + tiles + len(pairs)].tolist() == pairs
     for e in range(E):
         s = torch.nonzero(flat == e)[:, 0]
         want[seg[e]:seg[e] + len(s)] = s          # stable
