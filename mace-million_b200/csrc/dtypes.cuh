@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mb {
@@ -81,6 +83,45 @@ __device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
   else
     *reinterpret_cast<uint4*>(p) = pack16<T>(f);
 }
+// Arithmetic on one element or on a packed pair (one instruction for both); roundings are explicit, nothing is contracted
+template <int V>
+using Elem = std::conditional_t<V == 1, float, float2>;
+template <int V>
+constexpr int kElems = V == 1 ? 1 : V / 2;
+__device__ __forceinline__ float e_add(float a, float b) { return __fadd_rn(a, b); }
+__device__ __forceinline__ float e_mul(float a, float b) { return __fmul_rn(a, b); }
+__device__ __forceinline__ float e_fma(float a, float b, float c) { return __fmaf_rn(a, b, c); }
+__device__ __forceinline__ float2 e_add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 e_mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 e_fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+template <typename E>
+__device__ __forceinline__ E e_splat(float v);
+template <>
+__device__ __forceinline__ float e_splat<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float2 e_splat<float2>(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float e_sum(float a) { return a; }
+__device__ __forceinline__ float e_sum(float2 a) { return a.x + a.y; }
+// V floats as elements and back
+template <int V>
+__device__ __forceinline__ void to_elems(const float (&f)[V], Elem<V> (&e)[kElems<V>]) {
+  if constexpr (V == 1) {
+    e[0] = f[0];
+  } else {
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q) e[q] = make_float2(f[2 * q], f[2 * q + 1]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void from_elems(const Elem<V> (&e)[kElems<V>], float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = e[0];
+  } else {
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q) f[2 * q] = e[q].x, f[2 * q + 1] = e[q].y;
+  }
+}
+
 // The same, kept as loaded until used: V elements of T in the fewest registers
 template <typename T, int V>
 struct Raw {

@@ -23,7 +23,7 @@ struct LnArgs {
   float eps;
 };
 
-// Sums of K values over the G threads of a group (all threads of the block call it; `red` holds
+// Sums of K (a power of two) values over the G threads of a group (all threads of the block call it; `red` holds
 // (threads / 32) * K floats and is free to be overwritten two calls later: callers alternate two buffers).
 template <int G, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
@@ -83,13 +83,15 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
         for (int k = 0; k < K; ++k) red[warp * K + k] = v[k];
     }
     __syncthreads();
-    const int w0 = warp / W * W;
+    // the group's W x K partial sums, one or more per lane, then over the warps by shuffles
+    const float* r = red + warp / W * W * K;
+    float t = lane < W * K ? r[lane] : 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = 0.f;
+    for (int o = 32; o < W * K; o += 32) t += r[o + lane];
 #pragma unroll
-    for (int q = 0; q < W; ++q)
+    for (int o = (W * K < 32 ? W * K : 32) / 2; o >= K; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += red[(w0 + q) * K + k];
+    for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, t, k);
   }
 }
 
@@ -101,8 +103,8 @@ constexpr int ln_threads = G < 256 ? 256 : G;
 #endif
 template <int G, int NV, int V>
 constexpr int ln_fwd_blocks = (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> > 0 ? (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> : 1;
-template <int G>
-constexpr int ln_bwd_blocks = G == 32 || G == 256 ? 3 : G < 256 ? 2 : 1;
+template <int G, int NV, int V>
+constexpr int ln_bwd_blocks = G > 256 ? 1 : NV * V > 4 ? 2 : 3;
 
 // The row is held as loaded (16-bit rows take half the registers of fp32 values) and unpacked at each use.
 template <typename T, typename P, int G, int NV, int V>
@@ -131,31 +133,51 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_fwd_blocks<G, NV, V>) k_ln_f
     const int64_t row = r0 + g;
     const bool live = row < a.n;
     const T* x = (const T*)a.x + (live ? row : 0) * a.ldx;
+    using E = Elem<V>;
+    constexpr int NE = kElems<V>;
     Raw<T, V> v[NV];
-    float s[1] = {0.f}, f[V];
+    float s[1], f[V];
+    E e[NE], acc[NE] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * G + t) * V;
       v[i].zero();
       if (live && j < d) v[i].load(x + j);
     }
+    auto fold = [&] {
+      E p = acc[0];
+#pragma unroll
+      for (int q = 1; q < NE; ++q) p = e_add(p, acc[q]);
+      s[0] = e_sum(p);
+    };
+#pragma unroll
+    for (int q = 0; q < NE; ++q) acc[q] = e_splat<E>(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       v[i].get(f);
+      to_elems<V>(f, e);
 #pragma unroll
-      for (int q = 0; q < V; ++q) s[0] += f[q];
+      for (int q = 0; q < NE; ++q) acc[q] = e_add(acc[q], e[q]);
     }
+    fold();
     group_sum<G, 1>(s, red[0]);
     const float mu = s[0] * inv;
-    s[0] = 0.f;
+    const E neg = e_splat<E>(-mu);
+#pragma unroll
+    for (int q = 0; q < NE; ++q) acc[q] = e_splat<E>(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * G + t) * V < d) {
         v[i].again();
         v[i].get(f);
+        to_elems<V>(f, e);
 #pragma unroll
-        for (int q = 0; q < V; ++q) s[0] += (f[q] - mu) * (f[q] - mu);
+        for (int q = 0; q < NE; ++q) {
+          const E c = e_add(e[q], neg);
+          acc[q] = e_fma(c, c, acc[q]);
+        }
       }
+    fold();
     group_sum<G, 1>(s, red[1]);
     const float r = rsqrtf(s[0] * inv + a.eps);
     if (!live) continue;
@@ -165,12 +187,16 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_fwd_blocks<G, NV, V>) k_ln_f
       const int j = (i * G + t) * V;
       if (j >= d) continue;
       float fw[V], fb[V];
+      E ew[NE], eb[NE];
       if constexpr (!KEEP) params(i, fw, fb);
+      to_elems<V>(KEEP ? pw[KEEP ? i : 0] : fw, ew);
+      to_elems<V>(KEEP ? pb[KEEP ? i : 0] : fb, eb);
       v[i].again();
       v[i].get(f);
+      to_elems<V>(f, e);
 #pragma unroll
-      for (int q = 0; q < V; ++q)
-        f[q] = KEEP ? fmaf((f[q] - mu) * r, pw[KEEP ? i : 0][q], pb[KEEP ? i : 0][q]) : fmaf((f[q] - mu) * r, fw[q], fb[q]);
+      for (int q = 0; q < NE; ++q) e[q] = e_fma(e_mul(e_add(e[q], neg), e_splat<E>(r)), ew[q], eb[q]);
+      from_elems<V>(e, f);
       store_v<T, V>(y + j, f);
     }
     if (t == 0 && a.mean) {
@@ -212,19 +238,25 @@ __global__ void __launch_bounds__(1024) k_ln_fwd_wide(const LnArgs a) {
 // partial[block][0 .. d) = sum of dy xh, [d .. 2 d) = sum of dy over the block's rows.  RB rows at a time with one
 // synchronisation, and the next RB rows' loads in flight meanwhile (PRE).
 template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
-__global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G>) k_ln_bwd(const LnArgs a) {
+__global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G, NV, V>) k_ln_bwd(const LnArgs a) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
   __shared__ float red[2][TH / 32 * 2 * RB];
   extern __shared__ float cols[];                 // [RPB][2][d] when RPB > 1
   const int t = threadIdx.x % G, g = threadIdx.x / G, d = a.d;
   const P* w = (const P*)a.w;
-  float pw[NV][V], aw[NV][V], ab[NV][V];
+  using E = Elem<V>;
+  constexpr int NE = kElems<V>;
+  E pw[NV][NE], aw[NV][NE], ab[NV][NE];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = (i * G + t) * V;
+    float f[V];
 #pragma unroll
-    for (int q = 0; q < V; ++q) pw[i][q] = 1.f, aw[i][q] = 0.f, ab[i][q] = 0.f;
-    if (w && j < d) load_p<P, V>(w + j, pw[i]);
+    for (int q = 0; q < V; ++q) f[q] = 1.f;
+    if (w && j < d) load_p<P, V>(w + j, f);
+    to_elems<V>(f, pw[i]);
+#pragma unroll
+    for (int q = 0; q < NE; ++q) aw[i][q] = ab[i][q] = e_splat<E>(0.f);
   }
   const float inv = 1.f / (float)d;
   Raw<T, V> xv[RB][NV], dv[RB][NV];
@@ -255,37 +287,46 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G>) k_ln_bwd(cons
   if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB * RB);
   for (int64_t r0 = (int64_t)blockIdx.x * RPB * RB; r0 < a.n; r0 += step, buf ^= 1) {
     if constexpr (!PRE) fetch(r0);
-    Raw<T, V> xc[RB][NV], dc[RB][NV];
-    float rc[RB], mc[RB], s[2 * RB];
+    // xh and up = dy w stay in registers between the sums and dx
+    E xh[RB][NV][NE], up[RB][NV][NE];
+    float rc[RB], s[2 * RB];
 #pragma unroll
     for (int k = 0; k < RB; ++k) {
       rc[k] = rs[k];
-      mc[k] = mu[k];
+      const E neg = e_splat<E>(-mu[k]), r = e_splat<E>(rs[k]);
+      E s1[NE], s2[NE];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) xc[k][i] = xv[k][i], dc[k][i] = dv[k][i];
+      for (int q = 0; q < NE; ++q) s1[q] = s2[q] = e_splat<E>(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = (i * G + t) * V < d;
+        float f[V];
+        E dy[NE];
+        xv[k][i].get(f);
+        to_elems<V>(f, xh[k][i]);
+        dv[k][i].get(f);
+        to_elems<V>(f, dy);
+#pragma unroll
+        for (int q = 0; q < NE; ++q) {
+          // dy is 0 beyond the width, so nothing there reaches a sum; x - mu could be anything finite
+          xh[k][i][q] = e_mul(e_add(xh[k][i][q], neg), r);
+          up[k][i][q] = e_mul(dy[q], pw[i][q]);
+          s1[q] = e_add(s1[q], up[k][i][q]);
+          if (in) {
+            s2[q] = e_fma(up[k][i][q], xh[k][i][q], s2[q]);
+            aw[i][q] = e_fma(dy[q], xh[k][i][q], aw[i][q]);
+          }
+          ab[i][q] = e_add(ab[i][q], dy[q]);
+        }
+      }
+      E p1 = s1[0], p2 = s2[0];
+#pragma unroll
+      for (int q = 1; q < NE; ++q) p1 = e_add(p1, s1[q]), p2 = e_add(p2, s2[q]);
+      s[2 * k] = e_sum(p1);
+      s[2 * k + 1] = e_sum(p2);
     }
     if constexpr (PRE)
       if (r0 + step < a.n) fetch(r0 + step);
-#pragma unroll
-    for (int k = 0; k < RB; ++k) {
-      s[2 * k] = s[2 * k + 1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if ((i * G + t) * V >= d) continue;
-        float fx[V], fd[V];
-        xc[k][i].get(fx);
-        dc[k][i].get(fd);
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          const float xh = (fx[q] - mc[k]) * rc[k];
-          const float up = __fmul_rn(fd[q], pw[i][q]);   // the same rounding here and below: dx of a constant is 0
-          s[2 * k] += up;
-          s[2 * k + 1] += up * xh;
-          aw[i][q] += fd[q] * xh;
-          ab[i][q] += fd[q];
-        }
-      }
-    }
     group_sum<G, 2 * RB>(s, red[buf]);
     if (a.dx) {
 #pragma unroll
@@ -293,22 +334,17 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G>) k_ln_bwd(cons
         const int64_t row = r0 + g * RB + k;
         if (row >= a.n) continue;
         T* dx = (T*)a.dx + row * d;
-        const float m1 = s[2 * k] * inv, m2 = s[2 * k + 1] * inv;
+        const E m1 = e_splat<E>(-s[2 * k] * inv), m2 = e_splat<E>(-s[2 * k + 1] * inv), r = e_splat<E>(rc[k]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int j = (i * G + t) * V;
           if (j >= d) continue;
-          float fx[V], fd[V];
-          xc[k][i].again();
-          dc[k][i].again();
-          xc[k][i].get(fx);
-          dc[k][i].get(fd);
+          float f[V];
 #pragma unroll
-          for (int q = 0; q < V; ++q) {
-            const float xh = (fx[q] - mc[k]) * rc[k];
-            fx[q] = rc[k] * (__fmul_rn(fd[q], pw[i][q]) - m1 - xh * m2);
-          }
-          store_v<T, V>(dx + j, fx);
+          for (int q = 0; q < NE; ++q)
+            up[k][i][q] = e_mul(r, e_fma(xh[k][i][q], m2, e_add(up[k][i][q], m1)));
+          from_elems<V>(up[k][i], f);
+          store_v<T, V>(dx + j, f);
         }
       }
     }
@@ -317,26 +353,34 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G>) k_ln_bwd(cons
   float* out = a.partial + (int64_t)blockIdx.x * 2 * d;
   if constexpr (RPB == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float fw[V], fb[V];
+      from_elems<V>(aw[i], fw);
+      from_elems<V>(ab[i], fb);
 #pragma unroll
       for (int q = 0; q < V; ++q) {
         const int j = (i * G + t) * V + q;
         if (j < d) {
-          out[j] = aw[i][q];
-          out[d + j] = ab[i][q];
+          out[j] = fw[q];
+          out[d + j] = fb[q];
         }
       }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float fw[V], fb[V];
+      from_elems<V>(aw[i], fw);
+      from_elems<V>(ab[i], fb);
 #pragma unroll
       for (int q = 0; q < V; ++q) {
         const int j = (i * G + t) * V + q;
         if (j < d) {
-          cols[(2 * g) * d + j] = aw[i][q];
-          cols[(2 * g + 1) * d + j] = ab[i][q];
+          cols[(2 * g) * d + j] = fw[q];
+          cols[(2 * g + 1) * d + j] = fb[q];
         }
       }
+    }
     __syncthreads();
     for (int j = threadIdx.x; j < 2 * d; j += TH) {
       float s = 0.f;
@@ -439,6 +483,7 @@ static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
     if (a.d <= 640) return ln_fwd_launch<T, P, 128, 5, 1>(a, st);
     if (a.d <= 1024) return ln_fwd_launch<T, P, 128, 8, 1>(a, st);
     if (a.d <= 2048) return ln_fwd_launch<T, P, 256, 8, 1>(a, st);
+    if (a.d <= 4096) return ln_fwd_launch<T, P, 512, 8, 1>(a, st);
     if (a.d <= 8192) return ln_fwd_launch<T, P, 1024, 8, 1>(a, st);
   }
   const int64_t most = (int64_t)2 * sm_count();
@@ -450,7 +495,7 @@ static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
 template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
 static int ln_bwd_launch(const LnArgs& a, int* nb, cudaStream_t st) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
-  const int64_t want = (a.n + RPB * RB - 1) / (RPB * RB), most = (int64_t)ln_bwd_blocks<G> * sm_count();
+  const int64_t want = (a.n + RPB * RB - 1) / (RPB * RB), most = (int64_t)ln_bwd_blocks<G, NV, V> * sm_count();
   *nb = (int)(want < most ? want : most);
   const int smem = RPB > 1 && a.partial ? RPB * 2 * a.d * 4 : 0;
   static_assert(RPB == 1 || RPB * 2 * G * NV * V * 4 <= 40 * 1024, "column sums in shared memory");
@@ -475,7 +520,7 @@ static int ln_bwd_any(const LnArgs& a, bool vec, int* nb, cudaStream_t st) {
     if (a.d <= 640) return ln_bwd_launch<T, P, 128, 5, 1, 2, true>(a, nb, st);
     if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 2, true>(a, nb, st);
     if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 2, true>(a, nb, st);
-    if (a.d <= 4096) return ln_bwd_launch<T, P, 1024, 4, 1, 2, true>(a, nb, st);
+    if (a.d <= 4096) return ln_bwd_launch<T, P, 512, 8, 1, 1, true>(a, nb, st);
   }
   const int64_t most = (int64_t)2 * sm_count();
   *nb = (int)(a.n < 64 ? a.n : 64);

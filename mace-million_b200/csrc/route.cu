@@ -35,10 +35,10 @@ struct RouteArgs {
   float scale;
 };
 
-// float -> uint32 with the same order: -0 equals +0, NaN is above +inf, and -inf is 0 (closed)
+// float -> uint32 with the same order: -0 equals +0, NaN is above +inf; -inf (closed) is KEY_CLOSED, and so is 0
+constexpr unsigned KEY_CLOSED = 0x007FFFFFu;
 __device__ __forceinline__ unsigned order_key(float f) {
   if (f != f) return 0xFFFFFFFFu;
-  if (f == -INFINITY) return 0u;
   const unsigned u = __float_as_uint(f + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
@@ -72,7 +72,7 @@ __device__ __forceinline__ int lanes_first(bool p, int base) {
 }
 
 template <typename T, int L, int NE>
-__global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) {
+__global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs a) {
   constexpr int TPW = 32 / L;                     // tokens per warp
   extern __shared__ unsigned char sm_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (L - 1), base = lane & ~(L - 1);
@@ -83,10 +83,6 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
   const int per = a.e / a.groups;
   // a group's experts lie in the registers of a power of two of lanes: its best two by shuffles, else through `val`
   const int span = a.groups > 1 && per % c == 0 && ((per / c) & (per / c - 1)) == 0 ? per / c : 0;
-  float b[NE];
-  if (a.bias)
-#pragma unroll
-    for (int j = 0; j < NE; ++j) b[j] = j < n ? a.bias[i0 + j] : 0.f;
   const int64_t step = (int64_t)gridDim.x * RT_WARPS * TPW;
   // every lane of a warp runs the same number of passes (the collectives are warp-wide)
   for (int64_t r0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * TPW; r0 < a.t; r0 += step) {
@@ -141,7 +137,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
       }
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
-        if (a.bias) s[j] += b[j];
+        if (a.bias && j < n) s[j] += a.bias[i0 + j];
         if (l[j] == -INFINITY) s[j] = -INFINITY;  // closed
         key[j] = order_key(a.bias ? s[j] : l[j]);
       }
@@ -168,7 +164,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
           for (int q = 0; q < a.top_groups; ++q) {
             const unsigned best = lanes_max<L>(gk);
             const int g = lanes_first<L>(gk == best, base) / span;
-            if (best == 0u) continue;             // nothing open is left for this token
+            if (best <= KEY_CLOSED) continue;     // nothing open is left for this token
             open |= 1u << g;
             if (g == mine) gk = 0u;
           }
@@ -190,6 +186,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
             if (g < a.groups) {
               float m1 = -INFINITY, m2 = -INFINITY;
               bool nan = false;
+#pragma unroll 4
               for (int i = 0; i < per; ++i) {
                 const float f = val[g * per + i];
                 nan |= f != f;
@@ -212,7 +209,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
               const int f = lanes_first<L>(gk[u] == best, base);
               if (f < 32) g = f + u * L;
             }
-            if (best == 0u) continue;
+            if (best <= KEY_CLOSED) continue;
             open |= 1u << g;
 #pragma unroll
             for (int u = 0; u < GL; ++u)
@@ -225,18 +222,25 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_route_fwd(const RouteArgs a) 
       }
     }
     for (int q = 0; q < a.k; ++q) {
-      unsigned mx = 0u;
-      int at = 0;
+      unsigned t[NE];                             // the lane's best, as a tree
 #pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (key[j] > mx) mx = key[j], at = j;
-      const unsigned best = lanes_max<L>(mx);
-      const int first = lanes_first<L>(mx == best, base);
+      for (int j = 0; j < NE; ++j) t[j] = key[j];
+#pragma unroll
+      for (int w = NE; w > 1; w = (w + 1) / 2)
+#pragma unroll
+        for (int j = 0; j < w / 2; ++j) t[j] = max(t[j], t[j + (w + 1) / 2]);
+      const unsigned best = lanes_max<L>(t[0]);
+      const int first = lanes_first<L>(t[0] == best, base);
       if (sub == first) {
-        chosen[q] = best ? i0 + at : -1;
+        bool left = true;
+        int at = 0;
 #pragma unroll
-        for (int j = 0; j < NE; ++j)
-          if (j == at) key[j] = 0u;
+        for (int j = 0; j < NE; ++j) {            // the first of the lane's keys that has it
+          const bool hit = left && key[j] == best;
+          left = left && key[j] != best;
+          if (hit) key[j] = 0u, at = j;
+        }
+        chosen[q] = best > KEY_CLOSED ? i0 + at : -1;
       }
     }
     __syncwarp();

@@ -27,12 +27,22 @@ FEW_BYTES = 96 << 20
 FEW_SLOTS = 4096
 
 
+_OPS = {}
+
+
+def _op(name):
+    """The op's only overload (looked up once: resolving it again costs a small call a microsecond)."""
+    if name not in _OPS:
+        _OPS[name] = getattr(N.ops(), name).default
+    return _OPS[name]
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [.., D].
 
     x: float32, bfloat16 or float16; its rows may be strided.  weight / bias: [D] of the type of x or float32, or None.
     Statistics and parameter gradients are accumulated in fp32, in a fixed order."""
-    return N.ops().layer_norm(x, weight, bias, float(eps))
+    return _op("layer_norm")(x, weight, bias, float(eps))
 
 
 def route(logits, k, *, bias=None, score="softmax", groups=1, top_groups=1, renormalize=True, scale=1.0):
@@ -47,8 +57,8 @@ def route(logits, k, *, bias=None, score="softmax", groups=1, top_groups=1, reno
     `scale`.  Differentiable w.r.t. the logits."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"score must be 'softmax' or 'sigmoid' (got {score!r})")
-    return N.ops().route(logits, bias, int(k), score == "softmax", int(groups), int(top_groups), bool(renormalize),
-                         float(scale))
+    return _op("route")(logits, bias, int(k), score == "softmax", int(groups), int(top_groups), bool(renormalize),
+                        float(scale))
 
 
 class ExpertPlan:
@@ -68,7 +78,7 @@ class ExpertPlan:
     def words(self):
         """The plan as the kernels read it (int32)."""
         if self._words is None:
-            self._words = N.ops().expert_plan(self.experts, self.n_experts)
+            self._words = _op("expert_plan")(self.experts, self.n_experts)
         return self._words
 
     def check(self):
@@ -100,4 +110,4 @@ def expert_linear(x, w, plan, weights=None):
                                         (weights is not None and weights.requires_grad))
     slots = plan.experts.numel()
     few = not grad and slots <= FEW_SLOTS and slots * w[0].numel() * w.element_size() <= FEW_BYTES
-    return N.ops().expert_linear(x, w, plan.experts, None if few else plan.words, weights)
+    return _op("expert_linear")(x, w, plan.experts, None if few else plan.words, weights)
