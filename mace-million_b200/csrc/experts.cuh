@@ -54,7 +54,7 @@ struct XGemm {
   int32_t kc;                                    // WGRAD: K blocks of a part (xgemm_kc)
   float* parts;                                  // WGRAD: xgemm_parts partial sums [M][N] (null: there are none)
   int32_t* pre;                                  // WGRAD with parts: [E + 1] scratch
-  // DGRAD: dgpart[n tile][slot] = partial <x, C> of the slot's x row (null: off)
+  // DGRAD: dgpart[2 x n tile + half][slot] = partial <x, C> of the slot's x row (null: off)
   const void* x;
   int64_t ldx;
   int32_t kdiv;                                  // slot / kdiv = row of x

@@ -4,12 +4,16 @@
 //   WGRAD  C[e][o][d] = sum over e's rows dy[row][o] x[row][d]   both MN-major, K = the expert's rows
 // Rows are sorted by expert and padded to 128, so a 128-row tile (FWD, DGRAD) or a 64-row K block (WGRAD) has one expert,
 // and no matrix is transposed in memory: the MN-major operands are read as they lie.
-// fp32 data comes as three bf16 planes; a stage holds all three of both operands, and the products of the planes whose
-// ranks add up to at most 2 (six of nine, small ones first) go to the same fp32 accumulator; the rest is below 2^-24 of
+// fp32 data comes as three bf16 planes; a stage holds all three of both operands.  The product of the first planes has an
+// accumulator of its own, and the five others whose ranks add up to at most 2 share another; the rest is below 2^-24 of
 // the result.
+// The tensor cores truncate when they add to an fp32 accumulator: the result shrinks by about 1.7e-8 of itself for each
+// 16-wide step (measured: 3.2e-6 after 192 steps, 4.7e-7 after 32).  Where the result leaves in fp32 (fp32 data, and the
+// gradient of the weights) an accumulator therefore takes XG_ACC_K K blocks at most, and the chunks are added in registers
+// with rounding to nearest; 16-bit results are rounded a thousand times more coarsely and take the whole K.
 //
 // Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
-// into one of two TMEM accumulators, warps 2-5 drain the other one.  CG = 2: a cluster of two CTAs works on a 256-row tile
+// into one of two TMEM accumulators, warps 2-9 drain the other one (a lane holds half a row).  CG = 2: a cluster of two CTAs works on a 256-row tile
 // (cta_group::2, each CTA holds its 128 rows of A and half of B's columns), which halves the B bytes a CTA fetches.
 // The N tile is the smallest multiple of 64 that cuts N into ceil(N / 256) tiles.
 // WGRAD cuts an expert's rows into parts of kc K blocks when there are few tiles; parts of an expert with several are
@@ -26,9 +30,10 @@
 
 namespace mb {
 
-constexpr int XG_BM = XP_BM, XG_BK = 64, XG_THREADS = 192;
+constexpr int XG_BM = XP_BM, XG_BK = 64, XG_EPI_WARPS = 8, XG_THREADS = 64 + 32 * XG_EPI_WARPS;
 constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
-constexpr int XG_STG = 4096;                     // row staging of one epilogue warp
+constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
+constexpr int XG_ACC_K = 8;                      // K blocks of an accumulator whose result leaves in fp32
 
 // T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for
 template <typename T, int BN, int CG>
@@ -37,10 +42,11 @@ struct XgCfg {
   static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN / CG * XG_BK * 2;
   static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
   static constexpr int STAGES = 196608 / STAGE;
-  static constexpr int TMEM = 2 * BN;
+  static constexpr int ACC = PL == 3 ? 2 * BN : BN;          // TMEM columns of an accumulator (fp32: both of them)
+  static constexpr int TMEM = 2 * ACC;
   static constexpr int PRE = 4352;                           // [E + 1] first item of each expert (WGRAD)
-  static constexpr int SMEM = STAGES * STAGE + 4 * XG_STG + PRE + 256 + 1024;   // + barriers, alignment slack
-  static_assert(STAGES >= 2 && STAGES <= 8 && SMEM <= 227 * 1024 && PRE >= 4 * (MB_PLAN_MAX_EXPERTS + 1), "shared memory");
+  static constexpr int SMEM = STAGES * STAGE + XG_EPI_WARPS * XG_STG + PRE + 256 + 1024;   // + barriers, alignment slack
+  static_assert(STAGES >= 2 && STAGES <= 8 && SMEM <= 227 * 1024 && TMEM <= 512 && PRE >= 4 * (MB_PLAN_MAX_EXPERTS + 1), "shared memory");
 };
 
 struct XgParams {
@@ -71,114 +77,95 @@ struct XgTile {
   bool rows_ok;                                  // FWD / DGRAD: this CTA's rows belong to the expert
 };
 
-// Row staging of the epilogue: a warp's 32 rows x 128 bytes, 16-byte piece c of row r at piece c ^ (r % 8), so that a lane's
-// access to its own row and the warp's access to four whole row segments are both free of bank conflicts.
+// Row staging of the epilogue: a warp's 32 rows x 64 bytes, 16-byte piece c of row r at piece c ^ (r / 2 % 4), so that a
+// lane's access to its own row and the warp's access to eight whole row segments are both free of bank conflicts.
 __device__ __forceinline__ uint4* xg_stg(unsigned char* stg, int row, int c) {
-  return reinterpret_cast<uint4*>(stg + row * 128 + ((c ^ (row & 7)) << 4));
+  return reinterpret_cast<uint4*>(stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
 
-// Drains one accumulator: one row per lane out of TMEM, scaled, through shared memory in pieces of 128 bytes, so that
-// global accesses are whole 128-byte segments of four rows (one row per lane would be 32 scattered 16-byte pieces per
-// access, and held a tile for longer than its products at K <= 1024).  dst: this lane's row (null: not stored);
-// xr: the row of x that `dot` takes the scalar product with (DOT).
+// Writes 64 columns of the rows that the lanes of a warp hold (v, one row per lane, nc columns of it in use), scaled, through shared memory
+// in pieces of 64 bytes: global accesses are whole sectors of eight rows (one row per lane would be 32 scattered 16-byte
+// pieces per access, and held a tile for longer than its products at K <= 1024).  dst: this lane's row (null: not stored);
+// DOT: returns the scalar product of the row with that of x at xr.
 template <typename OUT, typename T, bool DOT>
-__device__ __forceinline__ float xg_drain(uint32_t tacc, bool zero, unsigned char* stg, OUT* dst, bool vec, float sc, int nc,
-                                          const T* xr, bool xvec, uint64_t* wait_bar, uint32_t wait_par, bool& ok) {
-  constexpr int NC = 128 / (int)sizeof(OUT);     // columns of a piece
-  constexpr int XV = kVec<T>;
-  const int lane = threadIdx.x & 31;
-  const int r8 = lane >> 3, c8 = lane & 7;       // this lane's row (of four) and 16-byte piece in whole-segment accesses
+__device__ __forceinline__ float xg_emit(const float (&v)[64], unsigned char* stg, OUT* dst, bool vec, float sc, int nc,
+                                         const T* xr, bool xvec) {
+  constexpr int NC = 64 / (int)sizeof(OUT), OV = kVec<OUT>, XV = kVec<T>;   // columns of a piece, of a vector
+  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
+  const bool any = __any_sync(0xffffffffu, dst != nullptr);
   float dot = 0.f;
-  // the x rows' pieces are loaded one piece ahead, the first before the accumulator is waited for
-  uint4 xq[DOT ? 8 : 1];
+  uint4 xq[DOT ? 4 : 1];                         // the x rows' next piece
   auto fetch_x = [&](int h) {
-    const int n = nc - h * NC < NC ? nc - h * NC : NC;
 #pragma unroll
-    for (int i = 0; i < (DOT ? 8 : 0); ++i) {
-      const T* xp = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 4 * i + r8));
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (xp) {
-        xp += h * NC + c8 * XV;
-        if (xvec && (c8 + 1) * XV <= n) {
-          v = *reinterpret_cast<const uint4*>(xp);
+    for (int i = 0; i < (DOT ? 4 : 0); ++i) {
+      const T* xp = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 8 * i + r4));
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      const int left = nc - h * NC - c4 * XV;
+      if (xp && left > 0) {
+        xp += h * NC + c4 * XV;
+        if (xvec && left >= XV) {
+          u = *reinterpret_cast<const uint4*>(xp);
         } else {
           float f[XV];
 #pragma unroll
-          for (int q = 0; q < XV; ++q) f[q] = c8 * XV + q < n ? to_f(xp[q]) : 0.f;
-          v = pack16<T>(f);
+          for (int q = 0; q < XV; ++q) f[q] = q < left ? to_f(xp[q]) : 0.f;
+          u = pack16<T>(f);
         }
       }
-      xq[i] = v;
+      xq[i] = u;
     }
   };
   if (DOT) fetch_x(0);
-  if (!zero) {
-    ok = __all_sync(0xffffffffu, mbar_wait_ns(wait_bar, wait_par, XG_WAIT_NS));
-    if (!ok) return 0.f;
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  }
-#pragma unroll 1
-  for (int h = 0; h * NC < nc; ++h) {
-    const int n = nc - h * NC < NC ? nc - h * NC : NC;
-    uint32_t u[NC];
-    if (!zero) {
 #pragma unroll
-      for (int q = 0; q < NC / 32; ++q) tmem_ld32(tacc + NC * h + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * q));
-      tmem_wait_ld();
-    } else {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) u[i] = 0u;
-    }
+  for (int h = 0; h < 64 / NC; ++h) {
+    if (h * NC >= nc) break;
     if constexpr (DOT) {
-      // a piece of 128 bytes of x holds as many columns as one of the output: T = OUT here
+      // a piece of x holds as many columns as one of the output: T = OUT here
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *xg_stg(stg, 4 * i + r8, c8) = xq[i];
+      for (int i = 0; i < 4; ++i) *xg_stg(stg, 8 * i + r4, c4) = xq[i];
       if ((h + 1) * NC < nc) fetch_x(h + 1);
       __syncwarp();
-      // one short chain per vector, added up as a tree: the rounding of 256 terms in a row would show
-      float part[8];
+      float part[4];                             // short chains, added up as a tree
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < 4; ++c) {
         float f[XV];
         unpack16(*xg_stg(stg, lane, c), f, T());
         part[c] = 0.f;
 #pragma unroll
-        for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], __uint_as_float(u[c * XV + q]), part[c]);
+        for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], v[h * NC + c * XV + q], part[c]);
       }
-      dot += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+      dot += (part[0] + part[1]) + (part[2] + part[3]);
       __syncwarp();
     }
-    if (!__any_sync(0xffffffffu, dst != nullptr)) continue;
+    if (!any) continue;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      float f[kVec<OUT>];
+    for (int c = 0; c < 4; ++c) {
+      float f[OV];
 #pragma unroll
-      for (int q = 0; q < kVec<OUT>; ++q) f[q] = __uint_as_float(u[c * kVec<OUT> + q]) * sc;
+      for (int q = 0; q < OV; ++q) f[q] = v[h * NC + c * OV + q] * sc;
       *xg_stg(stg, lane, c) = pack16<OUT>(f);
     }
     __syncwarp();
     if (vec) {
-      const int left = n - c8 * kVec<OUT>;       // columns of this lane's piece
+      const int left = nc - h * NC - c4 * OV;    // columns of this lane's piece
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 4 * i + r8));
+      for (int i = 0; i < 4; ++i) {
+        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 8 * i + r4));
         if (!p || left <= 0) continue;
-        p += h * NC + c8 * kVec<OUT>;
-        const uint4* s = xg_stg(stg, 4 * i + r8, c8);
-        if (left >= kVec<OUT>)
+        p += h * NC + c4 * OV;
+        const uint4* s = xg_stg(stg, 8 * i + r4, c4);
+        if (left >= OV)
           *reinterpret_cast<uint4*>(p) = *s;
         else
           for (int q = 0; q < left; ++q) p[q] = reinterpret_cast<const OUT*>(s)[q];
       }
-    } else {                                     // odd strides: one row at a time, lanes along it
+    } else {                                     // odd strides: one row at a time (two of 16 columns), lanes along it
+      constexpr int RP = 32 / NC;
 #pragma unroll 4
-      for (int r = 0; r < 32; ++r) {
-        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), r));
-#pragma unroll
-        for (int q = 0; q < NC / 32; ++q) {
-          const int c = lane + 32 * q;
-          if (p && c < n) p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, r, c / kVec<OUT>))[c % kVec<OUT>];
-        }
+      for (int r = 0; r < 32; r += RP) {
+        const int rr = r + lane / NC, c = lane % NC;
+        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), rr));
+        if (p && h * NC + c < nc) p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, rr, c / OV))[c % OV];
       }
     }
     __syncwarp();
@@ -194,8 +181,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* stg0 = smem + C::STAGES * C::STAGE;
-  int* pre = reinterpret_cast<int*>(stg0 + 4 * XG_STG);
-  XgBars& B = *reinterpret_cast<XgBars*>(stg0 + 4 * XG_STG + C::PRE);
+  int* pre = reinterpret_cast<int*>(stg0 + XG_EPI_WARPS * XG_STG);
+  XgBars& B = *reinterpret_cast<XgBars*>(stg0 + XG_EPI_WARPS * XG_STG + C::PRE);
   volatile int* failed = &B.failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CG == 2 ? (int)cluster_ctarank() : 0, cta = blockIdx.x / CG, ctas = gridDim.x / CG;
@@ -210,7 +197,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       }
       for (int a = 0; a < 2; ++a) {
         mbar_init(&B.acc_full[a], 1);
-        mbar_init(&B.acc_empty[a], 128 * CG);
+        mbar_init(&B.acc_empty[a], 32 * XG_EPI_WARPS * CG);
       }
       B.failed = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -281,6 +268,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     return o;
   };
   const int bh = g.bn / CG;                      // columns of B that this CTA loads
+  // K blocks of one accumulator
+  const int acc_k = sizeof(T) == 4 || (MODE == XG_DGRAD && g.dgpart) ? XG_ACC_K : 0x7fffffff;
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------ loads
@@ -344,101 +333,172 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         const int t = tile_at(r);
         if (t >= tiles) break;
         const int nk = tile_of(t).nk;
-        if (nk == 0) continue;
-        const int acc = tc & 1;
-        if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, XG_WAIT_NS)) {
-          *failed = 1;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d = tmem + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < nk; ++kb, ++seq) {
-          const int s = seq % C::STAGES;
-          if (!mbar_wait_ns(&B.full[s], (seq / C::STAGES) & 1, XG_WAIT_NS)) {
+        for (int kb0 = 0; ok && kb0 < nk; kb0 += acc_k < nk ? acc_k : nk, ++tc) {
+          const int acc = tc & 1, kb1 = nk - kb0 > acc_k ? kb0 + acc_k : nk;
+          if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, XG_WAIT_NS)) {
             *failed = 1;
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a0 = smem_u32(smem + s * C::STAGE), b0 = a0 + C::PL * C::A_BYTES;
-#pragma unroll
-          for (int p = 0; p < (C::PL == 3 ? 6 : 1); ++p) {
-            // planes (a, b): (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-            constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
-            const uint32_t a = a0 + (C::PL == 3 ? PA[p] * C::A_BYTES : 0), b = b0 + (C::PL == 3 ? PB[p] * C::B_BYTES : 0);
-#pragma unroll
-            for (int kk = 0; kk < XG_BK / 16; ++kk) {
-              // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
-              const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
-              const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
-              mma_f16_ss<CG>(d, ad, bd, idesc, (kb > 0 || kk > 0 || p > 0) ? 1u : 0u);
+          const uint32_t d = tmem + (uint32_t)(acc * C::ACC);
+          for (int kb = kb0; kb < kb1; ++kb, ++seq) {
+            const int s = seq % C::STAGES;
+            if (!mbar_wait_ns(&B.full[s], (seq / C::STAGES) & 1, XG_WAIT_NS)) {
+              *failed = 1;
+              ok = false;
+              break;
             }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t a0 = smem_u32(smem + s * C::STAGE), b0 = a0 + C::PL * C::A_BYTES;
+#pragma unroll
+            for (int p = 0; p < (C::PL == 3 ? 6 : 1); ++p) {
+              // planes (a, b): (0,2) (2,0) (1,1) (0,1) (1,0), then (0,0) in the other accumulator
+              constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
+              const uint32_t a = a0 + (C::PL == 3 ? PA[p] * C::A_BYTES : 0), b = b0 + (C::PL == 3 ? PB[p] * C::B_BYTES : 0);
+              const uint32_t dp = C::PL == 3 && p < 5 ? d + BN : d;
+#pragma unroll
+              for (int kk = 0; kk < XG_BK / 16; ++kk) {
+                // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
+                const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
+                const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
+                mma_f16_ss<CG>(dp, ad, bd, idesc, (kb > kb0 || kk > 0 || (p > 0 && p < 5)) ? 1u : 0u);
+              }
+            }
+            mma_commit_to<CG>(&B.empty[s]);
+            last_bar = &B.empty[s];
+            last_par = (seq / C::STAGES) & 1;
           }
-          mma_commit_to<CG>(&B.empty[s]);
-          last_bar = &B.empty[s];
-          last_par = (seq / C::STAGES) & 1;
+          if (!ok) break;
+          mma_commit_to<CG>(&B.acc_full[acc]);
+          last_bar = &B.acc_full[acc];
+          last_par = (tc >> 1) & 1;
         }
-        if (!ok) break;
-        mma_commit_to<CG>(&B.acc_full[acc]);
-        last_bar = &B.acc_full[acc];
-        last_par = (tc >> 1) & 1;
-        ++tc;
       }
       // after a timeout: wait (bounded) for the MMAs already issued before the TMEM is freed
       if (*failed && last_bar) mbar_wait_ns(last_bar, last_par, XG_WAIT_NS);
     }
   } else {
     // ------------------------------------------------------------------------------------------ epilogue
-    const int q4 = warp & 3, row = q4 * 32 + lane;
+    // warp w reads TMEM lanes 32 (w % 4) .., one row per lane, and the first or second half of the tile's columns
+    const int q4 = warp & 3, row = q4 * 32 + lane, hf = (warp - 2) >> 2, hw = g.bn / 2;
     unsigned char* stg = stg0 + (warp - 2) * XG_STG;
-    const bool out16 = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-    const bool vec = g.ldo % kVec<T> == 0 && out16;
+    const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
     const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
+    constexpr int NS = BN / 128;                   // pieces of 64 columns of a half row
+    constexpr bool CHUNKS = sizeof(T) == 4 || MODE == XG_DGRAD;   // K may be cut (acc_k)
     int tc = 0;
+    bool ok = true;
     // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
-    for (int r = 0; r < rounds; ++r) {
-      if (__shfl_sync(0xffffffffu, *failed, 0)) break;
+    for (int r = 0; ok && r < rounds; ++r) {
       const int t = tile_at(r);
       if (t >= tiles) break;
       const XgTile w = tile_of(t);
-      const int acc = tc & 1, nc = g.N - w.n0 < g.bn ? g.N - w.n0 : g.bn;
-      const uint32_t tacc = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN);
-      uint64_t* bar = &B.acc_full[acc];
-      const uint32_t par = (tc >> 1) & 1;
-      bool ok = true;
-      if constexpr (MODE == XG_WGRAD) {
-        const bool in = w.m0 + row < g.M;
-        if (w.part >= 0) {
-          float* dst = in ? g.parts + ((int64_t)w.part * g.M + w.m0 + row) * g.N + w.n0 : nullptr;
-          xg_drain<float, T, false>(tacc, w.nk == 0, stg, dst, g.N % 4 == 0, 1.f, nc, nullptr, false, bar, par, ok);
-        } else {
-          T* dst = in ? (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo + w.n0 : nullptr;
-          xg_drain<T, T, false>(tacc, w.nk == 0, stg, dst, vec, 1.f, nc, nullptr, false, bar, par, ok);
-        }
-      } else {
-        const int slot = w.rows_ok ? plan[g.lay.o_row + w.m0 + row] : -1;
-        T* dst = slot >= 0 && g.out ? (T*)g.out + (int64_t)slot * g.ldo + w.n0 : nullptr;
-        const float sc = slot >= 0 && g.scale ? g.scale[slot] : 1.f;
-        if (MODE == XG_DGRAD && g.dgpart) {
-          const T* xr = slot >= 0 ? (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + w.n0 : nullptr;
-          const float dot = xg_drain<T, T, true>(tacc, false, stg, dst, vec, sc, nc, xr, xvec, bar, par, ok);
-          if (ok && slot >= 0) g.dgpart[(int64_t)(w.n0 / g.bn) * g.lay.R + slot] = dot;
-        } else {
-          xg_drain<T, T, false>(tacc, false, stg, dst, vec, sc, nc, nullptr, false, bar, par, ok);
-        }
+      const int n0 = w.n0 + hf * hw, nc = g.N - n0 < hw ? g.N - n0 : hw;   // nc <= 0: nothing in this half
+      int slot = -1;
+      float sc = 1.f, dot = 0.f;
+      if constexpr (MODE != XG_WGRAD) {          // in flight during the wait
+        slot = w.rows_ok ? plan[g.lay.o_row + w.m0 + row] : -1;
+        if (slot >= 0 && g.scale) sc = g.scale[slot];
       }
-      if (!ok) {
-        *failed = 1;
-        break;
-      }
-      if (w.nk > 0) {
+      auto wait = [&](int acc) {
+        const bool got = !__shfl_sync(0xffffffffu, *failed, 0) &&
+                         __all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS));
+        if (!got) *failed = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return got;
+      };
+      auto release = [&](int acc) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         if constexpr (CG == 2)
           mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
         else
           mbar_arrive(&B.acc_empty[acc]);
-        ++tc;
+      };
+      auto add64 = [&](int acc, int q0, float (&v)[64]) {    // v += columns [64 q0, + 64) of the half row
+        const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * C::ACC + hf * hw + 64 * q0);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (64 * q0 + 32 * q < nc) {
+            uint32_t u[32];
+            tmem_ld32(ta + 32 * q, u);
+            if constexpr (C::PL == 3) {
+              uint32_t u2[32];
+              tmem_ld32(ta + BN + 32 * q, u2);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[32 * q + i] += __uint_as_float(u[i]) + __uint_as_float(u2[i]);
+            } else {
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[32 * q + i] += __uint_as_float(u[i]);
+            }
+          }
+      };
+      auto emit64 = [&](int q0, const float (&v)[64]) {
+        const int c0 = n0 + 64 * q0, left = nc - 64 * q0;
+        if (left <= 0) return;
+        if constexpr (MODE == XG_WGRAD) {
+          const bool in = w.m0 + row < g.M;
+          if (w.part >= 0) {
+            float* dst = in ? g.parts + ((int64_t)w.part * g.M + w.m0 + row) * g.N + c0 : nullptr;
+            xg_emit<float, T, false>(v, stg, dst, g.N % 4 == 0, 1.f, left, nullptr, false);
+          } else {
+            T* dst = in ? (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo + c0 : nullptr;
+            xg_emit<T, T, false>(v, stg, dst, vec, 1.f, left, nullptr, false);
+          }
+        } else {
+          T* dst = slot >= 0 && g.out ? (T*)g.out + (int64_t)slot * g.ldo + c0 : nullptr;
+          if (MODE == XG_DGRAD && g.dgpart) {
+            const T* xr = slot >= 0 ? (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + c0 : nullptr;
+            dot += xg_emit<T, T, true>(v, stg, dst, vec, sc, left, xr, xvec);
+          } else {
+            xg_emit<T, T, false>(v, stg, dst, vec, sc, left, nullptr, false);
+          }
+        }
+      };
+      if (!CHUNKS || w.nk <= acc_k) {            // one accumulator: 64 columns at a time straight from TMEM
+        const int acc = tc & 1;
+        if (w.nk > 0 && !wait(acc)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+          float v[64];
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = 0.f;
+          if (w.nk > 0) {
+            add64(acc, q, v);
+            if (q == NS - 1) {
+              release(acc);
+              ++tc;
+            }
+          }
+          emit64(q, v);
+        }
+      } else {                                   // chunks of K: their sum stays in registers
+        float v[NS][64];
+#pragma unroll
+        for (int q = 0; q < NS; ++q)
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[q][i] = 0.f;
+        for (int kb0 = 0; kb0 < w.nk; kb0 += acc_k, ++tc) {
+          const int acc = tc & 1;
+          if (!wait(acc)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int q = 0; q < NS; ++q) add64(acc, q, v[q]);
+          release(acc);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < NS; ++q) emit64(q, v[q]);
       }
+      if (MODE == XG_DGRAD && g.dgpart && slot >= 0)
+        g.dgpart[(int64_t)(2 * (w.n0 / g.bn) + hf) * g.lay.R + slot] = dot;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

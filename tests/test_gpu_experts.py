@@ -418,6 +418,34 @@ def test_expert_linear_more_tiles_than_sms():
         assert rel <= (n * U[torch.bfloat16] / math.sqrt(3) if n else 2e-6), rel
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_expert_linear_long_sums_keep_fp32_accuracy(dt):
+    """The tensor cores truncate when they accumulate (about 1.7e-8 of the sum for each 16 terms), so long sums whose
+    result leaves in fp32 are cut into chunks of 512: 32 x 1.7e-8 = 5.4e-7, and 1e-6 with the roundings of the rest.
+    One accumulator over 2048 terms would be 2.2e-6 off, over 6000 6.4e-6."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    dt = DT[dt]
+    T, D, O = 6000, 1024, 2048
+    x = torch.randn(T, D, device="cuda", generator=g).to(dt).requires_grad_()
+    w = (torch.randn(1, O, D, device="cuda", generator=g) / 32).to(dt).requires_grad_()
+    p = torch.rand(T, 1, device="cuda", generator=g).requires_grad_()
+    dy = torch.randn(T, O, device="cuda", generator=g).to(dt)
+    plan = X.plan_experts(torch.zeros(T, 1, dtype=torch.int32, device="cuda"), 1)
+    out = X.expert_linear(x, w, plan, p)
+    dx, dw, dp = torch.autograd.grad(out, (x, w, p), dy)
+    plan.check()
+    z = x.detach().double() @ w.detach()[0].double().T
+    dz = p.detach().double() * dy.double()
+    want = {"dp": (dy.double() * z).sum(1, keepdim=True)}
+    got = {"dp": dp}
+    if dt == torch.float32:
+        want |= {"out": p.detach().double() * z, "dx": dz @ w.detach()[0].double(), "dw": (dz.T @ x.detach().double())[None]}
+        got |= {"out": out.detach(), "dx": dx, "dw": dw}
+    for n in want:
+        rel = float((got[n].double() - want[n]).norm() / want[n].norm())
+        assert rel <= 1e-6, (n, rel)
+
+
 def test_expert_linear_padding_rows_do_not_spread_nan():
     """A NaN in one atom's row reaches that atom's output and its experts' gradients only."""
     g = _gen(11)
