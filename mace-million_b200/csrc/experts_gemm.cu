@@ -33,7 +33,7 @@ namespace mb {
 constexpr int XG_BM = XP_BM, XG_BK = 64, XG_EPI_WARPS = 8, XG_THREADS = 64 + 32 * XG_EPI_WARPS;
 constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
 constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
-constexpr int XG_ACC_K = 8;                      // K blocks of an accumulator whose result leaves in fp32
+constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12;     // K blocks of an accumulator whose result leaves in fp32 (fp32 / 16-bit data)
 
 // T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for
 template <typename T, int BN, int CG>
@@ -79,101 +79,115 @@ struct XgTile {
 
 // Row staging of the epilogue: a warp's 32 rows x 64 bytes, 16-byte piece c of row r at piece c ^ (r / 2 % 4), so that a
 // lane's access to its own row and the warp's access to eight whole row segments are both free of bank conflicts.
-__device__ __forceinline__ uint4* xg_stg(unsigned char* stg, int row, int c) {
-  return reinterpret_cast<uint4*>(stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+__device__ __forceinline__ uint32_t xg_stg(uint32_t stg, int row, int c) {
+  return stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+}
+// element i of a staged piece
+template <typename OUT>
+__device__ __forceinline__ OUT xg_elem(uint32_t piece, int i) {
+  if constexpr (sizeof(OUT) == 4) {
+    return __uint_as_float(lds32(piece + 4 * i));
+  } else {
+    const uint16_t u = lds16(piece + 2 * i);
+    return *reinterpret_cast<const OUT*>(&u);
+  }
 }
 
-// Writes 64 columns of the rows that the lanes of a warp hold (v, one row per lane, nc columns of it in use), scaled, through shared memory
-// in pieces of 64 bytes: global accesses are whole sectors of eight rows (one row per lane would be 32 scattered 16-byte
-// pieces per access, and held a tile for longer than its products at K <= 1024).  dst: this lane's row (null: not stored);
-// DOT: returns the scalar product of the row with that of x at xr.
-template <typename OUT, typename T, bool DOT>
-__device__ __forceinline__ float xg_emit(const float (&v)[64], unsigned char* stg, OUT* dst, bool vec, float sc, int nc,
-                                         const T* xr, bool xvec) {
-  constexpr int NC = 64 / (int)sizeof(OUT), OV = kVec<OUT>, XV = kVec<T>;   // columns of a piece, of a vector
-  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
-  const bool any = __any_sync(0xffffffffu, dst != nullptr);
-  float dot = 0.f;
-  uint4 xq[DOT ? 4 : 1];                         // the x rows' next piece
-  auto fetch_x = [&](int h) {
+// 16-byte piece l % 4 of the rows 8 i + l / 4 (i = 0 .. 3) is what lane l of a warp moves between shared and global memory;
+// row[i] is the row's place there, -1: none.
+template <typename T>
+__device__ __forceinline__ void xg_fetch(uint4 (&xq)[4], const int (&row)[4], const T* x, int64_t ldx, bool xvec, int left) {
+  constexpr int XV = kVec<T>;
+  const int c = (threadIdx.x & 3) * XV;
 #pragma unroll
-    for (int i = 0; i < (DOT ? 4 : 0); ++i) {
-      const T* xp = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(xr), 8 * i + r4));
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      const int left = nc - h * NC - c4 * XV;
-      if (xp && left > 0) {
-        xp += h * NC + c4 * XV;
-        if (xvec && left >= XV) {
-          u = *reinterpret_cast<const uint4*>(xp);
-        } else {
-          float f[XV];
-#pragma unroll
-          for (int q = 0; q < XV; ++q) f[q] = q < left ? to_f(xp[q]) : 0.f;
-          u = pack16<T>(f);
-        }
-      }
-      xq[i] = u;
-    }
-  };
-  if (DOT) fetch_x(0);
-#pragma unroll
-  for (int h = 0; h < 64 / NC; ++h) {
-    if (h * NC >= nc) break;
-    if constexpr (DOT) {
-      // a piece of x holds as many columns as one of the output: T = OUT here
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *xg_stg(stg, 8 * i + r4, c4) = xq[i];
-      if ((h + 1) * NC < nc) fetch_x(h + 1);
-      __syncwarp();
-      float part[4];                             // short chains, added up as a tree
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
+  for (int i = 0; i < 4; ++i) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (row[i] >= 0 && c < left) {
+      const T* xp = x + row[i] * ldx + c;
+      if (xvec && c + XV <= left) {
+        u = *reinterpret_cast<const uint4*>(xp);
+      } else {
         float f[XV];
-        unpack16(*xg_stg(stg, lane, c), f, T());
-        part[c] = 0.f;
 #pragma unroll
-        for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], v[h * NC + c * XV + q], part[c]);
+        for (int q = 0; q < XV; ++q) f[q] = c + q < left ? to_f(xp[q]) : 0.f;
+        u = pack16<T>(f);
       }
-      dot += (part[0] + part[1]) + (part[2] + part[3]);
-      __syncwarp();
     }
-    if (!any) continue;
+    xq[i] = u;
+  }
+}
+
+// Writes 32 columns of the rows that the lanes of a warp hold (v, one row per lane), scaled, through shared memory in pieces
+// of 64 bytes: global accesses are whole sectors of eight rows (one row per lane would be 32 scattered 16-byte pieces per
+// access, and held a tile for longer than its products at K <= 1024).  out: first column; left: columns that exist.
+template <typename OUT>
+__device__ __forceinline__ void xg_emit32(const float* v, uint32_t stg, const int (&row)[4], OUT* out, int64_t ldo,
+                                          bool vec, float sc, int left) {
+  constexpr int NC = 64 / (int)sizeof(OUT), OV = kVec<OUT>;   // columns of a piece, of a vector
+  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 32 / NC; ++h) {
+    const int n = left - h * NC;
+    if (n <= 0) break;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       float f[OV];
 #pragma unroll
       for (int q = 0; q < OV; ++q) f[q] = v[h * NC + c * OV + q] * sc;
-      *xg_stg(stg, lane, c) = pack16<OUT>(f);
+      sts128(xg_stg(stg, lane, c), pack16<OUT>(f));
     }
     __syncwarp();
     if (vec) {
-      const int left = nc - h * NC - c4 * OV;    // columns of this lane's piece
+      const int mine = n - c4 * OV;              // columns of this lane's piece
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), 8 * i + r4));
-        if (!p || left <= 0) continue;
-        p += h * NC + c4 * OV;
-        const uint4* s = xg_stg(stg, 8 * i + r4, c4);
-        if (left >= OV)
-          *reinterpret_cast<uint4*>(p) = *s;
+        if (row[i] < 0 || mine <= 0) continue;
+        OUT* p = out + row[i] * ldo + h * NC + c4 * OV;
+        const uint32_t s = xg_stg(stg, 8 * i + r4, c4);
+        if (mine >= OV)
+          *reinterpret_cast<uint4*>(p) = lds128(s);
         else
-          for (int q = 0; q < left; ++q) p[q] = reinterpret_cast<const OUT*>(s)[q];
+          for (int q = 0; q < mine; ++q) p[q] = xg_elem<OUT>(s, q);
       }
     } else {                                     // odd strides: one row at a time (two of 16 columns), lanes along it
       constexpr int RP = 32 / NC;
-#pragma unroll 4
-      for (int r = 0; r < 32; r += RP) {
-        const int rr = r + lane / NC, c = lane % NC;
-        OUT* p = reinterpret_cast<OUT*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), rr));
-        if (p && h * NC + c < nc) p[h * NC + c] = reinterpret_cast<const OUT*>(xg_stg(stg, rr, c / OV))[c % OV];
-      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll 2
+        for (int r = 0; r < 8; r += RP) {
+          const int rr = r + lane / NC, c = lane % NC;
+          const int at = __shfl_sync(0xffffffffu, row[i], rr * 4);
+          if (at >= 0 && c < n)
+            out[at * ldo + h * NC + c] = xg_elem<OUT>(xg_stg(stg, 8 * i + rr, c / OV), c % OV);
+        }
     }
     __syncwarp();
   }
-  return dot;
 }
 
-template <int MODE, typename T, int BN, int CG>
+// Scalar products of the columns of the lanes' rows that a piece of x (64 bytes a row, in xq by xg_fetch) covers
+template <typename T>
+__device__ __forceinline__ float xg_dot(const float* v, uint32_t stg, const uint4 (&xq)[4]) {
+  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
+  constexpr int XV = kVec<T>;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sts128(xg_stg(stg, 8 * i + r4, c4), xq[i]);
+  __syncwarp();
+  float part[4];                                 // short chains, added up as a tree
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float f[XV];
+    unpack16(lds128(xg_stg(stg, lane, c)), f, T());
+    part[c] = 0.f;
+#pragma unroll
+    for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], v[c * XV + q], part[c]);
+  }
+  __syncwarp();
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// DOT: DGRAD with dgpart
+template <int MODE, typename T, int BN, int CG, bool DOT>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
   using C = XgCfg<T, BN, CG>;
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       }
       for (int a = 0; a < 2; ++a) {
         mbar_init(&B.acc_full[a], 1);
-        mbar_init(&B.acc_empty[a], 32 * XG_EPI_WARPS * CG);
+        mbar_init(&B.acc_empty[a], XG_EPI_WARPS * CG);
       }
       B.failed = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   };
   const int bh = g.bn / CG;                      // columns of B that this CTA loads
   // K blocks of one accumulator
-  const int acc_k = sizeof(T) == 4 || (MODE == XG_DGRAD && g.dgpart) ? XG_ACC_K : 0x7fffffff;
+  constexpr int acc_k = sizeof(T) == 4 ? XG_ACC_K : DOT ? XG_ACC_K16 : 0x3fffffff;
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------ loads
@@ -333,7 +347,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         const int t = tile_at(r);
         if (t >= tiles) break;
         const int nk = tile_of(t).nk;
-        for (int kb0 = 0; ok && kb0 < nk; kb0 += acc_k < nk ? acc_k : nk, ++tc) {
+        for (int kb0 = 0; ok && kb0 < nk; kb0 += acc_k, ++tc) {
           const int acc = tc & 1, kb1 = nk - kb0 > acc_k ? kb0 + acc_k : nk;
           if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, XG_WAIT_NS)) {
             *failed = 1;
@@ -382,11 +396,11 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     // ------------------------------------------------------------------------------------------ epilogue
     // warp w reads TMEM lanes 32 (w % 4) .., one row per lane, and the first or second half of the tile's columns
     const int q4 = warp & 3, row = q4 * 32 + lane, hf = (warp - 2) >> 2, hw = g.bn / 2;
-    unsigned char* stg = stg0 + (warp - 2) * XG_STG;
+    const uint32_t stg = smem_u32(stg0) + (warp - 2) * XG_STG;
     const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
     const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
-    constexpr int NS = BN / 128;                   // pieces of 64 columns of a half row
-    constexpr bool CHUNKS = sizeof(T) == 4 || MODE == XG_DGRAD;   // K may be cut (acc_k)
+    constexpr int NG = BN / 64;                    // groups of 32 columns in a half row
+    constexpr int XC = 32 * 2 / (int)sizeof(T);    // columns of x in a fetch (64 bytes)
     int tc = 0;
     bool ok = true;
     // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
@@ -395,12 +409,34 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       if (t >= tiles) break;
       const XgTile w = tile_of(t);
       const int n0 = w.n0 + hf * hw, nc = g.N - n0 < hw ? g.N - n0 : hw;   // nc <= 0: nothing in this half
-      int slot = -1;
+      int slot = -1, orow[4], xrow[4];
       float sc = 1.f, dot = 0.f;
-      if constexpr (MODE != XG_WGRAD) {          // in flight during the wait
+      T* out = (T*)g.out + n0;
+      float* pout = nullptr;                       // WGRAD: partial sums
+      int64_t ldo = g.ldo;
+      if constexpr (MODE != XG_WGRAD) {            // in flight during the wait
         slot = w.rows_ok ? plan[g.lay.o_row + w.m0 + row] : -1;
         if (slot >= 0 && g.scale) sc = g.scale[slot];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          orow[i] = __shfl_sync(0xffffffffu, slot, 8 * i + (lane >> 2));
+          xrow[i] = DOT && orow[i] >= 0 ? orow[i] / g.kdiv : -1;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          orow[i] = w.m0 + q4 * 32 + 8 * i + (lane >> 2);
+          if (orow[i] >= g.M) orow[i] = -1;
+        }
+        out += (int64_t)w.e * g.M * ldo;
+        if (w.part >= 0) {
+          ldo = g.N;
+          pout = g.parts + (int64_t)w.part * g.M * ldo + n0;
+        }
       }
+      const T* x = (const T*)g.x + n0;
+      uint4 xq[4];
+      if constexpr (DOT) xg_fetch<T>(xq, xrow, x, g.ldx, xvec, nc);
       auto wait = [&](int acc) {
         const bool got = !__shfl_sync(0xffffffffu, *failed, 0) &&
                          __all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS));
@@ -408,81 +444,75 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         return got;
       };
-      auto release = [&](int acc) {
+      auto release = [&](int acc) {                // one arrival per warp
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        if constexpr (CG == 2)
-          mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
-        else
-          mbar_arrive(&B.acc_empty[acc]);
-      };
-      auto add64 = [&](int acc, int q0, float (&v)[64]) {    // v += columns [64 q0, + 64) of the half row
-        const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * C::ACC + hf * hw + 64 * q0);
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          if (64 * q0 + 32 * q < nc) {
-            uint32_t u[32];
-            tmem_ld32(ta + 32 * q, u);
-            if constexpr (C::PL == 3) {
-              uint32_t u2[32];
-              tmem_ld32(ta + BN + 32 * q, u2);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[32 * q + i] += __uint_as_float(u[i]) + __uint_as_float(u2[i]);
-            } else {
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[32 * q + i] += __uint_as_float(u[i]);
-            }
-          }
-      };
-      auto emit64 = [&](int q0, const float (&v)[64]) {
-        const int c0 = n0 + 64 * q0, left = nc - 64 * q0;
-        if (left <= 0) return;
-        if constexpr (MODE == XG_WGRAD) {
-          const bool in = w.m0 + row < g.M;
-          if (w.part >= 0) {
-            float* dst = in ? g.parts + ((int64_t)w.part * g.M + w.m0 + row) * g.N + c0 : nullptr;
-            xg_emit<float, T, false>(v, stg, dst, g.N % 4 == 0, 1.f, left, nullptr, false);
-          } else {
-            T* dst = in ? (T*)g.out + ((int64_t)w.e * g.M + w.m0 + row) * g.ldo + c0 : nullptr;
-            xg_emit<T, T, false>(v, stg, dst, vec, 1.f, left, nullptr, false);
-          }
-        } else {
-          T* dst = slot >= 0 && g.out ? (T*)g.out + (int64_t)slot * g.ldo + c0 : nullptr;
-          if (MODE == XG_DGRAD && g.dgpart) {
-            const T* xr = slot >= 0 ? (const T*)g.x + (int64_t)(slot / g.kdiv) * g.ldx + c0 : nullptr;
-            dot += xg_emit<T, T, true>(v, stg, dst, vec, sc, left, xr, xvec);
-          } else {
-            xg_emit<T, T, false>(v, stg, dst, vec, sc, left, nullptr, false);
-          }
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
+          else
+            mbar_arrive(&B.acc_empty[acc]);
         }
       };
-      if (!CHUNKS || w.nk <= acc_k) {            // one accumulator: 64 columns at a time straight from TMEM
+      auto load32 = [&](int acc, int q, float* v, bool add) {   // columns [32 q, + 32) of the half row
+        const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * C::ACC + hf * hw + 32 * q);
+        uint32_t u[32];
+        tmem_ld32(ta, u);
+        if constexpr (C::PL == 3) {
+          uint32_t u2[32];
+          tmem_ld32(ta + BN, u2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) + __uint_as_float(u2[i]));
+        } else {
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = add ? v[i] + __uint_as_float(u[i]) : __uint_as_float(u[i]);
+      };
+      auto emit = [&](int q, const float* v) {
+        if constexpr (DOT) {
+#pragma unroll
+          for (int h = 0; h < 32 / XC; ++h) {
+            dot += xg_dot<T>(v + h * XC, stg, xq);
+            const int c = 32 * q + (h + 1) * XC;
+            if (c < nc) xg_fetch<T>(xq, xrow, x + c, g.ldx, xvec, nc - c);
+          }
+          if (!g.out) return;
+        }
+        if (MODE == XG_WGRAD && pout)
+          xg_emit32<float>(v, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, 1.f, nc - 32 * q);
+        else
+          xg_emit32<T>(v, stg, orow, out + 32 * q, ldo, vec, sc, nc - 32 * q);
+      };
+      if constexpr (acc_k == 0x3fffffff) {         // one accumulator: 32 columns at a time straight from TMEM
         const int acc = tc & 1;
         if (w.nk > 0 && !wait(acc)) {
           ok = false;
           break;
         }
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          float v[64];
-#pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = 0.f;
+#pragma unroll 1
+        for (int q = 0; 32 * q < nc; ++q) {
+          float v[32];
           if (w.nk > 0) {
-            add64(acc, q, v);
-            if (q == NS - 1) {
-              release(acc);
-              ++tc;
-            }
+            load32(acc, q, v, false);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
-          emit64(q, v);
+          if (w.nk > 0 && 32 * (q + 1) >= nc) release(acc);
+          emit(q, v);
         }
-      } else {                                   // chunks of K: their sum stays in registers
-        float v[NS][64];
+        if (w.nk > 0) {
+          if (nc <= 0) release(acc);
+          ++tc;
+        }
+      } else {                                     // chunks of K: their sum stays in registers
+        float v[NG][32];
 #pragma unroll
-        for (int q = 0; q < NS; ++q)
+        for (int q = 0; q < NG; ++q)
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[q][i] = 0.f;
+          for (int i = 0; i < 32; ++i) v[q][i] = 0.f;
         for (int kb0 = 0; kb0 < w.nk; kb0 += acc_k, ++tc) {
           const int acc = tc & 1;
           if (!wait(acc)) {
@@ -490,15 +520,16 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
             break;
           }
 #pragma unroll
-          for (int q = 0; q < NS; ++q) add64(acc, q, v[q]);
+          for (int q = 0; q < NG; ++q)
+            if (32 * q < nc) load32(acc, q, v[q], true);
           release(acc);
         }
         if (!ok) break;
 #pragma unroll
-        for (int q = 0; q < NS; ++q) emit64(q, v[q]);
+        for (int q = 0; q < NG; ++q)
+          if (32 * q < nc) emit(q, v[q]);
       }
-      if (MODE == XG_DGRAD && g.dgpart && slot >= 0)
-        g.dgpart[(int64_t)(2 * (w.n0 / g.bn) + hf) * g.lay.R + slot] = dot;
+      if (DOT && slot >= 0) g.dgpart[(int64_t)(2 * (w.n0 / g.bn) + hf) * g.lay.R + slot] = dot;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -583,16 +614,18 @@ static int xg_map(CUtensorMap* m, bool is_bf16, int rank, const void* p, const i
   return 0;
 }
 
-static int xg_bn_max(int64_t N, int dtype) { return dtype == MB_F32 || N <= 128 ? 128 : 256; }
-int xgemm_n_tiles(int64_t N, int dtype) {
-  const int bn = xg_bn_max(N, dtype);
+// Widest tile: three planes of two operands fill a stage at 128 columns, and with `dot` the chunks' sums are 64 registers
+// of a thread at 128 columns (at 256 they spilled: dx and dweights of 262,144 slots 1024 <- 2048 took 1290 us for 890)
+static int xg_bn_max(int64_t N, int dtype, bool dot) { return dtype == MB_F32 || dot || N <= 128 ? 128 : 256; }
+int xgemm_n_tiles(int64_t N, int dtype, bool dot) {
+  const int bn = xg_bn_max(N, dtype, dot);
   return (int)((N + bn - 1) / bn);
 }
 
 // K blocks of a part in WGRAD: whole experts when that makes four or more rounds of tiles, else parts that make about
 // that many, of at least 8 K blocks (below that the partial sums' traffic outweighs the idle SMs)
 int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype) {
-  const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype), want = 4 * (int64_t)sm_count();
+  const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype, false), want = 4 * (int64_t)sm_count();
   const int64_t blocks = slots / XG_BK;          // K blocks of all experts
   if (E * per >= want) return 0x3fffffff;
   int64_t kc = blocks * per / want;
@@ -606,13 +639,13 @@ int64_t xgemm_parts(int64_t E, int64_t slots, int kc) {
   return blocks / kc + E;
 }
 
-template <int MODE, typename T, int BN, int CG>
+template <int MODE, typename T, int BN, int CG, bool DOT>
 static int xg_go(const XGemm& x, cudaStream_t st) {
   using C = XgCfg<T, BN, CG>;
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
-  auto kern = k_expert_gemm<MODE, T, BN, CG>;
+  auto kern = k_expert_gemm<MODE, T, BN, CG, DOT>;
   if (ready_dev != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -622,7 +655,7 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   }
   XgParams g{};
   g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K;
-  g.tn = xgemm_n_tiles(x.N, x.dtype);
+  g.tn = xgemm_n_tiles(x.N, x.dtype, DOT);
   g.bn = (int)(((x.N + g.tn - 1) / g.tn + 63) / 64 * 64);
   g.tm = (x.M + XG_BM * CG - 1) / (XG_BM * CG);
   g.kc = x.kc;
@@ -685,7 +718,7 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
 // 512 -> 515 (8 K blocks; 5 or 3 row tiles of dW) forward 36 / 43 us, dW 49 / 55; 65,536 slots on 128 experts, 512 -> 256
 // (two tiles an expert) forward and sum 60 / 69 us.
 static bool xg_pairs(const XGemm& x) {
-  const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype);
+  const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype, x.dgpart != nullptr);
   const int64_t blocks = x.mode == XG_WGRAD ? rows / XG_BK : x.K / XG_BK;
   const int64_t m = x.mode == XG_WGRAD ? x.M : rows, tiles = x.E * ((m + 255) / 256) * tn;
   const int64_t waste = x.mode == XG_WGRAD ? (m + 255) / 256 * 256 - m : 128;
@@ -694,12 +727,16 @@ static bool xg_pairs(const XGemm& x) {
 
 template <int MODE, typename T>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
-  if constexpr (sizeof(T) == 4) {
-    return xg_go<MODE, T, 128, 1>(x, st);
-  } else {
-    if (xg_bn_max(x.N, x.dtype) == 128) return xg_go<MODE, T, 128, 1>(x, st);
-    return xg_pairs(x) ? xg_go<MODE, T, 256, 2>(x, st) : xg_go<MODE, T, 256, 1>(x, st);
-  }
+  if constexpr (MODE == XG_DGRAD)
+    if (x.dgpart) {
+      if constexpr (sizeof(T) == 2)
+        if (xg_pairs(x)) return xg_go<MODE, T, 128, 2, true>(x, st);
+      return xg_go<MODE, T, 128, 1, true>(x, st);
+    }
+  if constexpr (sizeof(T) == 2)
+    if (xg_bn_max(x.N, x.dtype, false) == 256)
+      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, false>(x, st) : xg_go<MODE, T, 256, 1, false>(x, st);
+  return xg_go<MODE, T, 128, 1, false>(x, st);
 }
 
 template <int MODE>
