@@ -610,7 +610,7 @@ static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direc
   b.dys = c.take(row2 * s.Op);
   if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
   if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * dtype_size(s.dtype));
-  if (need_g) b.dgp = c.take(s.R * 4 * 2 * xgemm_n_tiles(s.D, s.dtype, true));
+  if (need_g) b.dgp = c.take(s.R * 4 * 2 * xgemm_n_tiles(s.D, s.dtype));
   if (need_w) {
     b.kc = xgemm_kc(s.E, s.O, s.D, s.R, s.dtype);
     const int64_t parts = xgemm_parts(s.E, s.R, b.kc);
@@ -877,6 +877,6 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
     if (int rc = xgemm_launch(g, st)) return rc;
     if (!sum && !dweights) return 0;
     return x_rows_sum<T>(sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, plan + s.lay.o_slot,
-                         dweights ? (const float*)(base + b.dgp) : nullptr, 2 * xgemm_n_tiles(D, dtype, true), dweights, st);
+                         dweights ? (const float*)(base + b.dgp) : nullptr, 2 * xgemm_n_tiles(D, dtype), dweights, st);
   });
 }

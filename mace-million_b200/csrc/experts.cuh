@@ -60,7 +60,7 @@ struct XGemm {
   int32_t kdiv;                                  // slot / kdiv = row of x
   float* dgpart;
 };
-int xgemm_n_tiles(int64_t N, int dtype, bool dot);
+int xgemm_n_tiles(int64_t N, int dtype);
 int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype);
 int64_t xgemm_parts(int64_t E, int64_t slots, int kc);
 int xgemm_launch(const XGemm& g, cudaStream_t st);

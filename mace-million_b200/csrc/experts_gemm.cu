@@ -13,7 +13,7 @@
 // with rounding to nearest; 16-bit results are rounded a thousand times more coarsely and take the whole K.
 //
 // Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
-// into one of two TMEM accumulators, warps 2-9 drain the other one (a lane holds half a row).  CG = 2: a cluster of two CTAs works on a 256-row tile
+// into one of two TMEM accumulators, warps 4-11 drain the other one (a lane holds half a row).  CG = 2: a cluster of two CTAs works on a 256-row tile
 // (cta_group::2, each CTA holds its 128 rows of A and half of B's columns), which halves the B bytes a CTA fetches.
 // The N tile is the smallest multiple of 64 that cuts N into ceil(N / 256) tiles.
 // WGRAD cuts an expert's rows into parts of kc K blocks when there are few tiles; parts of an expert with several are
@@ -30,7 +30,11 @@
 
 namespace mb {
 
-constexpr int XG_BM = XP_BM, XG_BK = 64, XG_EPI_WARPS = 8, XG_THREADS = 64 + 32 * XG_EPI_WARPS;
+constexpr int XG_BM = XP_BM, XG_BK = 64, XG_EPI_WARPS = 8, XG_EPI0 = 4, XG_THREADS = 32 * (XG_EPI0 + XG_EPI_WARPS);
+// Registers of a thread in the first four warps and in the epilogue's, where the latter hold half a row of 256 columns:
+// 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
+constexpr int XG_REGS = 168, XG_REGS_LOW = 72, XG_REGS_HIGH = 216;
+static_assert(32 * (XG_EPI0 * XG_REGS_LOW + XG_EPI_WARPS * XG_REGS_HIGH) <= XG_THREADS * XG_REGS, "registers");
 constexpr unsigned long long XG_WAIT_NS = 2000000000ull;   // a tile takes microseconds
 constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
 constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12;     // K blocks of an accumulator whose result leaves in fp32 (fp32 / 16-bit data)
@@ -282,9 +286,12 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     return o;
   };
   const int bh = g.bn / CG;                      // columns of B that this CTA loads
+  constexpr bool SPLIT = DOT && BN == 256;       // registers move from the first four warps to the epilogue's
   // K blocks of one accumulator
   constexpr int acc_k = sizeof(T) == 4 ? XG_ACC_K : DOT ? XG_ACC_K16 : 0x3fffffff;
 
+  if (warp < XG_EPI0) {
+  if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XG_REGS_LOW));
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------ loads
     if (lane == 0) {
@@ -392,11 +399,13 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       // after a timeout: wait (bounded) for the MMAs already issued before the TMEM is freed
       if (*failed && last_bar) mbar_wait_ns(last_bar, last_par, XG_WAIT_NS);
     }
+  }
   } else {
     // ------------------------------------------------------------------------------------------ epilogue
+    if constexpr (SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XG_REGS_HIGH));
     // warp w reads TMEM lanes 32 (w % 4) .., one row per lane, and the first or second half of the tile's columns
-    const int q4 = warp & 3, row = q4 * 32 + lane, hf = (warp - 2) >> 2, hw = g.bn / 2;
-    const uint32_t stg = smem_u32(stg0) + (warp - 2) * XG_STG;
+    const int q4 = warp & 3, row = q4 * 32 + lane, hf = (warp - XG_EPI0) >> 2, hw = g.bn / 2;
+    const uint32_t stg = smem_u32(stg0) + (warp - XG_EPI0) * XG_STG;
     const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
     const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
     constexpr int NG = BN / 64;                    // groups of 32 columns in a half row
@@ -614,18 +623,17 @@ static int xg_map(CUtensorMap* m, bool is_bf16, int rank, const void* p, const i
   return 0;
 }
 
-// Widest tile: three planes of two operands fill a stage at 128 columns, and with `dot` the chunks' sums are 64 registers
-// of a thread at 128 columns (at 256 they spilled: dx and dweights of 262,144 slots 1024 <- 2048 took 1290 us for 890)
-static int xg_bn_max(int64_t N, int dtype, bool dot) { return dtype == MB_F32 || dot || N <= 128 ? 128 : 256; }
-int xgemm_n_tiles(int64_t N, int dtype, bool dot) {
-  const int bn = xg_bn_max(N, dtype, dot);
+// Widest tile: three planes of two operands fill a stage at 128 columns
+static int xg_bn_max(int64_t N, int dtype) { return dtype == MB_F32 || N <= 128 ? 128 : 256; }
+int xgemm_n_tiles(int64_t N, int dtype) {
+  const int bn = xg_bn_max(N, dtype);
   return (int)((N + bn - 1) / bn);
 }
 
 // K blocks of a part in WGRAD: whole experts when that makes four or more rounds of tiles, else parts that make about
 // that many, of at least 8 K blocks (below that the partial sums' traffic outweighs the idle SMs)
 int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype) {
-  const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype, false), want = 4 * (int64_t)sm_count();
+  const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype), want = 4 * (int64_t)sm_count();
   const int64_t blocks = slots / XG_BK;          // K blocks of all experts
   if (E * per >= want) return 0x3fffffff;
   int64_t kc = blocks * per / want;
@@ -651,11 +659,16 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
       return MB_E_CUDA;
     }
+    cudaFuncAttributes at{};
+    if (DOT && BN == 256 && (cudaFuncGetAttributes(&at, kern) != cudaSuccess || at.numRegs < XG_REGS)) {
+      set_error("expert_linear: launched with %d registers a thread, %d are needed", at.numRegs, XG_REGS);
+      return MB_E_CUDA;
+    }
     ready_dev = dev;
   }
   XgParams g{};
   g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K;
-  g.tn = xgemm_n_tiles(x.N, x.dtype, DOT);
+  g.tn = xgemm_n_tiles(x.N, x.dtype);
   g.bn = (int)(((x.N + g.tn - 1) / g.tn + 63) / 64 * 64);
   g.tm = (x.M + XG_BM * CG - 1) / (XG_BM * CG);
   g.kc = x.kc;
@@ -718,25 +731,26 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
 // 512 -> 515 (8 K blocks; 5 or 3 row tiles of dW) forward 36 / 43 us, dW 49 / 55; 65,536 slots on 128 experts, 512 -> 256
 // (two tiles an expert) forward and sum 60 / 69 us.
 static bool xg_pairs(const XGemm& x) {
-  const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype, x.dgpart != nullptr);
+  const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype);
   const int64_t blocks = x.mode == XG_WGRAD ? rows / XG_BK : x.K / XG_BK;
   const int64_t m = x.mode == XG_WGRAD ? x.M : rows, tiles = x.E * ((m + 255) / 256) * tn;
   const int64_t waste = x.mode == XG_WGRAD ? (m + 255) / 256 * 256 - m : 128;
   return blocks >= 16 && 8 * waste <= m && tiles >= 8 * (int64_t)(sm_count() / 2);
 }
 
+template <int MODE, typename T, bool DOT>
+static int xg_dot_any(const XGemm& x, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (xg_bn_max(x.N, x.dtype) == 256)
+      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT>(x, st) : xg_go<MODE, T, 256, 1, DOT>(x, st);
+  return xg_go<MODE, T, 128, 1, DOT>(x, st);
+}
+
 template <int MODE, typename T>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
   if constexpr (MODE == XG_DGRAD)
-    if (x.dgpart) {
-      if constexpr (sizeof(T) == 2)
-        if (xg_pairs(x)) return xg_go<MODE, T, 128, 2, true>(x, st);
-      return xg_go<MODE, T, 128, 1, true>(x, st);
-    }
-  if constexpr (sizeof(T) == 2)
-    if (xg_bn_max(x.N, x.dtype, false) == 256)
-      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, false>(x, st) : xg_go<MODE, T, 256, 1, false>(x, st);
-  return xg_go<MODE, T, 128, 1, false>(x, st);
+    if (x.dgpart) return xg_dot_any<MODE, T, true>(x, st);
+  return xg_dot_any<MODE, T, false>(x, st);
 }
 
 template <int MODE>
