@@ -287,19 +287,53 @@ static int plan_one(const int32_t* experts, const XPlan& p, int32_t* plan, cudaS
 }
 
 // ------------------------------------------------------------------------------------------------ row movement
-// 8 columns [c0, c0 + 8) of a row as floats (0 beyond d)
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c0, int d, bool vec, float (&f)[8]) {
-  if (vec && c0 + 8 <= d) {
-    if constexpr (sizeof(T) == 2) {
-      unpack16(*reinterpret_cast<const uint4*>(row + c0), f, T());
-    } else {
-      load_p<float, 8>(row + c0, f);
-    }
+// 16 bytes at any even address: two aligned vectors and a shift.  [lo, hi): the bytes that may be read; where an aligned
+// vector would leave them the bytes come one element at a time.
+__device__ __forceinline__ uint4 load16_any(const uint16_t* p, const char* lo, const char* hi) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const unsigned s = (unsigned)(a & 15);
+  const char* base = reinterpret_cast<const char*>(a - s);
+  if (s == 0) return *reinterpret_cast<const uint4*>(p);
+  if (base < lo || base + 32 > hi) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const uint4 u = reinterpret_cast<const uint4*>(base)[0], v = reinterpret_cast<const uint4*>(base)[1];
+  uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  if (s & 8)
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (s & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const unsigned sh = (s & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+
+// 8 columns [c, c + 8) of a row of d elements as floats (0 beyond d); vec: 16-byte loads are aligned
+__device__ __forceinline__ void load8(const float* row, int c, int d, bool vec, const char*, const char*, float (&f)[8]) {
+  if (vec && c + 8 <= d) {
+    load_p<float, 8>(row + c, f);
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) f[q] = c0 + q < d ? to_f(row[c0 + q]) : 0.f;
+    for (int q = 0; q < 8; ++q) f[q] = c + q < d ? row[c + q] : 0.f;
   }
+}
+// the same of 16-bit elements, as they are
+template <typename T>
+__device__ __forceinline__ uint4 load8_raw(const T* row, int c, int d, bool vec, const char* lo, const char* hi) {
+  if (c + 8 <= d)
+    return vec ? *reinterpret_cast<const uint4*>(row + c)
+               : load16_any(reinterpret_cast<const uint16_t*>(row + c), lo, hi);
+  const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (c + 2 * i < d ? (uint32_t)r[c + 2 * i] : 0u) | ((c + 2 * i + 1 < d ? (uint32_t)r[c + 2 * i + 1] : 0u) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Writes 8 columns as one vector of a 16-bit plane, or of three bf16 planes (fp32 data)
@@ -323,7 +357,7 @@ __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64
   }
 }
 
-// One job of k_rows_move; a launch runs up to four side by side, each on its own blocks (few launches: every one costs a
+// One job of k_rows_move; a launch runs up to XMOVES side by side, each on its own blocks (few launches: every one costs a
 // small call more than its work).
 struct XMove {
   int kind;                                      // MOVE_*
@@ -331,18 +365,26 @@ struct XMove {
   unsigned block0, blocks;                       // first block and number of blocks
   int64_t rows, lds, plane;
   const void* src;
+  const char *lo, *hi;                           // the source's first and last byte + 1
   const float* scale;
   void* out;
 };
 enum {
-  // out[row] = scale[slot] src[slot / kdiv] in planes, rows in expert order, zeros in padding rows and padding columns
-  MOVE_GATHER = 0,
-  MOVE_STAGE = 1,                                // out[row] = src[row] in planes, zeros in padding columns
-  MOVE_ZERO = 2,                                 // out[slot] = 0 for slots without an expert (elements of T)
-};
+  // out[row of slot] = scale[slot] src[slot / kdiv], in planes, for the slots with an expert: each source row is read once
+  // and written to its kdiv rows (in expert order the rows of a token are far apart, and a gather would read it kdiv times)
+  MOVE_SCATTER = 0,
+  MOVE_STAGE = 1,                                // out[row] = src[row] in planes
+  MOVE_PAD = 2,                                  // out[row] = 0 in planes for the rows that pad the experts' segments
+  MOVE_ZERO = 3,                                 // out[slot] = 0 for slots without an expert (elements of T)
+};                                               // columns between d and dp are written as zeros
+constexpr int XMOVES = 6;                        // backward: dy, x, their padding, W, rows without an expert
 struct XMoves {
-  XMove m[4];
+  XMove m[XMOVES];
   int n;
+  __host__ void add(const XMove& j) {
+    if (n < XMOVES) m[n] = j;
+    ++n;                                         // x_moves refuses more than XMOVES
+  }
 };
 
 // Narrow rows share a warp (lpr lanes a row, a power of two); wide ones take several passes, four vectors in flight.
@@ -352,14 +394,11 @@ __global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_
   while (q + 1 < mv.n && blockIdx.x >= mv.m[q + 1].block0) ++q;
   const XMove& m = mv.m[q];
   const int lane = threadIdx.x & 31, nv = m.dp / 8;
-  int lpr = 1;
-  while (lpr < 32 && lpr < nv) lpr *= 2;
-  const int rpw = 32 / lpr, sub = lane & (lpr - 1);
-  const int64_t rows = m.kind == MOVE_GATHER ? (int64_t)plan[0] * XP_BM : m.rows;
-  const int64_t step = (int64_t)m.blocks * 8 * rpw;
-  if (m.kind == MOVE_ZERO) {                     // 32 slots a warp; the whole warp zeros a row (rpw = 32)
-    for (int64_t r0 = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * 32; r0 < rows; r0 += step) {
-      unsigned todo = __ballot_sync(0xffffffffu, r0 + lane < rows && plan[p.o_slot + r0 + lane] < 0);
+  const int64_t warp0 = (int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5), warps = (int64_t)m.blocks * 8;
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  if (m.kind == MOVE_ZERO) {                     // 32 slots a warp; the whole warp zeros a row
+    for (int64_t r0 = warp0 * 32; r0 < m.rows; r0 += warps * 32) {
+      unsigned todo = __ballot_sync(0xffffffffu, r0 + lane < m.rows && plan[p.o_slot + r0 + lane] < 0);
       for (; todo; todo &= todo - 1) {
         T* o = (T*)m.out + (r0 + __ffs(todo) - 1) * m.d;
         for (int c = lane; c < m.d; c += 32) o[c] = from_f<T>(0.f);
@@ -367,57 +406,69 @@ __global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_
     }
     return;
   }
-  const bool gather = m.kind == MOVE_GATHER;
-  const int32_t* row_slot = plan + p.o_row;
-  int64_t row = ((int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5)) * rpw + lane / lpr;
-  int next = gather && row < rows ? row_slot[row] : 0;
-  for (; row < rows; row += step) {
-    const int64_t slot = gather ? (int64_t)next : row;
-    if (gather && row + step < rows) next = row_slot[row + step];   // in flight while this row is copied
-    const T* s = (const T*)m.src + (slot < 0 ? 0 : gather ? (int)slot / m.kdiv : slot) * m.lds;
-    const float g = m.scale && slot >= 0 ? m.scale[slot] : 1.f;
-    uint16_t* out = (uint16_t*)m.out + row * m.dp;
-    if (sizeof(T) == 2 && m.vec) {
+  uint16_t* out = (uint16_t*)m.out;
+  if (m.kind == MOVE_PAD) {                      // candidate i: row i % 128 of the last tile of expert i / 128
+    for (int64_t i = warp0; i < m.rows; i += warps) {
+      const int e = (int)(i / XP_BM), c = plan[p.o_cnt + e] % XP_BM, r = (int)(i % XP_BM);
+      if (c == 0 || r < c) continue;
+      const int64_t row = plan[p.o_seg + e + 1] - XP_BM + r;
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl)
+        for (int v = lane; v < nv; v += 32)
+          *reinterpret_cast<uint4*>(out + pl * m.plane + row * m.dp + 8 * v) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
+  }
+  int lpr = 1;
+  while (lpr < 32 && lpr < nv) lpr *= 2;
+  const int rpw = 32 / lpr, sub = lane & (lpr - 1);
+  const bool scatter = m.kind == MOVE_SCATTER;
+  const int32_t* slot_row = plan + p.o_slot;
+  const int copies = scatter ? m.kdiv : 1;
+  for (int64_t row = warp0 * rpw + lane / lpr; row < m.rows; row += warps * rpw) {
+    const T* s = (const T*)m.src + row * m.lds;
+    if constexpr (sizeof(T) == 2) {
       for (int c0 = sub * 8; c0 < m.dp; c0 += 32 * lpr) {
         uint4 u[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = c0 + q * 8 * lpr;
-          u[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (slot >= 0 && c + 8 <= m.d) u[q] = *reinterpret_cast<const uint4*>(s + c);
+        for (int i = 0; i < 4; ++i) {
+          const int c = c0 + i * 8 * lpr;
+          if (c < m.dp) u[i] = load8_raw<T>(s, c, m.d, m.vec != 0, m.lo, m.hi);
         }
+#pragma unroll 4
+        for (int j = 0; j < copies; ++j) {
+          const int64_t to = scatter ? slot_row[row * copies + j] : row;
+          if (to < 0) continue;
+          const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = c0 + q * 8 * lpr;
-          if (slot >= 0 && c < m.d && c + 8 > m.d) {       // the ragged end of a row
-            float f[8];
-            load8(s, c, m.d, false, f);
-            if constexpr (sizeof(T) == 2) u[q] = pack16<T>(f);
-          }
-          if constexpr (sizeof(T) == 2)
+          for (int i = 0; i < 4; ++i) {
+            const int c = c0 + i * 8 * lpr;
+            if (c >= m.dp) break;
+            uint4 w = u[i];
             if (m.scale) {
               float f[8];
-              unpack16(u[q], f, T());
+              unpack16(w, f, T());
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] *= g;
-              u[q] = pack16<T>(f);
+              for (int x = 0; x < 8; ++x) f[x] *= g;
+              w = pack16<T>(f);
             }
-          if (c < m.dp) *reinterpret_cast<uint4*>(out + c) = u[q];
+            *reinterpret_cast<uint4*>(out + to * m.dp + c) = w;
+          }
         }
       }
     } else {
       for (int c = sub * 8; c < m.dp; c += 8 * lpr) {
         float f[8];
-        if (slot >= 0) {
-          load8(s, c, m.d, m.vec != 0, f);
-        } else {
+        load8(s, c, m.d, m.vec != 0, m.lo, m.hi, f);
+        for (int j = 0; j < copies; ++j) {
+          const int64_t to = scatter ? slot_row[row * copies + j] : row;
+          if (to < 0) continue;
+          float v[8];
+          const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = 0.f;
+          for (int x = 0; x < 8; ++x) v[x] = f[x] * g;
+          store_planes<T>(out, m.plane, to * m.dp + c, v);
         }
-        if (m.scale)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= g;
-        store_planes<T>(out, m.plane, c, f);
       }
     }
   }
@@ -440,24 +491,24 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
     }
     return;
   }
-  if constexpr (V == 1) {                        // odd widths: a warp per token, four columns a lane in flight
-    const int lane = threadIdx.x & 31;
-    for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)sum_blocks * 8) {
-      const unsigned have = __ballot_sync(0xffffffffu, lane < k && slot_row[t * k + (lane < k ? lane : 0)] >= 0);
-      for (int c0 = lane; c0 < d; c0 += 128) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (V == 1) {                        // odd widths: a warp per token and 128 columns, four a lane in flight
+    const int lane = threadIdx.x & 31, nch = (d + 127) / 128;
+    const int64_t items = tokens * nch;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)sum_blocks * 8) {
+      const int64_t t = it / nch;
+      const int c0 = (int)(it - t * nch) * 128 + lane;
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int j = 0; j < k; ++j) {
-          const bool ok = j < 32 ? (have >> j) & 1u : slot_row[t * k + j] >= 0;
-          const T* p = buf + (t * k + j) * ldb;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (ok && c0 + 32 * q < d) s[q] += to_f(p[c0 + 32 * q]);
-        }
+      for (int j = 0; j < k; ++j) {
+        const bool ok = slot_row[t * k + j] >= 0;
+        const T* p = buf + (t * k + j) * ldb;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (c0 + 32 * q < d) out[t * d + c0 + 32 * q] = from_f<T>(s[q]);
+          if (ok && c0 + 32 * q < d) s[q] += to_f(p[c0 + 32 * q]);
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (c0 + 32 * q < d) out[t * d + c0 + 32 * q] = from_f<T>(s[q]);
     }
     return;
   }
@@ -634,22 +685,31 @@ static int x_types(int dtype, const F& f) {
   return dtype == MB_BF16 ? f(bf16()) : f(f16());
 }
 
-static XMove move_gather(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const float* scale,
-                         void* out) {
+static XMove move_rows(int kind, const XShape& s, const void* src, int64_t rows, int64_t lds, int d, int dp, int64_t plane,
+                       void* out) {
+  const int size = dtype_size(s.dtype);
   XMove m{};
-  m.kind = MOVE_GATHER;
-  m.d = d; m.dp = dp; m.kdiv = kdiv; m.vec = aligned16(src) && lds % 8 == 0;
-  m.rows = s.rows; m.lds = lds; m.plane = s.rows * dp;
-  m.src = src; m.scale = scale; m.out = out;
+  m.kind = kind;
+  m.d = d; m.dp = dp; m.kdiv = 1; m.vec = aligned16(src) && lds % 8 == 0;
+  m.rows = rows; m.lds = lds; m.plane = plane;
+  m.src = src; m.out = out;
+  m.lo = (const char*)src;
+  m.hi = m.lo + ((rows - 1) * lds + d) * size;
+  return m;
+}
+static XMove move_scatter(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const float* scale,
+                          void* out) {
+  XMove m = move_rows(MOVE_SCATTER, s, src, s.R / kdiv, lds, d, dp, s.rows * dp, out);
+  m.kdiv = kdiv;
+  m.scale = scale;
   return m;
 }
 static XMove move_stage(const XShape& s, const void* w, void* out) {
-  XMove m{};
-  m.kind = MOVE_STAGE;
-  m.d = s.D; m.dp = s.Dp; m.kdiv = 1; m.vec = aligned16(w) && s.D % 8 == 0;
-  m.rows = (int64_t)s.E * s.O; m.lds = s.D; m.plane = m.rows * s.Dp;
-  m.src = w; m.out = out;
-  return m;
+  const int64_t rows = (int64_t)s.E * s.O;
+  return move_rows(MOVE_STAGE, s, w, rows, s.D, s.D, s.Dp, rows * s.Dp, out);
+}
+static XMove move_pad(const XShape& s, int dp, void* out) {
+  return move_rows(MOVE_PAD, s, nullptr, (int64_t)s.E * XP_BM, 0, 0, dp, s.rows * dp, out);
 }
 static XMove move_zero(const XShape& s, void* out, int d) {
   XMove m{};
@@ -662,9 +722,14 @@ static XMove move_zero(const XShape& s, void* out, int d) {
 // Blocks in proportion to the vectors that each job moves
 template <typename T>
 static int x_moves(const XShape& s, XMoves& mv, const int32_t* plan, cudaStream_t st) {
-  int64_t units[4], all = 0;
+  if (mv.n > XMOVES) {
+    set_error("expert_linear: %d row jobs in one launch", mv.n);
+    return MB_E_ARG;
+  }
+  int64_t units[XMOVES], all = 0;
   for (int q = 0; q < mv.n; ++q) {
-    units[q] = (mv.m[q].rows * (mv.m[q].dp / 8) + 255) / 256;
+    const bool pad = mv.m[q].kind == MOVE_PAD;   // half of the candidates on average, written only
+    units[q] = (mv.m[q].rows * mv.m[q].kdiv * (mv.m[q].dp / 8) / (pad ? 4 : 1) + 255) / 256;
     all += units[q];
   }
   const int64_t most = (int64_t)16 * sm_count();
@@ -685,7 +750,7 @@ static int x_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, 
                       const float* dgpart, int nparts, float* dg, cudaStream_t st) {
   constexpr int V = kVec<T>;
   const bool vec = d % V == 0 && aligned16(out);
-  const unsigned nb = buf ? x_grid(vec ? (tokens * (d / V) + 255) / 256 : (tokens + 7) / 8) : 0;
+  const unsigned nb = buf ? x_grid(vec ? (tokens * (d / V) + 255) / 256 : (tokens * ((d + 127) / 128) + 7) / 8) : 0;
   const unsigned ng = dg ? x_grid((tokens * k + 255) / 256) : 0;
   if (vec)
     k_rows_sum<T, V><<<nb + ng, 256, 0, st>>>(buf, ldb, out, tokens, k, d, slot_row, nb, dgpart, nparts, dg);
@@ -798,9 +863,9 @@ extern "C" int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x
     using T = decltype(t);
     const bool sum = f.y >= 0;
     XMoves mv{};
-    mv.m[mv.n++] = move_gather(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, nullptr, base + f.xs);
-    if (!direct) mv.m[mv.n++] = move_stage(s, w, base + f.ws);
-    if (!sum) mv.m[mv.n++] = move_zero(s, out, O);
+    mv.add(move_scatter(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, nullptr, base + f.xs));
+    if (!direct) mv.add(move_stage(s, w, base + f.ws));
+    if (!sum) mv.add(move_zero(s, out, O));
     if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
     XGemm g{};
     g.mode = XG_FWD; g.dtype = dtype;
@@ -840,11 +905,16 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
     using T = decltype(t);
     const bool sum = b.dxb >= 0;
     XMoves mv{};
-    mv.m[mv.n++] = move_gather(s, dy, O, O, s.Op, ky, nullptr, base + b.dys);
-    // the weights scale the rows of x, not those of dy: dy stays exact for dx and dweights, and x is read only here
-    if (dw) mv.m[mv.n++] = move_gather(s, x, ldx, D, s.Dp, kx, weights, base + b.xs);
-    if (b.ws >= 0) mv.m[mv.n++] = move_stage(s, w, base + b.ws);
-    if (dx && !sum) mv.m[mv.n++] = move_zero(s, dx, D);
+    mv.add(move_scatter(s, dy, O, O, s.Op, ky, nullptr, base + b.dys));
+    // the weights scale the rows of x, not those of dy: dy stays exact for dx and dweights, and x is read only here.
+    // dW sums over whole segments: their padding rows are zeros in both operands (elsewhere a padding row is never stored).
+    if (dw) {
+      mv.add(move_scatter(s, x, ldx, D, s.Dp, kx, weights, base + b.xs));
+      mv.add(move_pad(s, s.Op, base + b.dys));
+      mv.add(move_pad(s, s.Dp, base + b.xs));
+    }
+    if (b.ws >= 0) mv.add(move_stage(s, w, base + b.ws));
+    if (dx && !sum) mv.add(move_zero(s, dx, D));
     if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
     if (dw) {
       XGemm g{};

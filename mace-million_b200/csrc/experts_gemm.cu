@@ -48,9 +48,10 @@ struct XgCfg {
   static constexpr int STAGES = 196608 / STAGE;
   static constexpr int ACC = PL == 3 ? 2 * BN : BN;          // TMEM columns of an accumulator (fp32: both of them)
   static constexpr int TMEM = 2 * ACC;
-  static constexpr int PRE = 4352;                           // [E + 1] first item of each expert (WGRAD)
+  // WGRAD, per expert, longest first: first item [E + 1], expert, first row, K blocks
+  static constexpr int PRE = (4 * MB_PLAN_MAX_EXPERTS + 1) * 4 + 252;
   static constexpr int SMEM = STAGES * STAGE + XG_EPI_WARPS * XG_STG + PRE + 256 + 1024;   // + barriers, alignment slack
-  static_assert(STAGES >= 2 && STAGES <= 8 && SMEM <= 227 * 1024 && TMEM <= 512 && PRE >= 4 * (MB_PLAN_MAX_EXPERTS + 1), "shared memory");
+  static_assert(STAGES >= 2 && STAGES <= 8 && SMEM <= 227 * 1024 && TMEM <= 512 && PRE % 256 == 0, "shared memory");
 };
 
 struct XgParams {
@@ -221,14 +222,18 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
-  if (MODE == XG_WGRAD && warp == 0) {           // first item of each expert, longest first
+  int *by_ex = pre + g.E + 1, *by_row = by_ex + g.E, *by_nk = by_row + g.E;
+  if (MODE == XG_WGRAD && warp == 0) {
     int run = 0;
     for (int e0 = 0; e0 < g.E; e0 += 32) {
       const int e = e0 + lane;
       int n = 0;
       if (e < g.E) {
-        const int nk = (plan[g.lay.o_cnt + plan[g.lay.o_order + e]] + XG_BK - 1) / XG_BK;
+        const int ex = plan[g.lay.o_order + e], nk = (plan[g.lay.o_cnt + ex] + XG_BK - 1) / XG_BK;
         n = nk <= g.kc ? 1 : (nk + g.kc - 1) / g.kc;
+        by_ex[e] = ex;
+        by_row[e] = plan[g.lay.o_seg + ex];
+        by_nk[e] = nk;
       }
       int inc = n;
 #pragma unroll
@@ -269,10 +274,10 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         else
           hi = mid - 1;
       }
-      o.e = plan[g.lay.o_order + lo];
-      const int nk = (plan[g.lay.o_cnt + o.e] + XG_BK - 1) / XG_BK, parts = pre[lo + 1] - pre[lo], q = item - pre[lo];
+      o.e = by_ex[lo];
+      const int nk = by_nk[lo], parts = pre[lo + 1] - pre[lo], q = item - pre[lo];
       const int k0 = (int)((int64_t)nk * q / parts);
-      o.r0 = plan[g.lay.o_seg + o.e] + k0 * XG_BK;
+      o.r0 = by_row[lo] + k0 * XG_BK;
       o.nk = (int)((int64_t)nk * (q + 1) / parts) - k0;
       if (parts > 1) o.part = item;
     } else {
@@ -299,10 +304,12 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       bool ok = true;
       const uint32_t b_bytes = B_MN ? (uint32_t)((bh + 63) / 64) * 8192u : (uint32_t)bh * 128u;
       const uint32_t bytes = CG * C::PL * (C::A_BYTES + b_bytes);
+      XgTile next{};
+      if (tile_at(0) < tiles) next = tile_of(tile_at(0));
       for (int r = 0; ok && r < rounds; ++r) {
-        const int t = tile_at(r);
-        if (t >= tiles) break;                   // only in the last round
-        const XgTile w = tile_of(t);
+        if (tile_at(r) >= tiles) break;          // only in the last round
+        const XgTile w = next;
+        if (tile_at(r + 1) < tiles) next = tile_of(tile_at(r + 1));   // its table look-ups overlap this tile
         for (int kb = 0; kb < w.nk; ++kb, ++seq) {
           const int s = seq % C::STAGES;
           if (*failed || !mbar_wait_ns(&B.empty[s], ((seq / C::STAGES) & 1) ^ 1, XG_WAIT_NS)) {

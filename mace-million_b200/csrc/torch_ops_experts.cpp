@@ -2,6 +2,7 @@
 // autograd formulas.  As in torch_ops.cpp, the ops check devices, types and shapes with TORCH_CHECK, launch on torch's
 // current CUDA stream and allocate outputs and workspaces with torch's caching allocator.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -39,6 +40,7 @@ void on_device(const Tensor& t, const char* name, const Tensor& like) {
 
 bool given(const OptTensor& t) { return t && t->defined(); }
 const Tensor none;
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 const Tensor& or_none(const OptTensor& t) { return given(t) ? *t : none; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 template <typename T>
@@ -139,6 +141,12 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy, const Tensor
   return {dx, dw, db};
 }
 
+// An op through the dispatcher (below autograd: its device kernel, or the shape function of fake tensors)
+template <typename Sig>
+c10::TypedOperatorHandle<Sig> op_of(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " can be differentiated once: its gradients have no gradient formula");
 }
@@ -146,7 +154,8 @@ void once(const char* what) {
 struct LayerNormGrad : torch::autograd::Function<LayerNormGrad> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [y, mean, rstd] = ln_forward(x, or_none(w), or_none(b), eps, true);
+    static auto fwd = op_of<decltype(layer_norm_fwd)>("mace_b200::layer_norm_fwd");
+    auto [y, mean, rstd] = fwd.call(x, w, b, eps);
     ctx->save_for_backward({x, or_none(w), mean, rstd});
     ctx->saved_data["w"] = given(w);
     ctx->saved_data["b"] = given(b);
@@ -159,8 +168,10 @@ struct LayerNormGrad : torch::autograd::Function<LayerNormGrad> {
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     // needs_input_grad counts the tensors that were given
     const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["b"].toBool();
-    auto [dx, dw, db] = layer_norm_bwd(g[0], s[0], s[1], s[2], s[3], ctx->needs_input_grad(0),
-                                       has_w && ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(1 + has_w), ctx->saved_data["b_f32"].toBool());
+    static auto bwd = op_of<decltype(layer_norm_bwd)>("mace_b200::layer_norm_bwd");
+    auto [dx, dw, db] = bwd.call(g[0], s[0], opt(s[1]), s[2], s[3], ctx->needs_input_grad(0),
+                                 has_w && ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(1 + has_w),
+                                 ctx->saved_data["b_f32"].toBool());
     return {dx, dw, db, Tensor()};
   }
 };
@@ -178,7 +189,8 @@ Tensor layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor&
     return LayerNormGrad::apply(x, w, b, eps);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return layer_norm(x, w, b, eps);
+  static auto op = op_of<decltype(layer_norm)>("mace_b200::layer_norm");
+  return op.call(x, w, b, eps);
 }
 
 // ------------------------------------------------------------------------------------------------ routing
@@ -243,7 +255,8 @@ struct RouteGrad : torch::autograd::Function<RouteGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& bias, int64_t k, bool softmax,
                                int64_t groups, int64_t top_groups, bool renormalize, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [w, e] = route(logits, bias, k, softmax, groups, top_groups, renormalize, scale);
+    static auto op = op_of<decltype(route)>("mace_b200::route");
+    auto [w, e] = op.call(logits, bias, k, softmax, groups, top_groups, renormalize, scale);
     ctx->save_for_backward({logits, e});
     ctx->saved_data["softmax"] = softmax;
     ctx->saved_data["renormalize"] = renormalize;
@@ -255,9 +268,10 @@ struct RouteGrad : torch::autograd::Function<RouteGrad> {
     once("route");
     auto s = ctx->get_saved_variables();
     variable_list out(8);
+    static auto bwd = op_of<decltype(route_bwd)>("mace_b200::route_bwd");
     if (g[0].defined())
-      out[0] = route_bwd(g[0], s[0], s[1], ctx->saved_data["softmax"].toBool(), ctx->saved_data["renormalize"].toBool(),
-                         ctx->saved_data["scale"].toDouble());
+      out[0] = bwd.call(g[0], s[0], s[1], ctx->saved_data["softmax"].toBool(), ctx->saved_data["renormalize"].toBool(),
+                        ctx->saved_data["scale"].toDouble());
     return out;
   }
 };
@@ -269,7 +283,8 @@ std::tuple<Tensor, Tensor> route_autograd(const Tensor& logits, const OptTensor&
     return {r[0], r[1]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return route(logits, bias, k, softmax, groups, top_groups, renormalize, scale);
+  static auto op = op_of<decltype(route)>("mace_b200::route");
+  return op.call(logits, bias, k, softmax, groups, top_groups, renormalize, scale);
 }
 
 // ------------------------------------------------------------------------------------------------ expert products
@@ -391,14 +406,16 @@ struct ExpertLinearGrad : torch::autograd::Function<ExpertLinearGrad> {
                         const OptTensor& weights) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->save_for_backward({x, w, experts, plan, or_none(weights)});
-    return expert_linear(x, w, experts, plan, weights);
+    static auto op = op_of<decltype(expert_linear)>("mace_b200::expert_linear");
+    return op.call(x, w, experts, plan, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("expert_linear");
     auto s = ctx->get_saved_variables();
     if (!g[0].defined()) return variable_list(5);
-    auto [dx, dw, dg] = expert_linear_bwd(g[0], s[0], s[1], s[2], s[3], s[4], ctx->needs_input_grad(0),
-                                          ctx->needs_input_grad(1), s[4].defined() && ctx->needs_input_grad(4));
+    static auto bwd = op_of<decltype(expert_linear_bwd)>("mace_b200::expert_linear_bwd");
+    auto [dx, dw, dg] = bwd.call(g[0], s[0], s[1], s[2], s[3], opt(s[4]), ctx->needs_input_grad(0),
+                                 ctx->needs_input_grad(1), s[4].defined() && ctx->needs_input_grad(4));
     return {dx, dw, Tensor(), Tensor(), dg};
   }
 };
@@ -406,11 +423,13 @@ struct ExpertLinearGrad : torch::autograd::Function<ExpertLinearGrad> {
 Tensor expert_linear_autograd(const Tensor& x, const Tensor& w, const Tensor& experts, const OptTensor& plan,
                               const OptTensor& weights) {
   if (wants_grad({&x, &w, &or_none(weights)})) {
-    Tensor p = given(plan) ? *plan : expert_plan(experts, w.size(0));
+    static auto make = op_of<decltype(expert_plan)>("mace_b200::expert_plan");
+    Tensor p = given(plan) ? *plan : make.call(experts, w.size(0));
     return ExpertLinearGrad::apply(x, w, experts, p, weights);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return expert_linear(x, w, experts, plan, weights);
+  static auto op = op_of<decltype(expert_linear)>("mace_b200::expert_linear");
+  return op.call(x, w, experts, plan, weights);
 }
 
 }  // namespace

@@ -186,6 +186,32 @@ def _register_python_side(torch):
     def _ln_fake(x, weight, bias, eps):
         return x.new_empty(x.shape)
 
+    @tl.register_fake("mace_b200::layer_norm_fwd")
+    def _ln_fwd_fake(x, weight, bias, eps):
+        rows = x.numel() // x.shape[-1]
+        return (x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32),
+                x.new_empty((rows,), dtype=torch.float32))
+
+    @tl.register_fake("mace_b200::layer_norm_bwd")
+    def _ln_bwd_fake(dy, x, weight, mean, rstd, need_x, need_w, need_b, bias_f32):
+        dt = weight.dtype if weight is not None else torch.float32 if bias_f32 else x.dtype
+        par = [x.new_empty((x.shape[-1],), dtype=dt) for _ in range(2)]
+        return x.new_empty(x.shape), par[0], par[1]
+
+    @tl.register_fake("mace_b200::route_bwd")
+    def _route_bwd_fake(dweights, logits, experts, softmax, renormalize, scale):
+        return logits.new_empty(logits.shape)
+
+    @tl.register_fake("mace_b200::expert_plan")
+    def _plan_fake(experts, n_experts):
+        words = c_i64()
+        check(lib().mace_b200_expert_plan_words(experts.numel(), n_experts, ctypes.byref(words)), "expert_plan")
+        return experts.new_empty((words.value,))
+
+    @tl.register_fake("mace_b200::expert_linear_bwd")
+    def _expert_bwd_fake(dy, x, w, experts, plan, weights, need_x, need_w, need_weights):
+        return x.new_empty(x.shape), w.new_empty(w.shape), x.new_empty(experts.shape, dtype=torch.float32)
+
     @tl.register_fake("mace_b200::route")
     def _route_fake(logits, bias, k, softmax, groups, top_groups, renormalize, scale):
         shape = (logits.shape[0], k)

@@ -639,6 +639,11 @@ class ThreePassEngine:
 
     _PASSES = ("A", "xchg_fwd", "B", "xchg_rev", "C", "finalize")
 
+    def node_features(self, plan: Plan) -> torch.Tensor:
+        """Layer-1 features H1 [nt, 4, 128] (0e | 1o) of the last evaluation of `plan`: the engine's buffer, which the
+        next evaluation overwrites."""
+        return self._get("H1", (plan.nt, 4, C), torch.float32)
+
     def _pass_marks(self):
         if self._marks is None:
             self._marks = [torch.cuda.Event(enable_timing=True) for _ in range(len(self._PASSES) + 1)]

@@ -111,3 +111,99 @@ def expert_linear(x, w, plan, weights=None):
     slots = plan.experts.numel()
     few = not grad and slots <= FEW_SLOTS and slots * w[0].numel() * w.element_size() <= FEW_BYTES
     return _op("expert_linear")(x, w, plan.experts, None if few else plan.words, weights)
+
+
+class ExpertBlock(torch.nn.Module):
+    """Layer norm, router and a two-layer expert network per atom: out_t = sum_j g_tj W2[e_tj] silu(W1[e_tj] norm(x_t)).
+
+    x [T, dim] (rows may be strided) -> [T, out].  The router's bias (a buffer) only ranks; `balance` moves it towards
+    an even load after a step, so no loss term is needed for it."""
+
+    def __init__(self, dim, hidden, out, n_experts, k, score="sigmoid", dtype=torch.float32, device="cuda", seed=0):
+        super().__init__()
+        g = torch.Generator().manual_seed(seed)
+
+        def par(*shape, scale):
+            return torch.nn.Parameter((torch.randn(*shape, generator=g) * scale).to(device=device, dtype=dtype))
+
+        self.n_experts, self.k, self.score = int(n_experts), int(k), score
+        self.gamma = torch.nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+        self.beta = torch.nn.Parameter(torch.zeros(dim, device=device, dtype=dtype))
+        self.router = par(n_experts, dim, scale=dim ** -0.5)
+        self.w1 = par(n_experts, hidden, dim, scale=dim ** -0.5)
+        self.w2 = par(n_experts, out, hidden, scale=hidden ** -0.5)
+        self.register_buffer("bias", torch.zeros(n_experts, device=device))
+        self.plan = None                            # of the last forward call
+
+    def forward(self, x):
+        xn = layer_norm(x, self.gamma, self.beta)
+        weights, experts = route(xn @ self.router.T, self.k, bias=self.bias, score=self.score)
+        self.plan = plan = plan_experts(experts, self.n_experts)
+        h = torch.nn.functional.silu(expert_linear(xn, self.w1, plan))
+        return expert_linear(h, self.w2, plan, weights)
+
+    @torch.no_grad()
+    def balance(self, rate=1e-3):
+        """Raises the bias of experts that got less than the mean load in the last call, lowers the others'."""
+        load = torch.bincount(self.plan.experts.flatten() + 1, minlength=self.n_experts + 1)[1:].float()
+        self.bias += rate * torch.sign(load.mean() - load)
+        return load
+
+
+def train_readout(n=8, n_experts=8, k=2, hidden=64, steps=200, lr=3e-3, dtype=torch.float32, seed=0):
+    """Trains an ExpertBlock to give the per-atom energies of the model from its layer-1 scalar features H1[:, 0e] of a
+    water box of 3 n^3 atoms (random-init weights).  Returns a dict of what happened."""
+    import time
+
+    from . import model as M
+    from . import neighbors, structures
+    from .engine import ThreePassEngine
+
+    mdl = M.default_model(seed)
+    pos, Z, box = structures.water_box(n, seed=seed)
+    cols = structures.species_columns(Z, mdl.arch.atomic_numbers)
+    pi, pj, rij = neighbors.neighbor_list(pos, box, mdl.arch.r_max)
+    eng = ThreePassEngine(mdl, sorted(set(cols.tolist())), chunk=min(16384, len(Z)), device="cuda")
+    plan = eng.plan(pi, pj, rij, torch.as_tensor(cols), len(Z), len(Z))
+    eat, _ = eng.evaluate(plan)
+    h1 = eng.node_features(plan)
+    e = eat.double()
+    target = ((e - e.mean()) / e.std()).float()[:, None].to(dtype)
+    x = h1.to(dtype)[:, 0]                          # the 0e block: rows 512 apart
+    block = ExpertBlock(128, hidden, 1, n_experts, k, dtype=dtype, seed=seed)
+    opt = torch.optim.Adam(block.parameters(), lr=lr)
+    losses = []
+    t0 = time.perf_counter()
+    for _ in range(steps):
+        opt.zero_grad()
+        loss = torch.nn.functional.mse_loss(block(x).float(), target.float())
+        loss.backward()
+        opt.step()
+        load = block.balance(1e-2)
+        losses.append(loss.detach())
+    torch.cuda.synchronize()
+    dt = time.perf_counter() - t0
+    block.plan.check()
+    return {"atoms": len(Z), "experts": n_experts, "k": k, "steps": steps, "dtype": str(dtype).split(".")[-1],
+            "loss_first": float(losses[0]), "loss_last": float(losses[-1]), "steps_per_s": steps / dt,
+            "load": [int(v) for v in load.tolist()]}
+
+
+def main():
+    import argparse
+    import json
+
+    ap = argparse.ArgumentParser(description="Train a mixture-of-experts readout over layer-1 features of a water box")
+    ap.add_argument("--n", type=int, default=8, help="molecules along an edge (3 n^3 atoms)")
+    ap.add_argument("--experts", type=int, default=8)
+    ap.add_argument("--k", type=int, default=2)
+    ap.add_argument("--hidden", type=int, default=64)
+    ap.add_argument("--steps", type=int, default=200)
+    ap.add_argument("--lr", type=float, default=3e-3)
+    ap.add_argument("--dtype", default="float32", choices=["float32", "bfloat16", "float16"])
+    a = ap.parse_args()
+    print(json.dumps(train_readout(a.n, a.experts, a.k, a.hidden, a.steps, a.lr, getattr(torch, a.dtype))))
+
+
+if __name__ == "__main__":
+    main()

@@ -530,3 +530,73 @@ def test_expert_linear_refusals():
         X.expert_linear(x, w[:2], plan)
     with pytest.raises(TypeError, match="ExpertPlan"):
         X.expert_linear(x, w, ex)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_expert_block_matches_the_fp64_forms():
+    g = _gen(21)
+    T, D, F, O, E, k = 45, 96, 40, 24, 6, 2
+    block = X.ExpertBlock(D, F, O, E, k, seed=3)
+    x = torch.randn(T, 4, D, generator=g)
+    dy = torch.randn(T, O, generator=g)
+    xd = _cuda(x, True)
+    out = block(xd[:, 1])
+    names = ["gamma", "beta", "router", "w1", "w2"]
+    grads = torch.autograd.grad(out, [xd] + [getattr(block, n) for n in names], dy.cuda())
+    p = {n: getattr(block, n).detach().double().cpu().requires_grad_() for n in names}
+    x64 = x.double().requires_grad_()
+    xs = x64[:, 1]
+    c = xs - xs.mean(1, keepdim=True)
+    xn = c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5) * p["gamma"] + p["beta"]
+    ex = block.plan.experts.cpu().long()
+    w = R.route_weights(xn @ p["router"].T, ex, "sigmoid")
+    h = torch.nn.functional.silu(torch.einsum("td,tkfd->tkf", xn, p["w1"][ex]))
+    ref = (w[..., None] * torch.einsum("tkf,tkof->tko", h, p["w2"][ex])).sum(1)
+    want = torch.autograd.grad(ref, [x64] + [p[n] for n in names], dy.double())
+    assert (out.detach().double().cpu() - ref).abs().max() <= 2e-5 * ref.abs().max()
+    for a, b in zip(grads, want):
+        # a chain of six fp32 operators, each within a few 1e-7 of its largest value
+        assert (a.double().cpu() - b).abs().max() <= 2e-5 * b.abs().max()
+    load = block.balance(0.5)
+    assert int(load.sum()) == T * k and torch.equal(block.bias.cpu(), 0.5 * torch.sign(load.mean() - load).cpu())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_train_readout_learns(dt):
+    r = X.train_readout(n=4, n_experts=4, k=2, hidden=32, steps=60, dtype=DT[dt])
+    assert r["atoms"] == 192 and sum(r["load"]) == 384
+    assert r["loss_last"] < 0.5 * r["loss_first"]
+
+
+def test_experts_command_line(capsys, monkeypatch):
+    import json
+
+    monkeypatch.setattr("sys.argv", ["experts", "--n", "4", "--steps", "3", "--experts", "5", "--k", "1"])
+    X.main()
+    assert json.loads(capsys.readouterr().out)["experts"] == 5
+
+
+def test_operators_replay_in_a_cuda_graph():
+    """No call synchronises or depends on values read back: the whole chain is capturable, and a replay follows new inputs."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(300, 64, device="cuda", generator=g)
+    gamma, wr = torch.ones(64, device="cuda"), torch.randn(8, 64, device="cuda", generator=g)
+    w = torch.randn(8, 72, 64, device="cuda", generator=g) / 8
+
+    def chain():
+        xn = X.layer_norm(x, gamma)
+        wts, ex = X.route(xn @ wr.T, 2)
+        return N.ops().expert_linear(xn, w, ex, N.ops().expert_plan(ex, 8), wts)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = chain()
+    for seed in (6, 7):
+        x.copy_(torch.randn(300, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, chain())
