@@ -287,6 +287,20 @@ static int plan_one(const int32_t* experts, const XPlan& p, int32_t* plan, cudaS
 }
 
 // ------------------------------------------------------------------------------------------------ row movement
+// bytes [at, at + 16) of eight words, at = 0 .. 16 and even
+__device__ __forceinline__ uint4 take16(uint32_t (&w)[8], unsigned at) {
+  if (at & 16) return make_uint4(w[4], w[5], w[6], w[7]);
+  if (at & 8)
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (at & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const unsigned sh = (at & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+
 // 16 bytes at any even address: two aligned vectors and a shift.  [lo, hi): the bytes that may be read; where an aligned
 // vector would leave them the bytes come one element at a time.
 __device__ __forceinline__ uint4 load16_any(const uint16_t* p, const char* lo, const char* hi) {
@@ -302,15 +316,7 @@ __device__ __forceinline__ uint4 load16_any(const uint16_t* p, const char* lo, c
   }
   const uint4 u = reinterpret_cast<const uint4*>(base)[0], v = reinterpret_cast<const uint4*>(base)[1];
   uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-  if (s & 8)
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  if (s & 4)
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  const unsigned sh = (s & 2) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
-                    __funnelshift_r(w[3], w[4], sh));
+  return take16(w, s);
 }
 
 // 8 columns [c, c + 8) of a row of d elements as floats (0 beyond d); vec: 16-byte loads are aligned
@@ -389,7 +395,7 @@ struct XMoves {
 
 // Narrow rows share a warp (lpr lanes a row, a power of two); wide ones take several passes, four vectors in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_t* plan, const XPlan p) {
+__global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int32_t* plan, const XPlan p) {
   int q = 0;
   while (q + 1 < mv.n && blockIdx.x >= mv.m[q + 1].block0) ++q;
   const XMove& m = mv.m[q];
@@ -428,31 +434,33 @@ __global__ void __launch_bounds__(256) k_rows_move(const XMoves mv, const int32_
   for (int64_t row = warp0 * rpw + lane / lpr; row < m.rows; row += warps * rpw) {
     const T* s = (const T*)m.src + row * m.lds;
     if constexpr (sizeof(T) == 2) {
+      const bool whole = m.vec && m.d == m.dp;   // every piece is an aligned vector
       for (int c0 = sub * 8; c0 < m.dp; c0 += 32 * lpr) {
         uint4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = c0 + i * 8 * lpr;
-          if (c < m.dp) u[i] = load8_raw<T>(s, c, m.d, m.vec != 0, m.lo, m.hi);
+          if (c < m.dp) u[i] = whole ? *reinterpret_cast<const uint4*>(s + c) : load8_raw<T>(s, c, m.d, m.vec != 0, m.lo, m.hi);
         }
-#pragma unroll 4
         for (int j = 0; j < copies; ++j) {
           const int64_t to = scatter ? slot_row[row * copies + j] : row;
           if (to < 0) continue;
-          const float g = m.scale ? m.scale[row * copies + j] : 1.f;
+          uint16_t* o = out + to * m.dp + c0;
+          if (m.scale) {
+            const float g = m.scale[row * copies + j];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = c0 + i * 8 * lpr;
-            if (c >= m.dp) break;
-            uint4 w = u[i];
-            if (m.scale) {
-              float f[8];
-              unpack16(w, f, T());
+            for (int i = 0; i < 4; ++i)
+              if (c0 + i * 8 * lpr < m.dp) {
+                float f[8];
+                unpack16(u[i], f, T());
 #pragma unroll
-              for (int x = 0; x < 8; ++x) f[x] *= g;
-              w = pack16<T>(f);
-            }
-            *reinterpret_cast<uint4*>(out + to * m.dp + c) = w;
+                for (int x = 0; x < 8; ++x) f[x] *= g;
+                *reinterpret_cast<uint4*>(o + i * 8 * lpr) = pack16<T>(f);
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c0 + i * 8 * lpr < m.dp) *reinterpret_cast<uint4*>(o + i * 8 * lpr) = u[i];
           }
         }
       }
@@ -491,24 +499,63 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
     }
     return;
   }
-  if constexpr (V == 1) {                        // odd widths: a warp per token and 128 columns, four a lane in flight
-    const int lane = threadIdx.x & 31, nch = (d + 127) / 128;
-    const int64_t items = tokens * nch;
-    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)sum_blocks * 8) {
-      const int64_t t = it / nch;
-      const int c0 = (int)(it - t * nch) * 128 + lane;
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int j = 0; j < k; ++j) {
-        const bool ok = slot_row[t * k + j] >= 0;
-        const T* p = buf + (t * k + j) * ldb;
+  if constexpr (V == 1) {                        // odd widths: a warp per token, aligned loads, stores shifted into place
+    constexpr int VV = kVec<T>;
+    const int lane = threadIdx.x & 31;
+    for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)sum_blocks * 8) {
+      T* o = out + t * d;
+      const int sh = (int)(reinterpret_cast<uintptr_t>(o) & 15);
+      const T* p = buf + t * k * ldb;
+      const int32_t* row = slot_row + t * k;
+      uint32_t c[4] = {0u, 0u, 0u, 0u};            // the last lane's vector of the pass before
+      for (int n0 = 0; n0 * VV - sh / (int)sizeof(T) < d; n0 += 32) {
+        const int n = n0 + lane;
+        float s[VV];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (ok && c0 + 32 * q < d) s[q] += to_f(p[c0 + 32 * q]);
+        for (int q = 0; q < VV; ++q) s[q] = 0.f;
+        if (n * VV < d)
+          for (int j0 = 0; j0 < k; j0 += 4) {
+            Raw<T, VV> r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              r[j].zero();
+              if (j0 + j < k && row[j0 + j] >= 0) r[j].load(p + (j0 + j) * ldb + n * VV);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float f[VV];
+              r[j].get(f);
+#pragma unroll
+              for (int q = 0; q < VV; ++q) s[q] += f[q];
+            }
+          }
+        const uint4 u = pack16<T>(s);
+        // bytes [16 - sh, 32 - sh) of the neighbour's vector and this one go to the aligned address 16 n - sh
+        uint32_t w[8] = {c[0], c[1], c[2], c[3], u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t up = __shfl_up_sync(0xffffffffu, w[4 + q], 1);
+          if (lane > 0) w[q] = up;
+          c[q] = __shfl_sync(0xffffffffu, w[4 + q], 31);
+        }
+        const uint4 v = take16(w, 16 - sh);
+        const int e0 = n * VV - sh / (int)sizeof(T);   // first element of the store
+        if (e0 >= 0 && e0 + VV <= d) {
+          *reinterpret_cast<uint4*>(o + e0) = v;
+        } else {
+          const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int q = 0; q < VV; ++q) {
+            if (e0 + q < 0 || e0 + q >= d) continue;
+            if constexpr (sizeof(T) == 4) {
+              o[e0 + q] = __uint_as_float(vw[q]);
+            } else {
+              const uint16_t h = (uint16_t)(vw[q / 2] >> (16 * (q & 1)));
+              reinterpret_cast<uint16_t*>(o)[e0 + q] = h;
+            }
+          }
+        }
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (c0 + 32 * q < d) out[t * d + c0 + 32 * q] = from_f<T>(s[q]);
     }
     return;
   }
@@ -750,7 +797,7 @@ static int x_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, 
                       const float* dgpart, int nparts, float* dg, cudaStream_t st) {
   constexpr int V = kVec<T>;
   const bool vec = d % V == 0 && aligned16(out);
-  const unsigned nb = buf ? x_grid(vec ? (tokens * (d / V) + 255) / 256 : (tokens * ((d + 127) / 128) + 7) / 8) : 0;
+  const unsigned nb = buf ? x_grid(vec ? (tokens * (d / V) + 255) / 256 : (tokens + 7) / 8) : 0;
   const unsigned ng = dg ? x_grid((tokens * k + 255) / 256) : 0;
   if (vec)
     k_rows_sum<T, V><<<nb + ng, 256, 0, st>>>(buf, ldb, out, tokens, k, d, slot_row, nb, dgpart, nparts, dg);

@@ -451,8 +451,11 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         }
       }
       const T* x = (const T*)g.x + n0;
-      uint4 xq[4];
-      if constexpr (DOT) xg_fetch<T>(xq, xrow, x, g.ldx, xvec, nc);
+      uint4 xq[2][4];                              // pieces of x, two ahead (the first before the wait)
+      if constexpr (DOT) {
+        xg_fetch<T>(xq[0], xrow, x, g.ldx, xvec, nc);
+        xg_fetch<T>(xq[1], xrow, x + XC, g.ldx, xvec, nc - XC);
+      }
       auto wait = [&](int acc) {
         const bool got = !__shfl_sync(0xffffffffu, *failed, 0) &&
                          __all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, XG_WAIT_NS));
@@ -487,15 +490,6 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         for (int i = 0; i < 32; ++i) v[i] = add ? v[i] + __uint_as_float(u[i]) : __uint_as_float(u[i]);
       };
       auto emit = [&](int q, const float* v) {
-        if constexpr (DOT) {
-#pragma unroll
-          for (int h = 0; h < 32 / XC; ++h) {
-            dot += xg_dot<T>(v + h * XC, stg, xq);
-            const int c = 32 * q + (h + 1) * XC;
-            if (c < nc) xg_fetch<T>(xq, xrow, x + c, g.ldx, xvec, nc - c);
-          }
-          if (!g.out) return;
-        }
         if (MODE == XG_WGRAD && pout)
           xg_emit32<float>(v, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, 1.f, nc - 32 * q);
         else
@@ -541,9 +535,18 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
           release(acc);
         }
         if (!ok) break;
+        if constexpr (DOT) {
+#pragma unroll
+          for (int h = 0; h < 32 * NG / XC; ++h) {
+            if (h * XC >= nc) break;
+            dot += xg_dot<T>(&v[h * XC / 32][h * XC % 32], stg, xq[h & 1]);
+            const int c = (h + 2) * XC;
+            if (c < nc) xg_fetch<T>(xq[h & 1], xrow, x + c, g.ldx, xvec, nc - c);
+          }
+        }
 #pragma unroll
         for (int q = 0; q < NG; ++q)
-          if (32 * q < nc) emit(q, v[q]);
+          if (32 * q < nc && (!DOT || g.out)) emit(q, v[q]);
       }
       if (DOT && slot >= 0) g.dgpart[(int64_t)(2 * (w.n0 / g.bn) + hf) * g.lay.R + slot] = dot;
     }
