@@ -125,11 +125,27 @@ __device__ __forceinline__ void xg_fetch(uint4 (&xq)[4], const int (&row)[4], co
 // Writes 32 columns of the rows that the lanes of a warp hold (v, one row per lane), scaled, through shared memory in pieces
 // of 64 bytes: global accesses are whole sectors of eight rows (one row per lane would be 32 scattered 16-byte pieces per
 // access, and held a tile for longer than its products at K <= 1024).  out: first column; left: columns that exist.
+// Everything that does not change from piece to piece is in XgLane.
+struct XgLane {
+  uint32_t own[4], seg[4];                       // staging addresses: this lane's row, piece c; row 8 i + l / 4, piece l % 4
+};
+__device__ __forceinline__ XgLane xg_lane(uint32_t stg) {
+  const int lane = threadIdx.x & 31;
+  XgLane a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a.own[i] = xg_stg(stg, lane, i);
+    a.seg[i] = xg_stg(stg, 8 * i + (lane >> 2), lane & 3);
+  }
+  return a;
+}
+
 template <typename OUT>
-__device__ __forceinline__ void xg_emit32(const float* v, uint32_t stg, const int (&row)[4], OUT* out, int64_t ldo,
-                                          bool vec, float sc, int left) {
+__device__ __forceinline__ void xg_emit32(const float* v, const XgLane& a, uint32_t stg, const int (&row)[4], OUT* out,
+                                          int64_t ldo, bool vec, float sc, int left) {
   constexpr int NC = 64 / (int)sizeof(OUT), OV = kVec<OUT>;   // columns of a piece, of a vector
-  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
+  const int lane = threadIdx.x & 31, c4 = lane & 3;
+  const bool whole = vec && left >= 32;
 #pragma unroll
   for (int h = 0; h < 32 / NC; ++h) {
     const int n = left - h * NC;
@@ -139,32 +155,36 @@ __device__ __forceinline__ void xg_emit32(const float* v, uint32_t stg, const in
       float f[OV];
 #pragma unroll
       for (int q = 0; q < OV; ++q) f[q] = v[h * NC + c * OV + q] * sc;
-      sts128(xg_stg(stg, lane, c), pack16<OUT>(f));
+      sts128(a.own[c], pack16<OUT>(f));
     }
     __syncwarp();
-    if (vec) {
-      const int mine = n - c4 * OV;              // columns of this lane's piece
+    if (whole) {
+      OUT* p = out + h * NC + c4 * OV;
 #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row[i] >= 0) *reinterpret_cast<uint4*>(p + row[i] * ldo) = lds128(a.seg[i]);
+    } else if (vec) {
+      const int mine = n - c4 * OV;              // columns of this lane's piece
+      OUT* p = out + h * NC + c4 * OV;
+#pragma unroll 1
       for (int i = 0; i < 4; ++i) {
-        if (row[i] < 0 || mine <= 0) continue;
-        OUT* p = out + row[i] * ldo + h * NC + c4 * OV;
-        const uint32_t s = xg_stg(stg, 8 * i + r4, c4);
+        const int at = i == 0 ? row[0] : i == 1 ? row[1] : i == 2 ? row[2] : row[3];
+        const uint32_t s = xg_stg(stg, 8 * i + (lane >> 2), c4);
+        if (at < 0) continue;
         if (mine >= OV)
-          *reinterpret_cast<uint4*>(p) = lds128(s);
+          *reinterpret_cast<uint4*>(p + at * ldo) = lds128(s);
         else
-          for (int q = 0; q < mine; ++q) p[q] = xg_elem<OUT>(s, q);
+          for (int q = 0; q < mine; ++q) p[at * ldo + q] = xg_elem<OUT>(s, q);
       }
     } else {                                     // odd strides: one row at a time (two of 16 columns), lanes along it
       constexpr int RP = 32 / NC;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll 2
-        for (int r = 0; r < 8; r += RP) {
-          const int rr = r + lane / NC, c = lane % NC;
-          const int at = __shfl_sync(0xffffffffu, row[i], rr * 4);
-          if (at >= 0 && c < n)
-            out[at * ldo + h * NC + c] = xg_elem<OUT>(xg_stg(stg, 8 * i + rr, c / OV), c % OV);
-        }
+#pragma unroll 1
+      for (int r = 0; r < 32; r += RP) {
+        const int rr = r + lane / NC, c = lane % NC, i = r >> 3;
+        const int mine = i == 0 ? row[0] : i == 1 ? row[1] : i == 2 ? row[2] : row[3];
+        const int at = __shfl_sync(0xffffffffu, mine, (rr & 7) * 4);
+        if (at >= 0 && c < n) out[at * ldo + h * NC + c] = xg_elem<OUT>(xg_stg(stg, rr, c / OV), c % OV);
+      }
     }
     __syncwarp();
   }
@@ -172,17 +192,16 @@ __device__ __forceinline__ void xg_emit32(const float* v, uint32_t stg, const in
 
 // Scalar products of the columns of the lanes' rows that a piece of x (64 bytes a row, in xq by xg_fetch) covers
 template <typename T>
-__device__ __forceinline__ float xg_dot(const float* v, uint32_t stg, const uint4 (&xq)[4]) {
-  const int lane = threadIdx.x & 31, r4 = lane >> 2, c4 = lane & 3;
+__device__ __forceinline__ float xg_dot(const float* v, const XgLane& a, const uint4 (&xq)[4]) {
   constexpr int XV = kVec<T>;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sts128(xg_stg(stg, 8 * i + r4, c4), xq[i]);
+  for (int i = 0; i < 4; ++i) sts128(a.seg[i], xq[i]);
   __syncwarp();
   float part[4];                                 // short chains, added up as a tree
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     float f[XV];
-    unpack16(lds128(xg_stg(stg, lane, c)), f, T());
+    unpack16(lds128(a.own[c]), f, T());
     part[c] = 0.f;
 #pragma unroll
     for (int q = 0; q < XV; ++q) part[c] = fmaf(f[q], v[c * XV + q], part[c]);
@@ -415,6 +434,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     const uint32_t stg = smem_u32(stg0) + (warp - XG_EPI0) * XG_STG;
     const bool vec = g.ldo % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
     const bool xvec = MODE == XG_DGRAD && g.ldx % kVec<T> == 0 && (reinterpret_cast<uintptr_t>(g.x) & 15) == 0;
+    const XgLane at = xg_lane(stg);
     constexpr int NG = BN / 64;                    // groups of 32 columns in a half row
     constexpr int XC = 32 * 2 / (int)sizeof(T);    // columns of x in a fetch (64 bytes)
     int tc = 0;
@@ -491,9 +511,9 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       };
       auto emit = [&](int q, const float* v) {
         if (MODE == XG_WGRAD && pout)
-          xg_emit32<float>(v, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, 1.f, nc - 32 * q);
+          xg_emit32<float>(v, at, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, 1.f, nc - 32 * q);
         else
-          xg_emit32<T>(v, stg, orow, out + 32 * q, ldo, vec, sc, nc - 32 * q);
+          xg_emit32<T>(v, at, stg, orow, out + 32 * q, ldo, vec, sc, nc - 32 * q);
       };
       if constexpr (acc_k == 0x3fffffff) {         // one accumulator: 32 columns at a time straight from TMEM
         const int acc = tc & 1;
@@ -539,7 +559,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
 #pragma unroll
           for (int h = 0; h < 32 * NG / XC; ++h) {
             if (h * XC >= nc) break;
-            dot += xg_dot<T>(&v[h * XC / 32][h * XC % 32], stg, xq[h & 1]);
+            dot += xg_dot<T>(&v[h * XC / 32][h * XC % 32], at, xq[h & 1]);
             const int c = (h + 2) * XC;
             if (c < nc) xg_fetch<T>(xq[h & 1], xrow, x + c, g.ldx, xvec, nc - c);
           }
