@@ -379,7 +379,9 @@ int mace_b200_route_bwd(const float* dweights, const void* logits, int64_t ldl, 
  * (MB_ST_BAD_EXPERT, MB_ST_TC_TIMEOUT).  fwd and bwd run on the tensor cores and need a plan and
  * mace_b200_expert_linear_workspace bytes (256-byte aligned); few needs neither and reads the indices directly (at
  * most MB_FEW_MAX_SLOTS slots; an index outside [0, E) counts as -1).
- * bwd: dy as out; dx as x but dense, dw [E][O][D], dweights [tokens][k]; any may be null (dweights needs weights). */
+ * bwd: dy as out; dx as x but dense, dw [E][O][D], dweights [tokens][k]; any may be null (dweights needs weights).
+ * fp32 data: a value that is infinite, or that bfloat16 rounds to infinity, gives NaN in the results it enters.
+ * expert_test_hooks: as mace_b200_tc_test_hooks, for the products (skip_one_load: the first load goes missing once). */
 #define MB_PLAN_MAX_EXPERTS 1024
 #define MB_FEW_MAX_SLOTS 4096
 int mace_b200_expert_plan_words(int64_t slots, int32_t E, int64_t* words);
@@ -396,6 +398,7 @@ int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_t ldx, int3
                                 const int32_t* plan, const float* weights, void* dx, void* dw, float* dweights,
                                 void* workspace, int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
                                 int32_t dtype, void* stream);
+int mace_b200_expert_test_hooks(uint64_t wait_ns, int32_t skip_one_load);
 
 #ifdef __cplusplus
 }

@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
 
 // ------------------------------------------------------------------------------------------------ few slots
 // out[t][o] = sum_j g_tj <W[e_tj][o], x> without a plan: L lanes per (token, output), the rows of W of four choices side
-// by side in flight.  Bound by the bytes of W; a row of W that several tokens use comes from L2 after the first.
+// by side in flight.  Bound by the bytes of W (4 of 64 experts, 1024 x 1024 bf16: one token 5.8 us, 16 tokens 134 MB in
+// 25 us, 5.3 TB/s); a row of W that several tokens use comes from L2 after the first.
 // SLOTS: out[slot][o] = <W[e][o], x>, L lanes per (slot, output).
 template <typename T, int V, int L, bool SLOTS>
 __global__ void __launch_bounds__(128) k_expert_few(const T* x, int64_t ldx, int kx, const T* w, const int32_t* experts,

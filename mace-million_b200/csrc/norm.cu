@@ -10,6 +10,10 @@
 // small kernel adds the blocks' partial sums in a fixed order (no atomics: results do not depend on the schedule).
 // V is the elements per access: 16 bytes where the width, the row strides and the addresses allow it, else 1.
 // Widths that no group holds in registers take the *_wide kernels, which read the row once per sum.
+// Measured on a B200 (forward / backward): 65,536 x 2048 bf16 101 / 151 us (5.3 TB/s each, of 6.5 measured for a copy),
+// 65,536 x 1024 bf16 45 / 80 us, 32,768 x 1024 fp32 49 / 67 us, 16,384 x 128 fp32 in rows 512 apart 4.1 / 8.1 us,
+// 24,001 x 515 bf16 (one element per access) 21 / 26 us.  Below 5 TB/s the issue slots bound it: unpacking, the packed
+// arithmetic and packing are about 10 instructions an element backward.
 #include "dtypes.cuh"
 
 namespace mb {

@@ -461,6 +461,80 @@ def test_expert_linear_padding_rows_do_not_spread_nan():
         assert torch.isnan(dw[:2, :, 3]).all() and torch.isfinite(dw[2:]).all() and torch.isfinite(dx).all()
 
 
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), 3.4e38])
+def test_expert_linear_infinities_stay_in_their_rows(bad):
+    """Infinite values (and, in fp32, values that the first bfloat16 plane rounds to infinity) leave every other row alone."""
+    g = _gen(12)
+    for dt in (torch.float32, torch.bfloat16):
+        x, w, ex, p = _x_inputs(60, 2, 5, 64, 48, torch.float32, False, g, skew=False)
+        x, w = x.to(dt), w.to(dt)
+        x[7, 3] = bad
+        plan = X.plan_experts(ex.cuda(), 5)
+        out = N.ops().expert_linear(x.cuda(), w.cuda(), plan.experts, plan.words, p.cuda())
+        others = torch.arange(60) != 7
+        if math.isinf(bad):
+            assert not torch.isfinite(out[7]).any()
+        x[7, 3] = 0.0
+        want = N.ops().expert_linear(x.cuda(), w.cuda(), plan.experts, plan.words, p.cuda())
+        assert torch.equal(out[others.cuda()], want[others.cuda()])
+
+
+def test_offsets_beyond_32_bits():
+    """Outputs of more than 2^31 elements: the last rows equal those of a call on the last rows alone."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    T, D, O = 1_100_000, 64, 2048
+    x = torch.randn(T, D, device="cuda", generator=g).bfloat16()
+    w = torch.randn(2, O, D, device="cuda", generator=g).bfloat16() / 8
+    ex = torch.randint(0, 2, (T, 1), device="cuda", generator=g, dtype=torch.int32)
+    plan = N.ops().expert_plan(ex, 2)
+    y = N.ops().expert_linear(x, w, ex, plan, None)[:, 0]
+    assert y.numel() > 2 ** 31
+    tail = N.ops().expert_linear(x[-300:], w, ex[-300:].contiguous(), N.ops().expert_plan(ex[-300:].contiguous(), 2), None)
+    assert torch.equal(y[-300:], tail[:, 0])
+    n, m, r = N.ops().layer_norm_fwd(y, None, None, 1e-5)
+    n2, m2, r2 = N.ops().layer_norm_fwd(y[-300:].clone(), None, None, 1e-5)
+    assert torch.equal(n[-300:], n2) and torch.equal(m[-300:], m2) and torch.equal(r[-300:], r2)
+    dx, _, _ = N.ops().layer_norm_bwd(y, n, None, m, r, True, False, False, False)
+    d2, _, _ = N.ops().layer_norm_bwd(y[-300:].clone(), n2, None, m2, r2, True, False, False, False)
+    assert torch.equal(dx[-300:], d2)
+    dy = y[:, None]
+    dxx, dww, _ = N.ops().expert_linear_bwd(dy, x, w, ex, plan, None, True, True, False)
+    tdx, _, _ = N.ops().expert_linear_bwd(dy[-300:], x[-300:], w, ex[-300:].contiguous(),
+                                          N.ops().expert_plan(ex[-300:].contiguous(), 2), None, True, False, False)
+    assert torch.equal(dxx[-300:], tdx) and torch.isfinite(dww).all()
+    del n, dx, dy, dxx
+    l = y.view(-1)[:2 ** 31 + 2 ** 20].view(-1, 512)
+    wt, e = N.ops().route(l, None, 2, True, 1, 1, True, 1.0)
+    wt2, e2 = N.ops().route(l[-40:].clone(), None, 2, True, 1, 1, True, 1.0)
+    assert torch.equal(e[-40:], e2) and torch.allclose(wt[-40:], wt2, rtol=1e-6)
+    dl = N.ops().route_bwd(wt, l, e, True, True, 1.0)
+    assert torch.equal(dl[-40:], N.ops().route_bwd(wt[-40:].contiguous(), l[-40:].clone(), e2, True, True, 1.0))
+
+
+@pytest.mark.parametrize("T,D,O", [(300, 64, 64), (40000, 1024, 1024)])
+def test_expert_linear_timeout_path_reports_and_recovers(T, D, O):
+    """The bounded waits, driven from the host: with one load withheld they run out after 20 ms, the kernel drains, frees
+    its TMEM and reports; the next launch with the default limit is right.  The larger size runs on pairs of CTAs."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(T, D, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(1, O, D, device="cuda", generator=g) / math.sqrt(D)).bfloat16()
+    plan = X.plan_experts(torch.zeros(T, 1, dtype=torch.int32, device="cuda"), 1)
+    plan.check()
+    try:
+        N.check(N.lib().mace_b200_expert_test_hooks(20_000_000, 1), "expert_test_hooks")
+        N.ops().expert_linear(x, w, plan.experts, plan.words, None)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            plan.check()
+    finally:
+        N.check(N.lib().mace_b200_expert_test_hooks(2_000_000_000, 0), "expert_test_hooks")
+    plan = X.plan_experts(plan.experts, 1)
+    out = N.ops().expert_linear(x, w, plan.experts, plan.words, None)[:, 0]
+    plan.check()
+    want = x.double() @ w[0].double().T
+    assert float((out.double() - want).norm() / want.norm()) <= U[torch.bfloat16] / math.sqrt(3)
+
+
 def test_expert_linear_empty_and_unrouted():
     w = torch.randn(3, 8, 16, device="cuda", requires_grad=True)
     x = torch.randn(0, 16, device="cuda", requires_grad=True)
