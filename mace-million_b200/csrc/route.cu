@@ -23,7 +23,7 @@ namespace mb {
 constexpr int RT_WARPS = 8;
 
 struct RouteArgs {
-  int32_t c, vec, all;                            // forward: experts per lane, vector loads, all scores needed
+  int32_t c, span, vec, all;                      // forward: experts per lane, lanes per group, vector loads, all scores needed
   const void* logits;
   const float *bias, *dw;
   float* w;
@@ -77,12 +77,9 @@ __global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs 
   extern __shared__ unsigned char sm_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (L - 1), base = lane & ~(L - 1);
   int* chosen = reinterpret_cast<int*>(sm_raw) + (warp * TPW + lane / L) * a.k;            // [k] of this token
-  float* val = reinterpret_cast<float*>(sm_raw) + RT_WARPS * TPW * a.k + (warp * TPW + lane / L) * a.e;  // [E]
-  const int c = a.c, i0 = sub * c;
-  const int n = i0 >= a.e ? 0 : a.e - i0 < c ? a.e - i0 : c;                               // experts of this lane
-  const int per = a.e / a.groups;
-  // a group's experts lie in the registers of a power of two of lanes: its best two by shuffles, else through `val`
-  const int span = a.groups > 1 && per % c == 0 && ((per / c) & (per / c - 1)) == 0 ? per / c : 0;
+  // a group's `per` experts lie in a.span lanes (a power of two), a.c in each but the last ones
+  const int c = a.c, span = a.span, per = a.e / a.groups, mine = sub / span, q0 = (sub - mine * span) * c;
+  const int i0 = mine * per + q0, n = mine >= a.groups || q0 >= per ? 0 : per - q0 < c ? per - q0 : c;
   const int64_t step = (int64_t)gridDim.x * RT_WARPS * TPW;
   // every lane of a warp runs the same number of passes (the collectives are warp-wide)
   for (int64_t r0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * TPW; r0 < a.t; r0 += step) {
@@ -143,82 +140,31 @@ __global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs 
       }
       if (a.groups > 1) {
         unsigned open = 0u;                       // bit g: group g stays open (up to 32 groups)
-        if (span) {
-          float m1 = -INFINITY, m2 = -INFINITY;
-          bool nan = false;
+        float m1 = -INFINITY, m2 = -INFINITY;     // the group's two best
+        bool nan = false;
 #pragma unroll
-          for (int j = 0; j < NE; ++j) {
-            nan |= s[j] != s[j];
-            m2 = fmaxf(m2, fminf(m1, s[j]));
-            m1 = fmaxf(m1, s[j]);
-          }
-          for (int o = 1; o < span; o <<= 1) {
-            const float o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
-            m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
-            m1 = fmaxf(m1, o1);
-            nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
-          }
-          unsigned gk = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
-          if (n == 0) gk = 0u;
-          const int mine = sub / span;
-          for (int q = 0; q < a.top_groups; ++q) {
-            const unsigned best = lanes_max<L>(gk);
-            const int g = lanes_first<L>(gk == best, base) / span;
-            if (best <= KEY_CLOSED) continue;     // nothing open is left for this token
-            open |= 1u << g;
-            if (g == mine) gk = 0u;
-          }
-          if (!((open >> mine) & 1u))
-#pragma unroll
-            for (int j = 0; j < NE; ++j) key[j] = 0u;
-        } else {
-#pragma unroll
-          for (int j = 0; j < NE; ++j)
-            if (j < n) val[i0 + j] = s[j];
-          __syncwarp();
-          // lane q of the token's L lanes values the groups q, q + L, ..; their keys replace the first E / per values
-          unsigned gk[32 / L > 8 ? 8 : 32 / L];
-          constexpr int GL = 32 / L > 8 ? 8 : 32 / L;
-#pragma unroll
-          for (int u = 0; u < GL; ++u) {
-            const int g = sub + u * L;
-            gk[u] = 0u;
-            if (g < a.groups) {
-              float m1 = -INFINITY, m2 = -INFINITY;
-              bool nan = false;
-#pragma unroll 4
-              for (int i = 0; i < per; ++i) {
-                const float f = val[g * per + i];
-                nan |= f != f;
-                m2 = fmaxf(m2, fminf(m1, f));
-                m1 = fmaxf(m1, f);
-              }
-              gk[u] = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
-            }
-          }
-          __syncwarp();
-          for (int q = 0; q < a.top_groups; ++q) {
-            unsigned mx = 0u;
-#pragma unroll
-            for (int u = 0; u < GL; ++u) mx = max(mx, gk[u]);
-            const unsigned best = lanes_max<L>(mx);
-            // the lowest group index that has it: groups of the lower u come first
-            int g = 64;
-#pragma unroll
-            for (int u = GL - 1; u >= 0; --u) {
-              const int f = lanes_first<L>(gk[u] == best, base);
-              if (f < 32) g = f + u * L;
-            }
-            if (best <= KEY_CLOSED) continue;
-            open |= 1u << g;
-#pragma unroll
-            for (int u = 0; u < GL; ++u)
-              if (g == sub + u * L) gk[u] = 0u;
-          }
-#pragma unroll
-          for (int j = 0; j < NE; ++j)
-            if (j < n && !((open >> ((i0 + j) / per)) & 1u)) key[j] = 0u;
+        for (int j = 0; j < NE; ++j) {
+          nan |= s[j] != s[j];
+          m2 = fmaxf(m2, fminf(m1, s[j]));
+          m1 = fmaxf(m1, s[j]);
         }
+        for (int o = 1; o < span; o <<= 1) {
+          const float o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
+          m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+          m1 = fmaxf(m1, o1);
+          nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+        }
+        unsigned gk = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
+        for (int q = 0; q < a.top_groups; ++q) {
+          const unsigned best = lanes_max<L>(gk);
+          const int g = lanes_first<L>(gk == best, base) / span;
+          if (best <= KEY_CLOSED) continue;       // nothing open is left for this token
+          open |= 1u << g;
+          if (g == mine) gk = 0u;
+        }
+        if (!((open >> (mine & 31)) & 1u))
+#pragma unroll
+          for (int j = 0; j < NE; ++j) key[j] = 0u;
       }
     }
     for (int q = 0; q < a.k; ++q) {
@@ -430,38 +376,45 @@ static int route_bwd_any(const RouteArgs& a, cudaStream_t st) {
 }
 
 template <typename T, int L, int NE>
-static int route_fwd_launch(RouteArgs a, int c, cudaStream_t st) {
+static int route_fwd_launch(RouteArgs a, cudaStream_t st) {
   constexpr int TPW = 32 / L, V = kVec<T>;
-  a.c = c;
-  a.vec = c % V == 0 && a.e % V == 0 && a.ldl % V == 0 && aligned16(a.logits);
-  // the values pass through shared memory when a group is not a power of two of lanes
-  const int per = a.e / a.groups, m = per % c == 0 ? per / c : 0;
-  const bool through = a.groups > 1 && (m == 0 || (m & (m - 1)));
-  const int smem = RT_WARPS * TPW * (a.k + (through ? a.e : 0)) * 4;
-  k_route_fwd<T, L, NE><<<route_grid(a.t, RT_WARPS * TPW, 8), 32 * RT_WARPS, smem, st>>>(a);
+  const int per = a.e / a.groups;
+  a.vec = NE % V == 0 && a.c % V == 0 && per % V == 0 && a.ldl % V == 0 && aligned16(a.logits);
+  k_route_fwd<T, L, NE><<<route_grid(a.t, RT_WARPS * TPW, 8), 32 * RT_WARPS, RT_WARPS * TPW * a.k * 4, st>>>(a);
   return check_launch("route_fwd");
 }
 
-// Lanes per token and experts per lane.  Below 8 tokens per scheduler a whole warp takes a token.
+template <typename T, int L>
+static int route_fwd_lanes(const RouteArgs& a, cudaStream_t st) {
+  if (a.c <= 4) return route_fwd_launch<T, L, 4>(a, st);
+  if (a.c <= 8) return route_fwd_launch<T, L, 8>(a, st);
+  if (a.c <= 12) return route_fwd_launch<T, L, 12>(a, st);
+  if (a.c <= 16) return route_fwd_launch<T, L, 16>(a, st);
+  return route_fwd_launch<T, 32, 32>(a, st);      // c > 16 only when 32 lanes are in use
+}
+
+// Lanes per group (a power of two) and experts per lane.  Many tokens: the fewest lanes that hold 16 experts or fewer each;
+// below 8 tokens per scheduler: as many lanes as there are, for the shortest chain.
 template <typename T>
 static int route_fwd_any(RouteArgs a, cudaStream_t st) {
+  constexpr int V = kVec<T>;
   a.all = a.bias || a.groups > 1 || (a.softmax && !a.renorm);
-  const int e = a.e;
-  const bool few = a.t < (int64_t)32 * sm_count();
-  if (few || e > 256) {
-    const int c = (e + 31) / 32;
-    if (c <= 4) return route_fwd_launch<T, 32, 4>(a, c, st);
-    return route_fwd_launch<T, 32, 16>(a, c, st);
+  const int per = a.e / a.groups;
+  int most = 1;                                   // most lanes a group can have
+  while (2 * most * a.groups <= 32) most *= 2;
+  if (a.t < (int64_t)32 * sm_count()) {
+    a.span = most;
+  } else {
+    a.span = 1;
+    while (a.span < most && (per + a.span - 1) / a.span > 16) a.span *= 2;
   }
-  // groups of 4, 8 or 16 experts fit a lane
-  const int per = a.groups > 1 ? e / a.groups : 0;
-  if (per == 8 && e > 32 && e <= 64) return route_fwd_launch<T, 8, 8>(a, 8, st);
-  if (e <= 16) return route_fwd_launch<T, 4, 4>(a, 4, st);
-  if (e <= 32) return route_fwd_launch<T, 4, 8>(a, 8, st);
-  if (e <= 64) return route_fwd_launch<T, 4, 16>(a, 16, st);
-  if (e <= 96) return route_fwd_launch<T, 8, 12>(a, 12, st);
-  if (e <= 128) return route_fwd_launch<T, 8, 16>(a, 16, st);
-  return route_fwd_launch<T, 16, 16>(a, 16, st);
+  a.c = (per + a.span - 1) / a.span;
+  if (per % V == 0) a.c = (a.c + V - 1) / V * V;  // whole vectors; the group's last lanes hold fewer
+  const int lanes = a.groups * a.span;
+  if (lanes <= 4 && a.c <= 16) return route_fwd_lanes<T, 4>(a, st);
+  if (lanes <= 8 && a.c <= 16) return route_fwd_lanes<T, 8>(a, st);
+  if (lanes <= 16 && a.c <= 16) return route_fwd_lanes<T, 16>(a, st);
+  return route_fwd_lanes<T, 32>(a, st);
 }
 
 static int route_check(const char* who, const RouteArgs& a, int dtype) {

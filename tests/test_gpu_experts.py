@@ -180,6 +180,11 @@ ROUTES = [  # E, k, score, groups, top_groups, bias, renormalize, scale
     (200, 32, "sigmoid", 4, 2, False, False, 0.5),
     (512, 16, "softmax", 32, 5, True, True, 1.0),
     (512, 3, "sigmoid", 1, 1, True, True, 1.0),
+    (50, 4, "sigmoid", 5, 2, False, True, 1.0),
+    (510, 7, "softmax", 17, 6, False, False, 1.0),
+    (510, 9, "sigmoid", 3, 2, True, True, 1.0),
+    (148, 3, "softmax", 4, 2, False, True, 1.0),
+    (96, 6, "sigmoid", 32, 9, True, False, 1.0),
 ]
 
 
@@ -217,6 +222,19 @@ def test_route_choice_weights_and_gradient(E, k, score, groups, top, bias, renor
     assert not dl[dead.cuda()].any()
     err = (dl.double().cpu() - dl0).abs()[~dead]
     assert (err <= U[DT[dt]] * dl0.abs()[~dead] + 2e-6 * scale * dw.abs().max()).all()
+
+
+@pytest.mark.parametrize("E,groups,top", [(64, 8, 4), (200, 4, 2), (200, 8, 3), (148, 4, 2), (89, 1, 1), (510, 17, 5), (12, 1, 1)])
+def test_route_many_tokens_agree_with_few(E, groups, top):
+    """Many tokens take few lanes each, few tokens a whole warp: the same choices and weights, bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(E)
+    l = torch.randn(6000, E, device="cuda", generator=g)
+    b = 0.2 * torch.randn(E, device="cuda", generator=g)
+    kw = dict(score="sigmoid", groups=groups, top_groups=top, bias=b)
+    w, e = X.route(l, 3, **kw)
+    for r in (slice(0, 40), slice(5960, 6000)):
+        w2, e2 = X.route(l[r], 3, **kw)
+        assert torch.equal(e[r], e2) and (w[r] - w2).abs().max() <= 3e-7     # sums over slots in another order
 
 
 @pytest.mark.parametrize("T", [0, 1, 7, 5000])
