@@ -479,6 +479,27 @@ def test_expert_linear_padding_rows_do_not_spread_nan():
         assert torch.isnan(dw[:2, :, 3]).all() and torch.isfinite(dw[2:]).all() and torch.isfinite(dx).all()
 
 
+def test_expert_linear_bad_gradients_stay_in_their_experts():
+    """NaN and infinities in one token's upstream gradient reach its dx, its dweights and its experts' dW only."""
+    g = _gen(14)
+    for dt in (torch.float32, torch.bfloat16):
+        for bad in (float("nan"), float("inf")):
+            x, w, ex, p = _x_inputs(200, 2, 5, 64, 48, dt, False, g, skew=False)
+            ex[0] = torch.tensor([0, 1], dtype=torch.int32)
+            ex[1:] = torch.randint(2, 5, (199, 2), generator=g, dtype=torch.int32)
+            ex[50:90, 0] = 0
+            xd, wd, pd = _cuda(x, True), _cuda(w, True), _cuda(p, True)
+            dy = torch.randn(200, 48, generator=g).to(dt)
+            dy[0, 5] = bad
+            out = X.expert_linear(xd, wd, X.plan_experts(ex.cuda(), 5), pd)
+            dx, dw, dp = torch.autograd.grad(out, (xd, wd, pd), dy.cuda())
+            assert not torch.isfinite(dx[0]).any() and torch.isfinite(dx[1:]).all()
+            assert not torch.isfinite(dp[0]).any() and torch.isfinite(dp[1:]).all()
+            assert not torch.isfinite(dw[:2, 5]).any() and torch.isfinite(dw[2:]).all()
+            rest = [o for o in range(48) if o != 5]
+            assert torch.isfinite(dw[:2, rest]).all()
+
+
 @pytest.mark.parametrize("bad", [float("inf"), -float("inf"), 3.4e38])
 def test_expert_linear_infinities_stay_in_their_rows(bad):
     """Infinite values (and, in fp32, values that the first bfloat16 plane rounds to infinity) leave every other row alone."""
