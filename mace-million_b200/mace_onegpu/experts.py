@@ -66,12 +66,18 @@ class ExpertPlan:
     with the same choice.  An expert of -1 means none.  Sorted on the device at the first product that needs it."""
 
     def __init__(self, experts, n_experts):
-        if experts.dim() not in (1, 2) or experts.dtype not in (torch.int32, torch.int64):
+        n = experts.dim()
+        if n not in (1, 2) or experts.dtype not in (torch.int32, torch.int64):
             raise ValueError("experts must be an integer tensor [tokens, k] or [tokens]")
-        if not 1 <= int(n_experts):
-            raise ValueError("n_experts must be positive")
-        self.experts = (experts if experts.dim() == 2 else experts[:, None]).to(torch.int32).contiguous()
         self.n_experts = int(n_experts)
+        if self.n_experts < 1:
+            raise ValueError("n_experts must be positive")
+        if n == 1:
+            experts = experts[:, None]
+        if experts.dtype != torch.int32:
+            # 64-bit indices outside the range of int32 must not wrap into it: -2 is refused by check(), like any other
+            experts = torch.where((experts >= -1) & (experts < self.n_experts), experts, -2).to(torch.int32)
+        self.experts = experts if experts.is_contiguous() else experts.contiguous()
         self._words = None
 
     @property
@@ -106,10 +112,10 @@ def expert_linear(x, w, plan, weights=None):
         raise TypeError("plan must be an ExpertPlan (plan_experts(experts, n_experts))")
     if w.dim() != 3 or w.shape[0] != plan.n_experts:
         raise ValueError(f"w must be [{plan.n_experts}, out, in] (got {tuple(w.shape)})")
-    grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or
-                                        (weights is not None and weights.requires_grad))
     slots = plan.experts.numel()
-    few = not grad and slots <= FEW_SLOTS and slots * w[0].numel() * w.element_size() <= FEW_BYTES
+    few = slots <= FEW_SLOTS and slots * w.shape[1] * w.shape[2] * w.element_size() <= FEW_BYTES
+    if few and torch.is_grad_enabled():
+        few = not (x.requires_grad or w.requires_grad or (weights is not None and weights.requires_grad))
     return _op("expert_linear")(x, w, plan.experts, None if few else plan.words, weights)
 
 

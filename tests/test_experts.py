@@ -42,6 +42,8 @@ def test_module_checks_arguments():
         X.plan_experts(torch.zeros(2, 2, dtype=torch.int64), 0)
     plan = X.plan_experts(torch.zeros(3, dtype=torch.int64), 4)
     assert plan.experts.shape == (3, 1) and plan.experts.dtype == torch.int32
+    wide = X.plan_experts(torch.tensor([[0, 2 ** 32 + 1], [-1, 3]]), 3)     # never wraps into the range
+    assert wide.experts.tolist() == [[0, -2], [-1, -2]]
     with pytest.raises(TypeError, match="ExpertPlan"):
         X.expert_linear(torch.zeros(3, 8), torch.zeros(4, 8, 8), plan.experts)
     with pytest.raises(ValueError, match="w must be"):
