@@ -10,10 +10,11 @@
 // small kernel adds the blocks' partial sums in a fixed order (no atomics: results do not depend on the schedule).
 // V is the elements per access: 16 bytes where the width, the row strides and the addresses allow it, else 1.
 // Widths that no group holds in registers take the *_wide kernels, which read the row once per sum.
-// Measured on a B200 (forward / backward): 65,536 x 2048 bf16 101 / 151 us (5.3 TB/s each, of 6.5 measured for a copy),
-// 65,536 x 1024 bf16 45 / 80 us, 32,768 x 1024 fp32 49 / 67 us, 16,384 x 128 fp32 in rows 512 apart 4.1 / 8.1 us,
-// 24,001 x 515 bf16 (one element per access) 21 / 26 us.  Below 5 TB/s the issue slots bound it: unpacking, the packed
-// arithmetic and packing are about 10 instructions an element backward.
+// Measured on a B200 (forward / backward): 65,536 x 2048 bf16 100 / 151 us (5.3 TB/s each, of 6.5 measured for a copy),
+// 65,536 x 1024 bf16 45 / 80 us, 32,768 x 1024 fp32 49 / 67 us, 16,384 x 128 fp32 in rows 512 apart 3.7 / 7.9 us,
+// 24,001 x 515 bf16 (one element per access) 20 / 26 us, 100,000 x 64 fp16 (8 threads a row) 6.0 / 10.8 us, with a whole
+// warp a row 18 / 26.  Below 5 TB/s the issue slots bound it: unpacking, the packed arithmetic and packing are about 10
+// instructions an element backward.
 #include "dtypes.cuh"
 
 namespace mb {
@@ -31,9 +32,15 @@ struct LnArgs {
 // (threads / 32) * K floats and is free to be overwritten two calls later: callers alternate two buffers).
 template <int G, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
-  static_assert(G >= 32, "a group is whole warps");
+  if constexpr (G < 32) {                         // several groups in a warp
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int W = G / 32;
+  constexpr int W = G < 32 ? 1 : G / 32;
   float s = 0.f;
   if constexpr (K == 8) {
     // transposed: after three halving steps lane L holds a partial sum of value L >> 2 (9 shuffles instead of 40)
@@ -64,7 +71,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
-  if constexpr (G == 32) {
+  if constexpr (G <= 32) {
     if constexpr (K == 8 || K == 4) {
 #pragma unroll
       for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, 32 / K * k);
@@ -101,12 +108,13 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
 
 template <int G>
 constexpr int ln_threads = G < 256 ? 256 : G;
-// blocks per SM that the registers of a thread are budgeted for (nothing spills beyond a few words)
-#ifndef MB_LN8
-#define MB_LN8 768
-#endif
+// threads per SM that the registers of a thread are budgeted for, and whether the next row is fetched ahead: worth the
+// registers at up to 16 values a thread (65,536 x 512 bf16 27.1 -> 23.3 us, 16,000 x 2049 fp16 82 -> 71) and from 64
+// with half the threads (20,000 x 4096 bf16 88 -> 70), not at 32 (65,536 x 1024 bf16 45.3 us without, 48.2 with)
 template <int G, int NV, int V>
-constexpr int ln_fwd_blocks = (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> > 0 ? (NV * V >= 64 ? MB_LN8 : 1024) / ln_threads<G> : 1;
+constexpr int ln_fwd_blocks = (NV * V >= 64 ? 512 : 1024) / ln_threads<G>;
+template <int NV, int V>
+constexpr bool ln_fwd_pre = NV * V != 32;
 template <int G, int NV, int V>
 constexpr int ln_bwd_blocks = G > 256 ? 1 : NV * V > 4 ? 2 : 3;
 
@@ -132,21 +140,39 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_fwd_blocks<G, NV, V>) k_ln_f
 #pragma unroll
     for (int i = 0; i < NV; ++i) params(i, pw[i], pb[i]);
   const float inv = 1.f / (float)d;
+  constexpr bool PRE = ln_fwd_pre<NV, V>;
+  Raw<T, V> nx[PRE ? NV : 1];                     // the next row, in flight while this one is worked on
+  auto fetch = [&](int64_t row, auto& to) {
+    const T* x = (const T*)a.x + row * a.ldx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * G + t) * V;
+      to[i].zero();
+      if (j < d) to[i].load(x + j);
+    }
+  };
+  if constexpr (PRE) {
+    const int64_t row = (int64_t)blockIdx.x * RPB + g;
+    if (row < a.n) fetch(row, nx);
+  }
   // the trip count is the same for every group of a block (group_sum synchronises the block)
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.n; r0 += (int64_t)gridDim.x * RPB) {
     const int64_t row = r0 + g;
     const bool live = row < a.n;
-    const T* x = (const T*)a.x + (live ? row : 0) * a.ldx;
     using E = Elem<V>;
     constexpr int NE = kElems<V>;
     Raw<T, V> v[NV];
     float s[1], f[V];
     E e[NE], acc[NE] = {};
+    if constexpr (PRE) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (i * G + t) * V;
-      v[i].zero();
-      if (live && j < d) v[i].load(x + j);
+      for (int i = 0; i < NV; ++i) v[i] = nx[i];
+      if (row + (int64_t)gridDim.x * RPB < a.n) fetch(row + (int64_t)gridDim.x * RPB, nx);
+    } else {
+      if (live) fetch(row, v);
+      else
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i].zero();
     }
     auto fold = [&] {
       E p = acc[0];
@@ -473,8 +499,10 @@ static int ln_fwd_launch(const LnArgs& a, cudaStream_t st) {
 template <typename T, typename P>
 static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
   constexpr int V = kVec<T>;
-  if (vec) {                                      // one warp per row up to 8 vectors per lane, then 4 and 16 warps
+  if (vec) {                                      // up to a warp per row and 8 vectors per lane, then 4 and 16 warps
     const int nv = (a.d / V + 31) / 32;
+    if (a.d / V <= 8) return ln_fwd_launch<T, P, 8, 1, V>(a, st);
+    if (a.d / V <= 16) return ln_fwd_launch<T, P, 16, 1, V>(a, st);
     if (nv <= 1) return ln_fwd_launch<T, P, 32, 1, V>(a, st);
     if (nv <= 2) return ln_fwd_launch<T, P, 32, 2, V>(a, st);
     if (nv <= 4) return ln_fwd_launch<T, P, 32, 4, V>(a, st);
@@ -512,6 +540,8 @@ static int ln_bwd_any(const LnArgs& a, bool vec, int* nb, cudaStream_t st) {
   constexpr int V = kVec<T>;
   if (vec) {
     const int c = a.d / V;
+    if (c <= 8) return ln_bwd_launch<T, P, 8, 1, V, 2, true>(a, nb, st);
+    if (c <= 16) return ln_bwd_launch<T, P, 16, 1, V, 2, true>(a, nb, st);
     if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 2, true>(a, nb, st);
     if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 2, true>(a, nb, st);
     if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 2, true>(a, nb, st);

@@ -94,6 +94,33 @@ def test_layer_norm_rows_and_strides(n, dt):
     _ln_close(db, db0, n, dt, 8)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [4, 24, 40, 72, 136, 520])
+def test_layer_norm_narrow_rows_of_many_tokens(d, dt):
+    """Several rows to a warp, and more rows than one pass of the grid."""
+    dt, n = DT[dt], 100003
+    g = _gen(d)
+    x = (torch.randn(n, d, generator=g) * 2 - 1).to(dt)
+    w = (1 + 0.3 * torch.randn(d, generator=g)).to(dt)
+    b = torch.randn(d, generator=g).to(dt)
+    dy = torch.randn(n, d, generator=g).to(dt)
+    xd, wd, bd = _cuda(x, True), _cuda(w, True), _cuda(b, True)
+    y = X.layer_norm(xd, wd, bd)
+    dx, dw, db = torch.autograd.grad(y, (xd, wd, bd), dy.cuda())
+    y0, dx0, dw0, db0 = R.layer_norm(x, w, b, 1e-5, dy)
+    # a few values can have a small deviation 1 / r: x - mean is then off by (log2 d) ulp of the largest |x|, times r
+    x, w, b, dy = x.double(), w.double(), b.double(), dy.double()
+    c = x - x.mean(1, keepdim=True)
+    r = 1 / (c.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    off = (8 + math.log2(d)) * E32 * (1 + r * x.abs().amax(1, keepdim=True))
+    xh, up = (c * r).abs().amax(1, keepdim=True), (dy * w).abs().amax(1, keepdim=True)
+    for got, want, scale in ((y, y0, xh * w.abs().max() + b.abs().max()), (dx, dx0, 8 * r * up * (1 + xh * xh))):
+        assert got.dtype == dt and got.shape == want.shape
+        assert not ((got.detach().cpu().double() - want).abs() > U[dt] * want.abs() + off * scale).any()
+    _ln_close(dw, dw0, n, dt, 8)
+    _ln_close(db, db0, n, dt, 8)
+
+
 def test_layer_norm_views_parameters_and_shapes():
     g = _gen(3)
     base = torch.randn(6, 5, 80, generator=g)
