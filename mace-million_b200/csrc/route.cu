@@ -1,19 +1,25 @@
 // Routing of tokens (atoms) to experts: scores s = softmax(l) or sigmoid(l) over E logits, a choice of k experts, weights.
 // The choice ranks by v = s + bias, or by the logits themselves without a bias (the same order, and no two logits that
 // differ can tie after rounding); logits of -inf are closed to the token.  With groups, a group's value is the sum of its
-// two best open v (of s up to the row's common factor without a bias), and only the best top_groups groups stay open.  Ties
-// go to the lowest index, NaN ranks first.  Slot j gets the j-th best expert, or -1 with weight 0 when none is open.
+// two best open v (without a bias: of their s, up to the row's common factor), and only the best top_groups groups stay
+// open.  Ties go to the lowest index, NaN ranks first.  Slot j gets the j-th best expert, or -1 with weight 0 when none is
+// open.
 //   renormalise: w_j = scale s_j / S, S = sum_j s_j (0 when S = 0);  else w_j = scale s_j.
 // Backward (the choice is constant): with q_j = s_j / S,
 //   renormalise: ds_j = scale (dw_j - sum_i dw_i q_i) / S, else ds_j = scale dw_j;
 //   softmax: dl_i = s_i (ds_i - sum_j s_j ds_j), sigmoid: dl_i = ds_i s_i (1 - s_i).
 //
-// Forward: L lanes of a warp per token, lane q holding the c experts q c .. q c + c - 1 in registers, so that a warp
-// works on 32 / L tokens.  A choice is a maximum of order-preserving integer keys over the lane's registers and L lanes,
-// and the lowest lane that has it wins (the lowest index among equals); comparisons are exact.  Bound by issued
-// instructions (k maxima over E keys, E exponentials where all scores count), not by the logits' bytes: 131,072 x 128 bf16
-// sigmoid, 8 groups, k = 8 takes 85 us (480 instructions a token, two thirds of the issue slots) against 5.8 us for the bytes;
-// a whole warp per token took 162 us (its reductions cross 32 lanes for 4 keys a lane).  Few tokens take L = 32, which has the shortest chain.
+// Forward: L lanes of a warp per token, lane q holding the c experts q c .. q c + c - 1 in registers as order-preserving
+// integer keys, so that a warp works on 32 / L tokens.  For k > 2 each four keys of a lane are sorted, and a choice is a
+// maximum over the lists' heads in the lane and over the L lanes; the winner's list moves up.  Which expert it was is found
+// once all k are known, one slot per lane, by comparing with the winner's keys in shared memory (the d-th equal key for
+// the d-th equal slot, so the lowest index among equals).  Where the open groups are at most half of the experts, their
+// keys are first dealt out to all lanes.  k <= 2 takes its maxima from the unsorted keys: 131,072 x 256 in k = 1 40 us,
+// through sorted lists 51; at k = 4 of 128 the lists are ahead (35 us of 37), at k = 8 46 us of 57.
+// Bound by issued instructions, comparisons and selections at half rate above all, not by the logits' bytes: 131,072 x 128
+// bf16 sigmoid, 8 groups, k = 8 takes 59 us against 5.8 us for the bytes (85 us by maxima over unsorted keys; 85 us by a
+// lane per token over keys in shared memory, whose long chains leave half of the issue slots empty; 162 us by a whole warp
+// per token).  Few tokens take L = 32, which has the shortest chain.
 // Backward: only the chosen logits enter, except for plain softmax weights; a warp fills a tile of zeros in shared memory
 // with the k values of its tokens and copies it out in whole vectors (131,072 x 128 bf16: 11.5 us, 6.5 TB/s).
 #include "dtypes.cuh"
@@ -21,9 +27,12 @@
 namespace mb {
 
 constexpr int RT_WARPS = 8;
+// blocks per SM that registers are budgeted for: at 131,072 x 128 (k 8) 2 took 72 us, 3 60 us, 4 58.7 us
+template <int NE>
+constexpr int rt_blocks = NE <= 16 ? 4 : 3;
 
 struct RouteArgs {
-  int32_t c, span, vec, all;                      // forward: experts per lane, lanes per group, vector loads, all scores needed
+  int32_t c, span, vec;                           // forward: experts per lane, lanes per group, vector loads
   const void* logits;
   const float *bias, *dw;
   float* w;
@@ -35,12 +44,15 @@ struct RouteArgs {
   float scale;
 };
 
-// float -> uint32 with the same order: -0 equals +0, NaN is above +inf; -inf (closed) is KEY_CLOSED, and so is 0
-constexpr unsigned KEY_CLOSED = 0x007FFFFFu;
+// float -> uint32 with the same order: -0 equals +0; the sum's NaN is 0x7FFFFFFF and comes out above +inf, as 0xFFFFFFFF;
+// -inf (closed) is KEY_CLOSED, and so is 0
+constexpr unsigned KEY_CLOSED = 0x007FFFFFu, KEY_NAN = 0xFFFFFFFFu;
 __device__ __forceinline__ unsigned order_key(float f) {
-  if (f != f) return 0xFFFFFFFFu;
-  const unsigned u = __float_as_uint(f + 0.f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const int u = __float_as_int(f + 0.f);
+  return (unsigned)u ^ ((unsigned)(u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_float(unsigned key) {
+  return __uint_as_float(key ^ ((unsigned)~((int)key >> 31) | 0x80000000u));
 }
 
 // The score's parts in plain fp32 arithmetic (exp, and a correctly rounded reciprocal): the same bits as those operations
@@ -71,15 +83,41 @@ __device__ __forceinline__ int lanes_first(bool p, int base) {
   return b ? __ffs(b) - 1 : 32;
 }
 
-template <typename T, int L, int NE>
-__global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs a) {
+// words of shared memory between the keys of two lanes: their 16-byte accesses do not conflict
+template <int NE>
+constexpr int rt_pitch = NE == 12 ? 20 : NE + 4;
+// words per warp: keys, then per token the k best keys, who has them, and the open groups
+template <int L, int NE, int NC>
+__host__ __device__ constexpr int rt_words(int k) {
+  return (NC > 0 ? 32 * rt_pitch<NE> : 0) + (32 / L * (2 * k + L) + 3) / 4 * 4;
+}
+
+// NC < NE: the open groups fit in NC keys a lane, and are dealt out to all lanes before the choice; NC = 0: one or two
+// experts are chosen, straight from the keys
+template <typename T, int L, int NE, int NC>
+__global__ void __launch_bounds__(32 * RT_WARPS, rt_blocks<NE>) k_route_fwd(const RouteArgs a) {
   constexpr int TPW = 32 / L;                     // tokens per warp
-  extern __shared__ unsigned char sm_raw[];
+  constexpr int NL = NC > 0 ? NC / 4 : 1, P = rt_pitch<NE>;       // lists of four keys in a lane
+  extern __shared__ __align__(16) unsigned sm_rt[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (L - 1), base = lane & ~(L - 1);
-  int* chosen = reinterpret_cast<int*>(sm_raw) + (warp * TPW + lane / L) * a.k;            // [k] of this token
+  unsigned* keys = sm_rt + warp * rt_words<L, NE, NC>(a.k);                                    // [32][P]
+  unsigned* best_of = keys + (NC > 0 ? 32 * P : 0) + lane / L * (2 * a.k + L);   // [k] of this token
+  int* chosen = reinterpret_cast<int*>(best_of) + a.k;                                     // [k]
+  int* opened = chosen + a.k;                                                              // [L]
   // a group's `per` experts lie in a.span lanes (a power of two), a.c in each but the last ones
-  const int c = a.c, span = a.span, per = a.e / a.groups, mine = sub / span, q0 = (sub - mine * span) * c;
-  const int i0 = mine * per + q0, n = mine >= a.groups || q0 >= per ? 0 : per - q0 < c ? per - q0 : c;
+  const int c = a.c, span = a.span, shift = __ffs(span) - 1, per = a.e / a.groups, mine = sub >> shift;
+  const int q0 = (sub - (mine << shift)) * c, i0 = mine * per + q0;
+  const int n = mine >= a.groups || q0 >= per ? 0 : per - q0 < c ? per - q0 : c;
+  // the four keys from `off` on in the open group number `nth` become the lane's list u; `at`: their place from the group's
+  int nth[NL], off[NL], at[NL];
+  if constexpr (NC > 0 && NC < NE)
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+      nth[u] = (sub * NC + 4 * u) / per;
+      off[u] = (sub * NC + 4 * u) % per;
+      at[u] = off[u] / c * P + off[u] % c;
+    }
+  const bool sums = a.softmax && !a.renorm, known = a.softmax && (sums || a.bias || a.groups > 1);
   const int64_t step = (int64_t)gridDim.x * RT_WARPS * TPW;
   // every lane of a warp runs the same number of passes (the collectives are warp-wide)
   for (int64_t r0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * TPW; r0 < a.t; r0 += step) {
@@ -104,20 +142,19 @@ __global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs 
       for (int j = 0; j < NE; ++j)
         if (live && j < n) l[j] = to_f(p[i0 + j]);
     }
-    unsigned key[NE];
     float m = 0.f, sum = 1.f;
-    if (!a.all) {
+    if (known) {
+      m = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NE; ++j) key[j] = order_key(l[j]);
-    } else {
+      for (int j = 0; j < NE; ++j) m = fmaxf(m, l[j]);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (m == -INFINITY) m = 0.f;
+    }
+    unsigned key[NE];
+    if (a.bias) {
       float s[NE];
       if (a.softmax) {
-        m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) m = fmaxf(m, l[j]);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (m == -INFINITY) m = 0.f;
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < NE; ++j) {
@@ -125,73 +162,169 @@ __global__ void __launch_bounds__(32 * RT_WARPS, 3) k_route_fwd(const RouteArgs 
           sum += s[j];
         }
         sum = lanes_sum<L>(sum);
-        if (a.bias)
 #pragma unroll
-          for (int j = 0; j < NE; ++j) s[j] = s[j] / sum;
+        for (int j = 0; j < NE; ++j) s[j] = s[j] / sum;
       } else {
 #pragma unroll
         for (int j = 0; j < NE; ++j) s[j] = sigmoid_f(l[j]);
       }
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
-        if (a.bias && j < n) s[j] += a.bias[i0 + j];
-        if (l[j] == -INFINITY) s[j] = -INFINITY;  // closed
-        key[j] = order_key(a.bias ? s[j] : l[j]);
+        const float v = s[j] + (j < n ? a.bias[i0 + j] : 0.f);
+        key[j] = order_key(l[j] == -INFINITY ? -INFINITY : v);
       }
-      if (a.groups > 1) {
-        unsigned open = 0u;                       // bit g: group g stays open (up to 32 groups)
-        float m1 = -INFINITY, m2 = -INFINITY;     // the group's two best
-        bool nan = false;
+    } else {
+      if (sums) {
+        sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          nan |= s[j] != s[j];
-          m2 = fmaxf(m2, fminf(m1, s[j]));
-          m1 = fmaxf(m1, s[j]);
-        }
-        for (int o = 1; o < span; o <<= 1) {
-          const float o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
-          m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
-          m1 = fmaxf(m1, o1);
-          nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
-        }
-        unsigned gk = nan ? 0xFFFFFFFFu : order_key(m2 > -INFINITY ? m1 + m2 : m1);
-        for (int q = 0; q < a.top_groups; ++q) {
-          const unsigned best = lanes_max<L>(gk);
-          const int g = lanes_first<L>(gk == best, base) / span;
-          if (best <= KEY_CLOSED) continue;       // nothing open is left for this token
-          open |= 1u << g;
-          if (g == mine) gk = 0u;
-        }
-        if (!((open >> (mine & 31)) & 1u))
-#pragma unroll
-          for (int j = 0; j < NE; ++j) key[j] = 0u;
+        for (int j = 0; j < NE; ++j) sum += expf(l[j] - m);
+        sum = lanes_sum<L>(sum);
       }
+#pragma unroll
+      for (int j = 0; j < NE; ++j) key[j] = order_key(l[j]);
     }
-    for (int q = 0; q < a.k; ++q) {
-      unsigned t[NE];                             // the lane's best, as a tree
+    if constexpr (NC > 0)
 #pragma unroll
-      for (int j = 0; j < NE; ++j) t[j] = key[j];
+      for (int j = 0; j < NE; j += 4)
+        *reinterpret_cast<uint4*>(keys + lane * P + j) = make_uint4(key[j], key[j + 1], key[j + 2], key[j + 3]);
+    unsigned open = 0u;                           // bit g: group g stays open (up to 32 groups)
+    if (a.groups > 1) {
+      unsigned k1 = 0u, k2 = 0u;                  // the group's two best
 #pragma unroll
-      for (int w = NE; w > 1; w = (w + 1) / 2)
+      for (int j = 0; j < NE; ++j) {
+        k2 = max(k2, min(k1, key[j]));
+        k1 = max(k1, key[j]);
+      }
+      for (int o = 1; o < span; o <<= 1) {
+        const unsigned o1 = __shfl_xor_sync(0xffffffffu, k1, o), o2 = __shfl_xor_sync(0xffffffffu, k2, o);
+        k2 = max(min(k1, o1), max(k2, o2));
+        k1 = max(k1, o1);
+      }
+      const float f1 = key_float(k1), f2 = key_float(k2);
+      const float v1 = a.bias ? f1 : a.softmax ? expf(f1 - m) : sigmoid_f(f1);
+      const float v2 = a.bias ? f2 : a.softmax ? expf(f2 - m) : sigmoid_f(f2);
+      unsigned gk = k1 == KEY_NAN || k1 <= KEY_CLOSED ? k1 : order_key(k2 > KEY_CLOSED ? v1 + v2 : v1);
+      for (int q = 0; q < a.top_groups; ++q) {
+        const unsigned best = lanes_max<L>(gk);
+        const int g = lanes_first<L>(gk == best, base) >> shift;
+        if (best <= KEY_CLOSED) continue;         // nothing open is left for this token
+        open |= 1u << g;
+        if (g == mine) gk = 0u;
+      }
+      if (!((open >> (mine & 31)) & 1u))
 #pragma unroll
-        for (int j = 0; j < w / 2; ++j) t[j] = max(t[j], t[j + (w + 1) / 2]);
-      const unsigned best = lanes_max<L>(t[0]);
-      const int first = lanes_first<L>(t[0] == best, base);
-      if (sub == first) {
-        bool left = true;
-        int at = 0;
+        for (int j = 0; j < NE; ++j) key[j] = 0u;
+      else if (NC > 0 && NC < NE && sub == mine << shift)
+        opened[__popc(open & ((1u << mine) - 1u))] = mine;
+    }
+    if constexpr (NC == 0) {
+      for (int q = 0; q < a.k; ++q) {
+        unsigned t[NE];                           // the lane's best, as a tree
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {            // the first of the lane's keys that has it
-          const bool hit = left && key[j] == best;
-          left = left && key[j] != best;
-          if (hit) key[j] = 0u, at = j;
+        for (int j = 0; j < NE; ++j) t[j] = key[j];
+#pragma unroll
+        for (int w = NE; w > 1; w = (w + 1) / 2)
+#pragma unroll
+          for (int j = 0; j < w / 2; ++j) t[j] = max(t[j], t[j + (w + 1) / 2]);
+        const unsigned best = lanes_max<L>(t[0]);
+        if (sub == lanes_first<L>(t[0] == best, base)) {
+          bool left = true;
+          int at = 0;
+#pragma unroll
+          for (int j = 0; j < NE; ++j) {          // the first of the lane's keys that has it
+            const bool hit = left && key[j] == best;
+            left = left && key[j] != best;
+            if (hit) key[j] = 0u, at = j;
+          }
+          chosen[q] = best > KEY_CLOSED ? i0 + at : -1;
         }
-        chosen[q] = best > KEY_CLOSED ? i0 + at : -1;
+      }
+    } else {
+      __syncwarp();
+      unsigned h[4 * NL];
+      unsigned from[NL];                            // a list's place in shared memory, and its first expert
+      if constexpr (NC < NE) {
+        const int count = __popc(open);
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          from[u] = 0;
+          if (nth[u] < count) {
+            const int g = opened[nth[u]], place = (base + (g << shift)) * P + at[u];
+            v = *reinterpret_cast<const uint4*>(keys + place);
+            from[u] = place | (unsigned)(g * per + off[u]) << 16;
+          }
+          h[4 * u] = v.x, h[4 * u + 1] = v.y, h[4 * u + 2] = v.z, h[4 * u + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < NL; ++u) from[u] = (lane * P + 4 * u) | (unsigned)(i0 + 4 * u) << 16;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) h[j] = key[j];
+      }
+#pragma unroll
+      for (int u = 0; u < NL; ++u) {                // each four in descending order
+        auto order = [&](int i, int j) {
+          const unsigned hi = max(h[4 * u + i], h[4 * u + j]), lo = min(h[4 * u + i], h[4 * u + j]);
+          h[4 * u + i] = hi;
+          h[4 * u + j] = lo;
+        };
+        order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
+      }
+      unsigned before = 0u;                         // the lane's last best key, and how often it had the same one
+      int same = 0;
+      for (int q = 0; q < a.k; ++q) {
+        unsigned t[NL];                             // the best of the lists' heads, as a tree
+#pragma unroll
+        for (int u = 0; u < NL; ++u) t[u] = h[4 * u];
+#pragma unroll
+        for (int w = NL; w > 1; w = (w + 1) / 2)
+#pragma unroll
+          for (int u = 0; u < w / 2; ++u) t[u] = max(t[u], t[u + (w + 1) / 2]);
+        const unsigned best = lanes_max<L>(t[0]);
+        const bool win = sub == lanes_first<L>(t[0] == best, base);
+        bool left = win;
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {              // one of the lane's lists that have it gives its head away
+          const bool hit = left && h[4 * u] == best;
+          left = left && h[4 * u] != best;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) h[4 * u + x] = hit ? (x < 3 ? h[4 * u + x + 1] : 0u) : h[4 * u + x];
+        }
+        if (win) {
+          same = best == before ? same + 1 : 0;
+          before = best;
+          best_of[q] = best;
+          chosen[q] = lane | same << 8;
+        }
+      }
+      __syncwarp();
+      // whose key it was: the winner's keys compared once more, one slot per lane
+      for (int r = 0; r < a.k; r += L) {
+        const int q = r + sub;
+        const unsigned best = q < a.k ? best_of[q] : 0u;
+        const int who = q < a.k ? chosen[q] : lane;
+        int i = -1;
+        unsigned hits = 0u;
+        unsigned where[NL];
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {
+          where[u] = __shfl_sync(0xffffffffu, from[u], who & 31);
+          const uint4 v = *reinterpret_cast<const uint4*>(keys + (where[u] & 0xFFFF));
+          hits |= (v.x == best ? 1u : 0u) << 4 * u | (v.y == best ? 2u : 0u) << 4 * u | (v.z == best ? 4u : 0u) << 4 * u |
+                  (v.w == best ? 8u : 0u) << 4 * u;
+        }
+        for (int x = who >> 8; x > 0; --x) hits &= hits - 1u;      // equal keys: the first ones went to earlier slots
+        const int bit = __ffs(hits) - 1;
+#pragma unroll
+        for (int u = 0; u < NL; ++u)
+          if (bit >> 2 == u) i = (int)(where[u] >> 16) + (bit & 3);
+        if (q < a.k) chosen[q] = best > KEY_CLOSED ? i : -1;
       }
     }
     __syncwarp();
     // weights: the chosen logits once more, L slots at a time
-    if (!a.all && a.softmax) {                    // only the chosen ones count: relative to the best of them
+    if (a.softmax && !known) {                    // only the chosen ones count: relative to the best of them
       const int i = chosen[0];
       m = live && i >= 0 ? to_f(p[i]) : 0.f;
     }
@@ -375,13 +508,24 @@ static int route_bwd_any(const RouteArgs& a, cudaStream_t st) {
   return route_bwd_dense<T, 16>(a, st);
 }
 
+template <typename T, int L, int NE, int NC>
+static int route_fwd_go(const RouteArgs& a, cudaStream_t st) {
+  const int smem = RT_WARPS * rt_words<L, NE, NC>(a.k) * 4;
+  static_assert(RT_WARPS * rt_words<L, NE, NC>(MB_ROUTE_MAX_K) * 4 <= 48 * 1024, "shared memory of a block");
+  k_route_fwd<T, L, NE, NC><<<route_grid(a.t, RT_WARPS * (32 / L), 8), 32 * RT_WARPS, smem, st>>>(a);
+  return check_launch("route_fwd");
+}
+
 template <typename T, int L, int NE>
 static int route_fwd_launch(RouteArgs a, cudaStream_t st) {
-  constexpr int TPW = 32 / L, V = kVec<T>;
+  constexpr int V = kVec<T>;
   const int per = a.e / a.groups;
   a.vec = NE % V == 0 && a.c % V == 0 && per % V == 0 && a.ldl % V == 0 && aligned16(a.logits);
-  k_route_fwd<T, L, NE><<<route_grid(a.t, RT_WARPS * TPW, 8), 32 * RT_WARPS, RT_WARPS * TPW * a.k * 4, st>>>(a);
-  return check_launch("route_fwd");
+  if (a.k <= 2) return route_fwd_go<T, L, NE, 0>(a, st);
+  if constexpr (NE % 8 == 0 && NE <= 16)
+    if (a.groups > 1 && per % 4 == 0 && a.c % 4 == 0 && a.top_groups * per <= L * NE / 2)
+      return route_fwd_go<T, L, NE, NE / 2>(a, st);
+  return route_fwd_go<T, L, NE, NE>(a, st);
 }
 
 template <typename T, int L>
@@ -398,7 +542,6 @@ static int route_fwd_lanes(const RouteArgs& a, cudaStream_t st) {
 template <typename T>
 static int route_fwd_any(RouteArgs a, cudaStream_t st) {
   constexpr int V = kVec<T>;
-  a.all = a.bias || a.groups > 1 || (a.softmax && !a.renorm);
   const int per = a.e / a.groups;
   int most = 1;                                   // most lanes a group can have
   while (2 * most * a.groups <= 32) most *= 2;

@@ -264,6 +264,40 @@ def test_route_many_tokens_agree_with_few(E, groups, top):
         assert torch.equal(e[r], e2) and (w[r] - w2).abs().max() <= 3e-7     # sums over slots in another order
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("E,k,groups,top", [(128, 8, 8, 4), (128, 5, 8, 2), (256, 8, 8, 4), (64, 6, 4, 2), (96, 7, 8, 3),
+                                            (32, 4, 4, 2), (160, 3, 5, 2), (128, 32, 1, 1), (100, 9, 1, 1), (48, 2, 4, 2),
+                                            (128, 1, 8, 4), (12, 5, 1, 1), (512, 8, 16, 8)])
+def test_route_many_tokens_with_ties_and_closed_experts(E, k, groups, top, biased, dt):
+    """Logits of few values: whole lanes of equal keys, groups of equal value, closed experts and NaN among them; the same
+    200 rows over and over, more than a pass of the grid."""
+    g = _gen(E * k + groups)
+    l = torch.randint(-2, 3, (200, E), generator=g).double() / 2
+    l[50:120] = l[50:120].masked_fill(torch.rand(70, E, generator=g) < 0.5, float("-inf"))
+    l[120:150] = l[120:150].masked_fill(torch.rand(30, E, generator=g) < 0.97, float("-inf"))
+    l[150:160] = 0.5
+    l[160] = float("-inf")
+    l[161, E // 2:] = float("-inf")
+    l[162, E // 3] = float("inf")
+    l = l.to(DT[dt])
+    # biases that are multiples of an eighth: a biased sigmoid ties where logit and bias are equal, and is apart elsewhere
+    b = torch.randint(-1, 2, (E,), generator=g).float() / 8 if biased else None
+    kw = dict(score="sigmoid", groups=groups, top_groups=top)
+    w, e = X.route(l.cuda().repeat(50, 1), k, bias=_cuda(b), **kw)
+    w, e = w.cpu().view(50, 200, k), e.cpu().long().view(50, 200, k)
+    assert torch.equal(e, e[:1].expand_as(e)) and torch.equal(w, w[:1].expand_as(w))
+    w0, e0, gap = R.route(l, k, b, **kw)
+    clear = (gap > 1e-6) | (gap == 0)             # equal values are equal in any arithmetic: they come from equal inputs
+    assert clear.double().mean() > 0.9
+    assert torch.equal(e[0][clear], e0[clear])
+    assert (w[0].double() - w0)[clear].abs().max() <= 2e-6
+    l[170:180, ::7] = float("nan")                # NaN ranks first, in order
+    _, e = X.route(l[170:180].cuda().repeat(600, 1), k, score="sigmoid")
+    first = torch.arange(0, E, 7)[:k]
+    assert (e.cpu().long()[:, :len(first)] == first).all()
+
+
 @pytest.mark.parametrize("T", [0, 1, 7, 5000])
 def test_route_sizes_and_strides(T):
     g = _gen(T)
