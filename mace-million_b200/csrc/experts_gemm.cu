@@ -9,7 +9,7 @@
 // the result.
 // The tensor cores truncate when they add to an fp32 accumulator: the result shrinks by about 1.7e-8 of itself for each
 // 16-wide step (measured: 3.2e-6 after 192 steps, 4.7e-7 after 32).  Where the result leaves in fp32 (fp32 data, and the
-// gradient of the weights) an accumulator therefore takes XG_ACC_K K blocks at most, and the chunks are added in registers
+// gradient of the weights) an accumulator therefore takes a few K blocks at most, and the chunks are added in registers
 // with rounding to nearest; 16-bit results are rounded a thousand times more coarsely and take the whole K.
 //
 // Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
@@ -47,7 +47,10 @@ static_assert(32 * (XG_EPI0 * XG_REGS_LOW + XG_EPI_WARPS * XG_REGS_HIGH) <= XG_T
 __device__ unsigned long long g_xg_wait_ns = 2000000000ull;
 __device__ int g_xg_skip_load = 0;
 constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
-constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12;     // K blocks of an accumulator whose result leaves in fp32 (fp32 / 16-bit data)
+// Most K blocks of an accumulator whose result leaves in fp32: of fp32 data, of 16-bit data, and where each CTA has one tile
+// at most (its drains cost nothing then).  Gradients of the weights from 16-bit data, 2,048 columns: error 7e-7 at 12,
+// 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: backward 2251 us at 12, 2331 at 8.
+constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12, XG_ACC_K1 = 4;
 
 // T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for
 template <typename T, int BN, int CG>
@@ -87,7 +90,7 @@ struct XgBars {
 };
 
 struct XgTile {
-  int e, m0, n0, r0, nk;                         // expert; first row, column; first K row (WGRAD); K blocks
+  int e, m0, n0, r0, nk, ck;                     // expert; first row, column; first K row (WGRAD); K blocks, of a chunk
   int part;                                      // WGRAD: >= 0: the item's place in the partial sums
   bool rows_ok;                                  // FWD / DGRAD: this CTA's rows belong to the expert
 };
@@ -286,6 +289,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   const uint32_t tmem = B.tmem;
   const int tiles = MODE == XG_WGRAD ? pre[g.E] * g.tm * g.tn : plan[CG == 2 ? 2 : 0] * g.tn;
   const int rounds = (tiles + ctas - 1) / ctas;
+  constexpr bool CHUNKS = sizeof(T) == 4 || DOT;
   auto tile_at = [&](int n) { return n * ctas + (MODE == XG_WGRAD && (n & 1) ? ctas - 1 - cta : cta); };
   auto tile_of = [&](int t) {
     XgTile o;
@@ -318,12 +322,15 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       if (CG == 2 && rank == 1) o.rows_ok = o.m0 < plan[g.lay.o_seg + o.e + 1];
       o.nk = (g.K + XG_BK - 1) / XG_BK;
     }
+    o.ck = o.nk;                                 // K blocks of one accumulator: even chunks
+    if constexpr (CHUNKS) {
+      const int most = rounds == 1 ? XG_ACC_K1 : sizeof(T) == 4 ? XG_ACC_K : XG_ACC_K16, n = (o.nk + most - 1) / most;
+      if (n > 1) o.ck = (o.nk + n - 1) / n;
+    }
     return o;
   };
   const int bh = g.bn / CG;                      // columns of B that this CTA loads
   constexpr bool SPLIT = DOT && BN == 256;       // registers move from the first four warps to the epilogue's
-  // K blocks of one accumulator
-  constexpr int acc_k = sizeof(T) == 4 ? XG_ACC_K : DOT ? XG_ACC_K16 : 0x3fffffff;
 
   if (warp < XG_EPI0) {
   if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XG_REGS_LOW));
@@ -391,9 +398,9 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       for (int r = 0; ok && r < rounds; ++r) {
         const int t = tile_at(r);
         if (t >= tiles) break;
-        const int nk = tile_of(t).nk;
-        for (int kb0 = 0; ok && kb0 < nk; kb0 += acc_k, ++tc) {
-          const int acc = tc & 1, kb1 = nk - kb0 > acc_k ? kb0 + acc_k : nk;
+        const XgTile w = tile_of(t);
+        for (int kb0 = 0; ok && kb0 < w.nk; kb0 += w.ck, ++tc) {
+          const int acc = tc & 1, kb1 = w.nk - kb0 > w.ck ? kb0 + w.ck : w.nk;
           if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, wait_ns)) {
             *failed = 1;
             ok = false;
@@ -527,7 +534,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         else
           xg_emit32<T>(v, at, stg, orow, out + 32 * q, ldo, vec, sc, nc - 32 * q);
       };
-      if constexpr (acc_k == 0x3fffffff) {         // one accumulator: 32 columns at a time straight from TMEM
+      if constexpr (!CHUNKS) {                     // one accumulator: 32 columns at a time straight from TMEM
         const int acc = tc & 1;
         if (w.nk > 0 && !wait(acc)) {
           ok = false;
@@ -555,7 +562,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         for (int q = 0; q < NG; ++q)
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[q][i] = 0.f;
-        for (int kb0 = 0; kb0 < w.nk; kb0 += acc_k, ++tc) {
+        for (int kb0 = 0; kb0 < w.nk; kb0 += w.ck, ++tc) {
           const int acc = tc & 1;
           if (!wait(acc)) {
             ok = false;
