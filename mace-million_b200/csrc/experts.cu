@@ -482,11 +482,33 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
   }
 }
 
+// V fp32 values as loaded
+template <int V>
+struct RawF {
+  uint4 u[V / 4];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) u[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void add_to(float (&s)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      s[4 * i] += __uint_as_float(u[i].x), s[4 * i + 1] += __uint_as_float(u[i].y);
+      s[4 * i + 2] += __uint_as_float(u[i].z), s[4 * i + 3] += __uint_as_float(u[i].w);
+    }
+  }
+};
+
 // Blocks [0, sum_blocks): out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an
-// expert; a thread adds one vector of a token's rows, four loads in flight; ldb is padded to whole vectors.
+// expert; a thread adds one vector of a token's rows, four loads in flight; ldb is padded to whole vectors.  The rows are
+// fp32 whatever the type of out: one rounding of the sum, and a row need not fit fp16 where the sum does.
 // The other blocks: dg[slot] = sum of its nparts partial products (0 without an expert).
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
+__global__ void __launch_bounds__(256) k_rows_sum(const float* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,
                                                   const int32_t* slot_row, unsigned sum_blocks, const float* dgpart,
                                                   int nparts, float* dg) {
   if (blockIdx.x >= sum_blocks) {
@@ -505,7 +527,7 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
     for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)sum_blocks * 8) {
       T* o = out + t * d;
       const int sh = (int)(reinterpret_cast<uintptr_t>(o) & 15);
-      const T* p = buf + t * k * ldb;
+      const float* p = buf + t * k * ldb;
       const int32_t* row = slot_row + t * k;
       uint32_t c[4] = {0u, 0u, 0u, 0u};            // the last lane's vector of the pass before
       for (int n0 = 0; n0 * VV - sh / (int)sizeof(T) < d; n0 += 32) {
@@ -515,19 +537,14 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
         for (int q = 0; q < VV; ++q) s[q] = 0.f;
         if (n * VV < d)
           for (int j0 = 0; j0 < k; j0 += 4) {
-            Raw<T, VV> r[4];
+            RawF<VV> r[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               r[j].zero();
               if (j0 + j < k && row[j0 + j] >= 0) r[j].load(p + (j0 + j) * ldb + n * VV);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float f[VV];
-              r[j].get(f);
-#pragma unroll
-              for (int q = 0; q < VV; ++q) s[q] += f[q];
-            }
+            for (int j = 0; j < 4; ++j) r[j].add_to(s);
           }
         const uint4 u = pack16<T>(s);
         // bytes [16 - sh, 32 - sh) of the neighbour's vector and this one go to the aligned address 16 n - sh
@@ -557,34 +574,29 @@ __global__ void __launch_bounds__(256) k_rows_sum(const T* buf, int64_t ldb, T* 
         }
       }
     }
-    return;
-  }
-  const unsigned nv = d / V;
-  const int64_t total = tokens * nv, step = (int64_t)sum_blocks * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t t = total >> 32 ? i / nv : (unsigned)i / nv;
-    const int c = (int)(i - t * nv) * V;
-    float s[V];
+  } else {
+    const unsigned nv = d / V;
+    const int64_t total = tokens * nv, step = (int64_t)sum_blocks * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+      const int64_t t = total >> 32 ? i / nv : (unsigned)i / nv;
+      const int c = (int)(i - t * nv) * V;
+      float s[V];
 #pragma unroll
-    for (int q = 0; q < V; ++q) s[q] = 0.f;
-    const T* p = buf + t * k * ldb + c;
-    const int32_t* row = slot_row + t * k;
-    for (int j0 = 0; j0 < k; j0 += 4) {
-      Raw<T, V> r[4];
+      for (int q = 0; q < V; ++q) s[q] = 0.f;
+      const float* p = buf + t * k * ldb + c;
+      const int32_t* row = slot_row + t * k;
+      for (int j0 = 0; j0 < k; j0 += 4) {
+        RawF<V> r[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        r[j].zero();
-        if (j0 + j < k && row[j0 + j] >= 0) r[j].load(p + (j0 + j) * ldb);
+        for (int j = 0; j < 4; ++j) {
+          r[j].zero();
+          if (j0 + j < k && row[j0 + j] >= 0) r[j].load(p + (j0 + j) * ldb);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j].add_to(s);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f[V];
-        r[j].get(f);
-#pragma unroll
-        for (int q = 0; q < V; ++q) s[q] += f[q];
-      }
+      store_v<T, V>(out + t * d + c, s);
     }
-    store_v<T, V>(out + t * d + c, s);
   }
 }
 
@@ -691,7 +703,7 @@ static XFwd x_fwd_layout(const XShape& s, bool combine, bool direct) {
   XFwd f;
   f.xs = c.take((int64_t)s.np * s.rows * s.Dp * 2);
   if (!direct) f.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
-  if (combine && s.k > 1) f.y = c.take(s.R * s.Op * dtype_size(s.dtype));
+  if (combine && s.k > 1) f.y = c.take(s.R * s.Op * 4);
   f.bytes = c.used;
   return f;
 }
@@ -708,7 +720,7 @@ static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direc
   if (need_w) b.xs = c.take(row2 * s.Dp);
   b.dys = c.take(row2 * s.Op);
   if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
-  if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * dtype_size(s.dtype));
+  if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * 4);
   if (need_g) b.dgp = c.take(s.R * 4 * 2 * xgemm_n_tiles(s.D, s.dtype));
   if (need_w) {
     b.kc = xgemm_kc(s.E, s.O, s.D, s.R, s.dtype);
@@ -794,7 +806,7 @@ static int x_moves(const XShape& s, XMoves& mv, const int32_t* plan, cudaStream_
 
 // sums of rows (buf not null) and of partial weight gradients (dg not null) in one launch
 template <typename T>
-static int x_rows_sum(const T* buf, int64_t ldb, T* out, int64_t tokens, int k, int d, const int32_t* slot_row,
+static int x_rows_sum(const float* buf, int64_t ldb, T* out, int64_t tokens, int k, int d, const int32_t* slot_row,
                       const float* dgpart, int nparts, float* dg, cudaStream_t st) {
   constexpr int V = kVec<T>;
   const bool vec = d % V == 0 && aligned16(out);
@@ -923,9 +935,10 @@ extern "C" int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x
     g.plan = plan; g.lay = s.lay; g.scale = weights;
     g.out = sum ? (void*)(base + f.y) : out;
     g.ldo = sum ? s.Op : O;
+    g.out32 = sum;
     if (int rc = xgemm_launch(g, st)) return rc;
     if (!sum) return 0;
-    return x_rows_sum<T>((const T*)(base + f.y), s.Op, (T*)out, tokens, k, O, plan + s.lay.o_slot, nullptr, 0, nullptr, st);
+    return x_rows_sum<T>((const float*)(base + f.y), s.Op, (T*)out, tokens, k, O, plan + s.lay.o_slot, nullptr, 0, nullptr, st);
   });
 }
 
@@ -988,13 +1001,14 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
     g.plan = plan; g.lay = s.lay; g.scale = weights;
     g.out = sum ? (void*)(base + b.dxb) : dx;
     g.ldo = sum ? s.Dp : D;
+    g.out32 = sum;
     if (dweights) {
       g.x = x; g.ldx = ldx; g.kdiv = kx;
       g.dgpart = (float*)(base + b.dgp);
     }
     if (int rc = xgemm_launch(g, st)) return rc;
     if (!sum && !dweights) return 0;
-    return x_rows_sum<T>(sum ? (const T*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, plan + s.lay.o_slot,
+    return x_rows_sum<T>(sum ? (const float*)(base + b.dxb) : nullptr, s.Dp, (T*)dx, tokens, k, D, plan + s.lay.o_slot,
                          dweights ? (const float*)(base + b.dgp) : nullptr, 2 * xgemm_n_tiles(D, dtype), dweights, st);
   });
 }

@@ -51,6 +51,7 @@ struct XGemm {
   const float* scale;                            // per slot, or null
   void* out;                                     // FWD / DGRAD: [slots][ldo] (null: only dgpart); WGRAD: [E][M][N]
   int64_t ldo;
+  int32_t out32;                                 // FWD / DGRAD: the rows leave in fp32 whatever dtype is (to be summed)
   int32_t kc;                                    // WGRAD: K blocks of a part (xgemm_kc)
   float* parts;                                  // WGRAD: xgemm_parts partial sums [M][N] (null: there are none)
   int32_t* pre;                                  // WGRAD with parts: [E + 1] scratch

@@ -77,6 +77,7 @@ struct XgParams {
   float* parts;
   int32_t* pre;
   int64_t ldo;
+  int32_t out32;
   const void* x;
   int64_t ldx;
   int32_t kdiv;
@@ -467,9 +468,10 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       int slot = -1, orow[4], xrow[4];
       float sc = 1.f, dot = 0.f;
       T* out = (T*)g.out + n0;
-      float* pout = nullptr;                       // WGRAD: partial sums
+      float* pout = nullptr;                       // fp32 results of 16-bit data; WGRAD: partial sums
       int64_t ldo = g.ldo;
       if constexpr (MODE != XG_WGRAD) {            // in flight during the wait
+        if (sizeof(T) == 2 && g.out32) pout = (float*)g.out + n0;
         slot = w.rows_ok ? plan[g.lay.o_row + w.m0 + row] : -1;
         if (slot >= 0 && g.scale) sc = g.scale[slot];
 #pragma unroll
@@ -529,8 +531,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         for (int i = 0; i < 32; ++i) v[i] = add ? v[i] + __uint_as_float(u[i]) : __uint_as_float(u[i]);
       };
       auto emit = [&](int q, const float* v) {
-        if (MODE == XG_WGRAD && pout)
-          xg_emit32<float>(v, at, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, 1.f, nc - 32 * q);
+        if ((MODE == XG_WGRAD || sizeof(T) == 2) && pout)
+          xg_emit32<float>(v, at, stg, orow, pout + 32 * q, ldo, ldo % 4 == 0, sc, nc - 32 * q);
         else
           xg_emit32<T>(v, at, stg, orow, out + 32 * q, ldo, vec, sc, nc - 32 * q);
       };
@@ -740,7 +742,7 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   }
   g.rows = x.rows;
   g.plan = x.plan; g.lay = x.lay; g.scale = x.scale;
-  g.out = x.out; g.ldo = x.ldo;
+  g.out = x.out; g.ldo = x.ldo; g.out32 = x.out32;
   g.parts = x.parts; g.pre = x.pre;
   g.x = x.x; g.ldx = x.ldx; g.kdiv = x.kdiv; g.dgpart = x.dgpart;
   const int64_t items = MODE == XG_WGRAD ? (xgemm_parts(x.E, x.lay.R, x.kc) + x.E) * g.tm : x.lay.tiles;
