@@ -342,24 +342,20 @@ __device__ __forceinline__ uint4 load8_raw(const T* row, int c, int d, bool vec,
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Writes 8 columns as one vector of a 16-bit plane, or of three bf16 planes (fp32 data)
-template <typename T>
+// Writes 8 columns as one vector of each of NP bf16 planes
+template <int NP>
 __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64_t at, const float (&f)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(dst + at) = pack16<T>(f);
-  } else {
-    float r[8];
+  float r[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) r[q] = f[q];
+  for (int q = 0; q < 8; ++q) r[q] = f[q];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      const uint4 u = pack16<bf16>(r);
-      *reinterpret_cast<uint4*>(dst + p * plane + at) = u;
-      float h[8];
-      unpack16(u, h, bf16());
+  for (int p = 0; p < NP; ++p) {
+    const uint4 u = pack16<bf16>(r);
+    *reinterpret_cast<uint4*>(dst + p * plane + at) = u;
+    float h[8];
+    unpack16(u, h, bf16());
 #pragma unroll
-      for (int q = 0; q < 8; ++q) r[q] -= h[q];
-    }
+    for (int q = 0; q < 8; ++q) r[q] -= h[q];
   }
 }
 
@@ -367,12 +363,13 @@ __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64
 // small call more than its work).
 struct XMove {
   int kind;                                      // MOVE_*
+  int planes;                                    // fp32 data: 3 bf16 planes; 16-bit data: 1, the elements as they are, or 2 bf16 planes
   int d, dp, kdiv, vec;
   unsigned block0, blocks;                       // first block and number of blocks
   int64_t rows, lds, plane;
   const void* src;
   const char *lo, *hi;                           // the source's first and last byte + 1
-  const float* scale;
+  const float* scale;                            // not with one plane
   void* out;
 };
 enum {
@@ -383,7 +380,7 @@ enum {
   MOVE_PAD = 2,                                  // out[row] = 0 in planes for the rows that pad the experts' segments
   MOVE_ZERO = 3,                                 // out[slot] = 0 for slots without an expert (elements of T)
 };                                               // columns between d and dp are written as zeros
-constexpr int XMOVES = 6;                        // backward: dy, x, their padding, W, rows without an expert
+constexpr int XMOVES = 7;                        // backward: dy (fp16 with weights: twice), x, their padding, W, rows without an expert
 struct XMoves {
   XMove m[XMOVES];
   int n;
@@ -401,7 +398,6 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
   const XMove& m = mv.m[q];
   const int lane = threadIdx.x & 31, nv = m.dp / 8;
   const int64_t warp0 = (int64_t)(blockIdx.x - m.block0) * 8 + (threadIdx.x >> 5), warps = (int64_t)m.blocks * 8;
-  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   if (m.kind == MOVE_ZERO) {                     // 32 slots a warp; the whole warp zeros a row
     for (int64_t r0 = warp0 * 32; r0 < m.rows; r0 += warps * 32) {
       unsigned todo = __ballot_sync(0xffffffffu, r0 + lane < m.rows && plan[p.o_slot + r0 + lane] < 0);
@@ -418,8 +414,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
       const int e = (int)(i / XP_BM), c = plan[p.o_cnt + e] % XP_BM, r = (int)(i % XP_BM);
       if (c == 0 || r < c) continue;
       const int64_t row = plan[p.o_seg + e + 1] - XP_BM + r;
-#pragma unroll
-      for (int pl = 0; pl < NP; ++pl)
+      for (int pl = 0; pl < m.planes; ++pl)
         for (int v = lane; v < nv; v += 32)
           *reinterpret_cast<uint4*>(out + pl * m.plane + row * m.dp + 8 * v) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -446,8 +441,8 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
           const int64_t to = scatter ? slot_row[row * copies + j] : row;
           if (to < 0) continue;
           uint16_t* o = out + to * m.dp + c0;
-          if (m.scale) {
-            const float g = m.scale[row * copies + j];
+          if (m.planes == 2) {
+            const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (c0 + i * 8 * lpr < m.dp) {
@@ -455,7 +450,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
                 unpack16(u[i], f, T());
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] *= g;
-                *reinterpret_cast<uint4*>(o + i * 8 * lpr) = pack16<T>(f);
+                store_planes<2>(o, m.plane, i * 8 * lpr, f);
               }
           } else {
 #pragma unroll
@@ -475,7 +470,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
           const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
           for (int x = 0; x < 8; ++x) v[x] = f[x] * g;
-          store_planes<T>(out, m.plane, to * m.dp + c, v);
+          store_planes<3>(out, m.plane, to * m.dp + c, v);
         }
       }
     }
@@ -709,16 +704,22 @@ static XFwd x_fwd_layout(const XShape& s, bool combine, bool direct) {
 }
 
 struct XBwd {
-  int64_t xs = -1, dys = -1, ws = -1, dxb = -1, dgp = -1, parts = -1, pre = -1, bytes = 0;
+  int64_t xs = -1, dys = -1, dyw = -1, ws = -1, dxb = -1, dgp = -1, parts = -1, pre = -1, bytes = 0;
   int kc = 0;
+  bool split = false;                            // dW's operands in bf16 planes: 16-bit data with weights
+  int px = 1, pdy = 1;                           // planes of dW's operands
 };
 static XBwd x_bwd_layout(const XShape& s, bool combine, bool x_slots, bool direct, bool need_x, bool need_w,
                          bool need_g) {
   XWork c;
   XBwd b;
-  const int64_t row2 = (int64_t)s.np * s.rows * 2;
-  if (need_w) b.xs = c.take(row2 * s.Dp);
-  b.dys = c.take(row2 * s.Op);
+  b.split = combine && s.dtype != MB_F32;
+  b.px = b.split ? 2 : s.np;
+  b.pdy = b.split && s.dtype == MB_F16 ? 2 : s.np;
+  if (need_w) b.xs = c.take(b.px * s.rows * 2 * s.Dp);
+  // dx takes dy in its own type; dW reads the same rows unless it needs planes of them
+  if (need_x || need_g || b.pdy == s.np) b.dys = c.take(s.np * s.rows * 2 * s.Op);
+  if (need_w) b.dyw = b.pdy == s.np ? b.dys : c.take(b.pdy * s.rows * 2 * s.Op);
   if ((need_x || need_g) && !direct) b.ws = c.take((int64_t)s.np * s.E * s.O * s.Dp * 2);
   if (need_x && !x_slots && s.k > 1) b.dxb = c.take(s.R * s.Dp * 4);
   if (need_g) b.dgp = c.take(s.R * 4 * 2 * xgemm_n_tiles(s.D, s.dtype));
@@ -750,6 +751,7 @@ static XMove move_rows(int kind, const XShape& s, const void* src, int64_t rows,
   const int size = dtype_size(s.dtype);
   XMove m{};
   m.kind = kind;
+  m.planes = s.np;
   m.d = d; m.dp = dp; m.kdiv = 1; m.vec = aligned16(src) && lds % 8 == 0;
   m.rows = rows; m.lds = lds; m.plane = plane;
   m.src = src; m.out = out;
@@ -757,9 +759,10 @@ static XMove move_rows(int kind, const XShape& s, const void* src, int64_t rows,
   m.hi = m.lo + ((rows - 1) * lds + d) * size;
   return m;
 }
-static XMove move_scatter(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, const float* scale,
-                          void* out) {
+static XMove move_scatter(const XShape& s, const void* src, int64_t lds, int d, int dp, int kdiv, int planes,
+                          const float* scale, void* out) {
   XMove m = move_rows(MOVE_SCATTER, s, src, s.R / kdiv, lds, d, dp, s.rows * dp, out);
+  m.planes = planes;
   m.kdiv = kdiv;
   m.scale = scale;
   return m;
@@ -768,8 +771,10 @@ static XMove move_stage(const XShape& s, const void* w, void* out) {
   const int64_t rows = (int64_t)s.E * s.O;
   return move_rows(MOVE_STAGE, s, w, rows, s.D, s.D, s.Dp, rows * s.Dp, out);
 }
-static XMove move_pad(const XShape& s, int dp, void* out) {
-  return move_rows(MOVE_PAD, s, nullptr, (int64_t)s.E * XP_BM, 0, 0, dp, s.rows * dp, out);
+static XMove move_pad(const XShape& s, int dp, int planes, void* out) {
+  XMove m = move_rows(MOVE_PAD, s, nullptr, (int64_t)s.E * XP_BM, 0, 0, dp, s.rows * dp, out);
+  m.planes = planes;
+  return m;
 }
 static XMove move_zero(const XShape& s, void* out, int d) {
   XMove m{};
@@ -923,7 +928,7 @@ extern "C" int mace_b200_expert_linear_fwd(const void* x, int64_t ldx, int32_t x
     using T = decltype(t);
     const bool sum = f.y >= 0;
     XMoves mv{};
-    mv.add(move_scatter(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, nullptr, base + f.xs));
+    mv.add(move_scatter(s, x, ldx, D, s.Dp, x_per_slot ? 1 : k, s.np, nullptr, base + f.xs));
     if (!direct) mv.add(move_stage(s, w, base + f.ws));
     if (!sum) mv.add(move_zero(s, out, O));
     if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
@@ -966,21 +971,22 @@ extern "C" int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_
     using T = decltype(t);
     const bool sum = b.dxb >= 0;
     XMoves mv{};
-    mv.add(move_scatter(s, dy, O, O, s.Op, ky, nullptr, base + b.dys));
+    if (b.dys >= 0) mv.add(move_scatter(s, dy, O, O, s.Op, ky, s.np, nullptr, base + b.dys));
     // the weights scale the rows of x, not those of dy: dy stays exact for dx and dweights, and x is read only here.
     // dW sums over whole segments: their padding rows are zeros in both operands (elsewhere a padding row is never stored).
     if (dw) {
-      mv.add(move_scatter(s, x, ldx, D, s.Dp, kx, weights, base + b.xs));
-      mv.add(move_pad(s, s.Op, base + b.dys));
-      mv.add(move_pad(s, s.Dp, base + b.xs));
+      if (b.dyw != b.dys) mv.add(move_scatter(s, dy, O, O, s.Op, ky, b.pdy, nullptr, base + b.dyw));
+      mv.add(move_scatter(s, x, ldx, D, s.Dp, kx, b.px, weights, base + b.xs));
+      mv.add(move_pad(s, s.Op, b.pdy, base + b.dyw));
+      mv.add(move_pad(s, s.Dp, b.px, base + b.xs));
     }
     if (b.ws >= 0) mv.add(move_stage(s, w, base + b.ws));
     if (dx && !sum) mv.add(move_zero(s, dx, D));
     if (int rc = x_moves<T>(s, mv, plan, st)) return rc;
     if (dw) {
       XGemm g{};
-      g.mode = XG_WGRAD; g.dtype = dtype;
-      g.a = base + b.dys; g.lda = s.Op;
+      g.mode = XG_WGRAD; g.dtype = dtype; g.split = b.split;
+      g.a = base + b.dyw; g.lda = s.Op;
       g.b = base + b.xs; g.ldb = s.Dp;
       g.rows = s.rows;
       g.E = E; g.M = O; g.N = D; g.K = 0;

@@ -37,7 +37,8 @@ inline XPlan xplan(int64_t R, int32_t E) {
 
 enum { XG_FWD = 0, XG_DGRAD = 1, XG_WGRAD = 2 };
 
-// One launch of the tensor-core kernel.  Operands are 16-bit planes (fp32 data: three bf16 planes).
+// One launch of the tensor-core kernel.  Operands are 16-bit planes (fp32 data: three bf16 planes; WGRAD with `split`: two of
+// b, and of a where the data is fp16).
 //   FWD    rows of `a` [planes][rows][lda] (expert-sorted), b = w [planes][E][O][ldb]: C[row][o] = sum_d a[row][d] w[e][o][d]
 //   DGRAD  the same rows with width O, b = w: C[row][d] = sum_o a[row][o] w[e][o][d]
 //   WGRAD  a [planes][rows][lda] (width M = O), b [planes][rows][ldb] (width N = D): C[e][o][d] = sum over e's rows
@@ -52,6 +53,7 @@ struct XGemm {
   void* out;                                     // FWD / DGRAD: [slots][ldo] (null: only dgpart); WGRAD: [E][M][N]
   int64_t ldo;
   int32_t out32;                                 // FWD / DGRAD: the rows leave in fp32 whatever dtype is (to be summed)
+  int32_t split;                                 // WGRAD of 16-bit data: operands in bf16 planes
   int32_t kc;                                    // WGRAD: K blocks of a part (xgemm_kc)
   float* parts;                                  // WGRAD: xgemm_parts partial sums [M][N] (null: there are none)
   int32_t* pre;                                  // WGRAD with parts: [E + 1] scratch

@@ -7,6 +7,10 @@
 // fp32 data comes as three bf16 planes; a stage holds all three of both operands.  The product of the first planes has an
 // accumulator of its own, and the five others whose ranks add up to at most 2 share another; the rest is below 2^-24 of
 // the result.
+// WGRAD with routing weights multiplies rows by fp32 weights of any size: x g comes as two bf16 planes (2^-17 of it, and the
+// exponents of fp32), and fp16 dy as two, which hold it exactly.  The product of the second planes is left out (2^-18).
+// One plane in the type itself was 1.4 times as far off as one rounding, and left the range of fp16 (x g above 65,504,
+// or below 6e-5) where the gradient does not.
 // The tensor cores truncate when they add to an fp32 accumulator: the result shrinks by about 1.7e-8 of itself for each
 // 16-wide step (measured: 3.2e-6 after 192 steps, 4.7e-7 after 32).  Where the result leaves in fp32 (fp32 data, and the
 // gradient of the weights) an accumulator therefore takes a few K blocks at most, and the chunks are added in registers
@@ -52,14 +56,16 @@ constexpr int XG_STG = 2048;                     // row staging of one epilogue 
 // 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: backward 2251 us at 12, 2331 at 8.
 constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12, XG_ACC_K1 = 4;
 
-// T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for
-template <typename T, int BN, int CG>
+// T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for; SPL: XGemm::split
+template <typename T, int BN, int CG, bool SPL>
 struct XgCfg {
-  static constexpr int PL = sizeof(T) == 4 ? 3 : 1;          // planes of a stage
+  static constexpr bool F32 = sizeof(T) == 4, AS_BF16 = SPL || !std::is_same<T, f16>::value;
+  static constexpr int PA = F32 ? 3 : SPL && std::is_same<T, f16>::value ? 2 : 1, PB = F32 ? 3 : SPL ? 2 : 1;   // planes
+  static constexpr int PRODS = PA == 3 ? 6 : PA + PB - 1;    // products of planes: ranks that add up to 2 (fp32) or 1 at most
   static constexpr int A_BYTES = XG_BM * XG_BK * 2, B_BYTES = BN / CG * XG_BK * 2;
-  static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
+  static constexpr int STAGE = PA * A_BYTES + PB * B_BYTES;
   static constexpr int STAGES = 196608 / STAGE;
-  static constexpr int ACC = PL == 3 ? 2 * BN : BN;          // TMEM columns of an accumulator (fp32: both of them)
+  static constexpr int ACC = F32 ? 2 * BN : BN;              // TMEM columns of an accumulator (fp32: both of them)
   static constexpr int TMEM = 2 * ACC;
   // WGRAD, per expert, longest first: first item [E + 1], expert, first row, K blocks
   static constexpr int PRE = (4 * MB_PLAN_MAX_EXPERTS + 1) * 4 + 252;
@@ -225,10 +231,10 @@ __device__ __forceinline__ float xg_dot(const float* v, const XgLane& a, const u
 }
 
 // DOT: DGRAD with dgpart
-template <int MODE, typename T, int BN, int CG, bool DOT>
+template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
-  using C = XgCfg<T, BN, CG>;
+  using C = XgCfg<T, BN, CG, SPL>;
   constexpr bool A_MN = MODE == XG_WGRAD, B_MN = MODE != XG_FWD;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -341,7 +347,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       int seq = 0;
       bool ok = true;
       const uint32_t b_bytes = B_MN ? (uint32_t)((bh + 63) / 64) * 8192u : (uint32_t)bh * 128u;
-      const uint32_t bytes = CG * C::PL * (C::A_BYTES + b_bytes);
+      const uint32_t bytes = CG * (C::PA * C::A_BYTES + C::PB * b_bytes);
       XgTile next{};
       if (tile_at(0) < tiles) next = tile_of(tile_at(0));
       for (int r = 0; ok && r < rounds; ++r) {
@@ -360,14 +366,15 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
           if (rank == 0) mbar_arrive_tx(&B.full[s], bytes);   // both CTAs' bytes arrive at the first one's barrier
           const int k0 = kb * XG_BK;
 #pragma unroll
-          for (int p = 0; p < C::PL; ++p) {
+          for (int p = 0; p < (C::PA > C::PB ? C::PA : C::PB); ++p) {
             const uint32_t a = smem_u32(smem + s * C::STAGE) + p * C::A_BYTES;
-            const uint32_t b = smem_u32(smem + s * C::STAGE) + C::PL * C::A_BYTES + p * C::B_BYTES;
+            const uint32_t b = smem_u32(smem + s * C::STAGE) + C::PA * C::A_BYTES + p * C::B_BYTES;
             const int row0 = (int)(p * g.rows);
             if constexpr (MODE == XG_WGRAD) {
+              if (p < C::PA)
 #pragma unroll
-              for (int c = 0; c < XG_BM / 64; ++c)
-                tma_load_2d<CG>(a + c * 8192, &map_a, w.m0 + 64 * c, row0 + w.r0 + k0, bar);
+                for (int c = 0; c < XG_BM / 64; ++c)
+                  tma_load_2d<CG>(a + c * 8192, &map_a, w.m0 + 64 * c, row0 + w.r0 + k0, bar);
 #pragma unroll
               for (int c = 0; c < BN / CG / 64; ++c)
                 if (c * 64 < bh) tma_load_2d<CG>(b + c * 8192, &map_b, w.n0 + rank * bh + 64 * c, row0 + w.r0 + k0, bar);
@@ -391,7 +398,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------ MMA issue
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = f16_idesc(XG_BM * CG, g.bn, !std::is_same<T, f16>::value, A_MN, B_MN);
+      const uint32_t idesc = f16_idesc(XG_BM * CG, g.bn, C::AS_BF16, A_MN, B_MN);
       int seq = 0, tc = 0;
       bool ok = true;
       uint64_t* last_bar = nullptr;
@@ -417,19 +424,23 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
               break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t a0 = smem_u32(smem + s * C::STAGE), b0 = a0 + C::PL * C::A_BYTES;
+            const uint32_t a0 = smem_u32(smem + s * C::STAGE), b0 = a0 + C::PA * C::A_BYTES;
 #pragma unroll
-            for (int p = 0; p < (C::PL == 3 ? 6 : 1); ++p) {
-              // planes (a, b): (0,2) (2,0) (1,1) (0,1) (1,0), then (0,0) in the other accumulator
-              constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
-              const uint32_t a = a0 + (C::PL == 3 ? PA[p] * C::A_BYTES : 0), b = b0 + (C::PL == 3 ? PB[p] * C::B_BYTES : 0);
-              const uint32_t dp = C::PL == 3 && p < 5 ? d + BN : d;
+            for (int p = 0; p < C::PRODS; ++p) {
+              // planes (a, b), small products first.  fp32: (0,2) (2,0) (1,1) (0,1) (1,0), then (0,0) in the other
+              // accumulator; split: (1,0) of fp16, (0,1), (0,0)
+              constexpr int PA3[6] = {0, 2, 1, 0, 1, 0}, PB3[6] = {2, 0, 1, 1, 0, 0};
+              const int left = C::PRODS - 1 - p;
+              const int pa = C::F32 ? PA3[p] : left == 2 ? 1 : 0, pb = C::F32 ? PB3[p] : left == 1 ? 1 : 0;
+              const uint32_t a = a0 + pa * C::A_BYTES, b = b0 + pb * C::B_BYTES;
+              const bool second = C::F32 && p < 5;
+              const uint32_t dp = second ? d + BN : d;
 #pragma unroll
               for (int kk = 0; kk < XG_BK / 16; ++kk) {
                 // 16 K elements: 32 bytes along a K-major row, two 8-row atoms of an MN-major operand
                 const uint64_t ad = A_MN ? sw128_desc_mn(a + kk * 2048, 8192) : sw128_desc(a + kk * 32);
                 const uint64_t bd = B_MN ? sw128_desc_mn(b + kk * 2048, 8192) : sw128_desc(b + kk * 32);
-                mma_f16_ss<CG>(dp, ad, bd, idesc, (kb > kb0 || kk > 0 || (p > 0 && p < 5)) ? 1u : 0u);
+                mma_f16_ss<CG>(dp, ad, bd, idesc, (kb > kb0 || kk > 0 || (p > 0 && second == (C::F32 && p - 1 < 5))) ? 1u : 0u);
               }
             }
             mma_commit_to<CG>(&B.empty[s]);
@@ -518,7 +529,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
         const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * C::ACC + hf * hw + 32 * q);
         uint32_t u[32];
         tmem_ld32(ta, u);
-        if constexpr (C::PL == 3) {
+        if constexpr (C::F32) {
           uint32_t u2[32];
           tmem_ld32(ta + BN, u2);
           tmem_wait_ld();
@@ -698,13 +709,13 @@ int64_t xgemm_parts(int64_t E, int64_t slots, int kc) {
   return blocks / kc + E;
 }
 
-template <int MODE, typename T, int BN, int CG, bool DOT>
+template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL>
 static int xg_go(const XGemm& x, cudaStream_t st) {
-  using C = XgCfg<T, BN, CG>;
+  using C = XgCfg<T, BN, CG, SPL>;
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
-  auto kern = k_expert_gemm<MODE, T, BN, CG, DOT>;
+  auto kern = k_expert_gemm<MODE, T, BN, CG, DOT, SPL>;
   if (ready_dev != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -723,20 +734,20 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   g.bn = (int)(((x.N + g.tn - 1) / g.tn + 63) / 64 * 64);
   g.tm = (x.M + XG_BM * CG - 1) / (XG_BM * CG);
   g.kc = x.kc;
-  const bool is_bf16 = !std::is_same<T, f16>::value;
+  const bool is_bf16 = C::AS_BF16;
   CUtensorMap ma, mbm;
   {
-    const int64_t dims[2] = {x.lda, C::PL * x.rows}, str[1] = {x.lda};
+    const int64_t dims[2] = {x.lda, C::PA * x.rows}, str[1] = {x.lda};
     const int box[2] = {64, MODE == XG_WGRAD ? XG_BK : XG_BM};
     if (int rc = xg_map(&ma, is_bf16, 2, x.a, dims, str, box)) return rc;
   }
   if (MODE == XG_WGRAD) {
-    const int64_t dims[2] = {x.ldb, C::PL * x.rows}, str[1] = {x.ldb};
+    const int64_t dims[2] = {x.ldb, C::PB * x.rows}, str[1] = {x.ldb};
     const int box[2] = {64, XG_BK};
     if (int rc = xg_map(&mbm, is_bf16, 2, x.b, dims, str, box)) return rc;
   } else {
     const int64_t O = MODE == XG_FWD ? x.N : x.K;
-    const int64_t dims[3] = {x.ldb, O, (int64_t)C::PL * x.E}, str[2] = {x.ldb, x.ldb * O};
+    const int64_t dims[3] = {x.ldb, O, (int64_t)C::PB * x.E}, str[2] = {x.ldb, x.ldb * O};
     const int box[3] = {64, MODE == XG_FWD ? g.bn / CG : XG_BK, 1};
     if (int rc = xg_map(&mbm, is_bf16, 3, x.b, dims, str, box)) return rc;
   }
@@ -746,8 +757,8 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   g.parts = x.parts; g.pre = x.pre;
   g.x = x.x; g.ldx = x.ldx; g.kdiv = x.kdiv; g.dgpart = x.dgpart;
   const int64_t items = MODE == XG_WGRAD ? (xgemm_parts(x.E, x.lay.R, x.kc) + x.E) * g.tm : x.lay.tiles;
-  if (items * g.tn > 0x7fffffff || C::PL * x.rows > 0x7fffffff) {
-    set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)(items * g.tn), (long long)(C::PL * x.rows));
+  if (items * g.tn > 0x7fffffff || C::PB * x.rows > 0x7fffffff) {
+    set_error("expert_linear: too many tiles (%lld) or rows (%lld)", (long long)(items * g.tn), (long long)(C::PB * x.rows));
     return MB_E_ARG;
   }
   if (items == 0) return 0;
@@ -789,25 +800,27 @@ static bool xg_pairs(const XGemm& x) {
   return blocks >= 16 && 8 * waste <= m && tiles >= 8 * (int64_t)(sm_count() / 2);
 }
 
-template <int MODE, typename T, bool DOT>
-static int xg_dot_any(const XGemm& x, cudaStream_t st) {
+template <int MODE, typename T, bool DOT, bool SPL>
+static int xg_bn_any(const XGemm& x, cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
     if (xg_bn_max(x.N, x.dtype) == 256)
-      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT>(x, st) : xg_go<MODE, T, 256, 1, DOT>(x, st);
-  return xg_go<MODE, T, 128, 1, DOT>(x, st);
+      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT, SPL>(x, st) : xg_go<MODE, T, 256, 1, DOT, SPL>(x, st);
+  return xg_go<MODE, T, 128, 1, DOT, SPL>(x, st);
 }
 
 template <int MODE, typename T>
-static int xg_bn_any(const XGemm& x, cudaStream_t st) {
+static int xg_form(const XGemm& x, cudaStream_t st) {
   if constexpr (MODE == XG_DGRAD)
-    if (x.dgpart) return xg_dot_any<MODE, T, true>(x, st);
-  return xg_dot_any<MODE, T, false>(x, st);
+    if (x.dgpart) return xg_bn_any<MODE, T, true, false>(x, st);
+  if constexpr (MODE == XG_WGRAD && sizeof(T) == 2)
+    if (x.split) return xg_bn_any<MODE, T, false, true>(x, st);
+  return xg_bn_any<MODE, T, false, false>(x, st);
 }
 
 template <int MODE>
 static int xg_type(const XGemm& x, cudaStream_t st) {
-  if (x.dtype == MB_F32) return xg_bn_any<MODE, float>(x, st);
-  return x.dtype == MB_BF16 ? xg_bn_any<MODE, bf16>(x, st) : xg_bn_any<MODE, f16>(x, st);
+  if (x.dtype == MB_F32) return xg_form<MODE, float>(x, st);
+  return x.dtype == MB_BF16 ? xg_form<MODE, bf16>(x, st) : xg_form<MODE, f16>(x, st);
 }
 
 int xgemm_launch(const XGemm& x, cudaStream_t st) {
