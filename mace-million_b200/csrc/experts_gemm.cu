@@ -11,10 +11,12 @@
 // exponents of fp32), and fp16 dy as two, which hold it exactly.  The product of the second planes is left out (2^-18).
 // One plane in the type itself was 1.4 times as far off as one rounding, and left the range of fp16 (x g above 65,504,
 // or below 6e-5) where the gradient does not.
-// The tensor cores truncate when they add to an fp32 accumulator: the result shrinks by about 1.7e-8 of itself for each
-// 16-wide step (measured: 3.2e-6 after 192 steps, 4.7e-7 after 32).  Where the result leaves in fp32 (fp32 data, and the
-// gradient of the weights) an accumulator therefore takes a few K blocks at most, and the chunks are added in registers
-// with rounding to nearest; 16-bit results are rounded a thousand times more coarsely and take the whole K.
+// The tensor cores truncate when they add to an fp32 accumulator.  Sums of one sign lose 1e-7 of themselves for each 16-wide
+// step (measured: 2.5e-3 after 25,000 steps), products of either sign less (a deviation of 3.2e-6 after 192 steps, 4.7e-7
+// after 32).  Where the result leaves in fp32 (fp32 data, and the gradient of the routing weights) an accumulator therefore
+// takes a few K blocks at most, and the chunks are added in registers with rounding to nearest.  16-bit results take up to
+// XG_ACC_LONG K blocks in one accumulator: 4e-5, a fifth of the deviation of an fp16 rounding.  Longer sums are cut: WGRAD
+// into parts that are added in fp32 afterwards, FWD and DGRAD into chunks in registers.
 //
 // Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
 // into one of two TMEM accumulators, warps 4-11 drain the other one (a lane holds half a row).  CG = 2: a cluster of two
@@ -55,6 +57,7 @@ constexpr int XG_STG = 2048;                     // row staging of one epilogue 
 // at most (its drains cost nothing then).  Gradients of the weights from 16-bit data, 2,048 columns: error 7e-7 at 12,
 // 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: backward 2251 us at 12, 2331 at 8.
 constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12, XG_ACC_K1 = 4;
+constexpr int XG_ACC_LONG = 96;                  // and of one whose result leaves in 16 bits
 
 // T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for; SPL: XGemm::split
 template <typename T, int BN, int CG, bool SPL>
@@ -230,8 +233,8 @@ __device__ __forceinline__ float xg_dot(const float* v, const XgLane& a, const u
   return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// DOT: DGRAD with dgpart
-template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL>
+// DOT: DGRAD with dgpart; LONG: FWD or DGRAD of 16-bit data with K of more than XG_ACC_LONG blocks
+template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL, bool LONG>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
   using C = XgCfg<T, BN, CG, SPL>;
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
   const uint32_t tmem = B.tmem;
   const int tiles = MODE == XG_WGRAD ? pre[g.E] * g.tm * g.tn : plan[CG == 2 ? 2 : 0] * g.tn;
   const int rounds = (tiles + ctas - 1) / ctas;
-  constexpr bool CHUNKS = sizeof(T) == 4 || DOT;
+  constexpr bool CHUNKS = sizeof(T) == 4 || DOT || LONG;
   auto tile_at = [&](int n) { return n * ctas + (MODE == XG_WGRAD && (n & 1) ? ctas - 1 - cta : cta); };
   auto tile_of = [&](int t) {
     XgTile o;
@@ -331,7 +334,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     }
     o.ck = o.nk;                                 // K blocks of one accumulator: even chunks
     if constexpr (CHUNKS) {
-      const int most = rounds == 1 ? XG_ACC_K1 : sizeof(T) == 4 ? XG_ACC_K : XG_ACC_K16, n = (o.nk + most - 1) / most;
+      const int most = LONG ? XG_ACC_LONG : rounds == 1 ? XG_ACC_K1 : sizeof(T) == 4 ? XG_ACC_K : XG_ACC_K16;
+      const int n = (o.nk + most - 1) / most;
       if (n > 1) o.ck = (o.nk + n - 1) / n;
     }
     return o;
@@ -693,29 +697,30 @@ int xgemm_n_tiles(int64_t N, int dtype) {
 }
 
 // K blocks of a part in WGRAD: whole experts when that makes four or more rounds of tiles, else parts that make about
-// that many, of at least 8 K blocks (below that the partial sums' traffic outweighs the idle SMs)
+// that many, of at least 8 K blocks (below that the partial sums' traffic outweighs the idle SMs); for 16-bit data no more
+// than an accumulator takes
 int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype) {
   const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype), want = 4 * (int64_t)sm_count();
   const int64_t blocks = slots / XG_BK;          // K blocks of all experts
-  if (E * per >= want) return 0x3fffffff;
-  int64_t kc = blocks * per / want;
-  const int64_t least = dtype == MB_F32 ? 4 : 8;
-  return (int)(kc < least ? least : kc);
+  const int64_t most = dtype == MB_F32 ? 0x3fffffff : XG_ACC_LONG;
+  if (E * per >= want) return (int)most;
+  const int64_t kc = blocks * per / want, least = dtype == MB_F32 ? 4 : 8;
+  return (int)(kc < least ? least : kc < most ? kc : most);
 }
-// most partial sums there can be: a part has kc K blocks but the last of an expert, and an expert of one part has none
+// Most partial sums there can be.  The m experts with more than kc K blocks have more than 64 kc slots each, and come first
+// among the items; ceil(nk / kc) <= (nk - 1) / kc + 1 parts each, and their nk add up to slots / 64 + m at most.
 int64_t xgemm_parts(int64_t E, int64_t slots, int kc) {
-  if (kc >= 0x3fffffff) return 0;
-  const int64_t blocks = slots / XG_BK + E;
-  return blocks / kc + E;
+  const int64_t blocks = (slots + XG_BK - 1) / XG_BK, m = blocks / kc < E ? blocks / kc : E;
+  return blocks / kc + m;
 }
 
-template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL>
+template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL, bool LONG>
 static int xg_go(const XGemm& x, cudaStream_t st) {
   using C = XgCfg<T, BN, CG, SPL>;
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("expert_linear (device)");
-  auto kern = k_expert_gemm<MODE, T, BN, CG, DOT, SPL>;
+  auto kern = k_expert_gemm<MODE, T, BN, CG, DOT, SPL, LONG>;
   if (ready_dev != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
       set_error("expert_linear: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -730,7 +735,7 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
   }
   XgParams g{};
   g.E = x.E; g.M = x.M; g.N = x.N; g.K = x.K;
-  g.tn = xgemm_n_tiles(x.N, x.dtype);
+  g.tn = (x.N + BN - 1) / BN;
   g.bn = (int)(((x.N + g.tn - 1) / g.tn + 63) / 64 * 64);
   g.tm = (x.M + XG_BM * CG - 1) / (XG_BM * CG);
   g.kc = x.kc;
@@ -802,10 +807,12 @@ static bool xg_pairs(const XGemm& x) {
 
 template <int MODE, typename T, bool DOT, bool SPL>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2 && MODE != XG_WGRAD && !DOT)
+    if (x.K > XG_ACC_LONG * XG_BK) return xg_go<MODE, T, 128, 1, DOT, SPL, true>(x, st);
   if constexpr (sizeof(T) == 2)
     if (xg_bn_max(x.N, x.dtype) == 256)
-      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT, SPL>(x, st) : xg_go<MODE, T, 256, 1, DOT, SPL>(x, st);
-  return xg_go<MODE, T, 128, 1, DOT, SPL>(x, st);
+      return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT, SPL, false>(x, st) : xg_go<MODE, T, 256, 1, DOT, SPL, false>(x, st);
+  return xg_go<MODE, T, 128, 1, DOT, SPL, false>(x, st);
 }
 
 template <int MODE, typename T>

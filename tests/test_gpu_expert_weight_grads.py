@@ -66,3 +66,60 @@ def test_weighted_gradient_over_the_range_of_the_weights(weight, xs, dys):
     dw = _grad(x, torch.zeros(E, O, D, device="cuda", dtype=torch.float16), ex, p, dy)
     assert torch.isfinite(dw).all()
     _one_rounding(dw, want)
+
+
+def _skewed(T, E, D, O, dt, weighted, seed=3):
+    """T slots, all but E of them on expert 0, with products of one sign; columns of different size, so that the sums spread
+    over the steps of the type."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cx, cy = (torch.rand(n, device="cuda", generator=g) + 0.5 for n in (D, O))
+    x = ((torch.rand(T, D, device="cuda", generator=g) + 0.5) * cx / 64).to(dt)
+    dy = ((torch.rand(T, 1, O, device="cuda", generator=g) + 0.5) * cy).to(dt)
+    ex = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    ex[:E, 0] = torch.arange(E, device="cuda")
+    p = torch.rand(T, 1, device="cuda", generator=g) + 0.5 if weighted else None
+    return x, dy[:, 0] if weighted else dy, ex, p
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("E", [1, 8, 640])
+def test_long_sums_over_one_expert_do_not_shrink(E, weighted, dt):
+    """400,000 rows on one expert, whatever the number of experts.  The tensor cores cut off what they add to an accumulator:
+    sums of one sign lose 1e-7 for each 16 terms (measured: 2.5e-3 of this one when it is left alone).  5.3e-5 are 530 such steps.
+    Rounding to the type has a deviation of u / sqrt(3) at most, u = 2^-8 or 2^-11: 4 u / sqrt(3 D O) is four deviations
+    of the mean."""
+    T, D, O = 400_000, 64, 72
+    x, dy, ex, p = _skewed(T, E, D, O, dt, weighted)
+    dw = _grad(x, torch.zeros(E, O, D, device="cuda", dtype=dt), ex, p, dy)
+    z = dy.reshape(T, O).double() * (1.0 if p is None else p.double())
+    on = ex[:, 0] == 0
+    want = z[on].T @ x[on].double()
+    assert want.abs().max() < 6e4
+    mean = float(((dw[0].double() - want) / want).mean())
+    u = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -11
+    assert abs(mean) <= 5.3e-5 + 4 * u / (3 * D * O) ** 0.5, mean
+    last = min(E - 1, 5)
+    t = torch.nonzero(ex[:, 0] == last)[:, 0]
+    want = z[t].T @ x[t].double()
+    assert (dw[last].double() - want).norm() <= u * want.norm()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_very_wide_rows_do_not_shrink(dt):
+    """The same for the products along the widths: 300,000 columns of one sign, forward (D) and dx (O)."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    wide, n, T = 300_000, 72, 50
+    u = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -11
+    a = ((torch.rand(T, wide, device="cuda", generator=g) + 0.5) * (torch.rand(T, 1, device="cuda", generator=g) + 0.5)).to(dt)
+    c = ((torch.rand(1, n, wide, device="cuda", generator=g) + 0.5) * (torch.rand(1, n, 1, device="cuda", generator=g) + 0.5) / 64).to(dt)
+    want = a.double() @ c[0].double().T
+    plan = X.plan_experts(torch.zeros(T, 1, dtype=torch.int32, device="cuda"), 1)
+    fwd = X.expert_linear(a.requires_grad_(), c, plan)[:, 0].detach()
+    x = torch.zeros(T, n, device="cuda", dtype=dt).requires_grad_()
+    w = c.transpose(1, 2).contiguous()
+    dx, = torch.autograd.grad(X.expert_linear(x, w, plan), x, a.detach()[:, None])
+    plan.check()
+    for got in (fwd, dx):
+        mean = float(((got.double() - want) / want).mean())
+        assert abs(mean) <= 5.3e-5 + 4 * u / (3 * T * n) ** 0.5, mean
