@@ -399,6 +399,8 @@ int mace_b200_expert_linear_bwd(const void* dy, const void* x, int64_t ldx, int3
                                 void* workspace, int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
                                 int32_t dtype, void* stream);
 int mace_b200_expert_test_hooks(uint64_t wait_ns, int32_t skip_one_load);
+/* Number (unique in the process) of the CUDA graph capture that the stream is in; 0 when it is in none. */
+uint64_t mace_b200_capture_id(void* stream);
 
 #ifdef __cplusplus
 }

@@ -856,6 +856,16 @@ extern "C" int mace_b200_expert_plan(const int32_t* experts, int64_t slots, int3
   return check_launch("expert_plan");
 }
 
+extern "C" uint64_t mace_b200_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+    cudaGetLastError();                            // the legacy stream while another one captures: not in a capture itself
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 extern "C" int mace_b200_expert_linear_workspace(int64_t tokens, int32_t k, int32_t E, int32_t D, int32_t O,
                                                  int32_t dtype, int32_t x_per_slot, int32_t weighted, int32_t backward,
                                                  int64_t* bytes) {

@@ -111,6 +111,7 @@ _SIGS = {
     "mace_b200_expert_linear_fwd": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32,
                                             c_i32, c_i32, c_i32, c_vp]),
     "mace_b200_expert_test_hooks": (c_i32, [c_u64, c_i32]),
+    "mace_b200_capture_id": (c_u64, [c_vp]),
     "mace_b200_expert_linear_bwd": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                             c_i32, c_i32, c_i32, c_i32, c_i32, c_vp]),
 }

@@ -61,9 +61,37 @@ def route(logits, k, *, bias=None, score="softmax", groups=1, top_groups=1, reno
                         float(scale))
 
 
+def _place(device):
+    """The current stream (its handle) and the number of the CUDA graph capture it is in (0: none)."""
+    if device.type != "cuda" or not torch.cuda.is_initialized():
+        return 0, 0
+    stream = torch._C._cuda_getCurrentRawStream(device.index)   # a Stream object would cost a small call 2 us
+    return stream, N.lib().mace_b200_capture_id(stream)
+
+
+def _ready(device):
+    """An event of what the current stream holds so far."""
+    return torch.cuda.current_stream(device).record_event()
+
+
+def _after(device, event, *tensors):
+    """Makes the current stream wait for the event, and the tensors live for as long as it uses them."""
+    stream = torch.cuda.current_stream(device)
+    if event is not None:
+        stream.wait_event(event)
+    for t in tensors:
+        t.record_stream(stream)
+
+
 class ExpertPlan:
     """The slots (token, choice) of `experts` [T, k] (or [T]) in expert order, for any number of expert_linear calls
-    with the same choice.  An expert of -1 means none.  Sorted on the device at the first product that needs it."""
+    with the same choice.  An expert of -1 means none.
+
+    Contiguous int32 indices are kept as they are (a copy would cost a small call half of its time): products refuse a plan
+    whose indices torch has changed since.  Others are copied.  They are sorted at the first product that needs it, and
+    products on other streams wait for that.  A CUDA graph sorts for itself, at every replay what the indices' buffer holds
+    then; nothing sorted in a capture is used outside of it.  Where a graph's replays write the indices, make a new plan
+    after each (nothing tells an older one), or make it in the graph."""
 
     def __init__(self, experts, n_experts):
         n = experts.dim()
@@ -74,22 +102,47 @@ class ExpertPlan:
             raise ValueError("n_experts must be positive")
         if n == 1:
             experts = experts[:, None]
+        self._version = None                        # of indices that are the caller's
         if experts.dtype != torch.int32:
             # 64-bit indices outside the range of int32 must not wrap into it: -2 is refused by check(), like any other
-            experts = torch.where((experts >= -1) & (experts < self.n_experts), experts, -2).to(torch.int32)
-        self.experts = experts if experts.is_contiguous() else experts.contiguous()
-        self._words = None
+            experts = torch.where((experts >= -1) & (experts < self.n_experts), experts, -2).to(torch.int32).contiguous()
+        elif not experts.is_contiguous():
+            experts = experts.contiguous()
+        elif experts.is_inference():                # has no version
+            experts = experts.clone()
+        else:
+            self._version = experts._version
+        self.experts = experts
+        self._stream, self._capture = _place(experts.device)
+        self._sorted = None                         # (words, stream, capture, event)
+
+    def here(self):
+        """The current stream and capture.  Keeps the plan's indices alive for that stream, and checks that they are the ones
+        that the plan was made of."""
+        at = _place(self.experts.device)
+        if at[0] != self._stream:
+            _after(self.experts.device, None, self.experts)
+        if self._version is not None and self.experts._version != self._version:
+            raise RuntimeError("the indices of this plan were changed in place after plan_experts: make a new plan")
+        return at
 
     @property
     def words(self):
-        """The plan as the kernels read it (int32)."""
-        if self._words is None:
-            self._words = _op("expert_plan")(self.experts, self.n_experts)
-        return self._words
+        """The plan as the kernels read it (int32), for the current stream."""
+        stream, capture = self.here()
+        s = self._sorted
+        # tables of another capture hold nothing before its first replay; eager ones may be freed while a graph uses them;
+        # and the indices of a plan that was made in a capture are written anew by every replay
+        if s is None or s[2] != capture or (capture == 0 and self._capture != 0):
+            s = (_op("expert_plan")(self.experts, self.n_experts), stream, capture, _ready(self.experts.device))
+            self._sorted = s
+        elif s[1] != stream:
+            _after(self.experts.device, s[3], s[0])
+        return s[0]
 
     def check(self):
         """Reads the device status word (synchronises) and raises if an index was outside [-1, n_experts) or a product
-        gave up waiting."""
+        outside of CUDA graphs gave up waiting."""
         st = int(self.words[1].item())
         if st & N.ST_BAD_EXPERT:
             raise RuntimeError(f"expert index outside [-1, {self.n_experts})")
@@ -116,6 +169,8 @@ def expert_linear(x, w, plan, weights=None):
     few = slots <= FEW_SLOTS and slots * w.shape[1] * w.shape[2] * w.element_size() <= FEW_BYTES
     if few and torch.is_grad_enabled():
         few = not (x.requires_grad or w.requires_grad or (weights is not None and weights.requires_grad))
+    if few:
+        plan.here()
     return _op("expert_linear")(x, w, plan.experts, None if few else plan.words, weights)
 
 
