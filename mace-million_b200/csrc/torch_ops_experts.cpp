@@ -183,7 +183,14 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// a tangent would be dropped below autograd
+void no_dual(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 Tensor layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  no_dual("layer_norm", {&x, &or_none(w), &or_none(b)});
   if (wants_grad({&x, &or_none(w), &or_none(b)})) {
     TORCH_CHECK(!given(w) || !given(b) || w->scalar_type() == b->scalar_type(), "weight and bias differ in type");
     return LayerNormGrad::apply(x, w, b, eps);
@@ -278,6 +285,7 @@ struct RouteGrad : torch::autograd::Function<RouteGrad> {
 
 std::tuple<Tensor, Tensor> route_autograd(const Tensor& logits, const OptTensor& bias, int64_t k, bool softmax,
                                           int64_t groups, int64_t top_groups, bool renormalize, double scale) {
+  no_dual("route", {&logits});
   if (wants_grad({&logits})) {
     auto r = RouteGrad::apply(logits, bias, k, softmax, groups, top_groups, renormalize, scale);
     return {r[0], r[1]};
@@ -422,6 +430,7 @@ struct ExpertLinearGrad : torch::autograd::Function<ExpertLinearGrad> {
 
 Tensor expert_linear_autograd(const Tensor& x, const Tensor& w, const Tensor& experts, const OptTensor& plan,
                               const OptTensor& weights) {
+  no_dual("expert_linear", {&x, &w, &or_none(weights)});
   if (wants_grad({&x, &w, &or_none(weights)})) {
     static auto make = op_of<decltype(expert_plan)>("mace_b200::expert_plan");
     Tensor p = given(plan) ? *plan : make.call(experts, w.size(0));
