@@ -324,9 +324,22 @@ __global__ void __launch_bounds__(32 * RT_WARPS, rt_blocks<NE>) k_route_fwd(cons
     }
     __syncwarp();
     // weights: the chosen logits once more, L slots at a time
-    if (a.softmax && !known) {                    // only the chosen ones count: relative to the best of them
-      const int i = chosen[0];
-      m = live && i >= 0 ? to_f(p[i]) : 0.f;
+    // renormalised softmax weights depend on the chosen logits alone: relative to the best of them, as in the gradient (the
+    // row's largest logit may be out of exp's range above all that a bias or the groups left)
+    if (a.softmax && a.renorm) {
+      if (!a.bias) {                              // the first choice has it
+        const int i = chosen[0];
+        m = live && i >= 0 ? to_f(p[i]) : 0.f;
+      } else {
+        m = -INFINITY;
+        for (int q = sub; q < a.k; q += L) {
+          const int i = chosen[q];
+          if (live && i >= 0) m = fmaxf(m, to_f(p[i]));
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m == -INFINITY) m = 0.f;
+      }
     }
     float tot = 0.f;
     for (int q = sub; q < a.k; q += L) {
