@@ -26,8 +26,8 @@
 // WGRAD cuts an expert's rows into parts of kc K blocks when there are few tiles; parts of an expert with several are
 // added up afterwards in their order.  Items come longest expert first and odd rounds run backwards over the CTAs, so
 // that every CTA gets about the same number of K blocks.
-// Every wait is bounded: on expiry the kernel sets MB_ST_TC_TIMEOUT in the plan's status word, drains its copies and
-// MMAs, frees its TMEM and returns.
+// Every wait is bounded: on expiry the kernel sets MB_ST_TC_TIMEOUT in the plan's status word, fills the tiles that it has no
+// result for with NaN, drains its copies and MMAs, frees its TMEM and returns.
 //
 // What bounds it (B200; copy 6.5 TB/s, cuBLAS bf16 1.64 PFLOP/s in a burst and 1.37 sustained): 262,144 slots on 64 experts,
 // 1024 -> 2048 bf16, pairs: forward 833 us, dx alone about 780, dx with the gradient of the weights 942, dW 815 (1.32, 1.4,
@@ -473,9 +473,10 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     constexpr int NG = BN / 64;                    // groups of 32 columns in a half row
     constexpr int XC = 32 * 2 / (int)sizeof(T);    // columns of x in a fetch (64 bytes)
     int tc = 0;
-    bool ok = true;
-    // every exit decision is warp-uniform: the loop body holds warp-collective tcgen05.ld.sync.aligned
-    for (int r = 0; ok && r < rounds; ++r) {
+    // after a wait that expired the rest of this CTA's tiles is filled with NaN; the flag is warp-uniform (the loop body holds
+    // the warp-collective tcgen05.ld.sync.aligned)
+    bool lost = false;
+    for (int r = 0; r < rounds; ++r) {
       const int t = tile_at(r);
       if (t >= tiles) break;
       const XgTile w = tile_of(t);
@@ -553,26 +554,23 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
       };
       if constexpr (!CHUNKS) {                     // one accumulator: 32 columns at a time straight from TMEM
         const int acc = tc & 1;
-        if (w.nk > 0 && !wait(acc)) {
-          ok = false;
-          break;
-        }
+        if (w.nk > 0 && !lost) lost = !wait(acc);
+        const bool have = w.nk > 0 && !lost;
+        if (w.nk > 0 && lost) sc = __int_as_float(0x7fc00000);
 #pragma unroll 1
         for (int q = 0; 32 * q < nc; ++q) {
           float v[32];
-          if (w.nk > 0) {
+          if (have) {
             load32(acc, q, v, false);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
-          if (w.nk > 0 && 32 * (q + 1) >= nc) release(acc);
+          if (have && 32 * (q + 1) >= nc) release(acc);
           emit(q, v);
         }
-        if (w.nk > 0) {
-          if (nc <= 0) release(acc);
-          ++tc;
-        }
+        if (have && nc <= 0) release(acc);
+        if (w.nk > 0) ++tc;
       } else {                                     // chunks of K: their sum stays in registers
         float v[NG][32];
 #pragma unroll
@@ -581,16 +579,14 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
           for (int i = 0; i < 32; ++i) v[q][i] = 0.f;
         for (int kb0 = 0; kb0 < w.nk; kb0 += w.ck, ++tc) {
           const int acc = tc & 1;
-          if (!wait(acc)) {
-            ok = false;
-            break;
-          }
+          if (!lost) lost = !wait(acc);
+          if (lost) break;
 #pragma unroll
           for (int q = 0; q < NG; ++q)
             if (32 * q < nc) load32(acc, q, v[q], true);
           release(acc);
         }
-        if (!ok) break;
+        if (w.nk > 0 && lost) sc = dot = __int_as_float(0x7fc00000);
         if constexpr (DOT) {
 #pragma unroll
           for (int h = 0; h < 32 * NG / XC; ++h) {
