@@ -17,6 +17,7 @@ from __future__ import annotations
 import heapq
 import math
 import os
+import weakref
 
 import numpy as np
 import torch
@@ -438,6 +439,7 @@ class ThreePassEngine:
         self._marks_valid = False
         self._h2d_marks = None
         self._ev_cache = {}
+        self._features = None             # (weak reference to the plan of the last complete evaluation, its H1)
         self.host_pf_written = False
 
     # ------------------------------------------------------------------------------------------------ buffers
@@ -640,9 +642,11 @@ class ThreePassEngine:
     _PASSES = ("A", "xchg_fwd", "B", "xchg_rev", "C", "finalize")
 
     def node_features(self, plan: Plan) -> torch.Tensor:
-        """Layer-1 features H1 [nt, 4, 128] (0e | 1o) of the last evaluation of `plan`: the engine's buffer, which the
-        next evaluation overwrites."""
-        return self._get("H1", (plan.nt, 4, C), torch.float32)
+        """Layer-1 features H1 [nt, 4, 128] (0e | 1o) of the engine's last evaluation, which must have been one of `plan`:
+        the engine's buffer, which the next evaluation overwrites.  No gradient leads from it to the positions."""
+        if self._features is None or self._features[0]() is not plan:
+            raise RuntimeError("node_features: the engine's last evaluation was not one of this plan")
+        return self._features[1]
 
     def _pass_marks(self):
         if self._marks is None:
@@ -691,6 +695,7 @@ class ThreePassEngine:
         finished the chunk (self.host_pf_written tells whether that happened; the returned device array is then
         complete as well)."""
         self.host_pf_written = False
+        self._features = None
         deferred = plan.host_src is not None
         use_graph = self.graphs if graph is None else graph
         if use_graph and forward_exchange is None and reverse_exchange is None and not deferred:
@@ -768,9 +773,12 @@ class ThreePassEngine:
         self._last = b
         if deferred and int(b["status"].item()) & N.ST_UNSORTED:
             # the streamed pair list was not receiver-sorted after all: evaluate again from a sorted device copy
-            return self.evaluate(plan.sorted_copy(self), forward_exchange, reverse_exchange, check, graph, host_pf)
+            out = self.evaluate(plan.sorted_copy(self), forward_exchange, reverse_exchange, check, graph, host_pf)
+            self._features = (weakref.ref(plan), self._features[1])
+            return out
         if check:
             self._check_status(b, "evaluation")
+        self._features = (weakref.ref(plan), b["H1"])
         self.fmax = float(fbits.view(torch.float32).item()) if check else None
         return b["eat"][:plan.nl], PFd
 
