@@ -577,8 +577,8 @@ static int ln_types(int dtype, int ptype, const F& f) {
 }
 
 static int ln_check(const char* who, int64_t n, int32_t d, int64_t ldx, int32_t dtype, int32_t ptype) {
-  if (n < 0 || d < 1 || ldx < d) {
-    set_error("%s: bad sizes (rows %lld, width %d, row stride %lld)", who, (long long)n, d, (long long)ldx);
+  if (n < 0 || d < 1 || d > MB_NORM_MAX_WIDTH || ldx < d) {   // the kernels' column counters are 32 bits wide
+    set_error("%s: bad sizes (rows %lld, width %d of at most 2^30, row stride %lld)", who, (long long)n, d, (long long)ldx);
     return MB_E_ARG;
   }
   if (!dtype_ok(dtype) || (ptype != dtype && ptype != MB_F32)) {
@@ -623,7 +623,7 @@ extern "C" int mace_b200_layer_norm_fwd(const void* x, int64_t ldx, const void* 
 }
 
 extern "C" int mace_b200_layer_norm_bwd_workspace(int64_t n, int32_t d, int64_t* floats) {
-  if (n < 0 || d < 1 || !floats) {
+  if (n < 0 || d < 1 || d > MB_NORM_MAX_WIDTH || !floats) {
     set_error("layer_norm_bwd_workspace: bad arguments (rows %lld, width %d)", (long long)n, d);
     return MB_E_ARG;
   }
