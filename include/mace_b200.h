@@ -381,7 +381,7 @@ int mace_b200_route_bwd(const float* dweights, const void* logits, int64_t ldl, 
  * mace_b200_expert_linear_workspace bytes (256-byte aligned); few needs neither and reads the indices directly (at
  * most MB_FEW_MAX_SLOTS slots; an index outside [0, E) counts as -1).
  * bwd: dy as out; dx as x but dense, dw [E][O][D], dweights [tokens][k]; any may be null (dweights needs weights).
- * fp32 data: a value that is infinite, or that bfloat16 rounds to infinity, gives NaN in the results it enters.
+ * fp32 data: an infinite value gives NaN in the results it enters.
  * expert_test_hooks: as mace_b200_tc_test_hooks, for the products (skip_one_load: the first load goes missing once). */
 #define MB_PLAN_MAX_EXPERTS 1024
 #define MB_FEW_MAX_SLOTS 4096

@@ -4,8 +4,9 @@
 // This file holds the plan (slots sorted by expert), the few-slots form, and the kernels that move rows: gather into
 // expert order, sum of a token's rows.  The products themselves are in experts_gemm.cu.
 //
-// fp32 operands become three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits
-// of mantissa, and bf16 has the exponent range of fp32, so nothing overflows that fp32 holds.
+// fp32 operands become three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): the 24 bits
+// of the mantissa for values above 2^-109 (the planes end at 2^-133, so smaller ones lose low bits).  The planes of a finite
+// value are finite; an infinite one has a NaN among them.
 #include "experts.cuh"
 #include "tc.cuh"
 
@@ -342,7 +343,9 @@ __device__ __forceinline__ uint4 load8_raw(const T* row, int c, int d, bool vec,
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Writes 8 columns as one vector of each of NP bf16 planes
+// Writes 8 columns as one vector of each of NP bf16 planes.  The first plane of a finite value is finite: above the largest
+// bf16 (3.3895e38) rounding to nearest would give infinity, so it is that one, and the next plane has the rest.
+constexpr float BF16_MAX = 3.38953138925153547590470800371487867e+38f;   // (2 - 2^-7) 2^127
 template <int NP>
 __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64_t at, const float (&f)[8]) {
   float r[8];
@@ -350,7 +353,10 @@ __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64
   for (int q = 0; q < 8; ++q) r[q] = f[q];
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
-    const uint4 u = pack16<bf16>(r);
+    float c[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) c[q] = p == 0 ? fminf(fmaxf(r[q], -BF16_MAX), BF16_MAX) : r[q];
+    const uint4 u = pack16<bf16>(c);
     *reinterpret_cast<uint4*>(dst + p * plane + at) = u;
     float h[8];
     unpack16(u, h, bf16());
