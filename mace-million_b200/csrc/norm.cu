@@ -42,21 +42,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int W = G < 32 ? 1 : G / 32;
   float s = 0.f;
-  if constexpr (K == 8) {
-    // transposed: after three halving steps lane L holds a partial sum of value L >> 2 (9 shuffles instead of 40)
-#pragma unroll
-    for (int h = 4, bit = 16; h >= 1; h >>= 1, bit >>= 1) {
-      const bool up = lane & bit;
-#pragma unroll
-      for (int q = 0; q < h; ++q) {
-        const float send = up ? v[q] : v[q + h];
-        const float keep = up ? v[q + h] : v[q];
-        v[q] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
-      }
-    }
-    s = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 2);
-    s += __shfl_xor_sync(0xffffffffu, s, 1);
-  } else if constexpr (K == 4) {                  // likewise: lane L holds value L >> 3 (6 shuffles instead of 20)
+  if constexpr (K == 4) {                         // transposed: lane L ends with value L >> 3 (6 shuffles instead of 20)
 #pragma unroll
     for (int h = 2, bit = 16; h >= 1; h >>= 1, bit >>= 1) {
       const bool up = lane & bit;
@@ -72,7 +58,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
     for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
   if constexpr (G <= 32) {
-    if constexpr (K == 8 || K == 4) {
+    if constexpr (K == 4) {
 #pragma unroll
       for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, 32 / K * k);
     } else {
@@ -82,7 +68,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* red) {
         for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
   } else {
-    if constexpr (K == 8 || K == 4) {
+    if constexpr (K == 4) {
       if (lane % (32 / K) == 0) red[warp * K + lane / (32 / K)] = s;
     } else {
 #pragma unroll
@@ -266,8 +252,8 @@ __global__ void __launch_bounds__(1024) k_ln_fwd_wide(const LnArgs a) {
 }
 
 // partial[block][0 .. d) = sum of dy xh, [d .. 2 d) = sum of dy over the block's rows.  RB rows at a time with one
-// synchronisation, and the next RB rows' loads in flight meanwhile (PRE).
-template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
+// synchronisation, and the next RB rows' loads in flight meanwhile.
+template <typename T, typename P, int G, int NV, int V, int RB>
 __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G, NV, V>) k_ln_bwd(const LnArgs a) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
   __shared__ float red[2][TH / 32 * 2 * RB];
@@ -314,9 +300,8 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G, NV, V>) k_ln_b
   };
   int buf = 0;
   const int64_t step = (int64_t)gridDim.x * RPB * RB;
-  if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB * RB);
+  fetch((int64_t)blockIdx.x * RPB * RB);
   for (int64_t r0 = (int64_t)blockIdx.x * RPB * RB; r0 < a.n; r0 += step, buf ^= 1) {
-    if constexpr (!PRE) fetch(r0);
     // xh and up = dy w stay in registers between the sums and dx
     E xh[RB][NV][NE], up[RB][NV][NE];
     float rc[RB], s[2 * RB];
@@ -355,8 +340,7 @@ __global__ void __launch_bounds__(ln_threads<G>, ln_bwd_blocks<G, NV, V>) k_ln_b
       s[2 * k] = e_sum(p1);
       s[2 * k + 1] = e_sum(p2);
     }
-    if constexpr (PRE)
-      if (r0 + step < a.n) fetch(r0 + step);
+    if (r0 + step < a.n) fetch(r0 + step);
     group_sum<G, 2 * RB>(s, red[buf]);
     if (a.dx) {
 #pragma unroll
@@ -524,14 +508,14 @@ static int ln_fwd_any(const LnArgs& a, bool vec, cudaStream_t st) {
 }
 
 // Launches and says how many rows of partial sums there are
-template <typename T, typename P, int G, int NV, int V, int RB, bool PRE>
+template <typename T, typename P, int G, int NV, int V, int RB>
 static int ln_bwd_launch(const LnArgs& a, int* nb, cudaStream_t st) {
   constexpr int TH = ln_threads<G>, RPB = TH / G;
   const int64_t want = (a.n + RPB * RB - 1) / (RPB * RB), most = (int64_t)ln_bwd_blocks<G, NV, V> * sm_count();
   *nb = (int)(want < most ? want : most);
   const int smem = RPB > 1 && a.partial ? RPB * 2 * a.d * 4 : 0;
   static_assert(RPB == 1 || RPB * 2 * G * NV * V * 4 <= 40 * 1024, "column sums in shared memory");
-  k_ln_bwd<T, P, G, NV, V, RB, PRE><<<*nb, TH, smem, st>>>(a);
+  k_ln_bwd<T, P, G, NV, V, RB><<<*nb, TH, smem, st>>>(a);
   return check_launch("layer_norm_bwd");
 }
 
@@ -540,21 +524,21 @@ static int ln_bwd_any(const LnArgs& a, bool vec, int* nb, cudaStream_t st) {
   constexpr int V = kVec<T>;
   if (vec) {
     const int c = a.d / V;
-    if (c <= 8) return ln_bwd_launch<T, P, 8, 1, V, 2, true>(a, nb, st);
-    if (c <= 16) return ln_bwd_launch<T, P, 16, 1, V, 2, true>(a, nb, st);
-    if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 2, true>(a, nb, st);
-    if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 2, true>(a, nb, st);
-    if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 2, true>(a, nb, st);
-    if (c <= 256) return ln_bwd_launch<T, P, 256, 1, V, 2, true>(a, nb, st);
-    if (c <= 512) return ln_bwd_launch<T, P, 512, 1, V, 2, true>(a, nb, st);
-    if (c <= 1024) return ln_bwd_launch<T, P, 512, 2, V, 1, true>(a, nb, st);
+    if (c <= 8) return ln_bwd_launch<T, P, 8, 1, V, 2>(a, nb, st);
+    if (c <= 16) return ln_bwd_launch<T, P, 16, 1, V, 2>(a, nb, st);
+    if (c <= 32) return ln_bwd_launch<T, P, 32, 1, V, 2>(a, nb, st);
+    if (c <= 64) return ln_bwd_launch<T, P, 64, 1, V, 2>(a, nb, st);
+    if (c <= 128) return ln_bwd_launch<T, P, 128, 1, V, 2>(a, nb, st);
+    if (c <= 256) return ln_bwd_launch<T, P, 256, 1, V, 2>(a, nb, st);
+    if (c <= 512) return ln_bwd_launch<T, P, 512, 1, V, 2>(a, nb, st);
+    if (c <= 1024) return ln_bwd_launch<T, P, 512, 2, V, 1>(a, nb, st);
   } else {
-    if (a.d <= 128) return ln_bwd_launch<T, P, 32, 4, 1, 2, true>(a, nb, st);
-    if (a.d <= 256) return ln_bwd_launch<T, P, 64, 4, 1, 2, true>(a, nb, st);
-    if (a.d <= 640) return ln_bwd_launch<T, P, 128, 5, 1, 2, true>(a, nb, st);
-    if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 2, true>(a, nb, st);
-    if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 2, true>(a, nb, st);
-    if (a.d <= 4096) return ln_bwd_launch<T, P, 512, 8, 1, 1, true>(a, nb, st);
+    if (a.d <= 128) return ln_bwd_launch<T, P, 32, 4, 1, 2>(a, nb, st);
+    if (a.d <= 256) return ln_bwd_launch<T, P, 64, 4, 1, 2>(a, nb, st);
+    if (a.d <= 640) return ln_bwd_launch<T, P, 128, 5, 1, 2>(a, nb, st);
+    if (a.d <= 1024) return ln_bwd_launch<T, P, 256, 4, 1, 2>(a, nb, st);
+    if (a.d <= 2048) return ln_bwd_launch<T, P, 512, 4, 1, 2>(a, nb, st);
+    if (a.d <= 4096) return ln_bwd_launch<T, P, 512, 8, 1, 1>(a, nb, st);
   }
   const int64_t most = (int64_t)2 * sm_count();
   *nb = (int)(a.n < 64 ? a.n : 64);
