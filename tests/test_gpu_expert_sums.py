@@ -34,7 +34,8 @@ def _one_rounding(got, exact, slack=1.05):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("T,k,E,D,O", [(700, 2, 5, 192, 136), (1500, 4, 6, 256, 264), (333, 3, 4, 72, 515), (901, 8, 9, 130, 77)])
+@pytest.mark.parametrize("T,k,E,D,O", [(700, 2, 5, 192, 136), (1500, 4, 6, 256, 264), (333, 3, 4, 72, 515), (901, 8, 9, 130, 77),
+                                         (20_000, 2, 6, 192, 600)])
 @pytest.mark.parametrize("weighted", [False, True])
 def test_sums_over_choices_are_rounded_once(T, k, E, D, O, dt, weighted):
     g = torch.Generator(device="cuda").manual_seed(T)
