@@ -14,9 +14,9 @@
 // The tensor cores truncate when they add to an fp32 accumulator.  Sums of one sign lose 1e-7 of themselves for each 16-wide
 // step (measured: 2.5e-3 after 25,000 steps), products of either sign less (a deviation of 3.2e-6 after 192 steps, 4.7e-7
 // after 32).  Where the result leaves in fp32 (fp32 data, and the gradient of the routing weights) an accumulator therefore
-// takes a few K blocks at most, and the chunks are added in registers with rounding to nearest.  16-bit results take up to
-// XG_ACC_LONG K blocks in one accumulator: 4e-5, a fifth of the deviation of an fp16 rounding.  Longer sums are cut: WGRAD
-// into parts that are added in fp32 afterwards, FWD and DGRAD into chunks in registers.
+// takes a few K blocks at most, and the chunks are added in registers with rounding to nearest (7e-7 for sums of one sign).
+// 16-bit results take up to xg_acc_long K blocks in one accumulator.  Longer sums are cut: WGRAD into parts that are added in
+// fp32 afterwards, FWD and DGRAD into chunks in registers.
 //
 // Persistent CTAs, one per SM.  Warp 0 loads tiles with TMA (SWIZZLE_128B) into a ring of stages, warp 1 issues the MMAs
 // into one of two TMEM accumulators, warps 4-11 drain the other one (a lane holds half a row).  CG = 2: a cluster of two
@@ -57,7 +57,9 @@ constexpr int XG_STG = 2048;                     // row staging of one epilogue 
 // at most (its drains cost nothing then).  Gradients of the weights from 16-bit data, 2,048 columns: error 7e-7 at 12,
 // 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: backward 2251 us at 12, 2331 at 8.
 constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12, XG_ACC_K1 = 4;
-constexpr int XG_ACC_LONG = 96;                  // and of one whose result leaves in 16 bits
+// and of one whose result leaves in 16 bits: sums of one sign lose 5.2e-5 over 8,192 terms of fp16 (rounding: 2.1e-4), 1e-4 over
+// 16,384 of bf16 (rounding: 1.6e-3)
+__host__ __device__ constexpr int xg_acc_long(int dtype) { return dtype == MB_F16 ? 128 : 256; }
 
 // T: element type; BN: most columns of a tile that a CTA (of CG) holds operands and accumulators for; SPL: XGemm::split
 template <typename T, int BN, int CG, bool SPL>
@@ -233,7 +235,7 @@ __device__ __forceinline__ float xg_dot(const float* v, const XgLane& a, const u
   return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// DOT: DGRAD with dgpart; LONG: FWD or DGRAD of 16-bit data with K of more than XG_ACC_LONG blocks
+// DOT: DGRAD with dgpart; LONG: FWD or DGRAD of 16-bit data with K of more than xg_acc_long blocks
 template <int MODE, typename T, int BN, int CG, bool DOT, bool SPL, bool LONG>
 __global__ void __launch_bounds__(XG_THREADS, 1)
     k_expert_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XgParams g) {
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
     }
     o.ck = o.nk;                                 // K blocks of one accumulator: even chunks
     if constexpr (CHUNKS) {
-      const int most = LONG ? XG_ACC_LONG : rounds == 1 ? XG_ACC_K1 : sizeof(T) == 4 ? XG_ACC_K : XG_ACC_K16;
+      constexpr int LONGEST = xg_acc_long(std::is_same<T, f16>::value ? MB_F16 : MB_BF16);
+      const int most = LONG ? LONGEST : rounds == 1 ? XG_ACC_K1 : C::F32 ? XG_ACC_K : XG_ACC_K16;
       const int n = (o.nk + most - 1) / most;
       if (n > 1) o.ck = (o.nk + n - 1) / n;
     }
@@ -698,7 +701,7 @@ int xgemm_n_tiles(int64_t N, int dtype) {
 int xgemm_kc(int64_t E, int64_t M, int64_t N, int64_t slots, int dtype) {
   const int64_t per = ((M + XG_BM - 1) / XG_BM) * xgemm_n_tiles(N, dtype), want = 4 * (int64_t)sm_count();
   const int64_t blocks = slots / XG_BK;          // K blocks of all experts
-  const int64_t most = dtype == MB_F32 ? 0x3fffffff : XG_ACC_LONG;
+  const int64_t most = dtype == MB_F32 ? 0x3fffffff : xg_acc_long(dtype);
   if (E * per >= want) return (int)most;
   const int64_t kc = blocks * per / want, least = dtype == MB_F32 ? 4 : 8;
   return (int)(kc < least ? least : kc < most ? kc : most);
@@ -804,7 +807,7 @@ static bool xg_pairs(const XGemm& x) {
 template <int MODE, typename T, bool DOT, bool SPL>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
   if constexpr (sizeof(T) == 2 && MODE != XG_WGRAD && !DOT)
-    if (x.K > XG_ACC_LONG * XG_BK) return xg_go<MODE, T, 128, 1, DOT, SPL, true>(x, st);
+    if (x.K > xg_acc_long(x.dtype) * XG_BK) return xg_go<MODE, T, 128, 1, DOT, SPL, true>(x, st);
   if constexpr (sizeof(T) == 2)
     if (xg_bn_max(x.N, x.dtype) == 256)
       return xg_pairs(x) ? xg_go<MODE, T, 256, 2, DOT, SPL, false>(x, st) : xg_go<MODE, T, 256, 1, DOT, SPL, false>(x, st);
