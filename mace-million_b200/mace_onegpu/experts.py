@@ -102,7 +102,7 @@ class ExpertPlan:
             raise ValueError("n_experts must be positive")
         if n == 1:
             experts = experts[:, None]
-        self._version = None                        # of indices that are the caller's
+        mine = True                                 # a copy of the caller's indices
         if experts.dtype != torch.int32:
             # 64-bit indices outside the range of int32 must not wrap into it: -2 is refused by check(), like any other
             experts = torch.where((experts >= -1) & (experts < self.n_experts), experts, -2).to(torch.int32).contiguous()
@@ -111,10 +111,21 @@ class ExpertPlan:
         elif experts.is_inference():                # has no version
             experts = experts.clone()
         else:
-            self._version = experts._version
+            mine = False
         self.experts = experts
-        self._stream, self._capture = _place(experts.device)
+        self._start(None if mine else experts._version)
+
+    def _start(self, version):
+        self._version = version
+        self._stream, self._capture = _place(self.experts.device)
         self._sorted = None                         # (words, stream, capture, event)
+
+    def __getstate__(self):                         # copies and saved plans sort for themselves
+        return {"experts": self.experts, "n_experts": self.n_experts}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._start(None if self.experts.is_inference() else self.experts._version)
 
     def here(self):
         """The current stream and capture.  Keeps the plan's indices alive for that stream, and checks that they are the ones

@@ -169,3 +169,26 @@ def test_the_capture_number():
             assert N.lib().mace_b200_capture_id(torch.cuda.default_stream().cuda_stream) == 0
     assert seen[0] != 0 and seen[1] != 0 and seen[0] != seen[1]
     assert N.lib().mace_b200_capture_id(s.cuda_stream) == 0
+
+
+def test_a_plan_and_a_block_can_be_copied_and_saved(form, tmp_path):
+    """After calls, too (a block keeps its last plan): the copy sorts for itself."""
+    import copy
+    import pickle
+
+    x, w, ex = _case(10)
+    want = _want(x, w, ex)
+    plan = X.plan_experts(ex, E)
+    X.expert_linear(x, w, plan)
+    for other in (copy.deepcopy(plan), copy.copy(plan), pickle.loads(pickle.dumps(plan))):
+        _close(X.expert_linear(x, w, other), want)
+        other.check()
+    ex.fill_(0)
+    with pytest.raises(RuntimeError, match="changed in place"):
+        X.expert_linear(x, w, plan)
+    block = X.ExpertBlock(D, 32, 8, E, K)
+    y = block(x)
+    torch.save(block, tmp_path / "block.pt")
+    for other in (copy.deepcopy(block), torch.load(tmp_path / "block.pt", weights_only=False)):
+        assert torch.equal(other(x), y)
+        assert torch.equal(other.balance(), block.balance(0.0))
