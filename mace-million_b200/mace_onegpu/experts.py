@@ -61,12 +61,15 @@ def route(logits, k, *, bias=None, score="softmax", groups=1, top_groups=1, reno
                         float(scale))
 
 
-def _place(device):
-    """The current stream (its handle) and the number of the CUDA graph capture it is in (0: none)."""
-    if device.type != "cuda" or not torch.cuda.is_initialized():
-        return 0, 0
-    stream = torch._C._cuda_getCurrentRawStream(device.index)   # a Stream object would cost a small call 2 us
-    return stream, N.lib().mace_b200_capture_id(stream)
+def _stream(index):
+    """Handle of the current stream of CUDA device `index` (a Stream object would cost a small call 2 us); 0 elsewhere."""
+    return torch._C._cuda_getCurrentRawStream(index) if index >= 0 and torch.cuda.is_initialized() else 0
+
+
+def _place(index):
+    """The current stream and the number of the CUDA graph capture it is in (0: none)."""
+    stream = _stream(index)
+    return stream, N.lib().mace_b200_capture_id(stream) if index >= 0 and torch.cuda.is_initialized() else 0
 
 
 def _ready(device):
@@ -117,7 +120,8 @@ class ExpertPlan:
 
     def _start(self, version):
         self._version = version
-        self._stream, self._capture = _place(self.experts.device)
+        self._index = self.experts.get_device()
+        self._stream, self._capture = _place(self._index)
         self._sorted = None                         # (words, stream, capture, event)
 
     def __getstate__(self):                         # copies and saved plans sort for themselves
@@ -127,20 +131,18 @@ class ExpertPlan:
         self.__dict__.update(state)
         self._start(None if self.experts.is_inference() else self.experts._version)
 
-    def here(self):
-        """The current stream and capture.  Keeps the plan's indices alive for that stream, and checks that they are the ones
-        that the plan was made of."""
-        at = _place(self.experts.device)
-        if at[0] != self._stream:
-            _after(self.experts.device, None, self.experts)
+    def use(self, stream):
+        """Checks that the indices are the ones that the plan was made of, and keeps them alive for that stream."""
         if self._version is not None and self.experts._version != self._version:
             raise RuntimeError("the indices of this plan were changed in place after plan_experts: make a new plan")
-        return at
+        if stream != self._stream:
+            _after(self.experts.device, None, self.experts)
 
     @property
     def words(self):
         """The plan as the kernels read it (int32), for the current stream."""
-        stream, capture = self.here()
+        stream, capture = _place(self._index)
+        self.use(stream)
         s = self._sorted
         # tables of another capture hold nothing before its first replay; eager ones may be freed while a graph uses them;
         # and the indices of a plan that was made in a capture are written anew by every replay
@@ -181,7 +183,7 @@ def expert_linear(x, w, plan, weights=None):
     if few and torch.is_grad_enabled():
         few = not (x.requires_grad or w.requires_grad or (weights is not None and weights.requires_grad))
     if few:
-        plan.here()
+        plan.use(_stream(plan._index))
     return _op("expert_linear")(x, w, plan.experts, None if few else plan.words, weights)
 
 

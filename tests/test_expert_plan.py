@@ -12,7 +12,7 @@ class Place:
     def __init__(self, monkeypatch):
         self.stream, self.capture, self.sorts, self.waits = 1, 0, [], []
         monkeypatch.setattr(X, "_op", lambda name: self.sort)
-        monkeypatch.setattr(X, "_place", lambda device: (self.stream, self.capture), raising=False)
+        monkeypatch.setattr(X, "_place", lambda index: (self.stream, self.capture), raising=False)
         monkeypatch.setattr(X, "_ready", lambda device: ("event", self.stream), raising=False)
         monkeypatch.setattr(X, "_after", lambda device, event, *tensors: self.waits.append((event, self.stream)), raising=False)
 
