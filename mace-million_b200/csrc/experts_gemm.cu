@@ -6,7 +6,7 @@
 // and no matrix is transposed in memory: the MN-major operands are read as they lie.
 // fp32 data comes as three bf16 planes; a stage holds all three of both operands.  The product of the first planes has an
 // accumulator of its own, and the five others whose ranks add up to at most 2 share another; the rest is below 2^-24 of
-// the result.
+// the sum of the absolute products.
 // WGRAD with routing weights multiplies rows by fp32 weights of any size: x g comes as two bf16 planes (2^-17 of it, and the
 // exponents of fp32), and fp16 dy as two, which hold it exactly.  The product of the second planes is left out (2^-18).
 // One plane in the type itself was 1.4 times as far off as one rounding, and left the range of fp16 (x g above 65,504,
@@ -30,10 +30,12 @@
 // result for with NaN, drains its copies and MMAs, frees its TMEM and returns.
 //
 // What bounds it (B200; copy 6.5 TB/s, cuBLAS bf16 1.64 PFLOP/s in a burst and 1.37 sustained): 262,144 slots on 64 experts,
-// 1024 -> 2048 bf16, pairs: forward 833 us, dx alone about 780, dx with the gradient of the weights 942, dW 815 (1.32, 1.4,
-// 1.17, 1.35 PFLOP/s): the operands' way from L2 into shared memory (11 TB/s).  48,000 slots on 16 experts, 512 -> 515
-// fp16: 37 / 54 / 47 us: 8 or 9 K blocks a tile, and the drain of a tile takes about as long.  16,384 slots on 89 experts,
-// 128 -> 512 fp32: 24 / 32 / 28 us: two or three rounds of short tiles and the latency of their first loads.
+// 1024 -> 2048 bf16, pairs: forward 833 us, dx alone about 780, dW without weights 815 (1.32, 1.4, 1.35 PFLOP/s): the
+// operands' way from L2 into shared memory (11 TB/s).  With rows that leave in fp32 (k > 1): forward 951, dx with the gradient of
+// the weights 1044: their bytes.  dW with weights 1436 (1.53 PFLOP/s of its two products): the MMAs.  48,000 slots on 16
+// experts, 512 -> 515 fp16, k = 2: 41 / 66 / 88 us: 8 or 9 K blocks a tile, and the drain of a tile takes about as long.
+// 16,384 slots on 89 experts, 128 -> 512 fp32: 25 / 34 / 30 us: two or three rounds of short tiles and the latency of their first
+// loads.
 #include <cuda.h>
 
 #include <type_traits>
@@ -54,8 +56,8 @@ __device__ unsigned long long g_xg_wait_ns = 2000000000ull;
 __device__ int g_xg_skip_load = 0;
 constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
 // Most K blocks of an accumulator whose result leaves in fp32: of fp32 data, of 16-bit data, and where each CTA has one tile
-// at most (its drains cost nothing then).  Gradients of the weights from 16-bit data, 2,048 columns: error 7e-7 at 12,
-// 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: backward 2251 us at 12, 2331 at 8.
+// at most (its drains cost nothing then).  Gradients of the routing weights from 16-bit data, 2,048 columns: error 7e-7 at
+// 12, 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: dx with them 80 us longer at 8.
 constexpr int XG_ACC_K = 8, XG_ACC_K16 = 12, XG_ACC_K1 = 4;
 // and of one whose result leaves in 16 bits: sums of one sign lose 5.2e-5 over 8,192 terms of fp16 (rounding: 2.1e-4), 1e-4 over
 // 16,384 of bf16 (rounding: 1.6e-3)
@@ -793,9 +795,10 @@ static int xg_go(const XGemm& x, cudaStream_t st) {
 }
 
 // Pairs of CTAs pay with long K loops, full 256-row tiles and several rounds of them.  B200, one CTA / pairs: forward
-// 262,144 slots on 64 experts, 1024 -> 2048 853 / 821 us, its dx 878 / 766, its dW 950 / 842; 48,000 slots on 16 experts,
-// 512 -> 515 (8 K blocks; 5 or 3 row tiles of dW) forward 36 / 43 us, dW 49 / 55; 65,536 slots on 128 experts, 512 -> 256
-// (two tiles an expert) forward and sum 60 / 69 us.
+// 262,144 slots on 64 experts, 1024 -> 2048 853 / 821 us, its dx 878 / 766, its dW 950 / 842, with its row moves and weights
+// 2335 / 1974 (bf16) and 3138 / 2884 (fp16); 48,000 slots on 40 experts, 1024 -> 1024, dW with weights 303 / 247, but dx with
+// their gradient 154 / 173; 48,000 slots on 16 experts, 512 -> 515 (8 K blocks; 5 or 3 row tiles of dW) forward 36 / 43 us, dW
+// 49 / 55; 65,536 slots on 128 experts, 512 -> 256 (two tiles an expert) forward and sum 60 / 69 us.
 static bool xg_pairs(const XGemm& x) {
   const int64_t rows = x.lay.R / x.E, tn = xgemm_n_tiles(x.N, x.dtype);
   const int64_t blocks = x.mode == XG_WGRAD ? rows / XG_BK : x.K / XG_BK;
@@ -806,6 +809,8 @@ static bool xg_pairs(const XGemm& x) {
 
 template <int MODE, typename T, bool DOT, bool SPL>
 static int xg_bn_any(const XGemm& x, cudaStream_t st) {
+  // for accuracy: the sum over the chunks takes registers that 256 columns do not leave (20,000 rows to 1024 columns, bf16
+  // 16,384 wide 746 us, 16,448 wide 916)
   if constexpr (sizeof(T) == 2 && MODE != XG_WGRAD && !DOT)
     if (x.K > xg_acc_long(x.dtype) * XG_BK) return xg_go<MODE, T, 128, 1, DOT, SPL, true>(x, st);
   if constexpr (sizeof(T) == 2)
