@@ -347,7 +347,6 @@ int mace_b200_sender_range(const int32_t* pair_j, int64_t e0, int64_t e1, int32_
  * mean / rstd [n] are written when not null (both or none); the backward pass reads them.
  * bwd: dx (may be null) dense [n][d]; dw / db [d] of type ptype (may be null), summed over the rows in a fixed order
  * through `workspace` (mace_b200_layer_norm_bwd_workspace floats; unused when both are null). */
-#define MB_NORM_MAX_WIDTH (1 << 30)
 int mace_b200_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean,
                              float* rstd, int64_t n, int32_t d, double eps, int32_t dtype, int32_t ptype, void* stream);
 int mace_b200_layer_norm_bwd_workspace(int64_t n, int32_t d, int64_t* floats);

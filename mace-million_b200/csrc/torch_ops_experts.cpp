@@ -65,7 +65,7 @@ LnIn ln_in(const Tensor& x, const Tensor& w, const Tensor& b) {
   LnIn a;
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last dimension of at least 1 (got ", x.sizes(), ")");
-  TORCH_CHECK(x.size(-1) <= MB_NORM_MAX_WIDTH, "x: last dimension too large (at most 2^30)");
+  TORCH_CHECK(x.size(-1) <= INT32_MAX, "x: last dimension too large");
   a.dt = a.pt = type_code(x, "x");
   a.d = x.size(-1);
   a.n = x.numel() / a.d;
