@@ -172,8 +172,9 @@ def expert_linear(x, w, plan, weights=None):
     """Products with the matrices w [E, O, D] that the plan assigns.
 
     x: [T, D], or [T, k, D] with a row per slot.  weights [T, k] float32: out [T, O] = sum_j weights[t, j] w[e_tj] x;
-    None: out [T, k, O] = w[e_tj] x.  x and w: float32 (at fp32 accuracy; infinities come out as NaN), bfloat16 or float16.  Slots with expert -1
-    give zeros and no gradient.  Differentiable w.r.t. x, w and weights; sums run in a fixed order."""
+    None: out [T, k, O] = w[e_tj] x.  x and w: float32 (at fp32 accuracy; infinities come out as NaN), bfloat16 or float16
+    (results rounded once).  Slots with expert -1 give zeros and no gradient.  Differentiable w.r.t. x, w and weights; sums
+    run in a fixed order."""
     if not isinstance(plan, ExpertPlan):
         raise TypeError("plan must be an ExpertPlan (plan_experts(experts, n_experts))")
     if w.dim() != 3 or w.shape[0] != plan.n_experts:
