@@ -381,7 +381,7 @@ int mace_b200_route_bwd(const float* dweights, const void* logits, int64_t ldl, 
  * most MB_FEW_MAX_SLOTS slots; an index outside [0, E) counts as -1).
  * 16-bit results are rounded once, from fp32 sums; a tile whose bounded wait expired is NaN (MB_ST_TC_TIMEOUT).
  * bwd: dy as out; dx as x but dense, dw [E][O][D], dweights [tokens][k]; any may be null (dweights needs weights).
- * fp32 data: an infinite value gives NaN in the results it enters; so may infinite x (fp16: and dy) in a weighted dw.
+ * fp32 data: an infinite value gives NaN in the results it enters.
  * expert_test_hooks: as mace_b200_tc_test_hooks, for the products (skip_one_load: the first load goes missing once). */
 #define MB_PLAN_MAX_EXPERTS 1024
 #define MB_FEW_MAX_SLOTS 4096

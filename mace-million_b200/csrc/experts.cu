@@ -345,20 +345,29 @@ __device__ __forceinline__ uint4 load8_raw(const T* row, int c, int d, bool vec,
 
 // Writes 8 columns as one vector of each of NP bf16 planes.  The first plane of a finite value is finite: above the largest
 // bf16 (3.3895e38) rounding to nearest would give infinity, so it is that one, and the next plane has the rest.
+// CUT: the first of two planes is cut off instead of rounded, and the second is never zero beside it (2^-24 of it where
+// nothing is left): both have the sign of the value, so an infinite bf16 dy times both is that infinity.  (fp16 dy has planes
+// of its own, the first one finite; rounded planes of either sign lose less in long accumulators.)
 constexpr float BF16_MAX = 3.38953138925153547590470800371487867e+38f;   // (2 - 2^-7) 2^127
-template <int NP>
+template <int NP, bool CUT>
 __device__ __forceinline__ void store_planes(uint16_t* dst, int64_t plane, int64_t at, const float (&f)[8]) {
-  float r[8];
+  float r[8], h[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) r[q] = f[q];
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
-    float c[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) c[q] = p == 0 ? fminf(fmaxf(r[q], -BF16_MAX), BF16_MAX) : r[q];
-    const uint4 u = pack16<bf16>(c);
+    for (int q = 0; q < 8; ++q) {
+      if (p == 0) {
+        h[q] = fminf(fmaxf(r[q], -BF16_MAX), BF16_MAX);
+        if (CUT) h[q] = __uint_as_float(__float_as_uint(h[q]) & 0xFFFF0000u);
+      } else {
+        h[q] = CUT && r[q] == 0.f ? h[q] * 0x1p-24f : r[q];
+      }
+    }
+    const uint4 u = pack16<bf16>(h);
     *reinterpret_cast<uint4*>(dst + p * plane + at) = u;
-    float h[8];
+    if (p + 1 == NP) break;
     unpack16(u, h, bf16());
 #pragma unroll
     for (int q = 0; q < 8; ++q) r[q] -= h[q];
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
           const int64_t to = scatter ? slot_row[row * copies + j] : row;
           if (to < 0) continue;
           uint16_t* o = out + to * m.dp + c0;
-          if (m.planes == 2) {
+          if (m.planes == 2) {                     // x with its weight; dy (fp16), exact in two rounded planes
             const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
                 unpack16(u[i], f, T());
 #pragma unroll
                 for (int x = 0; x < 8; ++x) f[x] *= g;
-                store_planes<2>(o, m.plane, i * 8 * lpr, f);
+                store_planes<2, std::is_same<T, bf16>::value>(o, m.plane, i * 8 * lpr, f);
               }
           } else {
 #pragma unroll
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(256, 4) k_rows_move(const XMoves mv, const int
           const float g = m.scale ? m.scale[row * copies + j] : 1.f;
 #pragma unroll
           for (int x = 0; x < 8; ++x) v[x] = f[x] * g;
-          store_planes<3>(out, m.plane, to * m.dp + c, v);
+          store_planes<3, false>(out, m.plane, to * m.dp + c, v);
         }
       }
     }

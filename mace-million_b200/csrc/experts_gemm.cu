@@ -7,7 +7,7 @@
 // fp32 data comes as three bf16 planes; a stage holds all three of both operands.  The product of the first planes has an
 // accumulator of its own, and the five others whose ranks add up to at most 2 share another; the rest is below 2^-24 of
 // the sum of the absolute products.
-// WGRAD with routing weights multiplies rows by fp32 weights of any size: x g comes as two bf16 planes (2^-17 of it, and the
+// WGRAD with routing weights multiplies rows by fp32 weights of any size: x g comes as two bf16 planes (2^-16 of it, and the
 // exponents of fp32), and fp16 dy as two, which hold it exactly.  The product of the second planes is left out (2^-18).
 // One plane in the type itself was 1.4 times as far off as one rounding, and left the range of fp16 (x g above 65,504,
 // or below 6e-5) where the gradient does not.

@@ -123,3 +123,23 @@ def test_very_wide_rows_do_not_shrink(dt):
     for got in (fwd, dx):
         mean = float(((got.double() - want) / want).mean())
         assert abs(mean) <= 5.3e-5 + 4 * u / (3 * T * n) ** 0.5, mean
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_infinities_in_a_weighted_gradient(dt):
+    """An infinite x or dy gives what its products add up to: infinities of their sign, NaN where they meet zero or each other;
+    the rest is untouched."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    T, k, E, D, O = 200, 2, 3, 64, 72
+    x = torch.randn(T, D, device="cuda", generator=g).to(dt)
+    dy = torch.randn(T, O, device="cuda", generator=g).to(dt)
+    x[3, 5], x[9, 6], dy[20, 7], dy[3, 11] = float("inf"), -float("inf"), -float("inf"), 0.0
+    ex = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    p = torch.rand(T, k, device="cuda", generator=g) + 0.1
+    got = _grad(x, torch.zeros(E, O, D, device="cuda", dtype=dt), ex, p, dy)
+    want = _exact_dw(x, ex, p, dy, E)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)].double(), want[torch.isinf(want)]) and torch.isinf(want).any()
+    fine = torch.isfinite(want)
+    assert fine.double().mean() > 0.9
+    _one_rounding(got[fine], want[fine])
