@@ -20,7 +20,8 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-li
          "-Xcompiler", "-O3", "--expt-relaxed-constexpr", f"-I{INC}"]
 
 
-OPS_SRC = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_ops_experts.cpp")]
+OPS_SRC = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_ops_experts.cpp", "torch_ops_readout.cpp")]
+OPS_HDR = os.path.join(CSRC, "torch_ops_util.h")
 OPS_OUT = os.path.join(HERE, "mace_onegpu", "_lib", "libmace_b200_torch.so")
 
 
@@ -71,7 +72,7 @@ def build_ops(force: bool = False, verbose: bool = False) -> str:
     torch's headers and linked to libmace_b200.so (loaded with torch.ops.load_library)."""
     lib = build(force, verbose)
     if not force and os.path.exists(OPS_OUT) and all(os.path.getmtime(p) <= os.path.getmtime(OPS_OUT)
-                                                     for p in (*OPS_SRC, lib, os.path.join(INC, "mace_b200.h"))):
+                                                     for p in (*OPS_SRC, OPS_HDR, lib, os.path.join(INC, "mace_b200.h"))):
         return OPS_OUT
     import torch
 

@@ -16,7 +16,7 @@
 // 24,001 x 515 bf16 (one element per access) 20 / 26 us, 100,000 x 64 fp16 (8 threads a row) 6.0 / 10.8 us, with a whole
 // warp a row 18 / 26.  Below 5 TB/s the issue slots bound it: unpacking, the packed arithmetic and packing are about 10
 // instructions an element backward.
-#include "dtypes.cuh"
+#include "norm.cuh"
 
 namespace mb {
 
@@ -554,6 +554,17 @@ static int ln_bwd_any(const LnArgs& a, bool vec, int* nb, cudaStream_t st) {
   return 0;
 }
 
+int col_sums(const float* partial, int nb, int32_t d, void* dw, void* db, int ptype, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((2 * (int64_t)d + 31) / 32);
+  if (ptype == MB_F32)
+    k_ln_reduce<float><<<blocks, 1024, 0, st>>>(partial, nb, d, (float*)dw, (float*)db);
+  else if (ptype == MB_BF16)
+    k_ln_reduce<bf16><<<blocks, 1024, 0, st>>>(partial, nb, d, (bf16*)dw, (bf16*)db);
+  else
+    k_ln_reduce<f16><<<blocks, 1024, 0, st>>>(partial, nb, d, (f16*)dw, (f16*)db);
+  return check_launch("norm parameter gradients");
+}
+
 template <typename F>
 static int ln_types(int dtype, int ptype, const F& f) {
   if (dtype == MB_F32) return f(float(), float());
@@ -638,8 +649,6 @@ extern "C" int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void
     if (n > 0)
       if (int rc = ln_bwd_any<T, P>(a, vec, &nb, (cudaStream_t)stream)) return rc;
     if (!dw && !db) return 0;
-    k_ln_reduce<P><<<(unsigned)((2 * (int64_t)d + 31) / 32), 1024, 0, (cudaStream_t)stream>>>(workspace, nb, d, (P*)dw,
-                                                                                             (P*)db);
-    return check_launch("layer_norm_bwd");
+    return col_sums(workspace, nb, d, dw, db, ptype, (cudaStream_t)stream);
   });
 }

@@ -1,0 +1,163 @@
+// torch.ops.mace_b200.*: group norm with an activation over the C ABI (include/mace_b200.h), with its autograd formula.  As in
+// torch_ops.cpp, the ops check devices, types and shapes with TORCH_CHECK, launch on torch's current CUDA stream and
+// allocate outputs and workspaces with torch's caching allocator.
+#include "torch_ops_util.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ group norm
+struct GnIn {
+  Tensor rows, w, b, off;
+  int32_t dt, pt, off64 = 0;
+  int64_t n, len, r, c;
+};
+
+GnIn gn_in(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, const Tensor& offsets, int64_t act) {
+  GnIn a;
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  a.dt = a.pt = type_code(x, "x");
+  TORCH_CHECK(x.dim() >= 2 && x.size(-1) >= 1, "x must be [samples, .., channels] (got ", x.sizes(), ")");
+  TORCH_CHECK(x.size(-1) <= INT32_MAX, "x: too many channels");
+  a.c = x.size(-1);
+  TORCH_CHECK(groups >= 1 && groups <= a.c && a.c % groups == 0, "group_norm: ", a.c, " channels do not split into ", groups, " groups");
+  TORCH_CHECK(act >= MB_ACT_NONE && act <= MB_ACT_RELU, "group_norm: unknown activation ", act);
+  a.r = x.numel() / a.c;
+  if (offsets.defined()) {
+    on_device(offsets, "offsets", x);
+    TORCH_CHECK(x.dim() == 2, "x must be [rows, channels] with offsets (got ", x.sizes(), ")");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 1 &&
+                    (offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong),
+                "offsets must be int32 or int64 [samples + 1] (got ", offsets.sizes(), ", ", offsets.scalar_type(), ")");
+    a.off = offsets.contiguous();
+    a.off64 = offsets.scalar_type() == at::kLong;
+    a.n = offsets.size(0) - 1;
+    a.len = 0;
+  } else {
+    a.n = x.size(0);
+    a.len = a.n ? a.r / a.n : 0;
+  }
+  a.rows = a.r ? rows_of(x) : x;
+  for (const Tensor* t : {&w, &b}) {
+    if (!t->defined()) continue;
+    on_device(*t, "weight / bias", x);
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == a.c, "weight / bias must be [", a.c, "] (got ", t->sizes(), ")");
+    TORCH_CHECK(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat,
+                "weight / bias must have the type of x or float32");
+    TORCH_CHECK(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias differ in type");
+    a.pt = type_code(*t, "weight / bias");
+  }
+  a.w = w.defined() ? w.contiguous() : w;
+  a.b = b.defined() ? b.contiguous() : b;
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gn_forward(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps,
+                                              int64_t act, const Tensor& offsets, bool stats) {
+  GnIn a = gn_in(x, groups, w, b, offsets, act);
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous), mean, rstd;
+  if (stats) {
+    mean = at::empty({a.n, groups}, x.options().dtype(at::kFloat));
+    rstd = at::empty({a.n, groups}, x.options().dtype(at::kFloat));
+  }
+  if (a.r)
+    check_rc(mace_b200_group_norm_fwd(a.rows.data_ptr(), row_stride(a.rows), ptr(a.w), ptr(a.b), ptr(a.off), a.off64,
+                                      y.data_ptr(), ptr_as<float>(mean), ptr_as<float>(rstd), a.r, a.n, a.len, (int32_t)a.c,
+                                      (int32_t)groups, eps, (int32_t)act, a.dt, a.pt, stream_of(x)),
+             "group_norm");
+  return {y, mean, rstd};
+}
+
+Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps, int64_t act,
+                  const OptTensor& offsets) {
+  return std::get<0>(gn_forward(x, groups, or_none(w), or_none(b), eps, act, or_none(offsets), false));
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_fwd(const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b,
+                                                  double eps, int64_t act, const OptTensor& offsets) {
+  return gn_forward(x, groups, or_none(w), or_none(b), eps, act, or_none(offsets), true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& dy, const Tensor& x, int64_t groups, const OptTensor& w,
+                                                  const OptTensor& b, int64_t act, const OptTensor& offsets,
+                                                  const Tensor& mean, const Tensor& rstd, bool need_x, bool need_w,
+                                                  bool need_b) {
+  GnIn a = gn_in(x, groups, or_none(w), or_none(b), or_none(offsets), act);
+  on_device(dy, "dy", x);
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), "dy must have the shape and type of x");
+  for (const Tensor* t : {&mean, &rstd}) {
+    on_device(*t, "mean / rstd", x);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == a.n * groups,
+                "mean / rstd must be float32 with one value per sample and group");
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  auto popt = x.options().dtype(a.pt == MB_F32 ? at::kFloat : x.scalar_type());
+  Tensor dx = need_x ? at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous) : Tensor();
+  Tensor dw = need_w ? at::empty({a.c}, popt) : Tensor(), db = need_b ? at::empty({a.c}, popt) : Tensor(), ws;
+  if (need_w || need_b) {
+    int64_t words = 0;
+    check_rc(mace_b200_group_norm_bwd_workspace(a.n, (int32_t)a.c, &words), "group_norm_bwd");
+    ws = at::empty({words > 0 ? words : 1}, x.options().dtype(at::kFloat));
+  }
+  Tensor g = a.r ? rows_of(dy) : dy;
+  if (a.r || need_w || need_b)
+    check_rc(mace_b200_group_norm_bwd(ptr(g), a.r ? row_stride(g) : a.c, ptr(a.rows), a.r ? row_stride(a.rows) : a.c, ptr(a.w),
+                                      ptr(a.b), ptr(a.off), a.off64, mean.data_ptr<float>(), rstd.data_ptr<float>(), ptr(dx),
+                                      ptr(dw), ptr(db), ptr_as<float>(ws), a.r, a.n, a.len, (int32_t)a.c, (int32_t)groups,
+                                      (int32_t)act, a.dt, a.pt, stream_of(x)),
+             "group_norm_bwd");
+  return {dx, dw, db};
+}
+
+struct GroupNormGrad : torch::autograd::Function<GroupNormGrad> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps,
+                        int64_t act, const OptTensor& offsets) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto fwd = op_of<decltype(group_norm_fwd)>("mace_b200::group_norm_fwd");
+    auto [y, mean, rstd] = fwd.call(x, groups, w, b, eps, act, offsets);
+    ctx->save_for_backward({x, or_none(w), or_none(b), or_none(offsets), mean, rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("group_norm");
+    auto s = ctx->get_saved_variables();
+    if (!g[0].defined()) return variable_list(7);
+    // needs_input_grad counts the tensors that were given
+    const bool has_w = s[1].defined(), has_b = s[2].defined();
+    static auto bwd = op_of<decltype(group_norm_bwd)>("mace_b200::group_norm_bwd");
+    auto [dx, dw, db] = bwd.call(g[0], s[0], ctx->saved_data["groups"].toInt(), opt(s[1]), opt(s[2]),
+                                 ctx->saved_data["act"].toInt(), opt(s[3]), s[4], s[5], ctx->needs_input_grad(0),
+                                 has_w && ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(1 + has_w));
+    return {dx, Tensor(), dw, db, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor group_norm_autograd(const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps, int64_t act,
+                           const OptTensor& offsets) {
+  no_dual("group_norm", {&x, &or_none(w), &or_none(b)});
+  if (wants_grad({&x, &or_none(w), &or_none(b)})) return GroupNormGrad::apply(x, groups, w, b, eps, act, offsets);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = op_of<decltype(group_norm)>("mace_b200::group_norm");
+  return op.call(x, groups, w, b, eps, act, offsets);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(mace_b200, m) {
+  m.def("group_norm(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act, Tensor? offsets) -> Tensor");
+  m.def("group_norm_fwd(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act, Tensor? offsets) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("group_norm_bwd(Tensor dy, Tensor x, int groups, Tensor? weight, Tensor? bias, int act, Tensor? offsets, Tensor mean, "
+        "Tensor rstd, bool need_x, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(mace_b200, CUDA, m) {
+  m.impl("group_norm", &group_norm);
+  m.impl("group_norm_fwd", &group_norm_fwd);
+  m.impl("group_norm_bwd", &group_norm_bwd);
+}
+
+TORCH_LIBRARY_IMPL(mace_b200, AutogradCUDA, m) { m.impl("group_norm", &group_norm_autograd); }

@@ -98,6 +98,11 @@ _SIGS = {
     "mace_b200_layer_norm_bwd_workspace": (c_i32, [c_i64, c_i32, ctypes.POINTER(c_i64)]),
     "mace_b200_layer_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                          c_i32, c_i32, c_i32, c_vp]),
+    "mace_b200_group_norm_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32,
+                                         c_i32, c_f64, c_i32, c_i32, c_i32, c_vp]),
+    "mace_b200_group_norm_bwd_workspace": (c_i32, [c_i64, c_i32, ctypes.POINTER(c_i64)]),
+    "mace_b200_group_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                         c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp]),
     "mace_b200_route_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                     c_f32, c_i32, c_vp]),
     "mace_b200_route_bwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,
@@ -147,7 +152,8 @@ def lib():
 OPS_PATH = os.path.join(_HERE, "_lib", "libmace_b200_torch.so")
 OPS = ("conv_tp", "conv_tp_backward", "build_tables", "edge_l1_fwd", "edge_l1_bwd", "edge_l2_fwd", "edge_l2_bwd",
        "node_gemm", "symcon_fwd", "symcon_bwd", "pack_halo", "unpack_halo_add", "csr_rows", "guard", "layer_norm",
-       "layer_norm_fwd", "layer_norm_bwd", "route", "route_bwd", "expert_plan", "expert_linear", "expert_linear_bwd")
+       "layer_norm_fwd", "layer_norm_bwd", "route", "route_bwd", "expert_plan", "expert_linear", "expert_linear_bwd",
+       "group_norm", "group_norm_fwd", "group_norm_bwd")
 _ops = None
 
 
@@ -199,6 +205,22 @@ def _register_python_side(torch):
         dt = weight.dtype if weight is not None else torch.float32 if bias_f32 else x.dtype
         par = [x.new_empty((x.shape[-1],), dtype=dt) for _ in range(2)]
         return x.new_empty(x.shape), par[0], par[1]
+
+    @tl.register_fake("mace_b200::group_norm")
+    def _gn_fake(x, groups, weight, bias, eps, act, offsets):
+        return x.new_empty(x.shape)
+
+    @tl.register_fake("mace_b200::group_norm_fwd")
+    def _gn_fwd_fake(x, groups, weight, bias, eps, act, offsets):
+        n = x.shape[0] if offsets is None else offsets.shape[0] - 1
+        return (x.new_empty(x.shape), x.new_empty((n, groups), dtype=torch.float32),
+                x.new_empty((n, groups), dtype=torch.float32))
+
+    @tl.register_fake("mace_b200::group_norm_bwd")
+    def _gn_bwd_fake(dy, x, groups, weight, bias, act, offsets, mean, rstd, need_x, need_w, need_b):
+        par = weight if weight is not None else bias
+        shape, dt = (x.shape[-1],), x.dtype if par is None else par.dtype
+        return x.new_empty(x.shape), x.new_empty(shape, dtype=dt), x.new_empty(shape, dtype=dt)
 
     @tl.register_fake("mace_b200::route_bwd")
     def _route_bwd_fake(dweights, logits, experts, softmax, renormalize, scale):
