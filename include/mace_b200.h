@@ -373,6 +373,22 @@ int mace_b200_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_
                              void* db, float* workspace, int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups,
                              int32_t act, int32_t dtype, int32_t ptype, void* stream);
 
+/* ---------------------------------------------------------------- products in 8-bit integers (no counterpart)
+ * quantize_rows: scale[t] = max_k |x[t][k]| / 127 (fp32), q[t][k] = nearest whole number of the exact x / scale, ties to even;
+ * rows of q are ldq bytes apart, bytes [k, ldq) are zeroed.  A row with NaN or an infinity has that scale, and zeros.
+ * int8_linear: y[t][j] = (sum_k q[t][k] w[j][k]) xscale[t] wscale[j] + bias[j] for dense y [tokens][n] of type dtype; sums are
+ * exact (k <= MB_INT8_MAX_K), the rest fp32, rounded once.  wq: rows ldw bytes apart, 16-byte aligned, ldw a multiple of 16.
+ * x not null: tokens of type dtype (ldx elements apart), quantized on the way into xq (ldq bytes apart, aligned as wq) and xscale;
+ * where mace_b200_int8_linear_few(tokens, k) is 1 both may be null.  x null: xq and xscale are given.
+ * bias (may be null) has type btype (dtype or fp32).  A tile whose bounded wait expired is NaN. */
+#define MB_INT8_MAX_K 131071
+int mace_b200_quantize_rows(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int32_t k,
+                            int32_t dtype, void* stream);
+int mace_b200_int8_linear_few(int64_t tokens, int32_t k);
+int mace_b200_int8_linear(const void* x, int64_t ldx, int8_t* xq, int64_t ldq, float* xscale, const int8_t* wq, int64_t ldw,
+                          const float* wscale, const void* bias, void* y, int64_t tokens, int32_t k, int32_t n, int32_t dtype,
+                          int32_t btype, void* stream);
+
 /* ---------------------------------------------------------------- routing to experts (no counterpart in the reference)
  * For each of n rows of E logits (ldl apart): scores s = softmax or sigmoid; the k experts of highest s + bias[e]
  * (bias null: of highest logit), ties to the lowest index, NaN first.  Logits of -inf are closed.  groups > 1 (a

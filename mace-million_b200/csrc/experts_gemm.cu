@@ -42,6 +42,7 @@
 
 #include "experts.cuh"
 #include "tc.cuh"
+#include "tensor_map.cuh"
 
 namespace mb {
 
@@ -649,45 +650,11 @@ __global__ void __launch_bounds__(256) k_parts_sum(const float* parts, const int
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeTiled)p;
-  }();
-  return fn;
-}
-
 // Tensor map of a 16-bit tensor, dimensions inner to outer, SWIZZLE_128B boxes 64 elements wide
 static int xg_map(CUtensorMap* m, bool is_bf16, int rank, const void* p, const int64_t* dims, const int64_t* strides,
                   const int* box) {
-  EncodeTiled enc = encode_tiled();
-  if (!enc) {
-    set_error("expert_linear: the driver has no cuTensorMapEncodeTiled");
-    return MB_E_CUDA;
-  }
-  cuuint64_t d[3], s[2];
-  cuuint32_t b[3], es[3] = {1, 1, 1};
-  for (int i = 0; i < rank; ++i) {
-    d[i] = (cuuint64_t)dims[i];
-    b[i] = (cuuint32_t)box[i];
-    if (i) s[i - 1] = (cuuint64_t)strides[i - 1] * 2;
-  }
-  const CUresult rc = enc(m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
-                          const_cast<void*>(p), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (rc != CUDA_SUCCESS) {
-    set_error("expert_linear: cuTensorMapEncodeTiled failed (%d)", (int)rc);
-    return MB_E_CUDA;
-  }
-  return 0;
+  return tensor_map("expert_linear", m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rank, p,
+                    dims, strides, box);
 }
 
 // Widest tile: three planes of two operands fill a stage at 128 columns

@@ -1,4 +1,5 @@
-// torch.ops.mace_b200.*: group norm with an activation over the C ABI (include/mace_b200.h), with its autograd formula.  As in
+// torch.ops.mace_b200.*: group norm with an activation (with its autograd formula) and products in 8-bit integers over the C
+// ABI (include/mace_b200.h).  As in
 // torch_ops.cpp, the ops check devices, types and shapes with TORCH_CHECK, launch on torch's current CUDA stream and
 // allocate outputs and workspaces with torch's caching allocator.
 #include "torch_ops_util.h"
@@ -144,6 +145,122 @@ Tensor group_norm_autograd(const Tensor& x, int64_t groups, const OptTensor& w, 
   return op.call(x, groups, w, b, eps, act, offsets);
 }
 
+// ------------------------------------------------------------------------------------------------ products in 8-bit integers
+int64_t pad16(int64_t k) { return (k + 15) / 16 * 16; }
+
+// [rows, k] of 8-bit values as rows that start on 16 bytes: the tensor itself where it has them, else a copy
+Tensor rows16(const Tensor& q) {
+  const bool ok = q.stride(1) == 1 && (q.size(0) <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1))) &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
+  if (ok) return q;
+  Tensor r = at::empty({q.size(0), pad16(q.size(1))}, q.options()).narrow(1, 0, q.size(1));
+  r.copy_(q);
+  return r;
+}
+int64_t stride16(const Tensor& q) { return q.size(0) > 1 ? q.stride(0) : pad16(q.size(1)); }
+
+void no_grad_formula(const char* what, std::initializer_list<const Tensor*> ts) {
+  TORCH_CHECK(!wants_grad(ts), what, " rounds to whole numbers and has no gradient: call it under torch.no_grad()");
+}
+
+std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  const int32_t dt = type_code(x, "x");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= INT32_MAX - 16, "x must have a last dimension of at least 1 (got ",
+              x.sizes(), ")");
+  const int64_t k = x.size(-1), n = x.numel() / k, ld = pad16(k);
+  c10::cuda::CUDAGuard guard(x.device());
+  auto shape = x.sizes().vec();
+  shape.back() = ld;
+  Tensor q = at::empty(shape, x.options().dtype(at::kChar));
+  shape.pop_back();
+  Tensor scale = at::empty(shape, x.options().dtype(at::kFloat));
+  if (n) {
+    Tensor r = rows_of(x);
+    check_rc(mace_b200_quantize_rows(r.data_ptr(), row_stride(r), q.data_ptr<int8_t>(), ld, scale.data_ptr<float>(), n, (int32_t)k,
+                                     dt, stream_of(x)),
+             "quantize_rows");
+  }
+  return {ld == k ? q : q.narrow(-1, 0, k), scale};
+}
+
+at::ScalarType type_of_code(int64_t code) {
+  TORCH_CHECK(code == MB_F32 || code == MB_BF16 || code == MB_F16, "unknown type ", code);
+  return code == MB_F32 ? at::kFloat : code == MB_BF16 ? at::kBFloat16 : at::kHalf;
+}
+
+// x: float32 / bfloat16 / float16 tokens (quantized on the way), or 8-bit ones with xscale; out: type of the result
+Tensor int8_linear(const Tensor& x, const OptTensor& xscale, const Tensor& w, const Tensor& wscale, const OptTensor& bias,
+                   int64_t out) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  const bool is8 = x.scalar_type() == at::kChar;
+  TORCH_CHECK(is8 == given(xscale), is8 ? "8-bit x needs xscale" : "xscale goes with 8-bit x");
+  TORCH_CHECK(x.dim() >= 1, "x must be [.., in]");
+  on_device(w, "wq", x);
+  TORCH_CHECK(w.dim() == 2 && w.scalar_type() == at::kChar && w.size(0) >= 1 && w.size(1) >= 1, "wq must be int8 [out, in] (got ",
+              w.sizes(), ", ", w.scalar_type(), ")");
+  const int64_t k = w.size(1), n = w.size(0);
+  TORCH_CHECK(x.size(-1) == k, "x must be [.., ", k, "] (got ", x.sizes(), ")");
+  TORCH_CHECK(k <= MB_INT8_MAX_K && n <= INT32_MAX - 255, "wq: at most ", MB_INT8_MAX_K, " columns");
+  on_device(wscale, "wscale", x);
+  TORCH_CHECK(wscale.dim() == 1 && wscale.size(0) == n && wscale.scalar_type() == at::kFloat, "wscale must be float32 [", n, "]");
+  const at::ScalarType type = type_of_code(out);
+  if (!is8) TORCH_CHECK(x.scalar_type() == type, "the result has the type of x");
+  const int64_t t = x.numel() / k;
+  TORCH_CHECK(t <= INT32_MAX - 255, "too many tokens (", t, ")");
+  int32_t bt = (int32_t)out;
+  Tensor b, xs;
+  if (given(bias)) {
+    on_device(*bias, "bias", x);
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == n && (bias->scalar_type() == type || bias->scalar_type() == at::kFloat),
+                "bias must be [", n, "] of the result's type or float32");
+    b = bias->contiguous();
+    bt = type_code(b, "bias");
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  Tensor y = at::empty(shape, x.options().dtype(type));
+  if (t == 0) return y;
+  Tensor ws = wscale.contiguous(), wq = rows16(w), q, src;
+  if (is8) {
+    on_device(*xscale, "xscale", x);
+    TORCH_CHECK(xscale->scalar_type() == at::kFloat && xscale->sizes() == x.sizes().slice(0, x.dim() - 1),
+                "xscale must be float32 with a value for each token");
+    xs = xscale->contiguous();
+    q = rows16(rows_of(x));
+  } else {
+    src = rows_of(x);
+    if (!mace_b200_int8_linear_few(t, (int32_t)k)) {
+      q = at::empty({t, pad16(k)}, w.options());
+      xs = at::empty({t}, ws.options());
+    }
+  }
+  check_rc(mace_b200_int8_linear(ptr(src), src.defined() ? row_stride(src) : k, ptr_as<int8_t>(q),
+                                 q.defined() ? (is8 ? stride16(q) : pad16(k)) : k, ptr_as<float>(xs), wq.data_ptr<int8_t>(),
+                                 stride16(wq), ws.data_ptr<float>(), ptr(b), y.data_ptr(), t, (int32_t)k, (int32_t)n, (int32_t)out,
+                                 bt, stream_of(x)),
+           "int8_linear");
+  return y;
+}
+
+std::tuple<Tensor, Tensor> quantize_rows_autograd(const Tensor& x) {
+  no_dual("quantize_rows", {&x});
+  no_grad_formula("quantize_rows", {&x});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = op_of<decltype(quantize_rows)>("mace_b200::quantize_rows");
+  return op.call(x);
+}
+
+Tensor int8_linear_autograd(const Tensor& x, const OptTensor& xscale, const Tensor& w, const Tensor& wscale, const OptTensor& bias,
+                            int64_t out) {
+  no_dual("int8_linear", {&x, &or_none(xscale), &wscale, &or_none(bias)});
+  no_grad_formula("int8_linear", {&x, &or_none(xscale), &wscale, &or_none(bias)});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = op_of<decltype(int8_linear)>("mace_b200::int8_linear");
+  return op.call(x, xscale, w, wscale, bias, out);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mace_b200, m) {
@@ -152,12 +269,20 @@ TORCH_LIBRARY_FRAGMENT(mace_b200, m) {
         "(Tensor, Tensor, Tensor)");
   m.def("group_norm_bwd(Tensor dy, Tensor x, int groups, Tensor? weight, Tensor? bias, int act, Tensor? offsets, Tensor mean, "
         "Tensor rstd, bool need_x, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
+  m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
+  m.def("int8_linear(Tensor x, Tensor? xscale, Tensor wq, Tensor wscale, Tensor? bias, int out) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mace_b200, CUDA, m) {
   m.impl("group_norm", &group_norm);
   m.impl("group_norm_fwd", &group_norm_fwd);
   m.impl("group_norm_bwd", &group_norm_bwd);
+  m.impl("quantize_rows", &quantize_rows);
+  m.impl("int8_linear", &int8_linear);
 }
 
-TORCH_LIBRARY_IMPL(mace_b200, AutogradCUDA, m) { m.impl("group_norm", &group_norm_autograd); }
+TORCH_LIBRARY_IMPL(mace_b200, AutogradCUDA, m) {
+  m.impl("group_norm", &group_norm_autograd);
+  m.impl("quantize_rows", &quantize_rows_autograd);
+  m.impl("int8_linear", &int8_linear_autograd);
+}

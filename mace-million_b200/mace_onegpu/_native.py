@@ -103,6 +103,10 @@ _SIGS = {
     "mace_b200_group_norm_bwd_workspace": (c_i32, [c_i64, c_i32, ctypes.POINTER(c_i64)]),
     "mace_b200_group_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
                                          c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp]),
+    "mace_b200_quantize_rows": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp]),
+    "mace_b200_int8_linear_few": (c_i32, [c_i64, c_i32]),
+    "mace_b200_int8_linear": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32,
+                                      c_i32, c_i32, c_vp]),
     "mace_b200_route_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                     c_f32, c_i32, c_vp]),
     "mace_b200_route_bwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,
@@ -153,7 +157,7 @@ OPS_PATH = os.path.join(_HERE, "_lib", "libmace_b200_torch.so")
 OPS = ("conv_tp", "conv_tp_backward", "build_tables", "edge_l1_fwd", "edge_l1_bwd", "edge_l2_fwd", "edge_l2_bwd",
        "node_gemm", "symcon_fwd", "symcon_bwd", "pack_halo", "unpack_halo_add", "csr_rows", "guard", "layer_norm",
        "layer_norm_fwd", "layer_norm_bwd", "route", "route_bwd", "expert_plan", "expert_linear", "expert_linear_bwd",
-       "group_norm", "group_norm_fwd", "group_norm_bwd")
+       "group_norm", "group_norm_fwd", "group_norm_bwd", "quantize_rows", "int8_linear")
 _ops = None
 
 
@@ -221,6 +225,16 @@ def _register_python_side(torch):
         par = weight if weight is not None else bias
         shape, dt = (x.shape[-1],), x.dtype if par is None else par.dtype
         return x.new_empty(x.shape), x.new_empty(shape, dtype=dt), x.new_empty(shape, dtype=dt)
+
+    @tl.register_fake("mace_b200::quantize_rows")
+    def _quant_fake(x):
+        k = x.shape[-1]
+        q = x.new_empty((*x.shape[:-1], (k + 15) // 16 * 16), dtype=torch.int8)
+        return q[..., :k], x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+    @tl.register_fake("mace_b200::int8_linear")
+    def _int8_fake(x, xscale, wq, wscale, bias, out):
+        return x.new_empty((*x.shape[:-1], wq.shape[0]), dtype=(torch.float32, torch.bfloat16, torch.float16)[out])
 
     @tl.register_fake("mace_b200::route_bwd")
     def _route_bwd_fake(dweights, logits, experts, softmax, renormalize, scale):
