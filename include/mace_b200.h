@@ -389,6 +389,17 @@ int mace_b200_int8_linear(const void* x, int64_t ldx, int8_t* xq, int64_t ldq, f
                           const float* wscale, const void* bias, void* y, int64_t tokens, int32_t k, int32_t n, int32_t dtype,
                           int32_t btype, void* stream);
 
+/* ---------------------------------------------------------------- orthogonalised matrices (no counterpart)
+ * For each of `batch` matrices G [m][n] of type dtype (ldb and ldg elements apart): X = G / (|G|_F + eps), then `steps` (1 .. 16)
+ * times X <- a X + (b A + c A A) X with A = X X^T (m <= n; else X <- a X + X (b A + c A A), A = X^T X), with
+ * coefficients[step][3] = a, b, c (host memory).  out: bf16 [batch][m][n], dense.  The workspace holds
+ * mace_b200_orthogonalize_workspace bytes (256-byte aligned).  Polynomials that reach beyond 3.5 on the way are refused.
+ * A bounded wait that expired leaves NaN. */
+#define MB_ORTH_MAX_DIM 65536
+int mace_b200_orthogonalize_workspace(int64_t batch, int32_t m, int32_t n, int64_t* bytes);
+int mace_b200_orthogonalize(const void* g, int64_t ldb, int64_t ldg, void* out, void* workspace, int64_t batch, int32_t m,
+                            int32_t n, const double* coefficients, int32_t steps, double eps, int32_t dtype, void* stream);
+
 /* ---------------------------------------------------------------- routing to experts (no counterpart in the reference)
  * For each of n rows of E logits (ldl apart): scores s = softmax or sigmoid; the k experts of highest s + bias[e]
  * (bias null: of highest logit), ties to the lowest index, NaN first.  Logits of -inf are closed.  groups > 1 (a

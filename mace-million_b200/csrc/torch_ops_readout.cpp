@@ -1,5 +1,5 @@
-// torch.ops.mace_b200.*: group norm with an activation (with its autograd formula) and products in 8-bit integers over the C
-// ABI (include/mace_b200.h).  As in
+// torch.ops.mace_b200.*: group norm with an activation (with its autograd formula), products in 8-bit integers and orthogonalised
+// matrices over the C ABI (include/mace_b200.h).  As in
 // torch_ops.cpp, the ops check devices, types and shapes with TORCH_CHECK, launch on torch's current CUDA stream and
 // allocate outputs and workspaces with torch's caching allocator.
 #include "torch_ops_util.h"
@@ -261,6 +261,43 @@ Tensor int8_linear_autograd(const Tensor& x, const OptTensor& xscale, const Tens
   return op.call(x, xscale, w, wscale, bias, out);
 }
 
+// ------------------------------------------------------------------------------------------------ orthogonalised matrices
+// coefficients: float64 [steps, 3] in host memory
+Tensor orthogonalize(const Tensor& g, const Tensor& coefficients, double eps) {
+  TORCH_CHECK(g.is_cuda(), "g must be a CUDA tensor");
+  const int32_t dt = type_code(g, "g");
+  TORCH_CHECK(g.dim() >= 2, "g must be [.., m, n] (got ", g.sizes(), ")");
+  TORCH_CHECK(coefficients.device().is_cpu() && coefficients.scalar_type() == at::kDouble && coefficients.dim() == 2 &&
+                  coefficients.size(1) == 3 && coefficients.is_contiguous(),
+              "coefficients must be float64 [steps, 3] in host memory");
+  const int64_t m = g.size(-2), n = g.size(-1);
+  Tensor out = at::empty(g.sizes(), g.options().dtype(at::kBFloat16), at::MemoryFormat::Contiguous);
+  if (g.numel() == 0) return out;
+  const int64_t batch = g.numel() / (m * n);
+  TORCH_CHECK(batch <= 65535 && m <= MB_ORTH_MAX_DIM && n <= MB_ORTH_MAX_DIM, "g: at most 65535 matrices with sides of at most ",
+              MB_ORTH_MAX_DIM, " (got ", g.sizes(), ")");
+  c10::cuda::CUDAGuard guard(g.device());
+  Tensor x = g.dim() == 3 ? g : g.reshape({batch, m, n});
+  const bool ok = (n == 1 || x.stride(2) == 1) && (m == 1 || x.stride(1) >= n) && (batch == 1 || x.stride(0) > 0);
+  if (!ok) x = x.contiguous();
+  int64_t bytes = 0;
+  check_rc(mace_b200_orthogonalize_workspace(batch, (int32_t)m, (int32_t)n, &bytes), "orthogonalize");
+  Tensor ws = at::empty({bytes}, g.options().dtype(at::kByte));
+  check_rc(mace_b200_orthogonalize(x.data_ptr(), batch > 1 ? x.stride(0) : m * n, m > 1 ? x.stride(1) : n, out.data_ptr(),
+                                   ws.data_ptr(), batch, (int32_t)m, (int32_t)n, coefficients.data_ptr<double>(),
+                                   (int32_t)coefficients.size(0), eps, dt, stream_of(g)),
+           "orthogonalize");
+  return out;
+}
+
+Tensor orthogonalize_autograd(const Tensor& g, const Tensor& coefficients, double eps) {
+  no_dual("orthogonalize", {&g});
+  TORCH_CHECK(!wants_grad({&g}), "orthogonalize has no gradient formula: call it under torch.no_grad()");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = op_of<decltype(orthogonalize)>("mace_b200::orthogonalize");
+  return op.call(g, coefficients, eps);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mace_b200, m) {
@@ -269,6 +306,7 @@ TORCH_LIBRARY_FRAGMENT(mace_b200, m) {
         "(Tensor, Tensor, Tensor)");
   m.def("group_norm_bwd(Tensor dy, Tensor x, int groups, Tensor? weight, Tensor? bias, int act, Tensor? offsets, Tensor mean, "
         "Tensor rstd, bool need_x, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
+  m.def("orthogonalize(Tensor g, Tensor coefficients, float eps) -> Tensor");
   m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
   m.def("int8_linear(Tensor x, Tensor? xscale, Tensor wq, Tensor wscale, Tensor? bias, int out) -> Tensor");
 }
@@ -277,12 +315,14 @@ TORCH_LIBRARY_IMPL(mace_b200, CUDA, m) {
   m.impl("group_norm", &group_norm);
   m.impl("group_norm_fwd", &group_norm_fwd);
   m.impl("group_norm_bwd", &group_norm_bwd);
+  m.impl("orthogonalize", &orthogonalize);
   m.impl("quantize_rows", &quantize_rows);
   m.impl("int8_linear", &int8_linear);
 }
 
 TORCH_LIBRARY_IMPL(mace_b200, AutogradCUDA, m) {
   m.impl("group_norm", &group_norm_autograd);
+  m.impl("orthogonalize", &orthogonalize_autograd);
   m.impl("quantize_rows", &quantize_rows_autograd);
   m.impl("int8_linear", &int8_linear_autograd);
 }

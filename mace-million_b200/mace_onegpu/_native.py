@@ -107,6 +107,8 @@ _SIGS = {
     "mace_b200_int8_linear_few": (c_i32, [c_i64, c_i32]),
     "mace_b200_int8_linear": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32,
                                       c_i32, c_i32, c_vp]),
+    "mace_b200_orthogonalize_workspace": (c_i32, [c_i64, c_i32, c_i32, ctypes.POINTER(c_i64)]),
+    "mace_b200_orthogonalize": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_f64, c_i32, c_vp]),
     "mace_b200_route_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                     c_f32, c_i32, c_vp]),
     "mace_b200_route_bwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,
@@ -157,7 +159,8 @@ OPS_PATH = os.path.join(_HERE, "_lib", "libmace_b200_torch.so")
 OPS = ("conv_tp", "conv_tp_backward", "build_tables", "edge_l1_fwd", "edge_l1_bwd", "edge_l2_fwd", "edge_l2_bwd",
        "node_gemm", "symcon_fwd", "symcon_bwd", "pack_halo", "unpack_halo_add", "csr_rows", "guard", "layer_norm",
        "layer_norm_fwd", "layer_norm_bwd", "route", "route_bwd", "expert_plan", "expert_linear", "expert_linear_bwd",
-       "group_norm", "group_norm_fwd", "group_norm_bwd", "quantize_rows", "int8_linear")
+       "group_norm", "group_norm_fwd", "group_norm_bwd", "quantize_rows", "int8_linear",
+       "orthogonalize")
 _ops = None
 
 
@@ -235,6 +238,10 @@ def _register_python_side(torch):
     @tl.register_fake("mace_b200::int8_linear")
     def _int8_fake(x, xscale, wq, wscale, bias, out):
         return x.new_empty((*x.shape[:-1], wq.shape[0]), dtype=(torch.float32, torch.bfloat16, torch.float16)[out])
+
+    @tl.register_fake("mace_b200::orthogonalize")
+    def _orth_fake(g, coefficients, eps):
+        return g.new_empty(g.shape, dtype=torch.bfloat16)
 
     @tl.register_fake("mace_b200::route_bwd")
     def _route_bwd_fake(dweights, logits, experts, softmax, renormalize, scale):

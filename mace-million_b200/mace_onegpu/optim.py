@@ -1,0 +1,88 @@
+"""Training of the matrices of a readout: orthogonalised updates, and an optimiser that takes them.
+
+    u = orthogonalize(g)          # [.., m, n] -> bfloat16: singular values of every matrix moved towards one
+
+    opt = Muon([p for p in block.parameters() if p.dim() >= 2], lr=0.02)
+
+`orthogonalize` runs in sm_100a kernels behind torch.ops.mace_b200.*, on torch's current stream.  Expert matrices [E, O, D] are
+a batch of E matrices.
+"""
+from __future__ import annotations
+
+import torch
+
+from .experts import _op
+
+__all__ = ["orthogonalize", "Muon", "COEFFICIENTS"]
+
+# a, b, c of the odd polynomial a s + b s^3 + c s^5: steep at zero, and every s of (0, 1] stays near one after a few steps
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+_TABLES = {}
+
+
+def _table(steps, coefficients):
+    """float64 [steps, 3] in host memory, made once for each argument."""
+    key = (steps, tuple(map(tuple, coefficients)) if isinstance(coefficients[0], (tuple, list)) else tuple(coefficients))
+    if key not in _TABLES:
+        rows = key[1] if isinstance(key[1][0], tuple) else (key[1],) * steps
+        if len(rows) != steps or any(len(r) != 3 for r in rows):
+            raise ValueError(f"coefficients must be (a, b, c), or one such triple for each of the {steps} steps")
+        if len(_TABLES) > 64:
+            _TABLES.clear()
+        _TABLES[key] = torch.tensor(rows, dtype=torch.float64)
+    return _TABLES[key]
+
+
+def orthogonalize(g, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """g [.., m, n] (float32, bfloat16 or float16) -> bfloat16 [.., m, n]: X = g / (|g| + eps) with the Frobenius norm, then `steps`
+    times X = a X + (b A + c A A) X with A = X X^T (from the right with A = X^T X for m > n).  Every matrix of the batch for itself.
+
+    coefficients: (a, b, c), or a triple for each step; what they do to singular values in (0, 1] must stay below 3.5.
+    The last two dimensions' rows may be strided.  At most 16 steps and sides of 65,536.  No gradient."""
+    steps = int(steps)
+    if not 1 <= steps <= 16:
+        raise ValueError(f"steps must be in [1, 16] (got {steps})")
+    return _op("orthogonalize")(g, _table(steps, coefficients), float(eps))
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update of a matrix [.., m, n] is orthogonalised: p <- p (1 - lr weight_decay) - lr max(1, m / n)^0.5 U with
+    U = orthogonalize(g + momentum v) (nesterov) or of v, and v <- momentum v + g.  For parameters of two dimensions or more;
+    vectors (norms, biases) take another optimiser."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
+            raise ValueError(f"lr {lr}, momentum {momentum} or weight_decay {weight_decay} is out of range")
+        _table(int(steps), coefficients)
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes matrices [.., m, n] (got a parameter of shape {tuple(p.shape)})")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            lr, mu = group["lr"], group["momentum"]
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                v = self.state[p].get("momentum_buffer")
+                if v is None:
+                    v = self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                v.mul_(mu).add_(p.grad)
+                d = p.grad.add(v, alpha=mu) if group["nesterov"] else v
+                u = orthogonalize(d, steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+                if group["weight_decay"]:
+                    p.mul_(1 - lr * group["weight_decay"])
+                p.add_(u, alpha=-lr * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
+        return loss
