@@ -40,6 +40,7 @@
 
 #include <type_traits>
 
+#include "epilogue.cuh"
 #include "experts.cuh"
 #include "tc.cuh"
 #include "tensor_map.cuh"
@@ -55,7 +56,6 @@ static_assert(32 * (XG_EPI0 * XG_REGS_LOW + XG_EPI_WARPS * XG_REGS_HIGH) <= XG_T
 // mace_b200_expert_test_hooks sets them, so that a test drives the timeout path without any fault.
 __device__ unsigned long long g_xg_wait_ns = 2000000000ull;
 __device__ int g_xg_skip_load = 0;
-constexpr int XG_STG = 2048;                     // row staging of one epilogue warp
 // Most K blocks of an accumulator whose result leaves in fp32: of fp32 data, of 16-bit data, and where each CTA has one tile
 // at most (its drains cost nothing then).  Gradients of the routing weights from 16-bit data, 2,048 columns: error 7e-7 at
 // 12, 4.8e-7 at 8; 65,536 x 4 slots, 1024 -> 2048: dx with them 80 us longer at 8.
@@ -110,11 +110,6 @@ struct XgTile {
   bool rows_ok;                                  // FWD / DGRAD: this CTA's rows belong to the expert
 };
 
-// Row staging of the epilogue: a warp's 32 rows x 64 bytes, 16-byte piece c of row r at piece c ^ (r / 2 % 4), so that a
-// lane's access to its own row and the warp's access to eight whole row segments are both free of bank conflicts.
-__device__ __forceinline__ uint32_t xg_stg(uint32_t stg, int row, int c) {
-  return stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-}
 // element i of a staged piece
 template <typename OUT>
 __device__ __forceinline__ OUT xg_elem(uint32_t piece, int i) {
@@ -153,21 +148,7 @@ __device__ __forceinline__ void xg_fetch(uint4 (&xq)[4], const int (&row)[4], co
 // Writes 32 columns of the rows that the lanes of a warp hold (v, one row per lane), scaled, through shared memory in pieces
 // of 64 bytes: global accesses are whole sectors of eight rows (one row per lane would be 32 scattered 16-byte pieces per
 // access, and held a tile for longer than its products at K <= 1024).  out: first column; left: columns that exist.
-// Everything that does not change from piece to piece is in XgLane.
-struct XgLane {
-  uint32_t own[4], seg[4];                       // staging addresses: this lane's row, piece c; row 8 i + l / 4, piece l % 4
-};
-__device__ __forceinline__ XgLane xg_lane(uint32_t stg) {
-  const int lane = threadIdx.x & 31;
-  XgLane a;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a.own[i] = xg_stg(stg, lane, i);
-    a.seg[i] = xg_stg(stg, 8 * i + (lane >> 2), lane & 3);
-  }
-  return a;
-}
-
+// Everything that does not change from piece to piece is in XgLane (epilogue.cuh).
 template <typename OUT>
 __device__ __forceinline__ void xg_emit32(const float* v, const XgLane& a, uint32_t stg, const int (&row)[4], OUT* out,
                                           int64_t ldo, bool vec, float sc, int left) {

@@ -22,7 +22,7 @@ inline EncodeTiled encode_tiled() {
   return fn;
 }
 
-// Map of a tensor of `rank` dimensions (inner to outer), strides of the outer ones and the box in elements of `size` bytes;
+// Map of a tensor of `rank` (at most 4) dimensions (inner to outer), strides of the outer ones and the box in elements of `size` bytes;
 // elements outside are zero
 inline int tensor_map(const char* who, CUtensorMap* m, CUtensorMapDataType type, int size, int rank, const void* p,
                       const int64_t* dims, const int64_t* strides, const int* box) {
@@ -31,8 +31,8 @@ inline int tensor_map(const char* who, CUtensorMap* m, CUtensorMapDataType type,
     set_error("%s: the driver has no cuTensorMapEncodeTiled", who);
     return MB_E_CUDA;
   }
-  cuuint64_t d[3], s[2];
-  cuuint32_t b[3], es[3] = {1, 1, 1};
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], es[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     d[i] = (cuuint64_t)dims[i];
     b[i] = (cuuint32_t)box[i];
