@@ -388,9 +388,13 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
         const OrTile w = or_tile(p, t);
         const int acc = tc & 1, i0 = w.m0 + rank * 128 + q4 * 32, i = i0 + lane, rows = p.M - i0 < 32 ? p.M - i0 : 32;
         float4 nx[8];                             // the next piece of X, or in the first four of A, on its way
+        float dn = 0.f;                           // and the diagonal's entry of this lane's column
+        const float* dvec = (kind == OR_UPDATE ? g.e : g.d) + (int64_t)w.b * g.r;
+        const float di = !lost && (kind == OR_SQUARE || (kind == OR_UPDATE && !g.tall)) && lane < rows ? __ldcg(dvec + i) : 0.f;
         auto fetch = [&](int c) {
           const int j0 = w.n0 + hf * hw + c;
           if (lost || rows <= 0 || j0 >= p.N) return;
+          if (kind == OR_SQUARE || (kind == OR_UPDATE && g.tall)) dn = j0 + lane < p.N ? __ldcg(dvec + j0 + lane) : 0.f;
           if (kind == OR_UPDATE) {
             const float4* x = reinterpret_cast<const float4*>(g.X + w.b * g.pc + ((int64_t)(i0 >> 5) * g.cj + (j0 >> 5)) * 1024);
 #pragma unroll
@@ -439,17 +443,16 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
             } else {
 #pragma unroll
               for (int q = 0; q < 8; ++q) v[4 * q] = nx[q].x, v[4 * q + 1] = nx[q].y, v[4 * q + 2] = nx[q].z, v[4 * q + 3] = nx[q].w;
+              const float el = ca + dn;
               if (c + 32 < hw) fetch(c + 32);
-              const float* e = g.e + (int64_t)w.b * g.r;
               if (g.tall) {
-                const float el = ca + (lane < nc ? __ldcg(e + j0 + lane) : 0.f);
 #pragma unroll
                 for (int x = 0; x < 32; ++x)
                   v[x] = fmaf(__shfl_sync(0xffffffffu, el, x), v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
               } else {
-                const float el = ca + (lane < rows ? __ldcg(e + i) : 0.f);
+                const float f = ca + di;
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = fmaf(el, v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
+                for (int x = 0; x < 32; ++x) v[x] = fmaf(f, v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
               }
             }
             if (last) {
@@ -466,35 +469,35 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
             f16* dst = (kind == OR_GRAM ? g.A : g.B) + w.b * g.pr;
             float* diag = (kind == OR_GRAM ? g.d : g.e) + (int64_t)w.b * g.r;
             const bool on = i0 == j0;             // the diagonal runs through this piece: column x = lane
+            float dia = 0.f;
             if (kind == OR_GRAM) {
-              const float sc = g.poly.inv_s * g.poly.inv_s;
+              const float sc = g.poly.inv_s * g.poly.inv_s * OR_SA;
 #pragma unroll
-              for (int x = 0; x < 32; ++x) {
-                const float a = __uint_as_float(u[x]) * sc;
-                if (on && x == lane && lane < rows) diag[i] = a;
-                v[x] = on && x == lane ? 0.f : a * OR_SA;
-              }
+              for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(u[x]) * sc;
             } else {
-              const float* d = g.d + (int64_t)w.b * g.r;
-              const float di = lane < rows ? __ldcg(d + i) : 0.f, dl = lane < nc ? __ldcg(d + j0 + lane) : 0.f;
+              // b a1 + c (a1 (d_i + d_j) + sq), all times SB: a1's plane is SA a1, the accumulator SA^2 sq
+              const float k2 = cc * (OR_SB / OR_SA), k1 = fmaf(k2, di, cb * (OR_SB / OR_SA)), k3 = cc * (OR_SB / (OR_SA * OR_SA));
+              const float dl = k2 * dn;
 #pragma unroll
               for (int q = 0; q < 4; ++q) sts128(at.seg[q], *reinterpret_cast<const uint4*>(&nx[q]));
               __syncwarp();
+              if (c + 32 < hw) fetch(c + 32);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float f[8];
                 unpack16(lds128(at.own[q]), f, f16());
 #pragma unroll
-                for (int x = 0; x < 8; ++x) v[8 * q + x] = f[x] * (1.f / OR_SA);
+                for (int x = 0; x < 8; ++x)
+                  v[8 * q + x] = fmaf(f[x], k1 + __shfl_sync(0xffffffffu, dl, 8 * q + x), __uint_as_float(u[8 * q + x]) * k3);
               }
               __syncwarp();
-              if (c + 32 < hw) fetch(c + 32);
+            }
+            if (on) {
 #pragma unroll
-              for (int x = 0; x < 32; ++x) {
-                const float sq = __uint_as_float(u[x]) * (1.f / (OR_SA * OR_SA)), dj = __shfl_sync(0xffffffffu, dl, x);
-                if (on && x == lane && lane < rows) diag[i] = fmaf(cb, di, cc * fmaf(di, di, sq));
-                v[x] = on && x == lane ? 0.f : fmaf(cb, v[x], cc * fmaf(v[x], di + dj, sq)) * OR_SB;
-              }
+              for (int x = 0; x < 32; ++x)
+                if (x == lane) dia = v[x], v[x] = 0.f;
+              if (lane < rows)
+                diag[i] = kind == OR_GRAM ? dia * (1.f / OR_SA) : fmaf(cb, di, fmaf(cc * di, di, dia * (1.f / OR_SB)));
             }
             or_put<f16, true>(v, at, stg, dst + i0 * g.ldr + j0, g.ldr, rows, nc, true);
             // and to the other side of the diagonal, where no tile is computed

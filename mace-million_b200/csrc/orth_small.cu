@@ -31,7 +31,7 @@ struct OsArgs {
 struct OsShared {
   double norm[2];                                 // of the CTA, of the matrix
   double red[8];
-  float d[128], e[128];
+  alignas(16) float d[128], e[128];
   uint64_t bar;
   uint32_t tmem;
   int failed;
@@ -50,8 +50,8 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_cluster_u32x2(uint32_t a, uint32_t x, uint32_t y) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void st_cluster_u32x4(uint32_t a, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void st_cluster_f32(uint32_t a, float x) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
@@ -99,9 +99,16 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
     if (row < g.r && nc > 0) {
       if (g.tall) {
         const T* p = gp + (int64_t)j0 * g.ldg + row;
+        if (nc >= 32) {
+          T t[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x)
-          if (x < nc) f[x] = to_f(p[(int64_t)x * g.ldg]);
+          for (int x = 0; x < 32; ++x) t[x] = p[(int64_t)x * g.ldg];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) f[x] = to_f(t[x]);
+        } else {
+          for (int x = 0; x < 32; ++x)
+            if (x < nc) f[x] = to_f(p[(int64_t)x * g.ldg]);
+        }
       } else {
         const T* p = gp + (int64_t)row * g.ldg + j0;
         constexpr int V = kVec<T>;
@@ -202,23 +209,27 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
         mma_f16_ss_lead<1>(lead, td, a, a, id128, k ? 1u : 0u);
       }
     });
-    const float sc = g.poly.inv_s * g.poly.inv_s;
+    // eight columns of A at a time: the diagonal apart (dia: the column among them, or outside of 0 .. 7), the rest to the plane
+    const float sc = g.poly.inv_s * g.poly.inv_s * OR_SA;
     if (P == 1) {
 #pragma unroll 1
       for (int c = half * 64; c < half * 64 + 64; c += 32) {
         uint32_t u[32];
+        float v[32];
         tmem_ld32(td + lanes + c, u);
         tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(u[x]) * sc;
+        if (c == (warp & 3) * 32) {               // the diagonal runs through this piece
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (x == lane) S.d[row] = v[x] * (1.f / OR_SA), v[x] = 0.f;
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float f[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float a = __uint_as_float(u[8 * q + x]) * sc;
-            const bool dia = c + 8 * q + x == row;
-            if (dia) S.d[row] = a;
-            f[x] = dia ? 0.f : a * OR_SA;
-          }
+          for (int x = 0; x < 8; ++x) f[x] = v[8 * q + x];
           sts128(plane + os_piece(row, c / 8 + q), pack16<f16>(f));
         }
       }
@@ -234,32 +245,51 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
           sts128(sums + (uint32_t)((c / 4 + q) * 128 + row) * 16, make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
       }
       cluster_sync();
-      const int per = 4096 / P;                   // pieces of four columns of a row
-      for (int p = rank * per + tid; p < (rank + 1) * per; p += OS_THREADS) {
-        float4 t[OS_MAX_P];
+      // 2048 / P pieces of eight columns of a row for this CTA: 8 / P for a thread
+      auto slice = [&](auto np) {
+        constexpr int PP = decltype(np)::value, PER = 8 / PP;
+        float f[PER][8];
 #pragma unroll
-        for (int q = 0; q < OS_MAX_P; ++q)
-          if (q < P) t[q] = ld_cluster_f32x4(mapa_u32(sums + p * 16, q));
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < PER; ++k) {
+          const int p = rank * (2048 / PP) + k * OS_THREADS + tid;
+          const uint32_t at = sums + (uint32_t)((p / 128 * 2) * 128 + (p & 127)) * 16;
+          float4 t[PP][2];
 #pragma unroll
-        for (int q = 0; q < OS_MAX_P; ++q)
-          if (q < P) f[0] += t[q].x, f[1] += t[q].y, f[2] += t[q].z, f[3] += t[q].w;
-        const int i = p & 127, c = p / 128 * 4;
-        float dv = 0.f;
-        bool dia = false;
+          for (int q = 0; q < PP; ++q) {
+            const uint32_t from = mapa_u32(at, q);
+            t[q][0] = ld_cluster_f32x4(from);
+            t[q][1] = ld_cluster_f32x4(from + 2048);
+          }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          f[x] *= sc;
-          if (c + x == i) dia = true, dv = f[x], f[x] = 0.f;
-          f[x] *= OR_SA;
+          for (int h = 0; h < 2; ++h) {
+            float4 v = t[0][h];
+#pragma unroll
+            for (int q = 1; q < PP; ++q) v.x += t[q][h].x, v.y += t[q][h].y, v.z += t[q][h].z, v.w += t[q][h].w;
+            f[k][4 * h] = v.x * sc, f[k][4 * h + 1] = v.y * sc, f[k][4 * h + 2] = v.z * sc, f[k][4 * h + 3] = v.w * sc;
+          }
         }
-        const uint32_t at = plane + os_piece(i, c / 8) + (c & 7) * 2, da = smem_u32(&S.d[i]);
-        const uint32_t w0 = pack2(f[0], f[1], f16()), w1 = pack2(f[2], f[3], f16());
-        for (int q = 0; q < P; ++q) {
-          st_cluster_u32x2(mapa_u32(at, q), w0, w1);
-          if (dia) st_cluster_f32(mapa_u32(da, q), dv);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int p = rank * (2048 / PP) + k * OS_THREADS + tid, i = p & 127, c8 = p / 128, dia = i - 8 * c8;
+          float dv = 0.f;
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if (x == dia) dv = f[k][x] * (1.f / OR_SA), f[k][x] = 0.f;
+          const uint4 w = pack16<f16>(f[k]);
+          const uint32_t at = plane + os_piece(i, c8), da = smem_u32(&S.d[i]);
+#pragma unroll
+          for (int q = 0; q < PP; ++q) {
+            st_cluster_u32x4(mapa_u32(at, q), w);
+            if (dia >= 0 && dia < 8) st_cluster_f32(mapa_u32(da, q), dv);
+          }
         }
-      }
+      };
+      if (P == 2)
+        slice(std::integral_constant<int, 2>());
+      else if (P == 4)
+        slice(std::integral_constant<int, 4>());
+      else
+        slice(std::integral_constant<int, 8>());
       cluster_sync();
     }
     // -------------------------------------------------------------------------------------------- b A + c A A
@@ -271,26 +301,38 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       }
     });
     {
-      const float di = S.d[row];
+      // b a1 + c (a1 (d_i + d_j) + sq), all times SB: a1's plane is SA a1, the accumulator SA^2 sq
+      const float di = S.d[row], k2 = cc * (OR_SB / OR_SA), k1 = fmaf(k2, di, cb * (OR_SB / OR_SA)), k3 = cc * (OR_SB / (OR_SA * OR_SA));
 #pragma unroll 1
       for (int c = half * 64; c < half * 64 + 64; c += 32) {
         uint32_t u[32];
+        float v[32];
         tmem_ld32(td + lanes + c, u);
         tmem_wait_ld();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t at = plane + os_piece(row, c / 8 + q);
           float f[8];
-          unpack16(lds128(at), f, f16());
+          unpack16(lds128(plane + os_piece(row, c / 8 + q)), f, f16());
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int j = c + 8 * q + x;
-            const float s2 = __uint_as_float(u[8 * q + x]) * (1.f / (OR_SA * OR_SA)), a1 = f[x] * (1.f / OR_SA);
-            const bool dia = j == row;
-            if (dia) S.e[row] = fmaf(cb, di, cc * fmaf(di, di, s2));
-            f[x] = dia ? 0.f : fmaf(cb, a1, cc * fmaf(a1, di + S.d[j], s2)) * OR_SB;
+          for (int h = 0; h < 2; ++h) {
+            const float4 dj = *reinterpret_cast<const float4*>(&S.d[c + 8 * q + 4 * h]);
+            const float t[4] = {dj.x, dj.y, dj.z, dj.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              v[8 * q + 4 * h + x] = fmaf(f[4 * h + x], fmaf(k2, t[x], k1), __uint_as_float(u[8 * q + 4 * h + x]) * k3);
           }
-          sts128(at, pack16<f16>(f));
+        }
+        if (c == (warp & 3) * 32) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (x == lane) S.e[row] = fmaf(cb, di, fmaf(cc * di, di, v[x] * (1.f / OR_SB))), v[x] = 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float f[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) f[x] = v[8 * q + x];
+          sts128(plane + os_piece(row, c / 8 + q), pack16<f16>(f));
         }
       }
       __syncthreads();
