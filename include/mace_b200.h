@@ -361,13 +361,14 @@ int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_
  * [0, rows]: sample i is rows [offsets[i], offsets[i + 1]); rows outside of all samples give zeros; a sample whose offsets descend
  * or leave the rows is NaN (nothing is accessed out of range).
  * mean / rstd [n][groups] are written when not null (both or none); the backward pass reads them.
- * bwd: dx (may be null) dense; dw / db [c] of type ptype (may be null), summed in a fixed order through `workspace`
- * (mace_b200_group_norm_bwd_workspace floats; unused when both are null). */
+ * bwd: dx (may be null) dense; dw / db [c] of type ptype (may be null), summed in a fixed order.
+ * workspace: mace_b200_group_norm_workspace floats (may be null where that is 0; ragged: with offsets). */
 enum { MB_ACT_NONE = 0, MB_ACT_SILU = 1, MB_ACT_GELU = 2, MB_ACT_RELU = 3 };
 int mace_b200_group_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, const void* offsets, int32_t offsets64,
-                             void* y, float* mean, float* rstd, int64_t rows, int64_t n, int64_t len, int32_t c,
-                             int32_t groups, double eps, int32_t act, int32_t dtype, int32_t ptype, void* stream);
-int mace_b200_group_norm_bwd_workspace(int64_t n, int32_t c, int64_t* floats);
+                             void* y, float* mean, float* rstd, float* workspace, int64_t rows, int64_t n, int64_t len,
+                             int32_t c, int32_t groups, double eps, int32_t act, int32_t dtype, int32_t ptype, void* stream);
+int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups, int32_t ragged,
+                                   int32_t dtype, int32_t backward, int64_t* floats);
 int mace_b200_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b,
                              const void* offsets, int32_t offsets64, const float* mean, const float* rstd, void* dx, void* dw,
                              void* db, float* workspace, int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups,

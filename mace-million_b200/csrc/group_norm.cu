@@ -4,10 +4,14 @@
 //   dx = r (a - mean(a) - xh mean(a xh)), dw = sum over rows of dz xh, db = sum over rows of dz.
 // f: identity, silu z s(z), gelu z Phi(z) or relu.  Statistics and sums are fp32; every output is rounded once.
 //
-// Bound: HBM bytes (forward x and y, backward x, dy and dx, each once).  A cluster of P CTAs and a block of whole groups own a
-// sample's rows of those columns: a CTA keeps its rows in shared memory between the sums and the output, exchanges sums of
-// its groups with the cluster through distributed shared memory, and no row is read twice while P CTAs hold them.  Rows beyond
-// that are read again, last ones first, as L2 has those.
+// Bound: HBM bytes (forward x and y, backward x, dy and dx, each once).  Two forms of the same kernels:
+//  * on the chip (GN_WHOLE): a cluster of P <= 8 CTAs owns a sample's rows of a block of whole groups.  A CTA keeps its rows in shared
+//    memory between the sums and the output and exchanges sums of its groups with the cluster through distributed shared memory.
+//    Rows that do not fit (ragged samples far above the mean) are read again.
+//  * larger ones stream: GN_SUMS (partial sums of P parts of a sample to the workspace), a small kernel that adds up the parts, and
+//    GN_APPLY, which reads the rows again, last ones first, as L2 has those.  No barrier stands between the bytes, so both run near
+//    the copy rate.  (Large samples in clusters of 8 on the chip read once, but load and store in turns: 64 x 2048 x 512 bf16
+//    forward 124 us and backward 315.)
 // A thread owns V channels of one group (16 bytes, or what divides a group) and every TR-th row, and takes its sums relative to
 // its own first row: of one thread's few hundred rows they lose at most that number of fp32 roundings, whatever the mean.
 // Threads, CTAs and clusters are joined as (count, mean, sum of squared deviations), so nothing cancels.  No atomics: parameter
@@ -22,11 +26,18 @@ struct GnArgs {
   const void *x, *dy, *w, *b;
   void* out;                                      // y, or dx (null: parameter gradients only)
   float *mean, *rstd, *partial;                   // partial [cluster rows][2][C]: sums of dz xh, of dz (null: none)
+  float *sums, *stat;                             // [n][P][3][groups] of GN_SUMS, [n][groups][2] for GN_APPLY
   const void* off;                                // [n + 1], null: samples of `len` rows
   int64_t ldx, lddy, rows, n, len;
-  int32_t c, groups, cg, gpb, act, off64, p32, cap;   // gpb: groups of a column block; cap: row steps kept in shared memory
+  int32_t c, groups, cg, gpb, act, off64, p32, cap, pshift, pvec;   // gpb: groups of a column block; cap: row steps kept in shared memory
+                                                  // pshift: log2 of a cluster's CTAs; pvec: parameters are aligned vectors
   float eps;
 };
+
+// CTAs of 256 threads that the registers let be resident on an SM
+constexpr int GN_FWD_CTAS = 4, GN_BWD_CTAS = 2;
+
+enum { GN_WHOLE = 0, GN_SUMS = 1, GN_APPLY = 2 };
 
 // Rows of a sample; false: the offsets descend or leave the rows there
 __device__ __forceinline__ bool gn_range(const GnArgs& a, int64_t s, int64_t& lo, int64_t& hi) {
@@ -92,61 +103,137 @@ struct GnVec {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Word*>(p) = u; }
 };
 
-// f(z) and f'(z).  16-bit results take the fast exponential (2 ulp of fp32 and |z| 2^-24).
-template <typename T>
-__device__ __forceinline__ float gn_exp(float v) {
-  if constexpr (sizeof(T) == 4) return expf(v);
-  return __expf(v);
+// V elements as Elem<V> (packed pairs where V > 1) and back
+template <typename T, int V>
+__device__ __forceinline__ void gn_get(const GnVec<T, V>& v, Elem<V> (&e)[kElems<V>]) {
+  float f[V];
+  v.get(f);
+  to_elems<V>(f, e);
+}
+template <typename T, int V>
+__device__ __forceinline__ void gn_set(GnVec<T, V>& v, const Elem<V> (&e)[kElems<V>]) {
+  float f[V];
+  from_elems<V>(e, f);
+  v.set(f);
+}
+
+// 1 / (1 + exp(-z)).  fp32 results take expf and a division; 16-bit ones 2^(-z log2 e) and a reciprocal, each approximate to
+// 2^-22 (the exponent's rounding |z| 2^-24): 0 where the power is infinite.
+__device__ __forceinline__ float pow2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 template <typename T>
 __device__ __forceinline__ float gn_sigmoid(float z) {
   if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
-  return __fdividef(1.f, 1.f + __expf(-z));       // 0 where the exponential is above 2^126
+  return rcp_fast(1.f + pow2_fast(-1.4426950408889634f * z));
 }
-template <typename T, int V>
-__device__ __forceinline__ void gn_act(float (&z)[V], int act) {
+template <typename T>
+__device__ __forceinline__ float2 gn_sigmoid(float2 z) {
+  if constexpr (sizeof(T) == 4) return make_float2(gn_sigmoid<T>(z.x), gn_sigmoid<T>(z.y));
+  const float2 t = e_mul(z, e_splat<float2>(-1.4426950408889634f));
+  const float2 d = e_add(make_float2(pow2_fast(t.x), pow2_fast(t.y)), e_splat<float2>(1.f));
+  return make_float2(rcp_fast(d.x), rcp_fast(d.y));
+}
+// Phi(z) and the normal density of z.  16-bit results: Abramowitz and Stegun 7.1.26 for the tail, 0.5 poly(1 / (1 + p |z| / sqrt 2))
+// exp(-z^2 / 2), to 1e-7 absolute; the exponential is the density's, too (the complementary error function took 100 instructions).
+struct GnPhi {
+  float cdf, pdf;
+};
+template <typename T>
+__device__ __forceinline__ GnPhi gn_phi(float z) {
+  if constexpr (sizeof(T) == 4) return {normcdff(z), 0.3989422804014327f * expf(-0.5f * z * z)};
+  const float e = pow2_fast(-0.7213475204444817f * z * z), t = rcp_fast(fmaf(0.3275911f * 0.7071067811865476f, fabsf(z), 1.f));
+  float h = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  h = fmaf(h, t, 0.5f * 1.421413741f);
+  h = fmaf(h, t, 0.5f * -0.284496736f);
+  h = fmaf(h, t, 0.5f * 0.254829592f) * t * e;
+  return {z < 0.f ? h : 1.f - h, 0.3989422804014327f * e};
+}
+template <typename T>
+__device__ __forceinline__ float gn_gelu(float z) { return z * gn_phi<T>(z).cdf; }
+template <typename T>
+__device__ __forceinline__ float gn_gelu_slope(float z) {
+  const GnPhi p = gn_phi<T>(z);
+  return fmaf(z, p.pdf, p.cdf);
+}
+__device__ __forceinline__ float2 gn_each(float2 a, float (*f)(float)) { return make_float2(f(a.x), f(a.y)); }
+__device__ __forceinline__ float gn_each(float a, float (*f)(float)) { return f(a); }
+__device__ __forceinline__ float gn_relu(float z) { return z < 0.f ? 0.f : z; }                       // NaN stays
+__device__ __forceinline__ float gn_gate(float z, float d) { return z <= 0.f ? 0.f : d; }
+__device__ __forceinline__ float2 gn_gate(float2 z, float2 d) { return make_float2(gn_gate(z.x, d.x), gn_gate(z.y, d.y)); }
+
+template <typename T, typename E, int NE>
+__device__ __forceinline__ void gn_act(E (&z)[NE], int act) {
   if (act == MB_ACT_SILU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) z[q] *= gn_sigmoid<T>(z[q]);
+    for (int q = 0; q < NE; ++q) z[q] = e_mul(z[q], gn_sigmoid<T>(z[q]));
   } else if (act == MB_ACT_GELU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) z[q] *= normcdff(z[q]);
+    for (int q = 0; q < NE; ++q) z[q] = gn_each(z[q], gn_gelu<T>);
   } else if (act == MB_ACT_RELU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) z[q] = z[q] < 0.f ? 0.f : z[q];   // NaN stays
+    for (int q = 0; q < NE; ++q) z[q] = gn_each(z[q], gn_relu);
   }
 }
-template <typename T, int V>
-__device__ __forceinline__ void gn_act_grad(const float (&z)[V], float (&d)[V], int act) {   // d *= f'(z)
+template <typename T, typename E, int NE>
+__device__ __forceinline__ void gn_act_grad(const E (&z)[NE], E (&d)[NE], int act) {   // d *= f'(z)
+  const E one = e_splat<E>(1.f), minus = e_splat<E>(-1.f);
   if (act == MB_ACT_SILU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-      const float s = gn_sigmoid<T>(z[q]);
-      d[q] *= s * fmaf(z[q], 1.f - s, 1.f);
+    for (int q = 0; q < NE; ++q) {
+      const E s = gn_sigmoid<T>(z[q]);
+      d[q] = e_mul(d[q], e_mul(s, e_fma(z[q], e_fma(s, minus, one), one)));
     }
   } else if (act == MB_ACT_GELU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-      const float pdf = 0.3989422804014327f * gn_exp<T>(-0.5f * z[q] * z[q]);
-      d[q] *= fmaf(z[q], pdf, normcdff(z[q]));
-    }
+    for (int q = 0; q < NE; ++q) d[q] = e_mul(d[q], gn_each(z[q], gn_gelu_slope<T>));
   } else if (act == MB_ACT_RELU) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) d[q] = z[q] <= 0.f ? 0.f : d[q];
+    for (int q = 0; q < NE; ++q) d[q] = gn_gate(z[q], d[q]);
   }
 }
 
 // V parameters, fp32 or of type T
 template <typename T, int V>
-__device__ __forceinline__ void gn_param(const void* p, int32_t p32, int c, float other, float (&f)[V]) {
+__device__ __forceinline__ void gn_param(const void* p, const GnArgs& a, int c, float other, Elem<V> (&e)[kElems<V>]) {
+  float f[V];
 #pragma unroll
-  for (int q = 0; q < V; ++q) f[q] = !p ? other : p32 ? ((const float*)p)[c + q] : to_f(((const T*)p)[c + q]);
+  for (int q = 0; q < V; ++q) f[q] = other;
+  if (p && a.p32 && a.pvec && V % 4 == 0) {
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      const float4 t = *reinterpret_cast<const float4*>((const float*)p + c + q);
+      f[q] = t.x, f[q + 1] = t.y, f[q + 2] = t.z, f[q + 3] = t.w;
+    }
+  } else if (p && !a.p32 && a.pvec) {
+    GnVec<T, V> t;
+    t.load((const T*)p + c);
+    t.get(f);
+  } else if (p) {
+#pragma unroll
+    for (int q = 0; q < V; ++q) f[q] = a.p32 ? ((const float*)p)[c + q] : to_f(((const T*)p)[c + q]);
+  }
+  to_elems<V>(f, e);
+}
+// A CTA's (a part's) rows of a sample of len rows: the first of them, or (rank + 1) where they end
+template <int MODE>
+__device__ __forceinline__ int64_t gn_cut_row(const GnArgs& a, int64_t len, int rank, int P) {
+  return MODE == GN_WHOLE ? (len * rank) >> a.pshift : len * rank / P;
 }
 
-// How a thread of a CTA walks over the CTA's rows and columns
+// How a thread of a CTA walks over the CTA's rows and columns: TC vector columns at a time (`tiles` times), TR rows.
+// slots > 0: the groups lie within warps, in runs of cgv lanes (a power of two), so that warps take sums by shuffles and the sums of
+// a group come in that many places; 0: sums go through `red`, a thread each, into one place.
 struct GnWalk {
-  int g0, ng, c0, nvec, tc, tr, r, col, tiles;
-  bool on;
+  int g0, ng, c0, nvec, tc, tr, r, col, tiles, cgv, slots, grp;   // grp: of the thread's column in the first tile
+  bool on, writes;                                // writes: the lane that stores a warp's sums of its group
 };
 template <int V>
 __device__ __forceinline__ GnWalk gn_walk(const GnArgs& a) {
@@ -154,7 +241,8 @@ __device__ __forceinline__ GnWalk gn_walk(const GnArgs& a) {
   k.g0 = blockIdx.y * a.gpb;
   k.ng = a.groups - k.g0 < a.gpb ? a.groups - k.g0 : a.gpb;
   k.c0 = k.g0 * a.cg;
-  k.nvec = k.ng * a.cg / V;
+  k.cgv = a.cg / V;
+  k.nvec = k.ng * k.cgv;
   const int th = blockDim.x;
   k.tc = k.nvec < th ? k.nvec : th;
   k.tr = th / k.tc;
@@ -162,7 +250,26 @@ __device__ __forceinline__ GnWalk gn_walk(const GnArgs& a) {
   k.col = threadIdx.x - k.r * k.tc;
   k.tiles = (k.nvec + k.tc - 1) / k.tc;
   k.on = k.r < k.tr;
+  const bool fits = k.cgv <= 32 && (k.cgv & (k.cgv - 1)) == 0 && k.tiles == 1 && th % k.tc == 0;
+  k.slots = fits && (k.tc < 32 ? (k.tc & (k.tc - 1)) == 0 : k.tc % 32 == 0) ? (k.tc < 32 ? th / 32 : k.tr) : 0;
+  if (k.slots * a.gpb > (a.gpb < th ? th : a.gpb)) k.slots = 0;   // (a narrower last block has more rows than there is room for)
+  k.grp = k.col / k.cgv;
+  k.writes = (threadIdx.x & 31 & (k.cgv - 1)) == 0 && (k.tc >= 32 || (threadIdx.x & 31) < k.tc);
   return k;
+}
+// Rows of a thread among nr
+__device__ __forceinline__ int gn_count(int64_t nr, const GnWalk& k) {
+  const int64_t n = nr - k.r + k.tr - 1;
+  return (n >> 31) ? (int)(n / k.tr) : (int)((unsigned)n / (unsigned)k.tr);
+}
+// The place of this thread's warp among a group's slots
+__device__ __forceinline__ int gn_slot(const GnWalk& k) { return k.tc < 32 ? threadIdx.x >> 5 : k.r; }
+
+// Sum over the lanes of a warp that hold the same group (all of them have it)
+__device__ __forceinline__ float gn_warp_sum(const GnWalk& k, float v) {
+  for (int o = k.cgv >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = k.tc; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) { return __int_as_float(ld_cluster_s32(addr)); }
@@ -174,91 +281,114 @@ __device__ __forceinline__ float octet_sum(float v) {
   return v;
 }
 
-// Shared memory: red [threads] pairs | grp [2][3][gpb] (by parity of the sample: what this CTA found) | fin [2][gpb] | kept rows
-__device__ __forceinline__ size_t gn_shared_floats(int threads, int gpb) { return 2 * (size_t)threads + 8 * (size_t)gpb; }
+// Shared memory: red [threads] pairs | grp [2][slots][3][gpb] (by parity of the sample: what this CTA found) | fin [2][gpb] | rows.
+// slots gpb is at most the number of threads, or slots is one.
+__host__ __device__ __forceinline__ int gn_grp_floats(int threads, int gpb) { return 3 * (gpb < threads ? threads : gpb); }
+__host__ __device__ __forceinline__ int gn_shared_floats(int threads, int gpb) {
+  return (2 * threads + 2 * gn_grp_floats(threads, gpb) + 2 * gpb + 3) & ~3;
+}
 
-template <typename T, int V>
-__global__ void __launch_bounds__(512, 2) k_gn_fwd(const GnArgs a) {
-  constexpr int U = 4;
+template <int MODE, typename T, int V>
+__global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
+  constexpr int U = 4, NE = kElems<V>;
+  using E = Elem<V>;
+  using Vec = GnVec<T, V>;
   extern __shared__ __align__(16) float gn_smem[];
   const GnWalk k = gn_walk<V>(a);
   const int th = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = th >> 5;
-  const int P = gridDim.x, rank = blockIdx.x;
+  // the second launch goes through the rows backwards
+  const int P = gridDim.x, rank = MODE == GN_APPLY ? P - 1 - (int)blockIdx.x : (int)blockIdx.x;
+  const int cap = MODE == GN_WHOLE ? a.cap : 0, slots = k.slots ? k.slots : 1;
   float2* red = reinterpret_cast<float2*>(gn_smem);
   float* grp0 = gn_smem + 2 * th;
-  float* fin = grp0 + 6 * a.gpb;
-  using Vec = GnVec<T, V>;
-  Vec* kept = reinterpret_cast<Vec*>(gn_smem + ((gn_shared_floats(th, a.gpb) + 3) & ~(size_t)3)) + threadIdx.x;
-  const int cgv = a.cg / V;
-  gn_clear<T>(a);
+  float* fin = grp0 + 2 * gn_grp_floats(th, a.gpb);
+  Vec* kept = reinterpret_cast<Vec*>(gn_smem + gn_shared_floats(th, a.gpb)) + threadIdx.x;
+  const int64_t step = (int64_t)k.tr * a.ldx, ystep = (int64_t)k.tr * a.c;
+  if (MODE != GN_SUMS) gn_clear<T>(a);
   int par = 0;
-  for (int64_t s = blockIdx.z; s < a.n; s += gridDim.z, par ^= 1) {
+  for (int64_t z = blockIdx.z; z < a.n; z += gridDim.z, par ^= 1) {
+    const int64_t s = MODE == GN_APPLY ? a.n - 1 - z : z;
     int64_t lo, hi;
     const bool good = gn_range(a, s, lo, hi);
-    const int64_t len = hi - lo, r0 = lo + len * rank / P, nr = lo + len * (rank + 1) / P - r0;
-    float* grp = grp0 + par * 3 * a.gpb;
-    for (int g = threadIdx.x; g < 3 * k.ng; g += th) grp[g / k.ng * a.gpb + g % k.ng] = 0.f;
-    const int64_t mine = k.on && nr > k.r ? (nr - k.r + k.tr - 1) / k.tr : 0;   // rows of this thread
+    const int64_t len = hi - lo, r0 = lo + gn_cut_row<MODE>(a, len, rank, P), nr = lo + gn_cut_row<MODE>(a, len, rank + 1, P) - r0;
+    float* grp = grp0 + par * gn_grp_floats(th, a.gpb);
+    if (!k.slots)
+      for (int g = threadIdx.x; g < 3 * k.ng; g += th) grp[g / k.ng * a.gpb + g % k.ng] = 0.f;
     // ---------------------------------------------------------------------------------------- sums
-    for (int t = 0; t < k.tiles; ++t) {
+    for (int t = 0; MODE != GN_APPLY && t < k.tiles; ++t) {
       const int v0 = t * k.tc, cv = v0 + k.col;
-      const bool on = cv < k.nvec;
-      const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + k.c0 + cv * V;
-      const int64_t step = (int64_t)k.tr * a.ldx;
-      float piv[V], s1[V], s2[V];
-#pragma unroll
-      for (int q = 0; q < V; ++q) piv[q] = s1[q] = s2[q] = 0.f;
-      if (on && mine > 0) {
+      const bool on = cv < k.nvec && k.on && nr > k.r;
+      float mu = 0.f, m2 = 0.f, mine = 0.f;       // of this thread's rows, and how many
+      if (on) {
+        const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + k.c0 + cv * V;
+        E piv[NE], s1[NE], s2[NE];
         Vec v;
         v.load(x);
-        v.get(piv);
-        auto add = [&](const Vec& u, int64_t i) {
-          float f[V];
-          const int64_t at = i * k.tiles + t;
-          if (at < a.cap) kept[at * th] = u;
-          u.get(f);
+        gn_get<T, V>(v, piv);
 #pragma unroll
-          for (int q = 0; q < V; ++q) {
-            const float e = f[q] - piv[q];
-            s1[q] += e;
-            s2[q] = fmaf(e, e, s2[q]);
+        for (int q = 0; q < NE; ++q) piv[q] = e_mul(piv[q], e_splat<E>(-1.f)), s1[q] = s2[q] = e_splat<E>(0.f);
+        int at = t;                               // place among the kept vectors
+        auto add = [&](const Vec& u) {
+          E f[NE];
+          if (at < cap) kept[at * th] = u;
+          at += k.tiles;
+          gn_get<T, V>(u, f);
+#pragma unroll
+          for (int q = 0; q < NE; ++q) {
+            const E e = e_add(f[q], piv[q]);
+            s1[q] = e_add(s1[q], e);
+            s2[q] = e_fma(e, e, s2[q]);
           }
         };
-        int64_t i = 0;
-        for (; i + U <= mine; i += U) {
+        int64_t left = nr - k.r;                  // rows from this thread's next one on
+        int i = 0;
+        for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * step, i += U) {
           Vec u[U];
 #pragma unroll
-          for (int j = 0; j < U; ++j) u[j].load(x + (i + j) * step);
+          for (int j = 0; j < U; ++j) u[j].load(x + j * step);
 #pragma unroll
-          for (int j = 0; j < U; ++j) add(u[j], i + j);
+          for (int j = 0; j < U; ++j) add(u[j]);
         }
-        for (; i < mine; ++i) {
+        for (; left > 0; left -= k.tr, x += step, ++i) {
           Vec u;
-          u.load(x + i * step);
-          add(u, i);
+          u.load(x);
+          add(u);
         }
-      }
-      // V channels to (mean, squared deviations) of mine * V values
-      float mu = 0.f, m2 = 0.f;
-      if (on && mine > 0) {
-        const float inv = 1.f / (float)mine;
-        float m[V];
+        // V channels to (mean, squared deviations) of mine * V values
+        mine = (float)i;
+        const float inv = __fdividef(1.f, mine);
+        float p[V], u1[V], u2[V];
+        from_elems<V>(piv, p);
+        from_elems<V>(s1, u1);
+        from_elems<V>(s2, u2);
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-          const float d = s1[q] * inv;
-          m[q] = piv[q] + d;
-          mu += m[q];
-          m2 += fmaxf(fmaf(-s1[q], d, s2[q]), 0.f * s2[q]);   // not below 0, NaN stays
+          const float d = u1[q] * inv;
+          p[q] = d - p[q];
+          mu += p[q];
+          m2 += fmaxf(fmaf(-u1[q], d, u2[q]), 0.f * u2[q]);   // not below 0, NaN stays
         }
         mu *= 1.f / (float)V;
 #pragma unroll
-        for (int q = 0; q < V; ++q) m2 = fmaf((m[q] - mu) * (m[q] - mu), (float)mine, m2);
+        for (int q = 0; q < V; ++q) m2 = fmaf((p[q] - mu) * (p[q] - mu), mine, m2);
+      }
+      if (k.slots) {
+        const float n = mine * (float)V, cnt = gn_warp_sum(k, n), sum = gn_warp_sum(k, n * mu);
+        const float mean = cnt > 0.f ? __fdividef(sum, cnt) : 0.f;
+        const float dev = gn_warp_sum(k, n > 0.f ? fmaf((mu - mean) * (mu - mean), n, m2) : 0.f);
+        if (k.writes) {
+          float* o = grp + gn_slot(k) * 3 * a.gpb + k.grp;
+          o[0] = cnt;
+          o[a.gpb] = mean;
+          o[2 * a.gpb] = dev;
+        }
+        continue;
       }
       __syncthreads();                            // red is free (and grp is zero)
       red[threadIdx.x] = make_float2(mu, m2);
       __syncthreads();
       for (int g = warp; g < k.ng; g += warps) {
-        const int a0 = g * cgv - v0 > 0 ? g * cgv - v0 : 0, a1 = (g + 1) * cgv - v0;
+        const int a0 = g * k.cgv - v0 > 0 ? g * k.cgv - v0 : 0, a1 = (g + 1) * k.cgv - v0;
         const int w = (a1 < k.nvec - v0 ? (a1 < k.tc ? a1 : k.tc) : (k.nvec - v0 < k.tc ? k.nvec - v0 : k.tc)) - a0;
         if (w <= 0) continue;
         const int entries = w * k.tr;
@@ -273,7 +403,7 @@ __global__ void __launch_bounds__(512, 2) k_gn_fwd(const GnArgs a) {
         for (int e = lane; e < entries; e += 32) {
           const int r = e / w, n = nr > r ? (int)((nr - r + k.tr - 1) / k.tr) : 0;
           const float2 v = red[r * k.tc + a0 + (e - r * w)];
-          if (n > 0) dev += fmaf((v.x - mean) * (v.x - mean), (float)(n * V), v.y);
+          if (n > 0) dev += fmaf((v.x - mean) * (v.x - mean), (float)n * (float)V, v.y);
         }
         dev = warp_sum(dev);
         if (lane == 0 && cnt > 0.f) {             // join with the tiles before
@@ -284,30 +414,43 @@ __global__ void __launch_bounds__(512, 2) k_gn_fwd(const GnArgs a) {
         }
       }
     }
-    if (P > 1)
+    if (MODE == GN_WHOLE && P > 1)
       cluster_sync();
-    else
+    else if (MODE != GN_APPLY)
       __syncthreads();
-    // ---------------------------------------------------------------------------------------- statistics of the cluster
-    for (int g = threadIdx.x >> 3; g < (k.ng + 3) / 4 * 4; g += th >> 3) {
-      const int q = threadIdx.x & 7, gg = g < k.ng ? g : k.ng - 1;
-      float cnt = 0.f, m = 0.f, m2 = 0.f;
-      if (q < P) {
-        if (P > 1) {
-          const uint32_t at = mapa_u32(smem_u32(grp + gg), q);
-          cnt = ld_cluster_f32(at);
-          m = ld_cluster_f32(at + 4 * a.gpb);
-          m2 = ld_cluster_f32(at + 8 * a.gpb);
-        } else {
-          cnt = grp[gg], m = grp[a.gpb + gg], m2 = grp[2 * a.gpb + gg];
-        }
+    // ---------------------------------------------------------------------------------------- statistics
+    // eight lanes a group take the slots of its CTAs (GN_SUMS: of this one) in turn, twice: the mean, then the deviations from it
+    for (int g = threadIdx.x >> 3; MODE != GN_APPLY && g < (k.ng + 3) / 4 * 4; g += th >> 3) {
+      const int gg = g < k.ng ? g : k.ng - 1, all = MODE == GN_WHOLE ? slots << a.pshift : slots;
+      const uint32_t base = smem_u32(grp + gg);
+      auto word = [&](int q, int which) {
+        if (MODE == GN_WHOLE && P > 1)
+          return ld_cluster_f32(mapa_u32(base + 4u * (uint32_t)(((q >> a.pshift) * 3 + which) * a.gpb), q & (P - 1)));
+        return grp[gg + (q * 3 + which) * a.gpb];
+      };
+      float n = 0.f, m = 0.f, m2 = 0.f;
+      for (int q = threadIdx.x & 7; q < all; q += 8) {
+        const float cnt = word(q, 0);
+        n += cnt;
+        m = fmaf(cnt, word(q, 1), m);
       }
-      const float n = octet_sum(cnt), mean = n > 0.f ? octet_sum(cnt * m) / n : 0.f;
-      const float d = m - mean;
-      m2 = octet_sum(cnt > 0.f ? fmaf(d * d, cnt, m2) : 0.f);
-      if (q == 0 && g < k.ng) {
+      n = octet_sum(n);
+      m = octet_sum(m);
+      const float mean = n > 0.f ? __fdividef(m, n) : 0.f;
+      for (int q = threadIdx.x & 7; q < all; q += 8) {
+        const float cnt = word(q, 0), d = word(q, 1) - mean;
+        if (cnt > 0.f) m2 += fmaf(d * d, cnt, word(q, 2));
+      }
+      m2 = octet_sum(m2);
+      if ((threadIdx.x & 7) != 0 || g >= k.ng) continue;
+      if (MODE == GN_SUMS) {
+        float* part = a.sums + (s * P + rank) * 3 * a.groups + k.g0 + g;
+        part[0] = n;
+        part[a.groups] = mean;
+        part[2 * a.groups] = m2;
+      } else {
         const float bad = good ? 0.f : __int_as_float(0x7fc00000);
-        const float rs = rsqrtf((n > 0.f ? m2 / n : 0.f) + a.eps) + bad;
+        const float rs = rsqrtf((n > 0.f ? __fdividef(m2, n) : 0.f) + a.eps) + bad;
         fin[2 * g] = mean + bad;
         fin[2 * g + 1] = rs;
         if (a.mean && rank == 0) {
@@ -316,155 +459,205 @@ __global__ void __launch_bounds__(512, 2) k_gn_fwd(const GnArgs a) {
         }
       }
     }
-    __syncthreads();
+    if (MODE == GN_SUMS) continue;
+    if (MODE == GN_WHOLE) __syncthreads();
+    const float* st = MODE == GN_APPLY ? a.stat + (s * a.groups + k.g0) * 2 : fin;
     // ---------------------------------------------------------------------------------------- outputs
     for (int t = 0; t < k.tiles; ++t) {
       const int cv = t * k.tc + k.col;
-      if (cv >= k.nvec || mine == 0) continue;
-      const int c = k.c0 + cv * V, g = cv / cgv;
-      float w[V], b[V];
-      gn_param<T, V>(a.w, a.p32, c, 1.f, w);
-      gn_param<T, V>(a.b, a.p32, c, 0.f, b);
-      const float mean = fin[2 * g], rs = fin[2 * g + 1];
+      if (cv >= k.nvec || !k.on || nr <= k.r) continue;
+      const int c = k.c0 + cv * V, g = k.tiles == 1 ? k.grp : cv / k.cgv;
+      E w[NE], b[NE];
+      gn_param<T, V>(a.w, a, c, 1.f, w);
+      gn_param<T, V>(a.b, a, c, 0.f, b);
+      const E neg = e_splat<E>(-st[2 * g]), rs = e_splat<E>(st[2 * g + 1]);
 #pragma unroll
-      for (int q = 0; q < V; ++q) w[q] *= rs;
-      const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c;
-      T* y = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c;
-      const int64_t step = (int64_t)k.tr * a.ldx, ystep = (int64_t)k.tr * a.c;
-      auto put = [&](Vec v, int64_t i) {
-        float f[V];
-        v.get(f);
+      for (int q = 0; q < NE; ++q) w[q] = e_mul(w[q], rs);
+      auto put = [&](Vec v, T* y) {
+        E f[NE];
+        gn_get<T, V>(v, f);
 #pragma unroll
-        for (int q = 0; q < V; ++q) f[q] = fmaf(f[q] - mean, w[q], b[q]);
-        gn_act<T, V>(f, a.act);
-        v.set(f);
-        v.store(y + i * ystep);
+        for (int q = 0; q < NE; ++q) f[q] = e_fma(e_add(f[q], neg), w[q], b[q]);
+        gn_act<T>(f, a.act);
+        gn_set<T, V>(v, f);
+        v.store(y);
       };
-      const int64_t have = a.cap > t ? (a.cap - t + k.tiles - 1) / k.tiles : 0;   // rows kept
-      int64_t i = mine - 1;
-      for (; i >= have + U - 1; i -= U) {
+      const int have = cap > t ? (cap - t + k.tiles - 1) / k.tiles : 0;   // rows kept
+      int i = gn_count(nr, k);
+      const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c + (int64_t)i * step;   // one row behind the next
+      T* y = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c + (int64_t)i * ystep;
+      for (; i - U >= have; i -= U) {
+        x -= U * step;
+        y -= U * ystep;
         Vec u[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j].load(x + (i - j) * step);
+        for (int j = 0; j < U; ++j) u[j].load(x + j * step);
 #pragma unroll
-        for (int j = 0; j < U; ++j) put(u[j], i - j);
+        for (int j = 0; j < U; ++j) put(u[j], y + j * ystep);
       }
-      for (; i >= have; --i) {
+      for (; i > have; --i) {
+        x -= step;
+        y -= ystep;
         Vec u;
-        u.load(x + i * step);
-        put(u, i);
+        u.load(x);
+        put(u, y);
       }
+      const Vec* kp = kept + (i * k.tiles + t) * th;
+      const int kstep = k.tiles * th;
 #pragma unroll 2
-      for (; i >= 0; --i) put(kept[(i * k.tiles + t) * th], i);
+      for (; i > 0; --i) {
+        kp -= kstep;
+        y -= ystep;
+        put(*kp, y);
+      }
     }
   }
-  if (P > 1) cluster_sync();                      // no CTA leaves while its peers may read its sums
+  if (MODE == GN_WHOLE && P > 1) cluster_sync();  // no CTA leaves while its peers may read its sums
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256, 2) k_gn_bwd(const GnArgs a) {
-  constexpr int U = 2;
+template <int MODE, typename T, int V>
+__global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
+  constexpr int U = 4, NE = kElems<V>;
+  using E = Elem<V>;
+  using Vec = GnVec<T, V>;
   extern __shared__ __align__(16) float gn_smem[];
   const GnWalk k = gn_walk<V>(a);
   const int th = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = th >> 5;
-  const int P = gridDim.x, rank = blockIdx.x;
+  const int P = gridDim.x, rank = MODE == GN_APPLY ? P - 1 - (int)blockIdx.x : (int)blockIdx.x;
+  const int cap = MODE == GN_WHOLE ? a.cap : 0, slots = k.slots ? k.slots : 1;
   float2* red = reinterpret_cast<float2*>(gn_smem);
   float* grp0 = gn_smem + 2 * th;
-  float* fin = grp0 + 6 * a.gpb;
-  using Vec = GnVec<T, V>;
-  Vec* kept = reinterpret_cast<Vec*>(gn_smem + ((gn_shared_floats(th, a.gpb) + 3) & ~(size_t)3)) + threadIdx.x;
-  const int cgv = a.cg / V;
-  gn_clear<T>(a);
-  float tw[V], tb[V];                             // sums of dz xh and dz over the samples (one tile of columns)
+  float* fin = grp0 + 2 * gn_grp_floats(th, a.gpb);
+  Vec* kept = reinterpret_cast<Vec*>(gn_smem + gn_shared_floats(th, a.gpb)) + threadIdx.x;
+  if (MODE != GN_SUMS) gn_clear<T>(a);
+  // sums of dz xh and dz over the samples (one tile of columns): a thread's own places behind the kept rows
+  float* total = gn_smem + gn_shared_floats(th, a.gpb) + (size_t)2 * cap * th * V * sizeof(T) / 4 + threadIdx.x;
+  if (MODE != GN_APPLY && k.tiles == 1)
 #pragma unroll
-  for (int q = 0; q < V; ++q) tw[q] = tb[q] = 0.f;
-  float* part = a.partial ? a.partial + ((int64_t)blockIdx.z * P + rank) * 2 * a.c : nullptr;
+    for (int q = 0; q < 2 * V; ++q) total[q * th] = 0.f;
+  float* part = MODE != GN_APPLY && a.partial ? a.partial + ((int64_t)blockIdx.z * P + rank) * 2 * a.c : nullptr;
+  const int64_t xstep = (int64_t)k.tr * a.ldx, dstep = (int64_t)k.tr * a.lddy, ostep = (int64_t)k.tr * a.c;
   int par = 0;
   bool first = true;
-  for (int64_t s = blockIdx.z; s < a.n; s += gridDim.z, par ^= 1, first = false) {
+  for (int64_t z = blockIdx.z; z < a.n; z += gridDim.z, par ^= 1, first = false) {
+    const int64_t s = MODE == GN_APPLY ? a.n - 1 - z : z;
     int64_t lo, hi;
     gn_range(a, s, lo, hi);
-    const int64_t len = hi - lo, r0 = lo + len * rank / P, nr = lo + len * (rank + 1) / P - r0;
-    float* grp = grp0 + par * 3 * a.gpb;
-    for (int g = threadIdx.x; g < 2 * k.ng; g += th) grp[g / k.ng * a.gpb + g % k.ng] = 0.f;
-    const int64_t mine = k.on && nr > k.r ? (nr - k.r + k.tr - 1) / k.tr : 0;
-    const int64_t xstep = (int64_t)k.tr * a.ldx, dstep = (int64_t)k.tr * a.lddy, ostep = (int64_t)k.tr * a.c;
-    // ---------------------------------------------------------------------------------------- sums
-    for (int t = 0; t < k.tiles; ++t) {
-      const int v0 = t * k.tc, cv = v0 + k.col;
-      const bool on = cv < k.nvec && mine > 0;
-      const int c = k.c0 + cv * V;
-      float sw[V], sb[V], s1 = 0.f, s2 = 0.f;
+    const int64_t len = hi - lo, r0 = lo + gn_cut_row<MODE>(a, len, rank, P), nr = lo + gn_cut_row<MODE>(a, len, rank + 1, P) - r0;
+    float* grp = grp0 + par * gn_grp_floats(th, a.gpb);
+    if (!k.slots)
+      for (int g = threadIdx.x; g < 2 * k.ng; g += th) grp[g / k.ng * a.gpb + g % k.ng] = 0.f;
+    // what turns x and dy into xh and dz, for the columns of a tile
+    E w[NE], b[NE], neg, rs;
+    auto columns = [&](int c, int g) {
+      gn_param<T, V>(a.w, a, c, 1.f, w);
+      gn_param<T, V>(a.b, a, c, 0.f, b);
+      const int64_t st = s * a.groups + k.g0 + g;
+      neg = e_splat<E>(-a.mean[st]);
+      rs = e_splat<E>(a.rstd[st]);
+    };
+    auto both = [&](const Vec& u, const Vec& v, E (&f)[NE], E (&d)[NE]) {
+      E z[NE];
+      gn_get<T, V>(u, f);
+      gn_get<T, V>(v, d);
 #pragma unroll
-      for (int q = 0; q < V; ++q) sw[q] = sb[q] = 0.f;
+      for (int q = 0; q < NE; ++q) {
+        f[q] = e_mul(e_add(f[q], neg), rs);
+        z[q] = e_fma(f[q], w[q], b[q]);
+      }
+      gn_act_grad<T>(z, d, a.act);
+    };
+    // ---------------------------------------------------------------------------------------- sums
+    for (int t = 0; MODE != GN_APPLY && t < k.tiles; ++t) {
+      const int v0 = t * k.tc, cv = v0 + k.col;
+      const bool on = cv < k.nvec && k.on && nr > k.r;
+      const int c = k.c0 + cv * V;
+      E sw[NE], sb[NE];
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int q = 0; q < NE; ++q) sw[q] = sb[q] = e_splat<E>(0.f);
       if (on) {
-        float w[V], b[V];
-        gn_param<T, V>(a.w, a.p32, c, 1.f, w);
-        gn_param<T, V>(a.b, a.p32, c, 0.f, b);
-        const int64_t st = s * a.groups + k.g0 + cv / cgv;
-        const float mean = a.mean[st], rs = a.rstd[st];
+        columns(c, k.tiles == 1 ? k.grp : cv / k.cgv);
         const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c;
         const T* dy = (const T*)a.dy + (r0 + k.r) * a.lddy + c;
-        auto add = [&](const Vec& u, const Vec& v, int64_t i) {
-          const int64_t at = i * k.tiles + t;
-          if (at < a.cap) {
+        int at = t;
+        auto add = [&](const Vec& u, const Vec& v) {
+          if (at < cap) {
             kept[2 * at * th] = u;
             kept[(2 * at + 1) * th] = v;
           }
-          float f[V], d[V], z[V];
-          u.get(f);
-          v.get(d);
+          at += k.tiles;
+          E f[NE], d[NE];
+          both(u, v, f, d);
 #pragma unroll
-          for (int q = 0; q < V; ++q) {
-            f[q] = (f[q] - mean) * rs;
-            z[q] = fmaf(f[q], w[q], b[q]);
-          }
-          gn_act_grad<T, V>(z, d, a.act);
-#pragma unroll
-          for (int q = 0; q < V; ++q) {
-            sw[q] = fmaf(d[q], f[q], sw[q]);
-            sb[q] += d[q];
+          for (int q = 0; q < NE; ++q) {
+            sw[q] = e_fma(d[q], f[q], sw[q]);
+            sb[q] = e_add(sb[q], d[q]);
           }
         };
-        int64_t i = 0;
-        for (; i + U <= mine; i += U) {
+        int64_t left = nr - k.r;
+        for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * xstep, dy += U * dstep) {
           Vec u[U], v[U];
 #pragma unroll
-          for (int j = 0; j < U; ++j) u[j].load(x + (i + j) * xstep), v[j].load(dy + (i + j) * dstep);
+          for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
 #pragma unroll
-          for (int j = 0; j < U; ++j) add(u[j], v[j], i + j);
+          for (int j = 0; j < U; ++j) add(u[j], v[j]);
         }
-        for (; i < mine; ++i) {
+        for (; left > 0; left -= k.tr, x += xstep, dy += dstep) {
           Vec u, v;
-          u.load(x + i * xstep);
-          v.load(dy + i * dstep);
-          add(u, v, i);
+          u.load(x);
+          v.load(dy);
+          add(u, v);
         }
+        E p1 = e_splat<E>(0.f), p2 = p1;
+#pragma unroll
+        for (int q = 0; q < NE; ++q) {
+          p1 = e_fma(w[q], sb[q], p1);
+          p2 = e_fma(w[q], sw[q], p2);
+        }
+        if (k.tiles == 1) {
+          float f[V];
+          from_elems<V>(sw, f);
+#pragma unroll
+          for (int q = 0; q < V; ++q) total[q * th] += f[q];
+          from_elems<V>(sb, f);
+#pragma unroll
+          for (int q = 0; q < V; ++q) total[(V + q) * th] += f[q];
+        }
+        s1 = e_sum(p1);
+        s2 = e_sum(p2);
+      }
+      if (k.slots) {
+        s1 = gn_warp_sum(k, s1);
+        s2 = gn_warp_sum(k, s2);
+        if (k.writes) {
+          float* o = grp + gn_slot(k) * 3 * a.gpb + k.grp;
+          o[0] = s1;
+          o[a.gpb] = s2;
+        }
+        continue;
+      }
+      if (k.tiles > 1 && part && cv < k.nvec) {    // one thread a column: its sums of all samples lie in memory
+        float fw[V], fb[V];
+        from_elems<V>(sw, fw);
+        from_elems<V>(sb, fb);
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-          s1 = fmaf(w[q], sb[q], s1);
-          s2 = fmaf(w[q], sw[q], s2);
-          tw[q] += sw[q];
-          tb[q] += sb[q];
+          part[c + q] = first ? fw[q] : part[c + q] + fw[q];
+          part[a.c + c + q] = first ? fb[q] : part[a.c + c + q] + fb[q];
         }
       }
-      if (k.tiles > 1 && part && cv < k.nvec)      // one thread a column: its sums of all samples lie in memory
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          part[c + q] = first ? sw[q] : part[c + q] + sw[q];
-          part[a.c + c + q] = first ? sb[q] : part[a.c + c + q] + sb[q];
-        }
       __syncthreads();                            // red is free (and grp is zero)
       red[threadIdx.x] = make_float2(s1, s2);
       __syncthreads();
       for (int g = warp; g < k.ng; g += warps) {
-        const int a0 = g * cgv - v0 > 0 ? g * cgv - v0 : 0, a1 = (g + 1) * cgv - v0;
-        const int w = (a1 < k.nvec - v0 ? (a1 < k.tc ? a1 : k.tc) : (k.nvec - v0 < k.tc ? k.nvec - v0 : k.tc)) - a0;
-        if (w <= 0) continue;
+        const int a0 = g * k.cgv - v0 > 0 ? g * k.cgv - v0 : 0, a1 = (g + 1) * k.cgv - v0;
+        const int n = (a1 < k.nvec - v0 ? (a1 < k.tc ? a1 : k.tc) : (k.nvec - v0 < k.tc ? k.nvec - v0 : k.tc)) - a0;
+        if (n <= 0) continue;
         float u = 0.f, v = 0.f;
-        for (int e = lane; e < w * k.tr; e += 32) {
-          const int r = e / w;
-          const float2 p = red[r * k.tc + a0 + (e - r * w)];
+        for (int e = lane; e < n * k.tr; e += 32) {
+          const int r = e / n;
+          const float2 p = red[r * k.tc + a0 + (e - r * n)];
           u += p.x;
           v += p.y;
         }
@@ -477,139 +670,231 @@ __global__ void __launch_bounds__(256, 2) k_gn_bwd(const GnArgs a) {
       }
     }
     if (!a.out) continue;
-    if (P > 1)
+    if (MODE == GN_WHOLE && P > 1)
       cluster_sync();
-    else
+    else if (MODE != GN_APPLY)
       __syncthreads();
     const float inv = 1.f / ((float)len * (float)a.cg);
-    for (int g = threadIdx.x >> 3; g < (k.ng + 3) / 4 * 4; g += th >> 3) {
-      const int q = threadIdx.x & 7, gg = g < k.ng ? g : k.ng - 1;
+    for (int g = threadIdx.x >> 3; MODE != GN_APPLY && g < (k.ng + 3) / 4 * 4; g += th >> 3) {
+      const int gg = g < k.ng ? g : k.ng - 1, all = MODE == GN_WHOLE ? slots << a.pshift : slots;
+      const uint32_t base = smem_u32(grp + gg);
       float u = 0.f, v = 0.f;
-      if (q < P) {
-        if (P > 1) {
-          const uint32_t at = mapa_u32(smem_u32(grp + gg), q);
-          u = ld_cluster_f32(at);
-          v = ld_cluster_f32(at + 4 * a.gpb);
+      for (int q = threadIdx.x & 7; q < all; q += 8) {
+        if (MODE == GN_WHOLE && P > 1) {
+          const uint32_t at = mapa_u32(base + 12u * (uint32_t)((q >> a.pshift) * a.gpb), q & (P - 1));
+          u += ld_cluster_f32(at);
+          v += ld_cluster_f32(at + 4 * a.gpb);
         } else {
-          u = grp[gg], v = grp[a.gpb + gg];
+          u += grp[gg + q * 3 * a.gpb];
+          v += grp[gg + (q * 3 + 1) * a.gpb];
         }
       }
       u = octet_sum(u);
       v = octet_sum(v);
-      if (q == 0 && g < k.ng) {
+      if ((threadIdx.x & 7) != 0 || g >= k.ng) continue;
+      if (MODE == GN_SUMS) {
+        float* gp = a.sums + (s * P + rank) * 3 * a.groups + k.g0 + g;
+        gp[0] = u;
+        gp[a.groups] = v;
+      } else {
         fin[2 * g] = u * inv;
         fin[2 * g + 1] = v * inv;
       }
     }
-    __syncthreads();
+    if (MODE == GN_SUMS) continue;
+    if (MODE == GN_WHOLE) __syncthreads();
+    const float* fs = MODE == GN_APPLY ? a.stat + (s * a.groups + k.g0) * 2 : fin;
     // ---------------------------------------------------------------------------------------- dx
     for (int t = 0; t < k.tiles; ++t) {
       const int cv = t * k.tc + k.col;
-      if (cv >= k.nvec || mine == 0) continue;
-      const int c = k.c0 + cv * V, g = cv / cgv;
-      float w[V], b[V];
-      gn_param<T, V>(a.w, a.p32, c, 1.f, w);
-      gn_param<T, V>(a.b, a.p32, c, 0.f, b);
-      const int64_t st = s * a.groups + k.g0 + g;
-      const float mean = a.mean[st], rs = a.rstd[st], m1 = fin[2 * g], m2 = fin[2 * g + 1];
-      const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c;
-      const T* dy = (const T*)a.dy + (r0 + k.r) * a.lddy + c;
-      T* dx = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c;
-      auto put = [&](Vec u, const Vec& v, int64_t i) {
-        float f[V], d[V], z[V];
-        u.get(f);
-        v.get(d);
+      if (cv >= k.nvec || !k.on || nr <= k.r) continue;
+      const int c = k.c0 + cv * V, g = k.tiles == 1 ? k.grp : cv / k.cgv;
+      if (k.tiles > 1 || MODE == GN_APPLY) columns(c, g);
+      const E m1 = e_splat<E>(-fs[2 * g]), m2 = e_splat<E>(-fs[2 * g + 1]);
+      auto put = [&](Vec u, const Vec& v, T* dx) {
+        E f[NE], d[NE];
+        both(u, v, f, d);
 #pragma unroll
-        for (int q = 0; q < V; ++q) {
-          f[q] = (f[q] - mean) * rs;
-          z[q] = fmaf(f[q], w[q], b[q]);
-        }
-        gn_act_grad<T, V>(z, d, a.act);
-#pragma unroll
-        for (int q = 0; q < V; ++q) f[q] = rs * (fmaf(d[q], w[q], -m1) - f[q] * m2);
-        u.set(f);
-        u.store(dx + i * ostep);
+        for (int q = 0; q < NE; ++q) f[q] = e_mul(rs, e_fma(f[q], m2, e_fma(d[q], w[q], m1)));
+        gn_set<T, V>(u, f);
+        u.store(dx);
       };
-      const int64_t have = a.cap > t ? (a.cap - t + k.tiles - 1) / k.tiles : 0;
-      int64_t i = mine - 1;
-      for (; i >= have + U - 1; i -= U) {
+      const int have = cap > t ? (cap - t + k.tiles - 1) / k.tiles : 0;
+      int i = gn_count(nr, k);
+      const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c + (int64_t)i * xstep;
+      const T* dy = (const T*)a.dy + (r0 + k.r) * a.lddy + c + (int64_t)i * dstep;
+      T* dx = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c + (int64_t)i * ostep;
+      for (; i - U >= have; i -= U) {
+        x -= U * xstep;
+        dy -= U * dstep;
+        dx -= U * ostep;
         Vec u[U], v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j].load(x + (i - j) * xstep), v[j].load(dy + (i - j) * dstep);
+        for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
 #pragma unroll
-        for (int j = 0; j < U; ++j) put(u[j], v[j], i - j);
+        for (int j = 0; j < U; ++j) put(u[j], v[j], dx + j * ostep);
       }
-      for (; i >= have; --i) {
+      for (; i > have; --i) {
+        x -= xstep;
+        dy -= dstep;
+        dx -= ostep;
         Vec u, v;
-        u.load(x + i * xstep);
-        v.load(dy + i * dstep);
-        put(u, v, i);
+        u.load(x);
+        v.load(dy);
+        put(u, v, dx);
       }
-      for (; i >= 0; --i) {
-        const int64_t at = i * k.tiles + t;
-        put(kept[2 * at * th], kept[(2 * at + 1) * th], i);
+      const Vec* kp = kept + 2 * (i * k.tiles + t) * th;
+      const int kstep = 2 * k.tiles * th;
+      for (; i > 0; --i) {
+        kp -= kstep;
+        dx -= ostep;
+        put(kp[0], kp[th], dx);
       }
     }
   }
   if (part && k.tiles == 1) {                     // over the rows of threads, in their order
-    float* cols = gn_smem;                        // [th] at a time
-#pragma unroll
-    for (int q = 0; q < 2 * V; ++q) {
-      __syncthreads();
-      cols[threadIdx.x] = q < V ? tw[q < V ? q : 0] : tb[q < V ? 0 : q - V];
-      __syncthreads();
-      if (k.on && k.r == 0) {
-        float v = 0.f;
-        for (int r = 0; r < k.tr; ++r) v += cols[r * k.tc + k.col];
-        part[(q < V ? 0 : a.c) + k.c0 + k.col * V + (q < V ? q : q - V)] = v;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * V * k.tc; i += th) {
+      const int q = i / k.tc, col = i - q * k.tc;
+      float v = 0.f;
+      for (int r = 0; r < k.tr; ++r) v += total[(int)(q * th + r * k.tc + col) - (int)threadIdx.x];
+      part[(q < V ? 0 : a.c) + k.c0 + col * V + (q < V ? q : q - V)] = v;
+    }
+  }
+  if (MODE == GN_WHOLE && P > 1) cluster_sync();
+}
+
+// The parts' sums of each sample and group, a warp each: forward (count, mean, squared deviations) to mean and rstd, backward (sums
+// of a and a xh) to their means
+__global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P, bool backward) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.n * a.groups; i += (int64_t)gridDim.x * 8) {
+    const int64_t s = i / a.groups;
+    const float* p = a.sums + s * P * 3 * a.groups + (i - s * a.groups);
+    const int64_t step = 3 * (int64_t)a.groups;
+    int64_t lo, hi;
+    const bool good = gn_range(a, s, lo, hi);
+    float u = 0.f, v = 0.f;
+    if (backward) {
+#pragma unroll 4
+      for (int q = lane; q < P; q += 32) u += p[q * step], v += p[q * step + a.groups];
+      const float inv = 1.f / ((float)(hi - lo) * (float)a.cg);
+      u = warp_sum(u) * inv;
+      v = warp_sum(v) * inv;
+    } else {
+      float n = 0.f, m2 = 0.f;
+#pragma unroll 4
+      for (int q = lane; q < P; q += 32) {
+        const float c = p[q * step];
+        n += c;
+        u = fmaf(c, p[q * step + a.groups], u);
+      }
+      n = warp_sum(n);
+      u = n > 0.f ? warp_sum(u) / n : 0.f;
+#pragma unroll 4
+      for (int q = lane; q < P; q += 32) {
+        const float c = p[q * step], d = p[q * step + a.groups] - u;
+        if (c > 0.f) m2 += fmaf(d * d, c, p[q * step + 2 * a.groups]);
+      }
+      m2 = warp_sum(m2);
+      const float bad = good ? 0.f : __int_as_float(0x7fc00000);
+      u += bad;
+      v = rsqrtf((n > 0.f ? m2 / n : 0.f) + a.eps) + bad;
+    }
+    if (lane == 0) {
+      a.stat[2 * i] = u;
+      a.stat[2 * i + 1] = v;
+      if (!backward && a.mean) {
+        a.mean[i] = u;
+        a.rstd[i] = v;
       }
     }
   }
-  if (P > 1) cluster_sync();
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// How a call is cut: column blocks of whole groups, CTAs of a cluster, threads, row steps in shared memory, clusters in flight
+// How a call is cut: groups of a column block, blocks, CTAs of a cluster (or parts), threads, row steps in shared memory, samples in
+// the grid
 struct GnCut {
-  int gpb, ncb, p, th, cap, smem;
+  int gpb, ncb, p, pshift, th, cap, smem;
   int64_t nz;
+  bool split;
 };
 
-// Row segments of a column block are 64 bytes at least (two sectors).  A CTA keeps up to GN_KEEP bytes, so that two fit an SM and
-// one loads while the other stores; a sample takes as many CTAs as hold it, and while the GPU is not full, more, down to 8 KB each.
-constexpr int GN_KEEP = 96 * 1024;
+// A CTA keeps up to this much, so that four (forward) or two (backward) fit an SM and some load while others store
+constexpr int GN_KEEP_FWD = 48 * 1024, GN_KEEP_BWD = 64 * 1024, GN_WHOLE_BYTES = 4 << 20, GN_START = 16384;
+
+// Row segments of a column block of the whole form: 64 bytes at least (two sectors)
+constexpr int GN_SEGMENT = 64;
+
+static int64_t gn_rows(const GnArgs& a) { return a.off ? (a.n ? (a.rows + a.n - 1) / a.n : 0) : a.len; }
+static int gn_blocks(const GnArgs& a, int size) {   // most column blocks of the whole form
+  const int per = (GN_SEGMENT + a.cg * size - 1) / (a.cg * size), n = a.groups / per;
+  return n < 1 ? 1 : n;
+}
+// Parts of a sample in the split form; 0: the whole form.  Sizes alone decide, so that the workspace's size does not hang on
+// addresses.
+static int gn_split(const GnArgs& a, int size, int slabs) {
+  const int64_t bytes = gn_rows(a) * a.c * size * slabs, keep = slabs == 1 ? GN_KEEP_FWD : GN_KEEP_BWD;
+  if (bytes <= keep || a.n * bytes <= GN_WHOLE_BYTES) return 0;
+  // the number whose rounds over the resident CTAs take least, a CTA's start and end as long as GN_START bytes of its rows
+  const int64_t all = (int64_t)(slabs == 1 ? GN_FWD_CTAS : GN_BWD_CTAS) * sm_count(), most = (4 * all + a.n - 1) / a.n;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t p = 1; p <= most && (p == 1 || bytes / p >= 4096); ++p) {
+    const double t = (double)((a.n * p + all - 1) / all) * ((double)bytes / (double)p + GN_START);
+    if (p == 1 || t < least) best = p, least = t;
+  }
+  return (int)best;
+}
+
 template <int V>
-static GnCut gn_cut(const GnArgs& a, int size, int slabs, int threads_max) {
+static GnCut gn_cut(const GnArgs& a, int size, int slabs, int threads_sm) {
+  const int keep = slabs == 1 ? GN_KEEP_FWD : GN_KEEP_BWD;
   GnCut k{};
-  const int64_t rows = a.off ? (a.n ? (a.rows + a.n - 1) / a.n : 0) : a.len;
-  const int64_t bytes = rows * a.c * size * slabs, sms = sm_count();
-  int64_t want = (bytes + GN_KEEP - 1) / GN_KEEP;
-  const int64_t fill = (2 * sms + a.n - 1) / a.n, least = bytes / 8192;
-  if (want < (fill < least ? fill : least)) want = fill < least ? fill : least;
-  if (want < 1) want = 1;
-  const int gmin = (64 + a.cg * size - 1) / (a.cg * size);      // groups of the narrowest block
-  int64_t ncb = a.groups / gmin < want ? a.groups / gmin : want;
-  if (ncb < 1) ncb = 1;
+  const int64_t rows = gn_rows(a), bytes = rows * a.c * size * slabs, sms = sm_count();
+  k.p = gn_split(a, size, slabs);
+  k.split = k.p > 0;
+  int64_t ncb;
+  if (k.split) {                                  // whole rows, or as wide blocks as one pass of a CTA's threads takes
+    ncb = (a.c / V + 255) / 256;
+  } else {
+    int64_t want = (bytes + keep - 1) / keep;
+    const int64_t fill = (2 * sms + a.n - 1) / a.n, least = bytes / 8192;
+    if (want < (fill < least ? fill : least)) want = fill < least ? fill : least;
+    ncb = gn_blocks(a, size);
+    if (ncb > want) ncb = want;
+    if (ncb < 1) ncb = 1;
+    k.p = 1;
+    while (k.p < 8 && k.p * ncb < want && rows >= 2 * k.p) k.p *= 2;
+    for (k.pshift = 0; (1 << k.pshift) < k.p; ++k.pshift) {}
+  }
+  if (ncb > a.groups) ncb = a.groups;
   k.gpb = (int)((a.groups + ncb - 1) / ncb);
-  // the per-group words of a block stay below 32 KB
-  if (k.gpb > 1024) k.gpb = 1024;
+  if (k.gpb > 1024) k.gpb = 1024;                 // words of its groups in shared memory
   k.ncb = (a.groups + k.gpb - 1) / k.gpb;
-  k.p = 1;
-  while (k.p < 8 && (int64_t)k.p * k.ncb < want && rows >= 2 * k.p) k.p *= 2;
   const int64_t slab = (rows + k.p - 1) / k.p * k.gpb * a.cg * size * slabs;
-  const int nvec = k.gpb * a.cg / V, acc = V * size;
-  k.th = slab <= 8192 ? 128 : slab <= 32768 ? 256 : threads_max;
-  while (k.th < threads_max && k.th < nvec && nvec > 128) k.th *= 2;
+  const int nvec = k.gpb * a.cg / V;
+  k.th = slab <= 8192 && nvec <= 128 ? 128 : 256;
   const int tiles = (nvec + k.th - 1) / k.th, tr = nvec < k.th ? k.th / nvec : 1;
   const int64_t steps = ((rows + k.p - 1) / k.p + tr - 1) / tr * tiles;
-  const int per = k.th * acc * slabs, most = GN_KEEP / per;
-  k.cap = (int)(steps < most ? steps : most);
-  k.smem = (int)((((2 * (size_t)k.th + 8 * (size_t)k.gpb + 3) & ~(size_t)3) * 4) + (size_t)k.cap * per);
+  const int per = k.th * V * size * slabs, most = keep / per;
+  k.cap = k.split ? 0 : (int)(steps < most ? steps : most);
+  k.smem = 4 * gn_shared_floats(k.th, k.gpb) + k.cap * per + (slabs == 2 ? 8 * V * k.th : 0);
+  // samples in the grid: all where a CTA has much to do, else what is resident (a CTA then goes over several)
+  int res = threads_sm / k.th;
+  const int by_smem = (220 * 1024) / (k.smem + 1024);
+  if (by_smem < res) res = by_smem;
+  if (res < 1) res = 1;
+  k.nz = (int64_t)res * sms / ((int64_t)k.p * k.ncb);
+  if (k.nz < 1) k.nz = 1;
+  if (slab >= 16384 && a.n * k.p <= 1024) k.nz = a.n;
+  if (k.nz > a.n) k.nz = a.n;
   return k;
 }
 
 template <auto KERN>
-static int gn_launch(GnArgs& a, GnCut& k, cudaStream_t st, const char* what) {
+static int gn_launch(GnArgs& a, const GnCut& k, cudaStream_t st, const char* what) {
   static int ready_dev = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch(what);
@@ -622,6 +907,7 @@ static int gn_launch(GnArgs& a, GnCut& k, cudaStream_t st, const char* what) {
   }
   a.gpb = k.gpb;
   a.cap = k.cap;
+  a.pshift = k.pshift;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(k.p, k.ncb, (unsigned)k.nz);
   cfg.blockDim = dim3(k.th);
@@ -632,19 +918,9 @@ static int gn_launch(GnArgs& a, GnCut& k, cudaStream_t st, const char* what) {
   at[0].val.clusterDim.x = k.p;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = k.p > 1 ? 1 : 0;
+  cfg.numAttrs = !k.split && k.p > 1 ? 1 : 0;
   cudaLaunchKernelEx(&cfg, KERN, a);
   return check_launch(what);
-}
-
-// Clusters in flight: what threads (registers) and shared memory let be resident, and no more than there are samples
-static int64_t gn_depth(const GnArgs& a, const GnCut& k, int threads_sm) {
-  int per = threads_sm / k.th;
-  const int by_smem = (220 * 1024) / (k.smem + 1024);
-  if (by_smem < per) per = by_smem;
-  if (per < 1) per = 1;
-  const int64_t ctas = (int64_t)k.p * k.ncb, z = ((int64_t)per * sm_count() + ctas - 1) / ctas;
-  return z < a.n ? z : a.n;
 }
 
 // Elements of an access: 16 or 8 bytes where they divide a group and everything is aligned to them, else one
@@ -657,14 +933,21 @@ static int gn_vec(const GnArgs& a, int size) {
   return 1;
 }
 
-constexpr int GN_FWD_THREADS = 512, GN_FWD_SM = 1024, GN_BWD_THREADS = 256, GN_BWD_SM = 512;
+static int gn_join(const GnArgs& a, int p, bool backward, cudaStream_t st) {
+  const int64_t want = (a.n * a.groups + 7) / 8, most = 8 * (int64_t)sm_count();
+  k_gn_join<<<(unsigned)(want < most ? want : most), 256, 0, st>>>(a, p, backward);
+  return check_launch("group_norm");
+}
+
+constexpr int GN_FWD_SM = 256 * GN_FWD_CTAS, GN_BWD_SM = 256 * GN_BWD_CTAS;
 
 template <typename T, int V>
 static int gn_fwd_go(GnArgs& a, cudaStream_t st) {
-  GnCut k = gn_cut<V>(a, sizeof(T), 1, GN_FWD_THREADS);
-  k.nz = gn_depth(a, k, GN_FWD_SM);
-  if (k.nz < 1) k.nz = 1;
-  return gn_launch<k_gn_fwd<T, V>>(a, k, st, "group_norm_fwd");
+  const GnCut k = gn_cut<V>(a, sizeof(T), 1, GN_FWD_SM);
+  if (!k.split) return gn_launch<k_gn_fwd<GN_WHOLE, T, V>>(a, k, st, "group_norm_fwd");
+  if (int rc = gn_launch<k_gn_fwd<GN_SUMS, T, V>>(a, k, st, "group_norm_fwd")) return rc;
+  if (int rc = gn_join(a, k.p, false, st)) return rc;
+  return gn_launch<k_gn_fwd<GN_APPLY, T, V>>(a, k, st, "group_norm_fwd");
 }
 template <typename T>
 static int gn_fwd_any(GnArgs& a, cudaStream_t st) {
@@ -674,11 +957,14 @@ static int gn_fwd_any(GnArgs& a, cudaStream_t st) {
 }
 template <typename T, int V>
 static int gn_bwd_go(GnArgs& a, int64_t* parts, bool launch, cudaStream_t st) {
-  GnCut k = gn_cut<V>(a, sizeof(T), 2, GN_BWD_THREADS);
-  k.nz = gn_depth(a, k, GN_BWD_SM);
-  if (k.nz < 1) k.nz = 1;
+  const GnCut k = gn_cut<V>(a, sizeof(T), 2, GN_BWD_SM);
   *parts = k.nz * k.p;
-  return launch ? gn_launch<k_gn_bwd<T, V>>(a, k, st, "group_norm_bwd") : 0;
+  if (!launch) return 0;
+  if (!k.split) return gn_launch<k_gn_bwd<GN_WHOLE, T, V>>(a, k, st, "group_norm_bwd");
+  if (int rc = gn_launch<k_gn_bwd<GN_SUMS, T, V>>(a, k, st, "group_norm_bwd")) return rc;
+  if (!a.out) return 0;
+  if (int rc = gn_join(a, k.p, true, st)) return rc;
+  return gn_launch<k_gn_bwd<GN_APPLY, T, V>>(a, k, st, "group_norm_bwd");
 }
 template <typename T>
 static int gn_bwd_any(GnArgs& a, int64_t* parts, bool launch, cudaStream_t st) {
@@ -711,6 +997,7 @@ static GnArgs gn_args(const void* x, int64_t ldx, const void* w, const void* b, 
   a.x = x; a.w = w; a.b = b; a.off = offsets; a.off64 = off64;
   a.ldx = ldx; a.rows = rows; a.n = n; a.len = len; a.c = c; a.groups = groups; a.act = act;
   a.cg = groups > 0 ? c / groups : 0;
+  a.pvec = aligned16(w) && aligned16(b);
   a.p32 = ptype == MB_F32;
   return a;
 }
@@ -724,43 +1011,57 @@ static int gn_type(int dtype, const F& f) {
 
 using namespace mb;
 
-extern "C" int mace_b200_group_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, const void* offsets,
-                                        int32_t offsets64, void* y, float* mean, float* rstd, int64_t rows, int64_t n,
-                                        int64_t len, int32_t c, int32_t groups, double eps, int32_t act, int32_t dtype,
-                                        int32_t ptype, void* stream) {
-  GnArgs a = gn_args(x, ldx, w, b, offsets, offsets64, rows, n, len, c, groups, act, ptype);
-  if (int rc = gn_check("group_norm_fwd", a, dtype, ptype)) return rc;
-  if (rows > 0 && (!x || !y || !mean != !rstd)) {
-    set_error("group_norm_fwd: null pointer");
+// Floats of the split form's sums, and rows of partial sums of the parameters' gradients there can be
+static int64_t gn_sums(const GnArgs& a, int size, int slabs) {
+  const int64_t p = a.n ? gn_split(a, size, slabs) : 0;
+  return p ? a.n * (3 * p + 2) * (int64_t)a.groups : 0;
+}
+static void gn_place(GnArgs& a, float* ws, int size, int slabs) {
+  a.sums = ws;
+  a.stat = ws && a.n ? ws + a.n * gn_split(a, size, slabs) * 3 * (int64_t)a.groups : nullptr;
+}
+static int64_t gn_parts(const GnArgs& a, int size) {
+  const int64_t split = gn_split(a, size, 2), most = (int64_t)(GN_BWD_SM / 128) * (sm_count() > 0 ? sm_count() : 1);
+  const int64_t all = a.n * (split ? split : 8), some = most > 1024 ? most : 1024;
+  return all < some + 8 || split ? all : some + 8;
+}
+
+extern "C" int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups, int32_t ragged,
+                                              int32_t dtype, int32_t backward, int64_t* floats) {
+  GnArgs a = gn_args(nullptr, c, nullptr, nullptr, ragged ? "" : nullptr, 0, rows, n, len, c, groups, MB_ACT_NONE, MB_F32);
+  if (int rc = gn_check("group_norm_workspace", a, dtype, MB_F32)) return rc;
+  if (!floats) {
+    set_error("group_norm_workspace: null pointer");
     return MB_E_ARG;
   }
+  const int size = dtype_size(dtype);
+  *floats = n == 0 || rows == 0 ? 0 : gn_sums(a, size, backward ? 2 : 1) + (backward ? 2 * (int64_t)c * gn_parts(a, size) : 0);
+  return 0;
+}
+
+extern "C" int mace_b200_group_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, const void* offsets,
+                                        int32_t offsets64, void* y, float* mean, float* rstd, float* workspace, int64_t rows,
+                                        int64_t n, int64_t len, int32_t c, int32_t groups, double eps, int32_t act,
+                                        int32_t dtype, int32_t ptype, void* stream) {
+  GnArgs a = gn_args(x, ldx, w, b, offsets, offsets64, rows, n, len, c, groups, act, ptype);
+  if (int rc = gn_check("group_norm_fwd", a, dtype, ptype)) return rc;
   if (sm_count() < 1) {
     set_error("group_norm_fwd: no CUDA device");
     return MB_E_CUDA;
   }
+  if (rows > 0 && (!x || !y || !mean != !rstd || (!workspace && gn_sums(a, dtype_size(dtype), 1) > 0))) {
+    set_error("group_norm_fwd: null pointer");
+    return MB_E_ARG;
+  }
   a.out = y; a.mean = mean; a.rstd = rstd; a.eps = (float)eps;
-  if (n == 0 && rows > 0) {                       // rows of no sample
+  gn_place(a, workspace, dtype_size(dtype), 1);
+  if (rows == 0) return 0;
+  if (n == 0) {                                   // rows of no sample
     if (cudaMemsetAsync(y, 0, (size_t)rows * c * dtype_size(dtype), (cudaStream_t)stream) != cudaSuccess)
       return check_launch("group_norm_fwd");
     return 0;
   }
-  if (n == 0) return 0;
   return gn_type(dtype, [&](auto t) { return gn_fwd_any<decltype(t)>(a, (cudaStream_t)stream); });
-}
-
-// Rows of partial sums there can be: a cluster of at most 8 CTAs for each sample, or what is resident and one cluster more
-static int64_t gn_parts(int64_t n) {
-  const int64_t most = (int64_t)(GN_BWD_SM / 128) * (sm_count() > 0 ? sm_count() : 1) + 8;
-  return 8 * n < most ? 8 * n : most;
-}
-
-extern "C" int mace_b200_group_norm_bwd_workspace(int64_t n, int32_t c, int64_t* floats) {
-  if (n < 0 || c < 1 || !floats) {
-    set_error("group_norm_bwd_workspace: bad arguments (samples %lld, channels %d)", (long long)n, c);
-    return MB_E_ARG;
-  }
-  *floats = 2 * (int64_t)c * gn_parts(n);
-  return 0;
 }
 
 extern "C" int mace_b200_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b,
@@ -769,22 +1070,25 @@ extern "C" int mace_b200_group_norm_bwd(const void* dy, int64_t lddy, const void
                                         int32_t groups, int32_t act, int32_t dtype, int32_t ptype, void* stream) {
   GnArgs a = gn_args(x, ldx < lddy ? ldx : lddy, w, b, offsets, offsets64, rows, n, len, c, groups, act, ptype);
   if (int rc = gn_check("group_norm_bwd", a, dtype, ptype)) return rc;
-  if ((rows > 0 && (!dy || !x)) || (n > 0 && (!mean || !rstd)) || ((dw || db) && !workspace)) {
-    set_error("group_norm_bwd: null pointer");
-    return MB_E_ARG;
-  }
   if (sm_count() < 1) {
     set_error("group_norm_bwd: no CUDA device");
     return MB_E_CUDA;
   }
+  const bool work = n > 0 && rows > 0 && (dx || dw || db);
+  if (work && (!dy || !x || !mean || !rstd || !workspace)) {
+    set_error("group_norm_bwd: null pointer");
+    return MB_E_ARG;
+  }
   a.ldx = ldx; a.lddy = lddy; a.dy = dy; a.out = dx; a.mean = (float*)mean; a.rstd = (float*)rstd;
-  a.partial = dw || db ? workspace : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   int64_t parts = 0;
   if (n == 0 && rows > 0 && dx && cudaMemsetAsync(dx, 0, (size_t)rows * c * dtype_size(dtype), st) != cudaSuccess)
     return check_launch("group_norm_bwd");
-  if (n > 0 && rows > 0 && (dx || a.partial)) {
-    const int64_t most = gn_parts(n);
+  if (work) {
+    const int size = dtype_size(dtype);
+    gn_place(a, workspace, size, 2);
+    a.partial = dw || db ? workspace + gn_sums(a, size, 2) : nullptr;
+    const int64_t most = gn_parts(a, size);
     if (int rc = gn_type(dtype, [&](auto t) { return gn_bwd_any<decltype(t)>(a, &parts, false, st); })) return rc;
     if (parts > most) {
       set_error("group_norm_bwd: %lld rows of partial sums, room for %lld", (long long)parts, (long long)most);
@@ -792,6 +1096,6 @@ extern "C" int mace_b200_group_norm_bwd(const void* dy, int64_t lddy, const void
     }
     if (int rc = gn_type(dtype, [&](auto t) { return gn_bwd_any<decltype(t)>(a, &parts, true, st); })) return rc;
   }
-  if (!a.partial) return 0;
-  return col_sums(workspace, (int)parts, c, dw, db, ptype, st);
+  if (!dw && !db) return 0;
+  return col_sums(a.partial, (int)parts, c, dw, db, ptype, st);
 }

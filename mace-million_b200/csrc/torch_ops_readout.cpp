@@ -52,6 +52,13 @@ GnIn gn_in(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, co
   return a;
 }
 
+Tensor gn_workspace(const GnIn& a, int64_t groups, bool backward, const Tensor& like) {
+  int64_t floats = 0;
+  check_rc(mace_b200_group_norm_workspace(a.r, a.n, a.len, (int32_t)a.c, (int32_t)groups, a.off.defined(), a.dt, backward, &floats),
+           "group_norm");
+  return floats ? at::empty({floats}, like.options().dtype(at::kFloat)) : Tensor();
+}
+
 std::tuple<Tensor, Tensor, Tensor> gn_forward(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps,
                                               int64_t act, const Tensor& offsets, bool stats) {
   GnIn a = gn_in(x, groups, w, b, offsets, act);
@@ -62,11 +69,13 @@ std::tuple<Tensor, Tensor, Tensor> gn_forward(const Tensor& x, int64_t groups, c
     mean = at::empty({a.n, groups}, x.options().dtype(at::kFloat));
     rstd = at::empty({a.n, groups}, x.options().dtype(at::kFloat));
   }
-  if (a.r)
+  if (a.r) {
+    Tensor ws = gn_workspace(a, groups, false, x);
     check_rc(mace_b200_group_norm_fwd(a.rows.data_ptr(), row_stride(a.rows), ptr(a.w), ptr(a.b), ptr(a.off), a.off64,
-                                      y.data_ptr(), ptr_as<float>(mean), ptr_as<float>(rstd), a.r, a.n, a.len, (int32_t)a.c,
-                                      (int32_t)groups, eps, (int32_t)act, a.dt, a.pt, stream_of(x)),
+                                      y.data_ptr(), ptr_as<float>(mean), ptr_as<float>(rstd), ptr_as<float>(ws), a.r, a.n, a.len,
+                                      (int32_t)a.c, (int32_t)groups, eps, (int32_t)act, a.dt, a.pt, stream_of(x)),
              "group_norm");
+  }
   return {y, mean, rstd};
 }
 
@@ -96,11 +105,7 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& dy, const Tensor
   auto popt = x.options().dtype(a.pt == MB_F32 ? at::kFloat : x.scalar_type());
   Tensor dx = need_x ? at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous) : Tensor();
   Tensor dw = need_w ? at::empty({a.c}, popt) : Tensor(), db = need_b ? at::empty({a.c}, popt) : Tensor(), ws;
-  if (need_w || need_b) {
-    int64_t words = 0;
-    check_rc(mace_b200_group_norm_bwd_workspace(a.n, (int32_t)a.c, &words), "group_norm_bwd");
-    ws = at::empty({words > 0 ? words : 1}, x.options().dtype(at::kFloat));
-  }
+  if (need_x || need_w || need_b) ws = gn_workspace(a, groups, true, x);
   Tensor g = a.r ? rows_of(dy) : dy;
   if (a.r || need_w || need_b)
     check_rc(mace_b200_group_norm_bwd(ptr(g), a.r ? row_stride(g) : a.c, ptr(a.rows), a.r ? row_stride(a.rows) : a.c, ptr(a.w),
