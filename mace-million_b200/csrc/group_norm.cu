@@ -875,7 +875,10 @@ static GnCut gn_cut(const GnArgs& a, int size, int slabs, int threads_sm) {
   k.ncb = (a.groups + k.gpb - 1) / k.gpb;
   const int64_t slab = (rows + k.p - 1) / k.p * k.gpb * a.cg * size * slabs;
   const int nvec = k.gpb * a.cg / V;
-  k.th = slab <= 8192 && nvec <= 128 ? 128 : 256;
+  // about 16 vectors a thread where there are CTAs enough (what a thread does once a sample is as much as 30 of them), else 4; a
+  // thread for each vector column, too.  4,000 samples of 60 x 128 bf16: 256 threads 61 us, a warp a sample of 3 x 128 a third.
+  const int64_t vecs = slab / (V * size * slabs), each = a.n * k.p * k.ncb >= 4 * sms ? 16 : 4;
+  for (k.th = 32; k.th < 256 && (k.th * each < vecs || k.th < nvec); k.th *= 2) {}
   const int tiles = (nvec + k.th - 1) / k.th, tr = nvec < k.th ? k.th / nvec : 1;
   const int64_t steps = ((rows + k.p - 1) / k.p + tr - 1) / tr * tiles;
   const int per = k.th * V * size * slabs, most = keep / per;
@@ -1021,7 +1024,7 @@ static void gn_place(GnArgs& a, float* ws, int size, int slabs) {
   a.stat = ws && a.n ? ws + a.n * gn_split(a, size, slabs) * 3 * (int64_t)a.groups : nullptr;
 }
 static int64_t gn_parts(const GnArgs& a, int size) {
-  const int64_t split = gn_split(a, size, 2), most = (int64_t)(GN_BWD_SM / 128) * (sm_count() > 0 ? sm_count() : 1);
+  const int64_t split = gn_split(a, size, 2), most = (int64_t)(GN_BWD_SM / 32) * (sm_count() > 0 ? sm_count() : 1);
   const int64_t all = a.n * (split ? split : 8), some = most > 1024 ? most : 1024;
   return all < some + 8 || split ? all : some + 8;
 }
