@@ -3,7 +3,7 @@
 // The sums are exact in int32 (k <= MB_INT8_MAX_K), y is fp32 arithmetic on them, rounded once.  q is the nearest whole number
 // of the exact quotient, ties to even (a remainder by fma corrects the rounded quotient), so it does not depend on who divides.
 //
-// Three kernels.  k_quant_rows: a warp per row.  k_int8_few: up to 8 tokens; a CTA quantizes them into shared memory while its
+// Three kernels.  k_quant_rows: a row stays in the registers of 32 to 512 threads, read once.  k_int8_few: up to 4 tokens; a CTA quantizes them into shared memory while its
 // first weights are on their way, then each warp takes whole rows of w with dp4a: bound by the weights' bytes and latency.
 // k_int8_gemm: tcgen05 kind::i8 from TMA tiles (SWIZZLE_128B, 128 bytes of K a stage).  Output channels are the rows of an MMA
 // and tokens its columns: few tokens take a narrow tile, a lane holds one channel (its scale and bias stay in registers), and
@@ -21,15 +21,18 @@
 
 namespace mb {
 
-// Scale of a row, its reciprocal, and the power of two that keeps both normal (a tiny row's scale is subnormal)
+// Scale of a row, its reciprocal, and the power of two that keeps both normal (a tiny row's scale is subnormal); half: half of the
+// scale where the short way of q8x4 holds, else NaN
 struct Q8 {
-  float s, inv, up;
+  float scale, s, inv, up, half;
 };
 __device__ __forceinline__ Q8 q8_of(float scale) {
   Q8 k;
+  k.scale = scale;
   k.up = scale < 0x1p-100f ? 0x1p60f : 1.f;
   k.s = scale * k.up;
   k.inv = 1.f / k.s;
+  k.half = scale >= 0x1p-100f && scale < 0x1p120f ? 0.5f * scale : __int_as_float(0x7fc00000);
   return k;
 }
 // nearest(x / scale) of the exact quotient, in [-127, 127]; 0 where the scale is 0 or not finite
@@ -45,56 +48,164 @@ __device__ __forceinline__ int q8(float x, const Q8& k) {
   q = fminf(fmaxf(q, -127.f), 127.f);
   return s > 0.f && s < INFINITY && x == x ? (int)q : 0;
 }
+// Four of them as bytes.  Usually the rounded quotient is the one: x inv + 1.5 2^23 has it in its low bits, and the remainder shows
+// that it is (|x - q s| < s / 2; ties, tiny and unusual scales fail that and take the long way).
 __device__ __forceinline__ uint32_t q8x4(const float* f, const Q8& k) {
-  return (uint32_t)(q8(f[0], k) & 255) | (uint32_t)(q8(f[1], k) & 255) << 8 |
-         (uint32_t)(q8(f[2], k) & 255) << 16 | (uint32_t)q8(f[3], k) << 24;
+  constexpr float MAGIC = 12582912.f;
+  const float2 inv = make_float2(k.inv, k.inv), big = make_float2(MAGIC, MAGIC), less = make_float2(-MAGIC, -MAGIC);
+  const float2 neg = make_float2(-k.s, -k.s), a = make_float2(f[0], f[1]), b = make_float2(f[2], f[3]);
+  const float2 ta = __ffma2_rn(a, inv, big), tb = __ffma2_rn(b, inv, big);
+  const float2 ra = __ffma2_rn(__fadd2_rn(ta, less), neg, a), rb = __ffma2_rn(__fadd2_rn(tb, less), neg, b);
+  const float m = fmaxf(fmaxf(fabsf(ra.x), fabsf(ra.y)), fmaxf(fabsf(rb.x), fabsf(rb.y)));
+  if (m < k.half)
+    return __byte_perm(__byte_perm(__float_as_uint(ta.x), __float_as_uint(ta.y), 0x0040),
+                       __byte_perm(__float_as_uint(tb.x), __float_as_uint(tb.y), 0x0040), 0x5410);
+  return (uint32_t)(q8(f[0], k) & 255) | (uint32_t)(q8(f[1], k) & 255) << 8 | (uint32_t)(q8(f[2], k) & 255) << 16 |
+         (uint32_t)q8(f[3], k) << 24;
 }
 // max |x| that NaN passes through
 __device__ __forceinline__ float top_of(float m, float v) {
-  v = fabsf(v);
-  return m >= v || m != m ? m : v;
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
 }
 __device__ __forceinline__ float warp_top(float m) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = top_of(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
+// of a 16-byte vector: two 16-bit elements at a time
+__device__ __forceinline__ float top16(const uint4& u, float) {
+  return top_of(top_of(fabsf(__uint_as_float(u.x)), __uint_as_float(u.y)), top_of(fabsf(__uint_as_float(u.z)), __uint_as_float(u.w)));
+}
+template <typename T2>
+__device__ __forceinline__ T2 top_pair(const uint4& u) {
+  const T2 a = *reinterpret_cast<const T2*>(&u.x), b = *reinterpret_cast<const T2*>(&u.y), c = *reinterpret_cast<const T2*>(&u.z),
+           d = *reinterpret_cast<const T2*>(&u.w);
+  return __hmax2_nan(__hmax2_nan(__habs2(a), __habs2(b)), __hmax2_nan(__habs2(c), __habs2(d)));
+}
+__device__ __forceinline__ float top16(const uint4& u, bf16) {
+  const __nv_bfloat162 m = top_pair<__nv_bfloat162>(u);
+  return top_of(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float top16(const uint4& u, f16) {
+  const __half2 m = top_pair<__half2>(u);
+  return top_of(__low2float(m), __high2float(m));
+}
 __device__ __forceinline__ float q8_scale(float top) { return __fdiv_rn(top, 127.f); }
 
-// V elements an access: 16 bytes, or 1 element where rows are not aligned.  Bytes up to ldq that hold no value are zero.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) k_quant_rows(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
-                                                    float* __restrict__ scale, int64_t rows, int32_t k) {
+// Largest value of the G threads of a group (a block of 256 or G threads; `red` is one buffer of two that calls alternate)
+template <int G>
+__device__ __forceinline__ float group_top(float m, float* red) {
+  m = warp_top(m);
+  if constexpr (G > 32) {
+    constexpr int W = G / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = red[warp / W * W + (lane & (W - 1))];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) m = top_of(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
+  return m;
+}
+
+template <int G>
+constexpr int q8_threads = G < 256 ? 256 : G;
+// Rows of whole aligned vectors that G threads hold, NV vectors each: read once.  Bytes up to ldq that hold no value are zero.
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(q8_threads<G>) k_quant_rows(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q,
+                                                              int64_t ldq, float* __restrict__ scale, int64_t rows, int32_t k) {
+  constexpr int V = kVec<T>, RPB = q8_threads<G> / G;
+  __shared__ float red[2][q8_threads<G> / 32];
+  const int t = threadIdx.x % G, g = threadIdx.x / G;
+  int buf = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, buf ^= 1) {
+    const int64_t row = r0 + g;
+    const T* p = x + (row < rows ? row : r0) * ldx;
+    uint4 u[NV];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * G + t) * V;
+      u[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (j < k) u[i] = *reinterpret_cast<const uint4*>(p + j);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = top_of(top, top16(u[i], T()));
+    top = group_top<G>(top, red[buf]);
+    if (row >= rows) continue;
+    const Q8 qk = q8_of(q8_scale(top));
+    if (t == 0) scale[row] = qk.scale;
+    int8_t* o = q + row * ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * G + t) * V;
+      if (j >= ldq) continue;
+      float f[V];
+      unpack16(u[i], f, T());
+      if constexpr (V == 8)
+        *reinterpret_cast<uint2*>(o + j) = make_uint2(q8x4(f, qk), q8x4(f + 4, qk));
+      else
+        *reinterpret_cast<uint32_t*>(o + j) = q8x4(f, qk);
+    }
+  }
+}
+
+// Any rows, a warp each, an element an access and four neighbours a lane.  NV > 0: up to 128 NV values stay in registers; else the
+// row is read twice (the second time from L1 or L2).  words: rows of q are aligned to four bytes.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) k_quant_any(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+                                                   float* __restrict__ scale, int64_t rows, int32_t k, bool words) {
   const int lane = threadIdx.x & 31;
   const int64_t step = (int64_t)gridDim.x * 8;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += step) {
     const T* p = x + row * ldx;
-    float top = 0.f;
-#pragma unroll 4
-    for (int j = lane * V; j < k; j += 32 * V) {
-      float f[V];
-      load_v<T, V>(p + j, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = top_of(top, f[i]);
-    }
-    top = warp_top(top);
-    const float s = q8_scale(top);
-    const Q8 qk = q8_of(s);
-    if (lane == 0) scale[row] = s;
     int8_t* o = q + row * ldq;
-    if constexpr (V == 1) {
-      for (int j = lane; j < ldq; j += 32) o[j] = j < k ? (int8_t)q8(to_f(p[j]), qk) : (int8_t)0;
-    } else {
-#pragma unroll 4
-      for (int j = lane * V; j < ldq; j += 32 * V) {   // ldq is a multiple of 16, k of V
-        float f[V];
+    float top = 0.f;
+    auto put = [&](int j, const float (&f)[4], const Q8& qk) {
+      const uint32_t w = q8x4(f, qk);
+      if (words) {
+        if (j < ldq) *reinterpret_cast<uint32_t*>(o + j) = w;
+      } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = 0.f;
-        if (j < k) load_v<T, V>(p + j, f);
-        if constexpr (V == 8)
-          *reinterpret_cast<uint2*>(o + j) = make_uint2(q8x4(f, qk), q8x4(f + 4, qk));
-        else
-          *reinterpret_cast<uint32_t*>(o + j) = q8x4(f, qk);
+        for (int i = 0; i < 4; ++i)
+          if (j + i < ldq) o[j + i] = (int8_t)(w >> (8 * i));
+      }
+    };
+    if constexpr (NV > 0) {
+      T v[NV][4];
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 128 * n + 4 * lane + i;
+          v[n][i] = from_f<T>(0.f);
+          if (j < k) v[n][i] = p[j];
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = top_of(top, to_f(v[n][i]));
+      const Q8 qk = q8_of(q8_scale(warp_top(top)));
+      if (lane == 0) scale[row] = qk.scale;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const float f[4] = {to_f(v[n][0]), to_f(v[n][1]), to_f(v[n][2]), to_f(v[n][3])};
+        put(128 * n + 4 * lane, f, qk);
+      }
+      for (int j = 128 * NV + lane; j < ldq; j += 32) o[j] = 0;
+    } else {
+#pragma unroll 8
+      for (int j = lane; j < k; j += 32) top = top_of(top, to_f(p[j]));
+      const Q8 qk = q8_of(q8_scale(warp_top(top)));
+      if (lane == 0) scale[row] = qk.scale;
+#pragma unroll 2
+      for (int64_t j = 4 * lane; j < ldq; j += 128) {
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = j + i < k ? to_f(p[j + i]) : 0.f;
+        put((int)j, f, qk);
       }
     }
   }
@@ -158,9 +269,8 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
       float m = red[t][lane & 7];
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) m = top_of(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float s = q8_scale(m);
-      const Q8 qk = q8_of(s);
-      if (tid == 0) sc[t] = s;
+      const Q8 qk = q8_of(q8_scale(m));
+      if (tid == 0) sc[t] = qk.scale;
       if (t >= a.t) {
         for (int j = tid; j < kv; j += 256) qs[t * kv + j] = make_uint4(0u, 0u, 0u, 0u);
         continue;
@@ -259,29 +369,13 @@ struct I8Cfg {
 struct I8Bars {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   uint32_t tmem;
-  int failed;
+  int failed, never;                             // never: a flag that stays 0
 };
 
 // kind::i8: D int32 (bits 4-5 = 2), A and B signed 8-bit (1 at bits 7-9 and 10-12), both K-major
 __host__ __device__ constexpr uint32_t i8_idesc(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-template <int CG>
-__device__ __forceinline__ void mma_i8_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CG == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate));
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate));
-}
-
 template <typename T, int CG>
 __global__ void __launch_bounds__(I8_THREADS, 1)
     k_int8_gemm(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const I8Args g) {
@@ -303,7 +397,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         mbar_init(&B.acc_full[a], 1);
         mbar_init(&B.acc_empty[a], I8_EPI * CG);
       }
-      B.failed = 0;
+      B.failed = B.never = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -315,112 +409,140 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
   const int tiles = g.tm * (int)((g.t + g.bn - 1) / g.bn), nk = (g.k + I8_BK - 1) / I8_BK, bh = g.bn / CG;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int seq = 0;
-      bool ok = true;
-      const uint32_t bytes = CG * (uint32_t)(C::A_BYTES + bh * I8_BK);
-      for (int t = cta; ok && t < tiles; t += ctas) {
-        const int n0 = t / g.tm, m0 = (t - n0 * g.tm) * (128 * CG) + rank * 128;
-        for (int kb = 0; kb < nk; ++kb, ++seq) {
-          const int s = seq % C::STAGES;
-          if (*failed || !mbar_wait_ns(&B.empty[s], ((seq / C::STAGES) & 1) ^ 1, I8_WAIT)) {
-            *failed = 1;
-            ok = false;
-            break;
-          }
-          const uint32_t bar = CG == 2 ? mapa_u32(smem_u32(&B.full[s]), 0) : smem_u32(&B.full[s]);
-          if (rank == 0) mbar_arrive_tx(&B.full[s], bytes);
-          const uint32_t a = smem_u32(smem + s * C::STAGE);
-          tma_load_2d<CG>(a, &map_w, kb * I8_BK, m0, bar);
-          tma_load_2d<CG>(a + C::A_BYTES, &map_q, kb * I8_BK, n0 * g.bn + rank * bh, bar);
+    const uint32_t lead = elect_lane(), smem0 = smem_u32(smem), full0 = smem_u32(B.full), empty0 = smem_u32(B.empty);
+    const uint32_t target = CG == 2 ? mapa_u32(full0, 0) : full0, bytes = CG * (uint32_t)(C::A_BYTES + bh * I8_BK);
+    const int tm = g.tm;
+    int s = 0;
+    uint32_t par = 1;
+    bool ok = true, wrapped = false;
+    for (int t = cta; ok && t < tiles; t += ctas) {
+      const int tn = t / tm, m0 = (t - tn * tm) * (128 * CG) + rank * 128, n0 = tn * g.bn + rank * bh;
+      for (int kb = 0; kb < nk; ++kb) {
+        if (!mbar_wait_warp(empty0 + 8 * s, par, I8_WAIT, failed)) {
+          *failed = 1;
+          ok = false;
+          break;
         }
+        const uint32_t a = smem0 + s * C::STAGE;
+        // both CTAs' bytes arrive at the first one's barrier
+        mbar_arrive_tx_lead(rank == 0 ? lead : 0u, full0 + 8 * s, bytes);
+        tma_load_2d_lead<CG>(lead, a, &map_w, kb * I8_BK, m0, target + 8 * s);
+        tma_load_2d_lead<CG>(lead, a + C::A_BYTES, &map_q, kb * I8_BK, n0, target + 8 * s);
+        if (++s == C::STAGES) s = 0, par ^= 1, wrapped = true;
       }
-      if (!ok && rank == 0)                      // copies in flight land before the block ends (bounded)
-        for (int q = seq - C::STAGES < 0 ? 0 : seq - C::STAGES; q < seq; ++q)
-          mbar_wait_ns(&B.full[q % C::STAGES], (q / C::STAGES) & 1, I8_WAIT);
     }
+    if (!ok && rank == 0)                        // copies in flight land before the block ends (bounded)
+      for (int q = 0; q < C::STAGES; ++q) {      // places before s: this round's, the others: the round before
+        if (q >= s && !wrapped) break;
+        mbar_wait_ns(&B.full[q], q < s ? par ^ 1 : par, I8_WAIT);
+      }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const uint32_t lead = elect_lane(), smem0 = smem_u32(smem), full0 = smem_u32(B.full), empty0 = smem_u32(B.empty);
+      const uint32_t acc_full0 = smem_u32(B.acc_full), acc_empty0 = smem_u32(B.acc_empty);
       const uint32_t idesc = i8_idesc(128 * CG, g.bn);
-      int seq = 0, tc = 0;
+      const uint64_t a_base = sw128_desc(smem0), b_base = sw128_desc(smem0 + C::A_BYTES);
+      int s = 0, acc = 0;
+      uint32_t par = 0, acc_par = 1, last_bar = 0, last_par = 0;
       bool ok = true;
-      uint64_t* last_bar = nullptr;
-      uint32_t last_par = 0;
-      for (int t = cta; ok && t < tiles; t += ctas, ++tc) {
-        const int acc = tc & 1;
-        if (*failed || !mbar_wait_ns(&B.acc_empty[acc], ((tc >> 1) & 1) ^ 1, I8_WAIT)) {
+      for (int t = cta; ok && t < tiles; t += ctas) {
+        if (!mbar_wait_warp(acc_empty0 + 8 * acc, acc_par, I8_WAIT, failed)) {
           *failed = 1;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int kb = 0; kb < nk; ++kb, ++seq) {
-          const int s = seq % C::STAGES;
-          if (!mbar_wait_ns(&B.full[s], (seq / C::STAGES) & 1, I8_WAIT)) {
+        const uint32_t d = tmem + acc * 256;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait_warp(full0 + 8 * s, par, I8_WAIT, failed)) {
             *failed = 1;
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+          const uint64_t off = (uint64_t)((uint32_t)(s * C::STAGE) >> 4);
 #pragma unroll
           for (int kk = 0; kk < I8_BK / 32; ++kk)
-            mma_i8_ss<CG>(tmem + acc * 256, sw128_desc(a + kk * 32), sw128_desc(b + kk * 32), idesc, (kb | kk) ? 1u : 0u);
-          mma_commit_to<CG>(&B.empty[s]);
-          last_bar = &B.empty[s];
-          last_par = (seq / C::STAGES) & 1;
+            mma_i8_ss_lead<CG>(lead, d, a_base + off + kk * 2, b_base + off + kk * 2, idesc, (kb | kk) ? 1u : 0u);
+          mma_commit_lead<CG>(lead, empty0 + 8 * s);
+          last_bar = empty0 + 8 * s;
+          last_par = par;
+          if (++s == C::STAGES) s = 0, par ^= 1;
         }
         if (!ok) break;
-        mma_commit_to<CG>(&B.acc_full[acc]);
-        last_bar = &B.acc_full[acc];
-        last_par = (tc >> 1) & 1;
+        mma_commit_lead<CG>(lead, acc_full0 + 8 * acc);
+        last_bar = acc_full0 + 8 * acc;
+        last_par = acc_par ^ 1;
+        acc ^= 1;
+        if (acc == 0) acc_par ^= 1;
       }
-      if (*failed && last_bar) mbar_wait_ns(last_bar, last_par, I8_WAIT);
+      if (*failed && last_bar) mbar_wait_warp(last_bar, last_par, I8_WAIT, &B.never);
     }
   } else if (warp >= I8_EPI0) {
-    const int q4 = warp & 3, hf = (warp - I8_EPI0) >> 2, hw = g.bn / 2;
-    int tc = 0;
+    const int q4 = warp & 3, hf = (warp - I8_EPI0) >> 2, hw = g.bn / 2, tm = g.tm, n_all = g.n;
+    const int64_t tokens = g.t;
+    int acc = 0;
+    uint32_t acc_par = 0;
     bool lost = false;                           // warp-uniform
-    for (int t = cta; t < tiles; t += ctas, ++tc) {
-      const int tn = t / g.tm, acc = tc & 1;
-      const int n = (t - tn * g.tm) * (128 * CG) + rank * 128 + q4 * 32 + lane;
-      const bool on = n < g.n;
-      float ws = on ? g.ws[n] : 0.f;
+    for (int t = cta; t < tiles; t += ctas) {
+      const int tn = t / tm, n = (t - tn * tm) * (128 * CG) + rank * 128 + q4 * 32 + lane;
+      const int64_t first = (int64_t)tn * g.bn + hf * hw;
+      const bool on = n < n_all;
+      // this lane's channel, and the scales of the half's tokens (lane l holds those of l, 32 + l, ..), on their way during the wait
+      float ws = on ? g.ws[n] : 0.f, xs[4];
       const float b = !on || !g.bias ? 0.f : g.b32 ? ((const float*)g.bias)[n] : to_f(((const T*)g.bias)[n]);
-      if (!lost) {
-        lost = __shfl_sync(0xffffffffu, *failed, 0) || !__all_sync(0xffffffffu, mbar_wait_ns(&B.acc_full[acc], (tc >> 1) & 1, I8_WAIT));
-        if (lost) *failed = 1;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int q = 0; q < 4; ++q) xs[q] = 32 * q + lane < hw && first + 32 * q + lane < tokens ? g.xs[first + 32 * q + lane] : 0.f;
+      if (!lost) lost = !mbar_wait_warp(smem_u32(&B.acc_full[acc]), acc_par, I8_WAIT, failed);
+      if (lost) {
+        *failed = 1;
+        ws = __int_as_float(0x7fc00000);
       }
-      if (lost) ws = __int_as_float(0x7fc00000);
-      for (int c = 0; c < hw; c += 32) {
-        const int64_t t0 = (int64_t)tn * g.bn + hf * hw + c;
-        const int w = hw - c < 32 ? hw - c : 32, left = g.t - t0 < w ? (int)(g.t - t0) : w;   // tokens here
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      T* y = (T*)g.y + first * n_all + n;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * q;
+        if (c >= hw) break;
+        const int w = hw - c < 32 ? hw - c : 32;
+        const int64_t rest = tokens - first - c;
+        const int left = rest < w ? (int)rest : w;             // tokens here (<= 0: none)
         uint32_t u[32];
         if (!lost) {
           tmem_ld32(tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * 256 + hf * hw + c), u);
           tmem_wait_ld();
+          if (c + 32 >= hw) {                    // the accumulator is free
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 2)
+                mbar_arrive_remote(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
+              else
+                mbar_arrive(&B.acc_empty[acc]);
+            }
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) u[i] = 0;
         }
-        if (c + 32 >= hw && !lost) {             // the accumulator is free
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 2)
-              mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
-            else
-              mbar_arrive(&B.acc_empty[acc]);
+        // the tokens' rows one after the other, 32 neighbouring channels a store
+        if (left == 32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float v = fmaf((float)(int)u[i] * __shfl_sync(0xffffffffu, xs[q], i), ws, b);
+            if (on) *y = from_f<T>(v);
+            y += n_all;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float v = fmaf((float)(int)u[i] * __shfl_sync(0xffffffffu, xs[q], i), ws, b);
+            if (i < left && on) *y = from_f<T>(v);
+            y += n_all;
           }
         }
-        const float xs = lane < left ? g.xs[t0 + lane] : 0.f;
-        T* y = (T*)g.y + t0 * g.n + n;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float s = __shfl_sync(0xffffffffu, xs, i);
-          if (i < left && on) y[(int64_t)i * g.n] = from_f<T>(fmaf((float)(int)u[i] * s, ws, b));
-        }
       }
+      acc ^= 1;
+      if (acc == 0) acc_par ^= 1;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -434,20 +556,41 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+template <typename T, int G, int NV>
+static int quant_held(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int32_t k, cudaStream_t st) {
+  constexpr int RPB = q8_threads<G> / G;
+  const int64_t want = (rows + RPB - 1) / RPB, most = (2048 / q8_threads<G>) * (int64_t)sm_count();
+  k_quant_rows<T, G, NV><<<(unsigned)(want < most ? want : most), q8_threads<G>, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k);
+  return check_launch("quantize_rows");
+}
 template <typename T>
 static int quant_go(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int32_t k, cudaStream_t st) {
   constexpr int V = kVec<T>;
-  const bool vec = k % V == 0 && ldx % V == 0 && aligned16(x) && ldq % 16 == 0 && aligned16(q);
+  if (k % V == 0 && ldx % V == 0 && aligned16(x) && ldq % 16 == 0 && aligned16(q)) {   // (the pad of ldq < k + 16 is held, too)
+    const int64_t nv = (ldq + V - 1) / V;
+    if (ldq < k + 16) {
+      if (nv <= 32) return quant_held<T, 32, 1>(x, ldx, q, ldq, scale, rows, k, st);
+      if (nv <= 64) return quant_held<T, 32, 2>(x, ldx, q, ldq, scale, rows, k, st);
+      if (nv <= 128) return quant_held<T, 32, 4>(x, ldx, q, ldq, scale, rows, k, st);
+      if (nv <= 512) return quant_held<T, 128, 4>(x, ldx, q, ldq, scale, rows, k, st);
+      if (nv <= 2048) return quant_held<T, 512, 4>(x, ldx, q, ldq, scale, rows, k, st);
+    }
+  }
   const int64_t want = (rows + 7) / 8, most = 8 * (int64_t)sm_count();
+  const bool words = ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
   const unsigned grid = (unsigned)(want < most ? want : most);
-  if (vec)
-    k_quant_rows<T, V><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k);
+  if (k <= 256)
+    k_quant_any<T, 2><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
+  else if (k <= 640)
+    k_quant_any<T, 5><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
+  else if (k <= 1024)
+    k_quant_any<T, 8><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
   else
-    k_quant_rows<T, 1><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k);
+    k_quant_any<T, 0><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
   return check_launch("quantize_rows");
 }
 
-constexpr int I8_FEW = 8, I8_FEW_SMEM = 128 * 1024;   // most tokens of k_int8_few, most bytes of them
+constexpr int I8_FEW = 4, I8_FEW_SMEM = 128 * 1024;   // most tokens of k_int8_few, most bytes of them
 
 template <typename T, int TT, int R>
 static int few_go(const I8Args& a, cudaStream_t st) {
@@ -472,8 +615,7 @@ static int few_any(const I8Args& a, cudaStream_t st) {
   const bool wide = a.n >= 32 * sm_count();       // rows enough for several a warp
   if (a.t <= 1) return wide ? few_go<T, 1, 4>(a, st) : few_go<T, 1, 1>(a, st);
   if (a.t <= 2) return wide ? few_go<T, 2, 4>(a, st) : few_go<T, 2, 1>(a, st);
-  if (a.t <= 4) return wide ? few_go<T, 4, 4>(a, st) : few_go<T, 4, 1>(a, st);
-  return wide ? few_go<T, 8, 4>(a, st) : few_go<T, 8, 1>(a, st);
+  return wide ? few_go<T, 4, 4>(a, st) : few_go<T, 4, 1>(a, st);
 }
 
 template <typename T, int CG>
@@ -492,9 +634,16 @@ static int i8_go(I8Args a, cudaStream_t st) {
   }
   const int units = sm_count() / CG;
   a.tm = (a.n + 128 * CG - 1) / (128 * CG);
-  // the widest tile of tokens that leaves every SM one, 32 at least
-  a.bn = 256;
-  while (a.bn > 32 && (int64_t)a.tm * ((a.t + a.bn - 1) / a.bn) < units) a.bn /= 2;
+  // the tile of tokens whose rounds over the SMs take least: a tile's products (2 cycles a column and K block, 300 a K block at
+  // least) or its drain (40 cycles a column), whichever is longer, and what a tile costs besides
+  const int nk = (a.k + I8_BK - 1) / I8_BK;
+  double least = 0.0;
+  for (int bn = 256; bn >= 32 * CG; bn -= 32 * CG) {
+    const int64_t t = (int64_t)a.tm * ((a.t + bn - 1) / bn);
+    const double mma = (double)nk * (2 * bn > 300 ? 2 * bn : 300), drain = 40.0 * bn;
+    const double cost = (double)((t + units - 1) / units) * ((mma > drain ? mma : drain) + 800);
+    if (bn == 256 || cost <= least) least = cost, a.bn = bn;
+  }
   const int64_t tiles = (int64_t)a.tm * ((a.t + a.bn - 1) / a.bn);
   if (tiles > 0x7fffffff) {
     set_error("int8_linear: too many tiles (%lld)", (long long)tiles);
@@ -556,7 +705,7 @@ extern "C" int mace_b200_quantize_rows(const void* x, int64_t ldx, int8_t* q, in
 }
 
 extern "C" int mace_b200_int8_linear_few(int64_t tokens, int32_t k) {
-  return tokens <= I8_FEW && (tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8) * (int64_t)((k + 15) & ~15) <= I8_FEW_SMEM;
+  return tokens <= I8_FEW && (tokens <= 1 ? 1 : tokens <= 2 ? 2 : 4) * (int64_t)((k + 15) & ~15) <= I8_FEW_SMEM;
 }
 
 extern "C" int mace_b200_int8_linear(const void* x, int64_t ldx, int8_t* xq, int64_t ldq, float* xscale, const int8_t* wq,

@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
               __syncwarp();
               if (lane == 0) {
                 if constexpr (CG == 2)
-                  mbar_arrive_cluster(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
+                  mbar_arrive_remote(mapa_u32(smem_u32(&B.acc_empty[acc]), 0));
                 else
                   mbar_arrive(&B.acc_empty[acc]);
               }

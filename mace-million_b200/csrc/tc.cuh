@@ -157,6 +157,11 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// without waiting for the thread's own stores to memory, as the release at cluster scope above does: what it signals is a read of
+// TMEM, which tcgen05.fence::before_thread_sync orders
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -352,6 +357,26 @@ __device__ __forceinline__ void tma_load_4d_lead(uint32_t lead, uint32_t dst, co
         "[%2];\n\t}\n" ::"r"(dst),
         "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(lead)
         : "memory");
+}
+
+// One MMA of signed 8-bit operands, both K-major in shared memory, int32 accumulator in TMEM
+template <int CG>
+__device__ __forceinline__ void mma_i8_ss_lead(uint32_t lead, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead));
 }
 
 }  // namespace mb
