@@ -458,7 +458,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
             ok = false;
             break;
           }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint64_t off = (uint64_t)((uint32_t)(s * C::STAGE) >> 4);
 #pragma unroll
           for (int kk = 0; kk < I8_BK / 32; ++kk)

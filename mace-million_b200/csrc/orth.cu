@@ -281,13 +281,14 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
       const CUtensorMap *ma = &maps.a[(ph / 3) & 1][ph % 3], *mb = &maps.b[(ph / 3) & 1][ph % 3];
       const uint32_t bytes = CG * (uint32_t)(2 + bh / 64) * OR_BOX;
       const int adx = p.a_mn ? 0 : OR_BK, ady = p.a_mn ? OR_BK : 0, bdx = p.b_mn ? 0 : OR_BK, bdy = p.b_mn ? OR_BK : 0;
+      OrTile w{};
+      if (cta < tiles) w = or_tile(p, cta);       // before the wait, not after it
       if (ph > 0) {
         ok = or_wait(g, ph - 1);
         if (!ok) *failed = 1;
         if (lead) mbar_arrive(&B.phase);          // the epilogue may read what the phase before wrote
       }
       for (int t = cta; ok && t < tiles; t += ctas) {
-        const OrTile w = or_tile(p, t);
         // coordinates: K-major (k, row, 0, matrix), MN-major (0, k, column / 64, matrix)
         const int m0 = w.m0 + rank * 128, n0 = w.n0 + rank * bh;
         int ax = 0, ay = p.a_mn ? 0 : m0, bx = 0, by = p.b_mn ? 0 : n0;
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
           by += bdy;
           if (++s == stages) s = 0, par ^= 1, wrapped = true;
         }
+        if (t + ctas < tiles) w = or_tile(p, t + ctas);
       }
     }
     if (!ok && rank == 0)                         // copies in flight land before the block ends (bounded)
@@ -349,7 +351,6 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
               ok = false;
               break;
             }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t off = (uint64_t)((uint32_t)(s * stage_bytes) >> 4), ad = a_base + off, bd = b_base + off;
 #pragma unroll
             for (int kk = 0; kk < OR_BK / 16; ++kk)

@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
   __shared__ OsShared S;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = gridDim.x, rank = blockIdx.x;
-  const int row = (warp & 3) * 32 + lane, half = warp >> 2, ls = g.ls;
+  // rp: columns of A that are worked on, 64 where that is enough (with one CTA)
+  const int row = (warp & 3) * 32 + lane, half = warp >> 2, ls = g.ls, rp = g.r <= 64 && P == 1 ? 64 : 128;
   const uint32_t plane = smem_u32(smem), xs = plane + 2 * OS_BLOCK;   // A1 / B1, X, partial sums
   const uint32_t sums = xs + ls / 64 * OS_BLOCK;
   const uint32_t cols = ls == 64 ? 256u : ls == 128 ? 256u : 512u;
@@ -75,6 +76,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
+  if (tid < 128) S.d[tid] = S.e[tid] = 0.f;       // (rows from rp on have none)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -128,11 +130,23 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       }
     }
     __syncwarp();
+    // 32 squares in fp32 where they neither overflow nor vanish, else in fp64
+    float s32 = 0.f, top = 0.f;
 #pragma unroll
     for (int x = 0; x < 32; ++x) {
-      sq = fma((double)f[x], (double)f[x], sq);
+      s32 = fmaf(f[x], f[x], s32);
+      top = fmaxf(top, fabsf(f[x]));
       u[x] = __float_as_uint(f[x]);
     }
+    if (top > 1e-15f && top < 1e15f)
+      sq += (double)s32;
+    else
+#pragma unroll
+      for (int x = 0; x < 32; ++x) {
+        const double v = __uint_as_float(u[x]);
+        sq = fma(v, v, sq);
+      }
+    __syncwarp();
     tmem_st32(tx + lanes + h0 + c, u);
   }
   tmem_wait_st();
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
     ++phase;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   };
-  const uint32_t id128 = f16_idesc(128, 128, false, false, false), id_x = f16_idesc(128, ls, false, false, true);
+  const uint32_t id_a = f16_idesc(128, rp, false, false, false), id_x = f16_idesc(128, ls, false, false, true);
 
   for (int step = 0; step < g.poly.steps; ++step) {
     const float ca = g.poly.a[step], cb = g.poly.b[step], cc = g.poly.c[step];
@@ -206,14 +220,14 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
     products([&](uint32_t lead) {
       for (int k = 0; k < ls / 16; ++k) {
         const uint64_t a = sw128_desc(xs + (k >> 2) * OS_BLOCK + (k & 3) * 32);
-        mma_f16_ss_lead<1>(lead, td, a, a, id128, k ? 1u : 0u);
+        mma_f16_ss_lead<1>(lead, td, a, a, id_a, k ? 1u : 0u);
       }
     });
     // eight columns of A at a time: the diagonal apart (dia: the column among them, or outside of 0 .. 7), the rest to the plane
     const float sc = g.poly.inv_s * g.poly.inv_s * OR_SA;
     if (P == 1) {
 #pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      for (int c = half * (rp / 2); c < (half + 1) * (rp / 2); c += 32) {
         uint32_t u[32];
         float v[32];
         tmem_ld32(td + lanes + c, u);
@@ -236,7 +250,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       __syncthreads();
     } else {
 #pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      for (int c = half * (rp / 2); c < (half + 1) * (rp / 2); c += 32) {
         uint32_t u[32];
         tmem_ld32(td + lanes + c, u);
         tmem_wait_ld();
@@ -294,17 +308,16 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
     }
     // -------------------------------------------------------------------------------------------- b A + c A A
     products([&](uint32_t lead) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < rp / 16; ++k) {
         const uint64_t a = sw128_desc(plane + (k >> 2) * OS_BLOCK + (k & 3) * 32);
-        mma_f16_ss_lead<1>(lead, td, a, a, id128, k ? 1u : 0u);
+        mma_f16_ss_lead<1>(lead, td, a, a, id_a, k ? 1u : 0u);
       }
     });
     {
       // b a1 + c (a1 (d_i + d_j) + sq), all times SB: a1's plane is SA a1, the accumulator SA^2 sq
       const float di = S.d[row], k2 = cc * (OR_SB / OR_SA), k1 = fmaf(k2, di, cb * (OR_SB / OR_SA)), k3 = cc * (OR_SB / (OR_SA * OR_SA));
 #pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      for (int c = half * (rp / 2); c < (half + 1) * (rp / 2); c += 32) {
         uint32_t u[32];
         float v[32];
         tmem_ld32(td + lanes + c, u);
@@ -339,8 +352,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
     }
     // -------------------------------------------------------------------------------------------- X <- a X + (b A + c A A) X
     products([&](uint32_t lead) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < rp / 16; ++k)
         mma_f16_ss_lead<1>(lead, td, sw128_desc(plane + (k >> 2) * OS_BLOCK + (k & 3) * 32), sw128_desc_mn(xs + k * 2048, OS_BLOCK), id_x,
                            k ? 1u : 0u);
     });
