@@ -1037,6 +1037,10 @@ extern "C" int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t l
     set_error("group_norm_workspace: null pointer");
     return MB_E_ARG;
   }
+  if (sm_count() < 1) {
+    set_error("group_norm_workspace: no CUDA device");
+    return MB_E_CUDA;
+  }
   const int size = dtype_size(dtype);
   *floats = n == 0 || rows == 0 ? 0 : gn_sums(a, size, backward ? 2 : 1) + (backward ? 2 * (int64_t)c * gn_parts(a, size) : 0);
   return 0;

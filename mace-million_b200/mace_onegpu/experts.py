@@ -225,11 +225,9 @@ class ExpertBlock(torch.nn.Module):
         return load
 
 
-def train_readout(n=8, n_experts=8, k=2, hidden=64, steps=200, lr=3e-3, dtype=torch.float32, seed=0):
-    """Trains an ExpertBlock to give the per-atom energies of the model from its layer-1 scalar features H1[:, 0e] of a
-    water box of 3 n^3 atoms (random-init weights).  Returns a dict of what happened."""
-    import time
-
+def water_features(n, dtype, seed=0):
+    """Layer-1 scalar features H1[:, 0e] [3 n^3, 128] (rows 512 apart) of a water box under the random-init model, and the model's
+    per-atom energies [3 n^3, 1], centred and scaled to deviation one."""
     from . import model as M
     from . import neighbors, structures
     from .engine import ThreePassEngine
@@ -244,9 +242,42 @@ def train_readout(n=8, n_experts=8, k=2, hidden=64, steps=200, lr=3e-3, dtype=to
     h1 = eng.node_features(plan)
     e = eat.double()
     target = ((e - e.mean()) / e.std()).float()[:, None].to(dtype)
-    x = h1.to(dtype)[:, 0]                          # the 0e block: rows 512 apart
+    return h1.to(dtype)[:, 0], target
+
+
+class _Together:
+    """Several optimisers as one."""
+
+    def __init__(self, *opts):
+        self.opts = opts
+
+    def zero_grad(self):
+        for o in self.opts:
+            o.zero_grad()
+
+    def step(self):
+        for o in self.opts:
+            o.step()
+
+
+def train_readout(n=8, n_experts=8, k=2, hidden=64, steps=200, lr=3e-3, dtype=torch.float32, seed=0, optimizer="adam",
+                  lr_matrices=0.02):
+    """Trains an ExpertBlock to give the per-atom energies of the model from its layer-1 scalar features H1[:, 0e] of a
+    water box of 3 n^3 atoms (random-init weights).  optimizer: "adam", or "muon" for the experts' matrices and the router (with
+    lr_matrices) and Adam for the rest.  Returns a dict of what happened."""
+    import time
+
+    if optimizer not in ("adam", "muon"):
+        raise ValueError(f"optimizer must be 'adam' or 'muon' (got {optimizer!r})")
+    x, target = water_features(n, dtype, seed)
     block = ExpertBlock(128, hidden, 1, n_experts, k, dtype=dtype, seed=seed)
-    opt = torch.optim.Adam(block.parameters(), lr=lr)
+    if optimizer == "muon":
+        from . import optim
+
+        opt = _Together(optim.Muon([p for p in block.parameters() if p.dim() >= 2], lr=lr_matrices),
+                        torch.optim.Adam([p for p in block.parameters() if p.dim() < 2], lr=lr))
+    else:
+        opt = torch.optim.Adam(block.parameters(), lr=lr)
     losses = []
     t0 = time.perf_counter()
     for _ in range(steps):
@@ -259,7 +290,7 @@ def train_readout(n=8, n_experts=8, k=2, hidden=64, steps=200, lr=3e-3, dtype=to
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     block.plan.check()
-    return {"atoms": len(Z), "experts": n_experts, "k": k, "steps": steps, "dtype": str(dtype).split(".")[-1],
+    return {"atoms": len(x), "experts": n_experts, "k": k, "steps": steps, "dtype": str(dtype).split(".")[-1],
             "loss_first": float(losses[0]), "loss_last": float(losses[-1]), "steps_per_s": steps / dt,
             "load": [int(v) for v in load.tolist()]}
 
@@ -276,8 +307,11 @@ def main():
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--lr", type=float, default=3e-3)
     ap.add_argument("--dtype", default="float32", choices=["float32", "bfloat16", "float16"])
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"], help="muon: for the matrices, Adam for the rest")
+    ap.add_argument("--lr-matrices", type=float, default=0.02, help="of the matrices with --optimizer muon")
     a = ap.parse_args()
-    print(json.dumps(train_readout(a.n, a.experts, a.k, a.hidden, a.steps, a.lr, getattr(torch, a.dtype))))
+    print(json.dumps(train_readout(a.n, a.experts, a.k, a.hidden, a.steps, a.lr, getattr(torch, a.dtype), optimizer=a.optimizer,
+                                   lr_matrices=a.lr_matrices)))
 
 
 if __name__ == "__main__":
