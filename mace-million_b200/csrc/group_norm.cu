@@ -103,6 +103,23 @@ struct GnVec {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Word*>(p) = u; }
 };
 
+// Rows on their way through a thread's own places in shared memory (GN_SUMS and GN_APPLY): more bytes in flight than registers hold.
+// Elements of two bytes alone cannot be copied so.
+constexpr int GN_RING = 8;
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// fp32 rows forward are as fast through registers (1,029,000 x 128 267 us, through the ring 295; bf16 64 x 2048 x 512 94 and 76).
+template <int MODE, typename T, int V, bool BWD>
+constexpr bool gn_ring = MODE != GN_WHOLE && V * sizeof(T) >= 4 && (BWD || sizeof(T) == 2);
+
 // V elements as Elem<V> (packed pairs where V > 1) and back
 template <typename T, int V>
 __device__ __forceinline__ void gn_get(const GnVec<T, V>& v, Elem<V> (&e)[kElems<V>]) {
@@ -342,17 +359,43 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
         };
         int64_t left = nr - k.r;                  // rows from this thread's next one on
         int i = 0;
-        for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * step, i += U) {
-          Vec u[U];
+        if constexpr (gn_ring<MODE, T, V, false>) {
+          const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
+          int64_t todo = left;
+          auto issue = [&](int d) {
+            if (left > 0) {
+              copy_async<sizeof(Vec)>(ring + d * place, x);
+              x += step;
+              left -= k.tr;
+            }
+            copy_commit();
+          };
 #pragma unroll
-          for (int j = 0; j < U; ++j) u[j].load(x + j * step);
+          for (int d = 0; d < GN_RING; ++d) issue(d);
+          while (todo > 0) {
 #pragma unroll
-          for (int j = 0; j < U; ++j) add(u[j]);
-        }
-        for (; left > 0; left -= k.tr, x += step, ++i) {
-          Vec u;
-          u.load(x);
-          add(u);
+            for (int d = 0; d < GN_RING; ++d) {
+              if (todo <= 0) break;
+              copy_wait<GN_RING - 1>();
+              add(kept[d * th]);
+              issue(d);
+              todo -= k.tr;
+              ++i;
+            }
+          }
+        } else {
+          for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * step, i += U) {
+            Vec u[U];
+  #pragma unroll
+            for (int j = 0; j < U; ++j) u[j].load(x + j * step);
+  #pragma unroll
+            for (int j = 0; j < U; ++j) add(u[j]);
+          }
+          for (; left > 0; left -= k.tr, x += step, ++i) {
+            Vec u;
+            u.load(x);
+            add(u);
+          }
         }
         // V channels to (mean, squared deviations) of mine * V values
         mine = (float)i;
@@ -486,21 +529,47 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
       int i = gn_count(nr, k);
       const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c + (int64_t)i * step;   // one row behind the next
       T* y = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c + (int64_t)i * ystep;
-      for (; i - U >= have; i -= U) {
-        x -= U * step;
-        y -= U * ystep;
-        Vec u[U];
+      if constexpr (gn_ring<MODE, T, V, false>) {
+        const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
+        int left = i;
+        auto issue = [&](int d) {
+          if (left > 0) {
+            x -= step;
+            copy_async<sizeof(Vec)>(ring + d * place, x);
+            --left;
+          }
+          copy_commit();
+        };
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j].load(x + j * step);
+        for (int d = 0; d < GN_RING; ++d) issue(d);
+        while (i > 0) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) put(u[j], y + j * ystep);
-      }
-      for (; i > have; --i) {
-        x -= step;
-        y -= ystep;
-        Vec u;
-        u.load(x);
-        put(u, y);
+          for (int d = 0; d < GN_RING; ++d) {
+            if (i <= 0) break;
+            copy_wait<GN_RING - 1>();
+            y -= ystep;
+            put(kept[d * th], y);
+            issue(d);
+            --i;
+          }
+        }
+      } else {
+        for (; i - U >= have; i -= U) {
+          x -= U * step;
+          y -= U * ystep;
+          Vec u[U];
+  #pragma unroll
+          for (int j = 0; j < U; ++j) u[j].load(x + j * step);
+  #pragma unroll
+          for (int j = 0; j < U; ++j) put(u[j], y + j * ystep);
+        }
+        for (; i > have; --i) {
+          x -= step;
+          y -= ystep;
+          Vec u;
+          u.load(x);
+          put(u, y);
+        }
       }
       const Vec* kp = kept + (i * k.tiles + t) * th;
       const int kstep = k.tiles * th;
@@ -531,7 +600,7 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
   Vec* kept = reinterpret_cast<Vec*>(gn_smem + gn_shared_floats(th, a.gpb)) + threadIdx.x;
   if (MODE != GN_SUMS) gn_clear<T>(a);
   // sums of dz xh and dz over the samples (one tile of columns): a thread's own places behind the kept rows
-  float* total = gn_smem + gn_shared_floats(th, a.gpb) + (size_t)2 * cap * th * V * sizeof(T) / 4 + threadIdx.x;
+  float* total = gn_smem + gn_shared_floats(th, a.gpb) + (size_t)2 * (gn_ring<MODE, T, V, true> ? GN_RING : cap) * th * V * sizeof(T) / 4 + threadIdx.x;
   if (MODE != GN_APPLY && k.tiles == 1)
 #pragma unroll
     for (int q = 0; q < 2 * V; ++q) total[q * th] = 0.f;
@@ -596,18 +665,45 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
           }
         };
         int64_t left = nr - k.r;
-        for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * xstep, dy += U * dstep) {
-          Vec u[U], v[U];
+        if constexpr (gn_ring<MODE, T, V, true>) {
+          const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
+          int64_t todo = left;
+          auto issue = [&](int d) {
+            if (left > 0) {
+              copy_async<sizeof(Vec)>(ring + 2 * d * place, x);
+              copy_async<sizeof(Vec)>(ring + (2 * d + 1) * place, dy);
+              x += xstep;
+              dy += dstep;
+              left -= k.tr;
+            }
+            copy_commit();
+          };
 #pragma unroll
-          for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
+          for (int d = 0; d < GN_RING; ++d) issue(d);
+          while (todo > 0) {
 #pragma unroll
-          for (int j = 0; j < U; ++j) add(u[j], v[j]);
-        }
-        for (; left > 0; left -= k.tr, x += xstep, dy += dstep) {
-          Vec u, v;
-          u.load(x);
-          v.load(dy);
-          add(u, v);
+            for (int d = 0; d < GN_RING; ++d) {
+              if (todo <= 0) break;
+              copy_wait<GN_RING - 1>();
+              add(kept[2 * d * th], kept[(2 * d + 1) * th]);
+              issue(d);
+              todo -= k.tr;
+            }
+          }
+        } else {
+          for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * xstep, dy += U * dstep) {
+            Vec u[U], v[U];
+  #pragma unroll
+            for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
+  #pragma unroll
+            for (int j = 0; j < U; ++j) add(u[j], v[j]);
+          }
+          for (; left > 0; left -= k.tr, x += xstep, dy += dstep) {
+            Vec u, v;
+            u.load(x);
+            v.load(dy);
+            add(u, v);
+          }
         }
         E p1 = e_splat<E>(0.f), p2 = p1;
 #pragma unroll
@@ -724,24 +820,52 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
       const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c + (int64_t)i * xstep;
       const T* dy = (const T*)a.dy + (r0 + k.r) * a.lddy + c + (int64_t)i * dstep;
       T* dx = (T*)a.out + (r0 + k.r) * (int64_t)a.c + c + (int64_t)i * ostep;
-      for (; i - U >= have; i -= U) {
-        x -= U * xstep;
-        dy -= U * dstep;
-        dx -= U * ostep;
-        Vec u[U], v[U];
+      if constexpr (gn_ring<MODE, T, V, true>) {
+        const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
+        int left = i;
+        auto issue = [&](int d) {
+          if (left > 0) {
+            x -= xstep;
+            dy -= dstep;
+            copy_async<sizeof(Vec)>(ring + 2 * d * place, x);
+            copy_async<sizeof(Vec)>(ring + (2 * d + 1) * place, dy);
+            --left;
+          }
+          copy_commit();
+        };
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
+        for (int d = 0; d < GN_RING; ++d) issue(d);
+        while (i > 0) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) put(u[j], v[j], dx + j * ostep);
-      }
-      for (; i > have; --i) {
-        x -= xstep;
-        dy -= dstep;
-        dx -= ostep;
-        Vec u, v;
-        u.load(x);
-        v.load(dy);
-        put(u, v, dx);
+          for (int d = 0; d < GN_RING; ++d) {
+            if (i <= 0) break;
+            copy_wait<GN_RING - 1>();
+            dx -= ostep;
+            put(kept[2 * d * th], kept[(2 * d + 1) * th], dx);
+            issue(d);
+            --i;
+          }
+        }
+      } else {
+        for (; i - U >= have; i -= U) {
+          x -= U * xstep;
+          dy -= U * dstep;
+          dx -= U * ostep;
+          Vec u[U], v[U];
+  #pragma unroll
+          for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
+  #pragma unroll
+          for (int j = 0; j < U; ++j) put(u[j], v[j], dx + j * ostep);
+        }
+        for (; i > have; --i) {
+          x -= xstep;
+          dy -= dstep;
+          dx -= ostep;
+          Vec u, v;
+          u.load(x);
+          v.load(dy);
+          put(u, v, dx);
+        }
       }
       const Vec* kp = kept + 2 * (i * k.tiles + t) * th;
       const int kstep = 2 * k.tiles * th;
@@ -837,13 +961,17 @@ static int gn_blocks(const GnArgs& a, int size) {   // most column blocks of the
 static int gn_split(const GnArgs& a, int size, int slabs) {
   const int64_t bytes = gn_rows(a) * a.c * size * slabs, keep = slabs == 1 ? GN_KEEP_FWD : GN_KEEP_BWD;
   if (bytes <= keep || a.n * bytes <= GN_WHOLE_BYTES) return 0;
-  // the number whose rounds over the resident CTAs take least, a CTA's start and end as long as GN_START bytes of its rows
-  const int64_t all = (int64_t)(slabs == 1 ? GN_FWD_CTAS : GN_BWD_CTAS) * sm_count(), most = (4 * all + a.n - 1) / a.n;
+  // the number whose rounds over the resident CTAs take least, a CTA's start and end as long as GN_START bytes of its rows: for each
+  // number of rounds the most parts that need no more
+  const int64_t all = (int64_t)(slabs == 1 ? GN_FWD_CTAS : GN_BWD_CTAS) * sm_count(), r0 = (a.n + all - 1) / all;
+  const int64_t most = bytes / 4096 > 1 ? bytes / 4096 : 1;
   int64_t best = 1;
   double least = 0.0;
-  for (int64_t p = 1; p <= most && (p == 1 || bytes / p >= 4096); ++p) {
-    const double t = (double)((a.n * p + all - 1) / all) * ((double)bytes / (double)p + GN_START);
-    if (p == 1 || t < least) best = p, least = t;
+  for (int64_t r = r0; r <= r0 + 4; ++r) {
+    int64_t p = r * all / a.n;
+    if (p > most) p = most;
+    const double t = (double)r * ((double)bytes / (double)p + GN_START);
+    if (r == r0 || t < least) best = p, least = t;
   }
   return (int)best;
 }
@@ -883,7 +1011,7 @@ static GnCut gn_cut(const GnArgs& a, int size, int slabs, int threads_sm) {
   const int64_t steps = ((rows + k.p - 1) / k.p + tr - 1) / tr * tiles;
   const int per = k.th * V * size * slabs, most = keep / per;
   k.cap = k.split ? 0 : (int)(steps < most ? steps : most);
-  k.smem = 4 * gn_shared_floats(k.th, k.gpb) + k.cap * per + (slabs == 2 ? 8 * V * k.th : 0);
+  k.smem = 4 * gn_shared_floats(k.th, k.gpb) + (k.split ? (V * size >= 4 && (slabs == 2 || size == 2) ? GN_RING : 0) : k.cap) * per + (slabs == 2 ? 8 * V * k.th : 0);
   // samples in the grid: all where a CTA has much to do, else what is resident (a CTA then goes over several)
   int res = threads_sm / k.th;
   const int by_smem = (220 * 1024) / (k.smem + 1024);
