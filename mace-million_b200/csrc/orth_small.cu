@@ -5,8 +5,8 @@
 //    shared memory in blocks of 64 columns (128-byte swizzled rows), which the Gram product reads K-major (K = l) and the update as
 //    its MN-major operand (K = r) from the same bytes.
 //  * A1, then b A + c A A over it, is one 128 x 128 plane in shared memory; each thread turns its own elements.
-//  * With several CTAs the Gram product's partial sums are added through distributed shared memory: each CTA adds a slice in the
-//    order of the ranks and stores it, rounded, to all.
+//  * With several CTAs the Gram product's partial sums are added through distributed shared memory: of two each adds the other's to
+//    its own (the same sums in both), of more each adds a slice in the order of the ranks and stores it, rounded, to all.
 // 256 threads: eight warps hold the rows (two halves of the columns), one thread issues the products between block barriers.
 // Bound: latency.  A step is three products of 8 to 16 MMAs and three passes over TMEM, each behind a barrier.
 #include <type_traits>
@@ -55,6 +55,18 @@ __device__ __forceinline__ void st_cluster_u32x4(uint32_t a, const uint4& v) {
 }
 __device__ __forceinline__ void st_cluster_f32(uint32_t a, float x) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
+}
+
+// The lane's own of its 32 values, which becomes 0 (selects: a store in a branch for each was ten times as long)
+__device__ __forceinline__ float os_diagonal(float (&v)[32], int lane) {
+  float d = 0.f;
+#pragma unroll
+  for (int x = 0; x < 32; ++x) {
+    const bool on = x == lane;
+    d = on ? v[x] : d;
+    v[x] = on ? 0.f : v[x];
+  }
+  return d;
 }
 
 template <typename T>
@@ -196,6 +208,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
   tmem_wait_st();
 
   int phase = 0;
+  bool pending = false;                           // an arrival at the cluster's barrier that was not waited for
   // What the threads wrote is there for the products; `issue` runs in one thread; all wait for its products (bounded)
   auto products = [&](auto issue) {
     asm volatile("fence.proxy.async;" ::: "memory");
@@ -234,11 +247,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
         tmem_wait_ld();
 #pragma unroll
         for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(u[x]) * sc;
-        if (c == (warp & 3) * 32) {               // the diagonal runs through this piece
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (x == lane) S.d[row] = v[x] * (1.f / OR_SA), v[x] = 0.f;
-        }
+        if (c == (warp & 3) * 32) S.d[row] = os_diagonal(v, lane) * (1.f / OR_SA);   // it runs through this piece
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float f[8];
@@ -249,6 +258,8 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       }
       __syncthreads();
     } else {
+      if (pending) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      pending = false;
 #pragma unroll 1
       for (int c = half * (rp / 2); c < (half + 1) * (rp / 2); c += 32) {
         uint32_t u[32];
@@ -259,7 +270,36 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
           sts128(sums + (uint32_t)((c / 4 + q) * 128 + row) * 16, make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]));
       }
       cluster_sync();
-      // 2048 / P pieces of eight columns of a row for this CTA: 8 / P for a thread
+      if (P == 2) {                               // each CTA adds all of the other's to its own
+        const uint32_t peer = mapa_u32(sums, rank ^ 1);
+#pragma unroll 1
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+          uint32_t u[32];
+          float v[32];
+          float4 t[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) t[q] = ld_cluster_f32x4(peer + (uint32_t)((c / 4 + q) * 128 + row) * 16);
+          tmem_ld32(td + lanes + c, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            v[4 * q] = (__uint_as_float(u[4 * q]) + t[q].x) * sc, v[4 * q + 1] = (__uint_as_float(u[4 * q + 1]) + t[q].y) * sc;
+            v[4 * q + 2] = (__uint_as_float(u[4 * q + 2]) + t[q].z) * sc, v[4 * q + 3] = (__uint_as_float(u[4 * q + 3]) + t[q].w) * sc;
+          }
+          if (c == (warp & 3) * 32) S.d[row] = os_diagonal(v, lane) * (1.f / OR_SA);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] = v[8 * q + x];
+            sts128(plane + os_piece(row, c / 8 + q), pack16<f16>(f));
+          }
+        }
+        // this CTA has read its peer's sums; it waits for its peer before it writes its own again
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        pending = true;
+      }
+      // else 2048 / P pieces of eight columns of a row for this CTA: 8 / P for a thread
       auto slice = [&](auto np) {
         constexpr int PP = decltype(np)::value, PER = 8 / PP;
         float f[PER][8];
@@ -298,13 +338,14 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
           }
         }
       };
-      if (P == 2)
-        slice(std::integral_constant<int, 2>());
-      else if (P == 4)
+      if (P == 4)
         slice(std::integral_constant<int, 4>());
-      else
+      else if (P == 8)
         slice(std::integral_constant<int, 8>());
-      cluster_sync();
+      if (P > 2)
+        cluster_sync();
+      else
+        __syncthreads();
     }
     // -------------------------------------------------------------------------------------------- b A + c A A
     products([&](uint32_t lead) {
@@ -335,11 +376,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
               v[8 * q + 4 * h + x] = fmaf(f[4 * h + x], fmaf(k2, t[x], k1), __uint_as_float(u[8 * q + 4 * h + x]) * k3);
           }
         }
-        if (c == (warp & 3) * 32) {
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (x == lane) S.e[row] = fmaf(cb, di, fmaf(cc * di, di, v[x] * (1.f / OR_SB))), v[x] = 0.f;
-        }
+        if (c == (warp & 3) * 32) S.e[row] = fmaf(cb, di, fmaf(cc * di, di, os_diagonal(v, lane) * (1.f / OR_SB)));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float f[8];
@@ -357,6 +394,7 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
                            k ? 1u : 0u);
     });
     const float el = ca + S.e[row];
+    if (last && pending) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (last) barrier();                          // every CTA's S.failed is final
     float bad = 0.f;
     if (last) {
@@ -383,9 +421,14 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
         for (int x = 0; x < 32; ++x) v[x] = fmaf(v[x], g.poly.inv_s, bad);
         if (g.tall) {
           o += (int64_t)j0 * g.n + row;
+          if (nc >= 32) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (x < nc) o[(int64_t)x * g.n] = from_f<bf16>(v[x]);
+            for (int x = 0; x < 32; ++x) o[(int64_t)x * g.n] = from_f<bf16>(v[x]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (x < nc) o[(int64_t)x * g.n] = from_f<bf16>(v[x]);
+          }
         } else {
           o += (int64_t)row * g.n + j0;
           if (nc >= 32 && g.n % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0) {
