@@ -363,6 +363,7 @@ int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_
  * mean / rstd [n][groups] are written when not null (both or none); the backward pass reads them.
  * bwd: dx (may be null) dense; dw / db [c] of type ptype (may be null), summed in a fixed order.
  * workspace: mace_b200_group_norm_workspace floats (may be null where that is 0; ragged: with offsets). */
+#define MB_GN_MAX_GROUPS (1 << 24)
 enum { MB_ACT_NONE = 0, MB_ACT_SILU = 1, MB_ACT_GELU = 2, MB_ACT_RELU = 3 };
 int mace_b200_group_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, const void* offsets, int32_t offsets64,
                              void* y, float* mean, float* rstd, float* workspace, int64_t rows, int64_t n, int64_t len,

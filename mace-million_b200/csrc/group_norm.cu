@@ -1105,7 +1105,7 @@ static int gn_bwd_any(GnArgs& a, int64_t* parts, bool launch, cudaStream_t st) {
 }
 
 static int gn_check(const char* who, const GnArgs& a, int32_t dtype, int32_t ptype) {
-  if (a.rows < 0 || a.n < 0 || a.c < 1 || a.groups < 1 || a.c % a.groups || a.ldx < a.c ||
+  if (a.rows < 0 || a.n < 0 || a.c < 1 || a.groups < 1 || a.groups > MB_GN_MAX_GROUPS || a.c % a.groups || a.ldx < a.c ||
       (!a.off && (a.len < 0 || (a.n && a.rows / a.n != a.len) || a.rows != a.n * a.len))) {
     set_error("%s: bad sizes (rows %lld, samples %lld of %lld, channels %d, groups %d, row stride %lld)", who, (long long)a.rows,
               (long long)a.n, (long long)a.len, a.c, a.groups, (long long)a.ldx);

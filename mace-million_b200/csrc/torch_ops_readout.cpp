@@ -20,7 +20,7 @@ GnIn gn_in(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, co
   TORCH_CHECK(x.dim() >= 2 && x.size(-1) >= 1, "x must be [samples, .., channels] (got ", x.sizes(), ")");
   TORCH_CHECK(x.size(-1) <= INT32_MAX, "x: too many channels");
   a.c = x.size(-1);
-  TORCH_CHECK(groups >= 1 && groups <= a.c && a.c % groups == 0, "group_norm: ", a.c, " channels do not split into ", groups, " groups");
+  TORCH_CHECK(groups >= 1 && groups <= a.c && groups <= MB_GN_MAX_GROUPS && a.c % groups == 0, "group_norm: ", a.c, " channels do not split into ", groups, " groups");
   TORCH_CHECK(act >= MB_ACT_NONE && act <= MB_ACT_RELU, "group_norm: unknown activation ", act);
   a.r = x.numel() / a.c;
   if (offsets.defined()) {
@@ -236,13 +236,12 @@ Tensor int8_linear(const Tensor& x, const OptTensor& xscale, const Tensor& w, co
     q = rows16(rows_of(x));
   } else {
     src = rows_of(x);
-    if (!mace_b200_int8_linear_few(t, (int32_t)k)) {
-      q = at::empty({t, pad16(k)}, w.options());
-      xs = at::empty({t}, ws.options());
-    }
+    if (!mace_b200_int8_linear_few(t, (int32_t)k)) q = at::empty({t * (pad16(k) + 4)}, w.options());   // rows, then their scales
   }
-  check_rc(mace_b200_int8_linear(ptr(src), src.defined() ? row_stride(src) : k, ptr_as<int8_t>(q),
-                                 q.defined() ? (is8 ? stride16(q) : pad16(k)) : k, ptr_as<float>(xs), wq.data_ptr<int8_t>(),
+  int8_t* qp = ptr_as<int8_t>(q);
+  float* xp = is8 ? xs.data_ptr<float>() : qp ? reinterpret_cast<float*>(qp + t * pad16(k)) : nullptr;
+  check_rc(mace_b200_int8_linear(ptr(src), src.defined() ? row_stride(src) : k, qp, is8 ? stride16(q) : pad16(k), xp,
+                                 wq.data_ptr<int8_t>(),
                                  stride16(wq), ws.data_ptr<float>(), ptr(b), y.data_ptr(), t, (int32_t)k, (int32_t)n, (int32_t)out,
                                  bt, stream_of(x)),
            "int8_linear");

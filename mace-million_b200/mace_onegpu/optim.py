@@ -28,9 +28,12 @@ def _table(steps, coefficients):
         rows = key[1] if isinstance(key[1][0], tuple) else (key[1],) * steps
         if len(rows) != steps or any(len(r) != 3 for r in rows):
             raise ValueError(f"coefficients must be (a, b, c), or one such triple for each of the {steps} steps")
+        table = torch.tensor(rows, dtype=torch.float64, device="cpu")
+        if type(table) is not torch.Tensor:         # a shape tensor has no values to keep
+            return table
         if len(_TABLES) > 64:
             _TABLES.clear()
-        _TABLES[key] = torch.tensor(rows, dtype=torch.float64)
+        _TABLES[key] = table
     return _TABLES[key]
 
 
@@ -74,7 +77,7 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             lr, mu = group["lr"], group["momentum"]
             for p in group["params"]:
-                if p.grad is None:
+                if p.grad is None or p.numel() == 0:
                     continue
                 v = self.state[p].get("momentum_buffer")
                 if v is None:

@@ -149,6 +149,16 @@ def test_samples_beyond_shared_memory(dt, rows, c, groups):
     _check(x, groups, w, b, dy, "silu", edges, dt, y, dx, dw, db)
 
 
+@pytest.mark.parametrize("dt,n,l,c,groups", [("f32", 3, 300, 4096, 1), ("bf16", 2, 700, 8200, 2), ("f16", 2, 1501, 1030, 2), ("bf16", 700, 33, 1024, 4),
+                                             ("f32", 9, 1000, 36, 12), ("bf16", 1, 3, 70000, 7)])
+def test_streaming_cuts(dt, n, l, c, groups):
+    """Groups wider than one pass of a CTA's threads, odd widths, many samples, in the form of several launches."""
+    dt = DT[dt]
+    x, w, b, dy = _data(n * l, c, dt, l)
+    y, dx, dw, db = _run(x, groups, w, b, dy, "gelu", dt, (n, l, c))
+    _check(x, groups, w, b, dy, "gelu", [i * l for i in range(n + 1)], dt, y, dx, dw, db)
+
+
 @pytest.mark.parametrize("mean", [1e3, -3e4])
 def test_large_means(mean):
     x, w, b, dy = _data(4000, 64, torch.float32, 5)

@@ -130,6 +130,46 @@ def test_two_graphs_have_workspaces_of_their_own():
     assert torch.equal(held[0][1], want[2]) and torch.equal(held[1][1], want[3])
 
 
+@pytest.mark.parametrize("b,m,n", [(1, 1100, 1300), (1, 2304, 2304), (150, 90, 200)])
+def test_two_calls_at_once(b, m, n):
+    """Two grids whose CTAs wait on one another, each as wide as the GPU, on two streams."""
+    a, c = torch.randn(b, m, n, device="cuda"), torch.randn(b, m, n, device="cuda")
+    want = optim.orthogonalize(a), optim.orthogonalize(c)
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for st, g in zip(s, (a, c)):
+            with torch.cuda.stream(st):
+                got.append(optim.orthogonalize(g))
+    torch.cuda.synchronize()
+    for i, u in enumerate(got):
+        assert torch.equal(u, want[i % 2])
+
+
+def test_offsets_beyond_32_bits():
+    """Elements past 2^31: the last rows are those of a call of their own."""
+    rows, c = 70_000_003, 32
+    x = torch.empty(rows, c, device="cuda", dtype=torch.bfloat16).normal_()
+    y = X.group_norm(x, 4, activation="silu", offsets=torch.tensor([0, rows - 100, rows]).cuda())
+    # a sample in another cut: the same values but for the order of sums, an ulp of bf16 (2^-8 relative) of values up to 5
+    assert (y[-100:].float() - X.group_norm(x[None, -100:], 4, activation="silu")[0].float()).abs().max() < 0.04
+    head = x[:1000].double().view(1000, 4, 8)
+    mean = torch.stack([x[:-100, 8 * g:8 * g + 8].float().mean(0).double().mean() for g in range(4)])
+    assert mean.abs().max() < 1e-3                            # of 5.6e8 normal values: 4e-5 and the order of an fp32 sum
+    assert (y[:1000].double() - R.activation(head.reshape(1000, c), "silu")).abs().max() < 0.05
+    del x, y, head
+    t, k, n = 2_200_000, 64, 1000
+    x = torch.empty(t, k, device="cuda", dtype=torch.float16).normal_()
+    wq, ws = X.quantize_rows(torch.randn(n, k, device="cuda"))
+    y = X.int8_linear(x, wq, ws)
+    assert torch.equal(y[-50:], X.int8_linear(x[-50:], wq, ws)) and torch.equal(y[-2:], X.int8_linear(x[-2:], wq, ws))
+    del x, y
+    g = torch.empty(65535, 100, 330, device="cuda", dtype=torch.bfloat16).normal_()
+    u = optim.orthogonalize(g)
+    assert torch.equal(u[-3:], optim.orthogonalize(g[-3:]))
+
+
 @pytest.mark.parametrize("args", [["mace_onegpu.readout", "--n", "4", "--steps", "3", "--hidden", "32"],
                                   ["mace_onegpu.readout", "--n", "4", "--steps", "3", "--hidden", "32", "--dtype", "bfloat16"],
                                   ["mace_onegpu.experts", "--n", "4", "--steps", "3", "--optimizer", "muon"],
