@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
         // 16 K elements are 32 bytes of a K-major row, or two 8-row atoms of an MN-major operand
         const uint64_t a_base = p.a_mn ? sw128_desc_mn(smem0, OR_BOX) : sw128_desc(smem0);
         const uint64_t b_base = p.b_mn ? sw128_desc_mn(smem0 + 2 * OR_BOX, OR_BOX) : sw128_desc(smem0 + 2 * OR_BOX);
+        const uint32_t a_lo = (uint32_t)a_base, a_hi = (uint32_t)(a_base >> 32), b_lo = (uint32_t)b_base, b_hi = (uint32_t)(b_base >> 32);
         const int a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
         for (int t = cta; ok && t < tiles; t += ctas) {
           if (!mbar_wait_warp(acc_empty0 + 8 * acc, acc_par, OR_WAIT, failed)) {
@@ -344,21 +345,23 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t d = tmem + acc * 256;
+          bool here = false;                      // the next K block, looked for while this one's products are issued
           for (int kb = 0; kb < nk; ++kb) {
             // the first wait of a phase includes the grid's barrier
-            if (!mbar_wait_warp(full0 + 8 * s, par, 2 * OR_WAIT, failed)) {
+            if (!here && !mbar_wait_warp(full0 + 8 * s, par, 2 * OR_WAIT, failed)) {
               *failed = 1;
               ok = false;
               break;
             }
-            const uint64_t off = (uint64_t)((uint32_t)(s * stage_bytes) >> 4), ad = a_base + off, bd = b_base + off;
-#pragma unroll
-            for (int kk = 0; kk < OR_BK / 16; ++kk)
-              mma_f16_ss_lead<CG>(lead, d, ad + kk * a_step, bd + kk * b_step, idesc, (kb | kk) ? 1u : 0u);
-            mma_commit_lead<CG>(lead, empty0 + 8 * s);
+            const uint32_t off = (uint32_t)(s * stage_bytes) >> 4, ad = a_lo + off, bd = b_lo + off;
             last_bar = empty0 + 8 * s;
             last_par = par;
             if (++s == stages) s = 0, par ^= 1;
+            here = kb + 1 < nk && mbar_over_warp(full0 + 8 * s, par);
+#pragma unroll
+            for (int kk = 0; kk < OR_BK / 16; ++kk)
+              mma_f16_ss_lead<CG>(lead, d, ad + kk * a_step, a_hi, bd + kk * b_step, b_hi, idesc, (kb | kk) ? 1u : 0u);
+            mma_commit_lead<CG>(lead, last_bar);
           }
           if (!ok) break;
           mma_commit_lead<CG>(lead, acc_full0 + 8 * acc);
