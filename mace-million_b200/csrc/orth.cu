@@ -673,11 +673,9 @@ static int orth_steps(OrArgs& a, int r, int len, cudaStream_t st) {
   return check_launch("orthogonalize");
 }
 
-// Pairs of CTAs halve the bytes that an SM fetches of its operands: for long sums and at least two rounds of 256 x 256 tiles.  One
-// CTA / pairs: 4096 x 4096 1330 / 1150 us, 2048 x 2048 275 / 275, 16 of 1024 x 1024 667 / 726.
-static bool or_pairs(int64_t batch, int64_t r, int64_t len) {
-  return r >= 2048 && batch * ((r + 255) / 256) * ((len + 255) / 256) >= sm_count();
-}
+// Pairs of CTAs halve the bytes that an SM fetches of one operand: for long sums.  One CTA / pairs: 4096 x 4096 1281 / 1166 us,
+// 2048 x 2048 251 / 240, 1500 x 1500 197 / 187; 1024 x 1024 124 / 151, 16 of them 645 / 667, 4 of 1500 x 700 189 / 197.
+static bool or_pairs(int64_t r) { return r >= 1400; }
 
 }  // namespace mb
 
@@ -766,5 +764,5 @@ extern "C" int mace_b200_orthogonalize(const void* gp, int64_t ldb, int64_t ldg,
            : dtype == MB_BF16 ? orth_go<bf16>(gp, ldb, ldg, a, part, st)
                               : orth_go<f16>(gp, ldb, ldg, a, part, st);
   if (rc) return rc;
-  return or_pairs(batch, r, len) ? orth_steps<2>(a, r, len, st) : orth_steps<1>(a, r, len, st);
+  return or_pairs(r) ? orth_steps<2>(a, r, len, st) : orth_steps<1>(a, r, len, st);
 }
