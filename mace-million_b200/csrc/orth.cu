@@ -21,6 +21,12 @@
 // accumulators.  Tall matrices are not transposed: their Gram product reads both operands MN-major.  Two small kernels before
 // it take the norm (sums of squares in fp64) and split G into the planes.
 // Every wait is bounded; after one expires the grid stops and the tiles of the result that have none are NaN.
+//
+// Measured on a B200 (5 steps, bf16 matrices, all launches; rates count half of the symmetric products): 4096 x 4096 1.16 ms
+// (1.18 PFLOP/s; 2 or 4 rounds of tiles a phase for 1.8 and 3.5 rounds' worth, and a drain and a barrier of 15 us at each of 15 phases'
+// ends), 2048 x 2048 240 us, 1024 x 1024 124 us and 3 of 515 x 1023 140 us: 8 to 9 us a phase, of which 3 are products, 2 the drain, 3 the
+// stores' way to memory and the grid's barrier, 1 the first loads; 16 of 1024 x 1024 630 us (X, its planes, A and B are 190 MB, more
+// than L2 holds).
 #include <cuda.h>
 
 #include <type_traits>
