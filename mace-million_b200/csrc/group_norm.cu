@@ -1158,9 +1158,12 @@ static void gn_place(GnArgs& a, float* ws, int size, int slabs) {
   a.stat = ws && a.n ? ws + a.n * gn_split(a, size, slabs) * 3 * (int64_t)a.groups : nullptr;
 }
 static int64_t gn_parts(const GnArgs& a, int size) {
-  const int64_t split = gn_split(a, size, 2), most = (int64_t)(GN_BWD_SM / 32) * (sm_count() > 0 ? sm_count() : 1);
-  const int64_t all = a.n * (split ? split : 8), some = most > 1024 ? most : 1024;
-  return all < some + 8 || split ? all : some + 8;
+  // of a launch at most what is resident or 1024 (gn_cut), and no more than its samples have parts
+  const int64_t split = gn_split(a, size, 2), p = split ? split : 8;
+  int64_t some = (int64_t)(GN_BWD_SM / 32) * (sm_count() > 0 ? sm_count() : 1);
+  if (some < 1024) some = 1024;
+  if (some < p) some = p;
+  return a.n * p < some ? a.n * p : some;
 }
 
 extern "C" int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups, int32_t ragged,
