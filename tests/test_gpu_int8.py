@@ -43,6 +43,24 @@ def test_quantize_rows(rows, k, dt):
     assert torch.equal(s, s0) and torch.equal(q.double(), q0)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("k,ld", [(4, 4), (7, 9), (8, 11), (15, 15), (17, 40), (131, 131), (260, 263), (515, 515), (771, 772), (1023, 1025),
+                                  (4099, 4099), (8193, 8200), (17001, 17001)])
+def test_quantize_rows_of_any_alignment(k, ld, dt):
+    """Rows that start anywhere, up to the first and the last element of their storage; what lies between them is NaN."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    for first in (0, 1, 5):
+        rows = 9
+        store = torch.full((first + (rows - 1) * ld + k,), float("nan"), device="cuda", dtype=DT[dt])
+        x = store.as_strided((rows, k), (ld, 1), first)
+        x.copy_(torch.randn(rows, k, generator=g, device="cuda"))
+        q, s = X.quantize_rows(x)
+        q0, s0 = _quantize(x)
+        assert torch.equal(s, s0) and torch.equal(q.double(), q0)
+        pad = q.as_strided((rows, q.stride(0) - k), (q.stride(0), 1), q.storage_offset() + k)
+        assert not pad[:-1].any()
+
+
 def test_quantize_ties_and_extremes():
     """Rows whose largest value is 127 times a power of two have exact ties at every half; scales down to subnormal ones."""
     half = torch.arange(-254, 255, device="cuda").float() / 2
