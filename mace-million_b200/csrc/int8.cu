@@ -3,17 +3,18 @@
 // The sums are exact in int32 (k <= MB_INT8_MAX_K), y is fp32 arithmetic on them, rounded once.  q is the nearest whole number
 // of the exact quotient, ties to even (a remainder by fma corrects the rounded quotient), so it does not depend on who divides.
 //
-// Three kernels.  k_quant_rows: a row stays in the registers of 32 to 512 threads, read once.  k_int8_few: up to 4 tokens; a CTA quantizes them into shared memory while its
+// Three kernels.  k_quant_rows: a row stays in the registers of 32 to 256 threads, read once.  k_int8_few: up to 4 tokens; a CTA quantizes them into shared memory while its
 // first weights are on their way, then each warp takes whole rows of w with dp4a: bound by the weights' bytes and latency.
 // k_int8_gemm: tcgen05 kind::i8 from TMA tiles (SWIZZLE_128B, 128 bytes of K a stage).  Output channels are the rows of an MMA
 // and tokens its columns: few tokens take a narrow tile, a lane holds one channel (its scale and bias stay in registers), and
-// a warp stores 32 neighbouring channels of a token at once, whatever the alignment of y.
+// a warp stores 32 neighbouring channels of a token at once, whatever the alignment of y.  What drains a tile is short code on
+// scales in shared memory, fetched a tile ahead; 128 x 256 results take 2.9 us an SM, 5.4 cycles a store.
 // Persistent CTAs, one per SM: warp 0 loads, warp 1 issues, warps 4-11 drain one of two accumulators.  CG = 2: pairs of CTAs
 // (cta_group::2) on 256 channels, each with its own 128 and half of the tokens' rows.  Every wait is bounded; a tile whose
 // wait expired is NaN.
 //
-// Measured on a B200 (cuBLAS bf16 1.67 PFLOP/s, so 3.3 POP/s for 8 bits): 16,384 x 4096 x 4096 bf16 202 us, of it the quantization 46
-// (4.4 TB/s) and the product 167 (3.3 POP/s, the tensor cores 87% busy); 16,384 x 1024 x 1024 31 us (10 and 19; the drain of a tile takes as
+// Measured on a B200 (cuBLAS bf16 1.67 PFLOP/s, so 3.3 POP/s for 8 bits): 16,384 x 4096 x 4096 bf16 202 us, of it the quantization 42
+// (4.8 TB/s) and the product 167 (3.3 POP/s, the tensor cores 87% busy); 16,384 x 1024 x 1024 31 us (10 and 19; the drain of a tile takes as
 // long as its 8 K blocks); 24,001 x 515 x 1001 fp16 42 us (13 and 28: elements of two bytes in rows of any alignment); 192 x 128 x 512
 // fp32 6 us (two launches); one token 1024 x 1024 2.7 us, 4096 x 4096 5.0 us (3.4 TB/s of weights).  Few tokens by dp4a / by the
 // tensor cores, 512 x 2048: 4 tokens 5.1 / 6.3 us, 5 tokens 8.4 / 6.4.
@@ -373,18 +374,18 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
 constexpr int I8_EPI0 = 4, I8_EPI = 8, I8_THREADS = 32 * (I8_EPI0 + I8_EPI), I8_BK = 128;
 constexpr unsigned long long I8_WAIT = 2000000000ull;
 
-template <int CG>
-struct I8Cfg {
-  static constexpr int A_BYTES = 128 * I8_BK, B_BYTES = 256 / CG * I8_BK, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 196608 / STAGE, SMEM = STAGES * STAGE + 256 + 1024;
-  static_assert(STAGES <= 8 && SMEM <= 227 * 1024, "shared memory");
-};
 struct I8Bars {
+  float xs[I8_EPI][128];                         // the scales of a draining warp's tokens
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int failed, never;                             // never: a flag that stays 0
 };
-
+template <int CG>
+struct I8Cfg {
+  static constexpr int A_BYTES = 128 * I8_BK, B_BYTES = 256 / CG * I8_BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 196608 / STAGE, SMEM = STAGES * STAGE + sizeof(I8Bars) + 1024;
+  static_assert(STAGES <= 8 && SMEM <= 227 * 1024, "shared memory");
+};
 // kind::i8: D int32 (bits 4-5 = 2), A and B signed 8-bit (1 at bits 7-9 and 10-12), both K-major
 __host__ __device__ constexpr uint32_t i8_idesc(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -492,29 +493,41 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
   } else if (warp >= I8_EPI0) {
     const int q4 = warp & 3, hf = (warp - I8_EPI0) >> 2, hw = g.bn / 2, tm = g.tm, n_all = g.n;
     const int64_t tokens = g.t;
+    float* xs = B.xs[warp - I8_EPI0];
     int acc = 0;
     uint32_t acc_par = 0;
     bool lost = false;                           // warp-uniform
+    // the next tile's: this lane's channel, and the scales of the half's tokens (lane l has those of l, 32 + l, ..)
+    float next_ws = 0.f, next_b = 0.f, next_xs[4];
+    auto fetch = [&](int t) {
+      const int tn = t / tm, n = (t - tn * tm) * (128 * CG) + rank * 128 + q4 * 32 + lane;
+      const int64_t first = (int64_t)tn * g.bn + hf * hw;
+      const bool on = n < n_all;
+      next_ws = on ? g.ws[n] : 0.f;
+      next_b = !on || !g.bias ? 0.f : g.b32 ? ((const float*)g.bias)[n] : to_f(((const T*)g.bias)[n]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) next_xs[q] = 32 * q + lane < hw && first + 32 * q + lane < tokens ? g.xs[first + 32 * q + lane] : 0.f;
+    };
+    if (cta < tiles) fetch(cta);
     for (int t = cta; t < tiles; t += ctas) {
       const int tn = t / tm, n = (t - tn * tm) * (128 * CG) + rank * 128 + q4 * 32 + lane;
       const int64_t first = (int64_t)tn * g.bn + hf * hw;
       const bool on = n < n_all;
-      // this lane's channel, and the scales of the half's tokens (lane l holds those of l, 32 + l, ..), on their way during the wait
-      float ws = on ? g.ws[n] : 0.f, xs[4];
-      const float b = !on || !g.bias ? 0.f : g.b32 ? ((const float*)g.bias)[n] : to_f(((const T*)g.bias)[n]);
+      float ws = next_ws;
+      const float b = next_b;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) xs[q] = 32 * q + lane < hw && first + 32 * q + lane < tokens ? g.xs[first + 32 * q + lane] : 0.f;
+      for (int q = 0; q < 4; ++q) xs[32 * q + lane] = next_xs[q];
+      __syncwarp();
       if (!lost) lost = !mbar_wait_warp(smem_u32(&B.acc_full[acc]), acc_par, I8_WAIT, failed);
       if (lost) {
         *failed = 1;
         ws = __int_as_float(0x7fc00000);
       }
+      if (t + ctas < tiles) fetch(t + ctas);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       T* y = (T*)g.y + first * n_all + n;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * q;
-        if (c >= hw) break;
+#pragma unroll 1                                // short code: unrolled, 16,384 x 512 x 512 fp16 takes 10.4 us instead of 9.8
+      for (int c = 0; c < hw; c += 32) {
         const int w = hw - c < 32 ? hw - c : 32;
         const int64_t rest = tokens - first - c;
         const int left = rest < w ? (int)rest : w;             // tokens here (<= 0: none)
@@ -537,22 +550,33 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
           for (int i = 0; i < 32; ++i) u[i] = 0;
         }
         // the tokens' rows one after the other, 32 neighbouring channels a store
+        const float4* s4 = reinterpret_cast<const float4*>(xs + c);
+        auto put = [&](float sum, float s, bool here) {
+          const float v = fmaf(sum * s, ws, b);
+          if (here) *y = from_f<T>(v);
+          y += n_all;
+        };
         if (left == 32) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float v = fmaf((float)(int)u[i] * __shfl_sync(0xffffffffu, xs[q], i), ws, b);
-            if (on) *y = from_f<T>(v);
-            y += n_all;
+          for (int i = 0; i < 32; i += 4) {
+            const float4 f = s4[i / 4];
+            put((float)(int)u[i], f.x, on);
+            put((float)(int)u[i + 1], f.y, on);
+            put((float)(int)u[i + 2], f.z, on);
+            put((float)(int)u[i + 3], f.w, on);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float v = fmaf((float)(int)u[i] * __shfl_sync(0xffffffffu, xs[q], i), ws, b);
-            if (i < left && on) *y = from_f<T>(v);
-            y += n_all;
+          for (int i = 0; i < 32; i += 4) {
+            const float4 f = s4[i / 4];
+            put((float)(int)u[i], f.x, i < left && on);
+            put((float)(int)u[i + 1], f.y, i + 1 < left && on);
+            put((float)(int)u[i + 2], f.z, i + 2 < left && on);
+            put((float)(int)u[i + 3], f.w, i + 3 < left && on);
           }
         }
       }
+      __syncwarp();                              // the scales are read
       acc ^= 1;
       if (acc == 0) acc_par ^= 1;
     }
