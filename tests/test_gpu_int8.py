@@ -44,6 +44,21 @@ def test_quantize_rows(rows, k, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,k", [(2500, 256), (37, 504), (9, 1016), (2501, 1032), (300, 2048), (5, 2064), (601, 4112), (7, 8192), (601, 8208),
+                                    (3, 16384), (3, 16400)])
+def test_quantize_rows_of_each_width(rows, k, dt):
+    """Whole vectors on either side of the widths that a warp, half a block and a block hold; some rows of whole numbers, full of ties."""
+    g = torch.Generator(device="cuda").manual_seed(rows + k)
+    x = torch.randn(rows, k, generator=g, device="cuda")
+    x[1::3] = torch.randint(-254, 255, x[1::3].shape, generator=g, device="cuda").float() / 2
+    x[1::3, k // 2] = 127
+    x = x.to(DT[dt])
+    q, s = X.quantize_rows(x)
+    q0, s0 = _quantize(x)
+    assert torch.equal(s, s0) and torch.equal(q.double(), q0)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("k,ld", [(4, 4), (7, 9), (8, 11), (15, 15), (17, 40), (131, 131), (260, 263), (515, 515), (771, 772), (1023, 1025),
                                   (4099, 4099), (8193, 8200), (17001, 17001)])
 def test_quantize_rows_of_any_alignment(k, ld, dt):
