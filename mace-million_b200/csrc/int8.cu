@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
   __shared__ float red[TT][8], sc[TT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kp = (a.k + 15) & ~15, kv = kp / 16, whole = a.k / 16;
-  const int rows = a.n, first = (blockIdx.x * 8 + warp) * R;
+  const unsigned rows = a.n, first = (blockIdx.x * 8 + warp) * R;   // (a grid's step beyond 2^31 - 256 rows passes 31 bits)
   // the first vectors of this warp's rows, in flight while the tokens are quantized
   uint4 pre[R];
 #pragma unroll
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
     if (tid < TT) sc[tid] = tid < a.t ? a.xs[tid] : 0.f;
   }
   __syncthreads();
-  for (int n0 = first; n0 < rows; n0 += (int)gridDim.x * 8 * R) {
+  for (unsigned n0 = first; n0 < rows; n0 += gridDim.x * 8 * R) {
     int acc[R][TT];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
         if (lane == t * R + r) mine = acc[r][t];
-    const int t = lane / R, n = n0 + lane % R;
+    const int t = lane / R;
+    const unsigned n = n0 + lane % R;
     if (t < a.t && t < TT && n < rows) {
       const float b = !a.bias ? 0.f : a.b32 ? ((const float*)a.bias)[n] : to_f(((const T*)a.bias)[n]);
       ((T*)a.y)[(int64_t)t * rows + n] = from_f<T>(fmaf((float)mine * sc[t], a.ws[n], b));
@@ -652,10 +653,12 @@ static int few_go(const I8Args& a, cudaStream_t st) {
 
 template <typename T>
 static int few_any(const I8Args& a, cudaStream_t st) {
-  const bool wide = a.n >= 32 * sm_count();       // rows enough for several a warp
+  // rows enough for several a warp, which then read the tokens once (4096 x 4096, two rows against one: 2 tokens 6.1 and 7.3 us, 4 tokens 9.1
+  // and 11.5; 4096 x 2500 2 tokens 6.2 and 5.9)
+  const bool wide = a.n >= 32 * sm_count(), some = a.n >= 24 * sm_count();
   if (a.t <= 1) return wide ? few_go<T, 1, 4>(a, st) : few_go<T, 1, 1>(a, st);
-  if (a.t <= 2) return wide ? few_go<T, 2, 4>(a, st) : few_go<T, 2, 1>(a, st);
-  return wide ? few_go<T, 4, 4>(a, st) : few_go<T, 4, 1>(a, st);
+  if (a.t <= 2) return wide ? few_go<T, 2, 4>(a, st) : some ? few_go<T, 2, 2>(a, st) : few_go<T, 2, 1>(a, st);
+  return wide ? few_go<T, 4, 4>(a, st) : some ? few_go<T, 4, 2>(a, st) : few_go<T, 4, 1>(a, st);
 }
 
 template <typename T, int CG>

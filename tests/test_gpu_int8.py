@@ -58,6 +58,18 @@ def test_quantize_rows_of_each_width(rows, k, dt):
     assert torch.equal(s, s0) and torch.equal(q.double(), q0)
 
 
+@pytest.mark.parametrize("n", [3551, 3552, 3557, 4735, 4736, 4739])
+def test_few_tokens_and_many_channels(n):
+    """One, two and four rows of the weights a warp, the last ones incomplete."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    wq, ws = X.quantize_rows(torch.randn(n, 200, generator=g, device="cuda"))
+    for tokens in (1, 2, 3, 4):
+        x = torch.randn(tokens, 200, generator=g, device="cuda", dtype=torch.bfloat16)
+        q, s = _quantize(x)
+        b = torch.randn(n, generator=g, device="cuda")
+        _close(X.int8_linear(x, wq, ws, b), q, s, wq, ws, b, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("k,ld", [(4, 4), (7, 9), (8, 11), (15, 15), (17, 40), (131, 131), (260, 263), (515, 515), (771, 772), (1023, 1025),
                                   (4099, 4099), (8193, 8200), (17001, 17001)])
