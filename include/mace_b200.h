@@ -358,9 +358,10 @@ int mace_b200_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_
  * Channels last: n samples, each a run of rows of c channels (ldx apart, y dense); a group is c / groups channels of all rows of
  * a sample.  y = f((x - mean) rstd w + b), f one of MB_ACT_*; w / b may be null (1 / 0), of type ptype (the type of x, or fp32).
  * offsets null: samples of len rows, rows = n len.  Else offsets[n + 1] (int32, or int64 with offsets64) ascend within
- * [0, rows]: sample i is rows [offsets[i], offsets[i + 1]); rows outside of all samples give zeros; a sample whose offsets descend
- * or leave the rows is NaN (nothing is accessed out of range).
- * mean / rstd [n][groups] are written when not null (both or none); the backward pass reads them.
+ * [0, rows]: sample i is rows [offsets[i], offsets[i + 1]); rows outside of all samples give zeros; a sample whose offsets
+ * leave the rows is NaN, and where they descend anywhere all rows are (nothing is accessed out of range).
+ * mean / rstd [n][groups] are written when not null (both or none); the backward pass reads them (a NaN in rstd tells it, too,
+ * that the offsets descend).
  * bwd: dx (may be null) dense; dw / db [c] of type ptype (may be null), summed in a fixed order.
  * workspace: mace_b200_group_norm_workspace floats (may be null where that is 0; ragged: with offsets). */
 #define MB_GN_MAX_GROUPS (1 << 24)

@@ -34,7 +34,9 @@ struct GnArgs {
   float *mean, *rstd, *partial;                   // partial [cluster rows][2][C]: sums of dz xh, of dz (null: none)
   float *sums, *stat;                             // [n][P][3][groups] of GN_SUMS, [n][groups][2] for GN_APPLY
   const void* off;                                // [n + 1], null: samples of `len` rows
+  int* order;                                     // words of k_gn_order that say whether they ascend, null: each CTA looks for itself
   int64_t ldx, lddy, rows, n, len;
+  int32_t norder;
   int32_t c, groups, cg, gpb, act, off64, p32, cap, pshift, pvec;   // gpb: groups of a column block; cap: row steps kept in shared memory
                                                   // pshift: log2 of a cluster's CTAs; pvec: parameters are aligned vectors
   float eps;
@@ -45,34 +47,62 @@ constexpr int GN_FWD_CTAS = 4, GN_BWD_CTAS = 2;
 
 enum { GN_WHOLE = 0, GN_SUMS = 1, GN_APPLY = 2 };
 
-// Rows of a sample; false: the offsets descend or leave the rows there
+__device__ __forceinline__ int64_t gn_off(const GnArgs& a, int64_t i) {
+  return a.off64 ? ((const int64_t*)a.off)[i] : (int64_t)((const int32_t*)a.off)[i];
+}
+// Rows of a sample; false: the offsets leave the rows there
 __device__ __forceinline__ bool gn_range(const GnArgs& a, int64_t s, int64_t& lo, int64_t& hi) {
   if (!a.off) {
     lo = s * a.len;
     hi = lo + a.len;
     return true;
   }
-  auto at = [&](int64_t i) { return a.off64 ? ((const int64_t*)a.off)[i] : (int64_t)((const int32_t*)a.off)[i]; };
-  const int64_t u = at(s), v = at(s + 1), before = s ? at(s - 1) : 0;
+  const int64_t u = gn_off(a, s), v = gn_off(a, s + 1);
   lo = u < 0 ? 0 : u < a.rows ? u : a.rows;
   hi = v < lo ? lo : v < a.rows ? v : a.rows;
-  return u >= before && v >= u && v <= a.rows;
+  return u >= 0 && v <= a.rows;
 }
 
-// Rows outside of all samples are zero
+// Whether the offsets ascend everywhere, for a whole block.  Where they descend, samples far from there may share rows, and which
+// of them wrote last would be anyone's guess: then every block writes NaN alone.  Up to GN_SCAN samples a block reads all offsets
+// itself (16 a thread of 64; 900 samples of 60 x 128 bf16 17.1 -> 19.0 us), more are looked through by a launch of their own, and a
+// block reads its words (4,000 samples 60 -> 62 us).  rstd then holds GN_DESCENDS, a NaN that no arithmetic gives (that is 7fffffff),
+// where the backward pass finds the answer.
+constexpr int GN_SCAN = 1024;
+constexpr unsigned GN_DESCENDS = 0x7fc00d0du;
+__device__ __forceinline__ bool gn_ascend(const GnArgs& a) {
+  if (!a.off) return true;
+  int bad = 0;
+  if (a.order) {
+    for (int i = threadIdx.x; i < a.norder; i += blockDim.x) bad |= a.order[i];
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < (int)a.n; i += blockDim.x) bad |= gn_off(a, i + 1) < gn_off(a, i);
+  }
+  return !__syncthreads_or(bad);
+}
+__global__ void __launch_bounds__(256) k_gn_order(const GnArgs a) {
+  int bad = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 256) bad |= gn_off(a, i + 1) < gn_off(a, i);
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) a.order[blockIdx.x] = bad;
+}
+
+// Rows outside of all samples are zero (NaN where the offsets do not ascend)
 template <typename T>
-__device__ __forceinline__ void gn_clear(const GnArgs& a) {
+__device__ __forceinline__ void gn_clear(const GnArgs& a, bool ascend) {
   if (!a.off || !a.out) return;
   auto at = [&](int64_t i) {
-    const int64_t v = a.off64 ? ((const int64_t*)a.off)[i] : (int64_t)((const int32_t*)a.off)[i];
+    const int64_t v = gn_off(a, i);
     return v < 0 ? 0 : v < a.rows ? v : a.rows;
   };
+  const T none = from_f<T>(ascend ? 0.f : __int_as_float(0x7fc00000));
   const int64_t head = a.n ? at(0) : a.rows, tail = a.n ? at(a.n) : a.rows;
   const int64_t id = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
   const int64_t step = (int64_t)gridDim.x * gridDim.y * gridDim.z * blockDim.x;
   T* out = (T*)a.out;
-  for (int64_t i = id * blockDim.x + threadIdx.x; i < head * a.c; i += step) out[i] = from_f<T>(0.f);
-  for (int64_t i = tail * a.c + id * blockDim.x + threadIdx.x; i < a.rows * a.c; i += step) out[i] = from_f<T>(0.f);
+  for (int64_t i = id * blockDim.x + threadIdx.x; i < head * a.c; i += step) out[i] = none;
+  for (int64_t i = tail * a.c + id * blockDim.x + threadIdx.x; i < a.rows * a.c; i += step) out[i] = none;
 }
 
 // V consecutive elements of T as one access of 16, 8 or sizeof(T) bytes
@@ -327,7 +357,8 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
   float* fin = grp0 + 2 * gn_grp_floats(th, a.gpb);
   Vec* kept = reinterpret_cast<Vec*>(gn_smem + gn_shared_floats(th, a.gpb)) + threadIdx.x;
   const int64_t step = (int64_t)k.tr * a.ldx, ystep = (int64_t)k.tr * a.c;
-  if (MODE != GN_SUMS) gn_clear<T>(a);
+  const bool ascend = MODE == GN_SUMS || gn_ascend(a);
+  if (MODE != GN_SUMS) gn_clear<T>(a, ascend);
   int par = 0;
   for (int64_t z = blockIdx.z; z < a.n; z += gridDim.z, par ^= 1) {
     const int64_t s = MODE == GN_APPLY ? a.n - 1 - z : z;
@@ -498,8 +529,9 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
         part[a.groups] = mean;
         part[2 * a.groups] = m2;
       } else {
-        const float bad = good ? 0.f : __int_as_float(0x7fc00000);
-        const float rs = rsqrtf((n > 0.f ? __fdividef(m2, n) : 0.f) + a.eps) + bad;
+        const float bad = good && ascend ? 0.f : __int_as_float(0x7fc00000);
+        float rs = rsqrtf((n > 0.f ? __fdividef(m2, n) : 0.f) + a.eps) + bad;
+        if (!ascend) rs = __uint_as_float(GN_DESCENDS);
         fin[2 * g] = mean + bad;
         fin[2 * g + 1] = rs;
         if (a.mean && rank == 0) {
@@ -604,7 +636,7 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
   float* grp0 = gn_smem + 2 * th;
   float* fin = grp0 + 2 * gn_grp_floats(th, a.gpb);
   Vec* kept = reinterpret_cast<Vec*>(gn_smem + gn_shared_floats(th, a.gpb)) + threadIdx.x;
-  if (MODE != GN_SUMS) gn_clear<T>(a);
+  if (MODE != GN_SUMS && a.off) gn_clear<T>(a, __float_as_uint(a.rstd[0]) != GN_DESCENDS);
   // sums of dz xh and dz over the samples (one tile of columns): a thread's own places behind the kept rows
   float* total = gn_smem + gn_shared_floats(th, a.gpb) + (size_t)2 * (gn_ring<MODE, T, V, true> ? GN_RING : cap) * th * V * sizeof(T) / 4 + threadIdx.x;
   if (MODE != GN_APPLY && k.tiles == 1)
@@ -896,8 +928,12 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
 
 // The parts' sums of each sample and group, a warp each: forward (count, mean, squared deviations) to mean and rstd, backward (sums
 // of a and a xh) to their means
-__global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P, bool backward) {
+// ORDER: the offsets are looked through (forward, ragged).  Asked for at run time, or with four loads ahead instead of eight, the join of
+// 592 parts takes 2 us longer.
+template <bool BWD, bool ORDER>
+__global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P) {
   const int lane = threadIdx.x & 31;
+  const bool ascend = !ORDER || gn_ascend(a);
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.n * a.groups; i += (int64_t)gridDim.x * 8) {
     const int64_t s = i / a.groups;
     const float* p = a.sums + s * P * 3 * a.groups + (i - s * a.groups);
@@ -905,7 +941,7 @@ __global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P, bool bac
     int64_t lo, hi;
     const bool good = gn_range(a, s, lo, hi);
     float u = 0.f, v = 0.f;
-    if (backward) {
+    if constexpr (BWD) {
 #pragma unroll 4
       for (int q = lane; q < P; q += 32) u += p[q * step], v += p[q * step + a.groups];
       const float inv = 1.f / ((float)(hi - lo) * (float)a.cg);
@@ -913,7 +949,7 @@ __global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P, bool bac
       v = warp_sum(v) * inv;
     } else {
       float n = 0.f, m2 = 0.f;
-#pragma unroll 4
+#pragma unroll 8
       for (int q = lane; q < P; q += 32) {
         const float c = p[q * step];
         n += c;
@@ -921,20 +957,21 @@ __global__ void __launch_bounds__(256) k_gn_join(const GnArgs a, int P, bool bac
       }
       n = warp_sum(n);
       u = n > 0.f ? warp_sum(u) / n : 0.f;
-#pragma unroll 4
+#pragma unroll 8
       for (int q = lane; q < P; q += 32) {
         const float c = p[q * step], d = p[q * step + a.groups] - u;
         if (c > 0.f) m2 += fmaf(d * d, c, p[q * step + 2 * a.groups]);
       }
       m2 = warp_sum(m2);
-      const float bad = good ? 0.f : __int_as_float(0x7fc00000);
+      const float bad = good && ascend ? 0.f : __int_as_float(0x7fc00000);
       u += bad;
       v = rsqrtf((n > 0.f ? m2 / n : 0.f) + a.eps) + bad;
+      if (!ascend) v = __uint_as_float(GN_DESCENDS);
     }
     if (lane == 0) {
       a.stat[2 * i] = u;
       a.stat[2 * i + 1] = v;
-      if (!backward && a.mean) {
+      if (!BWD && a.mean) {
         a.mean[i] = u;
         a.rstd[i] = v;
       }
@@ -1070,9 +1107,25 @@ static int gn_vec(const GnArgs& a, int size) {
   return 1;
 }
 
-static int gn_join(const GnArgs& a, int p, bool backward, cudaStream_t st) {
+// Words of k_gn_order (0: blocks look at the offsets themselves), and its launch
+static int gn_order_words(const GnArgs& a) {
+  const int64_t want = (a.n + 1023) / 1024;
+  return !a.off || a.n <= GN_SCAN ? 0 : (int)(want < sm_count() ? want : sm_count());
+}
+static int gn_order(const GnArgs& a, cudaStream_t st) {
+  if (!a.order) return 0;
+  k_gn_order<<<a.norder, 256, 0, st>>>(a);
+  return check_launch("group_norm (offsets)");
+}
+
+template <bool BWD>
+static int gn_join(const GnArgs& a, int p, cudaStream_t st) {
   const int64_t want = (a.n * a.groups + 7) / 8, most = 8 * (int64_t)sm_count();
-  k_gn_join<<<(unsigned)(want < most ? want : most), 256, 0, st>>>(a, p, backward);
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  if (!BWD && a.off)
+    k_gn_join<BWD, !BWD><<<grid, 256, 0, st>>>(a, p);
+  else
+    k_gn_join<BWD, false><<<grid, 256, 0, st>>>(a, p);
   return check_launch("group_norm");
 }
 
@@ -1083,7 +1136,7 @@ static int gn_fwd_go(GnArgs& a, cudaStream_t st) {
   const GnCut k = gn_cut<V>(a, sizeof(T), 1, GN_FWD_SM);
   if (!k.split) return gn_launch<k_gn_fwd<GN_WHOLE, T, V>>(a, k, st, "group_norm_fwd");
   if (int rc = gn_launch<k_gn_fwd<GN_SUMS, T, V>>(a, k, st, "group_norm_fwd")) return rc;
-  if (int rc = gn_join(a, k.p, false, st)) return rc;
+  if (int rc = gn_join<false>(a, k.p, st)) return rc;
   return gn_launch<k_gn_fwd<GN_APPLY, T, V>>(a, k, st, "group_norm_fwd");
 }
 template <typename T>
@@ -1100,7 +1153,7 @@ static int gn_bwd_go(GnArgs& a, int64_t* parts, bool launch, cudaStream_t st) {
   if (!k.split) return gn_launch<k_gn_bwd<GN_WHOLE, T, V>>(a, k, st, "group_norm_bwd");
   if (int rc = gn_launch<k_gn_bwd<GN_SUMS, T, V>>(a, k, st, "group_norm_bwd")) return rc;
   if (!a.out) return 0;
-  if (int rc = gn_join(a, k.p, true, st)) return rc;
+  if (int rc = gn_join<true>(a, k.p, st)) return rc;
   return gn_launch<k_gn_bwd<GN_APPLY, T, V>>(a, k, st, "group_norm_bwd");
 }
 template <typename T>
@@ -1148,14 +1201,11 @@ static int gn_type(int dtype, const F& f) {
 
 using namespace mb;
 
-// Floats of the split form's sums, and rows of partial sums of the parameters' gradients there can be
+// The workspace: the split form's sums, then forward the words of k_gn_order, backward partial sums of the parameters' gradients.
+// Floats of the sums, and rows there can be of the partial ones
 static int64_t gn_sums(const GnArgs& a, int size, int slabs) {
   const int64_t p = a.n ? gn_split(a, size, slabs) : 0;
   return p ? a.n * (3 * p + 2) * (int64_t)a.groups : 0;
-}
-static void gn_place(GnArgs& a, float* ws, int size, int slabs) {
-  a.sums = ws;
-  a.stat = ws && a.n ? ws + a.n * gn_split(a, size, slabs) * 3 * (int64_t)a.groups : nullptr;
 }
 static int64_t gn_parts(const GnArgs& a, int size) {
   // of a launch at most what is resident or 1024 (gn_cut), and no more than its samples have parts
@@ -1164,6 +1214,16 @@ static int64_t gn_parts(const GnArgs& a, int size) {
   if (some < 1024) some = 1024;
   if (some < p) some = p;
   return a.n * p < some ? a.n * p : some;
+}
+
+static int64_t gn_floats(const GnArgs& a, int size, int slabs) {   // without the words of k_gn_order
+  return gn_sums(a, size, slabs) + (slabs == 2 ? 2 * (int64_t)a.c * gn_parts(a, size) : 0);
+}
+static void gn_place(GnArgs& a, float* ws, int size, int slabs) {
+  a.sums = ws;
+  a.stat = !ws ? nullptr : ws + a.n * gn_split(a, size, slabs) * 3 * (int64_t)a.groups;
+  a.norder = slabs == 1 ? gn_order_words(a) : 0;
+  a.order = a.norder ? reinterpret_cast<int*>(ws + gn_floats(a, size, slabs)) : nullptr;
 }
 
 extern "C" int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t len, int32_t c, int32_t groups, int32_t ragged,
@@ -1179,7 +1239,7 @@ extern "C" int mace_b200_group_norm_workspace(int64_t rows, int64_t n, int64_t l
     return MB_E_CUDA;
   }
   const int size = dtype_size(dtype);
-  *floats = n == 0 || rows == 0 ? 0 : gn_sums(a, size, backward ? 2 : 1) + (backward ? 2 * (int64_t)c * gn_parts(a, size) : 0);
+  *floats = n == 0 || rows == 0 ? 0 : gn_floats(a, size, backward ? 2 : 1) + (backward ? 0 : gn_order_words(a));
   return 0;
 }
 
@@ -1193,18 +1253,19 @@ extern "C" int mace_b200_group_norm_fwd(const void* x, int64_t ldx, const void* 
     set_error("group_norm_fwd: no CUDA device");
     return MB_E_CUDA;
   }
-  if (rows > 0 && (!x || !y || !mean != !rstd || (!workspace && gn_sums(a, dtype_size(dtype), 1) > 0))) {
+  if (rows > 0 && (!x || !y || !mean != !rstd || (!workspace && n > 0 && gn_floats(a, dtype_size(dtype), 1) + gn_order_words(a) > 0))) {
     set_error("group_norm_fwd: null pointer");
     return MB_E_ARG;
   }
   a.out = y; a.mean = mean; a.rstd = rstd; a.eps = (float)eps;
-  gn_place(a, workspace, dtype_size(dtype), 1);
   if (rows == 0) return 0;
   if (n == 0) {                                   // rows of no sample
     if (cudaMemsetAsync(y, 0, (size_t)rows * c * dtype_size(dtype), (cudaStream_t)stream) != cudaSuccess)
       return check_launch("group_norm_fwd");
     return 0;
   }
+  gn_place(a, workspace, dtype_size(dtype), 1);
+  if (int rc = gn_order(a, (cudaStream_t)stream)) return rc;
   return gn_type(dtype, [&](auto t) { return gn_fwd_any<decltype(t)>(a, (cudaStream_t)stream); });
 }
 
