@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) k_quant_any(const T* __restrict__ x, int6
     const T* p = x + row * ldx;
     int8_t* o = q + row * ldq;
     float top = 0.f;
-    auto put = [&](int j, const float (&f)[4], const Q8& qk) {
+    auto put = [&](int64_t j, const float (&f)[4], const Q8& qk) {
       const uint32_t w = q8x4(f, qk);
       if (words) {
         if (j < ldq) *reinterpret_cast<uint32_t*>(o + j) = w;
@@ -208,10 +208,10 @@ __global__ void __launch_bounds__(256) k_quant_any(const T* __restrict__ x, int6
         const float f[4] = {to_f(v[n][0]), to_f(v[n][1]), to_f(v[n][2]), to_f(v[n][3])};
         put(128 * n + 4 * lane, f, qk);
       }
-      for (int j = 128 * NV + lane; j < ldq; j += 32) o[j] = 0;
+      for (int64_t j = 128 * NV + lane; j < ldq; j += 32) o[j] = 0;
     } else {
 #pragma unroll 8
-      for (int j = lane; j < k; j += 32) top = top_of(top, to_f(p[j]));
+      for (unsigned j = lane; j < (unsigned)k; j += 32) top = top_of(top, to_f(p[j]));   // (a step beyond widths next to 2^31 passes 31 bits)
       const Q8 qk = q8_of(q8_scale(warp_top(top)));
       if (lane == 0) scale[row] = qk.scale;
 #pragma unroll 2
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) k_quant_any(const T* __restrict__ x, int6
         float f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = j + i < k ? to_f(p[j + i]) : 0.f;
-        put((int)j, f, qk);
+        put(j, f, qk);
       }
     }
   }
