@@ -13,7 +13,8 @@
 //    the copy rate.  (Large samples in clusters of 8 on the chip read once, but load and store in turns: 64 x 2048 x 512 bf16
 //    forward 124 us and backward 315.)
 // A thread owns V channels of one group (16 bytes, or what divides a group) and every TR-th row, and takes its sums relative to
-// its own first row: of one thread's few hundred rows they lose at most that number of fp32 roundings, whatever the mean.
+// its own first row, GN_RUN rows at a time: a sample far longer than the others, which gets no more threads than they, may have
+// 10^5 rows of a thread, and that many additions of like values in a row are 0.1% off (of 137,500 times 0.1; in runs of 512 1.5e-6).
 // Threads, CTAs and clusters are joined as (count, mean, sum of squared deviations), so nothing cancels.  No atomics: parameter
 // gradients are added up over a CTA's samples in registers, then over CTAs by a second small kernel in a fixed order.
 #include "dtypes.cuh"
@@ -41,6 +42,10 @@ struct GnArgs {
                                                   // pshift: log2 of a cluster's CTAs; pvec: parameters are aligned vectors
   float eps;
 };
+
+// Rows of a thread that are added one after the other (a multiple of GN_RING and of four); what a run gives is joined with the runs
+// before it.  Those wait in the thread's place of `red`: in registers they cost the usual case, one run, up to a fifth of its time.
+constexpr int GN_RUN = 512;
 
 // CTAs of 256 threads that the registers let be resident on an SM
 constexpr int GN_FWD_CTAS = 4, GN_BWD_CTAS = 2;
@@ -315,6 +320,12 @@ __device__ __forceinline__ int gn_count(int64_t nr, const GnWalk& k) {
   const int64_t n = nr - k.r + k.tr - 1;
   return (n >> 31) ? (int)(n / k.tr) : (int)((unsigned)n / (unsigned)k.tr);
 }
+// (mean relative to the first row, squared deviations) of c rows of V channels in r, joined with those of n rows more
+__device__ __forceinline__ void gn_join_run(float2& r, float c, float rel, float dev, float n, float v) {
+  const float d = rel - r.x, f = n / (c + n);
+  r.x = fmaf(d, f, r.x);
+  r.y += fmaf(d * d * v, c * f, dev);
+}
 // The place of this thread's warp among a group's slots
 __device__ __forceinline__ int gn_slot(const GnWalk& k) { return k.tc < 32 ? threadIdx.x >> 5 : k.r; }
 
@@ -373,6 +384,7 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
       const int v0 = t * k.tc, cv = v0 + k.col;
       const bool on = cv < k.nvec && k.on && nr > k.r;
       float mu = 0.f, m2 = 0.f, mine = 0.f;       // of this thread's rows, and how many
+      if (!k.slots && nr > GN_RUN * k.tr) __syncthreads();   // red is free
       if (on) {
         const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + k.c0 + cv * V;
         E piv[NE], s1[NE], s2[NE];
@@ -395,7 +407,43 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
           }
         };
         int64_t left = nr - k.r;                  // rows from this thread's next one on
-        int i = 0;
+        int n;                                    // rows of this run
+        // V channels of a run to (mean, mean relative to the first row, squared deviations) of n * V values
+        auto channels = [&](float& mean, float& rel, float& dev) {
+          const float rows = (float)n, inv = __fdividef(1.f, rows);
+          float p[V], u1[V], u2[V];
+          from_elems<V>(piv, p);
+          from_elems<V>(s1, u1);
+          from_elems<V>(s2, u2);
+          mean = rel = dev = 0.f;
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            const float d = u1[q] * inv;
+            p[q] = d - p[q];
+            mean += p[q];
+            rel += d;
+            dev += fmaxf(fmaf(-u1[q], d, u2[q]), 0.f * u2[q]);   // not below 0, NaN stays
+          }
+          mean *= 1.f / (float)V;
+          rel *= 1.f / (float)V;
+#pragma unroll
+          for (int q = 0; q < V; ++q) dev = fmaf((p[q] - mean) * (p[q] - mean), rows, dev);
+        };
+        int runs = 0;                             // before this one
+        auto next_run = [&] {
+          float mean, rel, dev;
+          channels(mean, rel, dev);
+          float2 r = make_float2(rel, dev);
+          if (runs > 0) {
+            r = red[threadIdx.x];
+            gn_join_run(r, (float)runs * GN_RUN, rel, dev, GN_RUN, (float)V);
+          }
+          red[threadIdx.x] = r;
+          ++runs;
+          n = 0;
+#pragma unroll
+          for (int q = 0; q < NE; ++q) s1[q] = s2[q] = e_splat<E>(0.f);
+        };
         if constexpr (gn_ring<MODE, T, V, false>) {
           const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
           int64_t todo = left;
@@ -409,7 +457,8 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
           };
 #pragma unroll
           for (int d = 0; d < GN_RING; ++d) issue(d);
-          while (todo > 0) {
+          for (n = 0; todo > 0;) {
+            if (n == GN_RUN) next_run();
 #pragma unroll
             for (int d = 0; d < GN_RING; ++d) {
               if (todo <= 0) break;
@@ -417,40 +466,38 @@ __global__ void __launch_bounds__(256, GN_FWD_CTAS) k_gn_fwd(const GnArgs a) {
               add(kept[d * th]);
               issue(d);
               todo -= k.tr;
-              ++i;
+              ++n;
             }
           }
         } else {
-          for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * step, i += U) {
+          for (n = 0; left > (U - 1) * k.tr; left -= U * k.tr, x += U * step, n += U) {
+            if (n == GN_RUN) next_run();
             Vec u[U];
   #pragma unroll
             for (int j = 0; j < U; ++j) u[j].load(x + j * step);
   #pragma unroll
             for (int j = 0; j < U; ++j) add(u[j]);
           }
-          for (; left > 0; left -= k.tr, x += step, ++i) {
+          for (; left > 0; left -= k.tr, x += step, ++n) {   // (fewer than U)
             Vec u;
             u.load(x);
             add(u);
           }
         }
-        // V channels to (mean, squared deviations) of mine * V values
-        mine = (float)i;
-        const float inv = __fdividef(1.f, mine);
-        float p[V], u1[V], u2[V];
-        from_elems<V>(piv, p);
-        from_elems<V>(s1, u1);
-        from_elems<V>(s2, u2);
+        float rel;
+        channels(mu, rel, m2);
+        mine = (float)n;
+        if (runs > 0) {
+          float2 r = red[threadIdx.x];
+          gn_join_run(r, (float)runs * GN_RUN, rel, m2, mine, (float)V);
+          float p[V], sum = 0.f;
+          from_elems<V>(piv, p);
 #pragma unroll
-        for (int q = 0; q < V; ++q) {
-          const float d = u1[q] * inv;
-          p[q] = d - p[q];
-          mu += p[q];
-          m2 += fmaxf(fmaf(-u1[q], d, u2[q]), 0.f * u2[q]);   // not below 0, NaN stays
+          for (int q = 0; q < V; ++q) sum += p[q];
+          mu = fmaf(sum, -1.f / (float)V, r.x);
+          m2 = r.y;
+          mine = fmaf((float)runs, GN_RUN, mine);
         }
-        mu *= 1.f / (float)V;
-#pragma unroll
-        for (int q = 0; q < V; ++q) m2 = fmaf((p[q] - mu) * (p[q] - mu), mine, m2);
       }
       if (k.slots) {
         const float n = mine * (float)V, cnt = gn_warp_sum(k, n), sum = gn_warp_sum(k, n * mu);
@@ -681,8 +728,21 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
       const int c = k.c0 + cv * V;
       E sw[NE], sb[NE];
       float s1 = 0.f, s2 = 0.f;
+      bool fresh = first;                         // nothing of these columns lies in memory
 #pragma unroll
       for (int q = 0; q < NE; ++q) sw[q] = sb[q] = e_splat<E>(0.f);
+      auto put_part = [&] {
+        if (k.tiles == 1 || !part || cv >= k.nvec) return;   // several tiles: one thread a column, its sums of all samples lie in memory
+        float fw[V], fb[V];
+        from_elems<V>(sw, fw);
+        from_elems<V>(sb, fb);
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          part[c + q] = fresh ? fw[q] : part[c + q] + fw[q];
+          part[a.c + c + q] = fresh ? fb[q] : part[a.c + c + q] + fb[q];
+        }
+      };
+      if (!k.slots && nr > GN_RUN * k.tr) __syncthreads();   // red is free
       if (on) {
         columns(c, k.tiles == 1 ? k.grp : cv / k.cgv);
         const T* x = (const T*)a.x + (r0 + k.r) * a.ldx + c;
@@ -702,6 +762,37 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
             sb[q] = e_add(sb[q], d[q]);
           }
         };
+        auto columns_sums = [&] {                 // of a run: to s1, s2 and the parameters' sums
+          E p1 = e_splat<E>(0.f), p2 = p1;
+#pragma unroll
+          for (int q = 0; q < NE; ++q) {
+            p1 = e_fma(w[q], sb[q], p1);
+            p2 = e_fma(w[q], sw[q], p2);
+          }
+          s1 = e_sum(p1);
+          s2 = e_sum(p2);
+          if (k.tiles == 1) {
+            float f[V];
+            from_elems<V>(sw, f);
+#pragma unroll
+            for (int q = 0; q < V; ++q) total[q * th] += f[q];
+            from_elems<V>(sb, f);
+#pragma unroll
+            for (int q = 0; q < V; ++q) total[(V + q) * th] += f[q];
+          }
+        };
+        int runs = 0, n = 0;                      // runs before this one, and rows of it
+        auto next_run = [&] {
+          columns_sums();
+          put_part();
+          fresh = false;
+          if (runs > 0) s1 += red[threadIdx.x].x, s2 += red[threadIdx.x].y;
+          red[threadIdx.x] = make_float2(s1, s2);
+          ++runs;
+          n = 0;
+#pragma unroll
+          for (int q = 0; q < NE; ++q) sw[q] = sb[q] = e_splat<E>(0.f);
+        };
         int64_t left = nr - k.r;
         if constexpr (gn_ring<MODE, T, V, true>) {
           const uint32_t ring = smem_u32(kept), place = (uint32_t)th * sizeof(Vec);
@@ -718,7 +809,8 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
           };
 #pragma unroll
           for (int d = 0; d < GN_RING; ++d) issue(d);
-          while (todo > 0) {
+          for (; todo > 0; n += GN_RING) {
+            if (n == GN_RUN) next_run();
 #pragma unroll
             for (int d = 0; d < GN_RING; ++d) {
               if (todo <= 0) break;
@@ -729,7 +821,8 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
             }
           }
         } else {
-          for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * xstep, dy += U * dstep) {
+          for (; left > (U - 1) * k.tr; left -= U * k.tr, x += U * xstep, dy += U * dstep, n += U) {
+            if (n == GN_RUN) next_run();
             Vec u[U], v[U];
   #pragma unroll
             for (int j = 0; j < U; ++j) u[j].load(x + j * xstep), v[j].load(dy + j * dstep);
@@ -743,23 +836,8 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
             add(u, v);
           }
         }
-        E p1 = e_splat<E>(0.f), p2 = p1;
-#pragma unroll
-        for (int q = 0; q < NE; ++q) {
-          p1 = e_fma(w[q], sb[q], p1);
-          p2 = e_fma(w[q], sw[q], p2);
-        }
-        if (k.tiles == 1) {
-          float f[V];
-          from_elems<V>(sw, f);
-#pragma unroll
-          for (int q = 0; q < V; ++q) total[q * th] += f[q];
-          from_elems<V>(sb, f);
-#pragma unroll
-          for (int q = 0; q < V; ++q) total[(V + q) * th] += f[q];
-        }
-        s1 = e_sum(p1);
-        s2 = e_sum(p2);
+        columns_sums();
+        if (runs > 0) s1 += red[threadIdx.x].x, s2 += red[threadIdx.x].y;
       }
       if (k.slots) {
         s1 = gn_warp_sum(k, s1);
@@ -771,16 +849,7 @@ __global__ void __launch_bounds__(256, GN_BWD_CTAS) k_gn_bwd(const GnArgs a) {
         }
         continue;
       }
-      if (k.tiles > 1 && part && cv < k.nvec) {    // one thread a column: its sums of all samples lie in memory
-        float fw[V], fb[V];
-        from_elems<V>(sw, fw);
-        from_elems<V>(sb, fb);
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          part[c + q] = first ? fw[q] : part[c + q] + fw[q];
-          part[a.c + c + q] = first ? fb[q] : part[a.c + c + q] + fb[q];
-        }
-      }
+      put_part();
       __syncthreads();                            // red is free (and grp is zero)
       red[threadIdx.x] = make_float2(s1, s2);
       __syncthreads();
