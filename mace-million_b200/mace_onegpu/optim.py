@@ -52,7 +52,11 @@ def orthogonalize(g, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 class Muon(torch.optim.Optimizer):
     """Momentum whose update of a matrix [.., m, n] is orthogonalised: p <- p (1 - lr weight_decay) - lr max(1, m / n)^0.5 U with
     U = orthogonalize(g + momentum v) (nesterov) or of v, and v <- momentum v + g.  For parameters of two dimensions or more;
-    vectors (norms, biases) take another optimiser."""
+    vectors (norms, biases) take another optimiser.
+
+    All of it is float32 whatever the parameter's type.  A bfloat16 or float16 parameter keeps what its rounding left off beside v
+    ("rounding"), p + rounding being the float32 value that the step goes on from: updates and decays below half a step of the type
+    add up, and a parameter that is set from outside stays set."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
@@ -79,13 +83,29 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None or p.numel() == 0:
                     continue
-                v = self.state[p].get("momentum_buffer")
-                if v is None:
-                    v = self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                state, narrow = self.state[p], p.dtype != torch.float32
+                for key in ("momentum_buffer", "rounding")[:1 + narrow]:
+                    if key not in state:
+                        state[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                v = state["momentum_buffer"]
                 v.mul_(mu).add_(p.grad)
-                d = p.grad.add(v, alpha=mu) if group["nesterov"] else v
+                d = p.grad.float().add(v, alpha=mu) if group["nesterov"] else v
                 u = orthogonalize(d, steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+                w = p.float().add_(state["rounding"]) if narrow else p
                 if group["weight_decay"]:
-                    p.mul_(1 - lr * group["weight_decay"])
-                p.add_(u, alpha=-lr * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
+                    w.mul_(1 - lr * group["weight_decay"])
+                w.add_(u, alpha=-lr * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
+                if narrow:
+                    p.copy_(w)
+                    torch.sub(w, p, out=state["rounding"])
         return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class has cast the state to the parameters' types
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
+            for key, value in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(value) and value.is_floating_point():
+                    self.state[p][key] = value.to(device=p.device, dtype=torch.float32, copy=True)
