@@ -24,17 +24,17 @@ _TABLES = {}
 def _table(steps, coefficients):
     """float64 [steps, 3] in host memory, made once for each argument."""
     key = (steps, tuple(map(tuple, coefficients)) if isinstance(coefficients[0], (tuple, list)) else tuple(coefficients))
-    if key not in _TABLES:
+    table = _TABLES.get(key)
+    if table is None:
         rows = key[1] if isinstance(key[1][0], tuple) else (key[1],) * steps
         if len(rows) != steps or any(len(r) != 3 for r in rows):
             raise ValueError(f"coefficients must be (a, b, c), or one such triple for each of the {steps} steps")
         table = torch.tensor(rows, dtype=torch.float64, device="cpu")
-        if type(table) is not torch.Tensor:         # a shape tensor has no values to keep
-            return table
-        if len(_TABLES) > 64:
-            _TABLES.clear()
-        _TABLES[key] = table
-    return _TABLES[key]
+        if type(table) is torch.Tensor:             # (a shape tensor has no values to keep)
+            if len(_TABLES) > 64:                   # other threads may have dropped or added tables meanwhile
+                _TABLES.clear()
+            _TABLES[key] = table
+    return table
 
 
 def orthogonalize(g, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
