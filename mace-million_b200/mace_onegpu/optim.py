@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from .experts import _op
 
 __all__ = ["orthogonalize", "Muon", "COEFFICIENTS"]
@@ -37,6 +38,25 @@ def _table(steps, coefficients):
     return table
 
 
+_TAKEN = set()
+
+
+def _check_polynomial(steps, coefficients, eps):
+    """ValueError for what orthogonalize refuses: the library looks at it before it looks at matrices, of which there are none."""
+    key = (int(steps), repr(coefficients), float(eps))
+    if key in _TAKEN:
+        return
+    if not 1 <= key[0] <= 16:
+        raise ValueError(f"steps must be in [1, 16] (got {steps})")
+    table = _table(key[0], coefficients)
+    L = _native.lib()
+    if type(table) is torch.Tensor and L.mace_b200_orthogonalize(None, 1, 1, None, None, 0, 1, 1, table.data_ptr(), key[0], key[2], 0, None):
+        raise ValueError(L.mace_b200_last_error().decode())
+    if len(_TAKEN) > 64:
+        _TAKEN.clear()
+    _TAKEN.add(key)
+
+
 def orthogonalize(g, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """g [.., m, n] (float32, bfloat16 or float16) -> bfloat16 [.., m, n]: X = g / (|g| + eps) with the Frobenius norm, then `steps`
     times X = a X + (b A + c A A) X with A = X X^T (from the right with A = X^T X for m > n).  Every matrix of the batch for itself.
@@ -59,18 +79,31 @@ class Muon(torch.optim.Optimizer):
     add up, and a parameter that is set from outside stays set."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
-        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
-            raise ValueError(f"lr {lr}, momentum {momentum} or weight_decay {weight_decay} is out of range")
-        _table(int(steps), coefficients)
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps))
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
+        try:
+            self._check(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check(group):
+        """ValueError for a group that a step would refuse."""
+        lr, momentum, weight_decay = group["lr"], group["momentum"], group["weight_decay"]
+        if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
+            raise ValueError(f"lr {lr}, momentum {momentum} or weight_decay {weight_decay} is out of range")
+        _check_polynomial(group["steps"], group["coefficients"], group["eps"])
+        for p in group["params"]:
             if p.dim() < 2:
-                self.param_groups.pop()
                 raise ValueError(f"Muon takes matrices [.., m, n] (got a parameter of shape {tuple(p.shape)})")
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                raise ValueError(f"Muon takes float32, bfloat16 or float16 parameters (got {p.dtype})")
+            if max(p.shape[-2:]) > 65536 or p.shape[:-2].numel() > 65535:
+                raise ValueError(f"Muon takes at most 65535 matrices with sides of at most 65536 (got {tuple(p.shape)})")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -78,6 +111,11 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:              # before any state changes: groups may be edited between steps
+            self._check(group)
+            for p in group["params"]:
+                if p.grad is not None and (not p.is_cuda or p.grad.is_sparse):
+                    raise ValueError("Muon takes CUDA parameters with dense gradients")
         for group in self.param_groups:
             lr, mu = group["lr"], group["momentum"]
             for p in group["params"]:

@@ -2,6 +2,7 @@
 import concurrent.futures
 import sys
 
+import pytest
 import torch
 
 from mace_onegpu import optim
@@ -19,6 +20,51 @@ def test_loaded_state_of_narrow_parameters_stays_float32():
     saved["state"][0]["momentum_buffer"] = state["momentum_buffer"].bfloat16()    # of a float32 checkpoint cast to 16 bits
     opt.load_state_dict(saved)
     assert opt.state[p]["momentum_buffer"].dtype == torch.float32
+
+
+def _matrix(dt=torch.float32):
+    return torch.nn.Parameter(torch.ones(4, 6, dtype=dt))
+
+
+BAD = [dict(lr=-1.0), dict(lr=float("nan")), dict(momentum=1.0), dict(weight_decay=-0.1), dict(steps=0), dict(steps=17),
+       dict(coefficients=(9.0, 0.0, 0.0)), dict(coefficients=((1.5, -0.5, 0.0),) * 4), dict(coefficients=(float("nan"), 0.0, 0.0)),
+       dict(eps=0.0)]
+
+
+@pytest.mark.parametrize("bad", BAD, ids=str)
+def test_muon_refuses_a_groups_own_values(bad):
+    """In the constructor, in a group of its own, and where a group was edited: before any state is there."""
+    with pytest.raises(ValueError):
+        optim.Muon([_matrix()], **bad)
+    with pytest.raises(ValueError):
+        optim.Muon([dict(params=[_matrix()]), dict(params=[_matrix()], **bad)])
+    p = _matrix()
+    opt = optim.Muon([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[_matrix()], **bad))
+    assert len(opt.param_groups) == 1
+    p.grad = torch.ones_like(p)
+    opt.param_groups[0].update(bad)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert not opt.state and torch.equal(p.detach(), torch.ones(4, 6))
+
+
+def test_muon_refuses_parameters_before_state_changes():
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        optim.Muon([_matrix(torch.float64)])
+    with pytest.raises(ValueError, match="matrices"):
+        optim.Muon([_matrix(), torch.nn.Parameter(torch.zeros(3))])
+    for shape in ((1, 65537), (65537, 1), (256, 256, 1, 1)):
+        with pytest.raises(ValueError, match="at most"):
+            optim.Muon([torch.nn.Parameter(torch.zeros(shape))])
+    p = _matrix()
+    opt = optim.Muon([p])
+    opt.step()                                                 # without a gradient there is nothing to do
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="CUDA"):
+        opt.step()
+    assert not opt.state
 
 
 def test_coefficient_tables_from_many_threads():
