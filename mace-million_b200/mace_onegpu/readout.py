@@ -100,9 +100,17 @@ class ReadoutBlock(torch.nn.Module):
         return Int8Readout(self)
 
 
+def _rows16(q):
+    """8-bit rows that lie whole 16 bytes apart: q itself, or a copy."""
+    if (q.shape[1] == 1 or q.stride(1) == 1) and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1]:
+        return q
+    return q.new_zeros(q.shape[0], (q.shape[1] + 15) // 16 * 16)[:, :q.shape[1]].copy_(q)
+
+
 class Int8Readout(torch.nn.Module):
     """A ReadoutBlock with its matrices in 8 bits and a scale per output channel; a scale per row of the activations is taken on the
-    way.  For inference: no gradient."""
+    way.  For inference: no gradient.  Casts of the module (.half(), .to(torch.bfloat16)) are casts of the norms and biases: the scales
+    stay float32, and rows of the matrices whole 16 bytes apart wherever the module is moved."""
 
     def __init__(self, block):
         super().__init__()
@@ -116,6 +124,16 @@ class Int8Readout(torch.nn.Module):
                 self.register_buffer(f"ws{i}", s)
 
     _norm = ReadoutBlock._norm
+
+    def _apply(self, fn, recurse=True):
+        scales = {name: self._buffers[name] for name in ("ws1", "ws2")}
+        super()._apply(fn, recurse)
+        for name, kept in scales.items():
+            if self._buffers[name].dtype != torch.float32:
+                self._buffers[name] = kept.to(self._buffers[name].device)
+        for name in ("wq1", "wq2"):
+            self._buffers[name] = _rows16(self._buffers[name])
+        return self
 
     @torch.no_grad()
     def forward(self, x, offsets=None):
