@@ -2,6 +2,8 @@
 // matrices over the C ABI (include/mace_b200.h).  As in
 // torch_ops.cpp, the ops check devices, types and shapes with TORCH_CHECK, launch on torch's current CUDA stream and
 // allocate outputs and workspaces with torch's caching allocator.
+#include <cmath>
+
 #include "torch_ops_util.h"
 
 namespace {
@@ -75,6 +77,9 @@ std::tuple<Tensor, Tensor, Tensor> gn_forward(const Tensor& x, int64_t groups, c
                                       y.data_ptr(), ptr_as<float>(mean), ptr_as<float>(rstd), ptr_as<float>(ws), a.r, a.n, a.len,
                                       (int32_t)a.c, (int32_t)groups, eps, (int32_t)act, a.dt, a.pt, stream_of(x)),
              "group_norm");
+  } else if (stats) {                             // empty samples, as those among others: the mean 0 and the variance 0
+    mean.zero_();
+    rstd.fill_(1.f / std::sqrt((float)eps));
   }
   return {y, mean, rstd};
 }
