@@ -1,6 +1,7 @@
 // Linear maps in 8-bit integers, a scale for each token and each output channel:
 //   s_t = max_k |x[t][k]| / 127,  q[t][k] = nearest(x[t][k] / s_t),  y[t][n] = (sum_k q[t][k] w[n][k]) s_t s_n + b_n
-// The sums are exact in int32 (k <= MB_INT8_MAX_K), y is fp32 arithmetic on them, rounded once.  q is the nearest whole number
+// The sums are exact in int32 (k <= MB_INT8_MAX_K), y is fp32 arithmetic on them, rounded once: (sum s_n) s_t + b_n, in this order, as
+// sum s_t of tokens beyond 1e33 would overflow where y does not.  q is the nearest whole number
 // of the exact quotient, ties to even (a remainder by fma corrects the rounded quotient), so it does not depend on who divides.
 //
 // Three kernels.  k_quant_rows: a row stays in the registers of 32 to 256 threads, read once.  k_int8_few: up to 4 tokens; a CTA quantizes them into shared memory while its
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(256) k_int8_few(const I8Args a) {
     const unsigned n = n0 + lane % R;
     if (t < a.t && t < TT && n < rows) {
       const float b = !a.bias ? 0.f : a.b32 ? ((const float*)a.bias)[n] : to_f(((const T*)a.bias)[n]);
-      ((T*)a.y)[(int64_t)t * rows + n] = from_f<T>(fmaf((float)mine * sc[t], a.ws[n], b));
+      ((T*)a.y)[(int64_t)t * rows + n] = from_f<T>(fmaf((float)mine * a.ws[n], sc[t], b));
     }
   }
 }
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         // the tokens' rows one after the other, 32 neighbouring channels a store
         const float4* s4 = reinterpret_cast<const float4*>(xs + c);
         auto put = [&](float sum, float s, bool here) {
-          const float v = fmaf(sum * s, ws, b);
+          const float v = fmaf(sum * ws, s, b);
           if (here) *y = from_f<T>(v);
           y += n_all;
         };
