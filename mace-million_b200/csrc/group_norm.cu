@@ -1079,7 +1079,8 @@ static int gn_split(const GnArgs& a, int size, int slabs) {
   // the number whose rounds over the resident CTAs take least, a CTA's start and end as long as GN_START bytes of its rows: for each
   // number of rounds the most parts that need no more
   const int64_t all = (int64_t)(slabs == 1 ? GN_FWD_CTAS : GN_BWD_CTAS) * sm_count(), r0 = (a.n + all - 1) / all;
-  const int64_t most = bytes / 4096 > 1 ? bytes / 4096 : 1;
+  int64_t most = bytes / 4096 < gn_rows(a) ? bytes / 4096 : gn_rows(a);   // (each part has a row of sums of every column backward)
+  if (most < 1) most = 1;
   int64_t best = 1;
   double least = 0.0;
   for (int64_t r = r0; r <= r0 + 4; ++r) {
@@ -1113,6 +1114,7 @@ static GnCut gn_cut(const GnArgs& a, int size, int slabs, int threads_sm) {
     for (k.pshift = 0; (1 << k.pshift) < k.p; ++k.pshift) {}
   }
   if (ncb > a.groups) ncb = a.groups;
+  if (ncb > 65535) ncb = 65535;                   // of a grid's second dimension
   k.gpb = (int)((a.groups + ncb - 1) / ncb);
   if (k.gpb > 1024) k.gpb = 1024;                 // words of its groups in shared memory
   k.ncb = (a.groups + k.gpb - 1) / k.gpb;
