@@ -14,8 +14,8 @@
 // (cta_group::2) on 256 channels, each with its own 128 and half of the tokens' rows.  Every wait is bounded; a tile whose
 // wait expired is NaN.
 //
-// Measured on a B200 (cuBLAS bf16 1.67 PFLOP/s, so 3.3 POP/s for 8 bits): 16,384 x 4096 x 4096 bf16 202 us, of it the quantization 42
-// (4.8 TB/s) and the product 167 (3.3 POP/s, the tensor cores 87% busy); 16,384 x 1024 x 1024 31 us (10 and 19; the drain of a tile takes as
+// Measured on a B200 (cuBLAS bf16 1.67 PFLOP/s, so 3.3 POP/s for 8 bits): 16,384 x 4096 x 4096 bf16 202 us; alone the quantization takes 42
+// (4.8 TB/s) and the product of 8-bit tokens 164 (3.4 POP/s, the tensor cores 87% busy); 16,384 x 1024 x 1024 31 us (10 and 19; the drain of a tile takes as
 // long as its 8 K blocks); 24,001 x 515 x 1001 fp16 42 us (13 and 28: elements of two bytes in rows of any alignment); 192 x 128 x 512
 // fp32 6 us (two launches); one token 1024 x 1024 2.7 us, 4096 x 4096 5.0 us (3.4 TB/s of weights).  Few tokens by dp4a / by the
 // tensor cores, 512 x 2048: 4 tokens 5.1 / 6.3 us, 5 tokens 8.4 / 6.4.
@@ -621,15 +621,23 @@ static int quant_go(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* s
   const int64_t want = (rows + 7) / 8, most = 8 * (int64_t)sm_count();
   const bool words = ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
   const unsigned grid = (unsigned)(want < most ? want : most);
-  if (k <= 256)
-    k_quant_any<T, 2><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
-  else if (k <= 640)
-    k_quant_any<T, 5><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
-  else if (k <= 1024)
-    k_quant_any<T, 8><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
-  else
-    k_quant_any<T, 0><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
-  return check_launch("quantize_rows");
+  // a row of up to 1024 values stays in registers, in as many pieces of 128 as it has: each piece more costs 0.5 to 1.5 us of 16,384 rows (300
+  // fp16: three 6.9 us, five 8.8; 515 fp16: five 9.5, eight 13.4, read twice 11.8; 900 fp16: eight 14.7, twice 18.0; 1200: ten and twice 12.5)
+  const auto any = [&](auto nv) {
+    k_quant_any<T, decltype(nv)::value><<<grid, 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, rows, k, words);
+    return check_launch("quantize_rows");
+  };
+  switch (k <= 1024 ? (k + 127) / 128 : 0) {
+    case 1: return any(std::integral_constant<int, 1>());
+    case 2: return any(std::integral_constant<int, 2>());
+    case 3: return any(std::integral_constant<int, 3>());
+    case 4: return any(std::integral_constant<int, 4>());
+    case 5: return any(std::integral_constant<int, 5>());
+    case 6: return any(std::integral_constant<int, 6>());
+    case 7: return any(std::integral_constant<int, 7>());
+    case 8: return any(std::integral_constant<int, 8>());
+    default: return any(std::integral_constant<int, 0>());
+  }
 }
 
 constexpr int I8_FEW = 4, I8_FEW_SMEM = 128 * 1024;   // most tokens of k_int8_few, most bytes of them
