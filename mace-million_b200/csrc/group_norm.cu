@@ -9,21 +9,24 @@
 //    memory between the sums and the output and exchanges sums of its groups with the cluster through distributed shared memory.
 //    Rows that do not fit (ragged samples far above the mean) are read again.
 //  * larger ones stream: GN_SUMS (partial sums of P parts of a sample to the workspace), a small kernel that adds up the parts, and
-//    GN_APPLY, which reads the rows again, last ones first, as L2 has those.  No barrier stands between the bytes, so both run near
-//    the copy rate.  (Large samples in clusters of 8 on the chip read once, but load and store in turns: 64 x 2048 x 512 bf16
-//    forward 124 us and backward 315.)
+//    GN_APPLY, which reads the rows again, last ones first: of tensors larger than L2 that one still has those (64 x 2048 x 512 bf16 75 + 130
+//    us, first ones first 75.5 + 133; 24,000 x 512 fp32, which L2 holds, 46 + 60 and 43 + 60).  No barrier stands between the bytes, so
+//    both run near the copy rate.  (Large samples in clusters of 8 on the chip read once, but load and store in turns: 64 x 2048 x 512
+//    bf16 forward 124 us and backward 315.)
 // A thread owns V channels of one group (16 bytes, or what divides a group) and every TR-th row, and takes its sums relative to
 // its own first row, GN_RUN rows at a time: a sample far longer than the others, which gets no more threads than they, may have
 // 10^5 rows of a thread, and that many additions of like values in a row are 0.1% off (of 137,500 times 0.1; in runs of 512 1.5e-6).
 // Threads, CTAs and clusters are joined as (count, mean, sum of squared deviations), so nothing cancels.  No atomics: parameter
-// gradients are added up over a CTA's samples in registers, then over CTAs by a second small kernel in a fixed order.
-#include "dtypes.cuh"
+// gradients are added up over a CTA's samples in a thread's own places of shared memory (of columns beyond one pass of the threads: in
+// the CTA's rows of the workspace), then over CTAs by a second small kernel in a fixed order.
 //
-// Measured on a B200 (kernels, forward / backward; a copy runs at 6.5 TB/s): 64 x 2048 x 512 bf16 in 32 groups with silu 77 / 128 us
-// (3 and 5 times the tensor's bytes at 5.3 TB/s; sums 33 us, with the issue slots 80% busy, outputs 47), one sample of 24,000 x 512 fp32
-// 44 / 60 us (three and four launches), one of 1,029,000 x 128 fp32 268 / 496 us (5.9 and 5.3 TB/s), 384 ragged samples of 63 x 128 fp16
-// with gelu 12.6 / 24 us, 192 x 128 fp32 6.2 / 8.6 us (latency of one launch, of two), 4,000 ragged samples of 60 x 128 bf16
-// 59 / 126 us (what a CTA does once a sample: its offsets, sums over threads, parameters).
+// Measured on a B200 (kernels, forward / backward; a copy runs at 6.5 TB/s): 64 x 2048 x 512 bf16 in 32 groups with silu 75 / 130 us
+// (3 and 5 times the tensor's bytes at 5.3 TB/s; sums 33 us, with the issue slots 80% busy, outputs 47), with gelu 92 / 163, one sample of
+// 24,000 x 512 fp32 46 / 60 us (three and four launches), one of 1,029,000 x 128 fp32 272 / 495 us (5.8 and 5.3 TB/s), 384 ragged samples of
+// 63 x 128 fp16 with gelu 12.2 / 25 us, 192 x 128 fp32 6.6 / 9.0 us (latency of one launch, of two), 4,000 ragged samples of 60 x 128
+// bf16 57 / 131 us (what a CTA does once a sample: its offsets, sums over threads, parameters).  Samples are cut by their mean length:
+// one far longer than the others gets no more CTAs than they (one of 1.1 million rows among 20,000 of 60 is 59 + 85 ms of one CTA).
+#include "dtypes.cuh"
 #include "norm.cuh"
 #include "tc.cuh"
 
@@ -176,7 +179,7 @@ __device__ __forceinline__ void gn_set(GnVec<T, V>& v, const Elem<V> (&e)[kElems
 }
 
 // 1 / (1 + exp(-z)).  fp32 results take expf and a division; 16-bit ones 2^(-z log2 e) and a reciprocal, each approximate to
-// 2^-22 (the exponent's rounding |z| 2^-24): 0 where the power is infinite.
+// 2^-22 (the exponent's rounding |z| 2^-24): 0 where the power is above 2^126, at z below -87.3.
 __device__ __forceinline__ float pow2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

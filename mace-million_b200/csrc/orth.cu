@@ -2,8 +2,10 @@
 //   X = G / (|G|_F + eps);  per step  A = X X^T,  X <- a X + (b A + c A A) X   (m <= n; else A = X^T X, products from the right)
 // so every singular value s moves to a s + b s^3 + c s^5, towards one.  The result is bf16.
 //
-// Products are tcgen05 kind::f16 with fp32 accumulators, on fp16 operands: everything is bounded (|X| <= 2, so powers of two
-// scale it into fp16's range) and fp16 has three bits more than bf16.  What is rounded, and why that is enough (fp64 simulation and
+// Products are tcgen05 kind::f16 with fp32 accumulators, on fp16 operands, which have three bits more than bf16.  Everything is bounded, and
+// powers of two scale it into fp16's range: a polynomial whose values pass 3.5 (or 200 in b s^2 + c s^4) for the singular values that
+// reach it, taken 2% larger, is refused, so X's entries are at most 3.5 (times 2^14 at most: 57,344 of 65,504), A's 12.8 (times 4096: 52,300)
+// and those of b A + c A A 200 (times 256: 51,200).  What is rounded, and why that is enough (fp64 simulation and
 // measurement, Frobenius error before the last rounding 2e-4 to 7e-4, of a bf16 result that rounds by 1.7e-3):
 //  * X itself stays in fp32, and the term a X is taken from that.  An error added to X grows by up to a^steps (485) in its weak
 //    directions: with X in fp16 a matrix of rank 8 over noise was 0.04 off.
@@ -680,7 +682,9 @@ static int orth_steps(OrArgs& a, int r, int len, cudaStream_t st) {
 }
 
 // Pairs of CTAs halve the bytes that an SM fetches of one operand: for long sums.  One CTA / pairs: 4096 x 4096 1281 / 1166 us,
-// 2048 x 2048 251 / 240, 1500 x 1500 197 / 187; 1024 x 1024 124 / 151, 16 of them 645 / 667, 4 of 1500 x 700 189 / 197.
+// 2048 x 2048 251 / 240, 1500 x 8192 539 / 459, 1500 x 1500 207 / 195; 1300 x 1300 182 / 197, 1280 x 4096 245 / 258, 1024 x 1024 124 / 151, 16 of
+// them 645 / 667, 4 of 1500 x 700 189 / 197.  Around the limit it is the rounds of tiles that decide: 1400 x 1400 178 / 193, but 4 of them
+// 406 / 373, 16 of them 1400 / 1327 and 4 of 1200 x 1200 311 / 293.
 static bool or_pairs(int64_t r) { return r >= 1400; }
 
 }  // namespace mb

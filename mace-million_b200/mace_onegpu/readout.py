@@ -26,8 +26,9 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     x: [N, .., C], N samples; or [rows, C] with offsets [N + 1] (int32 or int64 on the device, ascending within [0, rows]):
     sample i is rows offsets[i] to offsets[i + 1], rows of no sample give zeros (and get none).  float32, bfloat16 or float16;
     rows may be strided.  weight / bias: [C] of the type of x or float32, or None.  activation: None, "silu", "gelu" (z Phi(z))
-    or "relu".  Statistics and parameter gradients are accumulated in fp32, in a fixed order.  Differentiable once.  A sample
-    whose offsets leave the rows is NaN; where they descend anywhere, all rows are."""
+    or "relu".  Statistics and parameter gradients are accumulated in fp32, in a fixed order.  Samples are dealt out by
+    their mean length: one a thousand times as long as the others is right, but slow.  Differentiable once.  A sample whose offsets
+    leave the rows is NaN; where they descend anywhere, all rows are."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None, 'silu', 'gelu' or 'relu' (got {activation!r})")
     return _op("group_norm")(x, int(groups), weight, bias, float(eps), ACTIVATIONS[activation], offsets)
