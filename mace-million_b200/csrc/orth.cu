@@ -6,11 +6,16 @@
 // powers of two scale it into fp16's range: a polynomial whose values pass 3.5 (or 200 in b s^2 + c s^4) for the singular values that
 // reach it, taken 2% larger, is refused, so X's entries are at most 3.5 (times 2^14 at most: 57,344 of 65,504), A's 12.8 (times 4096: 52,300)
 // and those of b A + c A A 200 (times 256: 51,200).  What is rounded, and why that is enough (fp64 simulation and
-// measurement, Frobenius error before the last rounding 2e-4 to 7e-4, of a bf16 result that rounds by 1.7e-3):
+// measurement, Frobenius error before the last rounding 3e-4 to 1.4e-3, of a bf16 result that rounds by 1.7e-3; 2e-3 for matrices of 2 to 4
+// rows, one in a thousand of 2 x 2 1%):
 //  * X itself stays in fp32, and the term a X is taken from that.  An error added to X grows by up to a^steps (485) in its weak
 //    directions: with X in fp16 a matrix of rank 8 over noise was 0.04 off.
-//  * The products read X rounded to fp16.  An error of the left factor (A, b A + c A A) multiplies X, and the polar factor of
-//    (1 + E) X differs by |E| whatever the singular values; what B X loses lies in the strong directions, which do not grow.
+//  * The products read X rounded to fp16.  An error of the left factor (A, B = b A + c A A) multiplies X, and the polar factor of
+//    (1 + E) X differs by |E| whatever the singular values; what B X loses lies in the strong directions, which do not grow.  That
+//    holds for the whole of B: its diagonal alone has weak directions, too, so while they still grow by more than 8 (OR_GROW; the
+//    first three of five steps) the diagonal's term takes the same rounded X.  With the fp32 X there 4 x 64 matrices of rank 1 over
+//    noise of 1e-3 were 2.7% off, now 0.1%; 16 x 128 1.6% and 0.08%.  In the last steps the fp32 X is better (random 128 x 512 4.6e-4
+//    in every step, 7.9e-4 in the last two, 1.2e-3 in none).
 //  * The diagonals of A and of b A + c A A dominate them and stay apart in fp32: A = A1 + D gives A A = A1 A1 + A1 D + D A1 + D D, and
 //    the diagonal of the second multiplies X in the epilogue.  In the planes they cost 2 to 9 times the error.
 //  * The tensor cores truncate when they add: a diagonal loses 1e-7 of itself per 16 terms, 4e-4 at MB_ORTH_MAX_DIM.
@@ -455,17 +460,23 @@ __global__ void __launch_bounds__(OR_THREADS, 1)
             } else {
 #pragma unroll
               for (int q = 0; q < 8; ++q) v[4 * q] = nx[q].x, v[4 * q + 1] = nx[q].y, v[4 * q + 2] = nx[q].z, v[4 * q + 3] = nx[q].w;
-              const float el = ca + dn;
+              const float el = dn;
               if (c + 32 < hw) fetch(c + 32);
-              if (g.tall) {
+              auto update = [&](auto grow) {
+                constexpr bool GROW = decltype(grow)::value;
+                if (g.tall) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  v[x] = fmaf(__shfl_sync(0xffffffffu, el, x), v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
-              } else {
-                const float f = ca + di;
+                  for (int x = 0; x < 32; ++x)
+                    v[x] = or_update<GROW>(ca, __shfl_sync(0xffffffffu, el, x), v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
+                } else {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = fmaf(f, v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
-              }
+                  for (int x = 0; x < 32; ++x) v[x] = or_update<GROW>(ca, di, v[x], __uint_as_float(u[x]) * (1.f / OR_SB));
+                }
+              };
+              if (g.poly.grow >> step & 1)
+                update(std::true_type());
+              else
+                update(std::false_type());
             }
             if (last) {
 #pragma unroll
@@ -744,6 +755,11 @@ extern "C" int mace_b200_orthogonalize(const void* gp, int64_t ldb, int64_t ldg,
     poly.a[k] = (float)coefficients[3 * k];
     poly.b[k] = (float)coefficients[3 * k + 1];
     poly.c[k] = (float)coefficients[3 * k + 2];
+  }
+  double grows = 1.0;                             // of what the steps from k + 1 on do to weak directions
+  for (int k = steps - 1; k >= 0; --k) {
+    if (grows > OR_GROW) poly.grow |= 1u << k;
+    grows *= fabs(coefficients[3 * k]);
   }
   // X's scale: a power of two near the inverse of its first entries, 2^14 at most (values up to 3.5 stay below 65504)
   int ex = 0;

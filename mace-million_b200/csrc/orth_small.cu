@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
         mma_f16_ss_lead<1>(lead, td, sw128_desc(plane + (k >> 2) * OS_BLOCK + (k & 3) * 32), sw128_desc_mn(xs + k * 2048, OS_BLOCK), id_x,
                            k ? 1u : 0u);
     });
-    const float el = ca + S.e[row];
+    const float el = S.e[row];
+    const bool grow = g.poly.grow >> step & 1;
     if (last && pending) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (last) barrier();                          // every CTA's S.failed is final
     float bad = 0.f;
@@ -411,8 +412,13 @@ __global__ void __launch_bounds__(OS_THREADS, 1) k_orth_small(const __grid_const
       tmem_ld32(tx + lanes + h0 + c, u);
       tmem_ld32(td + lanes + h0 + c, w);
       tmem_wait_ld();
+      if (grow) {
 #pragma unroll
-      for (int x = 0; x < 32; ++x) v[x] = fmaf(el, __uint_as_float(u[x]), __uint_as_float(w[x]) * (1.f / OR_SB));
+        for (int x = 0; x < 32; ++x) v[x] = or_update<true>(ca, el, __uint_as_float(u[x]), __uint_as_float(w[x]) * (1.f / OR_SB));
+      } else {
+#pragma unroll
+        for (int x = 0; x < 32; ++x) v[x] = or_update<false>(ca, el, __uint_as_float(u[x]), __uint_as_float(w[x]) * (1.f / OR_SB));
+      }
       if (!last) {
         put_x(c, v, true);
         continue;
