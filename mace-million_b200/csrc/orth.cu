@@ -6,8 +6,8 @@
 // powers of two scale it into fp16's range: a polynomial whose values pass 3.5 (or 200 in b s^2 + c s^4) for the singular values that
 // reach it, taken 2% larger, is refused, so X's entries are at most 3.5 (times 2^14 at most: 57,344 of 65,504), A's 12.8 (times 4096: 52,300)
 // and those of b A + c A A 200 (times 256: 51,200).  What is rounded, and why that is enough (fp64 simulation and
-// measurement, Frobenius error before the last rounding 3e-4 to 1.4e-3, of a bf16 result that rounds by 1.7e-3; 2e-3 for matrices of 2 to 4
-// rows, one in a thousand of 2 x 2 1%):
+// measurement, Frobenius error before the last rounding 2e-4 to 1.2e-3, of a bf16 result that rounds by 1.7e-3; 2e-3 for 2 x 2 matrices, the
+// worst of millions of which was 1.6% off, where no errors average out):
 //  * X itself stays in fp32, and the term a X is taken from that.  An error added to X grows by up to a^steps (485) in its weak
 //    directions: with X in fp16 a matrix of rank 8 over noise was 0.04 off.
 //  * The products read X rounded to fp16.  An error of the left factor (A, B = b A + c A A) multiplies X, and the polar factor of
@@ -29,10 +29,10 @@
 // it take the norm (sums of squares in fp64) and split G into the planes.
 // Every wait is bounded; after one expires the grid stops and the tiles of the result that have none are NaN.
 //
-// Measured on a B200 (5 steps, bf16 matrices, all launches; rates count half of the symmetric products): 4096 x 4096 1.16 ms
-// (1.18 PFLOP/s; 2 or 4 rounds of tiles a phase for 1.8 and 3.5 rounds' worth, and a drain and a barrier of 15 us at each of 15 phases'
-// ends), 2048 x 2048 240 us, 1024 x 1024 124 us and 3 of 515 x 1023 140 us: 8 to 9 us a phase, of which 3 are products, 2 the drain, 3 the
-// stores' way to memory and the grid's barrier, 1 the first loads; 16 of 1024 x 1024 630 us (X, its planes, A and B are 190 MB, more
+// Measured on a B200 (5 steps, bf16 matrices, all launches; rates count half of the symmetric products): 4096 x 4096 1.17 ms
+// (1.17 PFLOP/s; 2 or 4 rounds of tiles a phase for 1.8 and 3.5 rounds' worth, and a drain and a barrier of 15 us at each of 15 phases'
+// ends), 2048 x 2048 238 us, 1024 x 1024 121 us and 3 of 515 x 1023 134 us: 8 to 9 us a phase, of which 3 are products, 2 the drain, 3 the
+// stores' way to memory and the grid's barrier, 1 the first loads; 16 of 1024 x 1024 560 us (X, its planes, A and B are 190 MB, more
 // than L2 holds).
 #include <cuda.h>
 

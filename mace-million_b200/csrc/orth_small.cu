@@ -9,8 +9,8 @@
 //    its own (the same sums in both), of more each adds a slice in the order of the ranks and stores it, rounded, to all.
 // 256 threads: eight warps hold the rows (two halves of the columns), one thread issues the products between block barriers.
 // Bound: latency.  A step is three products of 8 to 16 MMAs and three passes over TMEM, each behind a barrier (1,450 cycles for 8
-// MMAs of 64, 500 to 2,000 a pass).  Measured on a B200 (5 steps, bf16): 8 of 64 x 128 19 us, 128 x 128 25, 256 x 128 31,
-// 512 x 128 46 (two CTAs; a third of it the sums through distributed shared memory), 89 of 512 x 128 91 (178 CTAs on 148 SMs:
+// MMAs of 64, 500 to 2,000 a pass).  Measured on a B200 (5 steps, bf16): 8 of 64 x 128 20 us, 128 x 128 26, 256 x 128 33,
+// 512 x 128 47 (two CTAs; a third of it the sums through distributed shared memory), 89 of 512 x 128 95 (178 CTAs on 148 SMs:
 // two rounds).  The kernel over the whole GPU took 82, 82 and 187 us for the first, the second and the last.
 #include <type_traits>
 

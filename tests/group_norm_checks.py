@@ -3,7 +3,7 @@
 Inputs: dy = 1 + xh + noise, so that both means of the backward pass, mean(a) and mean(a xh), are of order one in samples of any length,
 and the sums over rows that give dw and db are as large as the sums of their terms' sizes.
 
-Bounds.  u is half a step of the type, e = (8 + log2 M) 2^-23 for groups of M values: x - mean is off by e of the largest |x - mean| and of
+Bounds.  u is half a step of the type (and half of its smallest value), e = (8 + log2 M) 2^-23 for groups of M values: x - mean is off by e of the largest |x - mean| and of
 |x|, at most 8 standard deviations here, so xh by 8 e.  y (slope at most 1.13) and f' (0.8) follow; dx is r times a sum of four terms
 of a size that dy w gives, each off by at most 8 e (1 + |xh|) and f' slopes, together 100 e of the norm of r dy w; dw and db are
 off by 20 e of the sums of their terms' sizes |dy| (1 + |xh|) w."""
@@ -14,6 +14,7 @@ import torch
 import readout_refs as R
 
 U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+LEAST = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}   # half of the smallest value
 EPS = 1e-5
 
 
@@ -39,7 +40,7 @@ def failures(x, groups, w, b, dy, act, edges, dt, y, dx, dw, db):
     u, e = U[dt], (8 + math.log2(m)) * 2.0 ** -23
     wmax, bad = float(w.abs().max()), []
     y, dx, dw, db = (t.detach().double() for t in (y, dx, dw, db))
-    if not bool(((y - y0).abs() <= u * y0.abs() + 10 * e * (1 + wmax * (1 + xh.abs()))).all()):
+    if not bool(((y - y0).abs() <= u * y0.abs() + LEAST[dt] + 10 * e * (1 + wmax * (1 + xh.abs()))).all()):
         bad.append("y")
 
     def by_group(t):                                          # norms of each sample's groups
@@ -51,11 +52,11 @@ def failures(x, groups, w, b, dy, act, edges, dt, y, dx, dw, db):
         if hi > lo:
             v = x[lo:hi].double().reshape(hi - lo, groups, -1)
             scale[lo:hi] = (1 / (v.var((0, 2), unbiased=False, keepdim=True) + EPS).sqrt()).expand_as(v).reshape(hi - lo, -1)
-    if not bool((off <= u * want + 100 * e * by_group(scale * dy.double() * w.double())).all()):
+    if not bool((off <= u * want + LEAST[dt] * by_group(torch.ones_like(dx0)) + 100 * e * by_group(scale * dy.double() * w.double())).all()):
         bad.append("dx")
     terms = (dy.double().abs() * (1 + xh.abs())).sum(0) * 20 * e * max(1.0, wmax)
     for name, got, ref in (("dw", dw, dw0), ("db", db, db0)):
-        tol = u * ref.abs() + terms
+        tol = u * ref.abs() + LEAST[dt] + terms
         over = (ref.abs() + tol > torch.finfo(dt).max) & (got == ref.sign() * float("inf"))   # beyond float16's 65504
         if bool((~((got - ref).abs() <= tol) & ~over).any()):
             bad.append(name)
