@@ -4,6 +4,7 @@ import sys
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from mace_onegpu import optim
 
@@ -87,3 +88,12 @@ def test_coefficient_tables_from_many_threads():
     finally:
         sys.setswitchinterval(before)
     assert not wrong
+
+
+def test_polynomials_seen_without_values_are_looked_at_later():
+    """Under FakeTensorMode a table has no values: what is refused is still refused afterwards."""
+    bad = dict(coefficients=(8.5, 0.25, 0.0))
+    with FakeTensorMode():
+        optim.Muon([_matrix()], **bad)
+    with pytest.raises(ValueError, match="reaches"):
+        optim.Muon([_matrix()], **bad)
